@@ -310,6 +310,90 @@ itts_status itts_qlinear_forward(itts_gpt *gpt, const itts_qlinear *ql, int32_t 
 itts_status itts_decode_timing(itts_gpt *gpt, itts_kv *kv, int32_t mel_token_id, int32_t pos_idx,
                                int32_t n_steps, float *ms_per_step);
 
+/* ---- operators on device memory: decoding with drafted trees (no reference counterpart) ----
+ * Unlike the rest of this header, every pointer in the structs below is memory of the current
+ * device, `stream` is a hipStream_t of it (NULL: its default stream), and a call only enqueues:
+ * it neither waits nor allocates, and may be captured into a graph.  Sizes, types and strides are
+ * checked on the host (ITTS_E_VALIDATION names the argument); what only the device knows (lengths,
+ * parents, paths, tokens) is checked there, out-of-range values never reach memory and give the
+ * results named below.  Strides are in elements; head_dim and vocab are contiguous.  Outputs
+ * overlap no input.  A workspace belongs to one call until that call has finished on the device;
+ * its contents need no initialisation. */
+
+/* Attention of the nodes of a tree of drafted tokens, one tree a sequence.  Node i of sequence b
+ * has its key and value at cache row lengths[b] + i; it sees rows 0 .. lengths[b] - 1 and the rows
+ * of the nodes on its path to the root, itself among them:
+ *   out_i = sum_t softmax_t(scale q_i . k_t) v_t.
+ * parents[b][i]: -1 for a node that follows the sequence itself, j < i for a child of node j;
+ * anything else marks an unused slot.  An unused slot, and any below one, sees nothing: its row
+ * is zeros.  Values in rows that a node does not see never reach it, NaN and infinities among
+ * them.  A sequence with lengths[b] < 0, or whose last used slot lies past max_seq rows, gets
+ * NaN rows.  n_nodes 1 with parents -1 is a decode step.
+ * q, out [batch][n_nodes][n_head][head_dim]; k, v [batch][n_kv_head][max_seq][head_dim], query
+ * head h with key head h / (n_head / n_kv_head); lengths [batch]; parents [batch][n_nodes].
+ * head_dim 64 or 128, n_nodes <= 256.  (q, kv) types: F32 F32, F32 BF16, BF16 BF16, F16 F16; out
+ * has q's.  All rows start at multiples of 16 bytes. */
+typedef struct itts_tree_attention_args {
+  const void *q, *k, *v;
+  void *out;
+  const int32_t *lengths;
+  const int32_t *parents;
+  int32_t batch, n_nodes, n_head, n_kv_head, head_dim;
+  int32_t max_seq; /* rows that a sequence may use (its memory may hold more) */
+  itts_dtype q_dtype, kv_dtype;
+  float scale;
+  int64_t q_batch, q_node, q_head;
+  int64_t out_batch, out_node, out_head;
+  int64_t k_batch, k_head, k_row;
+  int64_t v_batch, v_head, v_row;
+  int64_t parents_batch;
+} itts_tree_attention_args;
+/* Bytes of workspace that itts_tree_attention needs for these sizes (may be 0). */
+itts_status itts_tree_attention_workspace(const itts_tree_attention_args *args, uint64_t *bytes);
+itts_status itts_tree_attention(const itts_tree_attention_args *args, void *workspace, uint64_t workspace_bytes,
+                                void *stream);
+
+/* Scores of rows of logits [rows][vocab] (F32, BF16 or F16): the log-probabilities of n_tokens
+ * given tokens a row (0 for token -1: none; NaN for any other that is no token), the entropy in
+ * nats (entropy may be NULL), and the top_n most probable tokens with their log-probabilities,
+ * most probable first, the lowest token first among equals (top_n <= 64; 0: none).  A row of
+ * -inf alone gives every token -inf, and entropy 0; NaN or +inf anywhere in a row makes its
+ * log-probabilities and entropy NaN, and NaN counts as -inf in the order.
+ * log_probs [rows][n_tokens], top_tokens and top_log_probs [rows][top_n]. */
+typedef struct itts_token_scores_args {
+  const void *logits;
+  const int32_t *tokens;
+  float *log_probs;
+  float *entropy;
+  int32_t *top_tokens;
+  float *top_log_probs;
+  int32_t rows, vocab, n_tokens, top_n;
+  itts_dtype dtype;
+  int64_t logits_row, tokens_row;
+} itts_token_scores_args;
+itts_status itts_token_scores_workspace(const itts_token_scores_args *args, uint64_t *bytes);
+itts_status itts_token_scores(const itts_token_scores_args *args, void *workspace, uint64_t workspace_bytes,
+                              void *stream);
+
+/* Keeps the accepted nodes of a tree: in every layer and head, rows lengths[b] + path[b][i] of k
+ * and v [n_layer][batch][n_head][max_seq][head_dim] move, in place, to rows lengths[b] + i, for the
+ * entries of path[b] before its first negative one; new_lengths[b] = lengths[b] + their count.  A
+ * path rises and stays inside max_seq rows: for any other, or a negative length, nothing moves
+ * and new_lengths[b] = -1.  path [batch][n_path].  All rows are multiples of 16 bytes and start at
+ * them. */
+typedef struct itts_cache_keep_args {
+  void *k, *v;
+  const int32_t *lengths;
+  const int32_t *path;
+  int32_t *new_lengths;
+  int32_t n_layer, batch, n_head, max_seq, head_dim, n_path;
+  itts_dtype dtype;
+  int64_t k_layer, k_batch, k_head, k_row;
+  int64_t v_layer, v_batch, v_head, v_row;
+  int64_t path_batch;
+} itts_cache_keep_args;
+itts_status itts_cache_keep(const itts_cache_keep_args *args, void *stream);
+
 /* ---- Stage-2 CFM DiT estimator and Euler / CFG solver (crates/core/src/models/cfm.rs) ----
  * Replaces CfmDit (cfm.rs:411-761): the 13-layer U-ViT transformer (AdaLN over RMSNorm,
  * rope, SwiGLU, long skips), skip_linear / conv1, the 8-layer WaveNet, the final layer

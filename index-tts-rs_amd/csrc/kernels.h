@@ -305,6 +305,51 @@ hipError_t sampler_stage_init(int dev);
 // The staging area of device dev; false if sampler_stage_init has not run for it.
 bool sampler_stage(int dev, SamplerStage *out);
 
+// ---- decoding with drafted trees (kernels_tree.hip, kernels_scores.hip) ----
+enum OpType : int { kOpF32 = 0, kOpBf16 = 1, kOpF16 = 2 };
+constexpr int kTreeMaxNodes = 256;
+// Attention of the nodes of one tree a sequence over its cached rows and their own ancestors.
+// q, out [batch][n][H][D]; k, v [batch][Hk][max_seq][D] (strides in elements, D contiguous, rows at
+// multiples of 16 bytes); lengths [batch]; parents [batch][n] (par_b apart).  Types: q and the
+// caches alike, or fp32 queries over bf16 rows.
+struct TreeAttn {
+  const void *q, *k, *v;
+  void *out;
+  const int32_t *lengths, *parents;
+  int batch, n, H, Hk, D, max_seq, qt, kvt;
+  float scale;
+  int64_t q_b, q_n, q_h, o_b, o_n, o_h, k_b, k_h, k_r, v_b, v_h, v_r, par_b;
+  float *part;  // tree_attn_ws(a, n_cu) floats
+};
+size_t tree_attn_ws(const TreeAttn &a, int n_cu);
+hipError_t tree_attn(const TreeAttn &a, int n_cu, hipStream_t s);
+// Rows lengths[b] + path[b][i] -> lengths[b] + i of k and v [layers][batch][heads][max_seq][D], in
+// place; new_lengths[b] = lengths[b] + the path's entries before the first negative one (-1, and
+// nothing moved, where the path does not increase or leaves the cache).
+struct CacheKeep {
+  void *k, *v;
+  const int32_t *lengths, *path;
+  int32_t *new_lengths;
+  int layers, batch, heads, max_seq, row_pieces, n_path;  // row_pieces: 16-byte pieces of a row
+  int64_t k_l, k_b, k_h, k_r, v_l, v_b, v_h, v_r, path_b;   // cache strides in 16-byte pieces
+};
+hipError_t cache_keep(const CacheKeep &a, hipStream_t s);
+// Rows of logits: log-probabilities of given tokens, entropy, the top_n most probable tokens.
+constexpr int kScoresMaxTop = 64;
+struct TokenScores {
+  const void *x;  // [rows][vocab], x_row apart
+  const int32_t *tokens;  // [rows][given], tok_row apart
+  float *log_probs;       // [rows][given]
+  float *entropy;         // [rows] (may be null)
+  int32_t *top_tokens;    // [rows][top]
+  float *top_log_probs;
+  int rows, vocab, given, top, type;
+  int64_t x_row, tok_row;
+  void *ws;  // token_scores_ws(a, n_cu) bytes
+};
+size_t token_scores_ws(const TokenScores &a, int n_cu);
+hipError_t token_scores(const TokenScores &a, int n_cu, hipStream_t s);
+
 // ---- Stage-2 CFM DiT estimator (kernels_cfm.hip); activations [B][T][C] fp32 ----
 hipError_t cfm_temb(const float *t, int B, float *emb /*[B][256]*/, hipStream_t s);
 hipError_t cfm_silu(const float *x, float *y, int n, hipStream_t s);

@@ -114,6 +114,27 @@ class itts_cfm_config(C.Structure):
                                          "wn_layers", "wn_kernel")]
 
 
+class itts_tree_attention_args(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("q", "k", "v", "out", "lengths", "parents")] +
+                [(n, C.c_int32) for n in ("batch", "n_nodes", "n_head", "n_kv_head", "head_dim", "max_seq", "q_dtype",
+                                          "kv_dtype")] + [("scale", C.c_float)] +
+                [(n, C.c_int64) for n in ("q_batch", "q_node", "q_head", "out_batch", "out_node", "out_head", "k_batch",
+                                          "k_head", "k_row", "v_batch", "v_head", "v_row", "parents_batch")])
+
+
+class itts_token_scores_args(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("logits", "tokens", "log_probs", "entropy", "top_tokens", "top_log_probs")] +
+                [(n, C.c_int32) for n in ("rows", "vocab", "n_tokens", "top_n", "dtype")] +
+                [(n, C.c_int64) for n in ("logits_row", "tokens_row")])
+
+
+class itts_cache_keep_args(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("k", "v", "lengths", "path", "new_lengths")] +
+                [(n, C.c_int32) for n in ("n_layer", "batch", "n_head", "max_seq", "head_dim", "n_path", "dtype")] +
+                [(n, C.c_int64) for n in ("k_layer", "k_batch", "k_head", "k_row", "v_layer", "v_batch", "v_head", "v_row",
+                                          "path_batch")])
+
+
 _SIGS = {
     "itts_kv_last_timing": (C.c_int, [C.c_void_p, C.POINTER(itts_timing)]),
     "itts_version": (C.c_char_p, []),
@@ -179,6 +200,11 @@ _SIGS = {
                                        C.c_int32, C.c_int, C.c_void_p, C.c_int32, C.c_void_p]),
     "itts_decode_timing": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_int32,
                                      C.POINTER(C.c_float)]),
+    "itts_tree_attention_workspace": (C.c_int, [C.c_void_p, C.POINTER(C.c_uint64)]),
+    "itts_tree_attention": (C.c_int, [C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p]),
+    "itts_token_scores_workspace": (C.c_int, [C.c_void_p, C.POINTER(C.c_uint64)]),
+    "itts_token_scores": (C.c_int, [C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p]),
+    "itts_cache_keep": (C.c_int, [C.c_void_p, C.c_void_p]),
     "itts_cfm_create": (C.c_int, [C.POINTER(itts_cfm_config), C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32,
                                   C.POINTER(C.c_void_p)]),
     "itts_cfm_destroy": (None, [C.c_void_p]),

@@ -1,0 +1,198 @@
+"""The library's operators on device tensors: decoding with drafted trees.
+
+    tree_attention   attention of every node of a tree of drafted tokens over its sequence's
+                     cached rows and its own ancestors (one node: a decode step)
+    token_scores     log-probabilities of given tokens, entropy, the most probable tokens
+    cache_keep       the accepted nodes' key and value rows moved up in the caches
+
+They take torch tensors on one GPU and enqueue on that GPU's current stream: nothing waits, and
+a call may be captured into a graph.  Outputs and workspaces come from torch's allocator, so that
+calls on several streams, and captured ones, share nothing.  No gradients: the tensors are those of
+decoding.  Wrong arguments raise ``ValidationError`` naming the argument; what the operators do with
+lengths, parents, paths and tokens that are out of range (the host cannot see them) is written at
+each function.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import (ITTS_BF16, ITTS_E_VALIDATION, ITTS_F16, ITTS_F32, ValidationError, _check, itts_cache_keep_args,
+               itts_token_scores_args, itts_tree_attention_args, lib)
+
+_DTYPES = {torch.float32: ITTS_F32, torch.bfloat16: ITTS_BF16, torch.float16: ITTS_F16}
+
+
+def _refuse(message: str):
+    raise ValidationError(ITTS_E_VALIDATION, message)
+
+
+def _tensor(t, name: str, dims: int, device=None, dtype=None):
+    if not isinstance(t, torch.Tensor):
+        _refuse(f"{name}: a tensor is needed, got {type(t).__name__}")
+    if t.dim() != dims:
+        _refuse(f"{name}: {dims} dimensions expected, got {t.dim()}")
+    if dtype is None:
+        if t.dtype not in _DTYPES:
+            _refuse(f"{name}: float32, bfloat16 or float16 expected, got {t.dtype}")
+    elif t.dtype != dtype:
+        _refuse(f"{name}: {dtype} expected, got {t.dtype}")
+    if not t.is_cuda:
+        _refuse(f"{name}: a GPU tensor is needed, got one on {t.device}")
+    if device is not None and t.device != device:
+        _refuse(f"{name}: on {t.device}, the other tensors on {device}")
+    if t.requires_grad and torch.is_grad_enabled():
+        _refuse(f"{name}: requires a gradient, which this operator does not give")
+
+
+def _last_contiguous(t, name: str):
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        _refuse(f"{name}: the last dimension must be contiguous")
+
+
+def _run(fn, need, args, device):
+    """Enqueues on the device's current stream, with the workspace that the sizes need."""
+    with torch.cuda.device(device):
+        ws, size = None, C.c_uint64(0)
+        if need is not None:
+            _check(need(C.byref(args), C.byref(size)))
+            if size.value:
+                ws = torch.empty(size.value, dtype=torch.uint8, device=device)
+        stream = torch.cuda.current_stream(device).cuda_stream
+        if need is None:
+            _check(fn(C.byref(args), stream))
+        else:
+            _check(fn(C.byref(args), ws.data_ptr() if ws is not None else None, size, stream))
+
+
+def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: torch.Tensor, parents: torch.Tensor, *,
+                   scale: Optional[float] = None, max_length: Optional[int] = None,
+                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of the nodes of one tree of drafted tokens a sequence.
+
+    q        [batch][nodes][heads][dim], dim 64 or 128, at most 256 nodes
+    k, v     [batch][key heads][rows][dim]: the caches, node i's key and value in row lengths[b] + i.
+             q's type, or bfloat16 under float32 queries.  Any strides whose rows start at multiples
+             of 16 bytes (0 between sequences that share a cache)
+    lengths  [batch] int32: rows in front of the tree, which every node sees
+    parents  [batch][nodes] int32: -1 for a node that follows the sequence itself, j < i for a child
+             of node j.  Anything else marks an unused slot (padding); it and slots below it get
+             rows of zeros
+    scale    of the scores (default dim ** -0.5)
+    max_length  rows that a sequence with its nodes may use (default: the caches' rows); a tight one
+             lets short sequences be split better
+    out      where to write (default: a new tensor)
+
+    A node sees its sequence's rows, its ancestors and itself.  A negative length, or one whose nodes do not
+    fit, gives rows of NaN.  Returns out [batch][nodes][heads][dim] in q's type."""
+    _tensor(q, "q", 4)
+    dev = q.device
+    _tensor(k, "k", 4, dev)
+    _tensor(v, "v", 4, dev)
+    _tensor(lengths, "lengths", 1, dev, torch.int32)
+    _tensor(parents, "parents", 2, dev, torch.int32)
+    for t, name in ((q, "q"), (k, "k"), (v, "v"), (parents, "parents")):
+        _last_contiguous(t, name)
+    b, n, h, d = q.shape
+    if k.shape != v.shape or k.dtype != v.dtype:
+        _refuse(f"v: must be like k, {tuple(k.shape)} {k.dtype}, got {tuple(v.shape)} {v.dtype}")
+    if k.shape[0] != b or k.shape[3] != d:
+        _refuse(f"k: [{b}][heads][rows][{d}] expected, got {tuple(k.shape)}")
+    if lengths.shape[0] != b or parents.shape != (b, n):
+        _refuse(f"lengths, parents: [{b}] and [{b}][{n}] expected, got {tuple(lengths.shape)} and {tuple(parents.shape)}")
+    if lengths.shape[0] > 1 and lengths.stride(0) != 1:
+        _refuse("lengths: must be contiguous")
+    rows = k.shape[2] if max_length is None else int(max_length)
+    if rows > k.shape[2]:
+        _refuse(f"max_length: the caches have {k.shape[2]} rows, got {rows}")
+    if out is None:
+        out = torch.empty((b, n, h, d), dtype=q.dtype, device=dev)
+    else:
+        _tensor(out, "out", 4, dev, q.dtype)
+        _last_contiguous(out, "out")
+        if out.shape != q.shape:
+            _refuse(f"out: {tuple(q.shape)} expected, got {tuple(out.shape)}")
+    a = itts_tree_attention_args(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lengths.data_ptr(),
+                                 parents.data_ptr(), b, n, h, k.shape[1], d, rows, _DTYPES[q.dtype], _DTYPES[k.dtype],
+                                 d ** -0.5 if scale is None else scale, *q.stride()[:3], *out.stride()[:3], *k.stride()[:3],
+                                 *v.stride()[:3], parents.stride(0))
+    _run(lib.itts_tree_attention, lib.itts_tree_attention_workspace, a, dev)
+    return out
+
+
+class TokenScores(NamedTuple):
+    log_probs: Optional[torch.Tensor]      # [rows][given] float32 (None without tokens)
+    entropy: torch.Tensor                  # [rows] float32, nats
+    top_tokens: torch.Tensor               # [rows][top_n] int32
+    top_log_probs: torch.Tensor            # [rows][top_n] float32
+
+
+def token_scores(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, top_n: int = 0) -> TokenScores:
+    """Scores of rows of logits [rows][vocab] (float32, bfloat16 or float16; rows any distance apart).
+
+    tokens   [rows] or [rows][given] int32: tokens whose log-probabilities are wanted, -1 for none (0.0
+             comes back); another that is outside the vocabulary gives NaN
+    top_n    how many of the most probable tokens to return (at most 64), the most probable first and
+             the lowest token first among equals
+
+    A row of -inf alone gives every token -inf, and entropy 0.  A NaN or +inf makes its row's
+    log-probabilities and entropy NaN; NaN counts as -inf in the order.  log_probs has tokens' shape."""
+    _tensor(logits, "logits", 2)
+    _last_contiguous(logits, "logits")
+    dev = logits.device
+    r, vocab = logits.shape
+    given, log_probs, tok = 0, None, None
+    if tokens is not None:
+        one = isinstance(tokens, torch.Tensor) and tokens.dim() == 1
+        _tensor(tokens, "tokens", 1 if one else 2, dev, torch.int32)
+        if tokens.shape[0] != r:
+            _refuse(f"tokens: {r} rows expected, got {tokens.shape[0]}")
+        tok = tokens.unsqueeze(1) if one else tokens
+        _last_contiguous(tok, "tokens")
+        given = tok.shape[1]
+        log_probs = torch.empty(tokens.shape, dtype=torch.float32, device=dev)
+    top_n = int(top_n)
+    if not 0 <= top_n <= min(64, vocab):
+        _refuse(f"top_n: must be in 0..=64 and at most the vocabulary of {vocab}, got {top_n}")
+    entropy = torch.empty(r, dtype=torch.float32, device=dev)
+    top_tokens = torch.empty((r, top_n), dtype=torch.int32, device=dev)
+    top_log_probs = torch.empty((r, top_n), dtype=torch.float32, device=dev)
+    a = itts_token_scores_args(logits.data_ptr(), tok.data_ptr() if given else None, log_probs.data_ptr() if given else None,
+                               entropy.data_ptr(), top_tokens.data_ptr(), top_log_probs.data_ptr(), r, vocab, given, top_n,
+                               _DTYPES[logits.dtype], logits.stride(0), tok.stride(0) if given else 0)
+    _run(lib.itts_token_scores, lib.itts_token_scores_workspace, a, dev)
+    return TokenScores(log_probs, entropy, top_tokens, top_log_probs)
+
+
+def cache_keep(k: torch.Tensor, v: torch.Tensor, lengths: torch.Tensor, path: torch.Tensor) -> torch.Tensor:
+    """Keeps the accepted nodes of a tree: rows lengths[b] + path[b][i] of k and v [layers][batch][heads][rows][dim]
+    (or [batch][heads][rows][dim]) move, in place, to rows lengths[b] + i in every layer and head.
+
+    lengths  [batch] int32
+    path     [batch][n] int32: the kept nodes in rising order, ended by a negative entry
+
+    Returns the new lengths [batch], lengths[b] + the nodes kept; -1, with nothing moved, for a path that does not rise or
+    leaves the cache, or a negative length."""
+    dims = 4 if isinstance(k, torch.Tensor) and k.dim() == 4 else 5
+    _tensor(k, "k", dims)
+    dev = k.device
+    _tensor(v, "v", dims, dev, k.dtype)
+    _tensor(lengths, "lengths", 1, dev, torch.int32)
+    _tensor(path, "path", 2, dev, torch.int32)
+    if v.shape != k.shape:
+        _refuse(f"v: must be like k, {tuple(k.shape)}, got {tuple(v.shape)}")
+    for t, name in ((k, "k"), (v, "v"), (path, "path")):
+        _last_contiguous(t, name)
+    kk, vv = (k, v) if dims == 5 else (k.unsqueeze(0), v.unsqueeze(0))
+    layers, b, h, rows, d = kk.shape
+    if lengths.shape[0] != b or path.shape[0] != b:
+        _refuse(f"lengths, path: {b} sequences expected, got {lengths.shape[0]} and {path.shape[0]}")
+    if b > 1 and lengths.stride(0) != 1:
+        _refuse("lengths: must be contiguous")
+    new = torch.empty(b, dtype=torch.int32, device=dev)
+    a = itts_cache_keep_args(kk.data_ptr(), vv.data_ptr(), lengths.data_ptr(), path.data_ptr(), new.data_ptr(), layers, b,
+                             h, rows, d, path.shape[1], _DTYPES[k.dtype], *kk.stride()[:4], *vv.stride()[:4], path.stride(0))
+    _run(lib.itts_cache_keep, None, a, dev)
+    return new

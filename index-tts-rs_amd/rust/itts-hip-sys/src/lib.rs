@@ -162,6 +162,86 @@ pub struct itts_cfm {
     _private: [u8; 0],
 }
 
+/// Attention of drafted trees over caches, device memory (strides in elements).
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct itts_tree_attention_args {
+    pub q: *const c_void,
+    pub k: *const c_void,
+    pub v: *const c_void,
+    pub out: *mut c_void,
+    pub lengths: *const i32,
+    pub parents: *const i32,
+    pub batch: i32,
+    pub n_nodes: i32,
+    pub n_head: i32,
+    pub n_kv_head: i32,
+    pub head_dim: i32,
+    pub max_seq: i32,
+    pub q_dtype: itts_dtype,
+    pub kv_dtype: itts_dtype,
+    pub scale: f32,
+    pub q_batch: i64,
+    pub q_node: i64,
+    pub q_head: i64,
+    pub out_batch: i64,
+    pub out_node: i64,
+    pub out_head: i64,
+    pub k_batch: i64,
+    pub k_head: i64,
+    pub k_row: i64,
+    pub v_batch: i64,
+    pub v_head: i64,
+    pub v_row: i64,
+    pub parents_batch: i64,
+}
+
+/// Scores of rows of logits, device memory.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct itts_token_scores_args {
+    pub logits: *const c_void,
+    pub tokens: *const i32,
+    pub log_probs: *mut f32,
+    pub entropy: *mut f32,
+    pub top_tokens: *mut i32,
+    pub top_log_probs: *mut f32,
+    pub rows: i32,
+    pub vocab: i32,
+    pub n_tokens: i32,
+    pub top_n: i32,
+    pub dtype: itts_dtype,
+    pub logits_row: i64,
+    pub tokens_row: i64,
+}
+
+/// Rows of an accepted path moved up in caches, device memory.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct itts_cache_keep_args {
+    pub k: *mut c_void,
+    pub v: *mut c_void,
+    pub lengths: *const i32,
+    pub path: *const i32,
+    pub new_lengths: *mut i32,
+    pub n_layer: i32,
+    pub batch: i32,
+    pub n_head: i32,
+    pub max_seq: i32,
+    pub head_dim: i32,
+    pub n_path: i32,
+    pub dtype: itts_dtype,
+    pub k_layer: i64,
+    pub k_batch: i64,
+    pub k_head: i64,
+    pub k_row: i64,
+    pub v_layer: i64,
+    pub v_batch: i64,
+    pub v_head: i64,
+    pub v_row: i64,
+    pub path_batch: i64,
+}
+
 #[link(name = "itts_hip")]
 extern "C" {
     pub fn itts_version() -> *const c_char;
@@ -243,6 +323,14 @@ extern "C" {
                                 param_dtype: itts_dtype, x: *const f32, m: i32, y: *mut f32) -> itts_status;
     pub fn itts_decode_timing(gpt: *mut itts_gpt, kv: *mut itts_kv, mel_token_id: i32, pos_idx: i32,
                               n_steps: i32, ms_per_step: *mut f32) -> itts_status;
+
+    pub fn itts_tree_attention_workspace(args: *const itts_tree_attention_args, bytes: *mut u64) -> itts_status;
+    pub fn itts_tree_attention(args: *const itts_tree_attention_args, workspace: *mut c_void, workspace_bytes: u64,
+                               stream: *mut c_void) -> itts_status;
+    pub fn itts_token_scores_workspace(args: *const itts_token_scores_args, bytes: *mut u64) -> itts_status;
+    pub fn itts_token_scores(args: *const itts_token_scores_args, workspace: *mut c_void, workspace_bytes: u64,
+                             stream: *mut c_void) -> itts_status;
+    pub fn itts_cache_keep(args: *const itts_cache_keep_args, stream: *mut c_void) -> itts_status;
 
     pub fn itts_cfm_create(cfg: *const itts_cfm_config, names: *const *const c_char, data: *const *const f32,
                            numel: *const i64, n: i32, out: *mut *mut itts_cfm) -> itts_status;

@@ -1,0 +1,535 @@
+"""The operators on device tensors (itts_hip.ops) against their definitions in float64.
+
+Tolerances.  Attention: a score is a sum of dim products in float32, off by at most about
+2 sqrt(dim) roundings of its products' magnitudes (A = sum |q k| scale), and one or two roundings on
+its way through the exponential; a probability is then off by twice that, relative, and a row of
+n keys sums to within 2 sqrt(n) roundings.  Outputs of 16 bits add half a step of the result, and
+half a step of the probabilities that enter the product in that type (P = sum p |v|).
+Scores: log-probabilities are differences of float32 numbers up to the row's range."""
+import math
+import sys
+
+import pytest
+import torch
+
+import itts_hip as H
+
+pytestmark = pytest.mark.gpu
+
+EPS = 2.0 ** -24  # half a step of float32
+HALF = {torch.float32: EPS, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+TYPES = [(F32, BF16), (F32, F32), (BF16, BF16), (F16, F16)]
+NAN, INF = float("nan"), float("inf")
+
+
+def say(*a):
+    print(*a, flush=True)
+    sys.stdout.flush()
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from itts_hip import ops as o
+
+    return o
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def randn(g, *shape, dtype=F32):
+    return torch.randn(shape, generator=g, device="cuda").to(dtype)
+
+
+def ints(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+# ---- trees -------------------------------------------------------------------------------
+def shape_tree(kind, n, seed=0):
+    if kind == "chain":
+        return [i - 1 for i in range(n)]
+    if kind == "star":
+        return [-1] + [0] * (n - 1)
+    if kind == "forest":
+        return [-1 if i % 5 == 0 else i - 1 - i % 2 * (i > 1) for i in range(n)]
+    g = torch.Generator().manual_seed(seed)
+    r = torch.rand(n, generator=g).tolist()
+    return [-1 if i == 0 else int(r[i] * i) for i in range(n)]
+
+
+def paths(par):
+    """Each slot's nodes on its path to the root, [] for a slot that is not in the tree."""
+    out = []
+    for i, p in enumerate(par):
+        if p == -1:
+            out.append([i])
+        elif 0 <= p < i and out[p]:
+            out.append(out[p] + [i])
+        else:
+            out.append([])
+    return out
+
+
+def attention_ref(q, k, v, lengths, parents, scale=None, max_rows=None):
+    """(result, tolerance) in float64, row by row over the rows that a node sees."""
+    b, n, h, d = q.shape
+    group = h // k.shape[1]
+    scale = d ** -0.5 if scale is None else scale
+    ref = torch.zeros(q.shape, dtype=torch.float64, device=q.device)
+    tol = torch.zeros_like(ref)
+    for i in range(b):
+        length, pt = int(lengths[i]), paths([int(p) for p in parents[i]])
+        live = max([j + 1 for j in range(n) if pt[j]], default=0)
+        if length < 0 or length + live > (k.shape[2] if max_rows is None else max_rows):
+            ref[i] = NAN
+            continue
+        for j in range(n):
+            if not pt[j]:
+                continue
+            rows = list(range(length)) + [length + a for a in pt[j]]
+            kk = k[i][:, rows].double().repeat_interleave(group, 0)
+            vv = v[i][:, rows].double().repeat_interleave(group, 0)
+            qq = q[i, j].double().unsqueeze(1)
+            p = torch.softmax((qq * kk).sum(-1) * scale, -1).unsqueeze(-1)
+            mag = (qq * kk).abs().sum(-1).amax(-1, keepdim=True) * abs(scale)
+            pv = (p * vv.abs()).sum(1)
+            ref[i, j] = (p * vv).sum(1)
+            tol[i, j] = pv * EPS * (2 * 2 * (math.sqrt(d) + 2) * mag + 2 * math.sqrt(len(rows)) + 8)
+            if q.dtype != F32:
+                tol[i, j] += HALF[q.dtype] * (ref[i, j].abs() + pv)
+    return ref, tol + 1e-30
+
+
+def check(got, ref, tol, what=""):
+    bad_nan = torch.isnan(ref) != torch.isnan(got.double())
+    assert not bad_nan.any(), f"{what}: NaN in other places ({int(bad_nan.sum())})"
+    d = (got.double() - ref).abs().nan_to_num(0.0)
+    assert (d <= tol).all(), f"{what}: off by {(d / tol).max().item():.2f} of the tolerance"
+
+
+def attention_case(ops, types, b, n, h, hk, d, lengths, kind, rows=None, seed=0, par=None):
+    g = gen(seed)
+    rows = rows or max(lengths) + n
+    q, kv = types
+    args = (1.5 * randn(g, b, n, h, d)).to(q), randn(g, b, hk, rows, d, dtype=kv), randn(g, b, hk, rows, d, dtype=kv)
+    par = par or [shape_tree(kind, n, seed + i) for i in range(b)]
+    return args, ints(lengths), ints(par)
+
+
+# tiles of 32 keys, of 16 query rows, lengths and trees at and around them
+@pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("n,h,hk,d,lengths,kind", [
+    (1, 4, 4, 64, [0, 1, 31, 32, 33, 700], "chain"),
+    (1, 8, 2, 128, [5, 0, 1000], "chain"),
+    (2, 5, 5, 64, [30, 31, 0], "star"),
+    (7, 3, 1, 64, [64, 1, 250], "tree"),
+    (16, 2, 2, 64, [127, 16], "forest"),
+    (17, 2, 2, 128, [95, 0], "tree"),
+    (33, 6, 2, 64, [200, 3], "tree"),
+    (63, 2, 1, 128, [66, 1], "chain"),
+    (64, 2, 2, 64, [512, 0], "tree"),
+    (65, 1, 1, 64, [33, 2], "star"),
+    (200, 3, 3, 64, [77], "tree"),
+    (256, 2, 1, 64, [0, 1500], "tree"),
+    (256, 1, 1, 128, [31], "chain"),
+])
+def test_attention_matches_float64(ops, types, n, h, hk, d, lengths, kind):
+    say(f"[gpu] tree attention {types} n={n} h={h}/{hk} d={d} {lengths} {kind}")
+    (q, k, v), ln, par = attention_case(ops, types, len(lengths), n, h, hk, d, lengths, kind)
+    check(ops.tree_attention(q, k, v, ln, par), *attention_ref(q, k, v, ln, par))
+
+
+# long caches, split over blocks: few rows and many
+@pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("n,h,hk,d,lengths", [(1, 2, 1, 64, [20011, 5]), (9, 2, 2, 128, [6007]), (40, 1, 1, 64, [9001, 0, 300])])
+def test_attention_split_over_keys(ops, types, n, h, hk, d, lengths):
+    say(f"[gpu] tree attention split {types} n={n} h={h}/{hk} d={d} {lengths}")
+    (q, k, v), ln, par = attention_case(ops, types, len(lengths), n, h, hk, d, lengths, "tree", rows=max(lengths) + n + 3)
+    got = ops.tree_attention(q, k, v, ln, par)
+    check(got, *attention_ref(q, k, v, ln, par))
+    assert torch.equal(got, ops.tree_attention(q, k, v, ln, par))  # the same bits each time
+    # a tight bound on the rows changes the split, not what is computed
+    short = ops.tree_attention(q, k, v, ln, par, max_length=max(lengths) + n)
+    check(short, *attention_ref(q, k, v, ln, par))
+
+
+@pytest.mark.parametrize("types", TYPES)
+def test_attention_unused_slots(ops, types):
+    """Slots that are no nodes, in every form, and slots below them: rows of zeros, and nothing of
+    what their cache rows hold reaches the others."""
+    say(f"[gpu] tree attention unused slots {types}")
+    par = [[-1, -2, 0, 1, 2, 3, 9, -2], [-2] * 8, [-1, 0, 1, -7, 4, 5, 6, 2], [-2, -2, -2, -1, 3, 3, 4, 2 ** 31 - 1]]
+    (q, k, v), ln, _ = attention_case(ops, types, 4, 8, 4, 2, 64, [40, 40, 0, 700], "tree", rows=720)
+    for i, p in enumerate(par):
+        for j, pt in enumerate(paths(p)):
+            if not pt:
+                k[i, :, int(ln[i]) + j] = NAN
+                v[i, :, int(ln[i]) + j] = INF if j % 2 else NAN
+    v[0, :, 48:] = NAN
+    k[2, :, 8:] = INF
+    got = ops.tree_attention(q, k, v, ln, ints(par))
+    check(got, *attention_ref(q, k, v, ln, par))
+    assert (got[1] == 0).all() and (got[0, 1] == 0).all()
+
+
+@pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("value", [NAN, INF, -INF])
+def test_attention_odd_values_stay_where_they_are_seen(ops, types, value):
+    """A node whose value row holds an infinity or NaN: it reaches the nodes below it alone."""
+    say(f"[gpu] tree attention odd values {types} {value}")
+    par = [[-1, 0, 0, 1, 2, 3, 4, 4]]
+    (q, k, v), ln, _ = attention_case(ops, types, 1, 8, 4, 2, 64, [50], "tree")
+    v[0, 1, 52, 7] = value
+    k[0, 0, 51, 3] = value  # node 1: a score of either infinity (by the query's sign) or NaN; -inf weighs nothing
+    got = ops.tree_attention(q, k, v, ln, ints(par))
+    ref, tol = attention_ref(q, k, v, ln, par)
+    assert torch.equal(torch.isnan(got), torch.isnan(ref)) and torch.equal(torch.isinf(got), torch.isinf(ref))
+    fin = torch.isfinite(ref)
+    assert torch.equal(got[~fin & ~torch.isnan(ref)].double(), ref[~fin & ~torch.isnan(ref)])
+    assert ((got.double() - ref).abs()[fin] <= tol[fin]).all()
+    assert fin[0, 0].all() and fin[0, 4, 0].all() and not fin[0, 4, 2:].all()
+
+
+def test_attention_lengths_that_do_not_fit(ops):
+    say("[gpu] tree attention lengths that do not fit")
+    lengths = [-1, 57, 56, 2 ** 31 - 1, -2 ** 31, 0]
+    (q, k, v), _, par = attention_case(ops, (F32, BF16), 6, 8, 4, 4, 64, [56] * 6, "tree", rows=64)
+    ln = ints(lengths)
+    got = ops.tree_attention(q, k, v, ln, par)
+    check(got, *attention_ref(q, k, v, ln, par))
+    assert torch.isnan(got[[0, 1, 3, 4]]).all() and torch.isfinite(got[[2, 5]]).all()
+    part = ops.tree_attention(q, k, v, ln, par, max_length=60)
+    assert torch.isnan(part[2]).all() and torch.equal(part[5], got[5])
+    # 100 rows behind the bound, split over blocks
+    (q, k, v), _, par = attention_case(ops, (F32, BF16), 2, 4, 1, 1, 64, [9000, 9000], "tree", rows=9100)
+    got = ops.tree_attention(q, k, v, ints([9000, 8999]), par, max_length=9003)
+    assert torch.isnan(got[0]).all() and torch.isfinite(got[1]).all()
+
+
+@pytest.mark.parametrize("types", TYPES)
+def test_attention_strides(ops, types):
+    """Heads before nodes, rows with gaps, caches laid out row by row, one cache for all sequences."""
+    say(f"[gpu] tree attention strides {types}")
+    (q, k, v), ln, par = attention_case(ops, types, 3, 6, 4, 2, 64, [40, 90, 0], "tree", rows=100)
+    want = ops.tree_attention(q, k, v, ln, par)
+    q2 = torch.empty(3, 4, 6, 80, dtype=q.dtype, device="cuda").transpose(1, 2)[..., :64]
+    q2.copy_(q)
+    k2 = torch.empty(3, 100, 2, 64, dtype=k.dtype, device="cuda").transpose(1, 2)
+    k2.copy_(k)
+    v2 = torch.empty(2, 3, 120, 128, dtype=v.dtype, device="cuda").transpose(0, 1)[:, :, 10:110, 64:]
+    v2.copy_(v)
+    out = torch.full((3, 4, 6, 96), 7.0, dtype=q.dtype, device="cuda")
+    par2 = torch.zeros(3, 11, dtype=torch.int32, device="cuda")
+    par2[:, :6] = par
+    got = ops.tree_attention(q2, k2, v2, ln, par2[:, :6], out=out.transpose(1, 2)[..., :64])
+    assert torch.equal(got, want) and (out[..., 64:] == 7.0).all()
+    shared = ops.tree_attention(q, k[:1].expand(3, -1, -1, -1), v[:1].expand(3, -1, -1, -1), ln, par)
+    check(shared, *attention_ref(q, k[:1].expand(3, -1, -1, -1), v[:1].expand(3, -1, -1, -1), ln, par))
+
+
+@pytest.mark.parametrize("types", TYPES)
+def test_attention_large_scores(ops, types):
+    """Scores far apart, early and late (the running maximum moves), and negative scales."""
+    say(f"[gpu] tree attention large scores {types}")
+    (q, k, v), ln, par = attention_case(ops, types, 2, 12, 2, 2, 64, [900, 333], "tree")
+    for key, f in ((0, 30.0), (5, 3.0), (400, 20.0), (899, 40.0)):
+        k[:, :, key] *= f
+    for scale in (0.125, 1.0, -0.5, 0.0):
+        ref, tol = attention_ref(q, k, v, ln, par, scale=scale)
+        check(ops.tree_attention(q, k, v, ln, par, scale=scale), ref, tol, f"scale {scale}")
+
+
+def test_attention_past_32_bits(ops):
+    """A cache of more than 2^32 bytes (and 2^31 elements): the last sequence's rows lie behind them."""
+    say("[gpu] tree attention past 2^31 elements")
+    d = 64
+    big_k = torch.as_strided(torch.zeros(2_300_000_000, dtype=BF16, device="cuda"), (2, 1, 600, d),
+                             (2_200_000_000 // d * d, 600 * d, d, 1))
+    g = gen(3)
+    big_k.copy_(randn(g, 2, 1, 600, d))
+    q, v = randn(g, 2, 3, 1, d, dtype=BF16), big_k.flip(0).contiguous()
+    ln, par = ints([500, 590]), ints([[-1, 0, 1]] * 2)
+    check(ops.tree_attention(q, big_k, v, ln, par), *attention_ref(q, big_k, v, ln, par))
+
+
+# ---- scores --------------------------------------------------------------------------------
+def scores_ref(x, tokens, top):
+    x = x.double().cpu()
+    m = x.amax(-1, keepdim=True)
+    z = torch.where(m == -INF, torch.full_like(x, -INF), x - m)  # nothing but -inf: no probability at all
+    # log of the sum, less the maximum's own 1: log(1 + 2e-24) is 0 in float64 where log1p(2e-24) is 2e-24
+    others = torch.exp(z).scatter(1, z.argmax(-1, keepdim=True), 0.0).sum(-1, keepdim=True)
+    others = torch.where(torch.isnan(m) | torch.isinf(m), m + m * 0.0, others)  # (NaN: no such row has a sum)
+    lp = torch.where(m == -INF, z, z - torch.log1p(others))
+    p = torch.exp(lp)
+    ent = -torch.where(p == 0, 0.0, p * lp).sum(-1)
+    order = torch.sort(torch.where(torch.isnan(x), -INF, x), dim=-1, descending=True, stable=True)[1][:, :top]
+    t = tokens.long().cpu()
+    given = lp.gather(1, t.clamp(0, x.shape[1] - 1))
+    given = torch.where(t == -1, 0.0, torch.where((t < 0) | (t >= x.shape[1]), NAN, given))
+    return given, ent, order.int(), lp.gather(1, order.long())
+
+
+def scores_check(r, x, tokens, top):
+    given, ent, order, best = scores_ref(x, tokens, top)
+    assert torch.equal(r.top_tokens.cpu(), order)
+    v = x.shape[1]
+    # x - m is exact to half a step of the range; the sum's terms are off by their arguments' rounding (exp of a
+    # rounded argument), the sum by 2 sqrt(v) / 2^24 at most; log1p and the last subtraction round once more
+    fin = x.double().cpu()
+    fin = torch.where(torch.isfinite(fin), fin, 0.0)
+    rng = float(fin.max() - fin.min()) + math.log(v) + 1
+    for got, ref in ((r.log_probs, given), (r.top_log_probs, best)):
+        got, ref = got.double().cpu(), ref
+        same = (got == ref) | (torch.isnan(got) & torch.isnan(ref))
+        tol = EPS * (4 * ref.abs().nan_to_num(0, 0, 0) + (8 + math.log2(v)) * 2 * (1 - torch.exp(ref)).abs().nan_to_num(0) + 1e-3)
+        off = (got - ref).abs()
+        assert (same | (off <= tol)).all(), (off / tol)[~same].max()
+    same = (r.entropy.double().cpu() == ent) | (torch.isnan(ent) & torch.isnan(r.entropy.cpu()))
+    tol = EPS * (16 + 2 * math.log2(v) + 2 * rng) * ent + 1e-37
+    off = (r.entropy.double().cpu() - ent).abs()
+    assert (same | (off <= tol)).all(), (off / tol)[~same].max()
+
+
+def logits(g, r, v, dtype, spread=3.0):
+    return (spread * randn(g, r, v)).to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("r,v,given,top", [
+    (1, 1, 1, 1), (3, 2, 2, 2), (1, 8194, 1, 10), (64, 8194, 7, 8), (5, 63, 3, 63), (5, 65, 3, 64), (2, 255, 1, 3), (2, 257, 1, 64),
+    (9, 1000, 1, 0), (2, 4097, 16, 20), (300, 513, 1, 5), (3, 60510, 1, 20), (1, 131072, 4, 64), (2, 200003, 2, 33),
+])
+def test_scores_match_float64(ops, dtype, r, v, given, top):
+    say(f"[gpu] scores {dtype} {r} x {v}, {given} given, top {top}")
+    g = gen(r * v + top)
+    x = logits(g, r, v, dtype)
+    tokens = torch.randint(0, v, (r, given), generator=g, device="cuda").int()
+    scores_check(ops.token_scores(x, tokens, top), x, tokens, top)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("v", [70, 8194, 40000])
+def test_scores_ties_masks_and_odd_values(ops, dtype, v):
+    say(f"[gpu] scores ties, masks and odd values {dtype} {v}")
+    g = gen(v)
+    x = logits(g, 12, v, dtype, 2.0)
+    x[0] = 1.5                                  # all alike
+    x[1] = -INF                                 # nothing allowed
+    x[2] = -INF
+    x[2, v - 1] = 2.0                           # one token
+    x[3, torch.randperm(v, generator=g, device="cuda")[: v // 2]] = -INF
+    x[4] = (x[4] * 2).round() / 2               # many ties
+    x[5] = torch.arange(v, device="cuda").to(dtype) / v        # rising: the best last
+    x[6] = -torch.arange(v, device="cuda").to(dtype) / v
+    x[7, v // 3] = NAN
+    x[8, 5] = INF
+    x[9, 3], x[9, 9] = -0.0, 0.0
+    x[9] = torch.where(x[9] > 0, -x[9], x[9])   # the zeros of both signs come first, in their order
+    x[10, v // 2] = 60.0                        # nearly all the probability: entropy near 0
+    x[11] = torch.finfo(dtype).min              # a mask of the type's lowest value, in every place but one
+    x[11, 7] = 0.0
+    tokens = torch.randint(0, v, (12, 5), generator=g, device="cuda").int()
+    tokens[:, 1] = -1
+    tokens[:, 2] = v - 1
+    tokens[::2, 3], tokens[1::2, 3] = v, -2
+    tokens[10, 4] = v // 2
+    for top in (1, 64):
+        scores_check(ops.token_scores(x, tokens, top), x, tokens, top)
+
+
+def test_scores_forms(ops):
+    """One token a row, none, rows with gaps and rows that do not start at 16 bytes."""
+    say("[gpu] scores forms")
+    g = gen(1)
+    for dtype in (F32, BF16, F16):
+        whole = logits(g, 6, 3011, dtype)
+        x = whole[:, 3:3000]
+        t = torch.randint(0, x.shape[1], (6, 4), generator=g, device="cuda").int()
+        scores_check(ops.token_scores(x, t[:, ::2][:, :1].contiguous(), 4), x, t[:, :1], 4)
+        r = ops.token_scores(x, t[:, 0].contiguous(), 4)
+        assert r.log_probs.shape == (6,)
+        assert torch.equal(r.log_probs, ops.token_scores(x, t, 0).log_probs[:, 0])
+        a, b = ops.token_scores(x, None, 4), ops.token_scores(x.contiguous(), t[:, 1:3], 4)
+        assert a.log_probs is None and torch.equal(a.top_tokens, b.top_tokens) and torch.equal(a.entropy, b.entropy)
+        scores_check(b, x, t[:, 1:3], 4)
+        assert ops.token_scores(x[:0], t[:0], 4).top_tokens.shape == (0, 4)
+
+
+# ---- kept rows -----------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("layers,b,h,d,rows", [(1, 1, 1, 64, 40), (3, 4, 5, 64, 300), (2, 3, 2, 128, 290), (1, 2, 3, 24, 60)])
+def test_keep_matches_copies(ops, dtype, layers, b, h, d, rows):
+    say(f"[gpu] keep {dtype} {layers} x {b} x {h} x {rows} x {d}")
+    g = gen(rows)
+    for n_path in (1, 2, 7, 33):
+        k, v = randn(g, layers, b, h, rows, d, dtype=dtype), randn(g, layers, b, h, rows, d, dtype=dtype)
+        lengths = torch.randint(0, max(1, rows - 40), (b,), generator=g, device="cuda").int()
+        path = torch.full((b, n_path), -1)
+        for i in range(b):
+            m = n_path - i % (n_path + 1)
+            path[i, :m] = torch.randperm(min(40, rows - int(lengths[i])))[:m].sort()[0]
+            if i == 1 and n_path > 2:
+                path[i] = torch.arange(n_path)  # nothing moves
+        wk, wv, want = k.clone(), v.clone(), lengths.clone()
+        for i in range(b):
+            for j, p in enumerate(path[i].tolist()):
+                if p < 0:
+                    break
+                wk[:, i, :, int(lengths[i]) + j] = k[:, i, :, int(lengths[i]) + p]
+                wv[:, i, :, int(lengths[i]) + j] = v[:, i, :, int(lengths[i]) + p]
+                want[i] += 1
+        new = ops.cache_keep(k, v, lengths, path.int().cuda())
+        assert torch.equal(new, want) and torch.equal(k, wk) and torch.equal(v, wv)
+
+
+def test_keep_refuses_paths_on_the_device(ops):
+    """Paths that do not rise or leave the cache, negative lengths: nothing moves, -1 comes back, and
+    the other sequences are served."""
+    say("[gpu] keep: paths out of order and out of range")
+    g = gen(5)
+    k, v = randn(g, 2, 7, 2, 50, 64), randn(g, 2, 7, 2, 50, 64)
+    k0, v0 = k.clone(), v.clone()
+    lengths = ints([10, 10, 10, -1, 50, 48, 2 ** 31 - 1])
+    path = ints([[0, 2, 2], [3, 1, -1], [0, 40, -1], [0, 1, 2], [0, -1, -1], [1, -1, 5], [0, 1, -1]])
+    new = ops.cache_keep(k, v, lengths, path)
+    assert new.tolist() == [-1, -1, -1, -1, -1, 49, -1]
+    k0[:, 5, :, 48], v0[:, 5, :, 48] = k0[:, 5, :, 49], v0[:, 5, :, 49]
+    assert torch.equal(k, k0) and torch.equal(v, v0)
+
+
+def test_keep_strides_and_four_dimensions(ops):
+    say("[gpu] keep strides")
+    g = gen(6)
+    base = randn(g, 3, 40, 2, 5, 64, dtype=BF16)
+    k = base.permute(0, 3, 2, 1, 4)           # [3][5][2][40][64], rows interleaved
+    v = randn(g, 3, 5, 2, 60, 80, dtype=BF16)[:, :, :, 4:44, 16:]
+    wk, wv = k.clone(), v.clone()
+    lengths, path = ints([3, 0, 30, 7, 12]), ints([[0, 4, 9]] * 5)
+    for i, n in enumerate(lengths.tolist()):
+        for j, p in enumerate((0, 4, 9)):
+            wk[:, i, :, n + j], wv[:, i, :, n + j] = k[:, i, :, n + p], v[:, i, :, n + p]
+    four_k, four_v = k[1].clone(), v[1].contiguous()
+    assert torch.equal(ops.cache_keep(k, v, lengths, path), lengths + 3)
+    assert torch.equal(k, wk) and torch.equal(v, wv)
+    assert torch.equal(ops.cache_keep(four_k, four_v, lengths, path), lengths + 3)
+    assert torch.equal(four_k, wk[1]) and torch.equal(four_v, wv[1])
+
+
+# ---- streams, graphs, refusals -----------------------------------------------------------------
+def drafted(ops, s):
+    """The three as they are used: a draft's attention, its scores, the accepted rows kept."""
+    o = ops.tree_attention(s["q"], s["k"], s["v"], s["lengths"], s["parents"])
+    r = ops.token_scores(o.flatten(2)[:, :, :500].reshape(-1, 500), s["tokens"], 5)
+    k, v = s["k"].clone(), s["v"].clone()
+    new = ops.cache_keep(k, v, s["lengths"], s["path"])
+    again = ops.tree_attention(s["q"], k, v, new, s["parents"])
+    return [o, r.log_probs, r.entropy, r.top_tokens, r.top_log_probs, k, v, new, again]
+
+
+def drafted_state(seed, rows=2600):
+    g = gen(seed)
+    ln = [rows - 20 - 100 * i for i in range(3)]
+    par = ints([shape_tree("tree", 9, seed + i) for i in range(3)])
+    return dict(q=randn(g, 3, 9, 8, 64), k=randn(g, 3, 8, rows, 64, dtype=BF16), v=randn(g, 3, 8, rows, 64, dtype=BF16),
+                lengths=ints(ln), parents=par, tokens=torch.randint(0, 500, (27, 2), generator=g, device="cuda").int(),
+                path=ints([[0, 3, 5], [0, -1, -1], [1, 2, 8]]))
+
+
+def test_run_of_all_three(ops):
+    say("[gpu] a draft's attention, scores and kept rows together")
+    s = drafted_state(11)
+    o, lp, ent, top, toplp, k, v, new, again = drafted(ops, s)
+    check(o, *attention_ref(s["q"], s["k"], s["v"], s["lengths"], s["parents"]))
+    x = o.flatten(2)[:, :, :500].reshape(-1, 500)
+    scores_check(ops.token_scores(x, s["tokens"], 5), x, s["tokens"], 5)
+    assert new.tolist() == [n + c for n, c in zip(s["lengths"].tolist(), (3, 1, 3))]
+    check(again, *attention_ref(s["q"], k, v, new, s["parents"]))
+
+
+def test_streams(ops):
+    """Two streams at once, and tensors made on another stream than the one that uses them."""
+    say("[gpu] operators on two streams")
+    states = [drafted_state(s) for s in (1, 2)]
+    want = [drafted(ops, s) for s in states]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in states]
+    for _ in range(3):
+        got = []
+        for st, s in zip(streams, states):
+            st.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(st):
+                got.append(drafted(ops, s))
+        torch.cuda.synchronize()
+        for a, b in zip(want, got):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_graphs(ops):
+    """Captured and replayed on new inputs, two graphs in one pool, eager work in between."""
+    say("[gpu] operators in graphs")
+    states = [drafted_state(s) for s in (3, 4)]
+    for s in states:
+        drafted(ops, s)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for s in states:
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            outs.append(drafted(ops, s))
+        graphs.append(gr)
+    for turn in range(3):
+        new = [drafted_state(10 + 2 * turn + i) for i in range(2)]
+        want = [drafted(ops, s) for s in new]
+        for s, n in zip(states, new):
+            for key in s:
+                s[key].copy_(n[key])
+        torch.cuda.synchronize()
+        for gr in graphs:
+            gr.replay()
+        drafted(ops, new[0])
+        torch.cuda.synchronize()
+        for a, b in zip(want, outs):
+            assert all(torch.equal(x, y) for x, y in zip(a, b)), turn
+
+
+def test_gpu_refusals(ops):
+    say("[gpu] operator refusals")
+    (q, k, v), ln, par = attention_case(ops, (F32, BF16), 2, 4, 4, 2, 64, [10, 20], "tree")
+
+    def refuses(match, f, *a, **kw):
+        with pytest.raises(H.ValidationError, match=match):
+            f(*a, **kw)
+
+    t = ops.tree_attention
+    refuses("lengths", t, q, k, v, ln.long(), par)
+    refuses("lengths", t, q, k, v, ln.cpu(), par)
+    refuses("parents", t, q, k, v, ln, par[:, :3])
+    refuses("k:", t, q, k[:1], v[:1], ln, par)
+    refuses("v:", t, q, k, v.float(), ln, par)
+    refuses("kv_dtype", t, q.half(), k, v, ln, par)
+    refuses("q:", t, q[..., ::2], k, v, ln, par)
+    wide = torch.zeros(2, 2, 24, 72, dtype=BF16, device="cuda")
+    refuses("k: rows", t, q, wide[..., 4:68], wide[..., :64], ln, par)
+    refuses("head_dim", t, q[..., :32], k[..., :32], v[..., :32], ln, par)
+    refuses("max_length", t, q, k, v, ln, par, max_length=1000)
+    refuses("max_seq", t, q, k, v, ln, par, max_length=0)
+    refuses("out", t, q, k, v, ln, par, out=q.half())
+    refuses("out: rows", t, q, k, v, ln, par, out=torch.empty(1, 4, 4, 64, device="cuda").expand(2, 4, 4, 64))
+    refuses("scale", t, q, k, v, ln, par, scale=NAN)
+    refuses("q: requires", t, q.clone().requires_grad_(), k, v, ln, par)
+    refuses("tokens", ops.token_scores, torch.zeros(2, 9, device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda"))
+    refuses("tokens", ops.token_scores, torch.zeros(2, 9, device="cuda"), torch.zeros(2, device="cuda"))
+    refuses("top_n", ops.token_scores, torch.zeros(2, 9, device="cuda"), top_n=10)
+    refuses("vocab", ops.token_scores, torch.zeros(2, 0, device="cuda"))
+    refuses("path", ops.cache_keep, k, v, ln, torch.zeros(1, 2, dtype=torch.int32, device="cuda"))
+    # host memory at a C entry, where the kernel would fault
+    import ctypes as C
+
+    host = torch.zeros(2, 9)
+    a = H.itts_token_scores_args(host.data_ptr(), None, None, None, None, None, 2, 9, 0, 0, H.ITTS_F32, 9, 0)
+    refuses("logits: not device memory", lambda: H._check(H.lib.itts_token_scores(C.byref(a), None, 0, None)))
+    assert ops.token_scores(torch.zeros(2, 9, device="cuda")).entropy.shape == (2,)  # and the next call works

@@ -1,0 +1,107 @@
+"""Refusals of the operators on device memory, without a GPU: wrong sizes, types, strides and
+alignments at the C entries, and wrong tensors at the Python ones."""
+import ctypes as C
+
+import pytest
+import torch
+
+import itts_hip as H
+from itts_hip import ops
+
+P = 1 << 20  # an address that nothing reads: every call below is refused before its memory matters
+
+
+def tree(**over):
+    f = dict(q=P, k=P, v=P, out=P, lengths=P, parents=P, batch=2, n_nodes=5, n_head=4, n_kv_head=2, head_dim=64, max_seq=100,
+             q_dtype=H.ITTS_F32, kv_dtype=H.ITTS_BF16, scale=0.125, q_batch=5 * 256, q_node=256, q_head=64, out_batch=5 * 256,
+             out_node=256, out_head=64, k_batch=12800, k_head=6400, k_row=64, v_batch=12800, v_head=6400, v_row=64,
+             parents_batch=5)
+    f.update(over)
+    return H.itts_tree_attention_args(**f)
+
+
+def scores(**over):
+    f = dict(logits=P, tokens=P, log_probs=P, entropy=P, top_tokens=P, top_log_probs=P, rows=3, vocab=100, n_tokens=1, top_n=5,
+             dtype=H.ITTS_F32, logits_row=100, tokens_row=1)
+    f.update(over)
+    return H.itts_token_scores_args(**f)
+
+
+def keep(**over):
+    f = dict(k=P, v=P, lengths=P, path=P, new_lengths=2 * P, n_layer=2, batch=3, n_head=4, max_seq=50, head_dim=64, n_path=4,
+             dtype=H.ITTS_BF16, k_layer=38400, k_batch=12800, k_head=3200, k_row=64, v_layer=38400, v_batch=12800, v_head=3200,
+             v_row=64, path_batch=4)
+    f.update(over)
+    return H.itts_cache_keep_args(**f)
+
+
+def call(kind, a):
+    if kind is tree:
+        return H._check(H.lib.itts_tree_attention(C.byref(a), None, 0, None))
+    if kind is scores:
+        return H._check(H.lib.itts_token_scores(C.byref(a), None, 0, None))
+    return H._check(H.lib.itts_cache_keep(C.byref(a), None))
+
+
+REFUSED = [
+    (tree, "batch", dict(batch=-1)), (tree, "batch", dict(batch=65536)), (tree, "n_nodes", dict(n_nodes=257)),
+    (tree, "n_nodes", dict(n_nodes=-1)), (tree, "n_kv_head", dict(n_kv_head=3)), (tree, "n_kv_head", dict(n_kv_head=0)),
+    (tree, "n_kv_head", dict(n_head=0)), (tree, "head_dim", dict(head_dim=80)), (tree, "max_seq", dict(max_seq=0)),
+    (tree, "scale", dict(scale=float("nan"))), (tree, "scale", dict(scale=float("inf"))),
+    (tree, "kv_dtype", dict(q_dtype=H.ITTS_BF16, kv_dtype=H.ITTS_F32)), (tree, "kv_dtype", dict(kv_dtype=H.ITTS_F16)),
+    (tree, "kv_dtype", dict(kv_dtype=9)), (tree, "q", dict(q=P + 8)), (tree, "q", dict(q_node=257)), (tree, "q", dict(q_head=-64)),
+    (tree, "k", dict(k_row=60)), (tree, "v", dict(v=P + 2)), (tree, "v", dict(v_head=6404)), (tree, "out", dict(out_head=0)),
+    (tree, "out", dict(out_node=2)), (tree, "parents", dict(parents_batch=-5)), (tree, "q, k, v", dict(q=None)),
+    (tree, "q, k, v", dict(lengths=None)), (tree, "k", dict(k_row=1 << 60)),
+    (scores, "rows", dict(rows=-1)), (scores, "vocab", dict(vocab=0)), (scores, "vocab", dict(vocab=(1 << 24) + 1)),
+    (scores, "n_tokens", dict(n_tokens=-1)), (scores, "top_n", dict(top_n=65)), (scores, "top_n", dict(top_n=4, vocab=3)),
+    (scores, "top_n", dict(top_n=-1)), (scores, "dtype", dict(dtype=0)), (scores, "logits", dict(logits=P + 2)),
+    (scores, "logits_row", dict(logits_row=-100)), (scores, "logits", dict(logits=None)), (scores, "logits", dict(tokens=None)),
+    (scores, "logits", dict(top_tokens=None)),
+    (keep, "batch", dict(batch=-1)), (keep, "n_layer", dict(n_layer=-1)), (keep, "n_layer", dict(max_seq=0)),
+    (keep, "dtype", dict(dtype=0)), (keep, "head_dim", dict(head_dim=12)), (keep, "k", dict(k_row=4)), (keep, "v", dict(v=P + 4)),
+    (keep, "k, v", dict(k_row=0)), (keep, "path", dict(path_batch=-1)), (keep, "k, v", dict(path=None)),
+    (keep, "new_lengths", dict(new_lengths=P)),
+]
+
+
+@pytest.mark.parametrize("kind,field,over", REFUSED, ids=lambda x: getattr(x, "__name__", str(x)))
+def test_c_entries_refuse(kind, field, over):
+    with pytest.raises(H.ValidationError) as e:
+        call(kind, kind(**over))
+    assert e.value.message.split(":")[0].startswith(field), e.value.message
+
+
+def test_null_arguments():
+    n = C.c_uint64()
+    for f in (H.lib.itts_tree_attention, H.lib.itts_token_scores):
+        with pytest.raises(H.ValidationError, match="args"):
+            H._check(f(None, None, 0, None))
+    with pytest.raises(H.ValidationError, match="args"):
+        H._check(H.lib.itts_cache_keep(None, None))
+    for f, a in ((H.lib.itts_tree_attention_workspace, tree()), (H.lib.itts_token_scores_workspace, scores())):
+        with pytest.raises(H.ValidationError, match="args"):
+            H._check(f(None, C.byref(n)))
+        with pytest.raises(H.ValidationError, match="bytes"):
+            H._check(f(C.byref(a), None))
+
+
+def test_empty_calls_do_nothing():
+    for a in (tree(batch=0, q=None), tree(n_nodes=0, q=None)):
+        call(tree, a)
+    call(scores, scores(rows=0, logits=None))
+    call(keep, keep(batch=0, k=None))
+
+
+def test_python_entries_refuse():
+    q = torch.zeros(1, 2, 4, 64)
+    for bad in (q, q[0], "q"):
+        with pytest.raises(H.ValidationError, match="^.*q:"):
+            ops.tree_attention(bad, q, q, torch.zeros(1, dtype=torch.int32), torch.zeros(1, 2, dtype=torch.int32))
+    with pytest.raises(H.ValidationError, match="logits: a GPU tensor"):
+        ops.token_scores(torch.zeros(2, 5))
+    with pytest.raises(H.ValidationError, match="logits: float32"):
+        ops.token_scores(torch.zeros(2, 5, dtype=torch.float64))
+    with pytest.raises(H.ValidationError, match="k: a GPU tensor"):
+        ops.cache_keep(torch.zeros(2, 1, 4, 8, 64), torch.zeros(2, 1, 4, 8, 64), torch.zeros(1, dtype=torch.int32),
+                       torch.zeros(1, 2, dtype=torch.int32))
