@@ -200,6 +200,15 @@ itts_status itts_gpt_teacher_forced(itts_gpt *gpt, itts_kv *kv, const int32_t *t
                                     int32_t n_text, const float *conds, int32_t n_cond,
                                     int32_t lang_id, const int32_t *codes, int32_t n_codes,
                                     float *log_probs_out, float *attention_out);
+/* itts_gpt_teacher_forced's log-probabilities with the entropy (nats) of the row that predicted each
+ * code, entropy_out [n_codes], and the top_n (<= 64) most probable codes there with their
+ * log-probabilities, [n_codes][top_n], as in itts_token_scores (no reference counterpart beyond
+ * code_log_probs).  Outputs that are NULL are left out (top_n 0 for the last two).  The cache is
+ * scratch and left empty. */
+itts_status itts_gpt_code_scores(itts_gpt *gpt, itts_kv *kv, const int32_t *text_tokens, int32_t n_text,
+                                 const float *conds, int32_t n_cond, int32_t lang_id, const int32_t *codes,
+                                 int32_t n_codes, int32_t top_n, float *log_probs_out, float *entropy_out,
+                                 int32_t *top_tokens_out, float *top_log_probs_out);
 /* Gpt::alignment_attention: replays codes after prior_codes through the first alignment
  * layers only and writes the text attention [n_codes][n_text + 2] averaged over the
  * alignment heads.  The cache is scratch and left empty. */
@@ -259,6 +268,26 @@ itts_status itts_generate_codes_after(itts_gpt *gpt, itts_kv *kv, const itts_cod
  * [batch][mel_vocab] (may be NULL).  Per sequence the result is Gpt::step's. */
 itts_status itts_gpt_step_batch(itts_gpt *gpt, itts_kv *const *caches, int32_t batch,
                                 const int32_t *tokens, const int32_t *positions, float *logits_out);
+/* ---- decoding with drafts (no reference counterpart) ---- */
+/* One decode step for a tree of drafted tokens behind the cache's rows: tokens[i] follows
+ * tokens[parents[i]] (parents[i] < i; -1: it follows the cached sequence) and stands at position
+ * pos_idx + its depth.  Every node sees the cached rows, its ancestors and itself, so that row i of
+ * logits_out [n_nodes][mel_vocab] is what itts_gpt_step would give after the path to node i, and
+ * every weight byte is read once for the whole tree.  1..256 nodes; valid_len + n_nodes rows must
+ * fit the cache.  The tree's rows lie behind valid_len, which does not change, until itts_kv_keep
+ * takes a path of them or another call on the cache drops them.
+ * Also, each where its pointer is set: log_probs_out [n_nodes], the log-probability of tokens[i]
+ * after its parent (0 for parents[i] = -1: an earlier call had its logits); entropy_out [n_nodes]
+ * and the top_n (<= 64) most probable next tokens with their log-probabilities
+ * [n_nodes][top_n] of the rows, as in itts_token_scores. */
+itts_status itts_gpt_step_tree(itts_gpt *gpt, itts_kv *kv, const int32_t *tokens, const int32_t *parents,
+                               int32_t n_nodes, int32_t pos_idx, int32_t top_n, float *logits_out,
+                               float *log_probs_out, float *entropy_out, int32_t *top_tokens_out,
+                               float *top_log_probs_out);
+/* Keeps nodes[0..n) of the cache's drafted tree, a path from a node that follows the sequence
+ * downwards: their rows become rows valid_len .. valid_len + n - 1, as if the tokens had been
+ * stepped one by one.  The rest of the tree is dropped; n 0 drops all of it. */
+itts_status itts_kv_keep(itts_kv *kv, const int32_t *nodes, int32_t n);
 /* generate_codes_after for `batch` sequences at once: each prompt is prefilled into its
  * cache, then the sequences are sampled and stepped together (one batched step per token)
  * until every one has stopped (STOP after its min_codes, or its max steps); a finished

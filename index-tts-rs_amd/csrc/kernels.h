@@ -323,6 +323,9 @@ struct TreeAttn {
 };
 size_t tree_attn_ws(const TreeAttn &a, int n_cu);
 hipError_t tree_attn(const TreeAttn &a, int n_cu, hipStream_t s);
+// The n nodes of a tree as the rows of a batched step: in = tokens [n], positions [n], parents [n], the
+// cache's length; node i's control block gets its token, position and row (length + i).
+hipError_t launch_tree_seqs(const int32_t *in, int n, BatchSeq *seqs, DecodeCtl *ctl, void *k, void *v, hipStream_t s);
 // Rows lengths[b] + path[b][i] -> lengths[b] + i of k and v [layers][batch][heads][max_seq][D], in
 // place; new_lengths[b] = lengths[b] + the path's entries before the first negative one (-1, and
 // nothing moved, where the path does not increase or leaves the cache).

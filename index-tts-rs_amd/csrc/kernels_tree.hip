@@ -396,6 +396,16 @@ hipError_t launch_t(const TreeAttn &a, const Plan &p, hipStream_t s) {
   return a.D == 64 ? launch_d<64, TQ, TKV>(a, p, s) : launch_d<128, TQ, TKV>(a, p, s);
 }
 
+__global__ void tree_seqs_kernel(const int32_t *in, int n, BatchSeq *seqs, DecodeCtl *ctl, void *k, void *v) {
+  const int i = blockIdx.x * 64 + threadIdx.x;
+  if (i >= n) return;
+  ctl[i].tok = in[i];
+  ctl[i].pos = in[n + i];
+  ctl[i].valid_len = in[3 * n] + i;
+  ctl[i].done = 0;
+  seqs[i] = BatchSeq{ctl + i, k, v, nullptr};
+}
+
 // ---- kept rows ----
 // A thread per 16-byte piece of a (layer, sequence, head)'s rows of K or V takes the path's rows in
 // order: row i is read before a later row can be written over it, since path[i] >= i and rises.
@@ -443,6 +453,11 @@ hipError_t tree_attn(const TreeAttn &a, int n_cu, hipStream_t s) {
   if (a.qt == kOpBf16 && a.kvt == kOpBf16) return launch_t<Bf16, Bf16>(a, p, s);
   if (a.qt == kOpF16 && a.kvt == kOpF16) return launch_t<F16, F16>(a, p, s);
   return hipErrorInvalidValue;
+}
+
+hipError_t launch_tree_seqs(const int32_t *in, int n, BatchSeq *seqs, DecodeCtl *ctl, void *k, void *v, hipStream_t s) {
+  hipLaunchKernelGGL(tree_seqs_kernel, dim3((n + 63) / 64), dim3(64), 0, s, in, n, seqs, ctl, k, v);
+  return hipGetLastError();
 }
 
 hipError_t cache_keep(const CacheKeep &a, hipStream_t s) {

@@ -234,6 +234,10 @@ struct itts_gpt {
   // the per-sequence descriptors and sampling parameters
   DevBuf bx, bq, blog, bseqs, bps;
   SplitBuf bh, ba, bf;
+  // drafted trees: the upload (tokens, positions, parents, length, given tokens) and its staging, the
+  // nodes' control blocks, attention rows (fp32) and split partials; scores and their workspace
+  DevBuf tin, tctl, tattn, tpart, tscore, tsws;
+  HostStage h_tree;
   // sampler API scratch
   DevBuf s_logits, s_seen, s_rng, s_tok;
   int ptype() const { return cfg.param_dtype == ITTS_F32 ? kParamF32 : kParamF16; }
@@ -244,6 +248,9 @@ struct itts_kv {
   int max_seq = 0;
   int kvt = kKvBf16;
   int valid_len = 0;
+  // parents of the drafted tree whose rows lie behind valid_len (itts_gpt_step_tree), until a node
+  // path of it is kept or anything else writes rows
+  std::vector<int32_t> tree;
   DevBuf k, v;         // [n_layer][n_head][max_seq][64]
   DevBuf ctl;          // DecodeCtl
   DevBuf part;         // attention split partials [n_head][splits][66]
@@ -710,6 +717,7 @@ itts_status run_prefill(itts_gpt *g, itts_kv *kv, const int32_t *text, int32_t n
   if (st) return st;
   const int T = n_cond + n_text + 3 + n_prior;
   kv->valid_len = 0;
+  kv->tree.clear();
   if (T > kv->max_seq)
     return set_error(ITTS_E_CAPACITY, "kv_cache: sequence length %d exceeds KV cache capacity %d", T,
                      kv->max_seq);
@@ -772,6 +780,7 @@ itts_status replay(itts_gpt *g, itts_kv *kv, const int32_t *text, int32_t n_text
   const itts_config &c = g->cfg;
   const int T = n_cond + n_text + 3 + (int)fed.size();
   kv->valid_len = 0;  // the cache is scratch (gpt.rs:819, 836)
+  kv->tree.clear();
   const itts_code_prompt p{text, n_text, conds, n_cond, lang, fed.empty() ? nullptr : fed.data(), (int32_t)fed.size(),
                            0};
   if (itts_status st = validate_prefix(c, text, n_text, conds, n_cond, g->max_cond, lang, p.prior_codes, p.n_prior))
@@ -814,9 +823,22 @@ itts_status check_replay_args(itts_gpt *g, itts_kv *kv, const int32_t *codes, in
   return ITTS_OK;
 }
 
+// Grows the batch workspace to B rows.
+itts_status ensure_batch(itts_gpt *g, int B) {
+  const itts_config &c = g->cfg;
+  const int d = c.d_model;
+  HIP_TRY(g->bx.ensure(sizeof(float) * (size_t)B * d));
+  HIP_TRY(g->bq.ensure(sizeof(float) * (size_t)B * d));
+  HIP_TRY(g->bh.ensure(B, d));
+  HIP_TRY(g->ba.ensure(B, d));
+  HIP_TRY(g->bf.ensure(B, c.d_ffn));
+  HIP_TRY(g->blog.ensure(sizeof(float) * (size_t)B * c.mel_vocab));
+  HIP_TRY(g->bseqs.ensure(sizeof(BatchSeq) * B));
+  return ITTS_OK;
+}
+
 // Checks a batch of caches and uploads their descriptors; grows the batch workspace.
 itts_status prepare_batch(itts_gpt *g, itts_kv *const *caches, int B) {
-  const itts_config &c = g->cfg;
   if (!caches || B <= 0 || B > 64) return set_error(ITTS_E_VALIDATION, "caches: 1..64 caches expected");
   std::vector<BatchSeq> seqs(B);
   for (int b = 0; b < B; b++) {
@@ -828,14 +850,7 @@ itts_status prepare_batch(itts_gpt *g, itts_kv *const *caches, int B) {
       if (caches[j] == kv) return set_error(ITTS_E_VALIDATION, "kv_cache: a cache appears twice in the batch");
     seqs[b] = BatchSeq{kv->ctl.as<DecodeCtl>(), kv->k.p, kv->v.p, kv->codes.as<int32_t>()};
   }
-  const int d = c.d_model;
-  HIP_TRY(g->bx.ensure(sizeof(float) * (size_t)B * d));
-  HIP_TRY(g->bq.ensure(sizeof(float) * (size_t)B * d));
-  HIP_TRY(g->bh.ensure(B, d));
-  HIP_TRY(g->ba.ensure(B, d));
-  HIP_TRY(g->bf.ensure(B, c.d_ffn));
-  HIP_TRY(g->blog.ensure(sizeof(float) * (size_t)B * c.mel_vocab));
-  HIP_TRY(g->bseqs.ensure(sizeof(BatchSeq) * B));
+  if (itts_status st = ensure_batch(g, B)) return st;
   HIP_TRY(hipMemcpyAsync(g->bseqs.p, seqs.data(), sizeof(BatchSeq) * B, hipMemcpyHostToDevice, g->stream));
   HIP_TRY(hipStreamSynchronize(g->stream));
   return ITTS_OK;
@@ -845,7 +860,39 @@ itts_status prepare_batch(itts_gpt *g, itts_kv *const *caches, int B) {
 // and cache lengths read from their control blocks): logits land in gpt->blog [B][V] and
 // every unfinished sequence's cache length advances.  The linears run as M = B GEMMs, so
 // each weight byte is read once per step for the whole batch.
-itts_status enqueue_step_batch(itts_gpt *g, int B, int max_seq, int kvt) {
+// With tree set the rows are the B nodes of a drafted tree behind one cache's rows (gpt->bseqs
+// describes one node each, its length the node's row): attention is the tree's, and no length advances.
+struct TreeStep {
+  const itts_kv *kv;
+  const int32_t *parents, *length;  // device
+};
+// The attention of layer l over the n nodes' queries in gpt->bq, into gpt->tattn [n][d].
+TreeAttn tree_attn_args(const itts_gpt *g, const TreeStep &t, int l, int n) {
+  const itts_config &c = g->cfg;
+  const int64_t d = c.d_model, head = (int64_t)t.kv->max_seq * 64;
+  TreeAttn a{};
+  a.q = g->bq.p;
+  a.k = t.kv->k_layer(l);
+  a.v = t.kv->v_layer(l);
+  a.out = g->tattn.p;
+  a.lengths = t.length;
+  a.parents = t.parents;
+  a.batch = 1;
+  a.n = n;
+  a.H = a.Hk = c.n_head;
+  a.D = kHeadDim;
+  a.max_seq = t.kv->valid_len + n;
+  a.qt = kOpF32;
+  a.kvt = t.kv->kvt == kKvBf16 ? kOpBf16 : kOpF32;
+  a.scale = 0.125f;
+  a.q_n = a.o_n = d;
+  a.q_h = a.o_h = 64;
+  a.k_h = a.v_h = head;
+  a.k_r = a.v_r = 64;
+  a.part = g->tpart.as<float>();
+  return a;
+}
+itts_status enqueue_step_batch(itts_gpt *g, int B, int max_seq, int kvt, const TreeStep *tree = nullptr) {
   const itts_config &c = g->cfg;
   const int d = c.d_model, bits = c.quant_bits, pt = g->ptype();
   hipStream_t s = g->stream;
@@ -867,8 +914,13 @@ itts_status enqueue_step_batch(itts_gpt *g, int B, int max_seq, int kvt) {
       HIP_TRY(launch_ln_rows(X, L.ln1_w, L.ln1_b, B, d, g->bh.out(), s));
     ga.qkv = QkvDst{g->bq.as<float>(), nullptr, nullptr, max_seq, 0, d, seqs, layer_elems * l};
     HIP_TRY(launch_gemm(ga, bits, pt, kEpiQKV, kvt, s));
-    HIP_TRY(launch_decode_batch_rows(g->bq.as<float>(), seqs, B, layer_elems * l, c.n_head, max_seq, g->ba.out(),
-                                     kvt, s));
+    if (tree) {
+      HIP_TRY(tree_attn(tree_attn_args(g, *tree, l, B), g->n_cu, s));
+      HIP_TRY(launch_split_rows(g->tattn.as<float>(), B, d, g->ba.out(), s));
+    } else {
+      HIP_TRY(launch_decode_batch_rows(g->bq.as<float>(), seqs, B, layer_elems * l, c.n_head, max_seq, g->ba.out(),
+                                       kvt, s));
+    }
     ga = gemm_args(g, g->qls[4 * (size_t)l + 1], g->ba.act(), B);
     ga.y = X;
     HIP_TRY(launch_gemm(ga, bits, pt, kEpiResid, kvt, s));
@@ -888,13 +940,66 @@ itts_status enqueue_step_batch(itts_gpt *g, int B, int max_seq, int kvt) {
   GemmArgs ga = gemm_args(g, g->qls[4 * (size_t)c.n_layer], g->bh.act(), B);
   ga.y = g->blog.as<float>();
   HIP_TRY(launch_gemm(ga, bits, pt, kEpiStore, kvt, s));
-  HIP_TRY(launch_advance_batch(seqs, B, s));
+  if (!tree) HIP_TRY(launch_advance_batch(seqs, B, s));
   return ITTS_OK;
+}
+
+// Scores of R rows of logits [R][mel_vocab] on the device (kernels_scores.hip), with `given` tokens a
+// row at tokens; the outputs that are asked for come back to the host after one synchronisation.
+itts_status score_rows(itts_gpt *g, const float *logits, int R, const int32_t *tokens, int given, int top_n,
+                       float *log_probs, float *entropy, int32_t *top_tokens, float *top_log_probs) {
+  const size_t n_lp = (size_t)R * given, n_top = (size_t)R * top_n;
+  HIP_TRY(g->tscore.ensure(sizeof(float) * (n_lp + R + 2 * n_top)));
+  TokenScores a{};
+  a.x = logits;
+  a.tokens = tokens;
+  a.log_probs = g->tscore.as<float>();
+  a.entropy = a.log_probs + n_lp;
+  a.top_log_probs = a.entropy + R;
+  a.top_tokens = reinterpret_cast<int32_t *>(a.top_log_probs + n_top);
+  a.rows = R;
+  a.vocab = g->cfg.mel_vocab;
+  a.given = given;
+  a.top = top_n;
+  a.type = kOpF32;
+  a.x_row = g->cfg.mel_vocab;
+  a.tok_row = given;
+  HIP_TRY(g->tsws.ensure(token_scores_ws(a, g->n_cu)));
+  a.ws = g->tsws.p;
+  HIP_TRY(token_scores(a, g->n_cu, g->stream));
+  auto back = [&](void *to, const void *from, size_t n) {
+    return to && n ? hipMemcpyAsync(to, from, 4 * n, hipMemcpyDeviceToHost, g->stream) : hipSuccess;
+  };
+  HIP_TRY(back(log_probs, a.log_probs, n_lp));
+  HIP_TRY(back(entropy, a.entropy, R));
+  HIP_TRY(back(top_tokens, a.top_tokens, n_top));
+  HIP_TRY(back(top_log_probs, a.top_log_probs, n_top));
+  HIP_TRY(hipStreamSynchronize(g->stream));
+  return ITTS_OK;
+}
+
+itts_status check_top(const itts_gpt *g, int32_t top_n, const int32_t *top_tokens, const float *top_log_probs) {
+  if (top_n < 0 || top_n > kScoresMaxTop || top_n > g->cfg.mel_vocab)
+    return set_error(ITTS_E_VALIDATION, "top_n: must be in 0..=%d, got %d", std::min(kScoresMaxTop, g->cfg.mel_vocab),
+                     top_n);
+  if (top_n > 0 && (!top_tokens || !top_log_probs)) return set_error(ITTS_E_VALIDATION, "top_n: null output");
+  return ITTS_OK;
+}
+
+// No exception leaves the library (host memory may run out in a container).
+template <class F>
+itts_status guarded(F f) {
+  try {
+    return f();
+  } catch (...) {
+    return set_error(ITTS_E_INTERNAL, "out of host memory");
+  }
 }
 
 // Writes the host-known fields of the decode control block (the device-owned step
 // counter that follows them is left alone).
 itts_status write_ctl(itts_kv *kv, const DecodeCtl &h) {
+  kv->tree.clear();  // (the step that follows writes over a drafted tree's rows)
   *kv->host_ctl = h;
   HIP_TRY(hipMemcpyAsync(kv->ctl.p, kv->host_ctl, offsetof(DecodeCtl, xstep), hipMemcpyHostToDevice,
                          kv->gpt->stream));
@@ -1270,7 +1375,9 @@ void itts_kv_destroy(itts_kv *kv) {
 }
 
 void itts_kv_reset(itts_kv *kv) {
-  if (kv) kv->valid_len = 0;
+  if (!kv) return;
+  kv->valid_len = 0;
+  kv->tree.clear();
 }
 int32_t itts_kv_valid_len(const itts_kv *kv) { return kv ? kv->valid_len : 0; }
 int32_t itts_kv_max_seq(const itts_kv *kv) { return kv ? kv->max_seq : 0; }
@@ -1346,6 +1453,26 @@ itts_status itts_gpt_teacher_forced(itts_gpt *gpt, itts_kv *kv, const int32_t *t
   HIP_TRY(hipStreamSynchronize(gpt->stream));
   kv->valid_len = 0;
   return ITTS_OK;
+}
+
+itts_status itts_gpt_code_scores(itts_gpt *gpt, itts_kv *kv, const int32_t *text_tokens, int32_t n_text, const float *conds,
+                                 int32_t n_cond, int32_t lang_id, const int32_t *codes, int32_t n_codes, int32_t top_n,
+                                 float *log_probs_out, float *entropy_out, int32_t *top_tokens_out, float *top_log_probs_out) {
+  return guarded([&]() -> itts_status {
+    if (itts_status st = check_replay_args(gpt, kv, codes, n_codes)) return st;
+    if (itts_status st = check_top(gpt, top_n, top_tokens_out, top_log_probs_out)) return st;
+    // the rows of itts_gpt_teacher_forced
+    const std::vector<int32_t> fed(codes, codes + n_codes - 1);
+    int T = 0;
+    if (itts_status st = replay(gpt, kv, text_tokens, n_text, conds, n_cond, lang_id, fed, n_cond + n_text + 2, gpt->cfg.n_layer,
+                                n_codes, nullptr, &T))
+      return st;
+    if (itts_status st = head_rows(gpt, n_cond + n_text + 2, n_codes)) return st;
+    HIP_TRY(gpt->pcodes.ensure(sizeof(int32_t) * n_codes));
+    HIP_TRY(hipMemcpyAsync(gpt->pcodes.p, codes, sizeof(int32_t) * n_codes, hipMemcpyHostToDevice, gpt->stream));
+    return score_rows(gpt, gpt->plog.as<float>(), n_codes, gpt->pcodes.as<int32_t>(), 1, top_n, log_probs_out, entropy_out,
+                      top_tokens_out, top_log_probs_out);
+  });
 }
 
 itts_status itts_gpt_alignment_attention(itts_gpt *gpt, itts_kv *kv, const int32_t *text_tokens, int32_t n_text,
@@ -1737,6 +1864,115 @@ itts_status itts_gpt_step_batch(itts_gpt *gpt, itts_kv *const *caches, int32_t b
   HIP_TRY(hipStreamSynchronize(gpt->stream));
   for (int b = 0; b < batch; b++) caches[b]->valid_len += 1;
   return ITTS_OK;
+}
+
+itts_status itts_gpt_step_tree(itts_gpt *gpt, itts_kv *kv, const int32_t *tokens, const int32_t *parents,
+                               int32_t n_nodes, int32_t pos_idx, int32_t top_n, float *logits_out, float *log_probs_out,
+                               float *entropy_out, int32_t *top_tokens_out, float *top_log_probs_out) {
+  return guarded([&]() -> itts_status {
+    if (!gpt || !kv || kv->gpt != gpt) return set_error(ITTS_E_VALIDATION, "kv_cache: cache belongs to another decoder");
+    if (!tokens || !parents) return set_error(ITTS_E_VALIDATION, "tokens: null tokens or parents");
+    if (n_nodes < 1 || n_nodes > kTreeMaxNodes)
+      return set_error(ITTS_E_VALIDATION, "n_nodes: must be in 1..=%d, got %d", kTreeMaxNodes, n_nodes);
+    const itts_config &c = gpt->cfg;
+    if (itts_status st = check_top(gpt, top_n, top_tokens_out, top_log_probs_out)) return st;
+    std::vector<int32_t> pos(n_nodes), slot(n_nodes, 0), children(n_nodes, 0);
+    int given = 0;
+    for (int i = 0; i < n_nodes; i++) {
+      if (tokens[i] < 0 || tokens[i] >= c.mel_vocab)
+        return set_error(ITTS_E_VALIDATION, "mel_token_id: mel_token_id %d out of range 0..%d", tokens[i], c.mel_vocab);
+      if (parents[i] < -1 || parents[i] >= i)
+        return set_error(ITTS_E_VALIDATION, "parents: node %d follows node %d (-1 or an earlier node expected)", i, parents[i]);
+      const int64_t p = parents[i] < 0 ? (int64_t)pos_idx : (int64_t)pos[parents[i]] + 1;
+      if (p < 0 || p >= c.mel_pos_len)
+        return set_error(ITTS_E_VALIDATION, "pos_idx: pos_idx %lld out of range 0..%d", (long long)p, c.mel_pos_len);
+      pos[i] = (int32_t)p;
+      if (parents[i] >= 0) slot[i] = children[parents[i]]++, given = std::max(given, slot[i] + 1);
+    }
+    if (n_nodes > kv->max_seq - kv->valid_len)
+      return set_error(ITTS_E_CAPACITY, "kv_cache: sequence length %d exceeds KV cache capacity %d", kv->valid_len + n_nodes,
+                       kv->max_seq);
+    const bool scored = log_probs_out || entropy_out || top_n > 0;
+    if (!log_probs_out) given = 0;
+    kv->tree.clear();
+    std::vector<int32_t> parents_kept(parents, parents + n_nodes);
+    // one upload: tokens, positions, parents, the length, every row's children's tokens
+    const int n = n_nodes;
+    const size_t words = 3 * (size_t)n + 1 + (size_t)n * given;
+    if (itts_status st = ensure_batch(gpt, n)) return st;
+    HIP_TRY(gpt->tin.ensure(sizeof(int32_t) * words));
+    HIP_TRY(gpt->tctl.ensure(sizeof(DecodeCtl) * n));
+    HIP_TRY(gpt->tattn.ensure(sizeof(float) * (size_t)n * c.d_model));
+    HIP_TRY(gpt->h_tree.acquire(sizeof(int32_t) * words));
+    int32_t *h = gpt->h_tree.as<int32_t>();
+    memcpy(h, tokens, sizeof(int32_t) * n);
+    memcpy(h + n, pos.data(), sizeof(int32_t) * n);
+    memcpy(h + 2 * n, parents, sizeof(int32_t) * n);
+    h[3 * n] = kv->valid_len;
+    int32_t *table = h + 3 * n + 1;
+    for (size_t i = 0; i < (size_t)n * given; i++) table[i] = -1;
+    if (given)
+      for (int i = 0; i < n; i++)
+        if (parents[i] >= 0) table[(size_t)parents[i] * given + slot[i]] = tokens[i];
+    HIP_TRY(hipMemcpyAsync(gpt->tin.p, h, sizeof(int32_t) * words, hipMemcpyHostToDevice, gpt->stream));
+    HIP_TRY(gpt->h_tree.release(gpt->stream));
+    const int32_t *din = gpt->tin.as<int32_t>();
+    const TreeStep tree{kv, din + 2 * n, din + 3 * n};
+    HIP_TRY(gpt->tpart.ensure(sizeof(float) * tree_attn_ws(tree_attn_args(gpt, tree, 0, n), gpt->n_cu)));
+    HIP_TRY(launch_tree_seqs(din, n, gpt->bseqs.as<BatchSeq>(), gpt->tctl.as<DecodeCtl>(), kv->k.p, kv->v.p, gpt->stream));
+    if (itts_status st = enqueue_step_batch(gpt, n, kv->max_seq, kv->kvt, &tree)) return st;
+    if (logits_out)
+      HIP_TRY(hipMemcpyAsync(logits_out, gpt->blog.p, sizeof(float) * (size_t)n * c.mel_vocab, hipMemcpyDeviceToHost,
+                             gpt->stream));
+    std::vector<float> lp((size_t)n * given);
+    if (scored) {
+      if (itts_status st = score_rows(gpt, gpt->blog.as<float>(), n, din + 3 * n + 1, given, top_n, lp.data(), entropy_out,
+                                      top_tokens_out, top_log_probs_out))
+        return st;
+      if (log_probs_out)
+        for (int i = 0; i < n; i++) log_probs_out[i] = parents[i] < 0 ? 0.0f : lp[(size_t)parents[i] * given + slot[i]];
+    }
+    HIP_TRY(hipStreamSynchronize(gpt->stream));
+    kv->tree.swap(parents_kept);
+    return ITTS_OK;
+  });
+}
+
+itts_status itts_kv_keep(itts_kv *kv, const int32_t *nodes, int32_t n) {
+  return guarded([&]() -> itts_status {
+    if (!kv || n < 0 || (n > 0 && !nodes)) return set_error(ITTS_E_VALIDATION, "nodes: null argument");
+    itts_gpt *g = kv->gpt;
+    const int size = (int)kv->tree.size();
+    if (size == 0) return set_error(ITTS_E_VALIDATION, "kv_cache: no drafted tree lies behind its rows");
+    bool moves = false;
+    for (int i = 0, last = -1; i < n; last = nodes[i++]) {
+      if (nodes[i] < 0 || nodes[i] >= size)
+        return set_error(ITTS_E_VALIDATION, "nodes: node %d out of range 0..%d", nodes[i], size);
+      if (kv->tree[nodes[i]] != last)
+        return set_error(ITTS_E_VALIDATION, "nodes: node %d follows node %d, not node %d", nodes[i], kv->tree[nodes[i]], last);
+      moves = moves || nodes[i] != i;
+    }
+    if (moves) {
+      const itts_config &c = g->cfg;
+      HIP_TRY(g->tin.ensure(sizeof(int32_t) * (n + 2)));
+      HIP_TRY(g->h_tree.acquire(sizeof(int32_t) * (n + 1)));
+      int32_t *h = g->h_tree.as<int32_t>();
+      h[0] = kv->valid_len;
+      memcpy(h + 1, nodes, sizeof(int32_t) * n);
+      HIP_TRY(hipMemcpyAsync(g->tin.p, h, sizeof(int32_t) * (n + 1), hipMemcpyHostToDevice, g->stream));
+      HIP_TRY(g->h_tree.release(g->stream));
+      const int row = 64 * (kv->kvt == kKvBf16 ? 2 : 4) / 16;  // 16-byte pieces
+      const int64_t head = (int64_t)kv->max_seq * row, layer = head * c.n_head;
+      int32_t *din = g->tin.as<int32_t>();
+      const CacheKeep a{kv->k.p, kv->v.p, din, din + 1, din + n + 1, c.n_layer, 1, c.n_head, kv->max_seq, row, n,
+                        layer, 0, head, row, layer, 0, head, row, 0};
+      HIP_TRY(cache_keep(a, g->stream));
+      HIP_TRY(hipStreamSynchronize(g->stream));
+    }
+    kv->valid_len += n;
+    kv->tree.clear();
+    return ITTS_OK;
+  });
 }
 
 itts_status itts_generate_codes_batch(itts_gpt *gpt, itts_kv *const *caches, const itts_code_prompt *prompts,

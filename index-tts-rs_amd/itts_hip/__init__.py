@@ -22,6 +22,7 @@ from __future__ import annotations
 import ctypes as C
 import os
 from dataclasses import dataclass
+from typing import NamedTuple
 
 import numpy as np
 
@@ -165,6 +166,12 @@ _SIGS = {
     "itts_gpt_alignment_attention": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p,
                                                C.c_int32, C.c_int32, C.c_void_p, C.c_int32, C.c_void_p,
                                                C.c_int32, C.c_void_p]),
+    "itts_gpt_code_scores": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_int32, C.c_int32,
+                                       C.c_void_p, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p,
+                                       C.c_void_p]),
+    "itts_gpt_step_tree": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_int32,
+                                     C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "itts_kv_keep": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32]),
     "itts_gpt_set_alignment_heads": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32]),
     "itts_gpt_forward_logits": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p]),
     "itts_gpt_step_batch": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p]),
@@ -313,6 +320,21 @@ class SeenTokenBitSet:
 # Decoder
 # ----------------------------------------------------------------------------------
 
+class TokenScores(NamedTuple):
+    """Scores of rows of logits: log-probabilities of given tokens [rows], entropy in nats [rows], the
+    most probable tokens [rows][top_n] and their log-probabilities."""
+    log_probs: np.ndarray
+    entropy: np.ndarray
+    top_tokens: np.ndarray
+    top_log_probs: np.ndarray
+
+
+def _scores_out(rows: int, top_n: int) -> TokenScores:
+    n = max(0, min(int(top_n), 64))  # (the library refuses what is outside)
+    return TokenScores(np.empty(rows, np.float32), np.empty(rows, np.float32), np.empty((rows, n), np.int32),
+                       np.empty((rows, n), np.float32))
+
+
 class Gpt:
     """Gpt::from_weights over a weights description (see itts_hip.synth.ModelWeights)."""
 
@@ -401,6 +423,31 @@ class Gpt:
     def code_log_probs(self, text_tokens, conds, lang_id, codes, cache):
         return self.teacher_forced(text_tokens, conds, lang_id, codes, cache, attention=False)[0]
 
+    def code_scores(self, text_tokens, conds, lang_id, codes, cache, top_n=0):
+        """code_log_probs with the entropy of each code's row and its top_n most probable codes."""
+        t, c = self._tc(text_tokens, conds)
+        cd = np.ascontiguousarray(codes, dtype=np.int32)
+        r = _scores_out(len(cd), top_n)
+        _check(lib.itts_gpt_code_scores(self._h, cache._h, _ptr(t), len(t), _ptr(c), c.shape[0], int(lang_id), _ptr(cd),
+                                        len(cd), int(top_n), _ptr(r.log_probs), _ptr(r.entropy), _ptr(r.top_tokens),
+                                        _ptr(r.top_log_probs)))
+        return r
+
+    def step_tree(self, cache, tokens, parents, pos_idx, logits=True, scores=False, top_n=0):
+        """One step for a tree of drafted tokens behind the cache's rows: tokens[i] follows
+        tokens[parents[i]] (-1: the cached sequence) at position pos_idx + its depth.  Returns
+        (logits [n][mel_vocab] or None, TokenScores of the nodes or None); cache.keep(path) then takes
+        the accepted nodes."""
+        t = np.ascontiguousarray(tokens, dtype=np.int32)
+        p = np.ascontiguousarray(parents, dtype=np.int32)
+        if t.ndim != 1 or t.shape != p.shape:
+            raise ValidationError(ITTS_E_VALIDATION, f"parents: as many as tokens expected, got {p.shape} and {t.shape}")
+        out = np.empty((len(t), self.cfg["mel_vocab"]), np.float32) if logits else None
+        r = _scores_out(len(t), top_n) if scores or top_n else TokenScores(None, None, None, None)
+        _check(lib.itts_gpt_step_tree(self._h, cache._h, _ptr(t), _ptr(p), len(t), int(pos_idx), int(top_n), _ptr(out),
+                                      _ptr(r.log_probs), _ptr(r.entropy), _ptr(r.top_tokens), _ptr(r.top_log_probs)))
+        return out, (r if scores or top_n else None)
+
     def alignment_attention(self, text_tokens, conds, lang_id, prior_codes, codes, cache):
         t, c = self._tc(text_tokens, conds)
         pr = np.ascontiguousarray(prior_codes if prior_codes is not None else [], dtype=np.int32)
@@ -473,6 +520,12 @@ class KvCache:
 
     def max_seq(self) -> int:
         return lib.itts_kv_max_seq(self._h)
+
+    def keep(self, nodes):
+        """Keeps a path of the drafted tree of the last step_tree (its nodes from the first one down);
+        an empty one drops the tree."""
+        a = np.ascontiguousarray(nodes, dtype=np.int32).reshape(-1)
+        _check(lib.itts_kv_keep(self._h, _ptr(a), len(a)))
 
     def decode_path(self) -> int:
         return lib.itts_kv_decode_path(self._h)

@@ -280,6 +280,10 @@ extern "C" {
                                    conds: *const f32, n_cond: i32, lang_id: i32, codes: *const i32,
                                    n_codes: i32, log_probs_out: *mut f32, attention_out: *mut f32)
         -> itts_status;
+    pub fn itts_gpt_code_scores(gpt: *mut itts_gpt, kv: *mut itts_kv, text_tokens: *const i32, n_text: i32,
+                                conds: *const f32, n_cond: i32, lang_id: i32, codes: *const i32, n_codes: i32,
+                                top_n: i32, log_probs_out: *mut f32, entropy_out: *mut f32,
+                                top_tokens_out: *mut i32, top_log_probs_out: *mut f32) -> itts_status;
     pub fn itts_gpt_alignment_attention(gpt: *mut itts_gpt, kv: *mut itts_kv, text_tokens: *const i32,
                                         n_text: i32, conds: *const f32, n_cond: i32, lang_id: i32,
                                         prior_codes: *const i32, n_prior: i32, codes: *const i32,
@@ -305,6 +309,11 @@ extern "C" {
                                      codes_cap: i32, n_codes: *mut i32) -> itts_status;
     pub fn itts_gpt_step_batch(gpt: *mut itts_gpt, caches: *const *mut itts_kv, batch: i32, tokens: *const i32,
                                positions: *const i32, logits_out: *mut f32) -> itts_status;
+    pub fn itts_gpt_step_tree(gpt: *mut itts_gpt, kv: *mut itts_kv, tokens: *const i32, parents: *const i32,
+                              n_nodes: i32, pos_idx: i32, top_n: i32, logits_out: *mut f32,
+                              log_probs_out: *mut f32, entropy_out: *mut f32, top_tokens_out: *mut i32,
+                              top_log_probs_out: *mut f32) -> itts_status;
+    pub fn itts_kv_keep(kv: *mut itts_kv, nodes: *const i32, n: i32) -> itts_status;
     pub fn itts_generate_codes_batch(gpt: *mut itts_gpt, caches: *const *mut itts_kv,
                                      prompts: *const itts_code_prompt, params: *const itts_sampling, batch: i32,
                                      rng_states: *mut u64, codes_out: *mut i32, codes_cap: i32,
