@@ -9,16 +9,14 @@
 // second product, O^T = V^T P^T, as they stand, when V's rows are read in the same key order.
 // Softmax statistics stay in the lanes (max over the four lane groups of a column by two
 // exchanges, sums only at the end).
-#include <hip/hip_bf16.h>
-
 #include <algorithm>
+#include <type_traits>
 
+#include "frag.h"
 #include "kernels.h"
 
 namespace itts {
 namespace {
-
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kWaves = 4;       // waves of a block, each over its own tiles of keys
 constexpr int kTileKeys = 32;   // keys a wave takes at a time
@@ -29,56 +27,47 @@ struct F32 {
 };
 struct Bf16 {
   static constexpr int kBytes = 2;
+  static constexpr uint32_t kOddBits = 0x7f80u;  // exponent of infinities and NaN
 };
 struct F16 {
   static constexpr int kBytes = 2;
+  static constexpr uint32_t kOddBits = 0x7c00u;
 };
 
-// N consecutive elements at p (16-byte aligned where N elements fill 16 bytes) as floats.
-template <class T, int N>
-__device__ __forceinline__ void load_row(const void *p, float *o) {
-  if constexpr (T::kBytes == 4) {
+// One element at p as a float.
+template <class T>
+__device__ __forceinline__ float load1(const char *p) {
+  if constexpr (T::kBytes == 4) return *reinterpret_cast<const float *>(p);
+  else if constexpr (std::is_same_v<T, Bf16>) return bf16_bits_to_float(*reinterpret_cast<const uint16_t *>(p));
+  else return half_bits_to_float(*reinterpret_cast<const uint16_t *>(p));
+}
+
+// N dwords at p (16-byte aligned where they fill 16 bytes).
+template <int N>
+__device__ __forceinline__ void load_dwords(const char *p, uint32_t (&o)[N]) {
+  if constexpr (N == 2) {
+    const u32x2 v = *reinterpret_cast<const u32x2 *>(p);
+    o[0] = v[0], o[1] = v[1];
+  } else {
 #pragma unroll
     for (int i = 0; i < N; i += 4) {
-      const float4 v = *reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i);
-      o[i] = v.x, o[i + 1] = v.y, o[i + 2] = v.z, o[i + 3] = v.w;
-    }
-  } else {
-    uint32_t w[N / 2];
-#pragma unroll
-    for (int i = 0; i < N / 2; i += (N >= 8 ? 4 : 2)) {
-      if constexpr (N >= 8) {
-        const uint4 v = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p) + 2 * i);
-        w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
-      } else {
-        const uint2 v = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(p) + 2 * i);
-        w[i] = v.x, w[i + 1] = v.y;
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < N / 2; i++) {
-      if constexpr (std::is_same_v<T, Bf16>) {
-        o[2 * i] = __uint_as_float(w[i] << 16);
-        o[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-      } else {
-        o[2 * i] = half_bits_to_float(w[i] & 0xffffu);
-        o[2 * i + 1] = half_bits_to_float(w[i] >> 16);
-      }
+      const u32x4 v = *reinterpret_cast<const u32x4 *>(p + 4 * i);
+      o[i] = v[0], o[i + 1] = v[1], o[i + 2] = v[2], o[i + 3] = v[3];
     }
   }
 }
 
-// One rounding to the output's type.
+// Four values, one rounding to the output's type.
 template <class T>
-__device__ __forceinline__ void store4(void *p, float a, float b, float c, float d) {
+__device__ __forceinline__ void store4(char *p, float a, float b, float c, float d) {
   if constexpr (T::kBytes == 4) {
-    *static_cast<float4 *>(p) = make_float4(a, b, c, d);
+    *reinterpret_cast<float4 *>(p) = make_float4(a, b, c, d);
   } else if constexpr (std::is_same_v<T, Bf16>) {
-    *static_cast<uint2 *>(p) = make_uint2(float_to_bf16_bits(a) | float_to_bf16_bits(b) << 16,
-                                          float_to_bf16_bits(c) | float_to_bf16_bits(d) << 16);
+    const bf16x2v x = __builtin_convertvector((f32x2e){a, b}, bf16x2v), y = __builtin_convertvector((f32x2e){c, d}, bf16x2v);
+    *reinterpret_cast<uint2 *>(p) = make_uint2(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, y));
   } else {
     const f16x2v x = __builtin_convertvector((f32x2e){a, b}, f16x2v), y = __builtin_convertvector((f32x2e){c, d}, f16x2v);
-    *static_cast<uint2 *>(p) = make_uint2(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, y));
+    *reinterpret_cast<uint2 *>(p) = make_uint2(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, y));
   }
 }
 
@@ -91,191 +80,405 @@ __device__ __forceinline__ float col_sum(float v) {
   return v + __shfl_xor(v, 32, 64);
 }
 
+// The pair (a, b) as planes of 16-bit values, the first in the low half: plane 0 holds the leading
+// bits (cut, not rounded), the next what is left, so that every plane has its value's sign.  A
+// rest of exactly 0 becomes the smallest number of that sign: 0 times an infinity in the other
+// operand would turn what is an infinity into NaN.  bf16: 8 bits a plane, three hold a float;
+// fp16: 11 bits, two planes 22.
+template <class T, int N>
+__device__ __forceinline__ void cut2(float a, float b, uint32_t (&o)[N]) {
+  if constexpr (std::is_same_v<T, Bf16>) {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
+      o[i] = __builtin_amdgcn_perm(ub, ua, 0x07060302u);
+      if (i + 1 < N) {
+        a = __builtin_copysignf(fmaxf(fabsf(a - __uint_as_float(ua & 0xffff0000u)), 0x1p-120f), a);
+        b = __builtin_copysignf(fmaxf(fabsf(b - __uint_as_float(ub & 0xffff0000u)), 0x1p-120f), b);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
+      o[i] = __builtin_bit_cast(uint32_t, h);
+      if (i + 1 < N) {
+        a = __builtin_copysignf(fmaxf(fabsf(a - (float)h[0]), 0x1p-24f), a);
+        b = __builtin_copysignf(fmaxf(fabsf(b - (float)h[1]), 0x1p-24f), b);
+      }
+    }
+  }
+}
+// The same for probabilities (never negative).
+template <class T, int N>
+__device__ __forceinline__ void cut2_pos(float a, float b, uint32_t (&o)[N]) {
+  if constexpr (std::is_same_v<T, Bf16>) {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
+      o[i] = __builtin_amdgcn_perm(ub, ua, 0x07060302u);
+      if (i + 1 < N) {
+        a = fmaxf(a - __uint_as_float(ua & 0xffff0000u), 0x1p-120f);
+        b = fmaxf(b - __uint_as_float(ub & 0xffff0000u), 0x1p-120f);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
+      o[i] = __builtin_bit_cast(uint32_t, h);
+      if (i + 1 < N) {
+        a = fmaxf(a - (float)h[0], 0x1p-24f);
+        b = fmaxf(b - (float)h[1], 0x1p-24f);
+      }
+    }
+  }
+}
+
+template <class T>
+__device__ __forceinline__ floatx4 mfma16(const uint32_t *a, const uint32_t *b, floatx4 c) {
+  const u32x4 x = {a[0], a[1], a[2], a[3]}, y = {b[0], b[1], b[2], b[3]};
+  if constexpr (std::is_same_v<T, Bf16>)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, y), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, y), c, 0, 0, 0);
+}
+
 // The tree of one sequence: every node's ancestors (itself among them) as bits, none for a slot
-// that is unused or hangs below one, and the number of slots up to the last used one.
-struct Tree {
-  uint64_t anc[kTreeMaxNodes][4];
-  int up[kTreeMaxNodes];
+// that is unused or hangs below one, and the number of slots up to the last used one.  W words of
+// 64 nodes.  The parents are followed by doubling: after step k a node knows 2^k of its ancestors.
+template <int W>
+struct Tree;
+
+// Up to 64 nodes: node i in lane i of every wave, no memory.
+template <>
+struct Tree<1> {
+  uint64_t anc;
   int live;
+  struct Shared {};
+  __device__ void read(int par, int n, Shared &) {
+    const int i = threadIdx.x & 63;
+    int up = i < n && par >= -1 && par < i ? par : -2;  // -1: the root is reached; -2: not in the tree
+    anc = up != -2 ? 1ull << i : 0;
+    for (int s = 1; s < n; s *= 2) {
+      const int at = max(up, 0);
+      const uint64_t a = __shfl((unsigned long long)anc, at, 64);
+      const int u = __shfl(up, at, 64);
+      if (up >= 0) anc |= a, up = u;
+    }
+    if (up == -2) anc = 0;
+    live = 64 - __clzll(__ballot(anc != 0));
+  }
+  // node's words, in registers of the lanes that ask
+  struct Row {
+    uint64_t anc;
+    __device__ bool sees(int j) const { return j < 64 && (anc >> (j & 63) & 1); }
+    __device__ bool any() const { return anc != 0; }
+  };
+  __device__ Row row(int node, const Shared &) const { return Row{__shfl((unsigned long long)anc, node, 64)}; }
 };
 
-// Follows the parents by doubling: after step k a node knows 2^k of its ancestors.  All threads.
-__device__ inline void read_tree(const int32_t *par, int n, Tree &t) {
-  const int i = threadIdx.x;
-  static_assert(64 * kWaves >= kTreeMaxNodes, "a thread for each node");
-  if (i == 0) t.live = 0;
-  if (i < n) {
-    const int p = par[i];
-    t.up[i] = p >= -1 && p < i ? p : -2;  // -1: the root is reached; -2: not in the tree
-#pragma unroll
-    for (int w = 0; w < 4; w++) t.anc[i][w] = w == i >> 6 ? 1ull << (i & 63) : 0;
-  }
-  __syncthreads();
-  for (int s = 1; s < n; s *= 2) {
-    int up = -2;
-    uint64_t a[4] = {};
+template <>
+struct Tree<4> {
+  int live;
+  struct Shared {
+    uint64_t anc[kTreeMaxNodes][4];
+    int up[kTreeMaxNodes];
+    int live;
+  };
+  __device__ void read(int par, int n, Shared &t) {
+    const int i = threadIdx.x;
+    static_assert(64 * kWaves >= kTreeMaxNodes, "a thread for each node");
+    if (i == 0) t.live = 0;
     if (i < n) {
-      up = t.up[i];
+      t.up[i] = par >= -1 && par < i ? par : -2;
 #pragma unroll
-      for (int w = 0; w < 4; w++) a[w] = t.anc[i][w] | (up >= 0 ? t.anc[up][w] : 0);
-      if (up >= 0) up = t.up[up];
+      for (int w = 0; w < 4; w++) t.anc[i][w] = w == i >> 6 ? 1ull << (i & 63) : 0;
     }
     __syncthreads();
-    if (i < n) {
-      t.up[i] = up;
+    for (int s = 1; s < n; s *= 2) {
+      int up = -2;
+      uint64_t a[4] = {};
+      if (i < n) {
+        up = t.up[i];
 #pragma unroll
-      for (int w = 0; w < 4; w++) t.anc[i][w] = a[w];
+        for (int w = 0; w < 4; w++) a[w] = t.anc[i][w] | (up >= 0 ? t.anc[up][w] : 0);
+        if (up >= 0) up = t.up[up];
+      }
+      __syncthreads();
+      if (i < n) {
+        t.up[i] = up;
+#pragma unroll
+        for (int w = 0; w < 4; w++) t.anc[i][w] = a[w];
+      }
+      __syncthreads();
+    }
+    if (i < n) {
+      if (t.up[i] == -2) {
+#pragma unroll
+        for (int w = 0; w < 4; w++) t.anc[i][w] = 0;
+      } else {
+        atomicMax(&t.live, i + 1);
+      }
     }
     __syncthreads();
+    live = __builtin_amdgcn_readfirstlane(t.live);
   }
-  if (i < n) {
-    if (t.up[i] == -2) {
-#pragma unroll
-      for (int w = 0; w < 4; w++) t.anc[i][w] = 0;
-    } else {
-      atomicMax(&t.live, i + 1);
-    }
-  }
-  __syncthreads();
-}
+  struct Row {
+    const uint64_t *anc;
+    __device__ bool sees(int j) const { return j < kTreeMaxNodes && (anc[j >> 6] >> (j & 63) & 1); }
+    __device__ bool any() const { return (anc[0] | anc[1] | anc[2] | anc[3]) != 0; }
+  };
+  __device__ Row row(int node, const Shared &t) const { return Row{t.anc[node]}; }
+};
 
 // Partial results of key split s: o [batch][Hk][M][S][D], then (max, sum) [batch][Hk][M][S].
 __host__ __device__ inline size_t part_row(const TreeAttn &a, int S, int b, int hk, int row) {
   return (((size_t)b * a.Hk + hk) * (a.n * (a.H / a.Hk)) + row) * S;
 }
 
-template <int D, class TQ, class TKV, int RT>
-__global__ __launch_bounds__(64 * kWaves) void tree_attn_kernel(TreeAttn a, int S, float2 *ml) {
-  __shared__ Tree tree;
+// A wave's keys and values of one tile: key rows 16 h + c, in runs of 8 elements 32 j + 8 g, and value
+// rows 16 h + 4 g + r, elements D / 16 c ...
+template <int D, class T>
+struct TileRegs {
+  static constexpr int kK = 8 * T::kBytes / 4, kV = D / 16 * T::kBytes / 4;  // dwords of a run
+  uint32_t k[2][D / 32][kK];
+  uint32_t v[8][kV];
+  __device__ __forceinline__ void load_k(const char *base, uint32_t step, int key0, int last, int c, int g) {
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const char *row = base + (uint64_t)(uint32_t)min(key0 + 16 * h + c, last) * step + 8 * g * T::kBytes;
+#pragma unroll
+      for (int j = 0; j < D / 32; j++) load_dwords<kK>(row + 32 * j * T::kBytes, k[h][j]);
+    }
+  }
+  __device__ __forceinline__ void load_v(const char *base, uint32_t step, int key0, int last, int c, int g) {
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      load_dwords<kV>(base + (uint64_t)(uint32_t)min(key0 + 16 * (i >> 2) + 4 * g + (i & 3), last) * step +
+                          D / 16 * c * T::kBytes, v[i]);
+  }
+};
+
+// TQ queries over TKV rows, RT tiles of 16 query rows, W words of nodes.  16-bit caches go through the
+// 16-bit matrix instructions: queries in NQ planes (fp32 ones in three, exactly), probabilities in NP
+// (two hold 16 bits of bf16 and 22 of fp16, far below the result's rounding; three an fp32's).
+// fp32 caches take the fp32 ones.
+template <int D, class TQ, class TKV, int RT, int W>
+__global__ __launch_bounds__(64 * kWaves, 2) void tree_attn_kernel(TreeAttn a, int S, float2 *ml) {
+  constexpr bool kWide = TKV::kBytes == 4;
+  constexpr int NQ = kWide || TQ::kBytes == 2 ? 1 : 3, NP = TQ::kBytes == 2 ? 2 : 3;
+  // probabilities are held up to 2^(kLag + kUp): the running maximum moves only when a score passes
+  // it by 2^kLag; fp16 planes use their range below 1 too
+  constexpr float kLag = 5.0f, kUp = std::is_same_v<TKV, F16> ? 10.0f : 0.0f;
+  __shared__ typename Tree<W>::Shared tree_mem;
   __shared__ float so[kWaves][16 * RT][D + 4];
   __shared__ float sm[kWaves][16 * RT], sl[kWaves][16 * RT];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
+  __shared__ int sodd[kWaves];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
   const int split = blockIdx.x, b = blockIdx.z;
   const int group = a.H / a.Hk, M = a.n * group;
   const int hk = blockIdx.y % a.Hk, row0 = blockIdx.y / a.Hk * (16 * RT);
-  read_tree(a.parents + b * a.par_b, a.n, tree);
-  const int len = a.lengths[b], live = tree.live;
-  const bool bad = len < 0 || live > a.max_seq || len > a.max_seq - live;
-  const int total = bad ? 0 : len + live;
-  const int tiles = (total + kTileKeys - 1) / kTileKeys, per = (tiles + S - 1) / S;
-  const int t_end = min(tiles, (split + 1) * per);
 
-  // queries of this lane's columns, scaled for powers of two; k = 32 j + 8 g + e is element 8 j + e
-  float q[RT][D / 4];
-  int node[RT];
-#pragma unroll
-  for (int t = 0; t < RT; t++) {
-    const int row = min(row0 + 16 * t + c, M - 1);
-    node[t] = row / group;
-    const int64_t at = b * a.q_b + node[t] * a.q_n + (hk * group + row % group) * a.q_h;
-#pragma unroll
-    for (int j = 0; j < D / 32; j++)
-      load_row<TQ, 8>(static_cast<const char *>(a.q) + (at + 32 * j + 8 * g) * TQ::kBytes, &q[t][8 * j]);
-  }
-  const float scale = a.scale * kLog2e;
+  // Everything that does not wait for something else is loaded first: this wave's first tile too,
+  // whose place does not depend on the length.
   const char *kb = static_cast<const char *>(a.k) + (b * a.k_b + hk * a.k_h) * TKV::kBytes;
   const char *vb = static_cast<const char *>(a.v) + (b * a.v_b + hk * a.v_h) * TKV::kBytes;
-
-  f32x4 o[RT][D / 16] = {};
-  float m[RT], l[RT];
+  const uint32_t k_step = (uint32_t)a.k_r * TKV::kBytes, v_step = (uint32_t)a.v_r * TKV::kBytes;
+  const int last = a.max_seq - 1, stride = S * kWaves * kTileKeys;
+  int key0 = (split * kWaves + wave) * kTileKeys;
+  const int len = a.lengths[b];
+  const int par_at = W == 1 ? lane : threadIdx.x;
+  const int par = par_at < a.n ? a.parents[b * a.par_b + par_at] : -2;
+  int node[RT];
+  uint32_t q[NQ][RT][D / 32][kWide ? 8 : 4];
+  {
+    uint32_t raw[RT][D / 32][8 * TQ::kBytes / 4];
 #pragma unroll
-  for (int t = 0; t < RT; t++) m[t] = -INFINITY, l[t] = 0.0f;
-
-  for (int tile = split * per + wave; tile < t_end; tile += kWaves) {
-    const int key0 = tile * kTileKeys;
-    f32x4 s[2][RT] = {};
+    for (int t = 0; t < RT; t++) {
+      const int row = min(row0 + 16 * t + c, M - 1);
+      node[t] = row / group;
+      const char *at = static_cast<const char *>(a.q) +
+                       (b * a.q_b + node[t] * a.q_n + (hk * group + row % group) * a.q_h + 8 * g) * TQ::kBytes;
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-      float kk[D / 4];
-      const int64_t row = min(key0 + 16 * h + c, total - 1);
-#pragma unroll
-      for (int j = 0; j < D / 32; j++)
-        load_row<TKV, 8>(kb + (row * a.k_r + 32 * j + 8 * g) * TKV::kBytes, &kk[8 * j]);
+      for (int j = 0; j < D / 32; j++) load_dwords<8 * TQ::kBytes / 4>(at + 32 * j * TQ::kBytes, raw[t][j]);
+    }
+    if constexpr (kWide || NQ == 3) {  // fp32 queries carry the scale
+      const float scale = a.scale * kLog2e;
 #pragma unroll
       for (int t = 0; t < RT; t++)
 #pragma unroll
-        for (int e = 0; e < D / 4; e++)
-          s[h][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(kk[e], q[t][e], s[h][t], 0, 0, 0);
-    }
-    const bool edge = key0 + kTileKeys > len;  // holds nodes, or ends past the last row
+        for (int j = 0; j < D / 32; j++)
 #pragma unroll
-    for (int t = 0; t < RT; t++) {
-      float top = -INFINITY;
+          for (int e = 0; e < 8; e += 2) {
+            const float x = __uint_as_float(raw[t][j][e]) * scale, y = __uint_as_float(raw[t][j][e + 1]) * scale;
+            if constexpr (kWide) {
+              q[0][t][j][e] = __float_as_uint(x), q[0][t][j][e + 1] = __float_as_uint(y);
+            } else {
+              uint32_t o[3];
+              cut2<TKV, 3>(x, y, o);
 #pragma unroll
-      for (int h = 0; h < 2; h++)
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-          s[h][t][r] *= scale;
-          if (edge) {
-            const int j = key0 + 16 * h + 4 * g + r - len;
-            const bool sees = j < 0 || (j < live && (tree.anc[node[t]][(j >> 6) & 3] >> (j & 63) & 1));
-            s[h][t][r] = sees ? s[h][t][r] : -INFINITY;
+              for (int p = 0; p < 3; p++) q[p][t][j][e / 2] = o[p];
+            }
           }
-          top = fmaxf(top, s[h][t][r]);
-        }
-      const float mn = fmaxf(m[t], col_max(top)), ms = mn == -INFINITY ? 0.0f : mn;
-      const float f = __builtin_amdgcn_exp2f(m[t] - ms);
-      m[t] = mn;
-      l[t] *= f;
+    } else {  // 16-bit ones its sign
+      const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0;
 #pragma unroll
-      for (int d = 0; d < D / 16; d++) o[t][d] *= f;
+      for (int t = 0; t < RT; t++)
 #pragma unroll
-      for (int h = 0; h < 2; h++)
+        for (int j = 0; j < D / 32; j++)
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-          s[h][t][r] = __builtin_amdgcn_exp2f(s[h][t][r] - ms);
-          l[t] += s[h][t][r];
-        }
+          for (int e = 0; e < 4; e++) q[0][t][j][e] = raw[t][j][e] ^ flip;
     }
+  }
+  const float scale = kWide || NQ == 3 ? 1.0f : fabsf(a.scale) * kLog2e;
+  TileRegs<D, TKV> x;
+  x.load_k(kb, k_step, key0, last, c, g);
+  x.load_v(vb, v_step, key0, last, c, g);
+  Tree<W> tree;
+  tree.read(par, a.n, tree_mem);
+  const int live = tree.live;
+  const bool bad = len < 0 || live > a.max_seq || len > a.max_seq - live;
+  const int total = bad ? 0 : len + live;
+  typename Tree<W>::Row sees[RT];
+#pragma unroll
+  for (int t = 0; t < RT; t++) sees[t] = tree.row(node[t], tree_mem);
+
+  floatx4 o[RT][D / 16] = {};
+  float m[RT], l[RT];
+  uint32_t odd = 0;  // a node's value that is no finite number was taken out
+#pragma unroll
+  for (int t = 0; t < RT; t++) m[t] = -INFINITY, l[t] = 0.0f;
+
+  for (; key0 < total; key0 += stride) {
+    floatx4 s[2][RT] = {};
 #pragma unroll
     for (int h = 0; h < 2; h++)
 #pragma unroll
-      for (int r = 0; r < 4; r++) {
-        const int key = key0 + 16 * h + 4 * g + r;
-        float vv[D / 16];
-        load_row<TKV, D / 16>(vb + ((int64_t)min(key, total - 1) * a.v_r + D / 16 * c) * TKV::kBytes, vv);
-        if (edge) {
-          // rows of nodes count only where they are seen: 0 times what a masked row may hold
-          // (infinities, NaN) must stay out, so such values leave the product and are added
-          // below, query by query
-          bool odd = false;
+      for (int j = 0; j < D / 32; j++)
 #pragma unroll
-          for (int d = 0; d < D / 16; d++) {
-            const bool fin = key < len || fabsf(vv[d]) < INFINITY;
-            odd = odd || (key < total && !fin);
-            vv[d] = key < total && fin ? vv[d] : 0.0f;
+        for (int t = 0; t < RT; t++)
+          if constexpr (kWide) {
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+              s[h][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(x.k[h][j][e]), __uint_as_float(q[0][t][j][e]),
+                                                             s[h][t], 0, 0, 0);
+          } else {
+#pragma unroll
+            for (int p = NQ - 1; p >= 0; p--) s[h][t] = mfma16<TKV>(x.k[h][j], q[p][t][j], s[h][t]);
           }
-          if (__ballot(odd)) {
-            for (int gg = 0; gg < 4; gg++) {
-              const int kx = key0 + 16 * h + 4 * gg + r, j = kx - len;
-              if (j < 0 || j >= live) continue;
+    // the wave's next tile; past the last one every lane asks for the last row (one line), so that no
+    // register is left as it was on some path
+    const int next = min(key0 + stride, total - 1);
+    x.load_k(kb, k_step, next, total - 1, c, g);
+
+    const bool edge = key0 + kTileKeys > len;  // holds nodes, or ends past the last row
+    if (edge) {
 #pragma unroll
-              for (int t = 0; t < RT; t++) {
-                const float p = __shfl(s[h][t][r], c + 16 * gg, 64);
-                const bool sees = tree.anc[node[t]][j >> 6] >> (j & 63) & 1;
+      for (int t = 0; t < RT; t++)
 #pragma unroll
-                for (int d = 0; d < D / 16; d++)
+        for (int h = 0; h < 2; h++)
 #pragma unroll
-                  for (int rr = 0; rr < 4; rr++) {
-                    float x;
-                    const char *at = vb + ((int64_t)kx * a.v_r + D / 16 * (4 * g + rr) + d) * TKV::kBytes;
-                    if constexpr (TKV::kBytes == 4) x = *reinterpret_cast<const float *>(at);
-                    else if constexpr (std::is_same_v<TKV, Bf16>) x = bf16_bits_to_float(*reinterpret_cast<const uint16_t *>(at));
-                    else x = half_bits_to_float(*reinterpret_cast<const uint16_t *>(at));
-                    if (sees && !(fabsf(x) < INFINITY)) o[t][d][rr] += p * x;
-                  }
-              }
-            }
+          for (int r = 0; r < 4; r++) {
+            const int j = key0 + 16 * h + 4 * g + r - len;
+            if (j >= 0 && !(j < live && sees[t].sees(j))) s[h][t][r] = -INFINITY;
           }
+    }
+    float top[RT];
+    bool grows = false;
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+      top[t] = fmaxf(fmaxf(fmaxf(s[0][t][0], s[0][t][1]), fmaxf(s[0][t][2], s[0][t][3])),
+                     fmaxf(fmaxf(s[1][t][0], s[1][t][1]), fmaxf(s[1][t][2], s[1][t][3]))) * scale;
+      grows = grows || top[t] > m[t] + kLag;
+    }
+    if (__ballot(grows)) {
+#pragma unroll
+      for (int t = 0; t < RT; t++) {
+        const float mn = fmaxf(m[t], col_max(top[t]));
+        const float f = __builtin_amdgcn_exp2f(m[t] - (mn == -INFINITY ? 0.0f : mn));
+        m[t] = mn;
+        l[t] *= f;
+#pragma unroll
+        for (int d = 0; d < D / 16; d++) o[t][d] *= f;
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+      const float ms = (m[t] == -INFINITY ? 0.0f : m[t]) - kUp;
+#pragma unroll
+      for (int h = 0; h < 2; h++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[h][t][r], scale, -ms));
+          if (edge) {  // (a scale of 0 makes NaN of the mask's -inf)
+            const int j = key0 + 16 * h + 4 * g + r - len;
+            if (j >= 0 && !(j < live && sees[t].sees(j))) p = 0.0f;
+          }
+          s[h][t][r] = p;
+          l[t] += p;
         }
+    }
+
+    if (edge) {
+      // Rows of nodes count only where they are seen, and rows past the last one nowhere: 0 times
+      // what a masked row may hold (infinities, NaN) must stay out of the product, so such values
+      // leave it and are added at the end, row by row.
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const int key = key0 + 16 * (i >> 2) + 4 * g + (i & 3);
+#pragma unroll
+        for (int d = 0; d < TileRegs<D, TKV>::kV; d++) {
+          const uint32_t v = x.v[i][d];
+          uint32_t keep = ~0u;
+          if constexpr (kWide) {
+            if ((v & 0x7f800000u) == 0x7f800000u) keep = 0;
+          } else {
+            if ((v & TKV::kOddBits) == TKV::kOddBits) keep &= 0xffff0000u;
+            if ((v >> 16 & TKV::kOddBits) == TKV::kOddBits) keep &= 0x0000ffffu;
+          }
+          if (key < len) keep = ~0u;
+          odd |= key < total ? ~keep : 0;
+          x.v[i][d] = key < total ? v & keep : 0;
+        }
+      }
+    }
+    if constexpr (kWide) {
+#pragma unroll
+      for (int i = 0; i < 8; i++)
 #pragma unroll
         for (int t = 0; t < RT; t++)
 #pragma unroll
           for (int d = 0; d < D / 16; d++)
-            o[t][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(vv[d], s[h][t][r], o[t][d], 0, 0, 0);
+            o[t][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(x.v[i][d]), s[i >> 2][t][i & 3], o[t][d], 0, 0, 0);
+    } else {
+      // operands of 8 keys a lane: V^T by element pairs from its 8 rows, P as it stands
+      uint32_t vt[D / 16][4];
+#pragma unroll
+      for (int d = 0; d < D / 16; d++)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          vt[d][i] = __builtin_amdgcn_perm(x.v[2 * i + 1][d / 2], x.v[2 * i][d / 2], d % 2 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+      for (int t = 0; t < RT; t++) {
+        uint32_t p[NP][4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          uint32_t w[NP];
+          cut2_pos<TKV, NP>(s[i >> 1][t][2 * (i & 1)], s[i >> 1][t][2 * (i & 1) + 1], w);
+#pragma unroll
+          for (int k = 0; k < NP; k++) p[k][i] = w[k];
+        }
+#pragma unroll
+        for (int k = NP - 1; k >= 0; k--)
+#pragma unroll
+          for (int d = 0; d < D / 16; d++) o[t][d] = mfma16<TKV>(vt[d], p[k], o[t][d]);
       }
+    }
+    x.load_v(vb, v_step, next, total - 1, c, g);
   }
 
+  if (const bool any = __ballot(odd != 0) != 0; lane == 0) sodd[wave] = any;
   // the block's waves joined: lane (c, g) holds dims D/4 g .. of column c, in runs of D/16 a register
 #pragma unroll
   for (int t = 0; t < RT; t++) {
@@ -289,10 +492,15 @@ __global__ __launch_bounds__(64 * kWaves) void tree_attn_kernel(TreeAttn a, int 
             make_float4(o[t][d][r], o[t][d + 1][r], o[t][d + 2][r], o[t][d + 3][r]);
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < 16 * RT * (D / 4); i += 64 * kWaves) {
-    const int rr = i / (D / 4), d = i % (D / 4) * 4, row = row0 + rr;
+  const bool odd_any = (sodd[0] | sodd[1] | sodd[2] | sodd[3]) != 0;
+  static_assert(kWaves == 4, "flags of four waves");
+  for (int i0 = 0; i0 < 16 * RT * (D / 4); i0 += 64 * kWaves) {
+    const int i = i0 + threadIdx.x;
+    const int rr = i / (D / 4), d = i % (D / 4) * 4, row = row0 + rr, i_node = min(row, M - 1) / group;
+    const auto seen = tree.row(i_node, tree_mem);
+    const bool any = seen.any();
     if (row >= M) continue;
-    float top = -INFINITY, sum = 0.0f, x[4] = {};
+    float top = -INFINITY, sum = 0.0f, y[4] = {};
 #pragma unroll
     for (int w = 0; w < kWaves; w++) top = fmaxf(top, sm[w][rr]);
     const float ms = top == -INFINITY ? 0.0f : top;
@@ -301,95 +509,105 @@ __global__ __launch_bounds__(64 * kWaves) void tree_attn_kernel(TreeAttn a, int 
       const float f = __builtin_amdgcn_exp2f(sm[w][rr] - ms);
       const float4 v = *reinterpret_cast<const float4 *>(&so[w][rr][d]);
       sum += f * sl[w][rr];
-      x[0] += f * v.x, x[1] += f * v.y, x[2] += f * v.z, x[3] += f * v.w;
+      y[0] += f * v.x, y[1] += f * v.y, y[2] += f * v.z, y[3] += f * v.w;
     }
-    const int i_node = row / group;
-    uint64_t any = 0;
+    if (odd_any) {  // (a positive probability times an infinity or NaN is that)
+#pragma unroll 1
+      for (int j = 0; j < live; j++) {
+        if (!seen.sees(j)) continue;
+        const char *at = vb + (uint64_t)(uint32_t)(len + j) * v_step + d * TKV::kBytes;
 #pragma unroll
-    for (int w = 0; w < 4; w++) any |= tree.anc[i_node][w];
+        for (int e = 0; e < 4; e++) {
+          const float v = load1<TKV>(at + e * TKV::kBytes);
+          if (!(fabsf(v) < INFINITY)) y[e] += v;
+        }
+      }
+    }
     if (S == 1) {
       const float inv = 1.0f / sum;
 #pragma unroll
-      for (int e = 0; e < 4; e++) x[e] = bad ? NAN : any ? x[e] * inv : 0.0f;
+      for (int e = 0; e < 4; e++) y[e] = bad ? NAN : any ? y[e] * inv : 0.0f;
       const int64_t at = b * a.o_b + i_node * a.o_n + (hk * group + row % group) * a.o_h + d;
-      store4<TQ>(static_cast<char *>(a.out) + at * TQ::kBytes, x[0], x[1], x[2], x[3]);
+      store4<TQ>(static_cast<char *>(a.out) + at * TQ::kBytes, y[0], y[1], y[2], y[3]);
     } else {
       // what the joining kernel cannot tell by itself goes with the statistics: a row that sees
       // nothing has maximum +inf and sum 0, one of a bad sequence sum NaN
       const size_t at = part_row(a, S, b, hk, row) + split;
-      if (split * per < t_end) *reinterpret_cast<float4 *>(a.part + at * D + d) = make_float4(x[0], x[1], x[2], x[3]);
+      if (split * kWaves * kTileKeys < total)
+        *reinterpret_cast<float4 *>(a.part + at * D + d) = make_float4(y[0], y[1], y[2], y[3]);
       if (d == 0) ml[at] = bad ? make_float2(0.0f, NAN) : any ? make_float2(top, sum) : make_float2(INFINITY, 0.0f);
     }
   }
 }
 
-// Joins the splits of a row: a wave a row, in split order.
+// Joins the splits of a row, D / 4 lanes a row with four elements each, in split order.
 template <int D, class TQ>
 __global__ __launch_bounds__(256) void tree_join_kernel(TreeAttn a, int S, const float2 *ml) {
-  const int lane = threadIdx.x & 63, group = a.H / a.Hk, M = a.n * group;
-  const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  constexpr int kLanes = D / 4;
+  const int lane = threadIdx.x % kLanes, group = a.H / a.Hk, M = a.n * group;
+  const int64_t item = (int64_t)blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
   if (item >= (int64_t)a.batch * a.Hk * M) return;
   const int row = item % M, hk = item / M % a.Hk, b = item / M / a.Hk;
-  const size_t at = (size_t)item * S;
+  const float2 *w = ml + (size_t)item * S;
+  const float *part = a.part + (size_t)item * S * D + 4 * lane;
   float top = -INFINITY;
-  for (int s = lane; s < S; s += 64) top = fmaxf(top, ml[at + s].x);
-  top = wave_max(top);
-  const float2 first = ml[at];
-  const bool none = first.x == INFINITY && first.y == 0.0f;
+  for (int s = 0; s < S; s++) top = fmaxf(top, w[s].x);
+  const bool none = w[0].x == INFINITY && w[0].y == 0.0f;
   const float ms = top == -INFINITY ? 0.0f : top;
-  constexpr int E = D / 64;
-  float sum = 0.0f, x[E] = {};
+  float sum = 0.0f, x[4] = {};
   for (int s = 0; s < S; s++) {
-    const float2 w = ml[at + s];
-    if (w.x == -INFINITY && w.y == 0.0f) continue;  // no keys: nothing was stored
-    const float f = __builtin_amdgcn_exp2f(w.x - ms);
-    sum += f * w.y;
-    if (none || w.y != w.y) continue;
-#pragma unroll
-    for (int e = 0; e < E; e++) x[e] += f * a.part[(at + s) * D + E * lane + e];
+    const float2 v = w[s];
+    if ((v.x == -INFINITY && v.y == 0.0f) || none) continue;  // no keys: nothing was stored
+    const float f = fmaxf(__builtin_amdgcn_exp2f(v.x - ms), 0x1p-126f);  // (0 times an infinity: NaN)
+    sum += f * v.y;
+    if (v.y != v.y) continue;
+    const float4 p = *reinterpret_cast<const float4 *>(part + (size_t)s * D);
+    x[0] += f * p.x, x[1] += f * p.y, x[2] += f * p.z, x[3] += f * p.w;
   }
-  const float inv = 1.0f / sum;
-  const int64_t to = b * a.o_b + row / group * a.o_n + (hk * group + row % group) * a.o_h + E * lane;
-#pragma unroll
-  for (int e = 0; e < E; e++) {
-    const float y = none ? 0.0f : x[e] * inv;
-    if constexpr (TQ::kBytes == 4) static_cast<float *>(a.out)[to + e] = y;
-    else if constexpr (std::is_same_v<TQ, Bf16>) static_cast<uint16_t *>(a.out)[to + e] = (uint16_t)float_to_bf16_bits(y);
-    else static_cast<_Float16 *>(a.out)[to + e] = (_Float16)y;
-  }
+  const float inv = none ? 0.0f : 1.0f / sum;
+  const int64_t to = b * a.o_b + row / group * a.o_n + (hk * group + row % group) * a.o_h + 4 * lane;
+  store4<TQ>(static_cast<char *>(a.out) + to * TQ::kBytes, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
 }
 
 struct Plan {
   int S, RT, row_tiles;
 };
+// Most tiles of 16 query rows a wave takes: as many as its registers hold (256 a lane, two waves a
+// SIMD).  fp32 queries take up to three times the registers of 16-bit ones.
+constexpr int most_tiles(int D, int q_bytes) { return (q_bytes == 4 ? 128 : 256) / D; }
+
 Plan make_plan(const TreeAttn &a, int n_cu) {
   Plan p;
-  const int M = a.n * (a.H / a.Hk);
-  const int most = a.D == 64 ? 4 : 2;
-  p.RT = M <= 16 ? 1 : M <= 32 ? 2 : most;
+  const int M = a.n * (a.H / a.Hk), most = most_tiles(a.D, a.qt == kOpF32 ? 4 : 2);
+  p.RT = a.n > 64 ? most : std::min(most, M <= 16 ? 1 : M <= 32 ? 2 : 4);
   p.row_tiles = (M + 16 * p.RT - 1) / (16 * p.RT);
   const int tiles = (a.max_seq + kTileKeys - 1) / kTileKeys;
   const int64_t blocks = (int64_t)a.batch * a.Hk * p.row_tiles;
-  const int64_t want = (2 * n_cu + blocks - 1) / blocks, can = (tiles + 4 * kWaves - 1) / (4 * kWaves);
+  const int64_t want = (4 * n_cu + blocks - 1) / blocks, can = (tiles + 2 * kWaves - 1) / (2 * kWaves);
   p.S = (int)std::max<int64_t>(1, std::min<int64_t>({want, can, 64}));
   return p;
 }
 
-template <int D, class TQ, class TKV, int RT>
+template <int D, class TQ, class TKV, int RT, int W>
 hipError_t launch_rt(const TreeAttn &a, const Plan &p, hipStream_t s) {
   float2 *ml = reinterpret_cast<float2 *>(a.part + (size_t)a.batch * a.H * a.n * p.S * D);
-  hipLaunchKernelGGL((tree_attn_kernel<D, TQ, TKV, RT>), dim3(p.S, a.Hk * p.row_tiles, a.batch), dim3(64 * kWaves), 0, s,
+  hipLaunchKernelGGL((tree_attn_kernel<D, TQ, TKV, RT, W>), dim3(p.S, a.Hk * p.row_tiles, a.batch), dim3(64 * kWaves), 0, s,
                      a, p.S, ml);
   if (hipError_t e = hipGetLastError(); e != hipSuccess || p.S == 1) return e;
   const int64_t rows = (int64_t)a.batch * a.H * a.n;
-  hipLaunchKernelGGL((tree_join_kernel<D, TQ>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a, p.S, ml);
+  constexpr int kRows = 256 / (D / 4);
+  hipLaunchKernelGGL((tree_join_kernel<D, TQ>), dim3((unsigned)((rows + kRows - 1) / kRows)), dim3(256), 0, s, a, p.S, ml);
   return hipGetLastError();
 }
 template <int D, class TQ, class TKV>
 hipError_t launch_d(const TreeAttn &a, const Plan &p, hipStream_t s) {
-  if (p.RT == 1) return launch_rt<D, TQ, TKV, 1>(a, p, s);
-  if (D == 128 || p.RT == 2) return launch_rt<D, TQ, TKV, 2>(a, p, s);
-  return launch_rt<D, TQ, TKV, D == 64 ? 4 : 2>(a, p, s);
+  constexpr int kMost = most_tiles(D, TQ::kBytes);
+  if (a.n > 64) return launch_rt<D, TQ, TKV, kMost, 4>(a, p, s);
+  if constexpr (kMost >= 4)
+    if (p.RT == 4) return launch_rt<D, TQ, TKV, 4, 1>(a, p, s);
+  if constexpr (kMost >= 2)
+    if (p.RT == 2) return launch_rt<D, TQ, TKV, 2, 1>(a, p, s);
+  return launch_rt<D, TQ, TKV, 1, 1>(a, p, s);
 }
 template <class TQ, class TKV>
 hipError_t launch_t(const TreeAttn &a, const Plan &p, hipStream_t s) {

@@ -94,7 +94,8 @@ itts_status tree_args(const itts_tree_attention_args *a, TreeAttn *o) {
     return fail(ITTS_E_VALIDATION, "n_kv_head: %d key heads do not divide %d query heads (1..=1024)", a->n_kv_head, a->n_head);
   if (a->head_dim != 64 && a->head_dim != 128)
     return fail(ITTS_E_VALIDATION, "head_dim: must be 64 or 128, got %d", a->head_dim);
-  if (a->max_seq < 1 || a->max_seq > INT32_MAX - 1024) return fail(ITTS_E_VALIDATION, "max_seq: must be >= 1 (and below 2^31 - 1024), got %d", a->max_seq);
+  if (a->max_seq < 1 || a->max_seq > 1 << 30)
+    return fail(ITTS_E_VALIDATION, "max_seq: must be in 1..=2^30, got %d", a->max_seq);
   if (!(a->scale - a->scale == 0.0f)) return fail(ITTS_E_VALIDATION, "scale: must be finite");
   const int qt = op_type(a->q_dtype), kvt = op_type(a->kv_dtype);
   if (qt < 0 || kvt < 0 || !(qt == kvt || (qt == kOpF32 && kvt == kOpBf16)))
@@ -110,6 +111,8 @@ itts_status tree_args(const itts_tree_attention_args *a, TreeAttn *o) {
     return fail(ITTS_E_VALIDATION, "k: rows must start at multiples of 16 bytes");
   if (!row_stride(a->v_batch, b, ks) || !row_stride(a->v_head, hk, ks) || !row_stride(a->v_row, a->max_seq, ks) || !aligned16(a->v))
     return fail(ITTS_E_VALIDATION, "v: rows must start at multiples of 16 bytes");
+  if (a->max_seq > 1 && (a->k_row * ks > INT32_MAX || a->v_row * ks > INT32_MAX))
+    return fail(ITTS_E_VALIDATION, "k_row, v_row: rows must be less than 2^31 bytes apart");
   if (b > 1 && a->parents_batch < 0) return fail(ITTS_E_VALIDATION, "parents: negative stride");
   *o = TreeAttn{a->q, a->k, a->v, a->out, a->lengths, a->parents, b, n, h, hk, a->head_dim, a->max_seq, qt, kvt, a->scale,
                 a->q_batch, a->q_node, a->q_head, a->out_batch, a->out_node, a->out_head, a->k_batch, a->k_head, a->k_row,
