@@ -1,15 +1,31 @@
 // Scores of rows of logits x [rows][vocab]: with m the row's maximum, c the number of tokens at m
 // and s the sum of exp(x - m) over the others,
 //   log p(t) = x_t - m - log(c + s),   entropy = log(c + s) - sum (x - m) exp(x - m) / (c + s).
-// Keeping s apart from c makes log(c + s) = log1p(s) where one token has nearly all the
+// Keeping s apart from c makes log(c + s) = log1p(s + (c - 1)) where one token has nearly all the
 // probability, so that small entropies and log-probabilities near 0 keep their relative accuracy.
 // Alternatives are ordered by (logit, lowest token first); NaN counts as -inf there.
+//
+// One pass over the logits: a block holds 8 16-byte pieces a thread of its row in registers (rows that
+// are longer go on piece by piece), takes each thread's maximum, then its sums.  The same registers
+// give the alternatives: any n of the row's elements bound the n-th largest from below, so the
+// threads' maxima give a bound that few elements pass; those go to a list in LDS and are ranked
+// against each other.  Rows that are few and long are split over blocks and joined by a second
+// kernel.
+#include <algorithm>
+
 #include "kernels.h"
 
 namespace itts {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, kWaves = kThreads / 64;
+constexpr int kPieces = 8;       // 16-byte pieces a thread holds
+constexpr int kList = 1024;      // room for elements that pass the bound
+constexpr int kMaxSplits = 32;
+constexpr float kLog2e = 1.4426950408889634f;
+
+template <int TYPE>
+constexpr int kPer = TYPE == kOpF32 ? 4 : 8;  // elements of a 16-byte piece
 
 template <int TYPE>
 __device__ __forceinline__ float logit(const void *row, int i) {
@@ -17,86 +33,383 @@ __device__ __forceinline__ float logit(const void *row, int i) {
   else if constexpr (TYPE == kOpBf16) return bf16_bits_to_float(static_cast<const uint16_t *>(row)[i]);
   else return half_bits_to_float(static_cast<const uint16_t *>(row)[i]);
 }
-
-// (value, token) as one number that is larger for what comes first.
-__device__ __forceinline__ uint64_t rank_key(float x, int token) {
-  const uint32_t u = __float_as_uint(fmaxf(x, -INFINITY) + 0.0f);
-  return (uint64_t)(u & 0x80000000u ? ~u : u | 0x80000000u) << 32 | (uint32_t)~token;
+template <int TYPE>
+__device__ __forceinline__ float element(const uint4 &v, int e) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  if constexpr (TYPE == kOpF32) return __uint_as_float(w[e]);
+  else if constexpr (TYPE == kOpBf16) return e % 2 ? __uint_as_float(w[e / 2] & 0xffff0000u) : __uint_as_float(w[e / 2] << 16);
+  else return half_bits_to_float(e % 2 ? w[e / 2] >> 16 : w[e / 2] & 0xffffu);
 }
 
-__device__ inline uint64_t block_max(uint64_t v, uint64_t *red) {
+// The piece as a new value: what was unpacked from it before is not kept in registers for later.
+// Nor does the compiler start on the next piece before this one is done: it would hold both.
+__device__ __forceinline__ void again(uint4 &v) {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("" : "+v"(v.x), "+v"(v.y), "+v"(v.z), "+v"(v.w));
+}
+
+// Floats in order as integers (-inf and NaN alike; -0 as 0), and back.
+__device__ __forceinline__ uint32_t order(float x) {
+  const uint32_t u = __float_as_uint(fmaxf(x, -INFINITY) + 0.0f);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float unorder(uint32_t u) {
+  return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
+}
+constexpr uint32_t kOrderNone = 0x007fffffu;  // order(-inf)
+// (value, token) as one number, larger for what comes first; 0 is below every token's.
+__device__ __forceinline__ uint64_t rank_key(float x, int token) { return (uint64_t)order(x) << 32 | (uint32_t)~token; }
+__device__ __forceinline__ int key_token(uint64_t k) { return (int)~(uint32_t)k; }
+__device__ __forceinline__ float key_value(uint64_t k) { return unorder((uint32_t)(k >> 32)); }
+
+// Maximum, tokens at it, sums over the others of p = exp(x - m) and p (x - m).  m = -inf: none.
+struct Stats {
+  float m, c, s, d;
+  // what these sums are above a maximum `top` >= m (-inf: nothing was summed, but for a NaN in s)
+  __device__ Stats under(float top) const {
+    if (m == top || m == -INFINITY) return Stats{top, m == top && m != -INFINITY ? c : 0.0f, s, m == top ? d : 0.0f};
+    const float by = m - top, f = __builtin_amdgcn_exp2f(by * kLog2e), w = c + s;
+    return Stats{top, 0.0f, f * w, f == 0.0f ? 0.0f : f * (d + by * w)};
+  }
+  __device__ void join(const Stats &o) {
+    const float top = fmaxf(m, o.m);
+    const Stats x = under(top), y = o.under(top);
+    *this = Stats{top, x.c + y.c, x.s + y.s, x.d + y.d};
+  }
+};
+
+__device__ __forceinline__ float wave_sum_f(float v) { return wave64_sum_dpp(v); }
+
+// The block's statistics from the threads'; every thread gets them.
+__device__ inline Stats block_stats(Stats t, float (*red)[4]) {
+  const float m = wave64_max_dpp(t.m);
+  const Stats top = t.under(m);
+  const Stats w{m, wave_sum_f(top.c), wave_sum_f(top.s), wave_sum_f(top.d)};
+  if ((threadIdx.x & 63) == 0) {
+    float *r = red[threadIdx.x >> 6];
+    r[0] = w.m, r[1] = w.c, r[2] = w.s, r[3] = w.d;
+  }
+  __syncthreads();
+  Stats o{red[0][0], red[0][1], red[0][2], red[0][3]};
+#pragma unroll
+  for (int i = 1; i < kWaves; i++) o.join(Stats{red[i][0], red[i][1], red[i][2], red[i][3]});
+  return o;
+}
+
+// log-probabilities and entropy of a row with statistics t.
+struct Row {
+  float m, lz;
+  bool none;
+  float entropy;
+  __device__ explicit Row(const Stats &t) {
+    none = t.m == -INFINITY && t.s == 0.0f;  // every token is masked: probability 0 for all
+    lz = t.m == INFINITY ? NAN : log1pf(t.s + (t.c - 1.0f));
+    if (t.m == -INFINITY) lz = NAN;  // NaN and -inf alone
+    m = t.m;
+    entropy = none ? 0.0f : lz - t.d / (t.c + t.s);
+  }
+  __device__ float log_prob(float x) const { return none ? -INFINITY : (x - m) - lz; }
+};
+
+// The largest 16-bit prefix that at least n of a wave's values reach (0: none).
+__device__ __forceinline__ uint32_t reached(uint32_t v, int n) {
+  uint32_t p = 0;
+#pragma unroll
+  for (uint32_t bit = 1u << 31; bit >= 1u << 16; bit >>= 1)
+    if (__popcll(__ballot(v >= (p | bit))) >= n) p |= bit;
+  return p;
+}
+
+struct Select {
+  uint64_t list[kList + kScoresMaxTop];
+  uint64_t top[kScoresMaxTop];
+  uint32_t bound[2][kWaves];
+  int count;
+};
+
+// The n first of list[0 .. have), in order, to top (0 past have).  All threads.
+__device__ inline void rank_list(Select &sel, int have, int n) {
+  for (int i = threadIdx.x; i < have; i += kThreads) {
+    const uint64_t k = sel.list[i];
+    int r = 0;
+    for (int j = 0; j < have; j++) r += sel.list[j] > k;
+    if (r < n) sel.top[r] = k;
+  }
+  for (int i = threadIdx.x; i < n; i += kThreads)
+    if (i >= have) sel.top[i] = 0;
+  __syncthreads();
+}
+
+__device__ inline uint64_t block_max(uint64_t v, Select &sel) {
   for (int off = 32; off > 0; off >>= 1) {
     const uint64_t o = __shfl_xor((unsigned long long)v, off, 64);
     v = o > v ? o : v;
   }
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
-  for (int w = 0; w < kThreads / 64; w++) v = red[w] > v ? red[w] : v;
+  if ((threadIdx.x & 63) == 0) sel.list[threadIdx.x >> 6] = v;
   __syncthreads();
+  for (int w = 0; w < kWaves; w++) v = max(v, sel.list[w]);
   return v;
 }
 
+// Fills a list that the row's numbers leave short: tokens of -inf and NaN, the lowest first.  Wave 0.
 template <int TYPE>
-__global__ __launch_bounds__(kThreads) void token_scores_kernel(TokenScores a) {
-  __shared__ uint64_t red64[kThreads / 64];
-  __shared__ float red[kThreads / 64];
-  const int r = blockIdx.x;
-  const void *x = static_cast<const char *>(a.x) + r * a.x_row * (TYPE == kOpF32 ? 4 : 2);
-  uint64_t best = 0;
-  for (int i = threadIdx.x; i < a.vocab; i += kThreads) best = max(best, rank_key(logit<TYPE>(x, i), i));
-  best = block_max(best, red64);
-  const float m = logit<TYPE>(x, (int)~(uint32_t)best);
-  float cnt = 0.0f, s = 0.0f, sd = 0.0f;
-  for (int i = threadIdx.x; i < a.vocab; i += kThreads) {
-    const float v = logit<TYPE>(x, i);
-    const float d = v - m, p = expf(d);
-    if (v == m) {
-      cnt += 1.0f;
-    } else {
-      s += p;
-      sd += p == 0.0f ? 0.0f : p * d;
+__device__ inline void fill_masked(const void *x, int vocab, uint64_t *top, int n) {
+  const int lane = threadIdx.x & 63;
+  int have = 0;
+  while (have < n && top[have]) have++;
+  for (int i0 = 0; i0 < vocab && have < n; i0 += 64) {
+    const bool masked = i0 + lane < vocab && !(logit<TYPE>(x, min(i0 + lane, vocab - 1)) > -INFINITY);
+    const uint64_t b = __ballot(masked);
+    const int at = have + __popcll(b & ((1ull << lane) - 1));
+    if (masked && at < n) top[at] = rank_key(-INFINITY, i0 + lane);
+    have += __popcll(b);
+  }
+}
+
+template <int TYPE>
+__device__ inline void write_row(const TokenScores &a, int r, const void *x, const Row &row, Select &sel) {
+  if (threadIdx.x == 0 && a.entropy) a.entropy[r] = row.entropy;
+  if (a.top) {
+    if (threadIdx.x < 64 && !sel.top[a.top - 1]) fill_masked<TYPE>(x, a.vocab, sel.top, a.top);
+    __syncthreads();
+    for (int k = threadIdx.x; k < a.top; k += kThreads) {
+      const uint64_t key = sel.top[k];
+      a.top_tokens[(int64_t)r * a.top + k] = key_token(key);
+      // (from the logit itself: the order does not tell NaN from -inf)
+      a.top_log_probs[(int64_t)r * a.top + k] = row.log_prob(key >> 32 == kOrderNone ? logit<TYPE>(x, key_token(key)) : key_value(key));
     }
   }
-  cnt = block_sum<kThreads>(cnt, red);
-  s = block_sum<kThreads>(s, red);
-  sd = block_sum<kThreads>(sd, red);
-  const bool none = m == -INFINITY && s == 0.0f;  // every token is masked: probability 0 for all
-  const float lz = m == INFINITY ? NAN : log1pf(s + (cnt - 1.0f));
-  auto log_prob = [&](float v) { return none ? -INFINITY : (v - m) - lz; };
-  if (threadIdx.x == 0 && a.entropy) a.entropy[r] = none ? 0.0f : lz - sd / (cnt + s);
-  for (int i = threadIdx.x; i < a.given; i += kThreads) {
-    const int t = a.tokens[r * a.tok_row + i];
-    a.log_probs[(int64_t)r * a.given + i] = t == -1 ? 0.0f : t < 0 || t >= a.vocab ? NAN : log_prob(logit<TYPE>(x, t));
+}
+
+// The splits' results: statistics [rows][S], then ordered lists [rows][S][top].
+__host__ __device__ inline size_t list_offset(int rows, int S) { return sizeof(Stats) * (size_t)rows * S; }
+
+template <int TYPE>
+__global__ __launch_bounds__(kThreads, 4) void token_scores_kernel(TokenScores a, int S) {
+  __shared__ float red[kWaves][4];
+  __shared__ Select sel;
+  constexpr int P = kPer<TYPE>, kBytes = 16 / P, kRound = kThreads * kPieces * P;
+  const int r = blockIdx.x / S, split = blockIdx.x % S, t = threadIdx.x;
+  const char *x = static_cast<const char *>(a.x) + r * a.x_row * kBytes;
+  const int n = a.top;
+  // this block's tokens: i0 .. i1, in whole pieces from i0 (wherever in memory that is: a thread's share
+  // does not depend on it, nor do the results) and the rest
+  const int per = ((a.vocab + S - 1) / S + P - 1) / P * P;
+  const int i0 = min(split * per, a.vocab), i1 = min(i0 + per, a.vocab);
+  const int pieces = (i1 - i0) / P, rest = i1 - i0 - pieces * P;
+  const char *body = x + (int64_t)i0 * kBytes;
+  // a given token's logit, early
+  const int64_t tok_at = r * a.tok_row;
+  const int tok = split == 0 && t < a.given ? a.tokens[tok_at + t] : -1;
+  const float tok_x = tok >= 0 && tok < a.vocab ? logit<TYPE>(x, tok) : 0.0f;
+
+  Stats st{-INFINITY, 0.0f, 0.0f, 0.0f};
+  bool ranked = false;  // all of this block's tokens are
+  if (n > 0) {
+    if (t < n) sel.top[t] = 0;
+    if (t == 0) sel.count = 0;
   }
-  for (int k = 0; k < a.top; k++) {
-    if (threadIdx.x == 0) {
-      const int t = (int)~(uint32_t)best;
-      a.top_tokens[(int64_t)r * a.top + k] = t;
-      a.top_log_probs[(int64_t)r * a.top + k] = log_prob(logit<TYPE>(x, t));
+  for (int base = 0; base == 0 || base < pieces; base += kThreads * kPieces) {
+    uint4 v[kPieces];
+    const uint32_t none = TYPE == kOpF32 ? 0xff800000u : TYPE == kOpBf16 ? 0xff80ff80u : 0xfc00fc00u;  // -inf
+#pragma unroll
+    for (int k = 0; k < kPieces; k++) {
+      const int at = base + k * kThreads + t;
+      v[k] = make_uint4(none, none, none, none);
+      if (at < pieces) __builtin_memcpy(&v[k], body + (int64_t)at * 16, 16);  // (at any element's alignment)
     }
-    uint64_t next = 0;
-    for (int i = threadIdx.x; i < a.vocab; i += kThreads) {
-      const uint64_t key = rank_key(logit<TYPE>(x, i), i);
-      if (key < best) next = max(next, key);
+    const int odd = i1 - rest + t;  // one element a thread of the rest, in the first round
+    const bool has_odd = base == 0 && t < rest;
+    const float odd_x = has_odd ? logit<TYPE>(x, odd) : -INFINITY;
+
+    float gm[kPieces], mx = odd_x;
+#pragma unroll
+    for (int k = 0; k < kPieces; k++) {
+      again(v[k]);
+      gm[k] = element<TYPE>(v[k], 0);
+#pragma unroll
+      for (int e = 1; e < P; e++) gm[k] = fmaxf(gm[k], element<TYPE>(v[k], e));
+      mx = fmaxf(mx, gm[k]);
     }
-    best = block_max(next, red64);
+    Stats u{fmaxf(mx, -INFINITY), 0.0f, 0.0f, 0.0f};
+    const float ms = u.m == -INFINITY ? 0.0f : u.m;
+    auto add = [&](float y) {
+      const float d = y - ms, p = __builtin_amdgcn_exp2f(d * kLog2e);
+      const bool at_top = y == ms;
+      u.c += at_top ? 1.0f : 0.0f;
+      u.s += at_top ? 0.0f : p;
+      u.d += p * fmaxf(d, -3e38f);
+    };
+#pragma unroll
+    for (int k = 0; k < kPieces; k++) {
+      again(v[k]);
+#pragma unroll
+      for (int e = 0; e < P; e++) add(element<TYPE>(v[k], e));
+    }
+    if (has_odd) add(odd_x);
+    st.join(u);
+
+    if (n > 0 && !ranked) {
+      // A bound for the n-th largest: n of one wave's threads reach it, or an equal share of every
+      // wave's.  (-inf has no part in this: a row's last places go to masked tokens at the end.)
+      const uint32_t top = u.m > -INFINITY ? order(u.m) : 0;
+      const uint32_t all = reached(top, n), share = reached(top, (n + kWaves - 1) / kWaves);
+      __syncthreads();
+      if ((t & 63) == 0) sel.bound[0][t >> 6] = all, sel.bound[1][t >> 6] = share;
+      __syncthreads();
+      uint32_t b0 = 0, b1 = ~0u;
+#pragma unroll
+      for (int w = 0; w < kWaves; w++) b0 = max(b0, sel.bound[0][w]), b1 = min(b1, sel.bound[1][w]);
+      const uint64_t worst = sel.top[n - 1];  // (0 before n are found)
+      const uint32_t bound = max(max(max(b0, b1), (uint32_t)(worst >> 32)), kOrderNone + 1);
+      const float least = unorder(bound);
+      auto offer = [&](float y, int token) {
+        if (!(y >= least)) return;
+        const int at = atomicAdd(&sel.count, 1);
+        if (at < kList) sel.list[at] = rank_key(y, token);
+      };
+#pragma unroll
+      for (int k = 0; k < kPieces; k++) {
+        if (!(gm[k] >= least)) continue;
+        again(v[k]);
+#pragma unroll
+        for (int e = 0; e < P; e++) offer(element<TYPE>(v[k], e), i0 + (base + k * kThreads + t) * P + e);
+      }
+      if (has_odd) offer(odd_x, odd);
+      __syncthreads();
+      const int count = sel.count;
+      __syncthreads();  // (it grows below)
+      if (count > kList) {
+        // Ties by the thousand, or the largest all in a few threads: n rounds of the largest that
+        // is left, over all of this block's tokens in memory.
+        uint64_t last = ~0ull, mine = 0;
+        for (int round = 0; round < n; round++) {
+          uint64_t next = 0;
+          for (int i = i0 + t; i < i1; i += kThreads) {
+            const float y = logit<TYPE>(x, i);
+            const uint64_t key = y > -INFINITY ? rank_key(y, i) : 0;
+            if (key < last) next = max(next, key);
+          }
+          last = block_max(next, sel);
+          if (t == round) mine = last;
+        }
+        __syncthreads();
+        if (t < n) sel.top[t] = mine;
+        ranked = true;
+      } else if (count > 0) {
+        if (t < n) {
+          const uint64_t k = sel.top[t];  // what was found before joins the list
+          if (k) sel.list[atomicAdd(&sel.count, 1)] = k;
+        }
+        __syncthreads();
+        rank_list(sel, sel.count, n);
+      }
+      if (t == 0) sel.count = 0;
+    }
   }
+  st = block_stats(st, red);
+
+  if (S == 1) {
+    const Row row(st);
+    for (int i = t; i < a.given; i += kThreads) {
+      const int k = i == t ? tok : a.tokens[tok_at + i];
+      const bool in = k >= 0 && k < a.vocab;
+      const float y = i == t ? tok_x : in ? logit<TYPE>(x, k) : 0.0f;
+      a.log_probs[(int64_t)r * a.given + i] = k == -1 ? 0.0f : in ? row.log_prob(y) : NAN;
+    }
+    write_row<TYPE>(a, r, x, row, sel);
+  } else {
+    if (t == 0) static_cast<Stats *>(a.ws)[(int64_t)r * S + split] = st;
+    uint64_t *lists = reinterpret_cast<uint64_t *>(static_cast<char *>(a.ws) + list_offset(a.rows, S));
+    if (t < n) lists[((int64_t)r * S + split) * n + t] = sel.top[t];
+  }
+}
+
+// Joins a row's splits.  Lists are ordered: the first ceil(n / S) of each together, or n of one, bound
+// the n-th largest from below.
+template <int TYPE>
+__global__ __launch_bounds__(kThreads) void scores_join_kernel(TokenScores a, int S) {
+  __shared__ Select sel;
+  __shared__ uint64_t keys[kMaxSplits * kScoresMaxTop];
+  const int r = blockIdx.x, t = threadIdx.x, n = a.top;
+  const char *x = static_cast<const char *>(a.x) + r * a.x_row * (16 / kPer<TYPE>);
+  const Stats *parts = static_cast<const Stats *>(a.ws) + (int64_t)r * S;
+  const uint64_t *lists = reinterpret_cast<const uint64_t *>(static_cast<const char *>(a.ws) + list_offset(a.rows, S)) + (int64_t)r * S * n;
+  for (int i = t; i < S * n; i += kThreads) keys[i] = lists[i];
+  Stats st = parts[0];
+  for (int s = 1; s < S; s++) st.join(parts[s]);
+  const Row row(st);
+  for (int i = t; i < a.given; i += kThreads) {
+    const int k = a.tokens[r * a.tok_row + i];
+    const bool in = k >= 0 && k < a.vocab;
+    a.log_probs[(int64_t)r * a.given + i] = k == -1 ? 0.0f : in ? row.log_prob(logit<TYPE>(x, k)) : NAN;
+  }
+  if (n > 0) {
+    if (t == 0) sel.count = 0;
+    __syncthreads();
+    uint64_t all = 0, share = ~0ull;
+    const int q = (n + S - 1) / S - 1;
+    for (int s = 0; s < S; s++) all = max(all, keys[s * n + n - 1]), share = min(share, keys[s * n + q]);
+    const uint64_t least = max(max(all, share), (uint64_t)1);
+    for (int i = t; i < S * n; i += kThreads) {
+      if (keys[i] < least) continue;
+      const int at = atomicAdd(&sel.count, 1);
+      if (at < kList) sel.list[at] = keys[i];
+    }
+    __syncthreads();
+    const int count = sel.count;
+    if (count <= kList) {
+      rank_list(sel, count, n);
+    } else {  // (lists of many large ones each)
+      uint64_t last = ~0ull, mine = 0;
+      for (int round = 0; round < n; round++) {
+        uint64_t next = 0;
+        for (int i = t; i < S * n; i += kThreads)
+          if (keys[i] < last) next = max(next, keys[i]);
+        last = block_max(next, sel);
+        if (t == round) mine = last;
+      }
+      __syncthreads();
+      if (t < n) sel.top[t] = mine;
+      __syncthreads();
+    }
+  }
+  write_row<TYPE>(a, r, x, row, sel);
+}
+
+int splits(const TokenScores &a, int n_cu) {
+  const int round = kThreads * kPieces * (a.type == kOpF32 ? 4 : 8);
+  const int64_t want = (2 * (int64_t)n_cu + a.rows - 1) / a.rows, can = a.vocab / round;
+  return (int)std::max<int64_t>(1, std::min<int64_t>({want, can, kMaxSplits}));
+}
+
+template <int TYPE>
+hipError_t launch(const TokenScores &a, int S, hipStream_t s) {
+  hipLaunchKernelGGL(token_scores_kernel<TYPE>, dim3((unsigned)a.rows * S), dim3(kThreads), 0, s, a, S);
+  if (hipError_t e = hipGetLastError(); e != hipSuccess || S == 1) return e;
+  hipLaunchKernelGGL(scores_join_kernel<TYPE>, dim3(a.rows), dim3(kThreads), 0, s, a, S);
+  return hipGetLastError();
 }
 
 }  // namespace
 
-size_t token_scores_ws(const TokenScores &, int) { return 0; }
+size_t token_scores_ws(const TokenScores &a, int n_cu) {
+  const int S = splits(a, n_cu);
+  return S == 1 ? 0 : list_offset(a.rows, S) + sizeof(uint64_t) * (size_t)a.rows * S * a.top;
+}
 
-hipError_t token_scores(const TokenScores &a, int, hipStream_t s) {
+hipError_t token_scores(const TokenScores &a, int n_cu, hipStream_t s) {
   if (a.rows <= 0) return hipSuccess;
   if (a.top > kScoresMaxTop || a.top > a.vocab) return hipErrorInvalidValue;
+  const int S = splits(a, n_cu);
+  if (S > 1 && !a.ws) return hipErrorInvalidValue;
   switch (a.type) {
-    case kOpF32: hipLaunchKernelGGL(token_scores_kernel<kOpF32>, dim3(a.rows), dim3(kThreads), 0, s, a); break;
-    case kOpBf16: hipLaunchKernelGGL(token_scores_kernel<kOpBf16>, dim3(a.rows), dim3(kThreads), 0, s, a); break;
-    case kOpF16: hipLaunchKernelGGL(token_scores_kernel<kOpF16>, dim3(a.rows), dim3(kThreads), 0, s, a); break;
+    case kOpF32: return launch<kOpF32>(a, S, s);
+    case kOpBf16: return launch<kOpBf16>(a, S, s);
+    case kOpF16: return launch<kOpF16>(a, S, s);
     default: return hipErrorInvalidValue;
   }
-  return hipGetLastError();
 }
 
 }  // namespace itts
