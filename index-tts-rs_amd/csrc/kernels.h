@@ -308,6 +308,7 @@ bool sampler_stage(int dev, SamplerStage *out);
 // ---- decoding with drafted trees (kernels_tree.hip, kernels_scores.hip) ----
 enum OpType : int { kOpF32 = 0, kOpBf16 = 1, kOpF16 = 2 };
 constexpr int kTreeMaxNodes = 256;
+constexpr int kTreeMaxRowBytes = 1 << 26;  // cache rows apart: 32 of them within 32 bits of offset
 // Attention of the nodes of one tree a sequence over its cached rows and their own ancestors.
 // q, out [batch][n][H][D]; k, v [batch][Hk][max_seq][D] (strides in elements, D contiguous, rows at
 // multiples of 16 bytes); lengths [batch]; parents [batch][n] (par_b apart).  Types: q and the

@@ -18,8 +18,7 @@
 namespace itts {
 namespace {
 
-constexpr int kWaves = 4;       // waves of a block, each over its own tiles of keys
-constexpr int kTileKeys = 32;   // keys a wave takes at a time
+constexpr int kTileKeys = 32;  // keys a wave takes at a time
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct F32 {
@@ -173,6 +172,11 @@ struct Tree<1> {
   struct Row {
     uint64_t anc;
     __device__ bool sees(int j) const { return j < 64 && (anc >> (j & 63) & 1); }
+    // of the 32 rows from j0 on (counted from node 0's; negative: the sequence's) those that are seen
+    __device__ uint32_t tile(int j0) const {
+      if (j0 >= 0) return j0 < 64 ? (uint32_t)(anc >> (j0 & 63)) : 0;
+      return j0 > -32 ? (uint32_t)(anc << -j0) | ((1u << -j0) - 1) : ~0u;
+    }
     __device__ bool any() const { return anc != 0; }
   };
   __device__ Row row(int node, const Shared &) const { return Row{__shfl((unsigned long long)anc, node, 64)}; }
@@ -188,7 +192,7 @@ struct Tree<4> {
   };
   __device__ void read(int par, int n, Shared &t) {
     const int i = threadIdx.x;
-    static_assert(64 * kWaves >= kTreeMaxNodes, "a thread for each node");
+    // (a thread for each node: blocks have four waves at least)
     if (i == 0) t.live = 0;
     if (i < n) {
       t.up[i] = par >= -1 && par < i ? par : -2;
@@ -227,6 +231,14 @@ struct Tree<4> {
   struct Row {
     const uint64_t *anc;
     __device__ bool sees(int j) const { return j < kTreeMaxNodes && (anc[j >> 6] >> (j & 63) & 1); }
+    __device__ uint32_t tile(int j0) const {
+      if (j0 >= kTreeMaxNodes) return 0;
+      if (j0 >= 0) {
+        const int w = j0 >> 6, s = j0 & 63;
+        return (uint32_t)(anc[w] >> s | (s > 0 && w < 3 ? anc[w + 1] << (64 - s) : 0));
+      }
+      return j0 > -32 ? (uint32_t)(anc[0] << -j0) | ((1u << -j0) - 1) : ~0u;
+    }
     __device__ bool any() const { return (anc[0] | anc[1] | anc[2] | anc[3]) != 0; }
   };
   __device__ Row row(int node, const Shared &t) const { return Row{t.anc[node]}; }
@@ -238,55 +250,69 @@ __host__ __device__ inline size_t part_row(const TreeAttn &a, int S, int b, int 
 }
 
 // A wave's keys and values of one tile: key rows 16 h + c, in runs of 8 elements 32 j + 8 g, and value
-// rows 16 h + 4 g + r, elements D / 16 c ...
+// rows 16 h + 4 g + r, elements D / 16 c ...  Rows lie at the same offsets from every tile's first row
+// (32 bits, kept), so that a tile's loads need a new base alone, in scalar registers.
 template <int D, class T>
 struct TileRegs {
   static constexpr int kK = 8 * T::kBytes / 4, kV = D / 16 * T::kBytes / 4;  // dwords of a run
   uint32_t k[2][D / 32][kK];
   uint32_t v[8][kV];
-  __device__ __forceinline__ void load_k(const char *base, uint32_t step, int key0, int last, int c, int g) {
+  uint32_t k_at[2], v_at[8];
+  // offsets of a tile whose rows past row `last` are read as that one
+  __device__ __forceinline__ void place(uint32_t k_step, uint32_t v_step, int last, int c, int g) {
+#pragma unroll
+    for (int h = 0; h < 2; h++) k_at[h] = min(16 * h + c, last) * k_step + 8 * g * T::kBytes;
+#pragma unroll
+    for (int i = 0; i < 8; i++) v_at[i] = min(16 * (i >> 2) + 4 * g + (i & 3), last) * v_step + D / 16 * c * T::kBytes;
+  }
+  // (the offsets pass as new values, or they are kept widened to 64 bits)
+  __device__ __forceinline__ void load_k(const char *tile) {
 #pragma unroll
     for (int h = 0; h < 2; h++) {
-      const char *row = base + (uint64_t)(uint32_t)min(key0 + 16 * h + c, last) * step + 8 * g * T::kBytes;
+      asm volatile("" : "+v"(k_at[h]));
 #pragma unroll
-      for (int j = 0; j < D / 32; j++) load_dwords<kK>(row + 32 * j * T::kBytes, k[h][j]);
+      for (int j = 0; j < D / 32; j++) load_dwords<kK>(tile + 32 * j * T::kBytes + k_at[h], k[h][j]);
     }
   }
-  __device__ __forceinline__ void load_v(const char *base, uint32_t step, int key0, int last, int c, int g) {
+  __device__ __forceinline__ void load_v(const char *tile) {
 #pragma unroll
-    for (int i = 0; i < 8; i++)
-      load_dwords<kV>(base + (uint64_t)(uint32_t)min(key0 + 16 * (i >> 2) + 4 * g + (i & 3), last) * step +
-                          D / 16 * c * T::kBytes, v[i]);
+    for (int i = 0; i < 8; i++) {
+      asm volatile("" : "+v"(v_at[i]));
+      load_dwords<kV>(tile + v_at[i], v[i]);
+    }
   }
 };
 
-// TQ queries over TKV rows, RT tiles of 16 query rows, W words of nodes.  16-bit caches go through the
+// TQ queries over TKV rows, RT tiles of 16 query rows a wave, W words of nodes.  A block has WK x WR
+// waves: WK over tiles of keys, joined at the end, WR over query rows (which then read the same tiles
+// together: the first brings them into the cache next to the compute unit).  16-bit caches go through the
 // 16-bit matrix instructions: queries in NQ planes (fp32 ones in three, exactly), probabilities in NP
 // (two hold 16 bits of bf16 and 22 of fp16, far below the result's rounding; three an fp32's).
 // fp32 caches take the fp32 ones.
-template <int D, class TQ, class TKV, int RT, int W>
-__global__ __launch_bounds__(64 * kWaves, 2) void tree_attn_kernel(TreeAttn a, int S, float2 *ml) {
+template <int D, class TQ, class TKV, int RT, int W, int WK, int WR>
+__global__ __launch_bounds__(64 * WK * WR, WK * WR > 8 ? 4 : 2) void tree_attn_kernel(TreeAttn a, int S, float2 *ml) {
   constexpr bool kWide = TKV::kBytes == 4;
   constexpr int NQ = kWide || TQ::kBytes == 2 ? 1 : 3, NP = TQ::kBytes == 2 ? 2 : 3;
   // probabilities are held up to 2^(kLag + kUp): the running maximum moves only when a score passes
   // it by 2^kLag; fp16 planes use their range below 1 too
   constexpr float kLag = 5.0f, kUp = std::is_same_v<TKV, F16> ? 10.0f : 0.0f;
   __shared__ typename Tree<W>::Shared tree_mem;
-  __shared__ float so[kWaves][16 * RT][D + 4];
-  __shared__ float sm[kWaves][16 * RT], sl[kWaves][16 * RT];
-  __shared__ int sodd[kWaves];
+  __shared__ float so[WR][WK][16 * RT][D + 4];
+  __shared__ float sm[WR][WK][16 * RT], sl[WR][WK][16 * RT];
+  __shared__ int sodd[WR][WK];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
+  const int wk = wave % WK, wr = wave / WK;
   const int split = blockIdx.x, b = blockIdx.z;
   const int group = a.H / a.Hk, M = a.n * group;
-  const int hk = blockIdx.y % a.Hk, row0 = blockIdx.y / a.Hk * (16 * RT);
+  const int hk = blockIdx.y % a.Hk, row0 = (blockIdx.y / a.Hk * WR + wr) * (16 * RT);
 
   // Everything that does not wait for something else is loaded first: this wave's first tile too,
   // whose place does not depend on the length.
   const char *kb = static_cast<const char *>(a.k) + (b * a.k_b + hk * a.k_h) * TKV::kBytes;
   const char *vb = static_cast<const char *>(a.v) + (b * a.v_b + hk * a.v_h) * TKV::kBytes;
   const uint32_t k_step = (uint32_t)a.k_r * TKV::kBytes, v_step = (uint32_t)a.v_r * TKV::kBytes;
-  const int last = a.max_seq - 1, stride = S * kWaves * kTileKeys;
-  int key0 = (split * kWaves + wave) * kTileKeys;
+  const int stride = S * WK * kTileKeys;
+  int key0 = (split * WK + wk) * kTileKeys;
   const int len = a.lengths[b];
   const int par_at = W == 1 ? lane : threadIdx.x;
   const int par = par_at < a.n ? a.parents[b * a.par_b + par_at] : -2;
@@ -333,8 +359,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_attn_kernel(TreeAttn a, i
   }
   const float scale = kWide || NQ == 3 ? 1.0f : fabsf(a.scale) * kLog2e;
   TileRegs<D, TKV> x;
-  x.load_k(kb, k_step, key0, last, c, g);
-  x.load_v(vb, v_step, key0, last, c, g);
+  {
+    const int first = min(key0, a.max_seq - 1);
+    x.place(k_step, v_step, a.max_seq - 1 - first, c, g);
+    x.load_k(kb + (uint64_t)(uint32_t)first * k_step);
+    x.load_v(vb + (uint64_t)(uint32_t)first * v_step);
+  }
   Tree<W> tree;
   tree.read(par, a.n, tree_mem);
   const int live = tree.live;
@@ -370,19 +400,20 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_attn_kernel(TreeAttn a, i
     // the wave's next tile; past the last one every lane asks for the last row (one line), so that no
     // register is left as it was on some path
     const int next = min(key0 + stride, total - 1);
-    x.load_k(kb, k_step, next, total - 1, c, g);
+    if (next + kTileKeys > total) x.place(k_step, v_step, total - 1 - next, c, g);
+    x.load_k(kb + (uint64_t)(uint32_t)next * k_step);
 
     const bool edge = key0 + kTileKeys > len;  // holds nodes, or ends past the last row
+    uint32_t seen[RT];  // bit 16 h + r: key 16 h + 4 g + r
     if (edge) {
 #pragma unroll
-      for (int t = 0; t < RT; t++)
+      for (int t = 0; t < RT; t++) {
+        seen[t] = sees[t].tile(key0 - len) >> (4 * g);
 #pragma unroll
         for (int h = 0; h < 2; h++)
 #pragma unroll
-          for (int r = 0; r < 4; r++) {
-            const int j = key0 + 16 * h + 4 * g + r - len;
-            if (j >= 0 && !(j < live && sees[t].sees(j))) s[h][t][r] = -INFINITY;
-          }
+          for (int r = 0; r < 4; r++) s[h][t][r] = seen[t] & 1u << (16 * h + r) ? s[h][t][r] : -INFINITY;
+      }
     }
     float top[RT];
     bool grows = false;
@@ -411,10 +442,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_attn_kernel(TreeAttn a, i
 #pragma unroll
         for (int r = 0; r < 4; r++) {
           float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[h][t][r], scale, -ms));
-          if (edge) {  // (a scale of 0 makes NaN of the mask's -inf)
-            const int j = key0 + 16 * h + 4 * g + r - len;
-            if (j >= 0 && !(j < live && sees[t].sees(j))) p = 0.0f;
-          }
+          if (edge) p = seen[t] & 1u << (16 * h + r) ? p : 0.0f;  // (a scale of 0 makes NaN of the mask's -inf)
           s[h][t][r] = p;
           l[t] += p;
         }
@@ -427,19 +455,20 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_attn_kernel(TreeAttn a, i
 #pragma unroll
       for (int i = 0; i < 8; i++) {
         const int key = key0 + 16 * (i >> 2) + 4 * g + (i & 3);
+        const uint32_t own = key < len ? ~0u : 0, in = key < total ? ~0u : 0;
 #pragma unroll
         for (int d = 0; d < TileRegs<D, TKV>::kV; d++) {
           const uint32_t v = x.v[i][d];
-          uint32_t keep = ~0u;
+          uint32_t keep;
           if constexpr (kWide) {
-            if ((v & 0x7f800000u) == 0x7f800000u) keep = 0;
+            keep = (v & 0x7f800000u) == 0x7f800000u ? 0 : ~0u;
           } else {
-            if ((v & TKV::kOddBits) == TKV::kOddBits) keep &= 0xffff0000u;
-            if ((v >> 16 & TKV::kOddBits) == TKV::kOddBits) keep &= 0x0000ffffu;
+            keep = (v & TKV::kOddBits) == TKV::kOddBits ? 0xffff0000u : ~0u;
+            keep = (v & TKV::kOddBits << 16) == TKV::kOddBits << 16 ? keep & 0xffffu : keep;
           }
-          if (key < len) keep = ~0u;
-          odd |= key < total ? ~keep : 0;
-          x.v[i][d] = key < total ? v & keep : 0;
+          keep |= own;
+          odd |= ~keep & in;
+          x.v[i][d] = v & keep & in;
         }
       }
     }
@@ -475,40 +504,42 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_attn_kernel(TreeAttn a, i
           for (int d = 0; d < D / 16; d++) o[t][d] = mfma16<TKV>(vt[d], p[k], o[t][d]);
       }
     }
-    x.load_v(vb, v_step, next, total - 1, c, g);
+    x.load_v(vb + (uint64_t)(uint32_t)next * v_step);
   }
 
-  if (const bool any = __ballot(odd != 0) != 0; lane == 0) sodd[wave] = any;
-  // the block's waves joined: lane (c, g) holds dims D/4 g .. of column c, in runs of D/16 a register
+  // The waves over keys joined, each then a share of the rows' quarters: lane (c, g) holds dims D/4 g ..
+  // of column c, in runs of D/16 a register.
+  if (const bool any = __ballot(odd != 0) != 0; lane == 0) sodd[wr][wk] = any;
 #pragma unroll
   for (int t = 0; t < RT; t++) {
     l[t] = col_sum(l[t]);
-    if (g == 0) sm[wave][16 * t + c] = m[t], sl[wave][16 * t + c] = l[t];
+    if (g == 0) sm[wr][wk][16 * t + c] = m[t], sl[wr][wk][16 * t + c] = l[t];
 #pragma unroll
     for (int r = 0; r < 4; r++)
 #pragma unroll
       for (int d = 0; d < D / 16; d += 4)
-        *reinterpret_cast<float4 *>(&so[wave][16 * t + c][D / 16 * (4 * g + r) + d]) =
+        *reinterpret_cast<float4 *>(&so[wr][wk][16 * t + c][D / 16 * (4 * g + r) + d]) =
             make_float4(o[t][d][r], o[t][d + 1][r], o[t][d + 2][r], o[t][d + 3][r]);
   }
   __syncthreads();
-  const bool odd_any = (sodd[0] | sodd[1] | sodd[2] | sodd[3]) != 0;
-  static_assert(kWaves == 4, "flags of four waves");
-  for (int i0 = 0; i0 < 16 * RT * (D / 4); i0 += 64 * kWaves) {
-    const int i = i0 + threadIdx.x;
-    const int rr = i / (D / 4), d = i % (D / 4) * 4, row = row0 + rr, i_node = min(row, M - 1) / group;
+  int odd_any = 0;
+#pragma unroll
+  for (int w = 0; w < WK; w++) odd_any |= sodd[wr][w];
+  for (int i0 = 0; i0 < 16 * RT * (D / 4); i0 += 64 * WK) {
+    const int i = i0 + wk * 64 + lane;
+    const int rr = min(i / (D / 4), 16 * RT - 1), d = i % (D / 4) * 4, row = row0 + rr, i_node = min(row, M - 1) / group;
     const auto seen = tree.row(i_node, tree_mem);
     const bool any = seen.any();
-    if (row >= M) continue;
+    if (row >= M || i >= 16 * RT * (D / 4)) continue;
     float top = -INFINITY, sum = 0.0f, y[4] = {};
 #pragma unroll
-    for (int w = 0; w < kWaves; w++) top = fmaxf(top, sm[w][rr]);
+    for (int w = 0; w < WK; w++) top = fmaxf(top, sm[wr][w][rr]);
     const float ms = top == -INFINITY ? 0.0f : top;
 #pragma unroll
-    for (int w = 0; w < kWaves; w++) {
-      const float f = __builtin_amdgcn_exp2f(sm[w][rr] - ms);
-      const float4 v = *reinterpret_cast<const float4 *>(&so[w][rr][d]);
-      sum += f * sl[w][rr];
+    for (int w = 0; w < WK; w++) {
+      const float f = __builtin_amdgcn_exp2f(sm[wr][w][rr] - ms);
+      const float4 v = *reinterpret_cast<const float4 *>(&so[wr][w][rr][d]);
+      sum += f * sl[wr][w][rr];
       y[0] += f * v.x, y[1] += f * v.y, y[2] += f * v.z, y[3] += f * v.w;
     }
     if (odd_any) {  // (a positive probability times an infinity or NaN is that)
@@ -533,8 +564,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_attn_kernel(TreeAttn a, i
       // what the joining kernel cannot tell by itself goes with the statistics: a row that sees
       // nothing has maximum +inf and sum 0, one of a bad sequence sum NaN
       const size_t at = part_row(a, S, b, hk, row) + split;
-      if (split * kWaves * kTileKeys < total)
-        *reinterpret_cast<float4 *>(a.part + at * D + d) = make_float4(y[0], y[1], y[2], y[3]);
+      if (split * WK * kTileKeys < total) *reinterpret_cast<float4 *>(a.part + at * D + d) = make_float4(y[0], y[1], y[2], y[3]);
       if (d == 0) ml[at] = bad ? make_float2(0.0f, NAN) : any ? make_float2(top, sum) : make_float2(INFINITY, 0.0f);
     }
   }
@@ -569,45 +599,58 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeAttn a, int S, const
   store4<TQ>(static_cast<char *>(a.out) + to * TQ::kBytes, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
 }
 
-struct Plan {
-  int S, RT, row_tiles;
-};
 // Most tiles of 16 query rows a wave takes: as many as its registers hold (256 a lane, two waves a
 // SIMD).  fp32 queries take up to three times the registers of 16-bit ones.
 constexpr int most_tiles(int D, int q_bytes) { return (q_bytes == 4 ? 128 : 256) / D; }
+// Waves over keys of a large block: RT 1 at D 64 fits 128 registers, the others 256.
+constexpr int large_waves(int D, int RT, int kv_bytes) { return D == 64 && RT == 1 && kv_bytes == 2 ? 16 : 8; }
 
+struct Plan {
+  int S, RT, WK, WR, row_tiles;
+};
 Plan make_plan(const TreeAttn &a, int n_cu) {
   Plan p;
   const int M = a.n * (a.H / a.Hk), most = most_tiles(a.D, a.qt == kOpF32 ? 4 : 2);
   p.RT = a.n > 64 ? most : std::min(most, M <= 16 ? 1 : M <= 32 ? 2 : 4);
-  p.row_tiles = (M + 16 * p.RT - 1) / (16 * p.RT);
   const int tiles = (a.max_seq + kTileKeys - 1) / kTileKeys;
+  p.WR = a.qt != kOpF32 && M > 2 * 16 * p.RT ? 4 : 1;
+  p.row_tiles = (M + 16 * p.RT * p.WR - 1) / (16 * p.RT * p.WR);
   const int64_t blocks = (int64_t)a.batch * a.Hk * p.row_tiles;
-  const int64_t want = (4 * n_cu + blocks - 1) / blocks, can = (tiles + 2 * kWaves - 1) / (2 * kWaves);
+  p.WK = p.WR > 1 ? 1 : blocks >= 2 * n_cu ? 4 : large_waves(a.D, p.RT, a.kvt == kOpF32 ? 4 : 2);
+  if (a.n > 64 && p.WR == 1) p.WK = 4;
+  const int64_t want = (8 * n_cu / (p.WK * p.WR) + blocks - 1) / blocks, can = (tiles + 4 * p.WK - 1) / (4 * p.WK);
   p.S = (int)std::max<int64_t>(1, std::min<int64_t>({want, can, 64}));
   return p;
 }
 
-template <int D, class TQ, class TKV, int RT, int W>
+template <int D, class TQ, class TKV, int RT, int W, int WK, int WR>
 hipError_t launch_rt(const TreeAttn &a, const Plan &p, hipStream_t s) {
   float2 *ml = reinterpret_cast<float2 *>(a.part + (size_t)a.batch * a.H * a.n * p.S * D);
-  hipLaunchKernelGGL((tree_attn_kernel<D, TQ, TKV, RT, W>), dim3(p.S, a.Hk * p.row_tiles, a.batch), dim3(64 * kWaves), 0, s,
-                     a, p.S, ml);
+  hipLaunchKernelGGL((tree_attn_kernel<D, TQ, TKV, RT, W, WK, WR>), dim3(p.S, a.Hk * p.row_tiles, a.batch),
+                     dim3(64 * WK * WR), 0, s, a, p.S, ml);
   if (hipError_t e = hipGetLastError(); e != hipSuccess || p.S == 1) return e;
   const int64_t rows = (int64_t)a.batch * a.H * a.n;
   constexpr int kRows = 256 / (D / 4);
   hipLaunchKernelGGL((tree_join_kernel<D, TQ>), dim3((unsigned)((rows + kRows - 1) / kRows)), dim3(256), 0, s, a, p.S, ml);
   return hipGetLastError();
 }
+template <int D, class TQ, class TKV, int RT>
+hipError_t launch_keys(const TreeAttn &a, const Plan &p, hipStream_t s) {
+  if (p.WK == 4) return launch_rt<D, TQ, TKV, RT, 1, 4, 1>(a, p, s);
+  return launch_rt<D, TQ, TKV, RT, 1, large_waves(D, RT, TKV::kBytes), 1>(a, p, s);
+}
 template <int D, class TQ, class TKV>
 hipError_t launch_d(const TreeAttn &a, const Plan &p, hipStream_t s) {
   constexpr int kMost = most_tiles(D, TQ::kBytes);
-  if (a.n > 64) return launch_rt<D, TQ, TKV, kMost, 4>(a, p, s);
+  if constexpr (TQ::kBytes == 2)
+    if (p.WR == 4)
+      return a.n > 64 ? launch_rt<D, TQ, TKV, kMost, 4, 1, 4>(a, p, s) : launch_rt<D, TQ, TKV, kMost, 1, 1, 4>(a, p, s);
+  if (a.n > 64) return launch_rt<D, TQ, TKV, kMost, 4, 4, 1>(a, p, s);
   if constexpr (kMost >= 4)
-    if (p.RT == 4) return launch_rt<D, TQ, TKV, 4, 1>(a, p, s);
+    if (p.RT == 4) return launch_keys<D, TQ, TKV, 4>(a, p, s);
   if constexpr (kMost >= 2)
-    if (p.RT == 2) return launch_rt<D, TQ, TKV, 2, 1>(a, p, s);
-  return launch_rt<D, TQ, TKV, 1, 1>(a, p, s);
+    if (p.RT == 2) return launch_keys<D, TQ, TKV, 2>(a, p, s);
+  return launch_keys<D, TQ, TKV, 1>(a, p, s);
 }
 template <class TQ, class TKV>
 hipError_t launch_t(const TreeAttn &a, const Plan &p, hipStream_t s) {

@@ -111,8 +111,8 @@ itts_status tree_args(const itts_tree_attention_args *a, TreeAttn *o) {
     return fail(ITTS_E_VALIDATION, "k: rows must start at multiples of 16 bytes");
   if (!row_stride(a->v_batch, b, ks) || !row_stride(a->v_head, hk, ks) || !row_stride(a->v_row, a->max_seq, ks) || !aligned16(a->v))
     return fail(ITTS_E_VALIDATION, "v: rows must start at multiples of 16 bytes");
-  if (a->max_seq > 1 && (a->k_row * ks > INT32_MAX || a->v_row * ks > INT32_MAX))
-    return fail(ITTS_E_VALIDATION, "k_row, v_row: rows must be less than 2^31 bytes apart");
+  if (a->max_seq > 1 && (a->k_row * ks > kTreeMaxRowBytes || a->v_row * ks > kTreeMaxRowBytes))
+    return fail(ITTS_E_VALIDATION, "k_row, v_row: rows must be at most %d bytes apart", kTreeMaxRowBytes);
   if (b > 1 && a->parents_batch < 0) return fail(ITTS_E_VALIDATION, "parents: negative stride");
   *o = TreeAttn{a->q, a->k, a->v, a->out, a->lengths, a->parents, b, n, h, hk, a->head_dim, a->max_seq, qt, kvt, a->scale,
                 a->q_batch, a->q_node, a->q_head, a->out_batch, a->out_node, a->out_head, a->k_batch, a->k_head, a->k_row,

@@ -52,19 +52,22 @@ def _last_contiguous(t, name: str):
         _refuse(f"{name}: the last dimension must be contiguous")
 
 
+# The current stream's handle without a Stream object around it (2 us of a call's host time).
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+
+
 def _run(fn, need, args, device):
     """Enqueues on the device's current stream, with the workspace that the sizes need."""
-    with torch.cuda.device(device):
-        ws, size = None, C.c_uint64(0)
-        if need is not None:
-            _check(need(C.byref(args), C.byref(size)))
-            if size.value:
-                ws = torch.empty(size.value, dtype=torch.uint8, device=device)
-        stream = torch.cuda.current_stream(device).cuda_stream
-        if need is None:
-            _check(fn(C.byref(args), stream))
-        else:
-            _check(fn(C.byref(args), ws.data_ptr() if ws is not None else None, size, stream))
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _run(fn, need, args, device)
+    ref = C.byref(args)
+    if need is None:
+        return _check(fn(ref, _stream(device.index)))
+    size = C.c_uint64()
+    _check(need(ref, C.byref(size)))
+    ws = torch.empty(size.value, dtype=torch.uint8, device=device) if size.value else None
+    _check(fn(ref, None if ws is None else ws.data_ptr(), size, _stream(device.index)))
 
 
 def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: torch.Tensor, parents: torch.Tensor, *,
