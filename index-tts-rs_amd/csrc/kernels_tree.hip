@@ -244,10 +244,19 @@ struct Tree<4> {
   __device__ Row row(int node, const Shared &t) const { return Row{t.anc[node]}; }
 };
 
-// Partial results of key split s: o [batch][Hk][M][S][D], then (max, sum) [batch][Hk][M][S].
-__host__ __device__ inline size_t part_row(const TreeAttn &a, int S, int b, int hk, int row) {
-  return (((size_t)b * a.Hk + hk) * (a.n * (a.H / a.Hk)) + row) * S;
-}
+// A launch: the split over keys (S blocks of a sequence, key head and row tile), their results (o
+// [batch][Hk][M][S][D], then (max, sum) [batch][Hk][M][S]), and the query rows of a key head, row
+// r being head r % group of node r / group.
+struct Args {
+  TreeAttn a;
+  int S, M, group;
+  uint32_t group_mul;  // 2^32 / group, rounded up: exact for rows < 2^32 / group
+  float2 *ml;
+  __device__ int node(int row) const { return group == 1 ? row : __umulhi((uint32_t)row, group_mul); }
+  __device__ size_t part(int b, int hk, int row, int split) const {
+    return (((size_t)b * a.Hk + hk) * M + row) * S + split;
+  }
+};
 
 // A wave's keys and values of one tile: key rows 16 h + c, in runs of 8 elements 32 j + 8 g, and value
 // rows 16 h + 4 g + r, elements D / 16 c ...  Rows lie at the same offsets from every tile's first row
@@ -283,137 +292,95 @@ struct TileRegs {
   }
 };
 
-// TQ queries over TKV rows, RT tiles of 16 query rows a wave, W words of nodes.  A block has WK x WR
-// waves: WK over tiles of keys, joined at the end, WR over query rows (which then read the same tiles
-// together: the first brings them into the cache next to the compute unit).  16-bit caches go through the
-// 16-bit matrix instructions: queries in NQ planes (fp32 ones in three, exactly), probabilities in NP
-// (two hold 16 bits of bf16 and 22 of fp16, far below the result's rounding; three an fp32's).
-// fp32 caches take the fp32 ones.
-template <int D, class TQ, class TKV, int RT, int W, int WK, int WR>
-__global__ __launch_bounds__(64 * WK * WR, WK * WR > 8 ? 4 : 2) void tree_attn_kernel(TreeAttn a, int S, float2 *ml) {
-  constexpr bool kWide = TKV::kBytes == 4;
-  constexpr int NQ = kWide || TQ::kBytes == 2 ? 1 : 3, NP = TQ::kBytes == 2 ? 2 : 3;
+// What a wave holds of RT tiles of 16 query rows (lane (c, g): row c of each), and the three steps of
+// a tile of keys.  16-bit caches go through the 16-bit matrix instructions: queries in NQ planes (fp32
+// ones in three, exactly), probabilities in NP (two hold 16 bits of bf16 and 22 of fp16, far below
+// the result's rounding; three an fp32's).  fp32 caches take the fp32 ones.
+template <int D, class TQ, class TKV, int RT>
+struct Rows {
+  static constexpr bool kWide = TKV::kBytes == 4;
+  static constexpr int NQ = kWide || TQ::kBytes == 2 ? 1 : 3, NP = TQ::kBytes == 2 ? 2 : 3;
+  static constexpr int kV = D / 16 * TKV::kBytes / 4;
   // probabilities are held up to 2^(kLag + kUp): the running maximum moves only when a score passes
   // it by 2^kLag; fp16 planes use their range below 1 too
-  constexpr float kLag = 5.0f, kUp = std::is_same_v<TKV, F16> ? 10.0f : 0.0f;
-  __shared__ typename Tree<W>::Shared tree_mem;
-  __shared__ float so[WR][WK][16 * RT][D + 4];
-  __shared__ float sm[WR][WK][16 * RT], sl[WR][WK][16 * RT];
-  __shared__ int sodd[WR][WK];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
-  const int wk = wave % WK, wr = wave / WK;
-  const int split = blockIdx.x, b = blockIdx.z;
-  const int group = a.H / a.Hk, M = a.n * group;
-  const int hk = blockIdx.y % a.Hk, row0 = (blockIdx.y / a.Hk * WR + wr) * (16 * RT);
-
-  // Everything that does not wait for something else is loaded first: this wave's first tile too,
-  // whose place does not depend on the length.
-  const char *kb = static_cast<const char *>(a.k) + (b * a.k_b + hk * a.k_h) * TKV::kBytes;
-  const char *vb = static_cast<const char *>(a.v) + (b * a.v_b + hk * a.v_h) * TKV::kBytes;
-  const uint32_t k_step = (uint32_t)a.k_r * TKV::kBytes, v_step = (uint32_t)a.v_r * TKV::kBytes;
-  const int stride = S * WK * kTileKeys;
-  int key0 = (split * WK + wk) * kTileKeys;
-  const int len = a.lengths[b];
-  const int par_at = W == 1 ? lane : threadIdx.x;
-  const int par = par_at < a.n ? a.parents[b * a.par_b + par_at] : -2;
+  static constexpr float kLag = 5.0f, kUp = std::is_same_v<TKV, F16> ? 10.0f : 0.0f;
+  uint32_t q[NQ][RT][D / 32][kWide ? 8 : 4];  // elements 32 j + 8 g ..
   int node[RT];
-  uint32_t q[NQ][RT][D / 32][kWide ? 8 : 4];
-  {
+  float scale;  // what a score is still multiplied by, for powers of two
+  floatx4 o[RT][D / 16];
+  float m[RT], l[RT];
+
+  __device__ __forceinline__ void load(const Args &p, int b, int hk, int row0, int c, int g) {
     uint32_t raw[RT][D / 32][8 * TQ::kBytes / 4];
+    const TreeAttn &a = p.a;
 #pragma unroll
     for (int t = 0; t < RT; t++) {
-      const int row = min(row0 + 16 * t + c, M - 1);
-      node[t] = row / group;
-      const char *at = static_cast<const char *>(a.q) +
-                       (b * a.q_b + node[t] * a.q_n + (hk * group + row % group) * a.q_h + 8 * g) * TQ::kBytes;
+      const int row = min(row0 + 16 * t + c, p.M - 1);
+      node[t] = p.node(row);
+      const int64_t head = hk * p.group + (row - node[t] * p.group);
+      const char *at = static_cast<const char *>(a.q) + (b * a.q_b + node[t] * a.q_n + head * a.q_h + 8 * g) * TQ::kBytes;
 #pragma unroll
       for (int j = 0; j < D / 32; j++) load_dwords<8 * TQ::kBytes / 4>(at + 32 * j * TQ::kBytes, raw[t][j]);
+      m[t] = -INFINITY, l[t] = 0.0f;
+#pragma unroll
+      for (int d = 0; d < D / 16; d++) o[t][d] = floatx4{};
     }
-    if constexpr (kWide || NQ == 3) {  // fp32 queries carry the scale
-      const float scale = a.scale * kLog2e;
+    const float by = a.scale * kLog2e;
+    const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0;
+    scale = kWide || NQ == 3 ? 1.0f : fabsf(by);
 #pragma unroll
-      for (int t = 0; t < RT; t++)
+    for (int t = 0; t < RT; t++)
 #pragma unroll
-        for (int j = 0; j < D / 32; j++)
+      for (int j = 0; j < D / 32; j++) {
+        if constexpr (kWide) {  // fp32 queries carry the scale
 #pragma unroll
-          for (int e = 0; e < 8; e += 2) {
-            const float x = __uint_as_float(raw[t][j][e]) * scale, y = __uint_as_float(raw[t][j][e + 1]) * scale;
-            if constexpr (kWide) {
-              q[0][t][j][e] = __float_as_uint(x), q[0][t][j][e + 1] = __float_as_uint(y);
-            } else {
-              uint32_t o[3];
-              cut2<TKV, 3>(x, y, o);
+          for (int e = 0; e < 8; e++) q[0][t][j][e] = __float_as_uint(__uint_as_float(raw[t][j][e]) * by);
+        } else if constexpr (NQ == 3) {
 #pragma unroll
-              for (int p = 0; p < 3; p++) q[p][t][j][e / 2] = o[p];
-            }
+          for (int e = 0; e < 4; e++) {
+            uint32_t w[3];
+            cut2<TKV, 3>(__uint_as_float(raw[t][j][2 * e]) * by, __uint_as_float(raw[t][j][2 * e + 1]) * by, w);
+#pragma unroll
+            for (int i = 0; i < 3; i++) q[i][t][j][e] = w[i];
           }
-    } else {  // 16-bit ones its sign
-      const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0;
-#pragma unroll
-      for (int t = 0; t < RT; t++)
-#pragma unroll
-        for (int j = 0; j < D / 32; j++)
+        } else {  // 16-bit ones its sign
 #pragma unroll
           for (int e = 0; e < 4; e++) q[0][t][j][e] = raw[t][j][e] ^ flip;
+        }
+      }
+  }
+
+  // s[h][t]: keys 16 h + 4 g + r of tile t's row c; k[h]: the keys' elements 32 j + 8 g ..
+  template <int N>
+  __device__ __forceinline__ void scores(floatx4 (&s)[2][RT], int j, const uint32_t (&k0)[N], const uint32_t (&k1)[N]) const {
+    if constexpr (kWide) {
+#pragma unroll
+      for (int e = 0; e < 8; e++)
+#pragma unroll
+        for (int t = 0; t < RT; t++) {
+          s[0][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k0[e]), __uint_as_float(q[0][t][j][e]), s[0][t], 0, 0, 0);
+          s[1][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k1[e]), __uint_as_float(q[0][t][j][e]), s[1][t], 0, 0, 0);
+        }
+    } else {
+#pragma unroll
+      for (int i = NQ - 1; i >= 0; i--)
+#pragma unroll
+        for (int t = 0; t < RT; t++) {
+          s[0][t] = mfma16<TKV>(k0, q[i][t][j], s[0][t]);
+          s[1][t] = mfma16<TKV>(k1, q[i][t][j], s[1][t]);
+        }
     }
   }
-  const float scale = kWide || NQ == 3 ? 1.0f : fabsf(a.scale) * kLog2e;
-  TileRegs<D, TKV> x;
-  {
-    const int first = min(key0, a.max_seq - 1);
-    x.place(k_step, v_step, a.max_seq - 1 - first, c, g);
-    x.load_k(kb + (uint64_t)(uint32_t)first * k_step);
-    x.load_v(vb + (uint64_t)(uint32_t)first * v_step);
-  }
-  Tree<W> tree;
-  tree.read(par, a.n, tree_mem);
-  const int live = tree.live;
-  const bool bad = len < 0 || live > a.max_seq || len > a.max_seq - live;
-  const int total = bad ? 0 : len + live;
-  typename Tree<W>::Row sees[RT];
-#pragma unroll
-  for (int t = 0; t < RT; t++) sees[t] = tree.row(node[t], tree_mem);
 
-  floatx4 o[RT][D / 16] = {};
-  float m[RT], l[RT];
-  uint32_t odd = 0;  // a node's value that is no finite number was taken out
-#pragma unroll
-  for (int t = 0; t < RT; t++) m[t] = -INFINITY, l[t] = 0.0f;
-
-  for (; key0 < total; key0 += stride) {
-    floatx4 s[2][RT] = {};
-#pragma unroll
-    for (int h = 0; h < 2; h++)
-#pragma unroll
-      for (int j = 0; j < D / 32; j++)
-#pragma unroll
-        for (int t = 0; t < RT; t++)
-          if constexpr (kWide) {
-#pragma unroll
-            for (int e = 0; e < 8; e++)
-              s[h][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(x.k[h][j][e]), __uint_as_float(q[0][t][j][e]),
-                                                             s[h][t], 0, 0, 0);
-          } else {
-#pragma unroll
-            for (int p = NQ - 1; p >= 0; p--) s[h][t] = mfma16<TKV>(x.k[h][j], q[p][t][j], s[h][t]);
-          }
-    // the wave's next tile; past the last one every lane asks for the last row (one line), so that no
-    // register is left as it was on some path
-    const int next = min(key0 + stride, total - 1);
-    if (next + kTileKeys > total) x.place(k_step, v_step, total - 1 - next, c, g);
-    x.load_k(kb + (uint64_t)(uint32_t)next * k_step);
-
-    const bool edge = key0 + kTileKeys > len;  // holds nodes, or ends past the last row
-    uint32_t seen[RT];  // bit 16 h + r: key 16 h + 4 g + r
+  // Scores to probabilities, sums and (where a maximum moves) results rescaled.  At an edge bit
+  // 16 h + r of seen[t] says whether key 16 h + 4 g + r counts.
+  __device__ __forceinline__ void soften(floatx4 (&s)[2][RT], bool edge, const uint32_t (&seen)[RT]) {
     if (edge) {
 #pragma unroll
-      for (int t = 0; t < RT; t++) {
-        seen[t] = sees[t].tile(key0 - len) >> (4 * g);
+      for (int t = 0; t < RT; t++)
 #pragma unroll
-        for (int h = 0; h < 2; h++)
-#pragma unroll
-          for (int r = 0; r < 4; r++) s[h][t][r] = seen[t] & 1u << (16 * h + r) ? s[h][t][r] : -INFINITY;
-      }
+        for (int i = 0; i < 8; i++)
+          s[i >> 2][t][i & 3] = seen[t] & 1u << (16 * (i >> 2) + (i & 3)) ? s[i >> 2][t][i & 3] : -INFINITY;
     }
     float top[RT];
     bool grows = false;
@@ -438,40 +405,18 @@ __global__ __launch_bounds__(64 * WK * WR, WK * WR > 8 ? 4 : 2) void tree_attn_k
     for (int t = 0; t < RT; t++) {
       const float ms = (m[t] == -INFINITY ? 0.0f : m[t]) - kUp;
 #pragma unroll
-      for (int h = 0; h < 2; h++)
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-          float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[h][t][r], scale, -ms));
-          if (edge) p = seen[t] & 1u << (16 * h + r) ? p : 0.0f;  // (a scale of 0 makes NaN of the mask's -inf)
-          s[h][t][r] = p;
-          l[t] += p;
-        }
-    }
-
-    if (edge) {
-      // Rows of nodes count only where they are seen, and rows past the last one nowhere: 0 times
-      // what a masked row may hold (infinities, NaN) must stay out of the product, so such values
-      // leave it and are added at the end, row by row.
-#pragma unroll
       for (int i = 0; i < 8; i++) {
-        const int key = key0 + 16 * (i >> 2) + 4 * g + (i & 3);
-        const uint32_t own = key < len ? ~0u : 0, in = key < total ? ~0u : 0;
-#pragma unroll
-        for (int d = 0; d < TileRegs<D, TKV>::kV; d++) {
-          const uint32_t v = x.v[i][d];
-          uint32_t keep;
-          if constexpr (kWide) {
-            keep = (v & 0x7f800000u) == 0x7f800000u ? 0 : ~0u;
-          } else {
-            keep = (v & TKV::kOddBits) == TKV::kOddBits ? 0xffff0000u : ~0u;
-            keep = (v & TKV::kOddBits << 16) == TKV::kOddBits << 16 ? keep & 0xffffu : keep;
-          }
-          keep |= own;
-          odd |= ~keep & in;
-          x.v[i][d] = v & keep & in;
-        }
+        float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 2][t][i & 3], scale, -ms));
+        // (a scale of 0 makes NaN of the mask's -inf)
+        if (edge) p = seen[t] & 1u << (16 * (i >> 2) + (i & 3)) ? p : 0.0f;
+        s[i >> 2][t][i & 3] = p;
+        l[t] += p;
       }
     }
+  }
+
+  // o += P V; v[i]: elements D / 16 c .. of key 16 (i / 4) + 4 g + i % 4
+  __device__ __forceinline__ void add(const floatx4 (&s)[2][RT], const uint32_t (&v)[8][kV]) {
     if constexpr (kWide) {
 #pragma unroll
       for (int i = 0; i < 8; i++)
@@ -479,7 +424,7 @@ __global__ __launch_bounds__(64 * WK * WR, WK * WR > 8 ? 4 : 2) void tree_attn_k
         for (int t = 0; t < RT; t++)
 #pragma unroll
           for (int d = 0; d < D / 16; d++)
-            o[t][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(x.v[i][d]), s[i >> 2][t][i & 3], o[t][d], 0, 0, 0);
+            o[t][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v[i][d]), s[i >> 2][t][i & 3], o[t][d], 0, 0, 0);
     } else {
       // operands of 8 keys a lane: V^T by element pairs from its 8 rows, P as it stands
       uint32_t vt[D / 16][4];
@@ -487,7 +432,7 @@ __global__ __launch_bounds__(64 * WK * WR, WK * WR > 8 ? 4 : 2) void tree_attn_k
       for (int d = 0; d < D / 16; d++)
 #pragma unroll
         for (int i = 0; i < 4; i++)
-          vt[d][i] = __builtin_amdgcn_perm(x.v[2 * i + 1][d / 2], x.v[2 * i][d / 2], d % 2 ? 0x07060302u : 0x05040100u);
+          vt[d][i] = __builtin_amdgcn_perm(v[2 * i + 1][d / 2], v[2 * i][d / 2], d % 2 ? 0x07060302u : 0x05040100u);
 #pragma unroll
       for (int t = 0; t < RT; t++) {
         uint32_t p[NP][4];
@@ -504,81 +449,296 @@ __global__ __launch_bounds__(64 * WK * WR, WK * WR > 8 ? 4 : 2) void tree_attn_k
           for (int d = 0; d < D / 16; d++) o[t][d] = mfma16<TKV>(vt[d], p[k], o[t][d]);
       }
     }
+  }
+};
+
+// Rows of nodes count only where they are seen, and rows past the last one nowhere: 0 times what a
+// masked row may hold (infinities, NaN) must stay out of a tile's product, so such values leave it
+// and are added at the end, row by row (odd_values).  Returns whether there were any.
+template <class T, int N>
+__device__ __forceinline__ uint32_t take_odd(uint32_t (&v)[8][N], int key0, int len, int total, int g) {
+  uint32_t odd = 0;
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    const int key = key0 + 16 * (i >> 2) + 4 * g + (i & 3);
+    const uint32_t own = key < len ? ~0u : 0, in = key < total ? ~0u : 0;
+#pragma unroll
+    for (int d = 0; d < N; d++) {
+      const uint32_t w = v[i][d];
+      uint32_t keep;
+      if constexpr (T::kBytes == 4) {
+        keep = (w & 0x7f800000u) == 0x7f800000u ? 0 : ~0u;
+      } else {
+        keep = (w & T::kOddBits) == T::kOddBits ? 0xffff0000u : ~0u;
+        keep = (w & T::kOddBits << 16) == T::kOddBits << 16 ? keep & 0xffffu : keep;
+      }
+      keep |= own;
+      odd |= ~keep & in;
+      v[i][d] = w & keep & in;
+    }
+  }
+  return odd;
+}
+// y[0 .. N) += such values of the nodes that a row sees (a positive probability times an infinity or
+// NaN is that); at: element y[0]'s place in node 0's row.
+template <class T, int N, class Seen>
+__device__ inline void odd_values(float *y, const Seen &seen, int live, const char *at, uint32_t step) {
+#pragma unroll 1
+  for (int j = 0; j < live; j++) {
+    if (!seen.sees(j)) continue;
+#pragma unroll
+    for (int e = 0; e < N; e++) {
+      const float v = load1<T>(at + (uint64_t)(uint32_t)j * step + e * T::kBytes);
+      if (!(fabsf(v) < INFINITY)) y[e] += v;
+    }
+  }
+}
+
+// Four elements d .. of a row's result over this block's keys, to the output or the splits' results.
+// What the joining kernel cannot tell by itself goes with the statistics: a row that sees nothing
+// has maximum +inf and sum 0, one of a bad sequence sum NaN.
+template <int D, class TQ>
+__device__ __forceinline__ void put4(const Args &p, int b, int hk, int row, int node, int split, int d, float *y, float top,
+                                     float sum, bool bad, bool any, bool keys) {
+  if (p.S == 1) {
+    const float inv = 1.0f / sum;
+#pragma unroll
+    for (int e = 0; e < 4; e++) y[e] = bad ? NAN : any ? y[e] * inv : 0.0f;
+    const int64_t at = b * p.a.o_b + node * p.a.o_n + (hk * p.group + (row - node * p.group)) * p.a.o_h + d;
+    store4<TQ>(static_cast<char *>(p.a.out) + at * TQ::kBytes, y[0], y[1], y[2], y[3]);
+  } else {
+    const size_t at = p.part(b, hk, row, split);
+    if (keys) *reinterpret_cast<float4 *>(p.a.part + at * D + d) = make_float4(y[0], y[1], y[2], y[3]);
+    if (d == 0) p.ml[at] = bad ? make_float2(0.0f, NAN) : any ? make_float2(top, sum) : make_float2(INFINITY, 0.0f);
+  }
+}
+
+// Few query rows: WK waves over tiles of keys of their own, straight from memory into registers, one
+// tile ahead; joined at the end.
+template <int D, class TQ, class TKV, int RT, int W, int WK>
+__global__ __launch_bounds__(64 * WK, WK > 8 ? 4 : 2) void tree_attn_kernel(Args p) {
+  __shared__ typename Tree<W>::Shared tree_mem;
+  __shared__ float so[WK][16 * RT][D + 4];
+  __shared__ float sm[WK][16 * RT], sl[WK][16 * RT];
+  __shared__ int sodd[WK];
+  const TreeAttn &a = p.a;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
+  const int split = blockIdx.x, b = blockIdx.z, hk = blockIdx.y % a.Hk, row0 = blockIdx.y / a.Hk * (16 * RT);
+
+  // Everything that does not wait for something else is loaded first: this wave's first tile too,
+  // whose place does not depend on the length.
+  const char *kb = static_cast<const char *>(a.k) + (b * a.k_b + hk * a.k_h) * TKV::kBytes;
+  const char *vb = static_cast<const char *>(a.v) + (b * a.v_b + hk * a.v_h) * TKV::kBytes;
+  const uint32_t k_step = (uint32_t)a.k_r * TKV::kBytes, v_step = (uint32_t)a.v_r * TKV::kBytes;
+  const int stride = p.S * WK * kTileKeys;
+  int key0 = (split * WK + wave) * kTileKeys;
+  const int len = a.lengths[b];
+  const int par_at = W == 1 ? lane : threadIdx.x;
+  const int par = par_at < a.n ? a.parents[b * a.par_b + par_at] : -2;
+  TileRegs<D, TKV> x;
+  {
+    const int first = min(key0, a.max_seq - 1);
+    x.place(k_step, v_step, a.max_seq - 1 - first, c, g);
+    x.load_k(kb + (uint64_t)(uint32_t)first * k_step);
+    x.load_v(vb + (uint64_t)(uint32_t)first * v_step);
+  }
+  Rows<D, TQ, TKV, RT> rows;
+  rows.load(p, b, hk, row0, c, g);
+  Tree<W> tree;
+  tree.read(par, a.n, tree_mem);
+  const int live = tree.live;
+  const bool bad = len < 0 || live > a.max_seq || len > a.max_seq - live;
+  const int total = bad ? 0 : len + live;
+  typename Tree<W>::Row sees[RT];
+#pragma unroll
+  for (int t = 0; t < RT; t++) sees[t] = tree.row(rows.node[t], tree_mem);
+
+  uint32_t odd = 0;  // a node's value that is no finite number was taken out
+  for (; key0 < total; key0 += stride) {
+    floatx4 s[2][RT] = {};
+#pragma unroll
+    for (int j = 0; j < D / 32; j++) rows.scores(s, j, x.k[0][j], x.k[1][j]);
+    // the wave's next tile; past the last one every lane asks for the last row (one line), so that no
+    // register is left as it was on some path
+    const int next = min(key0 + stride, total - 1);
+    if (next + kTileKeys > total) x.place(k_step, v_step, total - 1 - next, c, g);
+    x.load_k(kb + (uint64_t)(uint32_t)next * k_step);
+    const bool edge = key0 + kTileKeys > len;  // holds nodes, or ends past the last row
+    uint32_t seen[RT] = {};
+    if (edge) {
+#pragma unroll
+      for (int t = 0; t < RT; t++) seen[t] = sees[t].tile(key0 - len) >> (4 * g);
+    }
+    rows.soften(s, edge, seen);
+    if (edge) odd |= take_odd<TKV>(x.v, key0, len, total, g);
+    rows.add(s, x.v);
     x.load_v(vb + (uint64_t)(uint32_t)next * v_step);
   }
 
-  // The waves over keys joined, each then a share of the rows' quarters: lane (c, g) holds dims D/4 g ..
-  // of column c, in runs of D/16 a register.
-  if (const bool any = __ballot(odd != 0) != 0; lane == 0) sodd[wr][wk] = any;
+  // The waves joined: lane (c, g) holds dims D/4 g .. of row c, in runs of D/16 a register.
+  if (const bool any = __ballot(odd != 0) != 0; lane == 0) sodd[wave] = any;
 #pragma unroll
   for (int t = 0; t < RT; t++) {
-    l[t] = col_sum(l[t]);
-    if (g == 0) sm[wr][wk][16 * t + c] = m[t], sl[wr][wk][16 * t + c] = l[t];
+    const float l = col_sum(rows.l[t]);
+    if (g == 0) sm[wave][16 * t + c] = rows.m[t], sl[wave][16 * t + c] = l;
 #pragma unroll
     for (int r = 0; r < 4; r++)
 #pragma unroll
       for (int d = 0; d < D / 16; d += 4)
-        *reinterpret_cast<float4 *>(&so[wr][wk][16 * t + c][D / 16 * (4 * g + r) + d]) =
-            make_float4(o[t][d][r], o[t][d + 1][r], o[t][d + 2][r], o[t][d + 3][r]);
+        *reinterpret_cast<float4 *>(&so[wave][16 * t + c][D / 16 * (4 * g + r) + d]) =
+            make_float4(rows.o[t][d][r], rows.o[t][d + 1][r], rows.o[t][d + 2][r], rows.o[t][d + 3][r]);
   }
   __syncthreads();
   int odd_any = 0;
 #pragma unroll
-  for (int w = 0; w < WK; w++) odd_any |= sodd[wr][w];
+  for (int w = 0; w < WK; w++) odd_any |= sodd[w];
   for (int i0 = 0; i0 < 16 * RT * (D / 4); i0 += 64 * WK) {
-    const int i = i0 + wk * 64 + lane;
-    const int rr = min(i / (D / 4), 16 * RT - 1), d = i % (D / 4) * 4, row = row0 + rr, i_node = min(row, M - 1) / group;
+    const int i = i0 + threadIdx.x;
+    const int rr = min(i / (D / 4), 16 * RT - 1), d = i % (D / 4) * 4, row = row0 + rr, i_node = p.node(min(row, p.M - 1));
     const auto seen = tree.row(i_node, tree_mem);
-    const bool any = seen.any();
-    if (row >= M || i >= 16 * RT * (D / 4)) continue;
+    if (row >= p.M || i >= 16 * RT * (D / 4)) continue;
     float top = -INFINITY, sum = 0.0f, y[4] = {};
 #pragma unroll
-    for (int w = 0; w < WK; w++) top = fmaxf(top, sm[wr][w][rr]);
+    for (int w = 0; w < WK; w++) top = fmaxf(top, sm[w][rr]);
     const float ms = top == -INFINITY ? 0.0f : top;
 #pragma unroll
     for (int w = 0; w < WK; w++) {
-      const float f = __builtin_amdgcn_exp2f(sm[wr][w][rr] - ms);
-      const float4 v = *reinterpret_cast<const float4 *>(&so[wr][w][rr][d]);
-      sum += f * sl[wr][w][rr];
+      const float f = __builtin_amdgcn_exp2f(sm[w][rr] - ms);
+      const float4 v = *reinterpret_cast<const float4 *>(&so[w][rr][d]);
+      sum += f * sl[w][rr];
       y[0] += f * v.x, y[1] += f * v.y, y[2] += f * v.z, y[3] += f * v.w;
     }
-    if (odd_any) {  // (a positive probability times an infinity or NaN is that)
-#pragma unroll 1
-      for (int j = 0; j < live; j++) {
-        if (!seen.sees(j)) continue;
-        const char *at = vb + (uint64_t)(uint32_t)(len + j) * v_step + d * TKV::kBytes;
+    if (odd_any) odd_values<TKV, 4>(y, seen, live, vb + (uint64_t)(uint32_t)len * v_step + d * TKV::kBytes, v_step);
+    put4<D, TQ>(p, b, hk, row, i_node, split, d, y, top, sum, bad, seen.any(), split * WK * kTileKeys < total);
+  }
+}
+
+// Many query rows over 16-bit caches: WR waves with rows of their own over the same tiles, which the
+// block copies to LDS (through registers, a tile ahead), so that a tile is read from memory once for
+// 16 RT WR rows.  A row's 16-byte pieces lie in the order p ^ row there: what 8 lanes read at a time
+// falls on different banks, keys (one piece of 8 rows) and values (8 pieces of a row) alike.
+template <int D, class TQ, class TKV, int RT, int W, int WR>
+__global__ __launch_bounds__(64 * WR, 2) void tree_attn_rows_kernel(Args p) {
+  constexpr int kPieces = D * TKV::kBytes / 16, kThreads = 64 * WR, kHalf = kTileKeys * kPieces, kCopy = 2 * kHalf / kThreads;
+  static_assert(2 * kHalf % kThreads == 0 && TKV::kBytes == 2, "whole pieces a thread");
+  __shared__ typename Tree<W>::Shared tree_mem;
+  __shared__ u32x4 tile_mem[2][2 * kHalf];  // keys, then values
+  const TreeAttn &a = p.a;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
+  const int split = blockIdx.x, b = blockIdx.z, hk = blockIdx.y % a.Hk, row0 = (blockIdx.y / a.Hk * WR + wave) * (16 * RT);
+  const char *kb = static_cast<const char *>(a.k) + (b * a.k_b + hk * a.k_h) * TKV::kBytes;
+  const char *vb = static_cast<const char *>(a.v) + (b * a.v_b + hk * a.v_h) * TKV::kBytes;
+  const uint32_t k_step = (uint32_t)a.k_r * TKV::kBytes, v_step = (uint32_t)a.v_r * TKV::kBytes;
+  const int stride = p.S * kTileKeys;
+  int key0 = split * kTileKeys;
+  const int len = a.lengths[b];
+  const int par_at = W == 1 ? lane : threadIdx.x;
+  const int par = par_at < a.n ? a.parents[b * a.par_b + par_at] : -2;
+
+  // this thread's pieces of a tile: row i / kPieces of the keys, then of the values, piece i % kPieces
+  u32x4 copy[kCopy];
+  auto fetch = [&](int first, int last) {  // rows past `last` are read as that one
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const float v = load1<TKV>(at + e * TKV::kBytes);
-          if (!(fabsf(v) < INFINITY)) y[e] += v;
-        }
+    for (int i = 0; i < kCopy; i++) {
+      const int at = i * kThreads + threadIdx.x, in = at % kHalf;
+      const uint64_t row = (uint32_t)min(first + in / kPieces, last);
+      copy[i] = *reinterpret_cast<const u32x4 *>((at < kHalf ? kb + row * k_step : vb + row * v_step) + in % kPieces * 16);
+    }
+  };
+  auto keep = [&](int buf) {
+#pragma unroll
+    for (int i = 0; i < kCopy; i++) {
+      const int at = i * kThreads + threadIdx.x, row = at / kPieces;
+      tile_mem[buf][row * kPieces + ((at ^ row) & (kPieces - 1))] = copy[i];
+    }
+  };
+  fetch(min(key0, a.max_seq - 1), a.max_seq - 1);
+  Rows<D, TQ, TKV, RT> rows;
+  rows.load(p, b, hk, row0, c, g);
+  Tree<W> tree;
+  tree.read(par, a.n, tree_mem);
+  const int live = tree.live;
+  const bool bad = len < 0 || live > a.max_seq || len > a.max_seq - live;
+  const int total = bad ? 0 : len + live;
+  typename Tree<W>::Row sees[RT];
+#pragma unroll
+  for (int t = 0; t < RT; t++) sees[t] = tree.row(rows.node[t], tree_mem);
+
+  uint32_t odd = 0;
+  const bool keys = key0 < total;
+  if (keys) {
+    keep(0);
+    fetch(min(key0 + stride, total - 1), total - 1);
+  }
+  __syncthreads();
+  for (int buf = 0; key0 < total; key0 += stride, buf ^= 1) {
+    const u32x4 *sk = tile_mem[buf], *sv = sk + kHalf;
+    // the next tile to the other buffer (all have left it), the one after it on its way
+    keep(buf ^ 1);
+    fetch(min(key0 + stride, total - 1) + min(stride, total), total - 1);
+    floatx4 s[2][RT] = {};
+#pragma unroll
+    for (int j = 0; j < D / 32; j++) {
+      uint32_t k[2][4];
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const u32x4 w = sk[(16 * h + c) * kPieces + ((4 * j + g) ^ (c & (kPieces - 1)))];
+        k[h][0] = w[0], k[h][1] = w[1], k[h][2] = w[2], k[h][3] = w[3];
+      }
+      rows.scores(s, j, k[0], k[1]);
+    }
+    const bool edge = key0 + kTileKeys > len;
+    uint32_t seen[RT] = {};
+    if (edge) {
+#pragma unroll
+      for (int t = 0; t < RT; t++) seen[t] = sees[t].tile(key0 - len) >> (4 * g);
+    }
+    rows.soften(s, edge, seen);
+    uint32_t v[8][Rows<D, TQ, TKV, RT>::kV];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const int row = 16 * (i >> 2) + 4 * g + (i & 3);
+      if constexpr (D == 128) {
+        const u32x4 w = sv[row * kPieces + (c ^ (row & (kPieces - 1)))];
+        v[i][0] = w[0], v[i][1] = w[1], v[i][2] = w[2], v[i][3] = w[3];
+      } else {
+        const u32x2 w = reinterpret_cast<const u32x2 *>(&sv[row * kPieces + ((c >> 1) ^ (row & (kPieces - 1)))])[c & 1];
+        v[i][0] = w[0], v[i][1] = w[1];
       }
     }
-    if (S == 1) {
-      const float inv = 1.0f / sum;
+    if (edge) odd |= take_odd<TKV>(v, key0, len, total, g);
+    rows.add(s, v);
+    __syncthreads();
+  }
+
+  const bool odd_any = __ballot(odd != 0) != 0;
 #pragma unroll
-      for (int e = 0; e < 4; e++) y[e] = bad ? NAN : any ? y[e] * inv : 0.0f;
-      const int64_t at = b * a.o_b + i_node * a.o_n + (hk * group + row % group) * a.o_h + d;
-      store4<TQ>(static_cast<char *>(a.out) + at * TQ::kBytes, y[0], y[1], y[2], y[3]);
-    } else {
-      // what the joining kernel cannot tell by itself goes with the statistics: a row that sees
-      // nothing has maximum +inf and sum 0, one of a bad sequence sum NaN
-      const size_t at = part_row(a, S, b, hk, row) + split;
-      if (split * WK * kTileKeys < total) *reinterpret_cast<float4 *>(a.part + at * D + d) = make_float4(y[0], y[1], y[2], y[3]);
-      if (d == 0) ml[at] = bad ? make_float2(0.0f, NAN) : any ? make_float2(top, sum) : make_float2(INFINITY, 0.0f);
-    }
+  for (int t = 0; t < RT; t++) {
+    const int row = row0 + 16 * t + c;
+    const float sum = col_sum(rows.l[t]);
+    if (row >= p.M) continue;
+#pragma unroll
+    for (int r = 0; r < 4; r++)
+#pragma unroll
+      for (int d = 0; d < D / 16; d += 4) {
+        float y[4] = {rows.o[t][d][r], rows.o[t][d + 1][r], rows.o[t][d + 2][r], rows.o[t][d + 3][r]};
+        const int e = D / 16 * (4 * g + r) + d;
+        if (odd_any) odd_values<TKV, 4>(y, sees[t], live, vb + (uint64_t)(uint32_t)len * v_step + e * TKV::kBytes, v_step);
+        put4<D, TQ>(p, b, hk, row, rows.node[t], split, e, y, rows.m[t], sum, bad, sees[t].any(), keys);
+      }
   }
 }
 
 // Joins the splits of a row, D / 4 lanes a row with four elements each, in split order.
 template <int D, class TQ>
-__global__ __launch_bounds__(256) void tree_join_kernel(TreeAttn a, int S, const float2 *ml) {
+__global__ __launch_bounds__(256) void tree_join_kernel(Args p) {
   constexpr int kLanes = D / 4;
-  const int lane = threadIdx.x % kLanes, group = a.H / a.Hk, M = a.n * group;
+  const TreeAttn &a = p.a;
+  const int lane = threadIdx.x % kLanes, M = p.M, S = p.S;
   const int64_t item = (int64_t)blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
   if (item >= (int64_t)a.batch * a.Hk * M) return;
   const int row = item % M, hk = item / M % a.Hk, b = item / M / a.Hk;
-  const float2 *w = ml + (size_t)item * S;
+  const float2 *w = p.ml + (size_t)item * S;
   const float *part = a.part + (size_t)item * S * D + 4 * lane;
   float top = -INFINITY;
   for (int s = 0; s < S; s++) top = fmaxf(top, w[s].x);
@@ -591,17 +751,20 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeAttn a, int S, const
     const float f = fmaxf(__builtin_amdgcn_exp2f(v.x - ms), 0x1p-126f);  // (0 times an infinity: NaN)
     sum += f * v.y;
     if (v.y != v.y) continue;
-    const float4 p = *reinterpret_cast<const float4 *>(part + (size_t)s * D);
-    x[0] += f * p.x, x[1] += f * p.y, x[2] += f * p.z, x[3] += f * p.w;
+    const float4 o = *reinterpret_cast<const float4 *>(part + (size_t)s * D);
+    x[0] += f * o.x, x[1] += f * o.y, x[2] += f * o.z, x[3] += f * o.w;
   }
   const float inv = none ? 0.0f : 1.0f / sum;
-  const int64_t to = b * a.o_b + row / group * a.o_n + (hk * group + row % group) * a.o_h + 4 * lane;
+  const int node = p.node(row);
+  const int64_t to = b * a.o_b + node * a.o_n + (hk * p.group + (row - node * p.group)) * a.o_h + 4 * lane;
   store4<TQ>(static_cast<char *>(a.out) + to * TQ::kBytes, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
 }
 
 // Most tiles of 16 query rows a wave takes: as many as its registers hold (256 a lane, two waves a
 // SIMD).  fp32 queries take up to three times the registers of 16-bit ones.
 constexpr int most_tiles(int D, int q_bytes) { return (q_bytes == 4 ? 128 : 256) / D; }
+// The same where the waves share tiles, and hold none themselves.
+constexpr int rows_tiles(int D, int q_bytes) { return D == 128 && q_bytes == 4 ? 1 : 2; }
 // Waves over keys of a large block: RT 1 at D 64 fits 128 registers, the others 256.
 constexpr int large_waves(int D, int RT, int kv_bytes) { return D == 64 && RT == 1 && kv_bytes == 2 ? 16 : 8; }
 
@@ -611,41 +774,60 @@ struct Plan {
 Plan make_plan(const TreeAttn &a, int n_cu) {
   Plan p;
   const int M = a.n * (a.H / a.Hk), most = most_tiles(a.D, a.qt == kOpF32 ? 4 : 2);
-  p.RT = a.n > 64 ? most : std::min(most, M <= 16 ? 1 : M <= 32 ? 2 : 4);
   const int tiles = (a.max_seq + kTileKeys - 1) / kTileKeys;
-  p.WR = a.qt != kOpF32 && M > 2 * 16 * p.RT ? 4 : 1;
-  p.row_tiles = (M + 16 * p.RT * p.WR - 1) / (16 * p.RT * p.WR);
+  p.WR = a.kvt == kOpF32 || M <= 64 ? 0 : M <= 128 ? 4 : 8;
+  if (p.WR > 0) {
+    p.RT = rows_tiles(a.D, a.qt == kOpF32 ? 4 : 2);
+    p.WK = 1;
+    p.row_tiles = (M + 16 * p.RT * p.WR - 1) / (16 * p.RT * p.WR);
+  } else {
+    p.RT = a.n > 64 ? most : std::min(most, M <= 16 ? 1 : M <= 32 ? 2 : 4);
+    p.row_tiles = (M + 16 * p.RT - 1) / (16 * p.RT);
+    const int64_t blocks = (int64_t)a.batch * a.Hk * p.row_tiles;
+    p.WK = a.n > 64 || blocks >= 2 * n_cu ? 4 : large_waves(a.D, p.RT, a.kvt == kOpF32 ? 4 : 2);
+  }
   const int64_t blocks = (int64_t)a.batch * a.Hk * p.row_tiles;
-  p.WK = p.WR > 1 ? 1 : blocks >= 2 * n_cu ? 4 : large_waves(a.D, p.RT, a.kvt == kOpF32 ? 4 : 2);
-  if (a.n > 64 && p.WR == 1) p.WK = 4;
-  const int64_t want = (8 * n_cu / (p.WK * p.WR) + blocks - 1) / blocks, can = (tiles + 4 * p.WK - 1) / (4 * p.WK);
+  const int64_t want = (8 * n_cu / (p.WK * std::max(1, p.WR)) + blocks - 1) / blocks, can = (tiles + 4 * p.WK - 1) / (4 * p.WK);
   p.S = (int)std::max<int64_t>(1, std::min<int64_t>({want, can, 64}));
   return p;
 }
 
-template <int D, class TQ, class TKV, int RT, int W, int WK, int WR>
-hipError_t launch_rt(const TreeAttn &a, const Plan &p, hipStream_t s) {
-  float2 *ml = reinterpret_cast<float2 *>(a.part + (size_t)a.batch * a.H * a.n * p.S * D);
-  hipLaunchKernelGGL((tree_attn_kernel<D, TQ, TKV, RT, W, WK, WR>), dim3(p.S, a.Hk * p.row_tiles, a.batch),
-                     dim3(64 * WK * WR), 0, s, a, p.S, ml);
+Args make_args(const TreeAttn &a, const Plan &p) {
+  const int group = a.H / a.Hk;
+  return Args{a, p.S, a.n * group, group, (uint32_t)(((1ull << 32) + group - 1) / group),
+              reinterpret_cast<float2 *>(a.part + (size_t)a.batch * a.H * a.n * p.S * a.D)};
+}
+template <int D, class TQ, class K>
+hipError_t launch_kernel(K kernel, int threads, const TreeAttn &a, const Plan &p, hipStream_t s) {
+  const Args args = make_args(a, p);
+  hipLaunchKernelGGL(kernel, dim3(p.S, a.Hk * p.row_tiles, a.batch), dim3(threads), 0, s, args);
   if (hipError_t e = hipGetLastError(); e != hipSuccess || p.S == 1) return e;
   const int64_t rows = (int64_t)a.batch * a.H * a.n;
   constexpr int kRows = 256 / (D / 4);
-  hipLaunchKernelGGL((tree_join_kernel<D, TQ>), dim3((unsigned)((rows + kRows - 1) / kRows)), dim3(256), 0, s, a, p.S, ml);
+  hipLaunchKernelGGL((tree_join_kernel<D, TQ>), dim3((unsigned)((rows + kRows - 1) / kRows)), dim3(256), 0, s, args);
   return hipGetLastError();
 }
 template <int D, class TQ, class TKV, int RT>
 hipError_t launch_keys(const TreeAttn &a, const Plan &p, hipStream_t s) {
-  if (p.WK == 4) return launch_rt<D, TQ, TKV, RT, 1, 4, 1>(a, p, s);
-  return launch_rt<D, TQ, TKV, RT, 1, large_waves(D, RT, TKV::kBytes), 1>(a, p, s);
+  constexpr int kLarge = large_waves(D, RT, TKV::kBytes);
+  if (p.WK == 4) return launch_kernel<D, TQ>(tree_attn_kernel<D, TQ, TKV, RT, 1, 4>, 256, a, p, s);
+  return launch_kernel<D, TQ>(tree_attn_kernel<D, TQ, TKV, RT, 1, kLarge>, 64 * kLarge, a, p, s);
+}
+template <int D, class TQ, class TKV, int WR>
+hipError_t launch_rows(const TreeAttn &a, const Plan &p, hipStream_t s) {
+  constexpr int kRT = rows_tiles(D, TQ::kBytes);
+  if (a.n > 64) return launch_kernel<D, TQ>(tree_attn_rows_kernel<D, TQ, TKV, kRT, 4, WR>, 64 * WR, a, p, s);
+  return launch_kernel<D, TQ>(tree_attn_rows_kernel<D, TQ, TKV, kRT, 1, WR>, 64 * WR, a, p, s);
 }
 template <int D, class TQ, class TKV>
 hipError_t launch_d(const TreeAttn &a, const Plan &p, hipStream_t s) {
   constexpr int kMost = most_tiles(D, TQ::kBytes);
-  if constexpr (TQ::kBytes == 2)
-    if (p.WR == 4)
-      return a.n > 64 ? launch_rt<D, TQ, TKV, kMost, 4, 1, 4>(a, p, s) : launch_rt<D, TQ, TKV, kMost, 1, 1, 4>(a, p, s);
-  if (a.n > 64) return launch_rt<D, TQ, TKV, kMost, 4, 4, 1>(a, p, s);
+  if constexpr (TKV::kBytes == 2) {
+    if (p.WR == 8) return launch_rows<D, TQ, TKV, 8>(a, p, s);
+    if (p.WR == 4) return launch_rows<D, TQ, TKV, 4>(a, p, s);
+  } else {
+    if (a.n > 64) return launch_kernel<D, TQ>(tree_attn_kernel<D, TQ, TKV, kMost, 4, 4>, 256, a, p, s);
+  }
   if constexpr (kMost >= 4)
     if (p.RT == 4) return launch_keys<D, TQ, TKV, 4>(a, p, s);
   if constexpr (kMost >= 2)
