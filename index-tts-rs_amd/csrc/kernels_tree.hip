@@ -159,7 +159,7 @@ struct Tree<1> {
     const int i = threadIdx.x & 63;
     int up = i < n && par >= -1 && par < i ? par : -2;  // -1: the root is reached; -2: not in the tree
     anc = up != -2 ? 1ull << i : 0;
-    for (int s = 1; s < n; s *= 2) {
+    while (__ballot(up >= 0)) {
       const int at = max(up, 0);
       const uint64_t a = __shfl((unsigned long long)anc, at, 64);
       const int u = __shfl(up, at, 64);
@@ -244,12 +244,13 @@ struct Tree<4> {
   __device__ Row row(int node, const Shared &t) const { return Row{t.anc[node]}; }
 };
 
-// A launch: the split over keys (S blocks of a sequence, key head and row tile), their results (o
-// [batch][Hk][M][S][D], then (max, sum) [batch][Hk][M][S]), and the query rows of a key head, row
+// A launch: the split over keys (S blocks of a sequence, key head and row tile, with `chunk` rows each:
+// a sequence that is shorter than max_seq has fewer of them at work, of the same size), their results
+// (o [batch][Hk][M][S][D], then (max, sum) [batch][Hk][M][S]), and the query rows of a key head, row
 // r being head r % group of node r / group.
 struct Args {
   TreeAttn a;
-  int S, M, group;
+  int S, chunk, M, group;
   uint32_t group_mul;  // 2^32 / group, rounded up: exact for rows < 2^32 / group
   float2 *ml;
   __device__ int node(int row) const { return group == 1 ? row : __umulhi((uint32_t)row, group_mul); }
@@ -327,7 +328,7 @@ struct Rows {
     }
     const float by = a.scale * kLog2e;
     const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0;
-    scale = kWide || NQ == 3 ? 1.0f : fabsf(by);
+    scale = kWide || NQ == 3 ? 1.0f : fmaxf(fabsf(by), 0x1p-120f);  // (0 times the mask's -inf would be NaN)
 #pragma unroll
     for (int t = 0; t < RT; t++)
 #pragma unroll
@@ -372,9 +373,9 @@ struct Rows {
     }
   }
 
-  // Scores to probabilities, sums and (where a maximum moves) results rescaled.  At an edge bit
+  // The running maxima for a tile's scores, and what was summed rescaled where one moves.  At an edge bit
   // 16 h + r of seen[t] says whether key 16 h + 4 g + r counts.
-  __device__ __forceinline__ void soften(floatx4 (&s)[2][RT], bool edge, const uint32_t (&seen)[RT]) {
+  __device__ __forceinline__ void limit(floatx4 (&s)[2][RT], bool edge, const uint32_t (&seen)[RT]) {
     if (edge) {
 #pragma unroll
       for (int t = 0; t < RT; t++)
@@ -386,8 +387,10 @@ struct Rows {
     bool grows = false;
 #pragma unroll
     for (int t = 0; t < RT; t++) {
-      top[t] = fmaxf(fmaxf(fmaxf(s[0][t][0], s[0][t][1]), fmaxf(s[0][t][2], s[0][t][3])),
-                     fmaxf(fmaxf(s[1][t][0], s[1][t][1]), fmaxf(s[1][t][2], s[1][t][3]))) * scale;
+      top[t] = s[0][t][0];
+#pragma unroll
+      for (int i = 1; i < 7; i += 2) top[t] = fmaxf(fmaxf(s[i >> 2][t][i & 3], s[i + 1 >> 2][t][i + 1 & 3]), top[t]);
+      top[t] = fmaxf(s[1][t][3], top[t]) * scale;
       grows = grows || top[t] > m[t] + kLag;
     }
     if (__ballot(grows)) {
@@ -401,54 +404,65 @@ struct Rows {
         for (int d = 0; d < D / 16; d++) o[t][d] *= f;
       }
     }
+  }
+
+  // Scores to probabilities, and their sums.
+  __device__ __forceinline__ void weigh(floatx4 (&s)[2][RT]) {
 #pragma unroll
     for (int t = 0; t < RT; t++) {
       const float ms = (m[t] == -INFINITY ? 0.0f : m[t]) - kUp;
 #pragma unroll
       for (int i = 0; i < 8; i++) {
-        float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 2][t][i & 3], scale, -ms));
-        // (a scale of 0 makes NaN of the mask's -inf)
-        if (edge) p = seen[t] & 1u << (16 * (i >> 2) + (i & 3)) ? p : 0.0f;
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 2][t][i & 3], scale, -ms));
         s[i >> 2][t][i & 3] = p;
         l[t] += p;
       }
     }
   }
 
-  // o += P V; v[i]: elements D / 16 c .. of key 16 (i / 4) + 4 g + i % 4
-  __device__ __forceinline__ void add(const floatx4 (&s)[2][RT], const uint32_t (&v)[8][kV]) {
-    if constexpr (kWide) {
+  // Probabilities as the second product's operand: 16-bit planes of a lane's 8 keys.
+  struct Probs {
+    uint32_t p[kWide ? 1 : RT][NP][4];
+  };
+  __device__ __forceinline__ void pack(const floatx4 (&s)[2][RT], Probs &x) const {
+    if constexpr (!kWide) {
 #pragma unroll
-      for (int i = 0; i < 8; i++)
-#pragma unroll
-        for (int t = 0; t < RT; t++)
-#pragma unroll
-          for (int d = 0; d < D / 16; d++)
-            o[t][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v[i][d]), s[i >> 2][t][i & 3], o[t][d], 0, 0, 0);
-    } else {
-      // operands of 8 keys a lane: V^T by element pairs from its 8 rows, P as it stands
-      uint32_t vt[D / 16][4];
-#pragma unroll
-      for (int d = 0; d < D / 16; d++)
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-          vt[d][i] = __builtin_amdgcn_perm(v[2 * i + 1][d / 2], v[2 * i][d / 2], d % 2 ? 0x07060302u : 0x05040100u);
-#pragma unroll
-      for (int t = 0; t < RT; t++) {
-        uint32_t p[NP][4];
+      for (int t = 0; t < RT; t++)
 #pragma unroll
         for (int i = 0; i < 4; i++) {
           uint32_t w[NP];
           cut2_pos<TKV, NP>(s[i >> 1][t][2 * (i & 1)], s[i >> 1][t][2 * (i & 1) + 1], w);
 #pragma unroll
-          for (int k = 0; k < NP; k++) p[k][i] = w[k];
+          for (int k = 0; k < NP; k++) x.p[t][k][i] = w[k];
         }
-#pragma unroll
-        for (int k = NP - 1; k >= 0; k--)
-#pragma unroll
-          for (int d = 0; d < D / 16; d++) o[t][d] = mfma16<TKV>(vt[d], p[k], o[t][d]);
-      }
     }
+  }
+
+  // o += P V for N elements from D / 16 c + d0 on; v[i]: those of key 16 (i / 4) + 4 g + i % 4.  A lane's
+  // operand of V^T takes element pairs from its 8 rows.
+  template <int N>
+  __device__ __forceinline__ void add(const Probs &x, int d0, const uint32_t (&v)[8][N / 2]) {
+    uint32_t vt[N][4];
+#pragma unroll
+    for (int d = 0; d < N; d++)
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        vt[d][i] = __builtin_amdgcn_perm(v[2 * i + 1][d / 2], v[2 * i][d / 2], d % 2 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+    for (int t = 0; t < RT; t++)
+#pragma unroll
+      for (int k = NP - 1; k >= 0; k--)
+#pragma unroll
+        for (int d = 0; d < N; d++) o[t][d0 + d] = mfma16<TKV>(vt[d], x.p[t][k], o[t][d0 + d]);
+  }
+  __device__ __forceinline__ void add_wide(const floatx4 (&s)[2][RT], const uint32_t (&v)[8][kV]) {
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+#pragma unroll
+      for (int t = 0; t < RT; t++)
+#pragma unroll
+        for (int d = 0; d < D / 16; d++)
+          o[t][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v[i][d]), s[i >> 2][t][i & 3], o[t][d], 0, 0, 0);
   }
 };
 
@@ -530,8 +544,8 @@ __global__ __launch_bounds__(64 * WK, WK > 8 ? 4 : 2) void tree_attn_kernel(Args
   const char *kb = static_cast<const char *>(a.k) + (b * a.k_b + hk * a.k_h) * TKV::kBytes;
   const char *vb = static_cast<const char *>(a.v) + (b * a.v_b + hk * a.v_h) * TKV::kBytes;
   const uint32_t k_step = (uint32_t)a.k_r * TKV::kBytes, v_step = (uint32_t)a.v_r * TKV::kBytes;
-  const int stride = p.S * WK * kTileKeys;
-  int key0 = (split * WK + wave) * kTileKeys;
+  constexpr int stride = WK * kTileKeys;
+  int key0 = split * p.chunk + wave * kTileKeys;
   const int len = a.lengths[b];
   const int par_at = W == 1 ? lane : threadIdx.x;
   const int par = par_at < a.n ? a.parents[b * a.par_b + par_at] : -2;
@@ -548,19 +562,19 @@ __global__ __launch_bounds__(64 * WK, WK > 8 ? 4 : 2) void tree_attn_kernel(Args
   tree.read(par, a.n, tree_mem);
   const int live = tree.live;
   const bool bad = len < 0 || live > a.max_seq || len > a.max_seq - live;
-  const int total = bad ? 0 : len + live;
+  const int total = bad ? 0 : len + live, end = min(total, (split + 1) * p.chunk);
   typename Tree<W>::Row sees[RT];
 #pragma unroll
   for (int t = 0; t < RT; t++) sees[t] = tree.row(rows.node[t], tree_mem);
 
   uint32_t odd = 0;  // a node's value that is no finite number was taken out
-  for (; key0 < total; key0 += stride) {
+  for (; key0 < end; key0 += stride) {
     floatx4 s[2][RT] = {};
 #pragma unroll
     for (int j = 0; j < D / 32; j++) rows.scores(s, j, x.k[0][j], x.k[1][j]);
     // the wave's next tile; past the last one every lane asks for the last row (one line), so that no
     // register is left as it was on some path
-    const int next = min(key0 + stride, total - 1);
+    const int next = key0 + stride < end ? key0 + stride : total - 1;
     if (next + kTileKeys > total) x.place(k_step, v_step, total - 1 - next, c, g);
     x.load_k(kb + (uint64_t)(uint32_t)next * k_step);
     const bool edge = key0 + kTileKeys > len;  // holds nodes, or ends past the last row
@@ -569,9 +583,16 @@ __global__ __launch_bounds__(64 * WK, WK > 8 ? 4 : 2) void tree_attn_kernel(Args
 #pragma unroll
       for (int t = 0; t < RT; t++) seen[t] = sees[t].tile(key0 - len) >> (4 * g);
     }
-    rows.soften(s, edge, seen);
+    rows.limit(s, edge, seen);
+    rows.weigh(s);
     if (edge) odd |= take_odd<TKV>(x.v, key0, len, total, g);
-    rows.add(s, x.v);
+    if constexpr (TKV::kBytes == 4) {
+      rows.add_wide(s, x.v);
+    } else {
+      typename Rows<D, TQ, TKV, RT>::Probs probs;
+      rows.pack(s, probs);
+      rows.template add<D / 16>(probs, 0, x.v);
+    }
     x.load_v(vb + (uint64_t)(uint32_t)next * v_step);
   }
 
@@ -609,107 +630,154 @@ __global__ __launch_bounds__(64 * WK, WK > 8 ? 4 : 2) void tree_attn_kernel(Args
       y[0] += f * v.x, y[1] += f * v.y, y[2] += f * v.z, y[3] += f * v.w;
     }
     if (odd_any) odd_values<TKV, 4>(y, seen, live, vb + (uint64_t)(uint32_t)len * v_step + d * TKV::kBytes, v_step);
-    put4<D, TQ>(p, b, hk, row, i_node, split, d, y, top, sum, bad, seen.any(), split * WK * kTileKeys < total);
+    put4<D, TQ>(p, b, hk, row, i_node, split, d, y, top, sum, bad, seen.any(), split * p.chunk < total);
   }
 }
 
 // Many query rows over 16-bit caches: WR waves with rows of their own over the same tiles, which the
-// block copies to LDS (through registers, a tile ahead), so that a tile is read from memory once for
-// 16 RT WR rows.  A row's 16-byte pieces lie in the order p ^ row there: what 8 lanes read at a time
-// falls on different banks, keys (one piece of 8 rows) and values (8 pieces of a row) alike.
+// block copies to LDS (through registers), so that a tile is read from memory once for 16 RT WR
+// rows.  A tile's scores are formed a tile ahead, so that their products run under the exponentials
+// of the one before: keys lie a tile further than values.  In LDS what a wave reads at a time falls
+// on different banks: one piece of 16 key rows (a row's pieces lie in the order p ^ row), and four
+// value rows' pieces of 8 bytes (every second group of four rows lies with its halves, D 64: its
+// rows, in the other order).
 template <int D, class TQ, class TKV, int RT, int W, int WR>
 __global__ __launch_bounds__(64 * WR, 2) void tree_attn_rows_kernel(Args p) {
-  constexpr int kPieces = D * TKV::kBytes / 16, kThreads = 64 * WR, kHalf = kTileKeys * kPieces, kCopy = 2 * kHalf / kThreads;
-  static_assert(2 * kHalf % kThreads == 0 && TKV::kBytes == 2, "whole pieces a thread");
+  constexpr int kPieces = D * TKV::kBytes / 16, kThreads = 64 * WR, kTile = kTileKeys * kPieces, kCopy = 2 * kTile / kThreads;
+  static_assert(2 * kTile % kThreads == 0 && TKV::kBytes == 2, "whole pieces a thread");
   __shared__ typename Tree<W>::Shared tree_mem;
-  __shared__ u32x4 tile_mem[2][2 * kHalf];  // keys, then values
+  __shared__ u32x4 key_mem[2][kTile], value_mem[2][kTile];
+  auto value_at = [](int row, int piece) {  // 8-byte piece of a value row
+    const int turn = row >> 2 & 1;
+    return D == 128 ? row * 32 + (((piece ^ turn) & 1) << 4) + (piece >> 1) : (row ^ turn) * 16 + piece;
+  };
   const TreeAttn &a = p.a;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
   const int split = blockIdx.x, b = blockIdx.z, hk = blockIdx.y % a.Hk, row0 = (blockIdx.y / a.Hk * WR + wave) * (16 * RT);
   const char *kb = static_cast<const char *>(a.k) + (b * a.k_b + hk * a.k_h) * TKV::kBytes;
   const char *vb = static_cast<const char *>(a.v) + (b * a.v_b + hk * a.v_h) * TKV::kBytes;
   const uint32_t k_step = (uint32_t)a.k_r * TKV::kBytes, v_step = (uint32_t)a.v_r * TKV::kBytes;
-  const int stride = p.S * kTileKeys;
-  int key0 = split * kTileKeys;
+  int key0 = split * p.chunk;
   const int len = a.lengths[b];
   const int par_at = W == 1 ? lane : threadIdx.x;
   const int par = par_at < a.n ? a.parents[b * a.par_b + par_at] : -2;
 
-  // this thread's pieces of a tile: row i / kPieces of the keys, then of the values, piece i % kPieces
-  u32x4 copy[kCopy];
-  auto fetch = [&](int first, int last) {  // rows past `last` are read as that one
+  // A thread's pieces of two tiles: row i / kPieces of the first, then of the second, piece i % kPieces.
+  // Rows past `last` are read as that one.
+  auto fetch = [&](u32x4 (&copy)[kCopy], int key, const char *other, uint32_t other_step, int other_key, int last) {
 #pragma unroll
     for (int i = 0; i < kCopy; i++) {
-      const int at = i * kThreads + threadIdx.x, in = at % kHalf;
-      const uint64_t row = (uint32_t)min(first + in / kPieces, last);
-      copy[i] = *reinterpret_cast<const u32x4 *>((at < kHalf ? kb + row * k_step : vb + row * v_step) + in % kPieces * 16);
+      const int at = i * kThreads + threadIdx.x, in = at % kTile;
+      const char *row = at < kTile ? kb + (uint64_t)(uint32_t)min(key + in / kPieces, last) * k_step
+                                   : other + (uint64_t)(uint32_t)min(other_key + in / kPieces, last) * other_step;
+      copy[i] = *reinterpret_cast<const u32x4 *>(row + in % kPieces * 16);
     }
   };
-  auto keep = [&](int buf) {
+  auto keep_key = [&](u32x4 *mem, int in, const u32x4 &piece) {
+    const int row = in / kPieces;
+    mem[row * kPieces + ((in ^ row) & (kPieces - 1))] = piece;
+  };
+  auto keep = [&](const u32x4 (&copy)[kCopy], u32x4 *keys, u32x4 *values) {
 #pragma unroll
     for (int i = 0; i < kCopy; i++) {
-      const int at = i * kThreads + threadIdx.x, row = at / kPieces;
-      tile_mem[buf][row * kPieces + ((at ^ row) & (kPieces - 1))] = copy[i];
+      const int at = i * kThreads + threadIdx.x, in = at % kTile, row = in / kPieces, piece = in % kPieces;
+      if (at < kTile) {
+        keep_key(keys, in, copy[i]);
+      } else {
+        u32x2 *mem = reinterpret_cast<u32x2 *>(values);
+        mem[value_at(row, 2 * piece)] = u32x2{copy[i][0], copy[i][1]};
+        mem[value_at(row, 2 * piece + 1)] = u32x2{copy[i][2], copy[i][3]};
+      }
     }
   };
-  fetch(min(key0, a.max_seq - 1), a.max_seq - 1);
+  // Everything that does not wait for something else is loaded first: the keys of tiles 0 and 1, then
+  // those of tile 2 and the values of tile 0, wherever the length ends.
+  u32x4 copy0[kCopy], copy[kCopy];
+  const int last_row = a.max_seq - 1;
+  fetch(copy0, min(key0, last_row), kb, k_step, min(key0 + kTileKeys, last_row), last_row);
+  fetch(copy, min(key0 + 2 * kTileKeys, last_row), vb, v_step, min(key0, last_row), last_row);
   Rows<D, TQ, TKV, RT> rows;
   rows.load(p, b, hk, row0, c, g);
   Tree<W> tree;
   tree.read(par, a.n, tree_mem);
   const int live = tree.live;
   const bool bad = len < 0 || live > a.max_seq || len > a.max_seq - live;
-  const int total = bad ? 0 : len + live;
+  const int total = bad ? 0 : len + live, end = min(total, (split + 1) * p.chunk);
   typename Tree<W>::Row sees[RT];
 #pragma unroll
   for (int t = 0; t < RT; t++) sees[t] = tree.row(rows.node[t], tree_mem);
 
   uint32_t odd = 0;
   const bool keys = key0 < total;
-  if (keys) {
-    keep(0);
-    fetch(min(key0 + stride, total - 1), total - 1);
-  }
-  __syncthreads();
-  for (int buf = 0; key0 < total; key0 += stride, buf ^= 1) {
-    const u32x4 *sk = tile_mem[buf], *sv = sk + kHalf;
-    // the next tile to the other buffer (all have left it), the one after it on its way
-    keep(buf ^ 1);
-    fetch(min(key0 + stride, total - 1) + min(stride, total), total - 1);
-    floatx4 s[2][RT] = {};
+  auto next = [&](int tiles) {  // (past the last tile: one row, once more)
+    const int key = key0 + tiles * kTileKeys;
+    return key < end ? key : total - 1;
+  };
+  auto scores = [&](floatx4 (&s)[2][RT], int buf) {
 #pragma unroll
     for (int j = 0; j < D / 32; j++) {
       uint32_t k[2][4];
 #pragma unroll
       for (int h = 0; h < 2; h++) {
-        const u32x4 w = sk[(16 * h + c) * kPieces + ((4 * j + g) ^ (c & (kPieces - 1)))];
+        const u32x4 w = key_mem[buf][(16 * h + c) * kPieces + ((4 * j + g) ^ (c & (kPieces - 1)))];
         k[h][0] = w[0], k[h][1] = w[1], k[h][2] = w[2], k[h][3] = w[3];
       }
       rows.scores(s, j, k[0], k[1]);
     }
-    const bool edge = key0 + kTileKeys > len;
+  };
+  floatx4 s[2][RT] = {};
+  if (keys) {
+#pragma unroll
+    for (int i = 0; i < kCopy; i++) {
+      const int at = i * kThreads + threadIdx.x;
+      keep_key(key_mem[at / kTile], at % kTile, copy0[i]);
+    }
+    __syncthreads();
+    scores(s, 0);
+    __syncthreads();
+    keep(copy, key_mem[0], value_mem[0]);
+    fetch(copy, next(2), vb, v_step, next(1), total - 1);
+    __syncthreads();
+  }
+  int buf = 0;
+  auto step = [&](auto is_edge) {
+    constexpr bool kEdge = decltype(is_edge)::value;
+    // here: this tile's scores and values (buf), the next one's keys (buf ^ 1); to LDS: the keys after
+    // those, the next values; on their way: what follows
+    keep(copy, key_mem[buf], value_mem[buf ^ 1]);
+    fetch(copy, next(3), vb, v_step, next(2), total - 1);
     uint32_t seen[RT] = {};
-    if (edge) {
+    if constexpr (kEdge) {
 #pragma unroll
       for (int t = 0; t < RT; t++) seen[t] = sees[t].tile(key0 - len) >> (4 * g);
     }
-    rows.soften(s, edge, seen);
-    uint32_t v[8][Rows<D, TQ, TKV, RT>::kV];
+    rows.limit(s, kEdge, seen);
+    floatx4 s_next[2][RT] = {};
+    scores(s_next, buf ^ 1);
+    rows.weigh(s);
+    typename Rows<D, TQ, TKV, RT>::Probs probs;
+    rows.pack(s, probs);
+    const u32x2 *sv = reinterpret_cast<const u32x2 *>(value_mem[buf]);
+    // values four elements at a time (8 bytes a row): half the registers of D 128's eight
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-      const int row = 16 * (i >> 2) + 4 * g + (i & 3);
-      if constexpr (D == 128) {
-        const u32x4 w = sv[row * kPieces + (c ^ (row & (kPieces - 1)))];
-        v[i][0] = w[0], v[i][1] = w[1], v[i][2] = w[2], v[i][3] = w[3];
-      } else {
-        const u32x2 w = reinterpret_cast<const u32x2 *>(&sv[row * kPieces + ((c >> 1) ^ (row & (kPieces - 1)))])[c & 1];
+    for (int d0 = 0; d0 < D / 16; d0 += 4) {
+      uint32_t v[8][2];
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const u32x2 w = sv[value_at(16 * (i >> 2) + 4 * g + (i & 3), D / 64 * c + d0 / 4)];
         v[i][0] = w[0], v[i][1] = w[1];
       }
+      if constexpr (kEdge) odd |= take_odd<TKV>(v, key0, len, total, g);
+      rows.template add<4>(probs, d0, v);
     }
-    if (edge) odd |= take_odd<TKV>(v, key0, len, total, g);
-    rows.add(s, v);
+#pragma unroll
+    for (int t = 0; t < RT; t++) s[0][t] = s_next[0][t], s[1][t] = s_next[1][t];
+    key0 += kTileKeys;
+    buf ^= 1;
     __syncthreads();
-  }
+  };
+  while (key0 + kTileKeys <= min(end, len)) step(std::false_type{});
+  while (key0 < end) step(std::true_type{});  // tiles with nodes, or past the last row
 
   const bool odd_any = __ballot(odd != 0) != 0;
 #pragma unroll
@@ -729,35 +797,47 @@ __global__ __launch_bounds__(64 * WR, 2) void tree_attn_rows_kernel(Args p) {
   }
 }
 
-// Joins the splits of a row, D / 4 lanes a row with four elements each, in split order.
+// Joins the splits of a row: a wave a row, D / 4 lanes with four elements each for every fourth (D 128:
+// second) split, added in split order there and then over the lane groups.
 template <int D, class TQ>
 __global__ __launch_bounds__(256) void tree_join_kernel(Args p) {
-  constexpr int kLanes = D / 4;
+  constexpr int kLanes = D / 4, kGroups = 64 / kLanes;
   const TreeAttn &a = p.a;
-  const int lane = threadIdx.x % kLanes, M = p.M, S = p.S;
-  const int64_t item = (int64_t)blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
+  const int lane = threadIdx.x & 63, d = lane % kLanes * 4, s0 = lane / kLanes, M = p.M, S = p.S;
+  const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (item >= (int64_t)a.batch * a.Hk * M) return;
   const int row = item % M, hk = item / M % a.Hk, b = item / M / a.Hk;
   const float2 *w = p.ml + (size_t)item * S;
-  const float *part = a.part + (size_t)item * S * D + 4 * lane;
-  float top = -INFINITY;
-  for (int s = 0; s < S; s++) top = fmaxf(top, w[s].x);
-  const bool none = w[0].x == INFINITY && w[0].y == 0.0f;
-  const float ms = top == -INFINITY ? 0.0f : top;
+  const float *part = a.part + (size_t)item * S * D + d;
+  const float2 own = w[min(lane, S - 1)];  // (at most 64 splits)
+  const float top = wave_max(own.x), ms = top == -INFINITY ? 0.0f : top;
+  const bool none = __ballot(own.x == INFINITY && own.y == 0.0f) != 0;
+  // (at least 2^-126: 0 times an infinity would be NaN)
+  const float f_own = fmaxf(__builtin_amdgcn_exp2f(own.x - ms), 0x1p-126f);
   float sum = 0.0f, x[4] = {};
-  for (int s = 0; s < S; s++) {
-    const float2 v = w[s];
-    if ((v.x == -INFINITY && v.y == 0.0f) || none) continue;  // no keys: nothing was stored
-    const float f = fmaxf(__builtin_amdgcn_exp2f(v.x - ms), 0x1p-126f);  // (0 times an infinity: NaN)
-    sum += f * v.y;
-    if (v.y != v.y) continue;
+#pragma unroll 4
+  for (int s1 = 0; s1 < S; s1 += kGroups) {
+    const int s = min(s1 + s0, S - 1);
+    const float m = __shfl(own.x, s, 64), l = __shfl(own.y, s, 64), f = __shfl(f_own, s, 64);
     const float4 o = *reinterpret_cast<const float4 *>(part + (size_t)s * D);
-    x[0] += f * o.x, x[1] += f * o.y, x[2] += f * o.z, x[3] += f * o.w;
+    const bool in = s1 + s0 < S && !(m == -INFINITY && l == 0.0f);  // without keys nothing was stored
+    const bool num = in && l == l;
+    sum += in ? f * l : 0.0f;
+    x[0] += num ? f * o.x : 0.0f, x[1] += num ? f * o.y : 0.0f, x[2] += num ? f * o.z : 0.0f, x[3] += num ? f * o.w : 0.0f;
   }
-  const float inv = none ? 0.0f : 1.0f / sum;
+#pragma unroll
+  for (int step = kLanes; step < 64; step *= 2) {
+    sum += __shfl_xor(sum, step, 64);
+#pragma unroll
+    for (int e = 0; e < 4; e++) x[e] += __shfl_xor(x[e], step, 64);
+  }
+  if (s0 > 0) return;
+  const float inv = 1.0f / sum;
+#pragma unroll
+  for (int e = 0; e < 4; e++) x[e] = none ? 0.0f : x[e] * inv;
   const int node = p.node(row);
-  const int64_t to = b * a.o_b + node * a.o_n + (hk * p.group + (row - node * p.group)) * a.o_h + 4 * lane;
-  store4<TQ>(static_cast<char *>(a.out) + to * TQ::kBytes, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+  const int64_t to = b * a.o_b + node * a.o_n + (hk * p.group + (row - node * p.group)) * a.o_h + d;
+  store4<TQ>(static_cast<char *>(a.out) + to * TQ::kBytes, x[0], x[1], x[2], x[3]);
 }
 
 // Most tiles of 16 query rows a wave takes: as many as its registers hold (256 a lane, two waves a
@@ -769,7 +849,7 @@ constexpr int rows_tiles(int D, int q_bytes) { return D == 128 && q_bytes == 4 ?
 constexpr int large_waves(int D, int RT, int kv_bytes) { return D == 64 && RT == 1 && kv_bytes == 2 ? 16 : 8; }
 
 struct Plan {
-  int S, RT, WK, WR, row_tiles;
+  int S, chunk, RT, WK, WR, row_tiles;
 };
 Plan make_plan(const TreeAttn &a, int n_cu) {
   Plan p;
@@ -782,19 +862,22 @@ Plan make_plan(const TreeAttn &a, int n_cu) {
     p.row_tiles = (M + 16 * p.RT * p.WR - 1) / (16 * p.RT * p.WR);
   } else {
     p.RT = a.n > 64 ? most : std::min(most, M <= 16 ? 1 : M <= 32 ? 2 : 4);
+    if (a.kvt == kOpF32 && M > 32 && M <= 48) p.RT = 1;  // (the fp32 products bound it: no empty fourth tile)
     p.row_tiles = (M + 16 * p.RT - 1) / (16 * p.RT);
     const int64_t blocks = (int64_t)a.batch * a.Hk * p.row_tiles;
     p.WK = a.n > 64 || blocks >= 2 * n_cu ? 4 : large_waves(a.D, p.RT, a.kvt == kOpF32 ? 4 : 2);
   }
   const int64_t blocks = (int64_t)a.batch * a.Hk * p.row_tiles;
   const int64_t want = (8 * n_cu / (p.WK * std::max(1, p.WR)) + blocks - 1) / blocks, can = (tiles + 4 * p.WK - 1) / (4 * p.WK);
-  p.S = (int)std::max<int64_t>(1, std::min<int64_t>({want, can, 64}));
+  const int S = (int)std::max<int64_t>(1, std::min<int64_t>({want, can, 64}));
+  p.chunk = ((tiles + S - 1) / S + p.WK - 1) / p.WK * p.WK * kTileKeys;
+  p.S = (a.max_seq + p.chunk - 1) / p.chunk;
   return p;
 }
 
 Args make_args(const TreeAttn &a, const Plan &p) {
   const int group = a.H / a.Hk;
-  return Args{a, p.S, a.n * group, group, (uint32_t)(((1ull << 32) + group - 1) / group),
+  return Args{a, p.S, p.chunk, a.n * group, group, (uint32_t)(((1ull << 32) + group - 1) / group),
               reinterpret_cast<float2 *>(a.part + (size_t)a.batch * a.H * a.n * p.S * a.D)};
 }
 template <int D, class TQ, class K>
@@ -803,8 +886,7 @@ hipError_t launch_kernel(K kernel, int threads, const TreeAttn &a, const Plan &p
   hipLaunchKernelGGL(kernel, dim3(p.S, a.Hk * p.row_tiles, a.batch), dim3(threads), 0, s, args);
   if (hipError_t e = hipGetLastError(); e != hipSuccess || p.S == 1) return e;
   const int64_t rows = (int64_t)a.batch * a.H * a.n;
-  constexpr int kRows = 256 / (D / 4);
-  hipLaunchKernelGGL((tree_join_kernel<D, TQ>), dim3((unsigned)((rows + kRows - 1) / kRows)), dim3(256), 0, s, args);
+  hipLaunchKernelGGL((tree_join_kernel<D, TQ>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, args);
   return hipGetLastError();
 }
 template <int D, class TQ, class TKV, int RT>
