@@ -135,6 +135,12 @@ __device__ __forceinline__ void cut2_pos(float a, float b, uint32_t (&o)[N]) {
 }
 
 template <class T>
+__device__ __forceinline__ uint32_t round2(float a, float b) {
+  if constexpr (std::is_same_v<T, Bf16>) return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2e){a, b}, bf16x2v));
+  else return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2e){a, b}, f16x2v));
+}
+
+template <class T>
 __device__ __forceinline__ floatx4 mfma16(const uint32_t *a, const uint32_t *b, floatx4 c) {
   const u32x4 x = {a[0], a[1], a[2], a[3]}, y = {b[0], b[1], b[2], b[3]};
   if constexpr (std::is_same_v<T, Bf16>)
@@ -293,14 +299,23 @@ struct TileRegs {
   }
 };
 
+// Planes of 16 bits that hold a probability.  Few query rows wait for memory, not for products: two
+// (16 bits of bf16, 22 of fp16) leave no more than the result's own rounding.  Many rows over 16-bit
+// queries wait for instructions: one, rounded (half a step of the result's type, and the same
+// rounded values in the sums), 12 x 64 nodes of 4 heads over 8,191 rows 144 -> 114 us.  fp32 queries: three,
+// an fp32's bits.
+template <class TQ>
+constexpr int prob_planes(bool many) {
+  return TQ::kBytes == 4 ? 3 : many ? 1 : 2;
+}
+
 // What a wave holds of RT tiles of 16 query rows (lane (c, g): row c of each), and the three steps of
 // a tile of keys.  16-bit caches go through the 16-bit matrix instructions: queries in NQ planes (fp32
-// ones in three, exactly), probabilities in NP (two hold 16 bits of bf16 and 22 of fp16, far below
-// the result's rounding; three an fp32's).  fp32 caches take the fp32 ones.
-template <int D, class TQ, class TKV, int RT>
+// ones in three, exactly), probabilities in NP (see prob_planes).  fp32 caches take the fp32 ones.
+template <int D, class TQ, class TKV, int RT, bool MANY>
 struct Rows {
   static constexpr bool kWide = TKV::kBytes == 4;
-  static constexpr int NQ = kWide || TQ::kBytes == 2 ? 1 : 3, NP = TQ::kBytes == 2 ? 2 : 3;
+  static constexpr int NQ = kWide || TQ::kBytes == 2 ? 1 : 3, NP = prob_planes<TQ>(MANY);
   static constexpr int kV = D / 16 * TKV::kBytes / 4;
   // probabilities are held up to 2^(kLag + kUp): the running maximum moves only when a score passes
   // it by 2^kLag; fp16 planes use their range below 1 too
@@ -309,7 +324,9 @@ struct Rows {
   int node[RT];
   float scale;  // what a score is still multiplied by, for powers of two
   floatx4 o[RT][D / 16];
-  float m[RT], l[RT];
+  float m[RT];
+  // the probabilities' sums: over this lane's keys, or (MANY) over all keys, by products with ones
+  typename std::conditional<MANY, floatx4, float>::type l[RT];
 
   __device__ __forceinline__ void load(const Args &p, int b, int hk, int row0, int c, int g) {
     uint32_t raw[RT][D / 32][8 * TQ::kBytes / 4];
@@ -322,7 +339,7 @@ struct Rows {
       const char *at = static_cast<const char *>(a.q) + (b * a.q_b + node[t] * a.q_n + head * a.q_h + 8 * g) * TQ::kBytes;
 #pragma unroll
       for (int j = 0; j < D / 32; j++) load_dwords<8 * TQ::kBytes / 4>(at + 32 * j * TQ::kBytes, raw[t][j]);
-      m[t] = -INFINITY, l[t] = 0.0f;
+      m[t] = -INFINITY, l[t] = {};
 #pragma unroll
       for (int d = 0; d < D / 16; d++) o[t][d] = floatx4{};
     }
@@ -415,7 +432,7 @@ struct Rows {
       for (int i = 0; i < 8; i++) {
         const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 2][t][i & 3], scale, -ms));
         s[i >> 2][t][i & 3] = p;
-        l[t] += p;
+        if constexpr (!MANY) l[t] += p;
       }
     }
   }
@@ -430,30 +447,44 @@ struct Rows {
       for (int t = 0; t < RT; t++)
 #pragma unroll
         for (int i = 0; i < 4; i++) {
+          const float a = s[i >> 1][t][2 * (i & 1)], b = s[i >> 1][t][2 * (i & 1) + 1];
           uint32_t w[NP];
-          cut2_pos<TKV, NP>(s[i >> 1][t][2 * (i & 1)], s[i >> 1][t][2 * (i & 1) + 1], w);
+          if constexpr (NP == 1) w[0] = round2<TKV>(a, b);
+          else cut2_pos<TKV, NP>(a, b, w);
 #pragma unroll
           for (int k = 0; k < NP; k++) x.p[t][k][i] = w[k];
         }
     }
   }
 
-  // o += P V for N elements from D / 16 c + d0 on; v[i]: those of key 16 (i / 4) + 4 g + i % 4.  A lane's
-  // operand of V^T takes element pairs from its 8 rows.
+  __device__ __forceinline__ void add_sums(const Probs &x) {
+    constexpr uint32_t kOne = std::is_same_v<TKV, Bf16> ? 0x3f803f80u : 0x3c003c00u;
+    const uint32_t ones[4] = {kOne, kOne, kOne, kOne};
+#pragma unroll
+    for (int t = 0; t < RT; t++)
+#pragma unroll
+      for (int k = NP - 1; k >= 0; k--) l[t] = mfma16<TKV>(ones, x.p[t][k], l[t]);
+  }
+  // o[.][d0 ..] += P V; vt[d]: the operand of V^T whose row c is element (d0 + d, c) of keys 4 g + r, then
+  // of keys 16 + 4 g + r.
   template <int N>
-  __device__ __forceinline__ void add(const Probs &x, int d0, const uint32_t (&v)[8][N / 2]) {
-    uint32_t vt[N][4];
-#pragma unroll
-    for (int d = 0; d < N; d++)
-#pragma unroll
-      for (int i = 0; i < 4; i++)
-        vt[d][i] = __builtin_amdgcn_perm(v[2 * i + 1][d / 2], v[2 * i][d / 2], d % 2 ? 0x07060302u : 0x05040100u);
+  __device__ __forceinline__ void add(const Probs &x, int d0, const uint32_t (&vt)[N][4]) {
 #pragma unroll
     for (int t = 0; t < RT; t++)
 #pragma unroll
       for (int k = NP - 1; k >= 0; k--)
 #pragma unroll
         for (int d = 0; d < N; d++) o[t][d0 + d] = mfma16<TKV>(vt[d], x.p[t][k], o[t][d0 + d]);
+  }
+  // The same from rows: v[i], elements D / 16 c .. of key 16 (i / 4) + 4 g + i % 4, in pairs of rows.
+  __device__ __forceinline__ void add_rows(const Probs &x, const uint32_t (&v)[8][kV]) {
+    uint32_t vt[D / 16][4];
+#pragma unroll
+    for (int d = 0; d < D / 16; d++)
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        vt[d][i] = __builtin_amdgcn_perm(v[2 * i + 1][d / 2], v[2 * i][d / 2], d % 2 ? 0x07060302u : 0x05040100u);
+    add(x, 0, vt);
   }
   __device__ __forceinline__ void add_wide(const floatx4 (&s)[2][RT], const uint32_t (&v)[8][kV]) {
 #pragma unroll
@@ -492,6 +523,33 @@ __device__ __forceinline__ uint32_t take_odd(uint32_t (&v)[8][N], int key0, int 
     }
   }
   return odd;
+}
+// The same where keys 4 g + 2 i, 4 g + 2 i + 1 (i < 2; then 16 more) share dword i.
+template <class T, int N>
+__device__ __forceinline__ uint32_t take_odd_columns(uint32_t (&v)[N][4], int key0, int len, int total, int g) {
+  uint32_t odd = 0;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const int key = key0 + 16 * (i >> 1) + 4 * g + 2 * (i & 1);
+    const uint32_t own = (key < len ? 0xffffu : 0) | (key + 1 < len ? 0xffff0000u : 0);
+    const uint32_t in = (key < total ? 0xffffu : 0) | (key + 1 < total ? 0xffff0000u : 0);
+#pragma unroll
+    for (int d = 0; d < N; d++) {
+      const uint32_t w = v[d][i];
+      uint32_t keep = (w & T::kOddBits) == T::kOddBits ? 0xffff0000u : ~0u;
+      keep = (w & T::kOddBits << 16) == T::kOddBits << 16 ? keep & 0xffffu : keep;
+      keep |= own;
+      odd |= ~keep & in;
+      v[d][i] = w & keep & in;
+    }
+  }
+  return odd;
+}
+// A 16-byte piece's half through LDS's transposing load (gfx950), over groups of 16 lanes.
+__device__ __forceinline__ u32x2 load_transposed(u32x4 *piece, int half) {
+  typedef short s16x4 __attribute__((ext_vector_type(4)));
+  using Lds = __attribute__((address_space(3))) s16x4;
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds *)(reinterpret_cast<s16x4 *>(piece) + half)));
 }
 // y[0 .. N) += such values of the nodes that a row sees (a positive probability times an infinity or
 // NaN is that); at: element y[0]'s place in node 0's row.
@@ -556,7 +614,8 @@ __global__ __launch_bounds__(64 * WK, WK > 8 ? 4 : 2) void tree_attn_kernel(Args
     x.load_k(kb + (uint64_t)(uint32_t)first * k_step);
     x.load_v(vb + (uint64_t)(uint32_t)first * v_step);
   }
-  Rows<D, TQ, TKV, RT> rows;
+  using Wave = Rows<D, TQ, TKV, RT, false>;
+  Wave rows;
   rows.load(p, b, hk, row0, c, g);
   Tree<W> tree;
   tree.read(par, a.n, tree_mem);
@@ -589,9 +648,9 @@ __global__ __launch_bounds__(64 * WK, WK > 8 ? 4 : 2) void tree_attn_kernel(Args
     if constexpr (TKV::kBytes == 4) {
       rows.add_wide(s, x.v);
     } else {
-      typename Rows<D, TQ, TKV, RT>::Probs probs;
+      typename Wave::Probs probs;
       rows.pack(s, probs);
-      rows.template add<D / 16>(probs, 0, x.v);
+      rows.add_rows(probs, x.v);
     }
     x.load_v(vb + (uint64_t)(uint32_t)next * v_step);
   }
@@ -637,20 +696,16 @@ __global__ __launch_bounds__(64 * WK, WK > 8 ? 4 : 2) void tree_attn_kernel(Args
 // Many query rows over 16-bit caches: WR waves with rows of their own over the same tiles, which the
 // block copies to LDS (through registers), so that a tile is read from memory once for 16 RT WR
 // rows.  A tile's scores are formed a tile ahead, so that their products run under the exponentials
-// of the one before: keys lie a tile further than values.  In LDS what a wave reads at a time falls
-// on different banks: one piece of 16 key rows (a row's pieces lie in the order p ^ row), and four
-// value rows' pieces of 8 bytes (every second group of four rows lies with its halves, D 64: its
-// rows, in the other order).
+// of the one before: keys lie a tile further than values.  In LDS a row's 16-byte pieces lie in the
+// order p ^ row: what a wave reads at a time, one piece of 16 key rows or two neighbours of 16 value
+// rows, falls on different banks.  Values are read through the transposing load: lane 4 j + a of 16
+// reads elements 4 a .. of row j, and lane i gets element i of the four rows.
 template <int D, class TQ, class TKV, int RT, int W, int WR>
 __global__ __launch_bounds__(64 * WR, 2) void tree_attn_rows_kernel(Args p) {
   constexpr int kPieces = D * TKV::kBytes / 16, kThreads = 64 * WR, kTile = kTileKeys * kPieces, kCopy = 2 * kTile / kThreads;
   static_assert(2 * kTile % kThreads == 0 && TKV::kBytes == 2, "whole pieces a thread");
   __shared__ typename Tree<W>::Shared tree_mem;
   __shared__ u32x4 key_mem[2][kTile], value_mem[2][kTile];
-  auto value_at = [](int row, int piece) {  // 8-byte piece of a value row
-    const int turn = row >> 2 & 1;
-    return D == 128 ? row * 32 + (((piece ^ turn) & 1) << 4) + (piece >> 1) : (row ^ turn) * 16 + piece;
-  };
   const TreeAttn &a = p.a;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
   const int split = blockIdx.x, b = blockIdx.z, hk = blockIdx.y % a.Hk, row0 = (blockIdx.y / a.Hk * WR + wave) * (16 * RT);
@@ -673,21 +728,11 @@ __global__ __launch_bounds__(64 * WR, 2) void tree_attn_rows_kernel(Args p) {
       copy[i] = *reinterpret_cast<const u32x4 *>(row + in % kPieces * 16);
     }
   };
-  auto keep_key = [&](u32x4 *mem, int in, const u32x4 &piece) {
-    const int row = in / kPieces;
-    mem[row * kPieces + ((in ^ row) & (kPieces - 1))] = piece;
-  };
-  auto keep = [&](const u32x4 (&copy)[kCopy], u32x4 *keys, u32x4 *values) {
+  auto keep = [&](const u32x4 (&copy)[kCopy], u32x4 *first, u32x4 *second) {
 #pragma unroll
     for (int i = 0; i < kCopy; i++) {
-      const int at = i * kThreads + threadIdx.x, in = at % kTile, row = in / kPieces, piece = in % kPieces;
-      if (at < kTile) {
-        keep_key(keys, in, copy[i]);
-      } else {
-        u32x2 *mem = reinterpret_cast<u32x2 *>(values);
-        mem[value_at(row, 2 * piece)] = u32x2{copy[i][0], copy[i][1]};
-        mem[value_at(row, 2 * piece + 1)] = u32x2{copy[i][2], copy[i][3]};
-      }
+      const int at = i * kThreads + threadIdx.x, in = at % kTile, row = in / kPieces;
+      (at < kTile ? first : second)[row * kPieces + ((in ^ row) & (kPieces - 1))] = copy[i];
     }
   };
   // Everything that does not wait for something else is loaded first: the keys of tiles 0 and 1, then
@@ -696,7 +741,8 @@ __global__ __launch_bounds__(64 * WR, 2) void tree_attn_rows_kernel(Args p) {
   const int last_row = a.max_seq - 1;
   fetch(copy0, min(key0, last_row), kb, k_step, min(key0 + kTileKeys, last_row), last_row);
   fetch(copy, min(key0 + 2 * kTileKeys, last_row), vb, v_step, min(key0, last_row), last_row);
-  Rows<D, TQ, TKV, RT> rows;
+  using Wave = Rows<D, TQ, TKV, RT, true>;
+  Wave rows;
   rows.load(p, b, hk, row0, c, g);
   Tree<W> tree;
   tree.read(par, a.n, tree_mem);
@@ -727,11 +773,7 @@ __global__ __launch_bounds__(64 * WR, 2) void tree_attn_rows_kernel(Args p) {
   };
   floatx4 s[2][RT] = {};
   if (keys) {
-#pragma unroll
-    for (int i = 0; i < kCopy; i++) {
-      const int at = i * kThreads + threadIdx.x;
-      keep_key(key_mem[at / kTile], at % kTile, copy0[i]);
-    }
+    keep(copy0, key_mem[0], key_mem[1]);
     __syncthreads();
     scores(s, 0);
     __syncthreads();
@@ -755,20 +797,22 @@ __global__ __launch_bounds__(64 * WR, 2) void tree_attn_rows_kernel(Args p) {
     floatx4 s_next[2][RT] = {};
     scores(s_next, buf ^ 1);
     rows.weigh(s);
-    typename Rows<D, TQ, TKV, RT>::Probs probs;
+    typename Wave::Probs probs;
     rows.pack(s, probs);
-    const u32x2 *sv = reinterpret_cast<const u32x2 *>(value_mem[buf]);
-    // values four elements at a time (8 bytes a row): half the registers of D 128's eight
+    rows.add_sums(probs);
 #pragma unroll
-    for (int d0 = 0; d0 < D / 16; d0 += 4) {
-      uint32_t v[8][2];
+    for (int d0 = 0; d0 < D / 16; d0 += 4) {  // (four at a time: fewer registers)
+      uint32_t vt[4][4];
 #pragma unroll
-      for (int i = 0; i < 8; i++) {
-        const u32x2 w = sv[value_at(16 * (i >> 2) + 4 * g + (i & 3), D / 64 * c + d0 / 4)];
-        v[i][0] = w[0], v[i][1] = w[1];
-      }
-      if constexpr (kEdge) odd |= take_odd<TKV>(v, key0, len, total, g);
-      rows.template add<4>(probs, d0, v);
+      for (int d = 0; d < 4; d++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          const int row = 16 * h + 4 * g + (c >> 2), piece = 2 * (d0 + d) + (c >> 1 & 1);
+          const u32x2 w = load_transposed(&value_mem[buf][row * kPieces + (piece ^ (row & (kPieces - 1)))], c & 1);
+          vt[d][2 * h] = w[0], vt[d][2 * h + 1] = w[1];
+        }
+      if constexpr (kEdge) odd |= take_odd_columns<TKV>(vt, key0, len, total, g);
+      rows.add(probs, d0, vt);
     }
 #pragma unroll
     for (int t = 0; t < RT; t++) s[0][t] = s_next[0][t], s[1][t] = s_next[1][t];
@@ -783,17 +827,14 @@ __global__ __launch_bounds__(64 * WR, 2) void tree_attn_rows_kernel(Args p) {
 #pragma unroll
   for (int t = 0; t < RT; t++) {
     const int row = row0 + 16 * t + c;
-    const float sum = col_sum(rows.l[t]);
     if (row >= p.M) continue;
 #pragma unroll
-    for (int r = 0; r < 4; r++)
-#pragma unroll
-      for (int d = 0; d < D / 16; d += 4) {
-        float y[4] = {rows.o[t][d][r], rows.o[t][d + 1][r], rows.o[t][d + 2][r], rows.o[t][d + 3][r]};
-        const int e = D / 16 * (4 * g + r) + d;
-        if (odd_any) odd_values<TKV, 4>(y, sees[t], live, vb + (uint64_t)(uint32_t)len * v_step + e * TKV::kBytes, v_step);
-        put4<D, TQ>(p, b, hk, row, rows.node[t], split, e, y, rows.m[t], sum, bad, sees[t].any(), keys);
-      }
+    for (int d = 0; d < D / 16; d++) {  // lane (c, g) holds dims 16 d + 4 g .. of row c
+      float y[4] = {rows.o[t][d][0], rows.o[t][d][1], rows.o[t][d][2], rows.o[t][d][3]};
+      const int e = 16 * d + 4 * g;
+      if (odd_any) odd_values<TKV, 4>(y, sees[t], live, vb + (uint64_t)(uint32_t)len * v_step + e * TKV::kBytes, v_step);
+      put4<D, TQ>(p, b, hk, row, rows.node[t], split, e, y, rows.m[t], rows.l[t][0], bad, sees[t].any(), keys);
+    }
   }
 }
 
