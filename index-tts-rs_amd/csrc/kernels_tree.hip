@@ -10,6 +10,7 @@
 // Softmax statistics stay in the lanes (max over the four lane groups of a column by two
 // exchanges, sums only at the end).
 #include <algorithm>
+#include <numeric>
 #include <type_traits>
 
 #include "frag.h"
@@ -19,6 +20,7 @@ namespace itts {
 namespace {
 
 constexpr int kTileKeys = 32;  // keys a wave takes at a time
+constexpr int kKeyWaves = 4;   // waves of a block that share a few rows' keys
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct F32 {
@@ -250,20 +252,74 @@ struct Tree<4> {
   __device__ Row row(int node, const Shared &t) const { return Row{t.anc[node]}; }
 };
 
-// A launch: the split over keys (S blocks of a sequence, key head and row tile, with `chunk` rows each:
-// a sequence that is shorter than max_seq has fewer of them at work, of the same size), their results
-// (o [batch][Hk][M][S][D], then (max, sum) [batch][Hk][M][S]), and the query rows of a key head, row
-// r being head r % group of node r / group.
+// A launch: the query rows of a key head (row r being head r % group of node r / group), and what
+// shares the keys: one block a sequence, key head and row tile (parts 0), or `parts` blocks for all
+// sequences of a key head and row tile, with results of their own (o [Hk][M][parts][D], then (max,
+// sum) [Hk][M][parts], then (first block, blocks) [batch]) that a second kernel joins.
 struct Args {
   TreeAttn a;
-  int S, chunk, M, group;
+  int parts, M, group;
   uint32_t group_mul;  // 2^32 / group, rounded up: exact for rows < 2^32 / group
+  int unit, least;     // a block's rows are at least `least` times 2^unit
   float2 *ml;
+  int2 *dealt;
   __device__ int node(int row) const { return group == 1 ? row : __umulhi((uint32_t)row, group_mul); }
-  __device__ size_t part(int b, int hk, int row, int split) const {
-    return (((size_t)b * a.Hk + hk) * M + row) * S + split;
-  }
 };
+
+// What block `index` of `parts` has to do: rows [first, end) of sequence b, whose rows are shared by
+// n blocks (0: nothing is left for this one).  Every block gets the same number of rows, whatever
+// the sequences' lengths and however long the cache could become: the smallest one with which `parts`
+// blocks are enough.  Every wave finds it by itself from the lengths, a lane a sequence; 12 lengths
+// from 1,000 to 8,191, 8 key heads: 115 us with the rows
+// of max_seq shared equally, xx us with these.
+struct Share {
+  int b, n, first, end, index, from;
+};
+__device__ __forceinline__ Share share_of(const Args &p) {
+  const TreeAttn &a = p.a;
+  const int index = blockIdx.x, lane = threadIdx.x & 63;
+  if (p.parts == 0) return Share{index, 1, 0, a.max_seq, 0, 0};
+  auto units = [&](int b) -> uint32_t {
+    if (b >= a.batch) return 0;
+    const int len = a.lengths[b];
+    return len < 0 || len > a.max_seq ? 1 : (uint32_t)(min(len + a.n, a.max_seq) - 1 >> p.unit) + 1;
+  };
+  float total = 0.0f, longest = 0.0f;
+  for (int b = lane; b < a.batch + lane; b += 64) {
+    const float u = units(b);
+    total += u, longest = fmaxf(longest, u);
+  }
+  total = wave_sum(total), longest = wave_max(longest);
+  // (64 blocks of a sequence at most: the joining kernel's lanes)
+  uint32_t size = (uint32_t)fmaxf(ceilf(fmaxf(total / p.parts, longest / 64)), (float)p.least);
+  for (int i = 0; i < 16; i++) {
+    float blocks = 0.0f;
+    for (int b = lane; b < a.batch + lane; b += 64) blocks += (units(b) + size - 1) / size;
+    blocks = wave_sum(blocks);
+    if (blocks <= p.parts) break;
+    size = i < 14 ? max(size + 1, (uint32_t)ceilf(size * (blocks / p.parts))) : (uint32_t)longest + 1;  // (parts >= batch)
+  }
+  size = __builtin_amdgcn_readfirstlane(size);
+  Share share{0, 0, 0, 0, index, 0};
+  int before = 0;
+  for (int b0 = 0; b0 < a.batch && share.n == 0; b0 += 64) {
+    const int own = (units(b0 + lane) + size - 1) / size;
+    int to = own;
+#pragma unroll
+    for (int step = 1; step < 64; step *= 2) {
+      const int up = __shfl_up(to, step, 64);
+      if (lane >= step) to += up;
+    }
+    if (const uint64_t at = __ballot(index >= before + to - own && index < before + to); at != 0) {
+      const int src = __builtin_ctzll(at);
+      share.b = b0 + src, share.n = __builtin_amdgcn_readlane(own, src);
+      share.from = before + __builtin_amdgcn_readlane(to, src) - share.n;
+    }
+    before += __builtin_amdgcn_readlane(to, 63);
+  }
+  share.first = (int)((uint32_t)(index - share.from) * size << p.unit), share.end = share.first + (int)(size << p.unit);
+  return share;
+}
 
 // A wave's keys and values of one tile: key rows 16 h + c, in runs of 8 elements 32 j + 8 g, and value
 // rows 16 h + 4 g + r, elements D / 16 c ...  Rows lie at the same offsets from every tile's first row
@@ -570,16 +626,16 @@ __device__ inline void odd_values(float *y, const Seen &seen, int live, const ch
 // What the joining kernel cannot tell by itself goes with the statistics: a row that sees nothing
 // has maximum +inf and sum 0, one of a bad sequence sum NaN.
 template <int D, class TQ>
-__device__ __forceinline__ void put4(const Args &p, int b, int hk, int row, int node, int split, int d, float *y, float top,
+__device__ __forceinline__ void put4(const Args &p, const Share &share, int hk, int row, int node, int d, float *y, float top,
                                      float sum, bool bad, bool any, bool keys) {
-  if (p.S == 1) {
+  if (share.n == 1) {
     const float inv = 1.0f / sum;
 #pragma unroll
     for (int e = 0; e < 4; e++) y[e] = bad ? NAN : any ? y[e] * inv : 0.0f;
-    const int64_t at = b * p.a.o_b + node * p.a.o_n + (hk * p.group + (row - node * p.group)) * p.a.o_h + d;
+    const int64_t at = share.b * p.a.o_b + node * p.a.o_n + (hk * p.group + (row - node * p.group)) * p.a.o_h + d;
     store4<TQ>(static_cast<char *>(p.a.out) + at * TQ::kBytes, y[0], y[1], y[2], y[3]);
   } else {
-    const size_t at = p.part(b, hk, row, split);
+    const size_t at = ((size_t)hk * p.M + row) * p.parts + share.index;
     if (keys) *reinterpret_cast<float4 *>(p.a.part + at * D + d) = make_float4(y[0], y[1], y[2], y[3]);
     if (d == 0) p.ml[at] = bad ? make_float2(0.0f, NAN) : any ? make_float2(top, sum) : make_float2(INFINITY, 0.0f);
   }
@@ -587,23 +643,28 @@ __device__ __forceinline__ void put4(const Args &p, int b, int hk, int row, int 
 
 // Few query rows: WK waves over tiles of keys of their own, straight from memory into registers, one
 // tile ahead; joined at the end.
-template <int D, class TQ, class TKV, int RT, int W, int WK>
-__global__ __launch_bounds__(64 * WK, WK > 8 ? 4 : 2) void tree_attn_kernel(Args p) {
+template <int D, class TQ, class TKV, int RT, int W>
+__global__ __launch_bounds__(256, 2) void tree_attn_kernel(Args p) {
+  constexpr int WK = kKeyWaves;
   __shared__ typename Tree<W>::Shared tree_mem;
   __shared__ float so[WK][16 * RT][D + 4];
   __shared__ float sm[WK][16 * RT], sl[WK][16 * RT];
   __shared__ int sodd[WK];
   const TreeAttn &a = p.a;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
-  const int split = blockIdx.x, b = blockIdx.z, hk = blockIdx.y % a.Hk, row0 = blockIdx.y / a.Hk * (16 * RT);
+  const int hk = blockIdx.y % a.Hk, row0 = blockIdx.y / a.Hk * (16 * RT);
+  const Share share = share_of(p);
+  if (share.n == 0) return;
+  const int b = share.b;
+  if (p.parts > 0 && share.first == 0 && blockIdx.y == 0 && threadIdx.x == 0) p.dealt[b] = make_int2(share.from, share.n);
 
   // Everything that does not wait for something else is loaded first: this wave's first tile too,
-  // whose place does not depend on the length.
+  // wherever the length ends.
   const char *kb = static_cast<const char *>(a.k) + (b * a.k_b + hk * a.k_h) * TKV::kBytes;
   const char *vb = static_cast<const char *>(a.v) + (b * a.v_b + hk * a.v_h) * TKV::kBytes;
   const uint32_t k_step = (uint32_t)a.k_r * TKV::kBytes, v_step = (uint32_t)a.v_r * TKV::kBytes;
   constexpr int stride = WK * kTileKeys;
-  int key0 = split * p.chunk + wave * kTileKeys;
+  int key0 = share.first + wave * kTileKeys;
   const int len = a.lengths[b];
   const int par_at = W == 1 ? lane : threadIdx.x;
   const int par = par_at < a.n ? a.parents[b * a.par_b + par_at] : -2;
@@ -621,7 +682,7 @@ __global__ __launch_bounds__(64 * WK, WK > 8 ? 4 : 2) void tree_attn_kernel(Args
   tree.read(par, a.n, tree_mem);
   const int live = tree.live;
   const bool bad = len < 0 || live > a.max_seq || len > a.max_seq - live;
-  const int total = bad ? 0 : len + live, end = min(total, (split + 1) * p.chunk);
+  const int total = bad ? 0 : len + live, end = min(total, share.end);
   typename Tree<W>::Row sees[RT];
 #pragma unroll
   for (int t = 0; t < RT; t++) sees[t] = tree.row(rows.node[t], tree_mem);
@@ -689,7 +750,7 @@ __global__ __launch_bounds__(64 * WK, WK > 8 ? 4 : 2) void tree_attn_kernel(Args
       y[0] += f * v.x, y[1] += f * v.y, y[2] += f * v.z, y[3] += f * v.w;
     }
     if (odd_any) odd_values<TKV, 4>(y, seen, live, vb + (uint64_t)(uint32_t)len * v_step + d * TKV::kBytes, v_step);
-    put4<D, TQ>(p, b, hk, row, i_node, split, d, y, top, sum, bad, seen.any(), split * p.chunk < total);
+    put4<D, TQ>(p, share, hk, row, i_node, d, y, top, sum, bad, seen.any(), share.first < total);
   }
 }
 
@@ -708,11 +769,15 @@ __global__ __launch_bounds__(64 * WR, 2) void tree_attn_rows_kernel(Args p) {
   __shared__ u32x4 key_mem[2][kTile], value_mem[2][kTile];
   const TreeAttn &a = p.a;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
-  const int split = blockIdx.x, b = blockIdx.z, hk = blockIdx.y % a.Hk, row0 = (blockIdx.y / a.Hk * WR + wave) * (16 * RT);
+  const int hk = blockIdx.y % a.Hk, row0 = (blockIdx.y / a.Hk * WR + wave) * (16 * RT);
+  const Share share = share_of(p);
+  if (share.n == 0) return;
+  const int b = share.b;
+  if (p.parts > 0 && share.first == 0 && blockIdx.y == 0 && threadIdx.x == 0) p.dealt[b] = make_int2(share.from, share.n);
   const char *kb = static_cast<const char *>(a.k) + (b * a.k_b + hk * a.k_h) * TKV::kBytes;
   const char *vb = static_cast<const char *>(a.v) + (b * a.v_b + hk * a.v_h) * TKV::kBytes;
   const uint32_t k_step = (uint32_t)a.k_r * TKV::kBytes, v_step = (uint32_t)a.v_r * TKV::kBytes;
-  int key0 = split * p.chunk;
+  int key0 = share.first;
   const int len = a.lengths[b];
   const int par_at = W == 1 ? lane : threadIdx.x;
   const int par = par_at < a.n ? a.parents[b * a.par_b + par_at] : -2;
@@ -748,7 +813,7 @@ __global__ __launch_bounds__(64 * WR, 2) void tree_attn_rows_kernel(Args p) {
   tree.read(par, a.n, tree_mem);
   const int live = tree.live;
   const bool bad = len < 0 || live > a.max_seq || len > a.max_seq - live;
-  const int total = bad ? 0 : len + live, end = min(total, (split + 1) * p.chunk);
+  const int total = bad ? 0 : len + live, end = min(total, share.end);
   typename Tree<W>::Row sees[RT];
 #pragma unroll
   for (int t = 0; t < RT; t++) sees[t] = tree.row(rows.node[t], tree_mem);
@@ -833,24 +898,28 @@ __global__ __launch_bounds__(64 * WR, 2) void tree_attn_rows_kernel(Args p) {
       float y[4] = {rows.o[t][d][0], rows.o[t][d][1], rows.o[t][d][2], rows.o[t][d][3]};
       const int e = 16 * d + 4 * g;
       if (odd_any) odd_values<TKV, 4>(y, sees[t], live, vb + (uint64_t)(uint32_t)len * v_step + e * TKV::kBytes, v_step);
-      put4<D, TQ>(p, b, hk, row, rows.node[t], split, e, y, rows.m[t], rows.l[t][0], bad, sees[t].any(), keys);
+      put4<D, TQ>(p, share, hk, row, rows.node[t], e, y, rows.m[t], rows.l[t][0], bad, sees[t].any(), keys);
     }
   }
 }
 
-// Joins the splits of a row: a wave a row, D / 4 lanes with four elements each for every fourth (D 128:
-// second) split, added in split order there and then over the lane groups.
+// Joins the blocks' results of a row: a wave a row, D / 4 lanes with four elements each for every fourth
+// (D 128: second) block, added in their order there and then over the lane groups.
 template <int D, class TQ>
 __global__ __launch_bounds__(256) void tree_join_kernel(Args p) {
   constexpr int kLanes = D / 4, kGroups = 64 / kLanes;
   const TreeAttn &a = p.a;
-  const int lane = threadIdx.x & 63, d = lane % kLanes * 4, s0 = lane / kLanes, M = p.M, S = p.S;
+  const int lane = threadIdx.x & 63, d = lane % kLanes * 4, s0 = lane / kLanes, M = p.M;
   const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (item >= (int64_t)a.batch * a.Hk * M) return;
   const int row = item % M, hk = item / M % a.Hk, b = item / M / a.Hk;
-  const float2 *w = p.ml + (size_t)item * S;
-  const float *part = a.part + (size_t)item * S * D + d;
-  const float2 own = w[min(lane, S - 1)];  // (at most 64 splits)
+  const int2 dealt = p.dealt[b];
+  const int S = dealt.y;
+  if (S == 1) return;  // (that block has written the row)
+  const size_t at = ((size_t)hk * M + row) * p.parts + dealt.x;
+  const float *part = a.part + at * D + d;
+  const float2 own = p.ml[at + min(lane, S - 1)];  // (at most 64 blocks)
+  float4 o = *reinterpret_cast<const float4 *>(part + (size_t)min(s0, S - 1) * D);  // (before what weighs it is there)
   const float top = wave_max(own.x), ms = top == -INFINITY ? 0.0f : top;
   const bool none = __ballot(own.x == INFINITY && own.y == 0.0f) != 0;
   // (at least 2^-126: 0 times an infinity would be NaN)
@@ -859,12 +928,13 @@ __global__ __launch_bounds__(256) void tree_join_kernel(Args p) {
 #pragma unroll 4
   for (int s1 = 0; s1 < S; s1 += kGroups) {
     const int s = min(s1 + s0, S - 1);
+    const float4 next = *reinterpret_cast<const float4 *>(part + (size_t)min(s + kGroups, S - 1) * D);
     const float m = __shfl(own.x, s, 64), l = __shfl(own.y, s, 64), f = __shfl(f_own, s, 64);
-    const float4 o = *reinterpret_cast<const float4 *>(part + (size_t)s * D);
     const bool in = s1 + s0 < S && !(m == -INFINITY && l == 0.0f);  // without keys nothing was stored
     const bool num = in && l == l;
     sum += in ? f * l : 0.0f;
     x[0] += num ? f * o.x : 0.0f, x[1] += num ? f * o.y : 0.0f, x[2] += num ? f * o.z : 0.0f, x[3] += num ? f * o.w : 0.0f;
+    o = next;
   }
 #pragma unroll
   for (int step = kLanes; step < 64; step *= 2) {
@@ -886,55 +956,61 @@ __global__ __launch_bounds__(256) void tree_join_kernel(Args p) {
 constexpr int most_tiles(int D, int q_bytes) { return (q_bytes == 4 ? 128 : 256) / D; }
 // The same where the waves share tiles, and hold none themselves.
 constexpr int rows_tiles(int D, int q_bytes) { return D == 128 && q_bytes == 4 ? 1 : 2; }
-// Waves over keys of a large block: RT 1 at D 64 fits 128 registers, the others 256.
-constexpr int large_waves(int D, int RT, int kv_bytes) { return D == 64 && RT == 1 && kv_bytes == 2 ? 16 : 8; }
 
 struct Plan {
-  int S, chunk, RT, WK, WR, row_tiles;
+  int parts, RT, WR, row_tiles, unit, least;
 };
 Plan make_plan(const TreeAttn &a, int n_cu) {
   Plan p;
   const int M = a.n * (a.H / a.Hk), most = most_tiles(a.D, a.qt == kOpF32 ? 4 : 2);
-  const int tiles = (a.max_seq + kTileKeys - 1) / kTileKeys;
   p.WR = a.kvt == kOpF32 || M <= 64 ? 0 : M <= 128 ? 4 : 8;
   if (p.WR > 0) {
     p.RT = rows_tiles(a.D, a.qt == kOpF32 ? 4 : 2);
-    p.WK = 1;
     p.row_tiles = (M + 16 * p.RT * p.WR - 1) / (16 * p.RT * p.WR);
+    p.unit = 5, p.least = 8;
   } else {
     p.RT = a.n > 64 ? most : std::min(most, M <= 16 ? 1 : M <= 32 ? 2 : 4);
     if (a.kvt == kOpF32 && M > 32 && M <= 48) p.RT = 1;  // (the fp32 products bound it: no empty fourth tile)
     p.row_tiles = (M + 16 * p.RT - 1) / (16 * p.RT);
-    const int64_t blocks = (int64_t)a.batch * a.Hk * p.row_tiles;
-    p.WK = a.n > 64 || blocks >= 2 * n_cu ? 4 : large_waves(a.D, p.RT, a.kvt == kOpF32 ? 4 : 2);
+    p.unit = 7, p.least = 2;
   }
-  const int64_t blocks = (int64_t)a.batch * a.Hk * p.row_tiles;
-  const int64_t want = (8 * n_cu / (p.WK * std::max(1, p.WR)) + blocks - 1) / blocks, can = (tiles + 4 * p.WK - 1) / (4 * p.WK);
-  const int S = (int)std::max<int64_t>(1, std::min<int64_t>({want, can, 64}));
-  p.chunk = ((tiles + S - 1) / S + p.WK - 1) / p.WK * p.WK * kTileKeys;
-  p.S = (a.max_seq + p.chunk - 1) / p.chunk;
+  // A block a compute unit: 2 x 16 heads over 40,001 and 65,500 rows 86 us, two a unit 90, half as many
+  // 128; 12 x 8 key heads of 128 dims over 1,000 .. 8,191 rows 95, 111, 160.  Two of shared tiles and 4
+  // waves: 2 x 20 heads, 84 nodes over 15,765 rows 48 us, one a unit 62; 24 x 4 key heads, 72 rows over
+  // 4,748 .. 5,359 58, 80.
+  p.parts = (int)std::min<int64_t>((p.WR == 4 ? 2 : 1) * n_cu / (a.Hk * p.row_tiles), 64ll * a.batch);
+  // (row tiles with the same keys on the same eighth of the card, which has an L2 of its own: 6 heads of a
+  // key head, 6 nodes, 2 x 52,834 rows 36 -> 29 us)
+  if (p.row_tiles > 1 && p.parts > 8) p.parts -= p.parts % (8 / std::gcd(8, a.Hk));
+  // Sharing costs 4.5 us (the lengths waited for, the second launch), and takes off the part of a block's
+  // time that others take over.  Lengths are not known here: at half of max_seq it has to pay.  20 heads,
+  // 8 nodes, a bf16 cache of 512, 1,024, 2,048, 4,096 rows: alone 8, 11, 16, 26 us, shared 11, 11, 12, 13;
+  // fp32: 11, 16, 24, 46 and 12, 13, 13, 16; 8 such sequences: 8, 12, 18, 29 and 12, 16, 22, 33.
+  const double alone = (p.WR > 0 ? 15.0 : a.kvt == kOpF32 ? 8.6 * p.RT : 3.5 + 0.9 * p.RT) * (a.D / 64) / 1024;  // us a row
+  const double taken = p.parts > a.batch ? 1.0 - (double)a.batch / p.parts : 0.0;
+  if (0.5 * a.max_seq * alone * taken < 4.5) p.parts = 0;
   return p;
 }
 
+size_t part_rows(const TreeAttn &a, const Plan &p) { return (size_t)a.H * a.n * p.parts; }
 Args make_args(const TreeAttn &a, const Plan &p) {
   const int group = a.H / a.Hk;
-  return Args{a, p.S, p.chunk, a.n * group, group, (uint32_t)(((1ull << 32) + group - 1) / group),
-              reinterpret_cast<float2 *>(a.part + (size_t)a.batch * a.H * a.n * p.S * a.D)};
+  float *ml = a.part + part_rows(a, p) * a.D;
+  return Args{a, p.parts, a.n * group, group, (uint32_t)(((1ull << 32) + group - 1) / group), p.unit, p.least,
+              reinterpret_cast<float2 *>(ml), reinterpret_cast<int2 *>(ml + 2 * part_rows(a, p))};
 }
 template <int D, class TQ, class K>
 hipError_t launch_kernel(K kernel, int threads, const TreeAttn &a, const Plan &p, hipStream_t s) {
   const Args args = make_args(a, p);
-  hipLaunchKernelGGL(kernel, dim3(p.S, a.Hk * p.row_tiles, a.batch), dim3(threads), 0, s, args);
-  if (hipError_t e = hipGetLastError(); e != hipSuccess || p.S == 1) return e;
+  hipLaunchKernelGGL(kernel, dim3(p.parts > 0 ? p.parts : a.batch, a.Hk * p.row_tiles), dim3(threads), 0, s, args);
+  if (hipError_t e = hipGetLastError(); e != hipSuccess || p.parts == 0) return e;
   const int64_t rows = (int64_t)a.batch * a.H * a.n;
   hipLaunchKernelGGL((tree_join_kernel<D, TQ>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, args);
   return hipGetLastError();
 }
 template <int D, class TQ, class TKV, int RT>
 hipError_t launch_keys(const TreeAttn &a, const Plan &p, hipStream_t s) {
-  constexpr int kLarge = large_waves(D, RT, TKV::kBytes);
-  if (p.WK == 4) return launch_kernel<D, TQ>(tree_attn_kernel<D, TQ, TKV, RT, 1, 4>, 256, a, p, s);
-  return launch_kernel<D, TQ>(tree_attn_kernel<D, TQ, TKV, RT, 1, kLarge>, 64 * kLarge, a, p, s);
+  return launch_kernel<D, TQ>(tree_attn_kernel<D, TQ, TKV, RT, 1>, 64 * kKeyWaves, a, p, s);
 }
 template <int D, class TQ, class TKV, int WR>
 hipError_t launch_rows(const TreeAttn &a, const Plan &p, hipStream_t s) {
@@ -949,7 +1025,7 @@ hipError_t launch_d(const TreeAttn &a, const Plan &p, hipStream_t s) {
     if (p.WR == 8) return launch_rows<D, TQ, TKV, 8>(a, p, s);
     if (p.WR == 4) return launch_rows<D, TQ, TKV, 4>(a, p, s);
   } else {
-    if (a.n > 64) return launch_kernel<D, TQ>(tree_attn_kernel<D, TQ, TKV, kMost, 4, 4>, 256, a, p, s);
+    if (a.n > 64) return launch_kernel<D, TQ>(tree_attn_kernel<D, TQ, TKV, kMost, 4>, 64 * kKeyWaves, a, p, s);
   }
   if constexpr (kMost >= 4)
     if (p.RT == 4) return launch_keys<D, TQ, TKV, 4>(a, p, s);
@@ -1006,14 +1082,14 @@ __global__ __launch_bounds__(256) void cache_keep_kernel(CacheKeep a) {
 
 size_t tree_attn_ws(const TreeAttn &a, int n_cu) {
   const Plan p = make_plan(a, n_cu);
-  return p.S == 1 ? 0 : (size_t)a.batch * a.H * a.n * p.S * (a.D + 2);
+  return p.parts == 0 ? 0 : part_rows(a, p) * (a.D + 2) + 2 * (size_t)a.batch;
 }
 
 hipError_t tree_attn(const TreeAttn &a, int n_cu, hipStream_t s) {
   if (a.batch <= 0 || a.n <= 0) return hipSuccess;
   if (a.n > kTreeMaxNodes || (a.D != 64 && a.D != 128) || a.H % a.Hk) return hipErrorInvalidValue;
   const Plan p = make_plan(a, n_cu);
-  if (p.S > 1 && !a.part) return hipErrorInvalidValue;
+  if (p.parts > 0 && !a.part) return hipErrorInvalidValue;
   if (a.qt == kOpF32 && a.kvt == kOpF32) return launch_t<F32, F32>(a, p, s);
   if (a.qt == kOpF32 && a.kvt == kOpBf16) return launch_t<F32, Bf16>(a, p, s);
   if (a.qt == kOpBf16 && a.kvt == kOpBf16) return launch_t<Bf16, Bf16>(a, p, s);
