@@ -80,8 +80,8 @@ struct Stats {
 
 __device__ __forceinline__ float wave_sum_f(float v) { return wave64_sum_dpp(v); }
 
-// The block's statistics from the threads'; every thread gets them.
-__device__ inline Stats block_stats(Stats t, float (*red)[4]) {
+// A wave's statistics from its threads', to LDS, and the block's from those.
+__device__ __forceinline__ void put_stats(const Stats &t, float (*red)[4]) {
   const float m = wave64_max_dpp(t.m);
   const Stats top = t.under(m);
   const Stats w{m, wave_sum_f(top.c), wave_sum_f(top.s), wave_sum_f(top.d)};
@@ -89,7 +89,8 @@ __device__ inline Stats block_stats(Stats t, float (*red)[4]) {
     float *r = red[threadIdx.x >> 6];
     r[0] = w.m, r[1] = w.c, r[2] = w.s, r[3] = w.d;
   }
-  __syncthreads();
+}
+__device__ __forceinline__ Stats get_stats(const float (*red)[4]) {
   Stats o{red[0][0], red[0][1], red[0][2], red[0][3]};
 #pragma unroll
   for (int i = 1; i < kWaves; i++) o.join(Stats{red[i][0], red[i][1], red[i][2], red[i][3]});
@@ -123,7 +124,7 @@ __device__ __forceinline__ uint32_t reached(uint32_t v, int n) {
 struct Select {
   uint64_t list[kList + kScoresMaxTop];
   uint64_t top[kScoresMaxTop];
-  uint32_t bound[2][kWaves];
+  uint32_t bound[kWaves];
   int count;
 };
 
@@ -167,13 +168,14 @@ __device__ inline void fill_masked(const void *x, int vocab, uint64_t *top, int 
   }
 }
 
+// Wave 0.
 template <int TYPE>
 __device__ inline void write_row(const TokenScores &a, int r, const void *x, const Row &row, Select &sel) {
   if (threadIdx.x == 0 && a.entropy) a.entropy[r] = row.entropy;
   if (a.top) {
-    if (threadIdx.x < 64 && !sel.top[a.top - 1]) fill_masked<TYPE>(x, a.vocab, sel.top, a.top);
-    __syncthreads();
-    for (int k = threadIdx.x; k < a.top; k += kThreads) {
+    if (!sel.top[a.top - 1]) fill_masked<TYPE>(x, a.vocab, sel.top, a.top);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    for (int k = threadIdx.x; k < a.top; k += 64) {
       const uint64_t key = sel.top[k];
       a.top_tokens[(int64_t)r * a.top + k] = key_token(key);
       // (from the logit itself: the order does not tell NaN from -inf)
@@ -185,8 +187,10 @@ __device__ inline void write_row(const TokenScores &a, int r, const void *x, con
 // The splits' results: statistics [rows][S], then ordered lists [rows][S][top].
 __host__ __device__ inline size_t list_offset(int rows, int S) { return sizeof(Stats) * (size_t)rows * S; }
 
-template <int TYPE>
-__global__ __launch_bounds__(kThreads, 4) void token_scores_kernel(TokenScores a, int S) {
+// LONG: a block's tokens are more than its threads hold, and the next ones are on their way while these
+// are counted.
+template <int TYPE, bool LONG>
+__global__ __launch_bounds__(kThreads, LONG ? 4 : 6) void token_scores_kernel(TokenScores a, int S) {
   __shared__ float red[kWaves][4];
   __shared__ Select sel;
   constexpr int P = kPer<TYPE>, kBytes = 16 / P, kRound = kThreads * kPieces * P;
@@ -201,7 +205,7 @@ __global__ __launch_bounds__(kThreads, 4) void token_scores_kernel(TokenScores a
   const char *body = x + (int64_t)i0 * kBytes;
   // a given token's logit, early
   const int64_t tok_at = r * a.tok_row;
-  const int tok = split == 0 && t < a.given ? a.tokens[tok_at + t] : -1;
+  const int tok = S == 1 && t < min(a.given, 64) ? a.tokens[tok_at + t] : -1;
   const float tok_x = tok >= 0 && tok < a.vocab ? logit<TYPE>(x, tok) : 0.0f;
 
   Stats st{-INFINITY, 0.0f, 0.0f, 0.0f};
@@ -210,22 +214,30 @@ __global__ __launch_bounds__(kThreads, 4) void token_scores_kernel(TokenScores a
     if (t < n) sel.top[t] = 0;
     if (t == 0) sel.count = 0;
   }
-  for (int base = 0; base == 0 || base < pieces; base += kThreads * kPieces) {
-    uint4 v[kPieces];
+  uint4 v[kPieces];
+  auto load = [&](uint4 (&to)[kPieces], int base) {
     const uint32_t none = TYPE == kOpF32 ? 0xff800000u : TYPE == kOpBf16 ? 0xff80ff80u : 0xfc00fc00u;  // -inf
 #pragma unroll
     for (int k = 0; k < kPieces; k++) {
       const int at = base + k * kThreads + t;
-      v[k] = make_uint4(none, none, none, none);
-      if (at < pieces) __builtin_memcpy(&v[k], body + (int64_t)at * 16, 16);  // (at any element's alignment)
+      to[k] = make_uint4(none, none, none, none);
+      if (at < pieces) __builtin_memcpy(&to[k], body + (int64_t)at * 16, 16);  // (at any element's alignment)
     }
+  };
+  load(v, 0);
+  for (int base = 0; base == 0 || base < pieces; base += kThreads * kPieces) {
+    uint4 coming[kPieces];
+    if constexpr (LONG) load(coming, base + kThreads * kPieces);
     const int odd = i1 - rest + t;  // one element a thread of the rest, in the first round
     const bool has_odd = base == 0 && t < rest;
     const float odd_x = has_odd ? logit<TYPE>(x, odd) : -INFINITY;
 
+    const int filled = (pieces - base + kThreads - 1) / kThreads;  // pieces of the first thread, and of others at most
     float gm[kPieces], mx = odd_x;
 #pragma unroll
     for (int k = 0; k < kPieces; k++) {
+      gm[k] = -INFINITY;
+      if (k >= filled) continue;
       again(v[k]);
       gm[k] = element<TYPE>(v[k], 0);
 #pragma unroll
@@ -234,35 +246,41 @@ __global__ __launch_bounds__(kThreads, 4) void token_scores_kernel(TokenScores a
     }
     Stats u{fmaxf(mx, -INFINITY), 0.0f, 0.0f, 0.0f};
     const float ms = u.m == -INFINITY ? 0.0f : u.m;
+    int at_top = 0;
     auto add = [&](float y) {
-      const float d = y - ms, p = __builtin_amdgcn_exp2f(d * kLog2e);
-      const bool at_top = y == ms;
-      u.c += at_top ? 1.0f : 0.0f;
-      u.s += at_top ? 0.0f : p;
+      // (at the maximum: as a token of probability 0, and counted)
+      const float d = y == ms ? -INFINITY : y - ms, p = __builtin_amdgcn_exp2f(d * kLog2e);
+      at_top += y == ms;
+      u.s += p;
       u.d += p * fmaxf(d, -3e38f);
     };
 #pragma unroll
     for (int k = 0; k < kPieces; k++) {
+      if (k >= filled) break;
       again(v[k]);
 #pragma unroll
       for (int e = 0; e < P; e++) add(element<TYPE>(v[k], e));
     }
     if (has_odd) add(odd_x);
-    st.join(u);
+    u.c = (float)at_top;
+    if constexpr (LONG) {
+      st.join(u);
+    } else {
+      put_stats(u, red);
+    }
 
     if (n > 0 && !ranked) {
-      // A bound for the n-th largest: n of one wave's threads reach it, or an equal share of every
-      // wave's.  (-inf has no part in this: a row's last places go to masked tokens at the end.)
-      const uint32_t top = u.m > -INFINITY ? order(u.m) : 0;
-      const uint32_t all = reached(top, n), share = reached(top, (n + kWaves - 1) / kWaves);
+      // A bound for the n-th largest: ceil(n / 4) threads of every wave reach it.  (-inf has no part in
+      // this: a row's last places go to masked tokens at the end.)
+      const uint32_t share = reached(u.m > -INFINITY ? order(u.m) : 0, (n + kWaves - 1) / kWaves);
+      if constexpr (LONG) __syncthreads();  // (the last round's are read)
+      if ((t & 63) == 0) sel.bound[t >> 6] = share;
       __syncthreads();
-      if ((t & 63) == 0) sel.bound[0][t >> 6] = all, sel.bound[1][t >> 6] = share;
-      __syncthreads();
-      uint32_t b0 = 0, b1 = ~0u;
+      uint32_t low = ~0u;
 #pragma unroll
-      for (int w = 0; w < kWaves; w++) b0 = max(b0, sel.bound[0][w]), b1 = min(b1, sel.bound[1][w]);
-      const uint64_t worst = sel.top[n - 1];  // (0 before n are found)
-      const uint32_t bound = max(max(max(b0, b1), (uint32_t)(worst >> 32)), kOrderNone + 1);
+      for (int w = 0; w < kWaves; w++) low = min(low, sel.bound[w]);
+      const uint64_t worst = LONG ? sel.top[n - 1] : 0;  // (0 before n are found)
+      const uint32_t bound = max(max(low, (uint32_t)(worst >> 32)), kOrderNone + 1);
       const float least = unorder(bound);
       auto offer = [&](float y, int token) {
         if (!(y >= least)) return;
@@ -279,7 +297,7 @@ __global__ __launch_bounds__(kThreads, 4) void token_scores_kernel(TokenScores a
       if (has_odd) offer(odd_x, odd);
       __syncthreads();
       const int count = sel.count;
-      __syncthreads();  // (it grows below)
+      if constexpr (LONG) __syncthreads();  // (it grows below)
       if (count > kList) {
         // Ties by the thousand, or the largest all in a few threads: n rounds of the largest that
         // is left, over all of this block's tokens in memory.
@@ -298,21 +316,31 @@ __global__ __launch_bounds__(kThreads, 4) void token_scores_kernel(TokenScores a
         if (t < n) sel.top[t] = mine;
         ranked = true;
       } else if (count > 0) {
-        if (t < n) {
-          const uint64_t k = sel.top[t];  // what was found before joins the list
-          if (k) sel.list[atomicAdd(&sel.count, 1)] = k;
+        int have = count;
+        if constexpr (LONG) {
+          if (t < n) {
+            const uint64_t k = sel.top[t];  // what was found before joins the list
+            if (k) sel.list[atomicAdd(&sel.count, 1)] = k;
+          }
+          __syncthreads();
+          have = sel.count;
         }
-        __syncthreads();
-        rank_list(sel, sel.count, n);
+        rank_list(sel, have, n);
       }
-      if (t == 0) sel.count = 0;
+      if (LONG && t == 0) sel.count = 0;
     }
+    if constexpr (!LONG) break;
+#pragma unroll
+    for (int k = 0; k < kPieces; k++) v[k] = coming[k];
   }
-  st = block_stats(st, red);
+  if constexpr (LONG) put_stats(st, red);
+  __syncthreads();
+  if (t >= 64) return;
+  st = get_stats(red);
 
   if (S == 1) {
     const Row row(st);
-    for (int i = t; i < a.given; i += kThreads) {
+    for (int i = t; i < a.given; i += 64) {
       const int k = i == t ? tok : a.tokens[tok_at + i];
       const bool in = k >= 0 && k < a.vocab;
       const float y = i == t ? tok_x : in ? logit<TYPE>(x, k) : 0.0f;
@@ -337,14 +365,6 @@ __global__ __launch_bounds__(kThreads) void scores_join_kernel(TokenScores a, in
   const Stats *parts = static_cast<const Stats *>(a.ws) + (int64_t)r * S;
   const uint64_t *lists = reinterpret_cast<const uint64_t *>(static_cast<const char *>(a.ws) + list_offset(a.rows, S)) + (int64_t)r * S * n;
   for (int i = t; i < S * n; i += kThreads) keys[i] = lists[i];
-  Stats st = parts[0];
-  for (int s = 1; s < S; s++) st.join(parts[s]);
-  const Row row(st);
-  for (int i = t; i < a.given; i += kThreads) {
-    const int k = a.tokens[r * a.tok_row + i];
-    const bool in = k >= 0 && k < a.vocab;
-    a.log_probs[(int64_t)r * a.given + i] = k == -1 ? 0.0f : in ? row.log_prob(logit<TYPE>(x, k)) : NAN;
-  }
   if (n > 0) {
     if (t == 0) sel.count = 0;
     __syncthreads();
@@ -375,6 +395,15 @@ __global__ __launch_bounds__(kThreads) void scores_join_kernel(TokenScores a, in
       __syncthreads();
     }
   }
+  if (t >= 64) return;
+  Stats st = parts[0];
+  for (int s = 1; s < S; s++) st.join(parts[s]);
+  const Row row(st);
+  for (int i = t; i < a.given; i += 64) {
+    const int k = a.tokens[r * a.tok_row + i];
+    const bool in = k >= 0 && k < a.vocab;
+    a.log_probs[(int64_t)r * a.given + i] = k == -1 ? 0.0f : in ? row.log_prob(logit<TYPE>(x, k)) : NAN;
+  }
   write_row<TYPE>(a, r, x, row, sel);
 }
 
@@ -386,7 +415,9 @@ int splits(const TokenScores &a, int n_cu) {
 
 template <int TYPE>
 hipError_t launch(const TokenScores &a, int S, hipStream_t s) {
-  hipLaunchKernelGGL(token_scores_kernel<TYPE>, dim3((unsigned)a.rows * S), dim3(kThreads), 0, s, a, S);
+  const int pieces = S == 1 ? a.vocab / kPer<TYPE> : ((a.vocab + S - 1) / S + kPer<TYPE> - 1) / kPer<TYPE>;  // of a block, at most
+  if (pieces > kThreads * kPieces) hipLaunchKernelGGL((token_scores_kernel<TYPE, true>), dim3((unsigned)a.rows * S), dim3(kThreads), 0, s, a, S);
+  else hipLaunchKernelGGL((token_scores_kernel<TYPE, false>), dim3((unsigned)a.rows * S), dim3(kThreads), 0, s, a, S);
   if (hipError_t e = hipGetLastError(); e != hipSuccess || S == 1) return e;
   hipLaunchKernelGGL(scores_join_kernel<TYPE>, dim3(a.rows), dim3(kThreads), 0, s, a, S);
   return hipGetLastError();

@@ -282,7 +282,7 @@ __device__ __forceinline__ Share share_of(const Args &p) {
   auto units = [&](int b) -> uint32_t {
     if (b >= a.batch) return 0;
     const int len = a.lengths[b];
-    return len < 0 || len > a.max_seq ? 1 : (uint32_t)(min(len + a.n, a.max_seq) - 1 >> p.unit) + 1;
+    return len < 0 || len > a.max_seq ? 1 : (uint32_t)((min(len + a.n, a.max_seq) - 1) >> p.unit) + 1;
   };
   float total = 0.0f, longest = 0.0f;
   for (int b = lane; b < a.batch + lane; b += 64) {
@@ -925,7 +925,6 @@ __global__ __launch_bounds__(256) void tree_join_kernel(Args p) {
   // (at least 2^-126: 0 times an infinity would be NaN)
   const float f_own = fmaxf(__builtin_amdgcn_exp2f(own.x - ms), 0x1p-126f);
   float sum = 0.0f, x[4] = {};
-#pragma unroll 4
   for (int s1 = 0; s1 < S; s1 += kGroups) {
     const int s = min(s1 + s0, S - 1);
     const float4 next = *reinterpret_cast<const float4 *>(part + (size_t)min(s + kGroups, S - 1) * D);
