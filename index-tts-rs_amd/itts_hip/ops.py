@@ -29,7 +29,9 @@ def _refuse(message: str):
     raise ValidationError(ITTS_E_VALIDATION, message)
 
 
-def _tensor(t, name: str, dims: int, device=None, dtype=None):
+def _tensor(t, name: str, dims: int, device=None, dtype=None, last=False):
+    """Checks a tensor; last: its last dimension must be contiguous.  (A call of an operator is host time before all
+    else: nothing is asked twice here, and strides are handed on.)"""
     if not isinstance(t, torch.Tensor):
         _refuse(f"{name}: a tensor is needed, got {type(t).__name__}")
     if t.dim() != dims:
@@ -39,17 +41,17 @@ def _tensor(t, name: str, dims: int, device=None, dtype=None):
             _refuse(f"{name}: float32, bfloat16 or float16 expected, got {t.dtype}")
     elif t.dtype != dtype:
         _refuse(f"{name}: {dtype} expected, got {t.dtype}")
-    if not t.is_cuda:
-        _refuse(f"{name}: a GPU tensor is needed, got one on {t.device}")
-    if device is not None and t.device != device:
-        _refuse(f"{name}: on {t.device}, the other tensors on {device}")
+    if device is None or t.device != device:
+        if not t.is_cuda:
+            _refuse(f"{name}: a GPU tensor is needed, got one on {t.device}")
+        if device is not None:
+            _refuse(f"{name}: on {t.device}, the other tensors on {device}")
     if t.requires_grad and torch.is_grad_enabled():
         _refuse(f"{name}: requires a gradient, which this operator does not give")
-
-
-def _last_contiguous(t, name: str):
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
+    strides = t.stride()
+    if last and strides[-1] != 1 and t.shape[-1] > 1:
         _refuse(f"{name}: the last dimension must be contiguous")
+    return strides
 
 
 # The current stream's handle without a Stream object around it (2 us of a call's host time).
@@ -66,8 +68,10 @@ def _run(fn, need, args, device):
         return _check(fn(ref, _stream(device.index)))
     size = C.c_uint64()
     _check(need(ref, C.byref(size)))
-    ws = torch.empty(size.value, dtype=torch.uint8, device=device) if size.value else None
-    _check(fn(ref, None if ws is None else ws.data_ptr(), size, _stream(device.index)))
+    if not size.value:
+        return _check(fn(ref, None, 0, _stream(device.index)))
+    ws = torch.empty(size.value, dtype=torch.uint8, device=device)
+    _check(fn(ref, ws.data_ptr(), size, _stream(device.index)))
 
 
 def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: torch.Tensor, parents: torch.Tensor, *,
@@ -85,42 +89,42 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: t
              rows of zeros
     scale    of the scores (default dim ** -0.5)
     max_length  rows that a sequence with its nodes may use (default: the caches' rows); a tight one
-             lets short sequences be split better
+             lets short sequences do with one launch
     out      where to write (default: a new tensor)
 
     A node sees its sequence's rows, its ancestors and itself.  A negative length, or one whose nodes do not
     fit, gives rows of NaN.  Returns out [batch][nodes][heads][dim] in q's type."""
-    _tensor(q, "q", 4)
+    sq = _tensor(q, "q", 4, last=True)
     dev = q.device
-    _tensor(k, "k", 4, dev)
-    _tensor(v, "v", 4, dev)
-    _tensor(lengths, "lengths", 1, dev, torch.int32)
-    _tensor(parents, "parents", 2, dev, torch.int32)
-    for t, name in ((q, "q"), (k, "k"), (v, "v"), (parents, "parents")):
-        _last_contiguous(t, name)
+    sk = _tensor(k, "k", 4, dev, last=True)
+    sv = _tensor(v, "v", 4, dev, last=True)
+    sl = _tensor(lengths, "lengths", 1, dev, torch.int32)
+    sp = _tensor(parents, "parents", 2, dev, torch.int32, last=True)
     b, n, h, d = q.shape
-    if k.shape != v.shape or k.dtype != v.dtype:
-        _refuse(f"v: must be like k, {tuple(k.shape)} {k.dtype}, got {tuple(v.shape)} {v.dtype}")
-    if k.shape[0] != b or k.shape[3] != d:
-        _refuse(f"k: [{b}][heads][rows][{d}] expected, got {tuple(k.shape)}")
+    kb, hk, rows, kd = shape = k.shape
+    if shape != v.shape or k.dtype != v.dtype:
+        _refuse(f"v: must be like k, {tuple(shape)} {k.dtype}, got {tuple(v.shape)} {v.dtype}")
+    if kb != b or kd != d:
+        _refuse(f"k: [{b}][heads][rows][{d}] expected, got {tuple(shape)}")
     if lengths.shape[0] != b or parents.shape != (b, n):
         _refuse(f"lengths, parents: [{b}] and [{b}][{n}] expected, got {tuple(lengths.shape)} and {tuple(parents.shape)}")
-    if lengths.shape[0] > 1 and lengths.stride(0) != 1:
+    if b > 1 and sl[0] != 1:
         _refuse("lengths: must be contiguous")
-    rows = k.shape[2] if max_length is None else int(max_length)
-    if rows > k.shape[2]:
-        _refuse(f"max_length: the caches have {k.shape[2]} rows, got {rows}")
+    if max_length is not None:
+        if int(max_length) > rows:
+            _refuse(f"max_length: the caches have {rows} rows, got {int(max_length)}")
+        rows = int(max_length)
     if out is None:
-        out = torch.empty((b, n, h, d), dtype=q.dtype, device=dev)
+        out = q.new_empty((b, n, h, d))
+        so = (n * h * d, h * d, d)
     else:
-        _tensor(out, "out", 4, dev, q.dtype)
-        _last_contiguous(out, "out")
+        so = _tensor(out, "out", 4, dev, q.dtype, last=True)
         if out.shape != q.shape:
             _refuse(f"out: {tuple(q.shape)} expected, got {tuple(out.shape)}")
     a = itts_tree_attention_args(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lengths.data_ptr(),
-                                 parents.data_ptr(), b, n, h, k.shape[1], d, rows, _DTYPES[q.dtype], _DTYPES[k.dtype],
-                                 d ** -0.5 if scale is None else scale, *q.stride()[:3], *out.stride()[:3], *k.stride()[:3],
-                                 *v.stride()[:3], parents.stride(0))
+                                 parents.data_ptr(), b, n, h, hk, d, rows, _DTYPES[q.dtype], _DTYPES[k.dtype],
+                                 d ** -0.5 if scale is None else scale, sq[0], sq[1], sq[2], so[0], so[1], so[2],
+                                 sk[0], sk[1], sk[2], sv[0], sv[1], sv[2], sp[0])
     _run(lib.itts_tree_attention, lib.itts_tree_attention_workspace, a, dev)
     return out
 
@@ -142,29 +146,27 @@ def token_scores(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, to
 
     A row of -inf alone gives every token -inf, and entropy 0.  A NaN or +inf makes its row's
     log-probabilities and entropy NaN; NaN counts as -inf in the order.  log_probs has tokens' shape."""
-    _tensor(logits, "logits", 2)
-    _last_contiguous(logits, "logits")
+    sx = _tensor(logits, "logits", 2, last=True)
     dev = logits.device
     r, vocab = logits.shape
-    given, log_probs, tok = 0, None, None
+    given, log_probs, tok, log_probs_at, tok_row = 0, None, None, None, 0
     if tokens is not None:
         one = isinstance(tokens, torch.Tensor) and tokens.dim() == 1
-        _tensor(tokens, "tokens", 1 if one else 2, dev, torch.int32)
+        st = _tensor(tokens, "tokens", 1 if one else 2, dev, torch.int32, last=not one)
         if tokens.shape[0] != r:
             _refuse(f"tokens: {r} rows expected, got {tokens.shape[0]}")
-        tok = tokens.unsqueeze(1) if one else tokens
-        _last_contiguous(tok, "tokens")
-        given = tok.shape[1]
+        given, tok_row = 1 if one else tokens.shape[1], st[0]
         log_probs = torch.empty(tokens.shape, dtype=torch.float32, device=dev)
+        if given:
+            tok, log_probs_at = tokens.data_ptr(), log_probs.data_ptr()
     top_n = int(top_n)
     if not 0 <= top_n <= min(64, vocab):
         _refuse(f"top_n: must be in 0..=64 and at most the vocabulary of {vocab}, got {top_n}")
     entropy = torch.empty(r, dtype=torch.float32, device=dev)
     top_tokens = torch.empty((r, top_n), dtype=torch.int32, device=dev)
     top_log_probs = torch.empty((r, top_n), dtype=torch.float32, device=dev)
-    a = itts_token_scores_args(logits.data_ptr(), tok.data_ptr() if given else None, log_probs.data_ptr() if given else None,
-                               entropy.data_ptr(), top_tokens.data_ptr(), top_log_probs.data_ptr(), r, vocab, given, top_n,
-                               _DTYPES[logits.dtype], logits.stride(0), tok.stride(0) if given else 0)
+    a = itts_token_scores_args(logits.data_ptr(), tok, log_probs_at, entropy.data_ptr(), top_tokens.data_ptr(),
+                               top_log_probs.data_ptr(), r, vocab, given, top_n, _DTYPES[logits.dtype], sx[0], tok_row)
     _run(lib.itts_token_scores, lib.itts_token_scores_workspace, a, dev)
     return TokenScores(log_probs, entropy, top_tokens, top_log_probs)
 
@@ -179,23 +181,25 @@ def cache_keep(k: torch.Tensor, v: torch.Tensor, lengths: torch.Tensor, path: to
     Returns the new lengths [batch], lengths[b] + the nodes kept; -1, with nothing moved, for a path that does not rise or
     leaves the cache, or a negative length."""
     dims = 4 if isinstance(k, torch.Tensor) and k.dim() == 4 else 5
-    _tensor(k, "k", dims)
+    sk = _tensor(k, "k", dims, last=True)
     dev = k.device
-    _tensor(v, "v", dims, dev, k.dtype)
-    _tensor(lengths, "lengths", 1, dev, torch.int32)
-    _tensor(path, "path", 2, dev, torch.int32)
+    sv = _tensor(v, "v", dims, dev, k.dtype, last=True)
+    sl = _tensor(lengths, "lengths", 1, dev, torch.int32)
+    sp = _tensor(path, "path", 2, dev, torch.int32, last=True)
     if v.shape != k.shape:
         _refuse(f"v: must be like k, {tuple(k.shape)}, got {tuple(v.shape)}")
-    for t, name in ((k, "k"), (v, "v"), (path, "path")):
-        _last_contiguous(t, name)
-    kk, vv = (k, v) if dims == 5 else (k.unsqueeze(0), v.unsqueeze(0))
-    layers, b, h, rows, d = kk.shape
+    if dims == 5:
+        layers, b, h, rows, d = k.shape
+    else:
+        layers, (b, h, rows, d) = 1, k.shape
+        sk, sv = (0, *sk), (0, *sv)
     if lengths.shape[0] != b or path.shape[0] != b:
         _refuse(f"lengths, path: {b} sequences expected, got {lengths.shape[0]} and {path.shape[0]}")
-    if b > 1 and lengths.stride(0) != 1:
+    if b > 1 and sl[0] != 1:
         _refuse("lengths: must be contiguous")
     new = torch.empty(b, dtype=torch.int32, device=dev)
-    a = itts_cache_keep_args(kk.data_ptr(), vv.data_ptr(), lengths.data_ptr(), path.data_ptr(), new.data_ptr(), layers, b,
-                             h, rows, d, path.shape[1], _DTYPES[k.dtype], *kk.stride()[:4], *vv.stride()[:4], path.stride(0))
+    a = itts_cache_keep_args(k.data_ptr(), v.data_ptr(), lengths.data_ptr(), path.data_ptr(), new.data_ptr(), layers, b, h,
+                             rows, d, path.shape[1], _DTYPES[k.dtype], sk[0], sk[1], sk[2], sk[3], sv[0], sv[1], sv[2], sv[3],
+                             sp[0])
     _run(lib.itts_cache_keep, None, a, dev)
     return new
