@@ -388,7 +388,7 @@ itts_status itts_tree_attention(const itts_tree_attention_args *args, void *work
  * most probable first, the lowest token first among equals (top_n <= 64; 0: none).  A row of
  * -inf alone gives every token -inf, and entropy 0; NaN or +inf anywhere in a row makes its
  * log-probabilities and entropy NaN, and NaN counts as -inf in the order.
- * log_probs [rows][n_tokens], top_tokens and top_log_probs [rows][top_n]. */
+ * log_probs [rows][n_tokens], top_tokens and top_log_probs [rows][top_n]; at most 2^23 rows. */
 typedef struct itts_token_scores_args {
   const void *logits;
   const int32_t *tokens;
@@ -409,7 +409,7 @@ itts_status itts_token_scores(const itts_token_scores_args *args, void *workspac
  * entries of path[b] before its first negative one; new_lengths[b] = lengths[b] + their count.  A
  * path rises and stays inside max_seq rows: for any other, or a negative length, nothing moves
  * and new_lengths[b] = -1.  path [batch][n_path].  All rows are multiples of 16 bytes and start at
- * them. */
+ * them.  k and v may be one memory with the same strides; otherwise no two rows overlap. */
 typedef struct itts_cache_keep_args {
   void *k, *v;
   const int32_t *lengths;

@@ -321,6 +321,7 @@ struct TreeAttn {
   float scale;
   int64_t q_b, q_n, q_h, o_b, o_n, o_h, k_b, k_h, k_r, v_b, v_h, v_r, par_b;
   float *part;  // tree_attn_ws(a, n_cu) floats
+  float used = 0.5f;  // of max_seq, by an average sequence
 };
 size_t tree_attn_ws(const TreeAttn &a, int n_cu);
 hipError_t tree_attn(const TreeAttn &a, int n_cu, hipStream_t s);
@@ -336,6 +337,7 @@ struct CacheKeep {
   int32_t *new_lengths;
   int layers, batch, heads, max_seq, row_pieces, n_path;  // row_pieces: 16-byte pieces of a row
   int64_t k_l, k_b, k_h, k_r, v_l, v_b, v_h, v_r, path_b;   // cache strides in 16-byte pieces
+  int caches = 2;                                           // 1: v is k
 };
 hipError_t cache_keep(const CacheKeep &a, hipStream_t s);
 // Rows of logits: log-probabilities of given tokens, entropy, the top_n most probable tokens.

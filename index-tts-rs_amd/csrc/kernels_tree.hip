@@ -269,9 +269,11 @@ struct Args {
 // What block `index` of `parts` has to do: rows [first, end) of sequence b, whose rows are shared by
 // n blocks (0: nothing is left for this one).  Every block gets the same number of rows, whatever
 // the sequences' lengths and however long the cache could become: the smallest one with which `parts`
-// blocks are enough.  Every wave finds it by itself from the lengths, a lane a sequence; 12 lengths
-// from 1,000 to 8,191, 8 key heads: 115 us with the rows
-// of max_seq shared equally, xx us with these.
+// blocks are enough (within a few percent).  Every wave finds it by itself from the lengths, a lane a
+// sequence.  12 x 64 nodes over 1,000 .. 8,191 rows, 8 key heads: 115 us with the rows of max_seq shared
+// equally, 106 with these.  A block still waits for the longest one, a fifth above the mean there; runs
+// that go on into the next sequence made that kernel 7 us faster and the one for few rows 1 to 10
+// slower (registers kept over the turns, a second start), and are not taken.
 struct Share {
   int b, n, first, end, index, from;
 };
@@ -358,8 +360,8 @@ struct TileRegs {
 // Planes of 16 bits that hold a probability.  Few query rows wait for memory, not for products: two
 // (16 bits of bf16, 22 of fp16) leave no more than the result's own rounding.  Many rows over 16-bit
 // queries wait for instructions: one, rounded (half a step of the result's type, and the same
-// rounded values in the sums), 12 x 64 nodes of 4 heads over 8,191 rows 144 -> 114 us.  fp32 queries: three,
-// an fp32's bits.
+// rounded values in the sums), 12 x 64 nodes, 32 heads of 8 over 1,000 .. 8,191 rows 144 -> 114 us at
+// the time.  fp32 queries: three, an fp32's bits.
 template <class TQ>
 constexpr int prob_planes(bool many) {
   return TQ::kBytes == 4 ? 3 : many ? 1 : 2;
@@ -462,7 +464,7 @@ struct Rows {
     for (int t = 0; t < RT; t++) {
       top[t] = s[0][t][0];
 #pragma unroll
-      for (int i = 1; i < 7; i += 2) top[t] = fmaxf(fmaxf(s[i >> 2][t][i & 3], s[i + 1 >> 2][t][i + 1 & 3]), top[t]);
+      for (int i = 1; i < 7; i += 2) top[t] = fmaxf(fmaxf(s[i >> 2][t][i & 3], s[(i + 1) >> 2][t][(i + 1) & 3]), top[t]);
       top[t] = fmaxf(s[1][t][3], top[t]) * scale;
       grows = grows || top[t] > m[t] + kLag;
     }
@@ -641,8 +643,12 @@ __device__ __forceinline__ void put4(const Args &p, const Share &share, int hk, 
   }
 }
 
-// Few query rows: WK waves over tiles of keys of their own, straight from memory into registers, one
-// tile ahead; joined at the end.
+// Few query rows: 4 waves over tiles of keys of their own, straight from memory into registers, one
+// tile ahead; joined at the end.  Long caches are bound by memory: 2 x 16 heads, 61 nodes, 40,001 and 65,500
+// fp16 rows, 433 MB, 81 us; 32 single tokens, 4 key heads of 128, 513 .. 4,097 bf16 rows, 152 MB, 27.  Short ones
+// by the chain from load to result: 8 nodes, 20 heads, 235 rows 6.0 us.  fp32 caches by the fp32
+// products, of 4 keys at a time: 33 nodes, 20 heads, 1,734 rows 12.7 us.  fp32 queries over bf16 by the
+// three planes' instructions: 8 x 27 nodes, 250 .. 1,400 rows 15.7 us.
 template <int D, class TQ, class TKV, int RT, int W>
 __global__ __launch_bounds__(256, 2) void tree_attn_kernel(Args p) {
   constexpr int WK = kKeyWaves;
@@ -761,6 +767,10 @@ __global__ __launch_bounds__(256, 2) void tree_attn_kernel(Args p) {
 // order p ^ row: what a wave reads at a time, one piece of 16 key rows or two neighbours of 16 value
 // rows, falls on different banks.  Values are read through the transposing load: lane 4 j + a of 16
 // reads elements 4 a .. of row j, and lane i gets element i of the four rows.
+// 12 x 64 nodes, 32 heads of 128 over 8 key heads, 1,000 .. 8,191 bf16 rows: 95 us, 490 TFLOP/s.  The matrix
+// units are busy 28% of that; the two waves of a SIMD share its issue with 120 vector and 50 other
+// instructions a tile, and meet at a barrier a tile.  Tiles two ahead spilled (161 us for 144 then),
+// blocks of 4 waves read every tile twice as often (127 for 115).
 template <int D, class TQ, class TKV, int RT, int W, int WR>
 __global__ __launch_bounds__(64 * WR, 2) void tree_attn_rows_kernel(Args p) {
   constexpr int kPieces = D * TKV::kBytes / 16, kThreads = 64 * WR, kTile = kTileKeys * kPieces, kCopy = 2 * kTile / kThreads;
@@ -904,7 +914,8 @@ __global__ __launch_bounds__(64 * WR, 2) void tree_attn_rows_kernel(Args p) {
 }
 
 // Joins the blocks' results of a row: a wave a row, D / 4 lanes with four elements each for every fourth
-// (D 128: second) block, added in their order there and then over the lane groups.
+// (D 128: second) block, added in their order there and then over the lane groups.  Bound by memory where
+// it counts: 33 MB of results 11 us.
 template <int D, class TQ>
 __global__ __launch_bounds__(256) void tree_join_kernel(Args p) {
   constexpr int kLanes = D / 4, kGroups = 64 / kLanes;
@@ -982,12 +993,13 @@ Plan make_plan(const TreeAttn &a, int n_cu) {
   // key head, 6 nodes, 2 x 52,834 rows 36 -> 29 us)
   if (p.row_tiles > 1 && p.parts > 8) p.parts -= p.parts % (8 / std::gcd(8, a.Hk));
   // Sharing costs 4.5 us (the lengths waited for, the second launch), and takes off the part of a block's
-  // time that others take over.  Lengths are not known here: at half of max_seq it has to pay.  20 heads,
-  // 8 nodes, a bf16 cache of 512, 1,024, 2,048, 4,096 rows: alone 8, 11, 16, 26 us, shared 11, 11, 12, 13;
-  // fp32: 11, 16, 24, 46 and 12, 13, 13, 16; 8 such sequences: 8, 12, 18, 29 and 12, 16, 22, 33.
+  // time that others take over.  Lengths are not known here: it has to pay at the part of max_seq that
+  // is used on average.  20 heads, 8 nodes, a bf16 cache, 512, 1,024, 2,048, 4,096 rows: alone 8, 11, 16, 26 us,
+  // shared 11, 11, 12, 13; fp32: 11, 16, 24, 46 and 12, 13, 13, 16; 8 sequences over bf16: 8, 12, 18, 29 and 12,
+  // 16, 22, 33.
   const double alone = (p.WR > 0 ? 15.0 : a.kvt == kOpF32 ? 8.6 * p.RT : 3.5 + 0.9 * p.RT) * (a.D / 64) / 1024;  // us a row
   const double taken = p.parts > a.batch ? 1.0 - (double)a.batch / p.parts : 0.0;
-  if (0.5 * a.max_seq * alone * taken < 4.5) p.parts = 0;
+  if (a.used * a.max_seq * alone * taken < 4.5) p.parts = 0;
   return p;
 }
 
@@ -1068,7 +1080,7 @@ __global__ __launch_bounds__(256) void cache_keep_kernel(CacheKeep a) {
   const int head = i % a.heads;
   i /= a.heads;
   const int layer = i % a.layers, is_v = (int)(i / a.layers);
-  if (is_v > 1) return;
+  if (is_v >= a.caches) return;
   uint4 *base = is_v ? static_cast<uint4 *>(a.v) + layer * a.v_l + b * a.v_b + head * a.v_h
                      : static_cast<uint4 *>(a.k) + layer * a.k_l + b * a.k_b + head * a.k_h;
   const int64_t step = is_v ? a.v_r : a.k_r;
@@ -1103,7 +1115,7 @@ hipError_t launch_tree_seqs(const int32_t *in, int n, BatchSeq *seqs, DecodeCtl 
 
 hipError_t cache_keep(const CacheKeep &a, hipStream_t s) {
   if (a.batch <= 0) return hipSuccess;
-  const int64_t items = 2ll * a.layers * a.heads * a.row_pieces;
+  const int64_t items = (int64_t)a.caches * a.layers * a.heads * a.row_pieces;
   hipLaunchKernelGGL(cache_keep_kernel, dim3((unsigned)std::max<int64_t>(1, (items + 255) / 256), a.batch), dim3(256), 0, s,
                      a);
   return hipGetLastError();

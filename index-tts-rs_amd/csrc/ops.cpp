@@ -122,7 +122,7 @@ itts_status tree_args(const itts_tree_attention_args *a, TreeAttn *o) {
 
 itts_status scores_args(const itts_token_scores_args *a, TokenScores *o) {
   if (!a) return fail(ITTS_E_VALIDATION, "args: null");
-  if (a->rows < 0) return fail(ITTS_E_VALIDATION, "rows: must be >= 0, got %d", a->rows);
+  if (a->rows < 0 || a->rows > 1 << 23) return fail(ITTS_E_VALIDATION, "rows: must be in 0..=2^23, got %d", a->rows);
   if (a->vocab < 1 || a->vocab > 1 << 24) return fail(ITTS_E_VALIDATION, "vocab: must be in 1..=2^24, got %d", a->vocab);
   if (a->n_tokens < 0) return fail(ITTS_E_VALIDATION, "n_tokens: must be >= 0, got %d", a->n_tokens);
   if (a->top_n < 0 || a->top_n > kScoresMaxTop || a->top_n > a->vocab)
@@ -221,7 +221,7 @@ itts_status itts_cache_keep(const itts_cache_keep_args *a, void *stream) {
   const int es = op_size(t);
   if ((int64_t)a->head_dim * es % 16 != 0) return fail(ITTS_E_VALIDATION, "head_dim: rows must be multiples of 16 bytes");
   const int64_t items = (int64_t)a->head_dim * es / 16 * 2;
-  if ((double)items * a->n_layer * a->n_head > 2e11) return fail(ITTS_E_VALIDATION, "n_layer: caches too large");
+  if ((double)items * a->n_layer * a->n_head > 4e9) return fail(ITTS_E_VALIDATION, "n_layer: caches too large");
   const int64_t ks[4] = {a->k_layer, a->k_batch, a->k_head, a->k_row}, vs[4] = {a->v_layer, a->v_batch, a->v_head, a->v_row};
   const int ext[4] = {a->n_layer, a->batch, a->n_head, a->max_seq};
   for (int i = 0; i < 4; i++) {
@@ -234,6 +234,10 @@ itts_status itts_cache_keep(const itts_cache_keep_args *a, void *stream) {
   if (!a->lengths || !a->new_lengths || (a->n_path && !a->path) || ((int64_t)a->n_layer * a->n_head && (!a->k || !a->v)))
     return fail(ITTS_E_VALIDATION, "k, v, lengths, path, new_lengths: null");
   if (a->lengths == a->new_lengths) return fail(ITTS_E_VALIDATION, "new_lengths: must not be lengths");
+  // One memory for both moves once: two would read rows that the other has moved.
+  const bool same = a->k == a->v && a->n_layer > 0 && a->n_head > 0;
+  for (int i = 0; i < 4; i++)
+    if (same && ext[i] > 1 && ks[i] != vs[i]) return fail(ITTS_E_VALIDATION, "k, v: rows must not overlap");
   int dev = 0, n_cu = 0;
   if (itts_status st = compute_units(&dev, &n_cu)) return st;
   if (itts_status st = check_device(dev, stream, {{a->k, "k"}, {a->v, "v"}, {a->lengths, "lengths"}, {a->n_path ? a->path : nullptr, "path"},
@@ -242,7 +246,7 @@ itts_status itts_cache_keep(const itts_cache_keep_args *a, void *stream) {
   const int per = 16 / es;
   const CacheKeep c{a->k, a->v, a->lengths, a->path, a->new_lengths, a->n_layer, a->batch, a->n_head, a->max_seq,
                     a->head_dim / per, a->n_path, ks[0] / per, ks[1] / per, ks[2] / per, ks[3] / per, vs[0] / per, vs[1] / per,
-                    vs[2] / per, vs[3] / per, a->path_batch};
+                    vs[2] / per, vs[3] / per, a->path_batch, same ? 1 : 2};
   if (hipError_t e = cache_keep(c, static_cast<hipStream_t>(stream)); e != hipSuccess) return hip_fail(e, "kept rows");
   return ITTS_OK;
 }

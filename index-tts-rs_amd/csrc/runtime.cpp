@@ -890,6 +890,7 @@ TreeAttn tree_attn_args(const itts_gpt *g, const TreeStep &t, int l, int n) {
   a.k_h = a.v_h = head;
   a.k_r = a.v_r = 64;
   a.part = g->tpart.as<float>();
+  a.used = 1.0f;
   return a;
 }
 itts_status enqueue_step_batch(itts_gpt *g, int B, int max_seq, int kvt, const TreeStep *tree = nullptr) {

@@ -419,6 +419,20 @@ def test_keep_strides_and_four_dimensions(ops):
     assert torch.equal(four_k, wk[1]) and torch.equal(four_v, wv[1])
 
 
+def test_keep_of_one_memory_for_keys_and_values(ops):
+    """k and v the same tensor: its rows move once (twice, rows would follow that have moved already)."""
+    say("[gpu] keep: v is k")
+    g = gen(8)
+    k = randn(g, 3, 2, 4, 40, 64)
+    lengths, path = ints([5, 20]), ints([[1, 2, 4, 7], [0, 3, 9, -1]])
+    want = k.clone()
+    for i, (n, p) in enumerate(((5, (1, 2, 4, 7)), (20, (0, 3, 9)))):
+        for j, node in enumerate(p):
+            want[:, i, :, n + j] = k[:, i, :, n + node]
+    assert ops.cache_keep(k, k, lengths, path).tolist() == [9, 23]
+    assert torch.equal(k, want)
+
+
 # ---- streams, graphs, refusals -----------------------------------------------------------------
 def drafted(ops, s):
     """The three as they are used: a draft's attention, its scores, the accepted rows kept."""

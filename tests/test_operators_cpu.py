@@ -105,3 +105,12 @@ def test_python_entries_refuse():
     with pytest.raises(H.ValidationError, match="k: a GPU tensor"):
         ops.cache_keep(torch.zeros(2, 1, 4, 8, 64), torch.zeros(2, 1, 4, 8, 64), torch.zeros(1, dtype=torch.int32),
                        torch.zeros(1, 2, dtype=torch.int32))
+
+
+@pytest.mark.parametrize("kind,field,over", [
+    (keep, "k, v", dict(v_head=6400, v_batch=25600, v_layer=76800)), (keep, "k, v", dict(v_row=128, v_head=6400)),
+    (keep, "n_layer", dict(n_layer=1 << 20, n_head=1 << 10)), (scores, "rows", dict(rows=(1 << 23) + 1)),
+], ids=lambda x: getattr(x, "__name__", str(x)))
+def test_c_entries_refuse_overlaps_and_sizes_past_a_grid(kind, field, over):
+    """One memory as keys and as values under two layouts; more blocks than a launch has."""
+    test_c_entries_refuse(kind, field, over)
