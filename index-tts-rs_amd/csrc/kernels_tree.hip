@@ -10,6 +10,7 @@
 // Softmax statistics stay in the lanes (max over the four lane groups of a column by two
 // exchanges, sums only at the end).
 #include <algorithm>
+#include <cmath>
 #include <numeric>
 #include <type_traits>
 
@@ -21,6 +22,7 @@ namespace {
 
 constexpr int kTileKeys = 32;  // keys a wave takes at a time
 constexpr int kKeyWaves = 4;   // waves of a block that share a few rows' keys
+constexpr int kRowWaves = 4;   // waves of a block with rows of their own over the same keys
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct F32 {
@@ -760,8 +762,8 @@ __global__ __launch_bounds__(256, 2) void tree_attn_kernel(Args p) {
   }
 }
 
-// Many query rows over 16-bit caches: WR waves with rows of their own over the same tiles, which the
-// block copies to LDS (through registers), so that a tile is read from memory once for 16 RT WR
+// Many query rows over 16-bit caches: 4 waves with rows of their own over the same tiles, which the
+// block copies to LDS (through registers), so that a tile is read from memory once for 64 RT
 // rows.  A tile's scores are formed a tile ahead, so that their products run under the exponentials
 // of the one before: keys lie a tile further than values.  In LDS a row's 16-byte pieces lie in the
 // order p ^ row: what a wave reads at a time, one piece of 16 key rows or two neighbours of 16 value
@@ -769,11 +771,11 @@ __global__ __launch_bounds__(256, 2) void tree_attn_kernel(Args p) {
 // reads elements 4 a .. of row j, and lane i gets element i of the four rows.
 // 12 x 64 nodes, 32 heads of 128 over 8 key heads, 1,000 .. 8,191 bf16 rows: 95 us, 490 TFLOP/s.  The matrix
 // units are busy 28% of that; the two waves of a SIMD share its issue with 120 vector and 50 other
-// instructions a tile, and meet at a barrier a tile.  Tiles two ahead spilled (161 us for 144 then),
-// blocks of 4 waves read every tile twice as often (127 for 115).
-template <int D, class TQ, class TKV, int RT, int W, int WR>
-__global__ __launch_bounds__(64 * WR, 2) void tree_attn_rows_kernel(Args p) {
-  constexpr int kPieces = D * TKV::kBytes / 16, kThreads = 64 * WR, kTile = kTileKeys * kPieces, kCopy = 2 * kTile / kThreads;
+// instructions a tile.  Tiles two ahead spilled (161 us for 144 then); blocks of 8 waves read every
+// tile half as often and are no faster (103 us with the joining for 104; 2 x 144 nodes over 3,700 rows 38, 38).
+template <int D, class TQ, class TKV, int RT, int W>
+__global__ __launch_bounds__(64 * kRowWaves, 2) void tree_attn_rows_kernel(Args p) {
+  constexpr int WR = kRowWaves, kPieces = D * TKV::kBytes / 16, kThreads = 64 * WR, kTile = kTileKeys * kPieces, kCopy = 2 * kTile / kThreads;
   static_assert(2 * kTile % kThreads == 0 && TKV::kBytes == 2, "whole pieces a thread");
   __shared__ typename Tree<W>::Shared tree_mem;
   __shared__ u32x4 key_mem[2][kTile], value_mem[2][kTile];
@@ -967,40 +969,75 @@ constexpr int most_tiles(int D, int q_bytes) { return (q_bytes == 4 ? 128 : 256)
 // The same where the waves share tiles, and hold none themselves.
 constexpr int rows_tiles(int D, int q_bytes) { return D == 128 && q_bytes == 4 ? 1 : 2; }
 
+// How a launch is laid out: every wave with keys of its own and all RT tiles of 16 query rows of its
+// block (tree_attn_kernel), or with RT tiles of its own and the block's keys (shared,
+// tree_attn_rows_kernel); one block a sequence (parts 0) or `parts` for all of them.
 struct Plan {
-  int parts, RT, WR, row_tiles, unit, least;
+  bool shared;
+  int parts, RT, row_tiles, unit, least;
+  double us;  // what it should take
 };
-Plan make_plan(const TreeAttn &a, int n_cu) {
+
+// The time of a layout: a block's start and end, and for every 2^unit keys `turn`, as often as a compute
+// unit has blocks (in pairs, those with shared tiles); dealing a sequence's keys
+// to several blocks adds a wait for the lengths, the second launch and its traffic.  The figures (us) are
+// those of launches that fill the card, right to about a tenth.  What they decide, over 3,000 | 300 rows:
+//   bf16, 4 x 16 heads of 64, 64 nodes            RT 1 22.6 | 6.6   RT 2 23.2 | 7.9    RT 4 20.8 | 10.4   shared 24.8 | 12.4
+//   bf16, 4 x 8 key heads of 128, 128 rows each   RT 1 35.1 | 8.7   RT 2 29.3 | 10.6   shared 31.2 | 16.2
+//   the same, 256 rows each                       RT 1 61.9 | 12.6  RT 2 35.8 | 11.0   shared 38.5 | 17.4
+//   fp32 over bf16, 2 x 20 heads of 64, 48 nodes  RT 1 22.2 | 7.1   RT 2 20.4 | 9.3    shared 27.6 | 16.7
+//   256 rows each, 12 sequences up to 8,191 rows  RT 2 232          shared 104
+// and fp32 caches, 20 heads of 64, 1,734 rows: 48 nodes RT 1 15, RT 2 18; 3 x 4 key heads, 189 rows each, up to
+// 5,936 rows 46, 43.
+Plan plan_of(const TreeAttn &a, int n_cu, int RT, bool shared) {
   Plan p;
-  const int M = a.n * (a.H / a.Hk), most = most_tiles(a.D, a.qt == kOpF32 ? 4 : 2);
-  p.WR = a.kvt == kOpF32 || M <= 64 ? 0 : M <= 128 ? 4 : 8;
-  if (p.WR > 0) {
-    p.RT = rows_tiles(a.D, a.qt == kOpF32 ? 4 : 2);
-    p.row_tiles = (M + 16 * p.RT * p.WR - 1) / (16 * p.RT * p.WR);
-    p.unit = 5, p.least = 8;
+  const int M = a.n * (a.H / a.Hk), per = 16 * RT * (shared ? kRowWaves : 1);
+  const bool wide = a.qt == kOpF32, d128 = a.D == 128;
+  p.shared = shared, p.RT = RT, p.row_tiles = (M + per - 1) / per;
+  p.unit = shared ? 5 : 7, p.least = shared ? 8 : 2;
+  double start, turn;
+  if (shared) {
+    start = d128 ? 10.0 : 8.5;
+    turn = wide ? (d128 ? 1.7 : 1.6) : d128 ? 1.6 : 0.95;
+  } else if (a.kvt == kOpF32) {
+    start = d128 ? 9.7 : 4.6 + 2.2 * RT;
+    turn = d128 ? 2.2 : 0.2 + 0.9 * RT;
   } else {
-    p.RT = a.n > 64 ? most : std::min(most, M <= 16 ? 1 : M <= 32 ? 2 : 4);
-    if (a.kvt == kOpF32 && M > 32 && M <= 48) p.RT = 1;  // (the fp32 products bound it: no empty fourth tile)
-    p.row_tiles = (M + 16 * p.RT - 1) / (16 * p.RT);
-    p.unit = 7, p.least = 2;
+    start = (wide ? 4.5 : 4.0) + (d128 ? 2.2 : 1.2) * RT;
+    turn = d128 ? 1.0 + 0.1 * RT : 0.63 + 0.08 * RT;
   }
+  const int at_once = n_cu * (shared ? 2 : 1), groups = a.Hk * p.row_tiles;
+  const double rows = std::max(1.0, (double)a.used * a.max_seq), units = std::ceil(rows / (1 << p.unit));
+  p.us = (start + units * turn) * (((int64_t)a.batch * groups + at_once - 1) / at_once);
   // A block a compute unit: 2 x 16 heads over 40,001 and 65,500 rows 86 us, two a unit 90, half as many
-  // 128; 12 x 8 key heads of 128 dims over 1,000 .. 8,191 rows 95, 111, 160.  Two of shared tiles and 4
-  // waves: 2 x 20 heads, 84 nodes over 15,765 rows 48 us, one a unit 62; 24 x 4 key heads, 72 rows over
+  // 128.  Two of shared tiles: 2 x 20 heads, 84 nodes over 15,765 rows 48 us, one a unit 62; 24 x 4 key heads, 72 rows over
   // 4,748 .. 5,359 58, 80.
-  p.parts = (int)std::min<int64_t>((p.WR == 4 ? 2 : 1) * n_cu / (a.Hk * p.row_tiles), 64ll * a.batch);
+  p.parts = (int)std::min<int64_t>(at_once / groups, 64ll * a.batch);
   // (row tiles with the same keys on the same eighth of the card, which has an L2 of its own: 6 heads of a
   // key head, 6 nodes, 2 x 52,834 rows 36 -> 29 us)
   if (p.row_tiles > 1 && p.parts > 8) p.parts -= p.parts % (8 / std::gcd(8, a.Hk));
-  // Sharing costs 4.5 us (the lengths waited for, the second launch), and takes off the part of a block's
-  // time that others take over.  Lengths are not known here: it has to pay at the part of max_seq that
-  // is used on average.  20 heads, 8 nodes, a bf16 cache, 512, 1,024, 2,048, 4,096 rows: alone 8, 11, 16, 26 us,
-  // shared 11, 11, 12, 13; fp32: 11, 16, 24, 46 and 12, 13, 13, 16; 8 sequences over bf16: 8, 12, 18, 29 and 12,
-  // 16, 22, 33.
-  const double alone = (p.WR > 0 ? 15.0 : a.kvt == kOpF32 ? 8.6 * p.RT : 3.5 + 0.9 * p.RT) * (a.D / 64) / 1024;  // us a row
-  const double taken = p.parts > a.batch ? 1.0 - (double)a.batch / p.parts : 0.0;
-  if (a.used * a.max_seq * alone * taken < 4.5) p.parts = 0;
+  // Lengths are not known here: dealing has to pay at the part of max_seq that is used on average.  20
+  // heads, 8 nodes, a bf16 cache of 512, 1,024, 2,048, 4,096 rows: one block 8, 11, 16, 26 us, dealt 11, 11, 12, 13; fp32:
+  // 11, 16, 24, 46 and 12, 13, 13, 16; 8 sequences over bf16: 8, 12, 18, 29 and 12, 16, 22, 33.
+  const double dealt = p.parts > a.batch ? start + 4.5 + std::max<double>(p.least, std::ceil(units * a.batch / p.parts)) * turn +
+                                               2e-6 * p.parts * a.H * a.n * a.D
+                                         : p.us;
+  if (dealt < p.us) p.us = dealt;
+  else p.parts = 0;
   return p;
+}
+Plan make_plan(const TreeAttn &a, int n_cu) {
+  const int bytes = a.qt == kOpF32 ? 4 : 2, most = most_tiles(a.D, bytes);
+  Plan best;
+  best.us = INFINITY;
+  auto offer = [&](int RT, bool shared) {
+    const Plan p = plan_of(a, n_cu, RT, shared);
+    if (p.us < best.us) best = p;
+  };
+  for (int rt = 1; rt <= most; rt *= 2)
+    if (a.n <= 64 || rt == std::min(most, 2)) offer(rt, false);  // (larger trees: one of them)
+  if (a.kvt != kOpF32) offer(rows_tiles(a.D, bytes), true);
+  return best;
 }
 
 size_t part_rows(const TreeAttn &a, const Plan &p) { return (size_t)a.H * a.n * p.parts; }
@@ -1019,30 +1056,19 @@ hipError_t launch_kernel(K kernel, int threads, const TreeAttn &a, const Plan &p
   hipLaunchKernelGGL((tree_join_kernel<D, TQ>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, args);
   return hipGetLastError();
 }
-template <int D, class TQ, class TKV, int RT>
-hipError_t launch_keys(const TreeAttn &a, const Plan &p, hipStream_t s) {
-  return launch_kernel<D, TQ>(tree_attn_kernel<D, TQ, TKV, RT, 1>, 64 * kKeyWaves, a, p, s);
-}
-template <int D, class TQ, class TKV, int WR>
-hipError_t launch_rows(const TreeAttn &a, const Plan &p, hipStream_t s) {
-  constexpr int kRT = rows_tiles(D, TQ::kBytes);
-  if (a.n > 64) return launch_kernel<D, TQ>(tree_attn_rows_kernel<D, TQ, TKV, kRT, 4, WR>, 64 * WR, a, p, s);
-  return launch_kernel<D, TQ>(tree_attn_rows_kernel<D, TQ, TKV, kRT, 1, WR>, 64 * WR, a, p, s);
-}
 template <int D, class TQ, class TKV>
 hipError_t launch_d(const TreeAttn &a, const Plan &p, hipStream_t s) {
-  constexpr int kMost = most_tiles(D, TQ::kBytes);
+  constexpr int kMost = most_tiles(D, TQ::kBytes), kRows = rows_tiles(D, TQ::kBytes), kKeyThreads = 64 * kKeyWaves;
   if constexpr (TKV::kBytes == 2) {
-    if (p.WR == 8) return launch_rows<D, TQ, TKV, 8>(a, p, s);
-    if (p.WR == 4) return launch_rows<D, TQ, TKV, 4>(a, p, s);
-  } else {
-    if (a.n > 64) return launch_kernel<D, TQ>(tree_attn_kernel<D, TQ, TKV, kMost, 4>, 64 * kKeyWaves, a, p, s);
+    if (p.shared && a.n > 64) return launch_kernel<D, TQ>(tree_attn_rows_kernel<D, TQ, TKV, kRows, 4>, 64 * kRowWaves, a, p, s);
+    if (p.shared) return launch_kernel<D, TQ>(tree_attn_rows_kernel<D, TQ, TKV, kRows, 1>, 64 * kRowWaves, a, p, s);
   }
+  if (a.n > 64) return launch_kernel<D, TQ>(tree_attn_kernel<D, TQ, TKV, std::min(kMost, 2), 4>, kKeyThreads, a, p, s);
   if constexpr (kMost >= 4)
-    if (p.RT == 4) return launch_keys<D, TQ, TKV, 4>(a, p, s);
+    if (p.RT == 4) return launch_kernel<D, TQ>(tree_attn_kernel<D, TQ, TKV, 4, 1>, kKeyThreads, a, p, s);
   if constexpr (kMost >= 2)
-    if (p.RT == 2) return launch_keys<D, TQ, TKV, 2>(a, p, s);
-  return launch_keys<D, TQ, TKV, 1>(a, p, s);
+    if (p.RT == 2) return launch_kernel<D, TQ>(tree_attn_kernel<D, TQ, TKV, 2, 1>, kKeyThreads, a, p, s);
+  return launch_kernel<D, TQ>(tree_attn_kernel<D, TQ, TKV, 1, 1>, kKeyThreads, a, p, s);
 }
 template <class TQ, class TKV>
 hipError_t launch_t(const TreeAttn &a, const Plan &p, hipStream_t s) {
