@@ -273,7 +273,7 @@ struct Args {
 // the sequences' lengths and however long the cache could become: the smallest one with which `parts`
 // blocks are enough (within a few percent).  Every wave finds it by itself from the lengths, a lane a
 // sequence.  12 x 64 nodes over 1,000 .. 8,191 rows, 8 key heads: 115 us with the rows of max_seq shared
-// equally, 106 with these.  A block still waits for the longest one, a fifth above the mean there; runs
+// equally, 107 with these.  A block still waits for the longest one, a fifth above the mean there; runs
 // that go on into the next sequence made that kernel 7 us faster and the one for few rows 1 to 10
 // slower (registers kept over the turns, a second start), and are not taken.
 struct Share {
@@ -769,10 +769,12 @@ __global__ __launch_bounds__(256, 2) void tree_attn_kernel(Args p) {
 // order p ^ row: what a wave reads at a time, one piece of 16 key rows or two neighbours of 16 value
 // rows, falls on different banks.  Values are read through the transposing load: lane 4 j + a of 16
 // reads elements 4 a .. of row j, and lane i gets element i of the four rows.
-// 12 x 64 nodes, 32 heads of 128 over 8 key heads, 1,000 .. 8,191 bf16 rows: 95 us, 490 TFLOP/s.  The matrix
-// units are busy 28% of that; the two waves of a SIMD share its issue with 120 vector and 50 other
-// instructions a tile.  Tiles two ahead spilled (161 us for 144 then); blocks of 8 waves read every
-// tile half as often and are no faster (103 us with the joining for 104; 2 x 144 nodes over 3,700 rows 38, 38).
+// 12 x 64 nodes, 32 heads of 128 over 8 key heads, 1,000 .. 8,191 bf16 rows: 98 us, 480 TFLOP/s.  The matrix
+// units are busy 38% of its cycles (at 1.65 GHz: the card lowers its clock under this load), the waves
+// wait a third of theirs for an issue slot and a third for data or the barrier.  Tiles two ahead in
+// registers spilled (161 us for 144 then), and two ahead by direct loads to LDS gain 4% at best; blocks of
+// 8 waves read every tile half as often and are no faster (103 us with the joining for 104; 2 x 144 nodes over
+// 3,700 rows 38, 38).
 template <int D, class TQ, class TKV, int RT, int W>
 __global__ __launch_bounds__(64 * kRowWaves, 2) void tree_attn_rows_kernel(Args p) {
   constexpr int WR = kRowWaves, kPieces = D * TKV::kBytes / 16, kThreads = 64 * WR, kTile = kTileKeys * kPieces, kCopy = 2 * kTile / kThreads;

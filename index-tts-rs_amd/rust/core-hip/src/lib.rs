@@ -127,6 +127,40 @@ pub struct TeacherForced {
     pub log_probs: Vec<f32>,
 }
 
+/// Scores of rows of logits, one row a code of a replay or a node of a drafted tree.
+#[derive(Clone, Debug, Default)]
+pub struct TokenScores {
+    /// Log-probability of every code given what precedes it (0 for a node that follows the sequence itself).
+    pub log_probs: Vec<f32>,
+    /// Entropy of every row, in nats.
+    pub entropy: Vec<f32>,
+    /// Row-major `[rows][top_n]`, the most probable first.
+    pub top_tokens: Vec<i32>,
+    /// Their log-probabilities.
+    pub top_log_probs: Vec<f32>,
+}
+
+impl TokenScores {
+    fn new(rows: usize, top_n: usize) -> Self {
+        Self {
+            log_probs: vec![0f32; rows],
+            entropy: vec![0f32; rows],
+            top_tokens: vec![0i32; rows * top_n],
+            top_log_probs: vec![0f32; rows * top_n],
+        }
+    }
+}
+
+/// Most alternatives a row's scores may name (`itts_token_scores`).
+const MAX_TOP: usize = 64;
+
+fn top_len(n: usize) -> Result<i32> {
+    if n > MAX_TOP {
+        return Err(IndexTtsError::validation("top_n", "at most 64 alternatives"));
+    }
+    i32_len(n, "top_n")
+}
+
 impl HipGpt {
     /// `Gpt::load_from_path` (gpt.rs:522): the library reads and validates
     /// `gpt_int8.safetensors` itself (header, names, shapes, dtypes).
@@ -221,6 +255,42 @@ impl HipGpt {
         Ok(log_probs)
     }
 
+    /// `code_log_probs` with the entropy of each code's row and its `top_n` most probable codes.
+    pub fn code_scores(&self, text_tokens: &[i32], conds: &[f32], lang_id: i32, codes: &[i32], top_n: usize,
+                       cache: &mut HipKvCache) -> Result<TokenScores> {
+        let top = top_len(top_n)?;
+        let mut out = TokenScores::new(codes.len(), top_n);
+        let n_cond = self.n_cond(conds)?;
+        // SAFETY: output buffers hold codes and codes * top_n values.
+        check(unsafe {
+            sys::itts_gpt_code_scores(self.raw, cache.raw, text_tokens.as_ptr(), i32_len(text_tokens.len(), "text_tokens")?,
+                                      conds.as_ptr(), n_cond, lang_id, codes.as_ptr(), i32_len(codes.len(), "codes")?, top,
+                                      out.log_probs.as_mut_ptr(), out.entropy.as_mut_ptr(), out.top_tokens.as_mut_ptr(),
+                                      out.top_log_probs.as_mut_ptr())
+        })?;
+        Ok(out)
+    }
+
+    /// One step for a tree of drafted codes behind the cache's rows: `tokens[i]` follows
+    /// `tokens[parents[i]]` (-1: the cached sequence) at position `pos_idx` plus its depth.
+    /// `HipKvCache::keep` then takes the accepted nodes.
+    pub fn step_tree(&self, cache: &mut HipKvCache, tokens: &[i32], parents: &[i32], pos_idx: i32, top_n: usize)
+                     -> Result<(Vec<f32>, TokenScores)> {
+        if tokens.len() != parents.len() {
+            return Err(IndexTtsError::validation("parents", "one parent a token expected"));
+        }
+        let (n, top) = (i32_len(tokens.len(), "n_nodes")?, top_len(top_n)?);
+        let mut logits = vec![0f32; tokens.len() * MEL_VOCAB];
+        let mut out = TokenScores::new(tokens.len(), top_n);
+        // SAFETY: logits holds n * MEL_VOCAB floats, the scores n and n * top_n values.
+        check(unsafe {
+            sys::itts_gpt_step_tree(self.raw, cache.raw, tokens.as_ptr(), parents.as_ptr(), n, pos_idx, top,
+                                    logits.as_mut_ptr(), out.log_probs.as_mut_ptr(), out.entropy.as_mut_ptr(),
+                                    out.top_tokens.as_mut_ptr(), out.top_log_probs.as_mut_ptr())
+        })?;
+        Ok((logits, out))
+    }
+
     /// `Gpt::alignment_attention` (gpt.rs:875).
     pub fn alignment_attention(&self, text_tokens: &[i32], conds: &[f32], lang_id: i32, prior_codes: &[i32],
                                codes: &[i32], cache: &mut HipKvCache) -> Result<Vec<f32>> {
@@ -255,6 +325,12 @@ impl HipKvCache {
     pub fn reset(&mut self) {
         // SAFETY: self.raw is a live handle.
         unsafe { sys::itts_kv_reset(self.raw) }
+    }
+
+    /// Keeps a path of the last drafted tree (its nodes from the first one down); an empty one drops the tree.
+    pub fn keep(&mut self, nodes: &[i32]) -> Result<()> {
+        // SAFETY: self.raw is a live handle; nodes is valid for its length.
+        check(unsafe { sys::itts_kv_keep(self.raw, nodes.as_ptr(), i32_len(nodes.len(), "nodes")?) })
     }
 
     /// `KvCache::valid_len` (gpt.rs:137).
