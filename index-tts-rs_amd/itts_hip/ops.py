@@ -15,6 +15,7 @@ each function.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from typing import NamedTuple, Optional
 
 import torch
@@ -54,26 +55,45 @@ def _tensor(t, name: str, dims: int, device=None, dtype=None, last=False):
     return strides
 
 
-# The current stream's handle without a Stream object around it (2 us of a call's host time).
+# Host time is most of a small call.  The current stream's handle without a Stream object around it saves
+# 2 us, a new tensor without torch.empty's reading of its arguments 0.5 to 0.9 (of 1.3 to 1.6).
 _stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+try:
+    from torch._C._dynamo.guards import _empty_strided_cuda as _empty
+except ImportError:
+    def _empty(shape, strides, dtype):
+        return torch.empty_strided(shape, strides, dtype=dtype, device="cuda")
+
+
+def _on_device(op):
+    """Runs an operator with its first tensor's device as the current one."""
+    name = op.__code__.co_varnames[0]
+
+    @functools.wraps(op)
+    def run(*args, **kwargs):
+        t = args[0] if args else kwargs.get(name)
+        if isinstance(t, torch.Tensor) and t.is_cuda and t.device.index != torch.cuda.current_device():
+            with torch.cuda.device(t.device):
+                return op(*args, **kwargs)
+        return op(*args, **kwargs)
+    return run
 
 
 def _run(fn, need, args, device):
-    """Enqueues on the device's current stream, with the workspace that the sizes need."""
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            return _run(fn, need, args, device)
+    """Enqueues on the current device's stream, with the workspace that the sizes need."""
     ref = C.byref(args)
     if need is None:
         return _check(fn(ref, _stream(device.index)))
     size = C.c_uint64()
     _check(need(ref, C.byref(size)))
-    if not size.value:
+    bytes_ = size.value
+    if not bytes_:
         return _check(fn(ref, None, 0, _stream(device.index)))
-    ws = torch.empty(size.value, dtype=torch.uint8, device=device)
-    _check(fn(ref, ws.data_ptr(), size, _stream(device.index)))
+    ws = _empty((bytes_,), (1,), torch.uint8)
+    _check(fn(ref, ws.data_ptr(), bytes_, _stream(device.index)))
 
 
+@_on_device
 def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: torch.Tensor, parents: torch.Tensor, *,
                    scale: Optional[float] = None, max_length: Optional[int] = None,
                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -115,8 +135,8 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: t
             _refuse(f"max_length: the caches have {rows} rows, got {int(max_length)}")
         rows = int(max_length)
     if out is None:
-        out = q.new_empty((b, n, h, d))
         so = (n * h * d, h * d, d)
+        out = _empty((b, n, h, d), (*so, 1), q.dtype)
     else:
         so = _tensor(out, "out", 4, dev, q.dtype, last=True)
         if out.shape != q.shape:
@@ -136,6 +156,7 @@ class TokenScores(NamedTuple):
     top_log_probs: torch.Tensor            # [rows][top_n] float32
 
 
+@_on_device
 def token_scores(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, top_n: int = 0) -> TokenScores:
     """Scores of rows of logits [rows][vocab] (float32, bfloat16 or float16; rows any distance apart).
 
@@ -156,21 +177,22 @@ def token_scores(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, to
         if tokens.shape[0] != r:
             _refuse(f"tokens: {r} rows expected, got {tokens.shape[0]}")
         given, tok_row = 1 if one else tokens.shape[1], st[0]
-        log_probs = torch.empty(tokens.shape, dtype=torch.float32, device=dev)
+        log_probs = _empty((r,) if one else (r, given), (1,) if one else (given, 1), torch.float32)
         if given:
             tok, log_probs_at = tokens.data_ptr(), log_probs.data_ptr()
     top_n = int(top_n)
     if not 0 <= top_n <= min(64, vocab):
         _refuse(f"top_n: must be in 0..=64 and at most the vocabulary of {vocab}, got {top_n}")
-    entropy = torch.empty(r, dtype=torch.float32, device=dev)
-    top_tokens = torch.empty((r, top_n), dtype=torch.int32, device=dev)
-    top_log_probs = torch.empty((r, top_n), dtype=torch.float32, device=dev)
+    entropy = _empty((r,), (1,), torch.float32)
+    top_tokens = _empty((r, top_n), (top_n, 1), torch.int32)
+    top_log_probs = _empty((r, top_n), (top_n, 1), torch.float32)
     a = itts_token_scores_args(logits.data_ptr(), tok, log_probs_at, entropy.data_ptr(), top_tokens.data_ptr(),
                                top_log_probs.data_ptr(), r, vocab, given, top_n, _DTYPES[logits.dtype], sx[0], tok_row)
     _run(lib.itts_token_scores, lib.itts_token_scores_workspace, a, dev)
     return TokenScores(log_probs, entropy, top_tokens, top_log_probs)
 
 
+@_on_device
 def cache_keep(k: torch.Tensor, v: torch.Tensor, lengths: torch.Tensor, path: torch.Tensor) -> torch.Tensor:
     """Keeps the accepted nodes of a tree: rows lengths[b] + path[b][i] of k and v [layers][batch][heads][rows][dim]
     (or [batch][heads][rows][dim]) move, in place, to rows lengths[b] + i in every layer and head.
@@ -197,7 +219,7 @@ def cache_keep(k: torch.Tensor, v: torch.Tensor, lengths: torch.Tensor, path: to
         _refuse(f"lengths, path: {b} sequences expected, got {lengths.shape[0]} and {path.shape[0]}")
     if b > 1 and sl[0] != 1:
         _refuse("lengths: must be contiguous")
-    new = torch.empty(b, dtype=torch.int32, device=dev)
+    new = _empty((b,), (1,), torch.int32)
     a = itts_cache_keep_args(k.data_ptr(), v.data_ptr(), lengths.data_ptr(), path.data_ptr(), new.data_ptr(), layers, b, h,
                              rows, d, path.shape[1], _DTYPES[k.dtype], sk[0], sk[1], sk[2], sk[3], sv[0], sv[1], sv[2], sv[3],
                              sp[0])

@@ -547,3 +547,18 @@ def test_gpu_refusals(ops):
     a = H.itts_token_scores_args(host.data_ptr(), None, None, None, None, None, 2, 9, 0, 0, H.ITTS_F32, 9, 0)
     refuses("logits: not device memory", lambda: H._check(H.lib.itts_token_scores(C.byref(a), None, 0, None)))
     assert ops.token_scores(torch.zeros(2, 9, device="cuda")).entropy.shape == (2,)  # and the next call works
+
+
+def test_arguments_by_name(ops):
+    """Every argument by its name, in any order."""
+    say("[gpu] arguments by name")
+    g = gen(77)
+    q, k, v = randn(g, 2, 3, 4, 64), randn(g, 2, 2, 20, 64), randn(g, 2, 2, 20, 64)
+    lengths, parents = ints([4, 9]), ints([[-1, 0, 1]] * 2)
+    assert torch.equal(ops.tree_attention(parents=parents, lengths=lengths, v=v, k=k, q=q), ops.tree_attention(q, k, v, lengths, parents))
+    x = randn(g, 5, 70)
+    one, other = ops.token_scores(top_n=3, logits=x), ops.token_scores(x, None, 3)
+    assert torch.equal(one.entropy, other.entropy) and torch.equal(one.top_tokens, other.top_tokens)
+    path = ints([[1, 2], [0, -1]])
+    k2, v2 = k.unsqueeze(0).clone(), v.unsqueeze(0).clone()
+    assert ops.cache_keep(path=path, lengths=lengths, v=v2, k=k2).tolist() == [6, 10]
