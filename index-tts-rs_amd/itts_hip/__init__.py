@@ -225,19 +225,32 @@ _SIGS = {
 EXPORTED_SYMBOLS = tuple(_SIGS)
 
 
-def _load():
-    if not os.path.exists(LIB_PATH):
-        raise ImportError(f"libitts_hip is not built: {LIB_PATH} is missing "
-                          "(run __graft_entry__.build() or make -C index-tts-rs_amd)")
-    lib = C.CDLL(LIB_PATH)
-    for name, (res, args) in _SIGS.items():
-        fn = getattr(lib, name)
-        fn.restype = res
-        fn.argtypes = args
-    return lib
+if not os.path.exists(LIB_PATH):
+    raise ImportError(f"libitts_hip is not built: {LIB_PATH} is missing "
+                      "(run __graft_entry__.build() or make -C index-tts-rs_amd)")
 
 
-lib = _load()
+class _Library:
+    """The library's functions, loaded with the first one that is asked for.  torch brings a HIP runtime of
+    its own, which the library uses if torch is there before it; the other way round a process would
+    have two, and only the first finds the GPU."""
+
+    def load(self):
+        lib = C.CDLL(LIB_PATH)
+        for name, (res, args) in _SIGS.items():
+            fn = getattr(lib, name)
+            fn.restype = res
+            fn.argtypes = args
+            setattr(self, name, fn)
+
+    def __getattr__(self, name):
+        if name not in _SIGS:
+            raise AttributeError(name)
+        self.load()
+        return self.__dict__[name]
+
+
+lib = _Library()
 
 
 def _check(status: int):

@@ -11,17 +11,38 @@ calls on several streams, and captured ones, share nothing.  No gradients: the t
 decoding.  Wrong arguments raise ``ValidationError`` naming the argument; what the operators do with
 lengths, parents, paths and tokens that are out of range (the host cannot see them) is written at
 each function.
+
+Import this module, or torch, before the library's first call (a decoder's, say): they have to share a HIP
+runtime, and an ImportError says so when they do not.
 """
 from __future__ import annotations
 
 import ctypes as C
 import functools
+import os
 from typing import NamedTuple, Optional
 
 import torch
 
 from . import (ITTS_BF16, ITTS_E_VALIDATION, ITTS_F16, ITTS_F32, ValidationError, _check, itts_cache_keep_args,
                itts_token_scores_args, itts_tree_attention_args, lib)
+
+
+
+def _one_runtime():
+    """Loads the library, and refuses a process with two HIP runtimes: the second one finds no GPU."""
+    lib.load()
+    try:
+        with open("/proc/self/maps") as f:
+            found = {os.path.realpath(line.split(maxsplit=5)[5].strip()) for line in f if "libamdhip64" in line}
+    except OSError:
+        return
+    if len(found) > 1:
+        raise ImportError(f"torch and libitts_hip use different HIP runtimes ({', '.join(sorted(found))}): import torch or "
+                          "itts_hip.ops before the library's first call")
+
+
+_one_runtime()
 
 _DTYPES = {torch.float32: ITTS_F32, torch.bfloat16: ITTS_BF16, torch.float16: ITTS_F16}
 

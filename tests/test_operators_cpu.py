@@ -1,6 +1,9 @@
 """Refusals of the operators on device memory, without a GPU: wrong sizes, types, strides and
 alignments at the C entries, and wrong tensors at the Python ones."""
 import ctypes as C
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -8,6 +11,7 @@ import torch
 import itts_hip as H
 from itts_hip import ops
 
+PKG = os.path.dirname(os.path.dirname(H.__file__))
 P = 1 << 20  # an address that nothing reads: every call below is refused before its memory matters
 
 
@@ -114,3 +118,17 @@ def test_python_entries_refuse():
 def test_c_entries_refuse_overlaps_and_sizes_past_a_grid(kind, field, over):
     """One memory as keys and as values under two layouts; more blocks than a launch has."""
     test_c_entries_refuse(kind, field, over)
+
+
+@pytest.mark.parametrize("first", ["from itts_hip import ops; H.version()", "H.version(); from itts_hip import ops"])
+def test_one_hip_runtime_or_a_refusal(first):
+    """The library loads with its first call and then shares torch's HIP runtime; called before torch is there it has
+    its own, and the operators say so (unless that is torch's too)."""
+    code = (f"import sys; sys.path.insert(0, {PKG!r})\nimport itts_hip as H\nassert 'amdhip64' not in open('/proc/self/maps').read()\n"
+            f"{first}\n"
+            "print(len({l.split()[5] for l in open('/proc/self/maps') if 'libamdhip64' in l}))")
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    if first.startswith("from"):
+        assert r.returncode == 0 and r.stdout.split()[-1] == "1", r.stdout + r.stderr
+    else:
+        assert (r.returncode == 0 and r.stdout.split()[-1] == "1") or "different HIP runtimes" in r.stderr, r.stdout + r.stderr
