@@ -255,6 +255,49 @@ def test_attention_past_32_bits(ops):
     check(ops.tree_attention(q, big_k, v, ln, par), *attention_ref(q, big_k, v, ln, par))
 
 
+@pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("n,h,hk,d,rows,lengths", [
+    (1, 2, 1, 64, 24000, [(i * 7919) % 23990 if i % 3 else i % 5 - 1 for i in range(150)]),  # more sequences than lanes
+    (3, 2, 2, 64, 9000, [8990] + [0] * 20), (3, 2, 2, 64, 9000, [0, -1, 7, 31, 8997, 8998, 2 ** 31 - 1]),
+    (20, 8, 2, 128, 9000, [1, 8000, 333, 4096, 2500]), (64, 8, 2, 128, 6000, [5900, 17, 3001]), (130, 2, 2, 64, 7000, [6850, 64, 1700]),
+])
+def test_attention_keys_dealt_to_blocks(ops, types, n, h, hk, d, rows, lengths):
+    """Sequences of any lengths over one cache (stride 0 between them) that is long enough for its keys to be
+    dealt to a launch's blocks in equal parts: parts that end inside tiles and sequences, sequences of one
+    part, of many, without rows, and ones that do not fit."""
+    say(f"[gpu] tree attention dealt {types} n={n} h={h}/{hk} d={d} {len(lengths)} lengths")
+    b, (q, kv) = len(lengths), types
+    g = gen(b + n)
+    x = (1.5 * randn(g, b, n, h, d)).to(q)
+    k, v = (randn(g, 1, hk, rows, d, dtype=kv).expand(b, -1, -1, -1) for _ in range(2))
+    par = ints([shape_tree("tree", n, i) for i in range(b)])
+    got = ops.tree_attention(x, k, v, ints(lengths), par)
+    some = sorted(set(range(0, b, max(1, b // 12))) | {b - 1})  # (the reference goes row by row)
+    check(got[some][:, ::9], *(t[:, ::9] for t in attention_ref(x[some], k[some], v[some], [lengths[i] for i in some], par[some])))
+    for i, length in enumerate(lengths):
+        assert torch.isnan(got[i]).all() == (length < 0 or length + n > rows)
+
+
+def test_attention_graph_follows_lengths(ops):
+    """A captured launch deals its keys by the lengths of each replay."""
+    say("[gpu] tree attention: lengths change under a graph")
+    g = gen(12)
+    q, k, v = randn(g, 3, 5, 4, 64), randn(g, 3, 2, 12000, 64, dtype=BF16), randn(g, 3, 2, 12000, 64, dtype=BF16)
+    par, ln = ints([shape_tree("tree", 5, i) for i in range(3)]), ints([11000, 5, 6000])
+    ops.tree_attention(q, k, v, ln, par)
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        out = ops.tree_attention(q, k, v, ln, par)
+    for lengths in ([0, 0, 0], [11995, 11995, 11995], [1, -1, 900], [11996, 3, 40], [11000, 5, 6000]):
+        ln.copy_(ints(lengths))
+        want = ops.tree_attention(q, k, v, ln, par)
+        gr.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out.nan_to_num(7.0), want.nan_to_num(7.0)), lengths
+        check(out, *attention_ref(q, k, v, lengths, par))
+
+
 # ---- scores --------------------------------------------------------------------------------
 def scores_ref(x, tokens, top):
     x = x.double().cpu()
@@ -309,6 +352,21 @@ def test_scores_match_float64(ops, dtype, r, v, given, top):
     x = logits(g, r, v, dtype)
     tokens = torch.randint(0, v, (r, given), generator=g, device="cuda").int()
     scores_check(ops.token_scores(x, tokens, top), x, tokens, top)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("v", [17001, 33000])
+def test_scores_of_many_long_rows(ops, dtype, v):
+    """Rows that one block reads in several turns, and whose best tokens come first, last or in between."""
+    say(f"[gpu] scores of 600 rows of {v} {dtype}")
+    g = gen(v)
+    x = logits(g, 600, v, dtype)
+    ramp = torch.linspace(0, 12, v, device="cuda")
+    x[0], x[1], x[2], x[3] = ramp.to(dtype), (-ramp).to(dtype), -(ramp - 6).abs().to(dtype), (ramp - 6).abs().to(dtype)
+    x[4] = -INF
+    x[4, -1], x[4, 8200] = 1.0, 2.0
+    tokens = torch.randint(0, v, (600, 2), generator=g, device="cuda").int()
+    scores_check(ops.token_scores(x, tokens, 12), x, tokens, 12)
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
