@@ -12,7 +12,7 @@
 // against each other.  Rows that are few and long are split over blocks and joined by a second
 // kernel.  Bound by instructions, 12 an element (one of them the exponential), where memory would
 // take half to three quarters of the time: 2,188 fp32 rows of 8,194 with 5 alternatives 19 us (72 MB), 1,000 bf16
-// rows of 60,510 with 20 50 us (121 MB); one row of 8,194 6.2 us.
+// rows of 60,510 with 20 48 us (121 MB); one row of 8,194 6.2 us.
 #include <algorithm>
 
 #include "kernels.h"
@@ -127,6 +127,7 @@ struct Select {
   uint64_t list[kList + kScoresMaxTop];
   uint64_t top[kScoresMaxTop];
   uint32_t bound[kWaves];
+  int hot[2][kWaves];
   int count;
 };
 
@@ -190,7 +191,8 @@ __device__ inline void write_row(const TokenScores &a, int r, const void *x, con
 __host__ __device__ inline size_t list_offset(int rows, int S) { return sizeof(Stats) * (size_t)rows * S; }
 
 // LONG: a block's tokens are more than its threads hold, and the next ones are on their way while these
-// are counted: 1,000 rows of 60,510 50 us, without 54 (also with half the registers and more blocks a unit).
+// are counted: 1,000 rows of 60,510 50 us, without 54 (also with half the registers and more blocks a unit), and 48
+// since later turns look for tokens above the n-th so far alone.
 template <int TYPE, bool LONG>
 __global__ __launch_bounds__(kThreads, LONG ? 4 : 6) void token_scores_kernel(TokenScores a, int S) {
   __shared__ float red[kWaves][4];
@@ -271,18 +273,38 @@ __global__ __launch_bounds__(kThreads, LONG ? 4 : 6) void token_scores_kernel(To
       put_stats(u, red);
     }
 
-    if (n > 0 && !ranked) {
-      // A bound for the n-th largest: ceil(n / 4) threads of every wave reach it.  (-inf has no part in
-      // this: a row's last places go to masked tokens at the end.)
-      const uint32_t share = reached(u.m > -INFINITY ? order(u.m) : 0, (n + kWaves - 1) / kWaves);
-      if constexpr (LONG) __syncthreads();  // (the last round's are read)
-      if ((t & 63) == 0) sel.bound[t >> 6] = share;
-      __syncthreads();
-      uint32_t low = ~0u;
+    uint32_t bound = kOrderNone + 1;
+    const uint32_t own = u.m > -INFINITY ? order(u.m) : 0;
+    bool any = n > 0 && !ranked, narrow = any;
+    if constexpr (LONG) {
+      // A token has to come before the n-th so far: to be larger, or as large where that one is of the row's
+      // rest, whose tokens are the last.  Where few threads have one, that is bound enough.
+      if (any) {
+        if (base > 0) {
+          const uint64_t worst = sel.top[n - 1];  // (0 before n are found)
+          bound = max(bound, (uint32_t)(worst >> 32) + (key_token(worst) < i1 - rest ? 1u : 0u));
+        }
+        int *hot = sel.hot[base / (kThreads * kPieces) & 1];
+        const uint64_t here = __ballot(own >= bound);
+        if ((t & 63) == 0) hot[t >> 6] = __popcll(here);
+        __syncthreads();
+        int threads = 0;
 #pragma unroll
-      for (int w = 0; w < kWaves; w++) low = min(low, sel.bound[w]);
-      const uint64_t worst = LONG ? sel.top[n - 1] : 0;  // (0 before n are found)
-      const uint32_t bound = max(max(low, (uint32_t)(worst >> 32)), kOrderNone + 1);
+        for (int w = 0; w < kWaves; w++) threads += hot[w];
+        any = threads > 0, narrow = threads > 64;
+      }
+    }
+    if (any) {
+      // (-inf has no part in this: a row's last places go to masked tokens at the end)
+      if (narrow) {  // a bound for the n-th largest: ceil(n / 4) threads of every wave reach it
+        const uint32_t share = reached(own, (n + kWaves - 1) / kWaves);
+        if ((t & 63) == 0) sel.bound[t >> 6] = share;
+        __syncthreads();
+        uint32_t low = ~0u;
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) low = min(low, sel.bound[w]);
+        bound = max(bound, low);
+      }
       const float least = unorder(bound);
       auto offer = [&](float y, int token) {
         if (!(y >= least)) return;
@@ -298,8 +320,7 @@ __global__ __launch_bounds__(kThreads, LONG ? 4 : 6) void token_scores_kernel(To
       }
       if (has_odd) offer(odd_x, odd);
       __syncthreads();
-      const int count = sel.count;
-      if constexpr (LONG) __syncthreads();  // (it grows below)
+      const int count = sel.count;  // (with what was found before)
       if (count > kList) {
         // Ties by the thousand, or the largest all in a few threads: n rounds of the largest that
         // is left, over all of this block's tokens in memory.
@@ -318,18 +339,12 @@ __global__ __launch_bounds__(kThreads, LONG ? 4 : 6) void token_scores_kernel(To
         if (t < n) sel.top[t] = mine;
         ranked = true;
       } else if (count > 0) {
-        int have = count;
+        rank_list(sel, count, n);
         if constexpr (LONG) {
-          if (t < n) {
-            const uint64_t k = sel.top[t];  // what was found before joins the list
-            if (k) sel.list[atomicAdd(&sel.count, 1)] = k;
-          }
-          __syncthreads();
-          have = sel.count;
+          if (t < n) sel.list[t] = sel.top[t];
+          if (t == 0) sel.count = min(count, n);
         }
-        rank_list(sel, have, n);
       }
-      if (LONG && t == 0) sel.count = 0;
     }
     if constexpr (!LONG) break;
 #pragma unroll

@@ -365,6 +365,12 @@ def test_scores_of_many_long_rows(ops, dtype, v):
     x[0], x[1], x[2], x[3] = ramp.to(dtype), (-ramp).to(dtype), -(ramp - 6).abs().to(dtype), (ramp - 6).abs().to(dtype)
     x[4] = -INF
     x[4, -1], x[4, 8200] = 1.0, 2.0
+    # the twelfth is one of three alike: the row's last token, which is read in the first turn, and two of later ones
+    x[5:8] = -5.0
+    x[5:8, 100:111], x[5:8, -1] = 10.0, 3.0
+    x[6, 16900], x[7, 16500:16510] = 3.0, 3.0
+    # the same value in every place but the first turn's
+    x[8], x[9, :16384], x[9, 16384:] = 1.0, 0.0, 1.0
     tokens = torch.randint(0, v, (600, 2), generator=g, device="cuda").int()
     scores_check(ops.token_scores(x, tokens, 12), x, tokens, 12)
 
