@@ -322,6 +322,9 @@ struct TreeAttn {
   int64_t q_b, q_n, q_h, o_b, o_n, o_h, k_b, k_h, k_r, v_b, v_h, v_r, par_b;
   float *part;  // tree_attn_ws(a, n_cu) floats
   float used = 0.5f;  // of max_seq, by an average sequence
+  // with planes.hi set (fp32 queries, D 64) the results [batch n][H 64] go there instead of `out`, as the
+  // operand of the product that follows
+  SplitOut planes{};
 };
 size_t tree_attn_ws(const TreeAttn &a, int n_cu);
 hipError_t tree_attn(const TreeAttn &a, int n_cu, hipStream_t s);

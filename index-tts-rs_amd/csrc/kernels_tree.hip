@@ -626,22 +626,54 @@ __device__ inline void odd_values(float *y, const Seen &seen, int live, const ch
   }
 }
 
+// Four elements d .. of a row's result to the output, or to the planes (their sum comes back).
+template <int D, class TQ>
+__device__ __forceinline__ float put_result(const Args &p, int b, int hk, int row, int node, int d, const float *y) {
+  const TreeAttn &a = p.a;
+  const int head = hk * p.group + (row - node * p.group);
+  if constexpr (D == 64 && std::is_same_v<TQ, F32>) {
+    if (a.planes.hi) {
+      const size_t at = (((size_t)b * a.n + node) * a.H + head) * 64 + d;
+      uint32_t h0, l0, h1, l1;
+      split_f16x2(y[0], y[1], h0, l0);
+      split_f16x2(y[2], y[3], h1, l1);
+      *reinterpret_cast<uint2 *>(a.planes.hi + at) = make_uint2(h0, h1);
+      *reinterpret_cast<uint2 *>(a.planes.lo + at) = make_uint2(l0, l1);
+      return (y[0] + y[1]) + (y[2] + y[3]);
+    }
+  }
+  const int64_t at = b * a.o_b + node * a.o_n + head * a.o_h + d;
+  store4<TQ>(static_cast<char *>(a.out) + at * TQ::kBytes, y[0], y[1], y[2], y[3]);
+  return 0.0f;
+}
+// The planes' sum of a row.
+template <int D, class TQ>
+__device__ __forceinline__ void put_sum(const Args &p, int b, int hk, int row, int node, float sum) {
+  if constexpr (D == 64 && std::is_same_v<TQ, F32>)
+    p.a.planes.gs[((size_t)b * p.a.n + node) * p.a.H + hk * p.group + (row - node * p.group)] = sum;
+}
+template <int D, class TQ>
+__device__ __forceinline__ bool has_planes(const Args &p) {
+  return D == 64 && std::is_same_v<TQ, F32> && p.a.planes.hi;
+}
+
 // Four elements d .. of a row's result over this block's keys, to the output or the splits' results.
 // What the joining kernel cannot tell by itself goes with the statistics: a row that sees nothing
 // has maximum +inf and sum 0, one of a bad sequence sum NaN.
+// Returns the sum of what went to the planes.
 template <int D, class TQ>
-__device__ __forceinline__ void put4(const Args &p, const Share &share, int hk, int row, int node, int d, float *y, float top,
-                                     float sum, bool bad, bool any, bool keys) {
+__device__ __forceinline__ float put4(const Args &p, const Share &share, int hk, int row, int node, int d, float *y, float top,
+                                      float sum, bool bad, bool any, bool keys) {
   if (share.n == 1) {
     const float inv = 1.0f / sum;
 #pragma unroll
     for (int e = 0; e < 4; e++) y[e] = bad ? NAN : any ? y[e] * inv : 0.0f;
-    const int64_t at = share.b * p.a.o_b + node * p.a.o_n + (hk * p.group + (row - node * p.group)) * p.a.o_h + d;
-    store4<TQ>(static_cast<char *>(p.a.out) + at * TQ::kBytes, y[0], y[1], y[2], y[3]);
+    return put_result<D, TQ>(p, share.b, hk, row, node, d, y);
   } else {
     const size_t at = ((size_t)hk * p.M + row) * p.parts + share.index;
     if (keys) *reinterpret_cast<float4 *>(p.a.part + at * D + d) = make_float4(y[0], y[1], y[2], y[3]);
     if (d == 0) p.ml[at] = bad ? make_float2(0.0f, NAN) : any ? make_float2(top, sum) : make_float2(INFINITY, 0.0f);
+    return 0.0f;
   }
 }
 
@@ -758,7 +790,12 @@ __global__ __launch_bounds__(256, 2) void tree_attn_kernel(Args p) {
       y[0] += f * v.x, y[1] += f * v.y, y[2] += f * v.z, y[3] += f * v.w;
     }
     if (odd_any) odd_values<TKV, 4>(y, seen, live, vb + (uint64_t)(uint32_t)len * v_step + d * TKV::kBytes, v_step);
-    put4<D, TQ>(p, share, hk, row, i_node, d, y, top, sum, bad, seen.any(), share.first < total);
+    float planes = put4<D, TQ>(p, share, hk, row, i_node, d, y, top, sum, bad, seen.any(), share.first < total);
+    if (has_planes<D, TQ>(p) && share.n == 1) {  // (a row's D / 4 lanes are neighbours)
+#pragma unroll
+      for (int step = 1; step < D / 4; step *= 2) planes += __shfl_xor(planes, step, 64);
+      if (d == 0) put_sum<D, TQ>(p, b, hk, row, i_node, planes);
+    }
   }
 }
 
@@ -907,12 +944,17 @@ __global__ __launch_bounds__(64 * kRowWaves, 2) void tree_attn_rows_kernel(Args 
   for (int t = 0; t < RT; t++) {
     const int row = row0 + 16 * t + c;
     if (row >= p.M) continue;
+    float planes = 0.0f;
 #pragma unroll
     for (int d = 0; d < D / 16; d++) {  // lane (c, g) holds dims 16 d + 4 g .. of row c
       float y[4] = {rows.o[t][d][0], rows.o[t][d][1], rows.o[t][d][2], rows.o[t][d][3]};
       const int e = 16 * d + 4 * g;
       if (odd_any) odd_values<TKV, 4>(y, sees[t], live, vb + (uint64_t)(uint32_t)len * v_step + e * TKV::kBytes, v_step);
-      put4<D, TQ>(p, share, hk, row, rows.node[t], e, y, rows.m[t], rows.l[t][0], bad, sees[t].any(), keys);
+      planes += put4<D, TQ>(p, share, hk, row, rows.node[t], e, y, rows.m[t], rows.l[t][0], bad, sees[t].any(), keys);
+    }
+    if (has_planes<D, TQ>(p) && share.n == 1) {
+      planes = col_sum(planes);
+      if (g == 0) put_sum<D, TQ>(p, b, hk, row, rows.node[t], planes);
     }
   }
 }
@@ -961,8 +1003,12 @@ __global__ __launch_bounds__(256) void tree_join_kernel(Args p) {
 #pragma unroll
   for (int e = 0; e < 4; e++) x[e] = none ? 0.0f : x[e] * inv;
   const int node = p.node(row);
-  const int64_t to = b * a.o_b + node * a.o_n + (hk * p.group + (row - node * p.group)) * a.o_h + d;
-  store4<TQ>(static_cast<char *>(a.out) + to * TQ::kBytes, x[0], x[1], x[2], x[3]);
+  float planes = put_result<D, TQ>(p, b, hk, row, node, d, x);
+  if (has_planes<D, TQ>(p)) {
+#pragma unroll
+    for (int step = 1; step < kLanes; step *= 2) planes += __shfl_xor(planes, step, 64);
+    if (d == 0) put_sum<D, TQ>(p, b, hk, row, node, planes);
+  }
 }
 
 // Most tiles of 16 query rows a wave takes: as many as its registers hold (256 a lane, two waves a
@@ -1129,6 +1175,7 @@ hipError_t tree_attn(const TreeAttn &a, int n_cu, hipStream_t s) {
   if (a.n > kTreeMaxNodes || (a.D != 64 && a.D != 128) || a.H % a.Hk) return hipErrorInvalidValue;
   const Plan p = make_plan(a, n_cu);
   if (p.parts > 0 && !a.part) return hipErrorInvalidValue;
+  if (a.planes.hi && (a.D != 64 || a.qt != kOpF32)) return hipErrorInvalidValue;
   if (a.qt == kOpF32 && a.kvt == kOpF32) return launch_t<F32, F32>(a, p, s);
   if (a.qt == kOpF32 && a.kvt == kOpBf16) return launch_t<F32, Bf16>(a, p, s);
   if (a.qt == kOpBf16 && a.kvt == kOpBf16) return launch_t<Bf16, Bf16>(a, p, s);

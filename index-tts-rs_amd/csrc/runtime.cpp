@@ -235,8 +235,8 @@ struct itts_gpt {
   DevBuf bx, bq, blog, bseqs, bps;
   SplitBuf bh, ba, bf;
   // drafted trees: the upload (tokens, positions, parents, length, given tokens) and its staging, the
-  // nodes' control blocks, attention rows (fp32) and split partials; scores and their workspace
-  DevBuf tin, tctl, tattn, tpart, tscore, tsws;
+  // nodes' control blocks and the attention's workspace; scores and their workspace
+  DevBuf tin, tctl, tpart, tscore, tsws;
   HostStage h_tree;
   // sampler API scratch
   DevBuf s_logits, s_seen, s_rng, s_tok;
@@ -866,7 +866,7 @@ struct TreeStep {
   const itts_kv *kv;
   const int32_t *parents, *length;  // device
 };
-// The attention of layer l over the n nodes' queries in gpt->bq, into gpt->tattn [n][d].
+// The attention of layer l over the n nodes' queries in gpt->bq, into gpt->ba [n][d].
 TreeAttn tree_attn_args(const itts_gpt *g, const TreeStep &t, int l, int n) {
   const itts_config &c = g->cfg;
   const int64_t d = c.d_model, head = (int64_t)t.kv->max_seq * 64;
@@ -874,7 +874,7 @@ TreeAttn tree_attn_args(const itts_gpt *g, const TreeStep &t, int l, int n) {
   a.q = g->bq.p;
   a.k = t.kv->k_layer(l);
   a.v = t.kv->v_layer(l);
-  a.out = g->tattn.p;
+  a.planes = g->ba.out();
   a.lengths = t.length;
   a.parents = t.parents;
   a.batch = 1;
@@ -917,7 +917,6 @@ itts_status enqueue_step_batch(itts_gpt *g, int B, int max_seq, int kvt, const T
     HIP_TRY(launch_gemm(ga, bits, pt, kEpiQKV, kvt, s));
     if (tree) {
       HIP_TRY(tree_attn(tree_attn_args(g, *tree, l, B), g->n_cu, s));
-      HIP_TRY(launch_split_rows(g->tattn.as<float>(), B, d, g->ba.out(), s));
     } else {
       HIP_TRY(launch_decode_batch_rows(g->bq.as<float>(), seqs, B, layer_elems * l, c.n_head, max_seq, g->ba.out(),
                                        kvt, s));
@@ -1903,7 +1902,6 @@ itts_status itts_gpt_step_tree(itts_gpt *gpt, itts_kv *kv, const int32_t *tokens
     if (itts_status st = ensure_batch(gpt, n)) return st;
     HIP_TRY(gpt->tin.ensure(sizeof(int32_t) * words));
     HIP_TRY(gpt->tctl.ensure(sizeof(DecodeCtl) * n));
-    HIP_TRY(gpt->tattn.ensure(sizeof(float) * (size_t)n * c.d_model));
     HIP_TRY(gpt->h_tree.acquire(sizeof(int32_t) * words));
     int32_t *h = gpt->h_tree.as<int32_t>();
     memcpy(h, tokens, sizeof(int32_t) * n);
