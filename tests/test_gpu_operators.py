@@ -626,3 +626,20 @@ def test_arguments_by_name(ops):
     path = ints([[1, 2], [0, -1]])
     k2, v2 = k.unsqueeze(0).clone(), v.unsqueeze(0).clone()
     assert ops.cache_keep(path=path, lengths=lengths, v=v2, k=k2).tolist() == [6, 10]
+
+
+def test_values_that_do_not_fit_are_refused(ops):
+    """What has no place in the library's 32-bit fields is refused, not cut."""
+    from itts_hip import ValidationError
+    say("[gpu] values past the library's types")
+    q, ln, par = torch.zeros(1, 1, 2, 64, device="cuda"), ints([1]), ints([[-1]])
+    k = torch.zeros(1, 2, 4, 64, device="cuda")
+    for scale in (1e300, -1e300):
+        with pytest.raises(ValidationError):
+            ops.tree_attention(q, k, k, ln, par, scale=scale)
+    with pytest.raises(ValidationError):
+        ops.tree_attention(q, k, k, ln, par, max_length=-(1 << 40))
+    with pytest.raises(ValidationError, match="rows"):
+        ops.token_scores(torch.zeros(1, 2, device="cuda").expand((1 << 23) + 1, 2))
+    with pytest.raises(ValidationError):
+        ops.cache_keep(k, k, ln, torch.zeros(1, 1, dtype=torch.int32, device="cuda").expand(1, 1 << 33))
