@@ -23,7 +23,7 @@ namespace {
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kPieces = 8;       // 16-byte pieces a thread holds
 constexpr int kList = 1024;      // room for elements that pass the bound
-constexpr int kMaxSplits = 32;
+constexpr int kMaxSplits = 16;
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <int TYPE>
@@ -296,13 +296,24 @@ __global__ __launch_bounds__(kThreads, LONG ? 4 : 6) void token_scores_kernel(To
     }
     if (any) {
       // (-inf has no part in this: a row's last places go to masked tokens at the end)
-      if (narrow) {  // a bound for the n-th largest: ceil(n / 4) threads of every wave reach it
-        const uint32_t share = reached(own, (n + kWaves - 1) / kWaves);
+      // A bound for the n-th largest: an equal share of n of every full wave's threads reach it.  (Without a
+      // full wave the list has room for all.)
+      const int full = min(pieces - base, kThreads) / 64;
+      if (narrow && full > 0) {
+        const uint32_t share = reached(own, (n + full - 1) / full);
         if ((t & 63) == 0) sel.bound[t >> 6] = share;
         __syncthreads();
         uint32_t low = ~0u;
 #pragma unroll
-        for (int w = 0; w < kWaves; w++) low = min(low, sel.bound[w]);
+        for (int w = 0; w < kWaves; w++) low = w < full ? min(low, sel.bound[w]) : low;
+        if (low == 0) {  // masks leave a wave fewer: n threads of one wave reach it
+          const uint32_t all = reached(own, n);
+          __syncthreads();
+          if ((t & 63) == 0) sel.bound[t >> 6] = all;
+          __syncthreads();
+#pragma unroll
+          for (int w = 0; w < kWaves; w++) low = max(low, sel.bound[w]);
+        }
         bound = max(bound, low);
       }
       const float least = unorder(bound);
@@ -424,10 +435,17 @@ __global__ __launch_bounds__(kThreads) void scores_join_kernel(TokenScores a, in
   write_row<TYPE>(a, r, x, row, sel);
 }
 
+// Blocks of a row: so many that each holds its tokens at once, up to 16 (the joining takes longer with
+// every one: an fp32 row of 131,000 15.5 us with 16, 18 with 8, 21 with 32; 64 rows with 64 alternatives 27, 37, 39).
+// Where that is more than eight blocks a compute unit: three, or one (300 rows of 131,000 40 us with 3, 44 with
+// 6, 54 with 1; 700 rows of 33,000 with 20 alternatives 41 with 2, 35 with 1).  A second turn costs less than a second
+// launch while few alternatives are asked for: a row of 12,000 with 10 11.5 and 10.2 us, a call 10.5 and 12.3;
+// 64 rows with 64 23 and 16 us.
 int splits(const TokenScores &a, int n_cu) {
-  const int round = kThreads * kPieces * (a.type == kOpF32 ? 4 : 8);
-  const int64_t want = (2 * (int64_t)n_cu + a.rows - 1) / a.rows, can = a.vocab / round;
-  return (int)std::max<int64_t>(1, std::min<int64_t>({want, can, kMaxSplits}));
+  const int pieces = a.vocab / (a.type == kOpF32 ? 4 : 8), turn = kThreads * kPieces;
+  if (pieces <= (a.top <= 16 ? 2 : 1) * turn) return 1;
+  const int want = std::min((pieces + turn - 1) / turn, kMaxSplits), room = 8 * n_cu / a.rows;
+  return want <= room ? want : room >= 3 ? 3 : 1;
 }
 
 template <int TYPE>

@@ -405,6 +405,20 @@ def test_scores_ties_masks_and_odd_values(ops, dtype, v):
         scores_check(ops.token_scores(x, tokens, top), x, tokens, top)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("v", [1030, 1300, 1543, 2047, 20000])
+def test_scores_few_waves_and_masked_ranges(ops, dtype, v):
+    """Vocabularies that leave a block's last waves without tokens, and masks that allow one range of them."""
+    say(f"[gpu] scores {v} {dtype}: waves without tokens")
+    g = gen(v + 1)
+    x = logits(g, 9, v, dtype)
+    for i, (lo, hi) in enumerate(((0, 70), (500, 1029), (100, 101), (v - 40, v), (0, v - 1), (256, 512))):
+        x[i, :lo], x[i, hi:] = -INF, -INF
+    tokens = torch.randint(0, v, (9, 2), generator=g, device="cuda").int()
+    for top in (1, 5, 20, 64):
+        scores_check(ops.token_scores(x, tokens, top), x, tokens, top)
+
+
 def test_scores_forms(ops):
     """One token a row, none, rows with gaps and rows that do not start at 16 bytes."""
     say("[gpu] scores forms")
