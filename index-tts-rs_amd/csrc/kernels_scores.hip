@@ -9,7 +9,9 @@
 // are longer go on piece by piece), takes each thread's maximum, then its sums.  The same registers
 // give the alternatives: any n of the row's elements bound the n-th largest from below, so the
 // threads' maxima give a bound that few elements pass; those go to a list in LDS and are ranked
-// against each other.  Rows that are few and long are split over blocks and joined by a second
+// against each other.  Where many pass (masks of one low value, ties, rising rows) the n-th value is found first:
+// 64 rows of 8,194 with all but five at the type's lowest value, 64 alternatives, 15 us a call (12 without a
+// mask); n rounds over the row took 438.  Rows that are few and long are split over blocks and joined by a second
 // kernel.  Bound by instructions, 12 an element (one of them the exponential), where memory would
 // take half to three quarters of the time: 2,188 fp32 rows of 8,194 with 5 alternatives 19 us (72 MB), 1,000 bf16
 // rows of 60,510 with 20 48 us (121 MB); one row of 8,194 6.2 us.
@@ -23,9 +25,13 @@ namespace {
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kPieces = 8;       // 16-byte pieces a thread holds
 constexpr int kList = 1024;      // room for elements that pass the bound
+constexpr int kRank = 256;       // most of them that are ranked against each other
 constexpr int kMaxSplits = 16;
+static_assert(kMaxSplits * kScoresMaxTop <= kList, "the joined lists fit");
 constexpr float kLog2e = 1.4426950408889634f;
 
+template <int TYPE>
+constexpr uint32_t kStep = TYPE == kOpF32 ? 1u : TYPE == kOpBf16 ? 1u << 16 : 1u << 13;  // between neighbours, as `order`s
 template <int TYPE>
 constexpr int kPer = TYPE == kOpF32 ? 4 : 8;  // elements of a 16-byte piece
 
@@ -127,7 +133,7 @@ struct Select {
   uint64_t list[kList + kScoresMaxTop];
   uint64_t top[kScoresMaxTop];
   uint32_t bound[kWaves];
-  int hot[2][kWaves];
+  int hot[2][kWaves], reach[2][kWaves];
   int count;
 };
 
@@ -142,18 +148,6 @@ __device__ inline void rank_list(Select &sel, int have, int n) {
   for (int i = threadIdx.x; i < n; i += kThreads)
     if (i >= have) sel.top[i] = 0;
   __syncthreads();
-}
-
-__device__ inline uint64_t block_max(uint64_t v, Select &sel) {
-  for (int off = 32; off > 0; off >>= 1) {
-    const uint64_t o = __shfl_xor((unsigned long long)v, off, 64);
-    v = o > v ? o : v;
-  }
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) sel.list[threadIdx.x >> 6] = v;
-  __syncthreads();
-  for (int w = 0; w < kWaves; w++) v = max(v, sel.list[w]);
-  return v;
 }
 
 // Fills a list that the row's numbers leave short: tokens of -inf and NaN, the lowest first.  Wave 0.
@@ -213,7 +207,7 @@ __global__ __launch_bounds__(kThreads, LONG ? 4 : 6) void token_scores_kernel(To
   const float tok_x = tok >= 0 && tok < a.vocab ? logit<TYPE>(x, tok) : 0.0f;
 
   Stats st{-INFINITY, 0.0f, 0.0f, 0.0f};
-  bool ranked = false;  // all of this block's tokens are
+  int found = 0;  // entries of the list that the last turn left
   if (n > 0) {
     if (t < n) sel.top[t] = 0;
     if (t == 0) sel.count = 0;
@@ -275,7 +269,7 @@ __global__ __launch_bounds__(kThreads, LONG ? 4 : 6) void token_scores_kernel(To
 
     uint32_t bound = kOrderNone + 1;
     const uint32_t own = u.m > -INFINITY ? order(u.m) : 0;
-    bool any = n > 0 && !ranked, narrow = any;
+    bool any = n > 0, narrow = any;
     if constexpr (LONG) {
       // A token has to come before the n-th so far: to be larger, or as large where that one is of the row's
       // rest, whose tokens are the last.  Where few threads have one, that is bound enough.
@@ -316,44 +310,110 @@ __global__ __launch_bounds__(kThreads, LONG ? 4 : 6) void token_scores_kernel(To
         }
         bound = max(bound, low);
       }
-      const float least = unorder(bound);
-      auto offer = [&](float y, int token) {
+      auto offer = [&](float y, int token, float least) {
         if (!(y >= least)) return;
         const int at = atomicAdd(&sel.count, 1);
         if (at < kList) sel.list[at] = rank_key(y, token);
       };
+      const float first = unorder(bound);
 #pragma unroll
       for (int k = 0; k < kPieces; k++) {
-        if (!(gm[k] >= least)) continue;
+        if (!(gm[k] >= first)) continue;
         again(v[k]);
 #pragma unroll
-        for (int e = 0; e < P; e++) offer(element<TYPE>(v[k], e), i0 + (base + k * kThreads + t) * P + e);
+        for (int e = 0; e < P; e++) offer(element<TYPE>(v[k], e), i0 + (base + k * kThreads + t) * P + e, first);
       }
-      if (has_odd) offer(odd_x, odd);
+      if (has_odd) offer(odd_x, odd, first);
       __syncthreads();
-      const int count = sel.count;  // (with what was found before)
-      if (count > kList) {
-        // Ties by the thousand, or the largest all in a few threads: n rounds of the largest that
-        // is left, over all of this block's tokens in memory.
-        uint64_t last = ~0ull, mine = 0;
-        for (int round = 0; round < n; round++) {
-          uint64_t next = 0;
-          for (int i = i0 + t; i < i1; i += kThreads) {
-            const float y = logit<TYPE>(x, i);
-            const uint64_t key = y > -INFINITY ? rank_key(y, i) : 0;
-            if (key < last) next = max(next, key);
+      int count = sel.count;  // (with the `found` ones from before)
+      bool ties = false;
+      if (count - found > kRank) {
+        // Ties by the hundred, or the largest all in a few threads: the n-th value itself, bit by bit from the
+        // top, until no more than can be ranked reach it; if that never is so, what is above it.  (From memory
+        // again: this is rare, and the registers are the others'.)
+        auto each = [&](auto &&f) {
+#pragma unroll 1
+          for (int at = base + t; at < min(base + kThreads * kPieces, pieces); at += kThreads) {
+            uint4 w;
+            __builtin_memcpy(&w, body + (int64_t)at * 16, 16);
+#pragma unroll
+            for (int e = 0; e < P; e++) f(element<TYPE>(w, e), i0 + at * P + e);
           }
-          last = block_max(next, sel);
-          if (t == round) mine = last;
+          if (has_odd) f(odd_x, odd);
+        };
+        int buf = 0;
+        auto reaching = [&](uint32_t from) {
+          const float least = unorder(from);
+          int c = 0;
+          each([&](float y, int) { c += y >= least; });
+          const float sum = wave_sum_f((float)c);
+          if ((t & 63) == 0) sel.reach[buf][t >> 6] = (int)sum;
+          __syncthreads();
+          int all = 0;
+#pragma unroll
+          for (int w = 0; w < kWaves; w++) all += sel.reach[buf][w];
+          buf ^= 1;
+          return all;
+        };
+        // The least of the threads' largest is that value where one stands in nearly every place (a mask's).
+        const float low = -wave64_max_dpp(own >= bound ? -u.m : -INFINITY);
+        if ((t & 63) == 0) sel.bound[t >> 6] = order(low);
+        __syncthreads();
+        uint32_t nth = ~0u;
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) nth = min(nth, sel.bound[w]);
+        int reach = reaching(nth);
+        if (reach >= n) bound = nth;
+        if (reach < n || (reach > kRank && reaching(nth + kStep<TYPE>) >= n)) {
+          nth = 0, reach = count - found;
+          for (uint32_t bit = 1u << 31; bit >= kStep<TYPE> && reach > kRank; bit >>= 1) {
+            const uint32_t to = nth | bit;
+            if (to > bound) {
+              const int all = reaching(to);
+              if (all < n) continue;
+              reach = all;
+            }
+            nth = to;
+          }
+        }
+        ties = reach > kRank;
+        bound = ties ? nth + kStep<TYPE> : max(nth, bound);
+        __syncthreads();  // (the list and its length are read)
+        if (t == 0) sel.count = found;
+        __syncthreads();
+        const float least = unorder(bound);
+        each([&](float y, int token) { offer(y, token, least); });
+        __syncthreads();
+        count = sel.count;
+      }
+      if (ties) {  // fewer than n are above that value: its lowest tokens follow
+        __syncthreads();
+        if (t < 64) {
+          int have = count;
+          const int body_end = i1 - rest;
+          for (int part = 0; part < (base == 0 ? 2 : 1); part++) {  // (the first turn has the row's rest too)
+            const int from = part == 0 ? i0 + base * P : body_end;
+            const int to = part == 0 ? min(from + kThreads * kPieces * P, body_end) : i1;
+            for (int at = from; at < to && have < found + n; at += 64) {
+              const uint32_t o = order(logit<TYPE>(x, min(at + t, to - 1)));
+              const bool tie = at + t < to && o < bound && bound - o <= kStep<TYPE>;
+              const uint64_t b = __ballot(tie);
+              const int place = have + __popcll(b & ((1ull << t) - 1));
+              if (tie && place < found + n) sel.list[place] = rank_key(unorder(o), at + t);
+              have = min(have + (int)__popcll(b), found + n);
+            }
+          }
+          if (t == 0) sel.count = have;
         }
         __syncthreads();
-        if (t < n) sel.top[t] = mine;
-        ranked = true;
-      } else if (count > 0) {
+        count = sel.count;
+      }
+      if (count > 0) {
         rank_list(sel, count, n);
         if constexpr (LONG) {
+          found = min(count, n);
           if (t < n) sel.list[t] = sel.top[t];
-          if (t == 0) sel.count = min(count, n);
+          if (t == 0) sel.count = found;
         }
       }
     }
@@ -402,26 +462,10 @@ __global__ __launch_bounds__(kThreads) void scores_join_kernel(TokenScores a, in
     const uint64_t least = max(max(all, share), (uint64_t)1);
     for (int i = t; i < S * n; i += kThreads) {
       if (keys[i] < least) continue;
-      const int at = atomicAdd(&sel.count, 1);
-      if (at < kList) sel.list[at] = keys[i];
+      sel.list[atomicAdd(&sel.count, 1)] = keys[i];
     }
     __syncthreads();
-    const int count = sel.count;
-    if (count <= kList) {
-      rank_list(sel, count, n);
-    } else {  // (lists of many large ones each)
-      uint64_t last = ~0ull, mine = 0;
-      for (int round = 0; round < n; round++) {
-        uint64_t next = 0;
-        for (int i = t; i < S * n; i += kThreads)
-          if (keys[i] < last) next = max(next, keys[i]);
-        last = block_max(next, sel);
-        if (t == round) mine = last;
-      }
-      __syncthreads();
-      if (t < n) sel.top[t] = mine;
-      __syncthreads();
-    }
+    rank_list(sel, sel.count, n);
   }
   if (t >= 64) return;
   Stats st = parts[0];
