@@ -1147,14 +1147,14 @@ __global__ __launch_bounds__(256) void cache_keep_kernel(CacheKeep a) {
     last = path[n];
   }
   if (blockIdx.x == 0 && threadIdx.x == 0) a.new_lengths[b] = ok ? len + n : -1;
-  if (!ok) return;
   int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  // (past the last piece; caches without layers or heads have none, only lengths)
+  if (!ok || i >= (int64_t)a.caches * a.layers * a.heads * a.row_pieces) return;
   const int piece = i % a.row_pieces;
   i /= a.row_pieces;
   const int head = i % a.heads;
   i /= a.heads;
   const int layer = i % a.layers, is_v = (int)(i / a.layers);
-  if (is_v >= a.caches) return;
   uint4 *base = is_v ? static_cast<uint4 *>(a.v) + layer * a.v_l + b * a.v_b + head * a.v_h
                      : static_cast<uint4 *>(a.k) + layer * a.k_l + b * a.k_b + head * a.k_h;
   const int64_t step = is_v ? a.v_r : a.k_r;

@@ -511,6 +511,15 @@ def test_keep_of_one_memory_for_keys_and_values(ops):
     assert torch.equal(k, want)
 
 
+@pytest.mark.parametrize("shape", [(2, 3, 0, 40, 64), (0, 3, 2, 40, 64), (0, 3, 0, 40, 64), (3, 0, 40, 64)])
+def test_keep_of_caches_without_layers_or_heads(ops, shape):
+    """No rows to move: the lengths alone, and -1 for paths that are refused."""
+    say(f"[gpu] keep without rows {shape}")
+    k, v = torch.zeros(shape, dtype=BF16, device="cuda"), torch.zeros(shape, dtype=BF16, device="cuda")
+    new = ops.cache_keep(k, v, ints([5, 0, 38]), ints([[1, 2, -1], [2, 1, -1], [0, 1, 2]]))
+    assert new.tolist() == [7, -1, -1]
+
+
 # ---- streams, graphs, refusals -----------------------------------------------------------------
 def drafted(ops, s):
     """The three as they are used: a draft's attention, its scores, the accepted rows kept."""
