@@ -83,65 +83,54 @@ __device__ __forceinline__ float col_sum(float v) {
   return v + __shfl_xor(v, 32, 64);
 }
 
-// The pair (a, b) as planes of 16-bit values, the first in the low half: plane 0 holds the leading
-// bits (cut, not rounded), the next what is left, so that every plane has its value's sign.  A
-// rest of exactly 0 becomes the smallest number of that sign: 0 times an infinity in the other
-// operand would turn what is an infinity into NaN.  bf16: 8 bits a plane, three hold a float;
-// fp16: 11 bits, two planes 22.
-template <class T, int N>
-__device__ __forceinline__ void cut2(float a, float b, uint32_t (&o)[N]) {
-  if constexpr (std::is_same_v<T, Bf16>) {
-#pragma unroll
-    for (int i = 0; i < N; i++) {
-      const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
-      o[i] = __builtin_amdgcn_perm(ub, ua, 0x07060302u);
-      if (i + 1 < N) {
-        a = __builtin_copysignf(fmaxf(fabsf(a - __uint_as_float(ua & 0xffff0000u)), 0x1p-120f), a);
-        b = __builtin_copysignf(fmaxf(fabsf(b - __uint_as_float(ub & 0xffff0000u)), 0x1p-120f), b);
-      }
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; i++) {
-      const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
-      o[i] = __builtin_bit_cast(uint32_t, h);
-      if (i + 1 < N) {
-        a = __builtin_copysignf(fmaxf(fabsf(a - (float)h[0]), 0x1p-24f), a);
-        b = __builtin_copysignf(fmaxf(fabsf(b - (float)h[1]), 0x1p-24f), b);
-      }
-    }
-  }
-}
-// The same for probabilities (never negative).
-template <class T, int N>
-__device__ __forceinline__ void cut2_pos(float a, float b, uint32_t (&o)[N]) {
-  if constexpr (std::is_same_v<T, Bf16>) {
-#pragma unroll
-    for (int i = 0; i < N; i++) {
-      const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
-      o[i] = __builtin_amdgcn_perm(ub, ua, 0x07060302u);
-      if (i + 1 < N) {
-        a = fmaxf(a - __uint_as_float(ua & 0xffff0000u), 0x1p-120f);
-        b = fmaxf(b - __uint_as_float(ub & 0xffff0000u), 0x1p-120f);
-      }
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; i++) {
-      const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
-      o[i] = __builtin_bit_cast(uint32_t, h);
-      if (i + 1 < N) {
-        a = fmaxf(a - (float)h[0], 0x1p-24f);
-        b = fmaxf(b - (float)h[1], 0x1p-24f);
-      }
-    }
-  }
-}
-
 template <class T>
 __device__ __forceinline__ uint32_t round2(float a, float b) {
   if constexpr (std::is_same_v<T, Bf16>) return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2e){a, b}, bf16x2v));
   else return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2e){a, b}, f16x2v));
+}
+
+// The pair (a, b) as planes of 16-bit values, the first in the low half: plane 0 holds the leading
+// bits (cut, not rounded), the next what is left, so that every plane has its value's sign.  A
+// rest of exactly 0 becomes a small number of that sign: 0 times an infinity in the other operand
+// would turn what is an infinity into NaN.  A value of 0 stays 0 in every plane: a masked key's finite
+// values, however large, must not weigh anything.  bf16: 8 bits a plane, three hold a float.
+__device__ __forceinline__ float cut_bits(float v) { return __uint_as_float(__float_as_uint(v) & 0xffff0000u); }
+__device__ __forceinline__ uint32_t cut_pair(float a, float b) {
+  return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+}
+__device__ __forceinline__ void cut3(float a, float b, uint32_t (&o)[3]) {
+  const float least_a = fminf(fabsf(a), 0x1p-120f), least_b = fminf(fabsf(b), 0x1p-120f);
+#pragma unroll
+  for (int i = 0; i < 3; i++) {
+    o[i] = cut_pair(a, b);
+    if (i < 2) {
+      a = __builtin_copysignf(fmaxf(fabsf(a - cut_bits(a)), least_a), a);
+      b = __builtin_copysignf(fmaxf(fabsf(b - cut_bits(b)), least_b), b);
+    }
+  }
+}
+// The same for probabilities (never negative).  Two planes of bf16: the second is rounded, 2^-16 of the
+// value at most, and its rest is raised by 2^-23 of the value in the subtraction itself.  fp16: 11 bits a
+// plane, two hold 22 (down to 2^-24, its smallest number).
+template <class T, int N>
+__device__ __forceinline__ void cut_pos(float a, float b, uint32_t (&o)[N]) {
+  if constexpr (std::is_same_v<T, F16>) {
+    static_assert(N == 2);
+    const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
+    o[0] = __builtin_bit_cast(uint32_t, h);
+    o[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(fmaxf(a - (float)h[0], a > 0.0f ? 0x1p-24f : 0.0f),
+                                                                   fmaxf(b - (float)h[1], b > 0.0f ? 0x1p-24f : 0.0f)));
+  } else if constexpr (N == 2) {
+    o[0] = cut_pair(a, b);
+    o[1] = round2<Bf16>(__builtin_fmaf(a, 1.0f + 0x1p-23f, -cut_bits(a)), __builtin_fmaf(b, 1.0f + 0x1p-23f, -cut_bits(b)));
+  } else {
+    const float least_a = fminf(a, 0x1p-120f), least_b = fminf(b, 0x1p-120f);
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      o[i] = cut_pair(a, b);
+      if (i + 1 < N) a = fmaxf(a - cut_bits(a), least_a), b = fmaxf(b - cut_bits(b), least_b);
+    }
+  }
 }
 
 template <class T>
@@ -417,7 +406,7 @@ struct Rows {
 #pragma unroll
           for (int e = 0; e < 4; e++) {
             uint32_t w[3];
-            cut2<TKV, 3>(__uint_as_float(raw[t][j][2 * e]) * by, __uint_as_float(raw[t][j][2 * e + 1]) * by, w);
+            cut3(__uint_as_float(raw[t][j][2 * e]) * by, __uint_as_float(raw[t][j][2 * e + 1]) * by, w);
 #pragma unroll
             for (int i = 0; i < 3; i++) q[i][t][j][e] = w[i];
           }
@@ -510,7 +499,7 @@ struct Rows {
           const float a = s[i >> 1][t][2 * (i & 1)], b = s[i >> 1][t][2 * (i & 1) + 1];
           uint32_t w[NP];
           if constexpr (NP == 1) w[0] = round2<TKV>(a, b);
-          else cut2_pos<TKV, NP>(a, b, w);
+          else cut_pos<TKV, NP>(a, b, w);
 #pragma unroll
           for (int k = 0; k < NP; k++) x.p[t][k][i] = w[k];
         }

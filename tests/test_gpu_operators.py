@@ -193,6 +193,36 @@ def test_attention_odd_values_stay_where_they_are_seen(ops, types, value):
     assert fin[0, 0].all() and fin[0, 4, 0].all() and not fin[0, 4, 2:].all()
 
 
+# each kernel and the joining of blocks: few rows, few rows over dealt keys, shared tiles, shared tiles over dealt keys
+@pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("b,n,h,hk,d,rows", [
+    (3, 8, 4, 2, 64, 90), (2, 33, 2, 2, 128, 90), (2, 150, 2, 1, 64, 200), (2, 21, 2, 2, 64, 9000), (12, 72, 8, 8, 64, 300),
+    (3, 130, 20, 20, 128, 2000),
+])
+def test_attention_large_values_stay_where_they_are_seen(ops, types, b, n, h, hk, d, rows):
+    """Rows of unused slots, inside the tree and behind it, hold the type's largest values, leaves' rows large ones: nothing
+    of them reaches a node that does not see them, whose own values are small."""
+    say(f"[gpu] tree attention large values {types} {b} x {n} h={h}/{hk} d={d} rows={rows}")
+    g = gen(n)
+    q, kv = types
+    (q, k, v), ln, par = attention_case(ops, types, b, n, h, hk, d, [rows - n - 3 - 5 * i for i in range(b)], "star", rows=rows, seed=n)
+    v *= 2.0 ** -6
+    top = torch.finfo(kv).max
+    par[:, 1::3] = -2                                       # unused slots between the root's children
+    large = 65504.0 if kv == F16 else 2.0 ** 120            # (a child's own result is that large too, and finite)
+    for i in range(b):
+        at = int(ln[i])
+        v[i, :, at + 2:at + n] = large
+        v[i, :, at + 1:at + n:3] = top
+        v[i, :, at + n:] = top
+    got = ops.tree_attention(q, k, v, ln, par)
+    some = sorted({0, b - 1})
+    nodes = sorted({0, 1, 2, 3, n // 2, n - 1})
+    ref, tol = attention_ref(q[some], k[some], v[some], ln[some], par[some])
+    check(got[some][:, nodes], ref[:, nodes], tol[:, nodes])
+    assert got[:, 0].abs().max() < 1.0 and torch.isfinite(got).all()
+
+
 def test_attention_lengths_that_do_not_fit(ops):
     say("[gpu] tree attention lengths that do not fit")
     lengths = [-1, 57, 56, 2 ** 31 - 1, -2 ** 31, 0]
