@@ -83,12 +83,6 @@ __device__ __forceinline__ float col_sum(float v) {
   return v + __shfl_xor(v, 32, 64);
 }
 
-template <class T>
-__device__ __forceinline__ uint32_t round2(float a, float b) {
-  if constexpr (std::is_same_v<T, Bf16>) return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2e){a, b}, bf16x2v));
-  else return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2e){a, b}, f16x2v));
-}
-
 // The pair (a, b) as planes of 16-bit values, the first in the low half: plane 0 holds the leading
 // bits (cut, not rounded), the next what is left, so that every plane has its value's sign.  A
 // rest of exactly 0 becomes a small number of that sign: 0 times an infinity in the other operand
@@ -109,27 +103,27 @@ __device__ __forceinline__ void cut3(float a, float b, uint32_t (&o)[3]) {
     }
   }
 }
-// The same for probabilities (never negative).  Two planes of bf16: the second is rounded, 2^-16 of the
-// value at most, and its rest is raised by 2^-23 of the value in the subtraction itself.  fp16: 11 bits a
-// plane, two hold 22 (down to 2^-24, its smallest number).
+// The same for probabilities (never negative).  bf16: the last rest is raised by 2^-23 of what it is the rest
+// of in the subtraction itself; the second of two planes is rounded, 2^-16 of the value at most.  fp16: 11 bits a
+// plane, two hold 22, down to its smallest number, 2^-24, which the rest always is at least: the test for
+// 0 took 4% of long caches' time and 12% of many rows', and pack clears masked keys' rests instead.
 template <class T, int N>
 __device__ __forceinline__ void cut_pos(float a, float b, uint32_t (&o)[N]) {
+  constexpr float kUp = 1.0f + 0x1p-23f, kLeast = 0x1.01p-118f;  // (more than the 8 bits of one plane)
   if constexpr (std::is_same_v<T, F16>) {
     static_assert(N == 2);
     const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
     o[0] = __builtin_bit_cast(uint32_t, h);
-    o[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(fmaxf(a - (float)h[0], a > 0.0f ? 0x1p-24f : 0.0f),
-                                                                   fmaxf(b - (float)h[1], b > 0.0f ? 0x1p-24f : 0.0f)));
+    o[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(fmaxf(a - (float)h[0], 0x1p-24f), fmaxf(b - (float)h[1], 0x1p-24f)));
   } else if constexpr (N == 2) {
     o[0] = cut_pair(a, b);
-    o[1] = round2<Bf16>(__builtin_fmaf(a, 1.0f + 0x1p-23f, -cut_bits(a)), __builtin_fmaf(b, 1.0f + 0x1p-23f, -cut_bits(b)));
+    const f32x2e rest = {__builtin_fmaf(a, kUp, -cut_bits(a)), __builtin_fmaf(b, kUp, -cut_bits(b))};
+    o[1] = __builtin_bit_cast(uint32_t, __builtin_convertvector(rest, bf16x2v));
   } else {
-    const float least_a = fminf(a, 0x1p-120f), least_b = fminf(b, 0x1p-120f);
-#pragma unroll
-    for (int i = 0; i < N; i++) {
-      o[i] = cut_pair(a, b);
-      if (i + 1 < N) a = fmaxf(a - cut_bits(a), least_a), b = fmaxf(b - cut_bits(b), least_b);
-    }
+    static_assert(N == 3);
+    const float rest_a = fmaxf(a - cut_bits(a), fminf(a, kLeast)), rest_b = fmaxf(b - cut_bits(b), fminf(b, kLeast));
+    o[0] = cut_pair(a, b), o[1] = cut_pair(rest_a, rest_b);
+    o[2] = cut_pair(__builtin_fmaf(rest_a, kUp, -cut_bits(rest_a)), __builtin_fmaf(rest_b, kUp, -cut_bits(rest_b)));
   }
 }
 
@@ -348,23 +342,18 @@ struct TileRegs {
   }
 };
 
-// Planes of 16 bits that hold a probability.  Few query rows wait for memory, not for products: two
-// (16 bits of bf16, 22 of fp16) leave no more than the result's own rounding.  Many rows over 16-bit
-// queries wait for instructions: one, rounded (half a step of the result's type, and the same
-// rounded values in the sums), 12 x 64 nodes, 32 heads of 8 over 1,000 .. 8,191 rows 144 -> 114 us at
-// the time.  fp32 queries: three, an fp32's bits.
+// Planes of 16 bits that hold a probability: two under 16-bit queries (16 bits of bf16, 22 of fp16) leave no
+// more than the result's own rounding, whichever kernel a launch takes; three under fp32 ones, an fp32's bits.
 template <class TQ>
-constexpr int prob_planes(bool many) {
-  return TQ::kBytes == 4 ? 3 : many ? 1 : 2;
-}
+constexpr int kProbPlanes = TQ::kBytes == 4 ? 3 : 2;
 
 // What a wave holds of RT tiles of 16 query rows (lane (c, g): row c of each), and the three steps of
 // a tile of keys.  16-bit caches go through the 16-bit matrix instructions: queries in NQ planes (fp32
-// ones in three, exactly), probabilities in NP (see prob_planes).  fp32 caches take the fp32 ones.
+// ones in three, exactly), probabilities in NP.  fp32 caches take the fp32 ones.
 template <int D, class TQ, class TKV, int RT, bool MANY>
 struct Rows {
   static constexpr bool kWide = TKV::kBytes == 4;
-  static constexpr int NQ = kWide || TQ::kBytes == 2 ? 1 : 3, NP = prob_planes<TQ>(MANY);
+  static constexpr int NQ = kWide || TQ::kBytes == 2 ? 1 : 3, NP = kProbPlanes<TQ>;
   static constexpr int kV = D / 16 * TKV::kBytes / 4;
   // probabilities are held up to 2^(kLag + kUp): the running maximum moves only when a score passes
   // it by 2^kLag; fp16 planes use their range below 1 too
@@ -486,11 +475,12 @@ struct Rows {
     }
   }
 
-  // Probabilities as the second product's operand: 16-bit planes of a lane's 8 keys.
+  // Probabilities as the second product's operand: 16-bit planes of a lane's 8 keys.  At an edge masked keys
+  // are 0 in all of them.
   struct Probs {
     uint32_t p[kWide ? 1 : RT][NP][4];
   };
-  __device__ __forceinline__ void pack(const floatx4 (&s)[2][RT], Probs &x) const {
+  __device__ __forceinline__ void pack(const floatx4 (&s)[2][RT], bool edge, const uint32_t (&seen)[RT], Probs &x) const {
     if constexpr (!kWide) {
 #pragma unroll
       for (int t = 0; t < RT; t++)
@@ -498,11 +488,19 @@ struct Rows {
         for (int i = 0; i < 4; i++) {
           const float a = s[i >> 1][t][2 * (i & 1)], b = s[i >> 1][t][2 * (i & 1) + 1];
           uint32_t w[NP];
-          if constexpr (NP == 1) w[0] = round2<TKV>(a, b);
-          else cut_pos<TKV, NP>(a, b, w);
+          cut_pos<TKV, NP>(a, b, w);
 #pragma unroll
           for (int k = 0; k < NP; k++) x.p[t][k][i] = w[k];
         }
+      if (std::is_same_v<TKV, F16> && edge) {
+#pragma unroll
+        for (int t = 0; t < RT; t++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const uint32_t at = seen[t] >> (16 * (i >> 1) + 2 * (i & 1));
+            x.p[t][1][i] &= (at & 1 ? 0xffffu : 0) | (at & 2 ? 0xffff0000u : 0);
+          }
+      }
     }
   }
 
@@ -739,7 +737,7 @@ __global__ __launch_bounds__(256, 2) void tree_attn_kernel(Args p) {
       rows.add_wide(s, x.v);
     } else {
       typename Wave::Probs probs;
-      rows.pack(s, probs);
+      rows.pack(s, edge, seen, probs);
       rows.add_rows(probs, x.v);
     }
     x.load_v(vb + (uint64_t)(uint32_t)next * v_step);
@@ -903,7 +901,7 @@ __global__ __launch_bounds__(64 * kRowWaves, 2) void tree_attn_rows_kernel(Args 
     scores(s_next, buf ^ 1);
     rows.weigh(s);
     typename Wave::Probs probs;
-    rows.pack(s, probs);
+    rows.pack(s, kEdge, seen, probs);
     rows.add_sums(probs);
 #pragma unroll
     for (int d0 = 0; d0 < D / 16; d0 += 4) {  // (four at a time: fewer registers)

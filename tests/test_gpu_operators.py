@@ -193,6 +193,22 @@ def test_attention_odd_values_stay_where_they_are_seen(ops, types, value):
     assert fin[0, 0].all() and fin[0, 4, 0].all() and not fin[0, 4, 2:].all()
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("b,n,h,hk,d,rows", [(3, 8, 4, 2, 64, 300), (12, 72, 8, 8, 64, 300), (12, 48, 16, 2, 128, 300), (3, 130, 20, 20, 128, 2000)])
+def test_attention_of_16_bits_rounds_its_result_alone(ops, dtype, b, n, h, hk, d, rows):
+    """Whatever a launch's layout: a probability's two planes are off by 2^-16 (bf16: 8 bits and a rounded 8; fp16 2^-21,
+    and less than 2^-33 of the largest) of it at most, in the product and in the sum, so that half a step of the result is nearly all."""
+    say(f"[gpu] tree attention's rounding {dtype} {b} x {n} h={h}/{hk} d={d} rows={rows}")
+    (q, k, v), ln, par = attention_case(ops, (dtype, dtype), b, n, h, hk, d, [rows - n - 7 * i for i in range(b)], "tree", rows=rows, seed=rows + d)
+    got = ops.tree_attention(q, k, v, ln, par)
+    some, nodes = sorted({0, b // 2, b - 1}), sorted({0, 1, n // 2, n - 1})
+    ref, tol = attention_ref(q[some], k[some], v[some], ln[some], par[some])
+    pv = attention_ref(q[some], k[some], v[some].abs(), ln[some], par[some])[0]  # the probabilities with the values' sizes
+    tol = tol - HALF[dtype] * (ref.abs() + pv)                                   # (the float32 part)
+    tol += HALF[dtype] * (ref.abs() + tol) + 2 * pv * (2.0 ** -16 + 2.0 ** -23 if dtype == BF16 else 2.0 ** -21) + 2.0 ** -33 * rows * 8
+    check(got[some][:, nodes], ref[:, nodes], tol[:, nodes])
+
+
 # each kernel and the joining of blocks: few rows, few rows over dealt keys, shared tiles, shared tiles over dealt keys
 @pytest.mark.parametrize("types", TYPES)
 @pytest.mark.parametrize("b,n,h,hk,d,rows", [
