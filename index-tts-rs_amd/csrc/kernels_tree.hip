@@ -966,8 +966,9 @@ __global__ __launch_bounds__(256) void tree_join_kernel(Args p) {
   float4 o = *reinterpret_cast<const float4 *>(part + (size_t)min(s0, S - 1) * D);  // (before what weighs it is there)
   const float top = wave_max(own.x), ms = top == -INFINITY ? 0.0f : top;
   const bool none = __ballot(own.x == INFINITY && own.y == 0.0f) != 0;
-  // (at least 2^-126: 0 times an infinity would be NaN)
-  const float f_own = fmaxf(__builtin_amdgcn_exp2f(own.x - ms), 0x1p-126f);
+  const float f_own = __builtin_amdgcn_exp2f(own.x - ms);
+  // (a weight that is positive, if not as a float: times an infinity it is that)
+  auto weighed = [](float f, float y) { return fabsf(y) < INFINITY ? f * y : y; };
   float sum = 0.0f, x[4] = {};
   for (int s1 = 0; s1 < S; s1 += kGroups) {
     const int s = min(s1 + s0, S - 1);
@@ -976,7 +977,8 @@ __global__ __launch_bounds__(256) void tree_join_kernel(Args p) {
     const bool in = s1 + s0 < S && !(m == -INFINITY && l == 0.0f);  // without keys nothing was stored
     const bool num = in && l == l;
     sum += in ? f * l : 0.0f;
-    x[0] += num ? f * o.x : 0.0f, x[1] += num ? f * o.y : 0.0f, x[2] += num ? f * o.z : 0.0f, x[3] += num ? f * o.w : 0.0f;
+    x[0] += num ? weighed(f, o.x) : 0.0f, x[1] += num ? weighed(f, o.y) : 0.0f;
+    x[2] += num ? weighed(f, o.z) : 0.0f, x[3] += num ? weighed(f, o.w) : 0.0f;
     o = next;
   }
 #pragma unroll

@@ -239,6 +239,24 @@ def test_attention_large_values_stay_where_they_are_seen(ops, types, b, n, h, hk
     assert got[:, 0].abs().max() < 1.0 and torch.isfinite(got).all()
 
 
+@pytest.mark.parametrize("types", [(F32, BF16), (F32, F32), (BF16, BF16)])
+def test_attention_blocks_of_no_weight(ops, types):
+    """A block's keys lie so far below the row's largest score that their weight is 0 as a float: what their values are, finite
+    or not, is then neither raised nor lost in the joining."""
+    say(f"[gpu] tree attention: a block without weight {types}")
+    q, kv = types
+    g = gen(21)
+    x = torch.ones(1, 2, 2, 64, device="cuda", dtype=q)
+    k, v = (0.05 * randn(g, 1, 2, 9000, 64)).to(kv), randn(g, 1, 2, 9000, 64, dtype=kv)
+    k[:, :, :4000], k[:, :, 5], k[:, :, 8000] = -25.0, -24.75, 2.5   # scores -200, -198 and 20, the others' about 0
+    v[:, :, 5] = 1e38
+    ln, par = ints([8990]), ints([[-1, 0]])
+    check(ops.tree_attention(x, k, v, ln, par), *attention_ref(x, k, v, ln, par))
+    v[:, 0, 5] = INF
+    got = ops.tree_attention(x, k, v, ln, par)
+    assert (got[:, :, 0] == INF).all() and torch.isfinite(got[:, :, 1]).all()
+
+
 def test_attention_lengths_that_do_not_fit(ops):
     say("[gpu] tree attention lengths that do not fit")
     lengths = [-1, 57, 56, 2 ** 31 - 1, -2 ** 31, 0]
