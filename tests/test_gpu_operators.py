@@ -239,6 +239,115 @@ def test_attention_large_values_stay_where_they_are_seen(ops, types, b, n, h, hk
     assert got[:, 0].abs().max() < 1.0 and torch.isfinite(got).all()
 
 
+# (batch, nodes, heads, key heads, dim, rows) that lead to: tiles shared by a block's waves, one block a sequence and keys
+# dealt to blocks, up to 64 nodes and more; four row tiles a wave, one block and dealt; a row tile a wave, dealt
+LAYOUTS = [(12, 72, 8, 8, 64, 300), (12, 48, 16, 2, 128, 300), (16, 32, 20, 20, 64, 300), (12, 72, 8, 8, 64, 2000), (8, 72, 16, 16, 128, 1000),
+           (8, 130, 16, 16, 64, 1000), (3, 130, 20, 20, 128, 2000), (8, 64, 32, 8, 128, 2500), (8, 48, 20, 20, 64, 300),
+           (3, 48, 16, 2, 64, 8000), (2, 9, 4, 4, 64, 9000)]
+
+
+def layout_case(ops, types, shape, kind, spread):
+    """Sequences of lengths from what fits down to none, at and around tiles' borders; every third has unused slots."""
+    b, n, h, hk, d, rows = shape
+    lengths = [max(0, rows - n - spread * i - i % 3) for i in range(b)]
+    lengths[-1] = 0 if b > 3 else 1
+    if b > 4:
+        lengths[1], lengths[2] = 32, 31
+    (q, k, v), ln, par = attention_case(ops, types, b, n, h, hk, d, lengths, kind, rows=rows, seed=n + rows)
+    for i in range(0, b, 3):
+        par[i, 2 + i % 2::7] = -2
+        par[i, n - 1 - i:] = -2
+    return q, k, v, ln, par
+
+
+def check_some(got, q, k, v, ln, par, what="", max_rows=None):
+    """The first two sequences and the last (the reference goes row by row)."""
+    some = sorted({0, 1, q.shape[0] - 1})
+    ref, tol = attention_ref(q[some], k[some], v[some], ln[some], par[some], max_rows=max_rows)
+    check(got[some], ref, tol, what)
+    return ref
+
+
+@pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("shape", LAYOUTS)
+def test_attention_layouts(ops, types, shape):
+    say(f"[gpu] tree attention layouts {types} {shape}")
+    q, k, v, ln, par = layout_case(ops, types, shape, "tree", 17)
+    got = ops.tree_attention(q, k, v, ln, par)
+    check_some(got, q, k, v, ln, par)
+    assert torch.equal(got, ops.tree_attention(q, k, v, ln, par))
+    # lengths that do not fit, before the others and between them; a bound on the rows below the caches'
+    ln[0], ln[-1] = -1, shape[5] - 10
+    got = ops.tree_attention(q, k, v, ln, par, max_length=shape[5] - 5)
+    check_some(got, q, k, v, ln, par, max_rows=shape[5] - 5)
+    assert torch.isnan(got[0]).all() and torch.isnan(got[-1]).all()
+
+
+@pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("shape", LAYOUTS)
+def test_attention_layouts_hidden_and_odd_values(ops, types, shape):
+    """Unused slots and rows behind the tree hold NaN and infinities, which no node gets; a node's own row holds one, which
+    the nodes below it get."""
+    say(f"[gpu] tree attention layouts, hidden and odd values {types} {shape}")
+    q, k, v, ln, par = layout_case(ops, types, shape, "forest", 40)
+    n, odd = shape[1], (INF, -INF, NAN)
+    for i in (0, 1, shape[0] - 1):
+        at = int(ln[i])
+        for j, path in enumerate(paths(par[i].tolist())):
+            if not path:
+                k[i, :, at + j], v[i, :, at + j] = odd[j % 3], odd[(i + j) % 3]
+        k[i, :, at + n:], v[i, :, at + n:] = NAN, odd[i % 3]
+        v[i, 0, at + 1, 5], v[i, -1, at + 5, 9] = odd[i % 3], odd[(i + 1) % 3]
+    got = ops.tree_attention(q, k, v, ln, par)
+    some = sorted({0, 1, shape[0] - 1})
+    ref, tol = attention_ref(q[some], k[some], v[some], ln[some], par[some])
+    got, fin = got[some], torch.isfinite(ref)
+    assert torch.equal(torch.isnan(got), torch.isnan(ref)) and torch.equal(torch.isinf(got), torch.isinf(ref))
+    assert torch.equal(got.double()[torch.isinf(ref)], ref[torch.isinf(ref)])
+    assert ((got.double() - ref).abs()[fin] <= tol[fin]).all() and not fin.all()
+
+
+@pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("shape", [LAYOUTS[0], LAYOUTS[1], LAYOUTS[6], LAYOUTS[9]])
+def test_attention_layouts_strides_and_scales(ops, types, shape):
+    say(f"[gpu] tree attention layouts, strides and scales {types} {shape}")
+    q, k, v, ln, par = layout_case(ops, types, shape, "chain", 5)
+    b, n, h, hk, d, rows = shape
+    want = ops.tree_attention(q, k, v, ln, par)
+    q2 = torch.empty(b, h, n, d + 16, dtype=q.dtype, device="cuda").transpose(1, 2)[..., :d]
+    k2 = torch.empty(rows, b, hk, d, dtype=k.dtype, device="cuda").permute(1, 2, 0, 3)
+    v2 = torch.empty(hk, b, rows + 9, 2 * d, dtype=v.dtype, device="cuda").transpose(0, 1)[:, :, 4:rows + 4, d:]
+    for to, t in ((q2, q), (k2, k), (v2, v)):
+        to.copy_(t)
+    out = torch.full((b, h, n, d + 32), 7.0, dtype=q.dtype, device="cuda")
+    got = ops.tree_attention(q2, k2, v2, ln, par, out=out.transpose(1, 2)[..., :d])
+    assert torch.equal(got, want) and (out[..., d:] == 7.0).all()
+    some = [0, b - 1]
+    for scale in (1.0, -0.25, 0.0):
+        ref, tol = attention_ref(q[some], k[some], v[some], ln[some], par[some], scale=scale)
+        check(ops.tree_attention(q, k, v, ln, par, scale=scale)[some], ref, tol, f"scale {scale}")
+
+
+@pytest.mark.parametrize("types", [(F32, BF16), (BF16, BF16), (F16, F16)])
+def test_attention_shared_tiles_in_a_graph(ops, types):
+    """Lengths and trees that change under a captured launch whose blocks share tiles and keys."""
+    say(f"[gpu] tree attention: shared tiles in a graph {types}")
+    q, k, v, ln, par = layout_case(ops, types, (3, 130, 20, 20, 128, 2000), "tree", 500)
+    ops.tree_attention(q, k, v, ln, par)
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        out = ops.tree_attention(q, k, v, ln, par)
+    for turn, lengths in enumerate(([1870, 0, 3], [0, 0, 0], [-1, 1871, 1870], [700, 900, 1100])):
+        ln.copy_(ints(lengths))
+        par.copy_(ints([shape_tree(("tree", "star", "chain")[(turn + i) % 3], 130, turn) for i in range(3)]))
+        want = ops.tree_attention(q, k, v, ln, par)
+        gr.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out.nan_to_num(7.0), want.nan_to_num(7.0)), lengths
+        check(out[1:2], *attention_ref(q[1:2], k[1:2], v[1:2], ln[1:2], par[1:2]))
+
+
 @pytest.mark.parametrize("types", [(F32, BF16), (F32, F32), (BF16, BF16)])
 def test_attention_blocks_of_no_weight(ops, types):
     """A block's keys lie so far below the row's largest score that their weight is 0 as a float: what their values are, finite
