@@ -346,7 +346,7 @@ itts_status itts_decode_timing(itts_gpt *gpt, itts_kv *kv, int32_t mel_token_id,
  * checked on the host (ITTS_E_VALIDATION names the argument); what only the device knows (lengths,
  * parents, paths, tokens) is checked there, out-of-range values never reach memory and give the
  * results named below.  Strides are in elements; head_dim and vocab are contiguous.  Outputs
- * overlap no input.  A workspace belongs to one call until that call has finished on the device;
+ * overlap no input, nor do rows of one another.  A workspace belongs to one call until that call has finished on the device;
  * its contents need no initialisation. */
 
 /* Attention of the nodes of a tree of drafted tokens, one tree a sequence.  Node i of sequence b

@@ -2,9 +2,12 @@
 // checks and launches.  Nothing here allocates, waits or throws.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+#include <array>
 #include <atomic>
 #include <cstdarg>
 #include <cstdio>
+#include <cstdlib>
 
 #include "../../include/itts_hip.h"
 #include "kernels.h"
@@ -85,6 +88,48 @@ bool row_stride(int64_t stride, int extent, int size) {
   return extent <= 1 || (stride >= 0 && stride <= INT64_MAX / (16ll * extent) && stride * size % 16 == 0);
 }
 
+// Whether two rows of `row` elements share one, rows starting wherever multiples of the axes' strides add up to.
+// Strides that each step over all that the smaller ones reach keep rows apart.  Others may (0, 2 | 0, 3): then
+// differences of two rows' indices are tried, all axes but the longest one, which follows from the others; more
+// than a million of them count as an overlap.
+struct Axis {
+  int64_t stride, extent;
+};
+template <int N>
+bool rows_overlap(std::array<Axis, N> axes, int64_t row) {
+  std::sort(axes.begin(), axes.end(), [](const Axis &x, const Axis &y) { return x.extent <= 1 ? y.extent > 1 : y.extent > 1 && x.stride < y.stride; });
+  int64_t span = row;
+  bool nested = true;
+  for (const Axis &x : axes) {
+    if (x.extent <= 1) continue;
+    if (x.stride < row) return true;
+    nested = nested && x.stride >= span;
+    span += (x.extent - 1) * x.stride;
+  }
+  if (nested) return false;
+  std::sort(axes.begin(), axes.end(), [](const Axis &x, const Axis &y) { return x.extent < y.extent; });
+  double tries = 1;
+  for (int i = 0; i + 1 < N; i++) tries *= 2.0 * std::max<int64_t>(1, axes[i].extent) - 1;
+  if (tries > 1e6) return true;
+  const Axis last = axes[N - 1];
+  int64_t d[N] = {};
+  for (int i = 0; i + 1 < N; i++) d[i] = 1 - std::max<int64_t>(1, axes[i].extent);
+  for (;;) {
+    int64_t at = 0;
+    bool zero = true;
+    for (int i = 0; i + 1 < N; i++) at += d[i] * axes[i].stride, zero = zero && d[i] == 0;
+    const int64_t near = -at / last.stride;
+    for (int64_t e = near - 1; e <= near + 1; e++) {
+      const int64_t apart = at + e * last.stride;
+      if (e > -last.extent && e < last.extent && apart > -row && apart < row && !(zero && e == 0)) return true;
+    }
+    int i = 0;
+    while (i + 1 < N && d[i] + 1 >= std::max<int64_t>(1, axes[i].extent)) d[i] = 1 - std::max<int64_t>(1, axes[i].extent), i++;
+    if (i + 1 >= N) return false;
+    d[i]++;
+  }
+}
+
 itts_status tree_args(const itts_tree_attention_args *a, TreeAttn *o) {
   if (!a) return fail(ITTS_E_VALIDATION, "args: null");
   if (a->batch < 0 || a->batch > kMaxGridYZ) return fail(ITTS_E_VALIDATION, "batch: must be in 0..=%d, got %d", kMaxGridYZ, a->batch);
@@ -105,7 +150,7 @@ itts_status tree_args(const itts_tree_attention_args *a, TreeAttn *o) {
     return fail(ITTS_E_VALIDATION, "q: rows must start at multiples of 16 bytes");
   if (!row_stride(a->out_batch, b, qs) || !row_stride(a->out_node, n, qs) || !row_stride(a->out_head, h, qs) || !aligned16(a->out))
     return fail(ITTS_E_VALIDATION, "out: rows must start at multiples of 16 bytes");
-  if ((b > 1 && a->out_batch < a->head_dim) || (n > 1 && a->out_node < a->head_dim) || (h > 1 && a->out_head < a->head_dim))
+  if (rows_overlap<3>({{{a->out_batch, b}, {a->out_node, n}, {a->out_head, h}}}, a->head_dim))
     return fail(ITTS_E_VALIDATION, "out: rows must not overlap");
   if (!row_stride(a->k_batch, b, ks) || !row_stride(a->k_head, hk, ks) || !row_stride(a->k_row, a->max_seq, ks) || !aligned16(a->k))
     return fail(ITTS_E_VALIDATION, "k: rows must start at multiples of 16 bytes");
@@ -227,17 +272,25 @@ itts_status itts_cache_keep(const itts_cache_keep_args *a, void *stream) {
   for (int i = 0; i < 4; i++) {
     if (!row_stride(ks[i], ext[i], es) || !aligned16(a->k)) return fail(ITTS_E_VALIDATION, "k: rows must start at multiples of 16 bytes");
     if (!row_stride(vs[i], ext[i], es) || !aligned16(a->v)) return fail(ITTS_E_VALIDATION, "v: rows must start at multiples of 16 bytes");
-    if (ext[i] > 1 && (ks[i] < a->head_dim || vs[i] < a->head_dim)) return fail(ITTS_E_VALIDATION, "k, v: rows must not overlap");
   }
   if (a->batch > 1 && a->path_batch < 0) return fail(ITTS_E_VALIDATION, "path: negative stride");
   if (a->batch == 0) return ITTS_OK;
   if (!a->lengths || !a->new_lengths || (a->n_path && !a->path) || ((int64_t)a->n_layer * a->n_head && (!a->k || !a->v)))
     return fail(ITTS_E_VALIDATION, "k, v, lengths, path, new_lengths: null");
   if (a->lengths == a->new_lengths) return fail(ITTS_E_VALIDATION, "new_lengths: must not be lengths");
+  // Keys and values apart are one more axis where their strides are the same.
+  bool alike = true;
+  for (int i = 0; i < 4; i++) alike = alike && (ext[i] <= 1 || ks[i] == vs[i]);
+  const int64_t from_k = std::llabs(reinterpret_cast<intptr_t>(a->v) - reinterpret_cast<intptr_t>(a->k)) / es;
+  const bool rows = a->n_layer > 0 && a->n_head > 0;
+  if (rows && (rows_overlap<4>({{{ks[0], ext[0]}, {ks[1], ext[1]}, {ks[2], ext[2]}, {ks[3], ext[3]}}}, a->head_dim) ||
+               rows_overlap<4>({{{vs[0], ext[0]}, {vs[1], ext[1]}, {vs[2], ext[2]}, {vs[3], ext[3]}}}, a->head_dim) ||
+               (alike && from_k > 0 && from_k < INT64_MAX / 16 &&
+                rows_overlap<5>({{{ks[0], ext[0]}, {ks[1], ext[1]}, {ks[2], ext[2]}, {ks[3], ext[3]}, {from_k, 2}}}, a->head_dim))))
+    return fail(ITTS_E_VALIDATION, "k, v: rows must not overlap");
   // One memory for both moves once: two would read rows that the other has moved.
-  const bool same = a->k == a->v && a->n_layer > 0 && a->n_head > 0;
-  for (int i = 0; i < 4; i++)
-    if (same && ext[i] > 1 && ks[i] != vs[i]) return fail(ITTS_E_VALIDATION, "k, v: rows must not overlap");
+  const bool same = a->k == a->v && rows;
+  if (same && !alike) return fail(ITTS_E_VALIDATION, "k, v: rows must not overlap");
   int dev = 0, n_cu = 0;
   if (itts_status st = compute_units(&dev, &n_cu)) return st;
   if (itts_status st = check_device(dev, stream, {{a->k, "k"}, {a->v, "v"}, {a->lengths, "lengths"}, {a->n_path ? a->path : nullptr, "path"},

@@ -233,3 +233,22 @@ def test_tree_step_at_full_size(full_model):
             for j, node in enumerate(path):
                 want = g.step(cache, int(tokens[node]), 702 + j)
             assert np.abs(got[i] - want).max() < tol
+
+
+def test_tree_step_of_many_heads():
+    """A wide decoder's large tree: its attention's blocks share tiles and write the next product's operand themselves."""
+    say("[gpu] tree step of 80 heads")
+    W = synth.make_weights(dict(synth.SMALL_CONFIG, n_layer=1, n_head=80, d_model=5120, d_ffn=512), seed=29, init="rich")
+    g = H.Gpt(W)
+    pr = synth.make_prompt(W.cfg, 3, 20, seed=2)
+    for n in (130, 256):
+        cache = g.kv_cache(420, H.ITTS_BF16)
+        tokens, parents = _tree(n, W.cfg["mel_vocab"], n)
+        g.prefill(pr.text_tokens, pr.conds, pr.lang_id, cache)
+        got, _ = g.step_tree(cache, tokens, parents, 2)
+        for i in (0, n // 2, n - 1):
+            g.prefill(pr.text_tokens, pr.conds, pr.lang_id, cache)
+            for j, node in enumerate(_path(parents, i)):
+                want = g.step(cache, int(tokens[node]), 2 + j)
+            _close(got[i], want, TOL[H.ITTS_BF16], f"{n} nodes, node {i}")
+    g.close()

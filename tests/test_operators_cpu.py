@@ -120,6 +120,56 @@ def test_c_entries_refuse_overlaps_and_sizes_past_a_grid(kind, field, over):
     test_c_entries_refuse(kind, field, over)
 
 
+@pytest.mark.parametrize("kind,field,over", [
+    (tree, "out", dict(out_node=256, out_head=256)), (tree, "out", dict(out_batch=256, out_node=64, out_head=64)),
+    (tree, "out", dict(out_batch=1216)), (tree, "out", dict(batch=4, out_batch=128, out_node=192, n_nodes=4, out_head=10 ** 6)),
+    (keep, "k, v", dict(v=99 * P, k_batch=6400)), (keep, "k, v", dict(v=99 * P, v_head=64, v_row=64)), (keep, "k, v", dict(v=99 * P, k_layer=12800)),
+    (keep, "k, v", dict(v=P + 2 * 64)), (keep, "k, v", dict(v=P - 2 * 12800)), (keep, "k, v", dict(v=P + 16)),
+], ids=lambda x: getattr(x, "__name__", str(x)))
+def test_c_entries_refuse_axes_that_meet(kind, field, over):
+    """Strides that each step over a row, but together reach the same one twice; values one row behind the keys."""
+    test_c_entries_refuse(kind, field, over)
+
+
+def takes(a, kind):
+    """Whether the sizes pass: without a GPU the call then fails for that."""
+    try:
+        call(kind, a)
+    except H.ValidationError as e:
+        return "must not overlap" not in e.message
+    except H.IttsError:
+        pass
+    return True
+
+
+def test_rows_that_interleave_are_taken():
+    """Heads between rows, sequences between heads, keys beside values; steps of two and three rows that never meet."""
+    assert takes(tree(out_batch=64, out_node=512, out_head=128), tree)
+    assert not takes(tree(out_batch=192, out_node=128, n_nodes=2, parents_batch=2, out_head=320, n_head=4), tree)  # 320 = 192 + 128
+    assert takes(tree(out_batch=192, out_node=128, n_nodes=3, parents_batch=3, out_head=1024), tree)   # 0 2 4 | 3 5 7
+    assert takes(tree(out_batch=0, batch=1), tree) and takes(tree(out_head=0, n_head=1, n_kv_head=1), tree)
+    assert takes(keep(k_row=2 * 256, k_head=64, k_batch=2 * 12800 * 2, k_layer=2 * 12800 * 2 * 3, v=P + 2 * 256, v_row=2 * 256, v_head=64,
+                      v_batch=2 * 12800 * 2, v_layer=2 * 12800 * 2 * 3), keep)
+    assert takes(keep(v=P + 2 * 76800), keep) and takes(keep(v=P), keep)
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_overlaps_as_counted(seed):
+    """Random strides of three axes against a count of every element."""
+    import itertools
+    import random
+
+    rng = random.Random(seed)
+    for _ in range(150):
+        b, n, h = rng.randint(1, 4), rng.randint(1, 5), rng.choice([1, 2, 3, 4])
+        st = [64 * rng.choice([0, 1, 1, 2, 3, 4, 5, 7, 12, 20]) + rng.choice([0, 0, 16]) for _ in range(3)]
+        starts = [sum(i * s for i, s in zip(ix, st)) for ix in itertools.product(range(b), range(n), range(h))]
+        starts.sort()
+        meets = any(y - x < 64 for x, y in zip(starts, starts[1:]))
+        a = tree(batch=b, n_nodes=n, n_head=h, n_kv_head=1, out_batch=st[0], out_node=st[1], out_head=st[2])
+        assert takes(a, tree) == (not meets), (b, n, h, st)
+
+
 @pytest.mark.parametrize("first", ["from itts_hip import ops; H.version()", "H.version(); from itts_hip import ops"])
 def test_one_hip_runtime_or_a_refusal(first):
     """The library loads with its first call and then shares torch's HIP runtime; called before torch is there it has
