@@ -7,8 +7,8 @@
 
 They take torch tensors on one GPU and enqueue on that GPU's current stream: nothing waits, and
 a call may be captured into a graph.  Outputs and workspaces come from torch's allocator, so that
-calls on several streams, and captured ones, share nothing.  No gradients: the tensors are those of
-decoding.  Wrong arguments raise ``ValidationError`` naming the argument; what the operators do with
+calls on several streams, and captured ones, share nothing.  No gradients, in either mode: the tensors are
+those of decoding.  Wrong arguments raise ``ValidationError`` naming the argument; what the operators do with
 lengths, parents, paths and tokens that are out of range (the host cannot see them) is written at
 each function.
 
@@ -24,6 +24,7 @@ import struct
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import (ITTS_BF16, ITTS_E_VALIDATION, ITTS_F16, ITTS_F32, ValidationError, _check, itts_cache_keep_args,
                itts_token_scores_args, itts_tree_attention_args, lib)
@@ -53,8 +54,8 @@ def _refuse(message: str):
 
 
 def _tensor(t, name: str, dims: int, device=None, dtype=None, last=False):
-    """Checks a tensor; last: its last dimension must be contiguous.  (A call of an operator is host time before all
-    else: nothing is asked twice here, and strides are handed on.)"""
+    """Checks a tensor; device: the others' index; last: its last dimension must be contiguous.  (A call of an
+    operator is host time before all else: nothing is asked twice here, and strides are handed on.)"""
     if not isinstance(t, torch.Tensor):
         _refuse(f"{name}: a tensor is needed, got {type(t).__name__}")
     if t.dim() != dims:
@@ -64,13 +65,18 @@ def _tensor(t, name: str, dims: int, device=None, dtype=None, last=False):
             _refuse(f"{name}: float32, bfloat16 or float16 expected, got {t.dtype}")
     elif t.dtype != dtype:
         _refuse(f"{name}: {dtype} expected, got {t.dtype}")
-    if device is None or t.device != device:
+    if device is None or t.get_device() != device:
         if not t.is_cuda:
             _refuse(f"{name}: a GPU tensor is needed, got one on {t.device}")
         if device is not None:
-            _refuse(f"{name}: on {t.device}, the other tensors on {device}")
+            _refuse(f"{name}: on {t.device}, the other tensors on cuda:{device}")
     if t.requires_grad and torch.is_grad_enabled():
         _refuse(f"{name}: requires a gradient, which this operator does not give")
+    if dtype is not torch.int32:  # (what its memory does not show)
+        if t.is_neg():
+            _refuse(f"{name}: is negated when it is read, its memory is not what it says (resolve_neg() gives one that is)")
+        if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+            _refuse(f"{name}: has a forward-mode tangent, which this operator does not give")
     strides = t.stride()
     if last and strides[-1] != 1 and t.shape[-1] > 1:
         _refuse(f"{name}: the last dimension must be contiguous")
@@ -120,14 +126,14 @@ def _on_device(op):
 def _run(fn, need, args, device):
     """Enqueues on the current device's stream, with the workspace that the sizes need."""
     if need is None:
-        return _check(fn(args, _stream(device.index)))
+        return _check(fn(args, _stream(device)))
     size = C.c_uint64()
     _check(need(args, C.byref(size)))
     bytes_ = size.value
     if not bytes_:
-        return _check(fn(args, None, 0, _stream(device.index)))
+        return _check(fn(args, None, 0, _stream(device)))
     ws = _empty((bytes_,), (1,), torch.uint8)
-    _check(fn(args, ws.data_ptr(), bytes_, _stream(device.index)))
+    _check(fn(args, ws.data_ptr(), bytes_, _stream(device)))
 
 
 @_on_device
@@ -152,7 +158,7 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: t
     A node sees its sequence's rows, its ancestors and itself.  A negative length, or one whose nodes do not
     fit, gives rows of NaN.  Returns out [batch][nodes][heads][dim] in q's type."""
     sq = _tensor(q, "q", 4, last=True)
-    dev = q.device
+    dev = q.get_device()
     sk = _tensor(k, "k", 4, dev, last=True)
     sv = _tensor(v, "v", 4, dev, last=True)
     sl = _tensor(lengths, "lengths", 1, dev, torch.int32)
@@ -205,7 +211,7 @@ def token_scores(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, to
     A row of -inf alone gives every token -inf, and entropy 0.  A NaN or +inf makes its row's
     log-probabilities and entropy NaN; NaN counts as -inf in the order.  log_probs has tokens' shape."""
     sx = _tensor(logits, "logits", 2, last=True)
-    dev = logits.device
+    dev = logits.get_device()
     r, vocab = logits.shape
     given, log_probs, tok, log_probs_at, tok_row = 0, None, 0, 0, 0
     if tokens is not None:
@@ -241,7 +247,7 @@ def cache_keep(k: torch.Tensor, v: torch.Tensor, lengths: torch.Tensor, path: to
     leaves the cache, or a negative length."""
     dims = 4 if isinstance(k, torch.Tensor) and k.dim() == 4 else 5
     sk = _tensor(k, "k", dims, last=True)
-    dev = k.device
+    dev = k.get_device()
     sv = _tensor(v, "v", dims, dev, k.dtype, last=True)
     sl = _tensor(lengths, "lengths", 1, dev, torch.int32)
     sp = _tensor(path, "path", 2, dev, torch.int32, last=True)

@@ -809,6 +809,40 @@ def test_gpu_refusals(ops):
     assert ops.token_scores(torch.zeros(2, 9, device="cuda")).entropy.shape == (2,)  # and the next call works
 
 
+def test_tensors_that_are_not_what_their_memory_holds(ops):
+    """Lazily negated tensors and ones with a forward-mode tangent: refused, by name; resolved and primal ones served."""
+    from torch.autograd import forward_ad
+    say("[gpu] lazy negations and forward-mode tangents")
+    g = gen(31)
+    q, k, v = randn(g, 1, 2, 2, 64), randn(g, 1, 2, 12, 64), randn(g, 1, 2, 12, 64)
+    ln, par, path = ints([5]), ints([[-1, 0]]), ints([[1]])
+    x = randn(g, 3, 20)
+    want, best = ops.tree_attention(q, k, v, ln, par), ops.token_scores(x, None, 2)
+
+    def negated(t):
+        return torch.complex(torch.zeros_like(t), -t).conj().imag  # reads as t, holds -t
+
+    def calls(change):
+        return [("q", lambda: ops.tree_attention(change(q), k, v, ln, par)), ("k", lambda: ops.tree_attention(q, change(k), v, ln, par)),
+                ("v", lambda: ops.tree_attention(q, k, change(v), ln, par)),
+                ("out", lambda: ops.tree_attention(q, k, v, ln, par, out=change(torch.zeros_like(q)))),
+                ("logits", lambda: ops.token_scores(change(x), None, 2)), ("k", lambda: ops.cache_keep(change(k), v.clone(), ln, path)),
+                ("v", lambda: ops.cache_keep(k.clone(), change(v), ln, path))]
+
+    n = negated(torch.ones(2, device="cuda"))
+    assert n.is_neg() and n.tolist() == [1.0, 1.0]
+    for name, call in calls(negated):
+        with pytest.raises(H.ValidationError, match=f"{name}: .*resolve_neg"):
+            call()
+    assert torch.equal(ops.tree_attention(negated(q.transpose(1, 2)).transpose(1, 2).resolve_neg().contiguous(), k, v, ln, par), want)
+    with forward_ad.dual_level():
+        for name, call in calls(lambda t: forward_ad.make_dual(t, torch.ones_like(t))):
+            with pytest.raises(H.ValidationError, match=f"{name}: .*tangent"):
+                call()
+        assert torch.equal(ops.tree_attention(q, k, v, ln, par), want)
+        assert torch.equal(ops.token_scores(x, None, 2).top_tokens, best.top_tokens)
+
+
 def test_arguments_by_name(ops):
     """Every argument by its name, in any order."""
     say("[gpu] arguments by name")
