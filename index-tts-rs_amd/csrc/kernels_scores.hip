@@ -191,7 +191,7 @@ template <int TYPE, bool LONG>
 __global__ __launch_bounds__(kThreads, LONG ? 4 : 6) void token_scores_kernel(TokenScores a, int S) {
   __shared__ float red[kWaves][4];
   __shared__ Select sel;
-  constexpr int P = kPer<TYPE>, kBytes = 16 / P, kRound = kThreads * kPieces * P;
+  constexpr int P = kPer<TYPE>, kBytes = 16 / P;
   const int r = blockIdx.x / S, split = blockIdx.x % S, t = threadIdx.x;
   const char *x = static_cast<const char *>(a.x) + r * a.x_row * kBytes;
   const int n = a.top;
