@@ -12,9 +12,11 @@
 // against each other.  Where many pass (masks of one low value, ties, rising rows) the n-th value is found first:
 // 64 rows of 8,194 with all but five at the type's lowest value, 64 alternatives, 15 us a call (12 without a
 // mask); n rounds over the row took 438.  Rows that are few and long are split over blocks and joined by a second
-// kernel.  Bound by instructions, 12 an element (one of them the exponential), where memory would
-// take half to three quarters of the time: 2,188 fp32 rows of 8,194 with 5 alternatives 19 us (72 MB), 1,000 bf16
-// rows of 60,510 with 20 49 us (121 MB); one row of 8,194 6.2 us.
+// kernel.  Vector instructions an element, as counted: 23 where a block holds its row at once, 19 in longer rows,
+// one of them the exponential; memory alone would take half to three quarters of the time.  Waves of short rows wait
+// 40% of their cycles for data or barriers and 39% for an issue slot, those of long rows 56% and 15%.  2,188 fp32
+// rows of 8,194 with 5 alternatives 19 us (72 MB), 1,000 bf16 rows of 60,510 with 20 50 us (121 MB); one row of
+// 8,194 6.2 us.
 #include <algorithm>
 
 #include "kernels.h"
@@ -185,7 +187,7 @@ __device__ inline void write_row(const TokenScores &a, int r, const void *x, con
 __host__ __device__ inline size_t list_offset(int rows, int S) { return sizeof(Stats) * (size_t)rows * S; }
 
 // LONG: a block's tokens are more than its threads hold, and the next ones are on their way while these
-// are counted: 1,000 rows of 60,510 50 us, without 54 (also with half the registers and more blocks a unit), and 49
+// are counted: 1,000 rows of 60,510 50 us, without 54 (also with half the registers and more blocks a unit), and 49 to 50
 // since later turns look for tokens above the n-th so far alone.
 template <int TYPE, bool LONG>
 __global__ __launch_bounds__(kThreads, LONG ? 4 : 6) void token_scores_kernel(TokenScores a, int S) {

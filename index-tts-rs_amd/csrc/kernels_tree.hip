@@ -255,10 +255,10 @@ struct Args {
 // n blocks (0: nothing is left for this one).  Every block gets the same number of rows, whatever
 // the sequences' lengths and however long the cache could become: the smallest one with which `parts`
 // blocks are enough (within a few percent).  Every wave finds it by itself from the lengths, a lane a
-// sequence.  12 x 64 nodes over 1,000 .. 8,191 rows, 8 key heads: 115 us with the rows of max_seq shared
-// equally, 107 with these.  A block still waits for the longest one, a fifth above the mean there; runs
-// that go on into the next sequence made that kernel 7 us faster and the one for few rows 1 to 10
-// slower (registers kept over the turns, a second start), and are not taken.
+// sequence.  12 x 64 nodes over 1,000 .. 8,191 rows, 8 key heads: with the rows of max_seq shared equally
+// 115 us, with these 107 (one plane of probabilities, 131 with two).  A block still waits for the longest
+// one, a fifth above the mean there; runs that go on into the next sequence made that kernel 7 us faster and the one
+// for few rows 1 to 10 slower (registers kept over the turns, a second start), and are not taken.
 struct Share {
   int b, n, first, end, index, from;
 };
@@ -666,10 +666,10 @@ __device__ __forceinline__ float put4(const Args &p, const Share &share, int hk,
 
 // Few query rows: 4 waves over tiles of keys of their own, straight from memory into registers, one
 // tile ahead; joined at the end.  Long caches are bound by memory: 2 x 16 heads, 61 nodes, 40,001 and 65,500
-// fp16 rows, 433 MB, 81 us; 32 single tokens, 4 key heads of 128, 513 .. 4,097 bf16 rows, 152 MB, 27.  Short ones
-// by the chain from load to result: 8 nodes, 20 heads, 235 rows 6.0 us.  fp32 caches by the fp32
-// products, of 4 keys at a time: 33 nodes, 20 heads, 1,734 rows 12.7 us.  fp32 queries over bf16 by the
-// three planes' instructions: 8 x 27 nodes, 250 .. 1,400 rows 15.7 us.
+// fp16 rows, 433 MB, 79 us; 32 single tokens, 4 key heads of 128, 513 .. 4,097 bf16 rows, 152 MB, 27.  Short ones
+// by the chain from load to result: 8 nodes, 20 heads, 235 rows 6.3 us.  fp32 caches by the fp32
+// products, of 4 keys at a time: 33 nodes, 20 heads, 1,734 rows 13.3 us.  fp32 queries over bf16 by the
+// three planes' instructions: 8 x 27 nodes, 250 .. 1,400 rows 16.3 us.
 template <int D, class TQ, class TKV, int RT, int W>
 __global__ __launch_bounds__(256, 2) void tree_attn_kernel(Args p) {
   constexpr int WK = kKeyWaves;
@@ -793,12 +793,12 @@ __global__ __launch_bounds__(256, 2) void tree_attn_kernel(Args p) {
 // order p ^ row: what a wave reads at a time, one piece of 16 key rows or two neighbours of 16 value
 // rows, falls on different banks.  Values are read through the transposing load: lane 4 j + a of 16
 // reads elements 4 a .. of row j, and lane i gets element i of the four rows.
-// 12 x 64 nodes, 32 heads of 128 over 8 key heads, 1,000 .. 8,191 bf16 rows: 98 us, 480 TFLOP/s.  The matrix
-// units are busy 38% of its cycles (at 1.65 GHz: the card lowers its clock under this load), the waves
-// wait a third of theirs for an issue slot and a third for data or the barrier.  Tiles two ahead in
-// registers spilled (161 us for 144 then), and two ahead by direct loads to LDS gain 4% at best; blocks of
-// 8 waves read every tile half as often and are no faster (103 us with the joining for 104; 2 x 144 nodes over
-// 3,700 rows 38, 38).
+// 12 x 64 nodes, 32 heads of 128 over 8 key heads, 1,000 .. 8,191 bf16 rows: 132 us, 355 TFLOP/s.  The matrix
+// units are busy 43% of its cycles (at 1.6 GHz: the card lowers its clock under this load), the waves
+// wait 41% of theirs for an issue slot and 20% for data or the barrier.  With one plane of probabilities
+// (98 us) tiles two ahead in registers spilled (161 us for 144 then), and two ahead by direct loads to LDS gained 4% at
+// best; blocks of 8 waves read every tile half as often and were no faster (103 us with the joining for 104;
+// 2 x 144 nodes over 3,700 rows 38, 38).
 template <int D, class TQ, class TKV, int RT, int W>
 __global__ __launch_bounds__(64 * kRowWaves, 2) void tree_attn_rows_kernel(Args p) {
   constexpr int WR = kRowWaves, kPieces = D * TKV::kBytes / 16, kThreads = 64 * WR, kTile = kTileKeys * kPieces, kCopy = 2 * kTile / kThreads;
@@ -948,7 +948,7 @@ __global__ __launch_bounds__(64 * kRowWaves, 2) void tree_attn_rows_kernel(Args 
 
 // Joins the blocks' results of a row: a wave a row, D / 4 lanes with four elements each for every fourth
 // (D 128: second) block, added in their order there and then over the lane groups.  Bound by memory where
-// it counts: 33 MB of results 11 us.
+// it counts: 33 MB of results 12 us.
 template <int D, class TQ>
 __global__ __launch_bounds__(256) void tree_join_kernel(Args p) {
   constexpr int kLanes = D / 4, kGroups = 64 / kLanes;
@@ -1018,14 +1018,18 @@ struct Plan {
 // The time of a layout: a block's start and end, and for every 2^unit keys `turn`, as often as a compute
 // unit has blocks (in pairs, those with shared tiles); dealing a sequence's keys
 // to several blocks adds a wait for the lengths, the second launch and its traffic.  The figures (us) are
-// those of launches that fill the card, right to about a tenth.  What they decide, over 3,000 | 300 rows:
-//   bf16, 4 x 16 heads of 64, 64 nodes            RT 1 22.6 | 6.6   RT 2 23.2 | 7.9    RT 4 20.8 | 10.4   shared 24.8 | 12.4
-//   bf16, 4 x 8 key heads of 128, 128 rows each   RT 1 35.1 | 8.7   RT 2 29.3 | 10.6   shared 31.2 | 16.2
-//   the same, 256 rows each                       RT 1 61.9 | 12.6  RT 2 35.8 | 11.0   shared 38.5 | 17.4
-//   fp32 over bf16, 2 x 20 heads of 64, 48 nodes  RT 1 22.2 | 7.1   RT 2 20.4 | 9.3    shared 27.6 | 16.7
-//   256 rows each, 12 sequences up to 8,191 rows  RT 2 232          shared 104
-// and fp32 caches, 20 heads of 64, 1,734 rows: 48 nodes RT 1 15, RT 2 18; 3 x 4 key heads, 189 rows each, up to
-// 5,936 rows 46, 43.
+// those of launches that fill the card.  Given the sequences' mean length, they lie between 0.65 and 1.09 of what nine in ten of
+// 304 layouts of 16-bit caches take (median 0.94; low where lengths differ or trees are larger than 64 nodes).  Of
+// 311 shapes whose sequences use 0.65 to 1 of max_seq, where half is expected, the layout taken was 4% slower than the
+// best of all on average, more than 10% in 40, 43% at worst.  What they decide, over 3,000 | 300 rows that all
+// sequences use (one block a sequence or dealt, whichever is faster):
+//   bf16, 4 x 16 heads of 64, 64 nodes            RT 1 21.8 | 6.5   RT 2 20.4 | 7.6    RT 4 20.2 | 10.0   shared 28.2 | 13.8
+//   bf16, 4 x 8 key heads of 128, 128 rows each   RT 1 32.5 | 8.2   RT 2 27.9 | 10.4   shared 34.3 | 17.2
+//   the same, 256 rows each                       RT 1 58.8 | 12.9  RT 2 35.2 | 11.0   shared 44.1 | 19.2
+//   fp32 over bf16, 2 x 20 heads of 64, 48 nodes  RT 1 19.0 | 7.0   RT 2 19.6 | 9.2    shared 28.1 | 15.5
+//   256 rows each, 12 sequences up to 8,191 rows  RT 2 235          shared 139
+// and fp32 caches, 20 heads of 64, 1,734 rows: 48 nodes RT 1 15.7, RT 2 18.6; 3 x 4 key heads, 189 rows each, up to
+// 5,936 rows 51, 44.
 Plan plan_of(const TreeAttn &a, int n_cu, int RT, bool shared) {
   Plan p;
   const int M = a.n * (a.H / a.Hk), per = 16 * RT * (shared ? kRowWaves : 1);
@@ -1047,8 +1051,8 @@ Plan plan_of(const TreeAttn &a, int n_cu, int RT, bool shared) {
   const double rows = std::max(1.0, (double)a.used * a.max_seq), units = std::ceil(rows / (1 << p.unit));
   p.us = (start + units * turn) * (((int64_t)a.batch * groups + at_once - 1) / at_once);
   // A block a compute unit: 2 x 16 heads over 40,001 and 65,500 rows 86 us, two a unit 90, half as many
-  // 128.  Two of shared tiles: 2 x 20 heads, 84 nodes over 15,765 rows 48 us, one a unit 62; 24 x 4 key heads, 72 rows over
-  // 4,748 .. 5,359 58, 80.
+  // 128.  Two of shared tiles, with one plane of probabilities: 2 x 20 heads, 84 nodes over 15,765 rows 48 us, one a unit 62;
+  // 24 x 4 key heads, 72 rows over 4,748 .. 5,359 58, 80 (with two planes 64 and 77, two a unit).
   p.parts = (int)std::min<int64_t>(at_once / groups, 64ll * a.batch);
   // (row tiles with the same keys on the same eighth of the card, which has an L2 of its own: 6 heads of a
   // key head, 6 nodes, 2 x 52,834 rows 36 -> 29 us)
