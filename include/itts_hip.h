@@ -40,7 +40,8 @@ typedef enum itts_status {
   ITTS_E_INTERNAL = 5
 } itts_status;
 
-typedef enum itts_dtype { ITTS_F16 = 1, ITTS_F32 = 2, ITTS_BF16 = 3 } itts_dtype;
+/* ITTS_I4: paged caches alone (itts_pages). */
+typedef enum itts_dtype { ITTS_F16 = 1, ITTS_F32 = 2, ITTS_BF16 = 3, ITTS_I4 = 4 } itts_dtype;
 
 /* Decoder shape.  The reference fixes it (gpt.rs:31-54): 24 layers, d_model 1280,
  * 20 heads of 64, d_ffn 5120, Mel vocab 8194, text vocab 60510, lang vocab 107,
@@ -422,6 +423,113 @@ typedef struct itts_cache_keep_args {
   int64_t path_batch;
 } itts_cache_keep_args;
 itts_status itts_cache_keep(const itts_cache_keep_args *args, void *stream);
+
+/* ---- operators on device memory: paged caches (no reference counterpart) ----
+ * The conventions of the operators above.  Keys and values lie in n_pages pages of page_size rows a key head, k and v
+ * [n_pages][n_kv_head][page_size][head_dim]; row r of sequence b is row r % page_size of page table[b][r / page_size]
+ * (table [batch][n_table]; sequences may share pages that nothing writes).  Entries of a table that no visible row lies in are
+ * not used.  page_size is a multiple of 16, up to 65536; head_dim 64 or 128; a sequence has at most 2^24 rows.
+ * dtype F32, BF16, F16, or I4: rows are then head_dim / 2 bytes (strides in bytes), two codes each, the lower half first, and
+ * k_params and v_params hold (scale, base) pairs of float16 for every 64 elements, [n_pages][n_kv_head][page_size]
+ * [head_dim / 64][2] (the last two dimensions contiguous; strides in float16): value = scale * code + base.  Rows start at
+ * multiples of 16 bytes, pairs at multiples of 4 * (head_dim / 64).
+ *
+ * Tokens of a batch stand one sequence after the other, those of sequence b from starts[b] to starts[b + 1] - 1 (starts
+ * [batch + 1], rising, equal for a sequence without any).  A sequence whose starts fall or leave the n_tokens has none. */
+typedef struct itts_pages {
+  void *k, *v;
+  void *k_params, *v_params;
+  int32_t n_pages, page_size, n_kv_head, head_dim;
+  itts_dtype dtype;
+  int64_t k_page, k_head, k_row;
+  int64_t v_page, v_head, v_row;
+  int64_t k_params_page, k_params_head, k_params_row;
+  int64_t v_params_page, v_params_head, v_params_row;
+} itts_pages;
+
+/* Appends tokens' keys and values k, v [n_tokens][n_kv_head][head_dim] to their sequences: token i of sequence b becomes row
+ * lengths[b] + i; new_lengths[b] = lengths[b] + its tokens.  With `rotation` [n_positions][n_rotated], each row n_rotated / 2
+ * cosines, then the sines of the same angles, the first n_rotated elements of keys turn by those of the token's position
+ * (positions[token], or its row where positions is NULL): (x, y) -> (x cos - y sin, y cos + x sin), pairs being elements
+ * i and i + n_rotated / 2, or with `interleaved` 2 i and 2 i + 1.  q [n_tokens][n_head][head_dim] (n_head 0: none) turns the same
+ * way into q_out, which may be q.  A position outside the table gives NaN.
+ * I4: base = min x and scale = (max x - min x) / 15 of every 64 turned elements x, each rounded to float32 and to
+ * float16, code = (x - base) / scale to the nearest (ties to even) in 0 .. 15, 0 where scale is 0; 64 elements with
+ * one that is no finite number, or beyond float16's, read back as NaN.
+ * A sequence with a negative length or no room (n_table pages, 2^24 rows) is not written, nor is a row whose page is not in
+ * 0 .. n_pages - 1: its new length is -1 (and its q_out NaN in the first case).  Rows of q_out of tokens outside all sequences are
+ * zeros.  Rows of one page must not be written by two sequences.
+ * dtype (of k, v, q): the pages', F32 over BF16, or any over I4.  n_rotated is a multiple of 16. */
+typedef struct itts_paged_append_args {
+  itts_pages pages;
+  const void *k, *v, *q;
+  void *q_out;
+  const float *rotation;
+  const int32_t *starts, *lengths, *table, *positions;
+  int32_t *new_lengths;
+  int32_t batch, n_tokens, n_head, n_table, n_rotated, n_positions, interleaved;
+  itts_dtype dtype;
+  int64_t k_token, k_head, v_token, v_head, q_token, q_head, q_out_token, q_out_head;
+  int64_t rotation_row, table_batch;
+} itts_paged_append_args;
+itts_status itts_paged_append(const itts_paged_append_args *args, void *stream);
+
+/* Attention of tokens over their sequences' rows.  The n tokens of sequence b are its last ones (appended before): token i
+ * has position p = lengths[b] - n + i and sees the rows t <= p, with window > 0 only those with t > p - window or
+ * t < sinks (sinks first rows that stay in sight):
+ *   out_i = sum_t softmax_t(scale q_i . k_t) v_t.
+ * A token at a negative position sees nothing: zeros.  Tokens of a sequence with a length that is negative or above max_rows,
+ * and tokens that see a row whose page is not in 0 .. n_pages - 1, get NaN.  Values in rows that a token does not see never
+ * reach it, NaN and infinities among them.  Rows of tokens outside all sequences are zeros.
+ * q, out [n_tokens][n_head][head_dim], query head h with key head h / (n_head / n_kv_head).  q_dtype: as in itts_paged_append.
+ * max_rows: the longest length that may come, at most n_table pages. */
+typedef struct itts_paged_attention_args {
+  itts_pages pages;
+  const void *q;
+  void *out;
+  const int32_t *starts, *lengths, *table;
+  int32_t batch, n_tokens, n_head, n_table, max_rows, window, sinks;
+  itts_dtype q_dtype;
+  float scale;
+  int64_t q_token, q_head, out_token, out_head, table_batch;
+} itts_paged_attention_args;
+itts_status itts_paged_attention_workspace(const itts_paged_attention_args *args, uint64_t *bytes);
+itts_status itts_paged_attention(const itts_paged_attention_args *args, void *workspace, uint64_t workspace_bytes, void *stream);
+
+/* The first n_rows rows of every sequence out of its pages into k and v [batch][n_kv_head][n_rows][head_dim], zeros from
+ * lengths[b] on: caches of one piece, as itts_tree_attention takes them.  Rows of a sequence with a bad length, and rows in a page
+ * that does not exist, are NaN.  dtype: the pages', or for I4 any (the codes' values, rounded once). */
+typedef struct itts_paged_gather_args {
+  itts_pages pages;
+  void *k, *v;
+  const int32_t *lengths, *table;
+  int32_t batch, n_rows, n_table;
+  itts_dtype dtype;
+  int64_t k_batch, k_head, k_row, v_batch, v_head, v_row, table_batch;
+} itts_paged_gather_args;
+itts_status itts_paged_gather(const itts_paged_gather_args *args, void *stream);
+
+/* Rows of logits [rows][vocab] (F32, BF16, F16) as the next token is to be chosen from them, to out (of the same type; it
+ * may be logits, with the same stride).  With c the times that token t stands in history[row] [n_history]:
+ *   c > 0:  x = (x < 0 ? x * repetition : x / repetition) - (frequency * c + presence)
+ *   then    x += bias of t in the row's (bias_tokens, bias) [n_bias] (the last one, where t is there more than once)
+ *   then    x = -inf unless bit t % 32 of allowed[row][t / 32] is set (allowed NULL: every token may follow).
+ * Computed in float32, rounded once to the type.  Entries of lists outside the vocabulary count for nothing.  repetition,
+ * frequency, presence: [rows], or NULL for the value in *_all.  n_history and n_bias <= 65535; row strides may be 0. */
+typedef struct itts_adjust_logits_args {
+  const void *logits;
+  void *out;
+  const int32_t *history;
+  const int32_t *bias_tokens;
+  const float *bias;
+  const uint32_t *allowed;
+  const float *repetition, *frequency, *presence;
+  float repetition_all, frequency_all, presence_all;
+  int32_t rows, vocab, n_history, n_bias;
+  itts_dtype dtype;
+  int64_t logits_row, out_row, history_row, bias_tokens_row, bias_row, allowed_row;
+} itts_adjust_logits_args;
+itts_status itts_adjust_logits(const itts_adjust_logits_args *args, void *stream);
 
 /* ---- Stage-2 CFM DiT estimator and Euler / CFG solver (crates/core/src/models/cfm.rs) ----
  * Replaces CfmDit (cfm.rs:411-761): the 13-layer U-ViT transformer (AdaLN over RMSNorm,

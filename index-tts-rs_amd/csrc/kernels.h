@@ -306,7 +306,7 @@ hipError_t sampler_stage_init(int dev);
 bool sampler_stage(int dev, SamplerStage *out);
 
 // ---- decoding with drafted trees (kernels_tree.hip, kernels_scores.hip) ----
-enum OpType : int { kOpF32 = 0, kOpBf16 = 1, kOpF16 = 2 };
+enum OpType : int { kOpF32 = 0, kOpBf16 = 1, kOpF16 = 2, kOpI4 = 3 };
 constexpr int kTreeMaxNodes = 256;
 constexpr int kTreeMaxRowBytes = 1 << 26;  // cache rows apart: 32 of them within 32 bits of offset
 // Attention of the nodes of one tree a sequence over its cached rows and their own ancestors.
@@ -343,6 +343,64 @@ struct CacheKeep {
   int caches = 2;                                           // 1: v is k
 };
 hipError_t cache_keep(const CacheKeep &a, hipStream_t s);
+// ---- paged caches ----
+// Pages of `size` rows a key head; row r of sequence b is row r % size of page table[b][r / size].  kOpI4: rows of D / 2
+// bytes, two codes each, and D / 64 (scale, base) pairs of fp16.  Strides in bytes.
+constexpr int kPagesMaxRows = 1 << 24;  // of a sequence
+struct Pages {
+  char *k, *v, *kp, *vp;
+  int n, size, Hk, D, type;
+  int64_t k_p, k_h, k_r, v_p, v_h, v_r, kp_p, kp_h, kp_r, vp_p, vp_h, vp_r;
+};
+// Tokens starts[b] .. starts[b + 1] - 1 of k and v [tokens][Hk][D] into rows lengths[b] .. of sequence b, those of k rotated, and
+// of q [tokens][H][D] rotated to q_out.  Strides of tensors in elements.
+struct PagedAppend {
+  Pages pages;
+  const void *k, *v, *q;
+  void *q_out;
+  const float *rotation;  // [positions][rot]: cosines, then sines (null: none)
+  const int32_t *starts, *lengths, *table, *positions;
+  int32_t *new_lengths;
+  int batch, tokens, H, n_table, rot, n_positions, interleaved, type;
+  int64_t k_t, k_h, v_t, v_h, q_t, q_h, o_t, o_h, rot_r, tab_b;
+};
+hipError_t paged_append(const PagedAppend &a, hipStream_t s);
+// Rows of sequences to k and v [batch][Hk][rows][D] of `type`; zeros behind a sequence's length.
+struct PagedGather {
+  Pages pages;
+  void *k, *v;
+  const int32_t *lengths, *table;
+  int batch, rows, n_table, type;
+  int64_t k_b, k_h, k_r, v_b, v_h, v_r, tab_b;
+};
+hipError_t paged_gather(const PagedGather &a, hipStream_t s);
+// Attention of tokens [tokens][H][D], the last ones of their sequences, over their sequences' rows.
+struct PagedAttn {
+  Pages pages;
+  const void *q;
+  void *out;
+  const int32_t *starts, *lengths, *table;
+  int batch, tokens, H, n_table, max_rows, type, window, sinks;
+  float scale;
+  int64_t q_t, q_h, o_t, o_h, tab_b;
+  float *part;  // paged_attn_ws(a, n_cu) floats
+};
+size_t paged_attn_ws(const PagedAttn &a, int n_cu);
+hipError_t paged_attn(const PagedAttn &a, int n_cu, hipStream_t s);
+// Logits [rows][vocab] under penalties for the tokens of a history, biases and a mask of allowed tokens.
+constexpr int kAdjustMaxList = 65535;  // entries of a history, or of biases
+struct AdjustLogits {
+  const void *x;
+  void *out;
+  const int32_t *history, *bias_tokens;
+  const float *bias;
+  const uint32_t *allowed;
+  const float *repetition, *frequency, *presence;  // [rows], or null: the value below for every row
+  float repetition_all, frequency_all, presence_all;
+  int rows, vocab, n_history, n_bias, type;
+  int64_t x_row, out_row, history_row, bias_tokens_row, bias_row, allowed_row;
+};
+hipError_t adjust_logits(const AdjustLogits &a, int n_cu, hipStream_t s);
 // Rows of logits: log-probabilities of given tokens, entropy, the top_n most probable tokens.
 constexpr int kScoresMaxTop = 64;
 struct TokenScores {

@@ -1,0 +1,773 @@
+// Attention over paged caches: the tokens of ragged sequences (single ones, pieces of prompts) over their sequences' rows.
+//
+// The n tokens of sequence b are its last ones: token i has position P = lengths[b] - n + i and sees the rows t <= P, with a
+// window W the rows t > P - W and t < S (the first ones, which stay in sight) alone:
+//   o_i = sum_t p_it v_t / sum_t p_it,   p_it = exp(scale q_i . k_t - m_i).
+// The rows (token, head of the group) that share a key head are the columns of the products (attn_tiles.h); row r is head
+// r % group of token r / group.  Keys go by in tiles of 32; pages are multiples of 16 rows, so that each half of a tile lies in
+// one page, whose number comes through the scalar cache a tile ahead of its rows.
+#include <algorithm>
+#include <cmath>
+#include <numeric>
+#include <type_traits>
+
+#include "attn_tiles.h"
+#include "pages.h"
+
+namespace itts {
+namespace {
+
+// A cache of 4 bits.
+struct I4 {};
+
+// A launch: blocks of kTileRows rows of a sequence and key head, each with all keys that they see (parts 0) or with a share
+// of them and results of its own (o [Hk][parts][rows][D], then (max, sum) [Hk][parts][rows], then (first block, blocks of a
+// row tile) [batch]) that a second kernel joins.
+struct Args {
+  PagedAttn a;
+  int blocks, parts, group;
+  uint32_t group_mul;  // 2^32 / group, rounded up: exact for rows < 2^32 / group
+  uint64_t page_mul;
+  int unit, least;     // a share is at least `least` times 2^unit tiles of keys
+  float2 *ml;
+  int2 *dealt;
+  __device__ int token(int row) const { return group == 1 ? row : __umulhi((uint32_t)row, group_mul); }
+};
+
+// The tiles of 32 keys that the tokens at positions p0 .. p1 of a sequence see, counted through: those with rows < S,
+// then from the window's first one on.
+struct Tiles {
+  int front, skip, n;
+  __device__ __forceinline__ Tiles(const PagedAttn &a, int p0, int p1) {
+    const int from = a.window > 0 ? max(0, p0 - a.window + 1) >> 5 : 0;
+    front = min((a.sinks >> 5) + ((a.sinks & 31) != 0), from);
+    skip = from - front;
+    n = p1 < 0 ? 0 : front + (p1 >> 5) + 1 - from;
+  }
+  __device__ __forceinline__ int key(int u) const { return (u < front ? u : u + skip) * kTileKeys; }
+};
+
+// What block `index` has to do: tiles [first, end) of row tile `tile` of sequence b, whose rows are shared by n blocks (0:
+// nothing is left for this one).  Every share has the same size, the smallest one with which `blocks` are enough.  Found by
+// every wave from the starts and lengths, a lane a sequence.  A sequence's last tokens, which see most, come first.
+struct Share {
+  int b, tile, n, first, end, from;
+};
+template <int ROWS>
+__device__ __forceinline__ Share share_of(const Args &p, int index) {
+  const PagedAttn &a = p.a;
+  const int lane = threadIdx.x & 63;
+  // row tiles of a sequence, and the units of keys that one of them sees at most
+  auto count = [&](int b, int &tiles, int &units) {
+    tiles = 0, units = 0;
+    if (b >= a.batch) return;
+    const Span span = span_of(a.starts[b], a.starts[b + 1], a.tokens);
+    const int len = a.lengths[b], rows = span.n * p.group;
+    tiles = (rows + ROWS - 1) / ROWS;
+    int seen = len < 0 || len > a.max_rows ? 1 : max(len, 1);
+    if (a.window > 0) seen = (int)min((int64_t)seen, (int64_t)a.window + min(a.sinks, a.max_rows) + (ROWS - 1) / p.group + 1 + 2 * kTileKeys);
+    units = tiles == 0 ? 0 : ((seen + kTileKeys - 1) / kTileKeys + (1 << p.unit) - 1) >> p.unit;
+  };
+  int size = 1 << 30;
+  if (p.parts > 0) {
+    float total = 0.0f, longest = 0.0f;
+    for (int b0 = 0; b0 < a.batch; b0 += 64) {
+      int tiles, units;
+      count(b0 + lane, tiles, units);
+      total += (float)tiles * units, longest = fmaxf(longest, units);
+    }
+    total = wave_sum(total), longest = wave_max(longest);
+    // (64 blocks of a row tile at most: the joining kernel's lanes)
+    size = (int)fmaxf(ceilf(fmaxf(total / p.parts, longest / 64)), (float)p.least);
+    for (int i = 0; i < 16; i++) {
+      float blocks = 0.0f;
+      for (int b0 = 0; b0 < a.batch; b0 += 64) {
+        int tiles, units;
+        count(b0 + lane, tiles, units);
+        blocks += (float)tiles * ((units + size - 1) / size);
+      }
+      blocks = wave_sum(blocks);
+      if (blocks <= p.parts) break;
+      // (at last a share for each row tile; blocks are enough for those)
+      size = i < 14 ? max(size + 1, (int)ceilf(size * (blocks / p.parts))) : (int)longest + 1;
+    }
+    size = __builtin_amdgcn_readfirstlane(size);
+  }
+  Share share{0, 0, 0, 0, 0, 0};
+  int before = 0;
+  for (int b0 = 0; b0 < a.batch && share.n == 0; b0 += 64) {
+    int tiles, units;
+    count(b0 + lane, tiles, units);
+    const int each = (int)(((int64_t)units + size - 1) / size), own = tiles * each;
+    int to = own;
+#pragma unroll
+    for (int step = 1; step < 64; step *= 2) {
+      const int up = __shfl_up(to, step, 64);
+      if (lane >= step) to += up;
+    }
+    if (const uint64_t at = __ballot(index >= before + to - own && index < before + to); at != 0) {
+      const int src = __builtin_ctzll(at);
+      share.b = b0 + src, share.n = __builtin_amdgcn_readlane(each, src);
+      share.from = before + __builtin_amdgcn_readlane(to, src) - __builtin_amdgcn_readlane(own, src);
+      const int local = index - share.from, tile = local / share.n;
+      share.tile = __builtin_amdgcn_readlane(tiles, src) - 1 - tile;
+      const int part = local - tile * share.n;
+      share.first = share.n == 1 ? 0 : part * size << p.unit;
+      share.end = share.n == 1 ? 1 << 30 : share.first + (size << p.unit);
+    }
+    before += __builtin_amdgcn_readlane(to, 63);
+  }
+  return share;
+}
+
+// What a block knows of its rows.
+struct Seq {
+  int first_token, n, len, rows;  // tokens of the sequence, its length (0 for a bad one), its rows n * group
+  int p0, p1;                     // positions of the block's first and last token
+  bool bad;
+};
+template <int ROWS>
+__device__ __forceinline__ Seq seq_of(const Args &p, const Share &share) {
+  const PagedAttn &a = p.a;
+  const Span span = span_of(uniform_load(a.starts + share.b), uniform_load(a.starts + share.b + 1), a.tokens);
+  const int len = uniform_load(a.lengths + share.b);
+  Seq s;
+  s.bad = len < 0 || len > a.max_rows;
+  s.first_token = span.first, s.n = span.n, s.len = s.bad ? 0 : len, s.rows = span.n * p.group;
+  const int before = s.len - s.n;
+  s.p0 = before + p.token(share.tile * ROWS), s.p1 = s.bad ? -1 : before + p.token(min(s.rows, (share.tile + 1) * ROWS) - 1);
+  return s;
+}
+
+// Rows of a tile that the token at position pos sees, as bits.
+__device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0 : n >= 32 ? ~0u : (1u << n) - 1; }
+__device__ __forceinline__ uint32_t seen_bits(const PagedAttn &a, int pos, int key0) {
+  uint32_t seen = below(pos + 1 - key0);
+  if (a.window > 0) seen &= ~below(pos + 1 - a.window - key0) | below(a.sinks - key0);
+  return seen;
+}
+// Whether the tokens at p0 .. p1 all see the whole tile.
+__device__ __forceinline__ bool all_see(const PagedAttn &a, int p0, int p1, int key0) {
+  return key0 + kTileKeys <= p0 + 1 && (a.window == 0 || key0 > p1 - a.window || key0 + kTileKeys <= a.sinks);
+}
+
+// The pages of a tile's halves.  Rows from `end` on are not looked up: nothing sees them, the other half's page stands in.
+struct Ids {
+  int page[2], at[2];  // at: the half's first row in its page
+  // halves whose page does not exist: no memory is read for them (page 0 stands in)
+  __device__ __forceinline__ int missing(const PagedAttn &a) const {
+    return ((uint32_t)page[0] >= (uint32_t)a.pages.n ? 1 : 0) | ((uint32_t)page[1] >= (uint32_t)a.pages.n ? 2 : 0);
+  }
+};
+__device__ __forceinline__ Ids ids_of(const Args &p, const int32_t *table, int key0, int end) {
+  Ids ids;
+#pragma unroll
+  for (int h = 0; h < 2; h++) {
+    const int key = h == 1 && key0 + 16 >= end ? key0 : key0 + 16 * h, page = page_of(key, p.page_mul);
+    ids.page[h] = uniform_load(table + page);
+    ids.at[h] = key - page * p.a.pages.size;
+  }
+  return ids;
+}
+__device__ __forceinline__ void bases_of(const Args &p, const Ids &ids, const char *pages, int64_t page_step, int64_t row_step,
+                                         const char *(&base)[2]) {
+#pragma unroll
+  for (int h = 0; h < 2; h++) {
+    const int page = (uint32_t)ids.page[h] < (uint32_t)p.a.pages.n ? ids.page[h] : 0;
+    base[h] = pages + page * page_step + ids.at[h] * row_step;
+  }
+}
+
+// A wave's keys and values of one tile: key rows 16 h + c, in runs of 8 elements 32 j + 8 g, and value rows 16 h + 4 g + r,
+// elements D / 16 c ...
+template <int D, class T>
+struct PageRegs {
+  static constexpr int kK = 8 * T::kBytes / 4, kV = D / 16 * T::kBytes / 4;  // dwords of a run
+  uint32_t k[2][D / 32][kK];
+  uint32_t v[8][kV];
+  uint32_t k_at, v_at[4];
+  __device__ __forceinline__ void place(const Pages &g, int c, int q) {
+    k_at = c * (uint32_t)g.k_r + 8 * q * T::kBytes;
+#pragma unroll
+    for (int r = 0; r < 4; r++) v_at[r] = (4 * q + r) * (uint32_t)g.v_r + D / 16 * c * T::kBytes;
+  }
+  __device__ __forceinline__ void load_k(const Args &p, const Ids &ids, int hk) {
+    const char *base[2];
+    bases_of(p, ids, p.a.pages.k + hk * p.a.pages.k_h, p.a.pages.k_p, p.a.pages.k_r, base);
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      asm volatile("" : "+v"(k_at));  // (kept as 32 bits)
+#pragma unroll
+      for (int j = 0; j < D / 32; j++) load_dwords<kK>(base[h] + 32 * j * T::kBytes + k_at, k[h][j]);
+    }
+  }
+  __device__ __forceinline__ void load_v(const Args &p, const Ids &ids, int hk) {
+    const char *base[2];
+    bases_of(p, ids, p.a.pages.v + hk * p.a.pages.v_h, p.a.pages.v_p, p.a.pages.v_r, base);
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      asm volatile("" : "+v"(v_at[i & 3]));
+      load_dwords<kV>(base[i >> 2] + v_at[i & 3], v[i]);
+    }
+  }
+};
+
+// The same of 4 bits: of each key row 16 h + c codes 64 G + 16 g .. + 15, of each value row 16 h + 4 g + r codes 64 G + 4 c .. + 3
+// (two bytes a register: joined where they are loaded, they would be waited for there), and the pairs of rows 16 h + 4 g + r
+// of both.
+template <int D>
+struct PageRegs<D, I4> {
+  static constexpr int G = D / 64;
+  uint32_t k[2][G][2], v[8][G];
+  uint32_t kp[8][G], vp[8][G];
+  uint32_t k_at, v_at[4], kp_at[4], vp_at[4];
+  __device__ __forceinline__ void place(const Pages &g, int c, int q) {
+    k_at = c * (uint32_t)g.k_r + 8 * q;
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+      v_at[r] = (4 * q + r) * (uint32_t)g.v_r + 2 * c;
+      kp_at[r] = (4 * q + r) * (uint32_t)g.kp_r, vp_at[r] = (4 * q + r) * (uint32_t)g.vp_r;
+    }
+  }
+  static __device__ __forceinline__ void load_pairs(const char *at, uint32_t (&o)[G]) {
+    if constexpr (G == 1) o[0] = *reinterpret_cast<const uint32_t *>(at);
+    else load_dwords<2>(at, o);
+  }
+  __device__ __forceinline__ void load_k(const Args &p, const Ids &ids, int hk) {
+    const char *base[2], *pairs[2];
+    bases_of(p, ids, p.a.pages.k + hk * p.a.pages.k_h, p.a.pages.k_p, p.a.pages.k_r, base);
+    bases_of(p, ids, p.a.pages.kp + hk * p.a.pages.kp_h, p.a.pages.kp_p, p.a.pages.kp_r, pairs);
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      asm volatile("" : "+v"(k_at));
+#pragma unroll
+      for (int i = 0; i < G; i++) load_dwords<2>(base[h] + 32 * i + k_at, k[h][i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      asm volatile("" : "+v"(kp_at[i & 3]));
+      load_pairs(pairs[i >> 2] + kp_at[i & 3], kp[i]);
+    }
+  }
+  __device__ __forceinline__ void load_v(const Args &p, const Ids &ids, int hk) {
+    const char *base[2], *pairs[2];
+    bases_of(p, ids, p.a.pages.v + hk * p.a.pages.v_h, p.a.pages.v_p, p.a.pages.v_r, base);
+    bases_of(p, ids, p.a.pages.vp + hk * p.a.pages.vp_h, p.a.pages.vp_p, p.a.pages.vp_r, pairs);
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      asm volatile("" : "+v"(v_at[i & 3]));
+#pragma unroll
+      for (int j = 0; j < G; j++) v[i][j] = *reinterpret_cast<const uint16_t *>(base[i >> 2] + 32 * j + v_at[i & 3]);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      asm volatile("" : "+v"(vp_at[i & 3]));
+      load_pairs(pairs[i >> 2] + vp_at[i & 3], vp[i]);
+    }
+  }
+};
+
+// Of a dword with four codes in each half, codes d as bf16 pairs 1 + code / 16: one shift and one mask, the bits above are
+// the exponent of 1.  Sums of such products minus the sum of the other operand are 1/16 of those of the codes.
+template <int d>
+__device__ __forceinline__ uint32_t code_pair(uint32_t w) {
+  if constexpr (d == 0) w <<= 3;
+  else w >>= 4 * d - 3;
+  return (w & 0x00780078u) | 0x3f803f80u;
+}
+__device__ __forceinline__ void code_pairs(uint32_t w, uint32_t (&o)[4]) {
+  o[0] = code_pair<0>(w), o[1] = code_pair<1>(w), o[2] = code_pair<2>(w), o[3] = code_pair<3>(w);
+}
+__device__ __forceinline__ float low_half(uint32_t w) { return (float)__builtin_bit_cast(f16x2v, w)[0]; }
+__device__ __forceinline__ float high_half(uint32_t w) { return (float)__builtin_bit_cast(f16x2v, w)[1]; }
+
+// Rows (attn_tiles.h) over 4 bits.  With key t's codes c, scale s and base b in each group of 64 elements,
+//   q . k_t = sum_groups s sum_e q_e c_e + b sum_e q_e,
+// so the products run on codes, exact in 16 bits, and the pairs come in by two multiply-adds a score and group.  In the second
+// product the scale goes with the probability, and sum_t p_t b_t is one number a row and group.  Everything in bf16, whose
+// range holds a probability times any scale.
+template <int D, class TQ, int RT>
+struct Rows4 {
+  static constexpr int G = D / 64, NQ = TQ::kBytes == 4 ? 3 : std::is_same_v<TQ, Bf16> ? 1 : 2, NP = kProbPlanes<TQ>;
+  static constexpr float kLag = 5.0f;
+  uint32_t q[NQ][RT][G][2][4];  // elements 64 G + 16 g + 8 j + (i, i + 4)
+  float qs[RT][G];              // sums of a group's elements
+  float scale;
+  floatx4 o[RT][D / 16];        // element 64 G + 4 (4 g + r) + d in register r of 4 G + d: sums with 1 + code / 16
+  float ob[RT][G];              // sums of p (base - 16 scale), over this lane's keys
+  float m[RT], l[RT];
+
+  // at[t]: the first element of tile t's row c
+  __device__ __forceinline__ void load(const char *const (&at)[RT], float score_scale, int g) {
+    const float by = score_scale * kLog2e;
+    // (fp32 queries carry the scale, rounded once as their caller's own product would; 16-bit ones stay exact)
+    const float in = NQ == 3 ? by : 1.0f;
+    scale = NQ == 3 ? 16.0f : 16.0f * by;
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+#pragma unroll
+      for (int i = 0; i < G; i++) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          uint32_t raw[2 * TQ::kBytes];
+          load_dwords<2 * TQ::kBytes>(at[t] + (64 * i + 16 * g + 8 * j) * TQ::kBytes, raw);
+          float x[8];
+#pragma unroll
+          for (int e = 0; e < 8; e++) {
+            if constexpr (TQ::kBytes == 4) x[e] = __uint_as_float(raw[e]) * in;
+            else if constexpr (std::is_same_v<TQ, Bf16>) x[e] = __uint_as_float(e % 2 ? raw[e / 2] & 0xffff0000u : raw[e / 2] << 16);
+            else x[e] = e % 2 ? high_half(raw[e / 2]) : low_half(raw[e / 2]);
+            sum += x[e];
+          }
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            float a = x[e], b = x[e + 4];
+#pragma unroll
+            for (int k = 0; k < NQ; k++) {
+              q[k][t][i][j][e] = cut_pair(a, b);
+              a -= cut_bits(a), b -= cut_bits(b);
+            }
+          }
+        }
+        qs[t][i] = col_sum(sum);
+        ob[t][i] = 0.0f;
+      }
+      m[t] = -INFINITY, l[t] = 0.0f;
+#pragma unroll
+      for (int d = 0; d < D / 16; d++) o[t][d] = floatx4{};
+    }
+  }
+
+  __device__ __forceinline__ void scores(floatx4 (&s)[2][RT], const PageRegs<D, I4> &x) const {
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      floatx4 acc[G][RT];
+#pragma unroll
+      for (int i = 0; i < G; i++) {
+#pragma unroll
+        for (int t = 0; t < RT; t++) acc[i][t] = floatx4{-qs[t][i], -qs[t][i], -qs[t][i], -qs[t][i]};
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          uint32_t codes[4];
+          code_pairs(x.k[h][i][j], codes);
+#pragma unroll
+          for (int k = NQ - 1; k >= 0; k--)
+#pragma unroll
+            for (int t = 0; t < RT; t++) acc[i][t] = mfma16<Bf16>(codes, q[k][t][i][j], acc[i][t]);
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < RT; t++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          float v = 0.0f;
+#pragma unroll
+          for (int i = 0; i < G; i++) {
+            const uint32_t pair = x.kp[4 * h + r][i];
+            v = __builtin_fmaf(high_half(pair), qs[t][i] * 0.0625f, v);
+            v = __builtin_fmaf(low_half(pair), acc[i][t][r], v);
+          }
+          s[h][t][r] = v;
+        }
+    }
+  }
+  // Running maxima; at an edge keys that are not seen count as -inf, those of a missing page as NaN.
+  __device__ __forceinline__ void limit(floatx4 (&s)[2][RT], bool edge, const uint32_t (&seen)[RT]) {
+    float top[RT];
+    bool grows = false;
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        s[i >> 2][t][i & 3] *= scale;
+        if (edge) s[i >> 2][t][i & 3] = seen[t] & 1u << (16 * (i >> 2) + (i & 3)) ? s[i >> 2][t][i & 3] : -INFINITY;
+      }
+      top[t] = s[0][t][0];
+#pragma unroll
+      for (int i = 1; i < 8; i++) top[t] = fmaxf(top[t], s[i >> 2][t][i & 3]);
+      grows = grows || top[t] > m[t] + kLag;
+    }
+    if (__ballot(grows)) {
+#pragma unroll
+      for (int t = 0; t < RT; t++) {
+        const float mn = fmaxf(m[t], col_max(top[t]));
+        const float f = __builtin_amdgcn_exp2f(m[t] - (mn == -INFINITY ? 0.0f : mn));
+        m[t] = mn;
+        l[t] *= f;
+#pragma unroll
+        for (int i = 0; i < G; i++) ob[t][i] *= f;
+#pragma unroll
+        for (int d = 0; d < D / 16; d++) o[t][d] *= f;
+      }
+    }
+  }
+  __device__ __forceinline__ void weigh(floatx4 (&s)[2][RT]) {
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+      const float ms = m[t] == -INFINITY ? 0.0f : m[t];
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const float p = __builtin_amdgcn_exp2f(s[i >> 2][t][i & 3] - ms);
+        s[i >> 2][t][i & 3] = p;
+        l[t] += p;
+      }
+    }
+  }
+  __device__ __forceinline__ void add(const floatx4 (&s)[2][RT], bool edge, const uint32_t (&seen)[RT], const PageRegs<D, I4> &x) {
+#pragma unroll
+    for (int i = 0; i < G; i++) {
+      uint32_t planes[RT][NP][4];
+#pragma unroll
+      for (int n = 0; n < 4; n++) {
+        const float s0 = low_half(x.vp[2 * n][i]), s1 = low_half(x.vp[2 * n + 1][i]);
+        const float b0 = __builtin_fmaf(s0, -16.0f, high_half(x.vp[2 * n][i])), b1 = __builtin_fmaf(s1, -16.0f, high_half(x.vp[2 * n + 1][i]));
+#pragma unroll
+        for (int t = 0; t < RT; t++) {
+          const float p0 = s[n >> 1][t][2 * (n & 1)], p1 = s[n >> 1][t][2 * (n & 1) + 1];
+          float a0 = p0 * s0, a1 = p1 * s1, c0 = p0 * b0, c1 = p1 * b1;
+          if (edge) {  // (0 times what a row that is not seen may hold: NaN)
+            const uint32_t at = seen[t] >> (16 * (n >> 1) + 2 * (n & 1));
+            a0 = at & 1 ? a0 : 0.0f, c0 = at & 1 ? c0 : 0.0f, a1 = at & 2 ? a1 : 0.0f, c1 = at & 2 ? c1 : 0.0f;
+          }
+          ob[t][i] += c0 + c1;
+          uint32_t w[NP];
+          cut_pos<Bf16, NP>(a0, a1, w);
+#pragma unroll
+          for (int k = 0; k < NP; k++) planes[t][k][n] = w[k];
+        }
+      }
+      uint32_t codes[4][4];  // [element][pair of keys]
+#pragma unroll
+      for (int n = 0; n < 4; n++) {
+        uint32_t w[4];
+        code_pairs(x.v[2 * n][i] | x.v[2 * n + 1][i] << 16, w);
+#pragma unroll
+        for (int d = 0; d < 4; d++) codes[d][n] = w[d];
+      }
+#pragma unroll
+      for (int t = 0; t < RT; t++)
+#pragma unroll
+        for (int k = NP - 1; k >= 0; k--)
+#pragma unroll
+          for (int d = 0; d < 4; d++) o[t][4 * i + d] = mfma16<Bf16>(codes[d], planes[t][k], o[t][4 * i + d]);
+    }
+  }
+};
+
+// Element of a row's run of four d .. d + 3 that register r of a lane group g holds.
+template <int D, class TKV>
+__device__ __forceinline__ int run_at(int g, int r, int d) {
+  return std::is_same_v<TKV, I4> ? 16 * d + 4 * (4 * g + r) : D / 16 * (4 * g + r) + d;
+}
+
+// Tokens in front of the first sequence (x) and from y on belong to none: their rows are zeros, which all blocks write.
+__device__ __forceinline__ int2 rest_of(const PagedAttn &a) {
+  const int front = min(max(uniform_load(a.starts), 0), a.tokens);
+  return make_int2(front, min(max(uniform_load(a.starts + a.batch), front), a.tokens));
+}
+template <int D, class TQ>
+__device__ __forceinline__ void clear_rest(const PagedAttn &a, int2 rest) {
+  const int64_t n = (int64_t)(rest.x + a.tokens - rest.y) * a.H * (D / 4);
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
+    const int d = (int)(i % (D / 4)) * 4, head = (int)(i / (D / 4) % a.H), k = (int)(i / (D / 4) / a.H);
+    const int token = k < rest.x ? k : rest.y + k - rest.x;
+    store4<TQ>(static_cast<char *>(a.out) + (token * a.o_t + head * a.o_h + d) * TQ::kBytes, 0.0f, 0.0f, 0.0f, 0.0f);
+  }
+}
+
+// Four elements d .. of row `row` of the block's row tile, to the output or the shares' results.  What the joining kernel
+// cannot tell by itself goes with the statistics: a row that sees nothing has maximum +inf and sum 0, one of a bad sequence
+// sum NaN.
+template <int D, class TQ, int ROWS>
+__device__ __forceinline__ void put4(const Args &p, const Share &share, const Seq &seq, int index, int hk, int row, int d, float *y,
+                                     float top, float sum, bool any, bool keys) {
+  const PagedAttn &a = p.a;
+  if (share.n == 1) {
+    const float inv = 1.0f / sum;
+#pragma unroll
+    for (int e = 0; e < 4; e++) y[e] = seq.bad ? NAN : any ? y[e] * inv : 0.0f;
+    const int r = share.tile * ROWS + row, i = p.token(r), head = hk * p.group + r - i * p.group;
+    store4<TQ>(static_cast<char *>(a.out) + ((seq.first_token + i) * a.o_t + head * a.o_h + d) * TQ::kBytes, y[0], y[1], y[2], y[3]);
+  } else {
+    const size_t at = ((size_t)hk * p.parts + index) * ROWS + row;
+    if (keys) *reinterpret_cast<float4 *>(a.part + at * D + d) = make_float4(y[0], y[1], y[2], y[3]);
+    if (d == 0) p.ml[at] = seq.bad ? make_float2(0.0f, NAN) : any ? make_float2(top, sum) : make_float2(INFINITY, 0.0f);
+  }
+}
+
+// y[0 .. 4) += the values in tiles that not all rows see which are no finite numbers, of the keys that this row sees.
+template <int D, class T>
+__device__ inline void odd_values(float *y, const Args &p, const Seq &seq, const Tiles &tiles, int first, int end, const int32_t *table,
+                                  int hk, int pos, int d) {
+  const PagedAttn &a = p.a;
+#pragma unroll 1
+  for (int u = first; u < end; u++) {
+    const int key0 = tiles.key(u);
+    if (all_see(a, seq.p0, seq.p1, key0)) continue;
+    const Ids ids = ids_of(p, table, key0, seq.p1 + 1);
+    const int missing = ids.missing(a);
+    const char *base[2];
+    bases_of(p, ids, a.pages.v + hk * a.pages.v_h, a.pages.v_p, a.pages.v_r, base);
+    const uint32_t seen = seen_bits(a, pos, key0);
+#pragma unroll 1
+    for (int i = 0; i < kTileKeys; i++) {
+      if (!(seen >> i & 1) || (missing >> (i >> 4) & 1)) continue;
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const float v = load1<T>(base[i >> 4] + (i & 15) * a.pages.v_r + (d + e) * T::kBytes);
+        if (!(fabsf(v) < INFINITY)) y[e] += v;
+      }
+    }
+  }
+}
+
+// Few query rows: 4 waves over tiles of keys of their own, straight from memory into registers, one tile ahead; joined at
+// the end.
+template <int D, class TQ, class TKV, int RT>
+__global__ __launch_bounds__(256, (D == 128 && std::is_same_v<TKV, F32> ? 1 : 2)) void paged_attn_kernel(Args p) {
+  constexpr int WK = 4, kRows = 16 * RT;
+  constexpr bool kCodes = std::is_same_v<TKV, I4>;
+  __shared__ float so[WK][kRows][D + 4];
+  __shared__ float sm[WK][kRows], sl[WK][kRows];
+  __shared__ int sodd[WK];
+  const PagedAttn &a = p.a;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
+  const int hk = blockIdx.x % a.pages.Hk, index = blockIdx.x / a.pages.Hk;
+  const int2 rest = rest_of(a);
+  const Share share = share_of<kRows>(p, index);
+  if (share.n == 0) return clear_rest<D, TQ>(a, rest);
+  if (p.parts > 0 && index == share.from && hk == 0 && threadIdx.x == 0) p.dealt[share.b] = make_int2(share.from, share.n);
+  const Seq seq = seq_of<kRows>(p, share);
+  const Tiles tiles(a, seq.p0, seq.p1);
+  const int first = min(share.first, tiles.n), end = min(share.end, tiles.n);
+  const int32_t *table = a.table + share.b * a.tab_b;
+
+  const char *at[RT];
+  int pos[RT];
+#pragma unroll
+  for (int t = 0; t < RT; t++) {
+    const int r = min(share.tile * kRows + 16 * t + c, seq.rows - 1), i = p.token(r), head = hk * p.group + r - i * p.group;
+    pos[t] = seq.len - seq.n + i;
+    at[t] = static_cast<const char *>(a.q) + ((seq.first_token + i) * a.q_t + head * a.q_h + (kCodes ? 0 : 8 * g)) * TQ::kBytes;
+  }
+  typename std::conditional<kCodes, Rows4<D, TQ, RT>, Rows<D, TQ, typename std::conditional<kCodes, Bf16, TKV>::type, RT, false>>::type rows;
+  PageRegs<D, TKV> x;
+  x.place(a.pages, c, g);
+  uint32_t odd = 0;  // a value that is no finite number was taken out
+  int u = first + wave;
+  Ids ids, next;
+  if (u < end) {
+    ids = ids_of(p, table, tiles.key(u), seq.p1 + 1);
+    next = ids_of(p, table, tiles.key(min(u + WK, end - 1)), seq.p1 + 1);
+    x.load_k(p, ids, hk);
+    x.load_v(p, ids, hk);
+  }
+  if constexpr (kCodes) rows.load(at, a.scale, g);
+  else rows.load(at, a.scale);
+
+  for (; u < end; u += WK) {
+    const int key0 = tiles.key(u), missing = ids.missing(a);
+    floatx4 s[2][RT] = {};
+    if constexpr (kCodes) {
+      rows.scores(s, x);
+    } else {
+#pragma unroll
+      for (int j = 0; j < D / 32; j++) rows.scores(s, j, x.k[0][j], x.k[1][j]);
+    }
+    // the wave's next tile (past the last one: that one again)
+    ids = next;
+    x.load_k(p, ids, hk);
+    next = ids_of(p, table, tiles.key(min(u + 2 * WK, end - 1)), seq.p1 + 1);
+    const bool edge = !all_see(a, seq.p0, seq.p1, key0) || missing != 0;
+    uint32_t seen[RT] = {};
+    if (edge) {
+#pragma unroll
+      for (int t = 0; t < RT; t++) seen[t] = seen_bits(a, pos[t], key0) >> (4 * g);
+      if (missing) {  // scores of rows that are seen but not there
+#pragma unroll
+        for (int t = 0; t < RT; t++)
+#pragma unroll
+          for (int i = 0; i < 8; i++)
+            if (missing >> (i >> 2) & 1) s[i >> 2][t][i & 3] = NAN;
+      }
+    }
+    rows.limit(s, edge, seen);
+    rows.weigh(s);
+    if constexpr (kCodes) {
+      rows.add(s, edge, seen, x);
+    } else {
+      if (edge) odd |= take_odd<TKV>(x.v, key0, 0, seq.p1 + 1, g);
+      if constexpr (TKV::kBytes == 4) {
+        rows.add_wide(s, x.v);
+      } else {
+        typename decltype(rows)::Probs probs;
+        rows.pack(s, edge, seen, probs);
+        rows.add_rows(probs, x.v);
+      }
+    }
+    x.load_v(p, ids, hk);
+  }
+
+  // The waves joined.
+  if (const bool any = __ballot(odd != 0) != 0; lane == 0) sodd[wave] = any;
+#pragma unroll
+  for (int t = 0; t < RT; t++) {
+    const float l = col_sum(rows.l[t]);
+    if (g == 0) sm[wave][16 * t + c] = rows.m[t], sl[wave][16 * t + c] = l;
+    float by = 1.0f, plus[D / 64] = {};
+    if constexpr (kCodes) {
+      by = 16.0f;
+#pragma unroll
+      for (int i = 0; i < D / 64; i++) plus[i] = col_sum(rows.ob[t][i]);
+    }
+#pragma unroll
+    for (int r = 0; r < 4; r++)
+#pragma unroll
+      for (int d = 0; d < D / 16; d += 4) {
+        float y[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) y[e] = kCodes ? __builtin_fmaf(rows.o[t][d + e][r], by, plus[d / 4 % (D / 64)]) : rows.o[t][d + e][r];
+        *reinterpret_cast<float4 *>(&so[wave][16 * t + c][run_at<D, TKV>(g, r, d)]) = make_float4(y[0], y[1], y[2], y[3]);
+      }
+  }
+  __syncthreads();
+  int odd_any = 0;
+#pragma unroll
+  for (int w = 0; w < WK; w++) odd_any |= sodd[w];
+  for (int i = threadIdx.x; i < kRows * (D / 4); i += 64 * WK) {
+    const int rr = i / (D / 4), d = i % (D / 4) * 4, r = share.tile * kRows + rr;
+    if (r >= seq.rows) continue;
+    const int own = seq.len - seq.n + p.token(r);
+    float top = -INFINITY, sum = 0.0f, y[4] = {};
+#pragma unroll
+    for (int w = 0; w < WK; w++) top = fmaxf(top, sm[w][rr]);
+    const float ms = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+    for (int w = 0; w < WK; w++) {
+      const float f = __builtin_amdgcn_exp2f(sm[w][rr] - ms);
+      const float4 v = *reinterpret_cast<const float4 *>(&so[w][rr][d]);
+      sum += f * sl[w][rr];
+      y[0] += f * v.x, y[1] += f * v.y, y[2] += f * v.z, y[3] += f * v.w;
+    }
+    if constexpr (!kCodes)
+      if (odd_any) odd_values<D, TKV>(y, p, seq, tiles, first, end, table, hk, own, d);
+    put4<D, TQ, kRows>(p, share, seq, index, hk, rr, d, y, top, sum, own >= 0, first < end);
+  }
+  clear_rest<D, TQ>(a, rest);
+}
+
+// Joins the shares' results of a row: a wave a row, D / 4 lanes with four elements each for every fourth (D 128: second)
+// share, added in their order there and then over the lane groups.
+template <int D, class TQ, int ROWS>
+__global__ __launch_bounds__(256) void paged_join_kernel(Args p) {
+  constexpr int kLanes = D / 4, kGroups = 64 / kLanes;
+  const PagedAttn &a = p.a;
+  const int lane = threadIdx.x & 63, d = lane % kLanes * 4, s0 = lane / kLanes;
+  const int item = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
+  if (item >= a.tokens * a.H) return;
+  const int token = item / a.H, head = item - token * a.H, hk = head / p.group;
+  const int b = sequence_of(a.starts, a.batch, token);
+  if (b < 0) return;
+  const Span span = span_of(uniform_load(a.starts + b), uniform_load(a.starts + b + 1), a.tokens);
+  if (token < span.first || token >= span.first + span.n) return;
+  const int2 dealt = p.dealt[b];
+  const int S = dealt.y;
+  if (S == 1) return;  // (that block has written the row)
+  const int r = (token - span.first) * p.group + head - hk * p.group, tile = r / ROWS, tiles = (span.n * p.group + ROWS - 1) / ROWS;
+  const int index = dealt.x + (tiles - 1 - tile) * S;
+  const size_t at = ((size_t)hk * p.parts + index) * ROWS + (r - tile * ROWS);
+  const float *part = a.part + at * D + d;
+  const float2 own = p.ml[at + (size_t)min(lane, S - 1) * ROWS];  // (at most 64 blocks)
+  float4 o = *reinterpret_cast<const float4 *>(part + (size_t)min(s0, S - 1) * ROWS * D);  // (before what weighs it is there)
+  const float top = wave_max(own.x), ms = top == -INFINITY ? 0.0f : top;
+  const bool none = __ballot(own.x == INFINITY && own.y == 0.0f) != 0;
+  const float f_own = __builtin_amdgcn_exp2f(own.x - ms);
+  // (a weight that is positive, if not as a float: times an infinity it is that)
+  auto weighed = [](float f, float y) { return fabsf(y) < INFINITY ? f * y : y; };
+  float sum = 0.0f, x[4] = {};
+  for (int s1 = 0; s1 < S; s1 += kGroups) {
+    const int s = min(s1 + s0, S - 1);
+    const float4 next = *reinterpret_cast<const float4 *>(part + (size_t)min(s + kGroups, S - 1) * ROWS * D);
+    const float m = __shfl(own.x, s, 64), l = __shfl(own.y, s, 64), f = __shfl(f_own, s, 64);
+    const bool in = s1 + s0 < S && !(m == -INFINITY && l == 0.0f);  // without keys nothing was stored
+    const bool num = in && l == l;  // (else the sum is NaN, and nothing may have been stored)
+    sum += in ? f * l : 0.0f;
+    x[0] += num ? weighed(f, o.x) : 0.0f, x[1] += num ? weighed(f, o.y) : 0.0f;
+    x[2] += num ? weighed(f, o.z) : 0.0f, x[3] += num ? weighed(f, o.w) : 0.0f;
+    o = next;
+  }
+#pragma unroll
+  for (int step = kLanes; step < 64; step *= 2) {
+    sum += __shfl_xor(sum, step, 64);
+#pragma unroll
+    for (int e = 0; e < 4; e++) x[e] += __shfl_xor(x[e], step, 64);
+  }
+  if (s0 > 0) return;
+  const float inv = 1.0f / sum;
+#pragma unroll
+  for (int e = 0; e < 4; e++) x[e] = none ? 0.0f : x[e] * inv;
+  store4<TQ>(static_cast<char *>(a.out) + (token * a.o_t + head * a.o_h + d) * TQ::kBytes, x[0], x[1], x[2], x[3]);
+}
+
+struct Plan {
+  int blocks, parts, RT, unit, least;
+};
+Plan make_plan(const PagedAttn &a, int n_cu) {
+  Plan p;
+  const int group = a.H / a.pages.Hk, rows = 16;
+  p.RT = 1, p.unit = 2, p.least = 2;
+  const int64_t most = std::min<int64_t>((int64_t)a.tokens * group / rows + std::min(a.batch, a.tokens), (int64_t)a.tokens * ((group + rows - 1) / rows));
+  p.parts = 0, p.blocks = (int)most;
+  const int at_once = n_cu * 2 / a.pages.Hk;
+  if (most < at_once && a.max_rows > 512) p.parts = p.blocks = std::max(at_once, (int)most);
+  return p;
+}
+
+size_t part_rows(const PagedAttn &a, const Plan &p) { return (size_t)a.pages.Hk * p.parts * 16 * p.RT; }
+Args make_args(const PagedAttn &a, const Plan &p) {
+  const int group = a.H / a.pages.Hk;
+  float *ml = a.part + part_rows(a, p) * a.pages.D;
+  return Args{a, p.blocks, p.parts, group, (uint32_t)(((1ull << 32) + group - 1) / group), page_mul(a.pages.size), p.unit, p.least,
+              reinterpret_cast<float2 *>(ml), reinterpret_cast<int2 *>(ml + 2 * part_rows(a, p))};
+}
+template <int D, class TQ, class TKV, int RT>
+hipError_t launch_rt(const PagedAttn &a, const Plan &p, hipStream_t s) {
+  const Args args = make_args(a, p);
+  hipLaunchKernelGGL((paged_attn_kernel<D, TQ, TKV, RT>), dim3((unsigned)((int64_t)p.blocks * a.pages.Hk)), dim3(256), 0, s, args);
+  if (hipError_t e = hipGetLastError(); e != hipSuccess || p.parts == 0) return e;
+  hipLaunchKernelGGL((paged_join_kernel<D, TQ, 16 * RT>), dim3((unsigned)(((int64_t)a.tokens * a.H + 3) / 4)), dim3(256), 0, s, args);
+  return hipGetLastError();
+}
+template <class TQ, class TKV>
+hipError_t launch(const PagedAttn &a, const Plan &p, hipStream_t s) {
+  return a.pages.D == 64 ? launch_rt<64, TQ, TKV, 1>(a, p, s) : launch_rt<128, TQ, TKV, 1>(a, p, s);
+}
+
+}  // namespace
+
+size_t paged_attn_ws(const PagedAttn &a, int n_cu) {
+  const Plan p = make_plan(a, n_cu);
+  return p.parts == 0 ? 0 : part_rows(a, p) * (a.pages.D + 2) + 2 * (size_t)a.batch;
+}
+
+hipError_t paged_attn(const PagedAttn &a, int n_cu, hipStream_t s) {
+  if (a.batch <= 0 || a.tokens <= 0) return hipSuccess;
+  const Plan p = make_plan(a, n_cu);
+  if (p.parts > 0 && !a.part) return hipErrorInvalidValue;
+  const int kv = a.pages.type;
+  if (a.type == kOpF32) {
+    if (kv == kOpF32) return launch<F32, F32>(a, p, s);
+    if (kv == kOpBf16) return launch<F32, Bf16>(a, p, s);
+    if (kv == kOpI4) return launch<F32, I4>(a, p, s);
+  } else if (a.type == kOpBf16) {
+    if (kv == kOpBf16) return launch<Bf16, Bf16>(a, p, s);
+    if (kv == kOpI4) return launch<Bf16, I4>(a, p, s);
+  } else if (a.type == kOpF16) {
+    if (kv == kOpF16) return launch<F16, F16>(a, p, s);
+    if (kv == kOpI4) return launch<F16, I4>(a, p, s);
+  }
+  return hipErrorInvalidValue;
+}
+
+}  // namespace itts

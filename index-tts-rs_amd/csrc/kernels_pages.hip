@@ -1,0 +1,293 @@
+// Rows of keys and values into pages and out of them.
+//
+// Append.  Token i of sequence b has row r = lengths[b] + i.  With (a, b) a pair of its key's (or query's) elements and t the
+// pair's angle at the row's position,
+//   (a, b) -> (a cos t - b sin t, b cos t + a sin t),
+// the cosines and sines from a table.  A cache of 4 bits takes every 64 elements x as
+//   base = min x, scale = (max x - min x) / 15 (to fp32 and to fp16), code = rint((x - base) / scale) in 0 .. 15 (scale 0: 0),
+// the quantiser of the decoder's weights.  Rotation and quantiser work in 64 bits, which run at the rate of 32 here and hide
+// behind memory: codes are those of the definition, also where a value lies next to the border of two.
+#include <algorithm>
+#include <type_traits>
+
+#include "attn_tiles.h"
+#include "pages.h"
+
+namespace itts {
+namespace {
+
+struct I4 {};
+
+// Eight elements of 16 bits or 32 at p.
+template <class T>
+__device__ __forceinline__ void load8(const char *p, float (&x)[8]) {
+  uint32_t w[2 * T::kBytes];
+  load_dwords<2 * T::kBytes>(p, w);
+#pragma unroll
+  for (int e = 0; e < 8; e++) {
+    if constexpr (T::kBytes == 4) x[e] = __uint_as_float(w[e]);
+    else if constexpr (std::is_same_v<T, Bf16>) x[e] = __uint_as_float(e % 2 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+    else x[e] = half_bits_to_float(e % 2 ? w[e / 2] >> 16 : w[e / 2] & 0xffffu);
+  }
+}
+template <class T, class X>
+__device__ __forceinline__ void store8(char *p, const X (&x)[8]) {
+  store4<T>(p, (float)x[0], (float)x[1], (float)x[2], (float)x[3]);
+  store4<T>(p + 4 * T::kBytes, (float)x[4], (float)x[5], (float)x[6], (float)x[7]);
+}
+
+// A row's lanes (D / 16 of them, 16 elements each in two runs of 8 with numbers run[0], run[1]) to codes and pairs.
+template <int D>
+__device__ __forceinline__ void store_codes(char *codes, char *pairs, const int (&run)[2], int j, const double (&x)[2][8]) {
+  constexpr int kLanes = D / 16, kGroups = D / 64;
+  double lo[kGroups], hi[kGroups];
+#pragma unroll
+  for (int G = 0; G < kGroups; G++) {
+    lo[G] = INFINITY, hi[G] = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        if (run[i] >> 3 != G) continue;
+        lo[G] = fmin(lo[G], x[i][e]);
+        // (a value that is no number makes the range infinite)
+        hi[G] = fabs(x[i][e]) < INFINITY ? fmax(hi[G], x[i][e]) : INFINITY;
+      }
+#pragma unroll
+    for (int step = 1; step < kLanes; step *= 2) {
+      lo[G] = fmin(lo[G], __shfl_xor(lo[G], step, 64));
+      hi[G] = fmax(hi[G], __shfl_xor(hi[G], step, 64));
+    }
+  }
+  double scale[kGroups], base[kGroups];
+#pragma unroll
+  for (int G = 0; G < kGroups; G++) {
+    // (to 32 bits and from there to 16, as the definition has it: left alone, the compiler makes one rounding of the two)
+    float s32 = (float)((hi[G] - lo[G]) / 15.0), b32 = (float)lo[G];
+    asm volatile("" : "+v"(s32), "+v"(b32));
+    const _Float16 s = (_Float16)s32, b = (_Float16)b32;
+    const bool ok = fabsf((float)s) < INFINITY && fabsf((float)b) < INFINITY;
+    scale[G] = ok ? (double)(float)s : 0.0, base[G] = ok ? (double)(float)b : 0.0;
+    const uint32_t pair = (uint32_t)__builtin_bit_cast(uint16_t, s) | (uint32_t)__builtin_bit_cast(uint16_t, b) << 16;
+    if (j == 0) *reinterpret_cast<uint32_t *>(pairs + 4 * G) = ok ? pair : 0x7e007e00u;
+  }
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    const double s = kGroups == 1 || run[i] >> 3 == 0 ? scale[0] : scale[kGroups - 1];
+    const double b = kGroups == 1 || run[i] >> 3 == 0 ? base[0] : base[kGroups - 1];
+    uint32_t w = 0;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      const double c = s == 0.0 ? 0.0 : fmin(fmax(__builtin_rint((x[i][e] - b) / s), 0.0), 15.0);
+      w |= (uint32_t)c << (4 * e);
+    }
+    *reinterpret_cast<uint32_t *>(codes + 4 * run[i]) = w;
+  }
+}
+
+// A wave takes 64 pieces of one token: D / 16 lanes a row, query heads first, then those of keys and values.  A lane's 16
+// elements are two runs of 8 that rotate with each other (halves of the rotated part, or neighbours in pairs).  The last
+// waves take a sequence each, for its new length.
+template <int D, class TX, class TKV>
+__global__ __launch_bounds__(256) void append_kernel(PagedAppend a, int pieces, uint64_t mul) {
+  constexpr int kLanes = D / 16;
+  const int lane = threadIdx.x & 63;
+  int64_t job = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
+  const int64_t jobs = (int64_t)a.tokens * pieces;
+  const int max_rows = (int)min((int64_t)a.n_table * a.pages.size, (int64_t)kPagesMaxRows);
+  if (job >= jobs) {
+    const int b = (int)(job - jobs);
+    if (b >= a.batch) return;
+    const int start = a.starts[b], end = a.starts[b + 1], len = a.lengths[b], n = end - start;
+    bool ok = start >= 0 && end >= start && end <= a.tokens && len >= 0 && len <= max_rows - n;
+    if (ok && n > 0) {
+      const int last = page_of(len + n - 1, mul);
+      for (int p = page_of(len, mul) + lane; p <= last; p += 64) ok = ok && (uint32_t)a.table[b * a.tab_b + p] < (uint32_t)a.pages.n;
+    }
+    const bool all = __ballot(!ok) == 0;
+    if (lane == 0) a.new_lengths[b] = all ? len + n : -1;
+    return;
+  }
+  const int token = __builtin_amdgcn_readfirstlane((int)(job / pieces)), item = (int)(job - (int64_t)token * pieces) * 64 + lane;
+  const int head = item / kLanes, j = item % kLanes, Hk = a.pages.Hk;
+  const bool is_q = head < a.H, is_k = !is_q && head < a.H + Hk, is_v = !is_q && !is_k && head < a.H + 2 * Hk;
+  const int own = is_q ? head : is_k ? head - a.H : head - a.H - Hk;
+
+  // its runs, on their way before anything is known of its sequence
+  const int turned = a.rot >> 4;  // lanes of a row that rotate
+  int run[2];
+  if (a.interleaved) run[0] = 2 * j, run[1] = 2 * j + 1;
+  else if (j < turned) run[0] = j, run[1] = j + turned;
+  else run[0] = 2 * j, run[1] = 2 * j + 1;
+  float raw[2][8] = {};
+  if (is_q || is_k || is_v) {
+    const char *from = is_q ? static_cast<const char *>(a.q) + (token * a.q_t + own * a.q_h) * TX::kBytes
+                     : is_k ? static_cast<const char *>(a.k) + (token * a.k_t + own * a.k_h) * TX::kBytes
+                            : static_cast<const char *>(a.v) + (token * a.v_t + own * a.v_h) * TX::kBytes;
+#pragma unroll
+    for (int i = 0; i < 2; i++) load8<TX>(from + 8 * run[i] * TX::kBytes, raw[i]);
+  }
+
+  const int b = sequence_of(a.starts, a.batch, token);
+  int row = -1, page = -1, pos = -1;  // row: -2 for a token of a sequence that is refused
+  if (b >= 0) {
+    const int start = uniform_load(a.starts + b), end = uniform_load(a.starts + b + 1), len = uniform_load(a.lengths + b);
+    const Span span = span_of(start, end, a.tokens);
+    if (token >= span.first && token < span.first + span.n) {
+      row = len >= 0 && len <= max_rows - span.n ? len + token - span.first : -2;
+      if (row >= 0) {
+        page = uniform_load(a.table + b * a.tab_b + page_of(row, mul));
+        pos = a.positions ? uniform_load(a.positions + token) : row;
+      }
+    }
+  }
+  const bool place = row >= 0 && (uint32_t)page < (uint32_t)a.pages.n, known = (uint32_t)pos < (uint32_t)a.n_positions;
+  double x[2][8];
+#pragma unroll
+  for (int i = 0; i < 2; i++)
+#pragma unroll
+    for (int e = 0; e < 8; e++) x[i][e] = raw[i][e];
+  if (a.rotation && !is_v) {
+    const float *table = a.rotation + (int64_t)(known ? pos : 0) * a.rot_r;
+    if (!known) {
+#pragma unroll
+      for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[i][e] = NAN;
+    } else if (!a.interleaved) {
+      if (j < turned) {
+        float c[8], s[8];
+        load8<F32>(reinterpret_cast<const char *>(table + 8 * j), c);
+        load8<F32>(reinterpret_cast<const char *>(table + a.rot / 2 + 8 * j), s);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const double u = x[0][e], w = x[1][e];
+          x[0][e] = u * c[e] - w * s[e], x[1][e] = w * c[e] + u * s[e];
+        }
+      }
+    } else if (j < turned) {
+      float c[8], s[8];
+      load8<F32>(reinterpret_cast<const char *>(table + 8 * j), c);
+      load8<F32>(reinterpret_cast<const char *>(table + a.rot / 2 + 8 * j), s);
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const double u = x[e / 4][2 * (e % 4)], w = x[e / 4][2 * (e % 4) + 1];
+        x[e / 4][2 * (e % 4)] = u * c[e] - w * s[e], x[e / 4][2 * (e % 4) + 1] = w * c[e] + u * s[e];
+      }
+    }
+  }
+  if (is_q) {
+    char *to = static_cast<char *>(a.q_out) + (token * a.o_t + own * a.o_h) * TX::kBytes;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      if (row < 0) {  // no sequence's token, or one of a refused sequence
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[i][e] = row == -1 ? 0.0 : NAN;
+      }
+      store8<TX>(to + 8 * run[i] * TX::kBytes, x[i]);
+    }
+  } else if ((is_k || is_v) && place) {
+    const int64_t at = row - page_of(row, mul) * a.pages.size;
+    char *to = is_k ? a.pages.k + page * a.pages.k_p + own * a.pages.k_h + at * a.pages.k_r
+                    : a.pages.v + page * a.pages.v_p + own * a.pages.v_h + at * a.pages.v_r;
+    if constexpr (std::is_same_v<TKV, I4>) {
+      char *pairs = is_k ? a.pages.kp + page * a.pages.kp_p + own * a.pages.kp_h + at * a.pages.kp_r
+                         : a.pages.vp + page * a.pages.vp_p + own * a.pages.vp_h + at * a.pages.vp_r;
+      store_codes<D>(to, pairs, run, j, x);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; i++) store8<TKV>(to + 8 * run[i] * TKV::kBytes, x[i]);
+    }
+  }
+}
+
+// A thread per eight elements of an output row; blocks of a sequence, key head and cache.
+template <int D, class TKV, class TO>
+__global__ __launch_bounds__(256) void gather_kernel(PagedGather a, uint64_t mul) {
+  const int b = blockIdx.y, is_v = blockIdx.z & 1, head = blockIdx.z >> 1;
+  const int i = blockIdx.x * 256 + threadIdx.x, row = i / (D / 8), run = i % (D / 8);
+  if (row >= a.rows) return;
+  const int len = uniform_load(a.lengths + b);
+  const bool bad = len < 0 || len > (int)min((int64_t)a.n_table * a.pages.size, (int64_t)kPagesMaxRows);
+  float x[8] = {};
+  if (!bad && row < len) {
+    const int p = page_of(row, mul), page = a.table[b * a.tab_b + p];
+    const int64_t at = row - p * a.pages.size;
+    if ((uint32_t)page < (uint32_t)a.pages.n) {
+      const char *from = is_v ? a.pages.v + page * a.pages.v_p + head * a.pages.v_h + at * a.pages.v_r
+                              : a.pages.k + page * a.pages.k_p + head * a.pages.k_h + at * a.pages.k_r;
+      if constexpr (std::is_same_v<TKV, I4>) {
+        const char *pairs = is_v ? a.pages.vp + page * a.pages.vp_p + head * a.pages.vp_h + at * a.pages.vp_r
+                                 : a.pages.kp + page * a.pages.kp_p + head * a.pages.kp_h + at * a.pages.kp_r;
+        const uint32_t w = *reinterpret_cast<const uint32_t *>(from + 4 * run);
+        const uint32_t pair = *reinterpret_cast<const uint32_t *>(pairs + 4 * (run >> 3));
+        const float s = half_bits_to_float(pair & 0xffffu), base = half_bits_to_float(pair >> 16);
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = __builtin_fmaf((float)(w >> (4 * e) & 15u), s, base);
+      } else {
+        load8<TKV>(from + 8 * run * TKV::kBytes, x);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; e++) x[e] = NAN;
+    }
+  } else if (bad) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) x[e] = NAN;
+  }
+  const int64_t to = is_v ? b * a.v_b + head * a.v_h + row * a.v_r : b * a.k_b + head * a.k_h + row * a.k_r;
+  store8<TO>(static_cast<char *>(is_v ? a.v : a.k) + (to + 8 * run) * TO::kBytes, x);
+}
+
+template <int D, class TX, class TKV>
+hipError_t launch_append(const PagedAppend &a, hipStream_t s) {
+  const int pieces = ((a.H + 2 * a.pages.Hk) * (D / 16) + 63) / 64;
+  const int64_t jobs = (int64_t)a.tokens * pieces + a.batch;
+  hipLaunchKernelGGL((append_kernel<D, TX, TKV>), dim3((unsigned)((jobs + 3) / 4)), dim3(256), 0, s, a, pieces, page_mul(a.pages.size));
+  return hipGetLastError();
+}
+template <class TX, class TKV>
+hipError_t launch_append(const PagedAppend &a, hipStream_t s) {
+  return a.pages.D == 64 ? launch_append<64, TX, TKV>(a, s) : launch_append<128, TX, TKV>(a, s);
+}
+template <class TKV, class TO>
+hipError_t launch_gather(const PagedGather &a, hipStream_t s) {
+  const int D = a.pages.D;
+  const dim3 grid((unsigned)(((int64_t)a.rows * (D / 8) + 255) / 256), a.batch, 2 * a.pages.Hk);
+  if (D == 64) hipLaunchKernelGGL((gather_kernel<64, TKV, TO>), grid, dim3(256), 0, s, a, page_mul(a.pages.size));
+  else hipLaunchKernelGGL((gather_kernel<128, TKV, TO>), grid, dim3(256), 0, s, a, page_mul(a.pages.size));
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t paged_append(const PagedAppend &a, hipStream_t s) {
+  if (a.batch <= 0) return hipSuccess;
+  const int kv = a.pages.type;
+  if (a.type == kOpF32) {
+    if (kv == kOpF32) return launch_append<F32, F32>(a, s);
+    if (kv == kOpBf16) return launch_append<F32, Bf16>(a, s);
+    if (kv == kOpI4) return launch_append<F32, I4>(a, s);
+  } else if (a.type == kOpBf16) {
+    if (kv == kOpBf16) return launch_append<Bf16, Bf16>(a, s);
+    if (kv == kOpI4) return launch_append<Bf16, I4>(a, s);
+  } else if (a.type == kOpF16) {
+    if (kv == kOpF16) return launch_append<F16, F16>(a, s);
+    if (kv == kOpI4) return launch_append<F16, I4>(a, s);
+  }
+  return hipErrorInvalidValue;
+}
+
+hipError_t paged_gather(const PagedGather &a, hipStream_t s) {
+  if (a.batch <= 0 || a.rows <= 0) return hipSuccess;
+  const int kv = a.pages.type;
+  if (kv == kOpF32 && a.type == kOpF32) return launch_gather<F32, F32>(a, s);
+  if (kv == kOpBf16 && a.type == kOpBf16) return launch_gather<Bf16, Bf16>(a, s);
+  if (kv == kOpF16 && a.type == kOpF16) return launch_gather<F16, F16>(a, s);
+  if (kv == kOpI4 && a.type == kOpF32) return launch_gather<I4, F32>(a, s);
+  if (kv == kOpI4 && a.type == kOpBf16) return launch_gather<I4, Bf16>(a, s);
+  if (kv == kOpI4 && a.type == kOpF16) return launch_gather<I4, F16>(a, s);
+  return hipErrorInvalidValue;
+}
+
+}  // namespace itts

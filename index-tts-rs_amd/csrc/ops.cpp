@@ -1,4 +1,4 @@
-// The operators on device memory of include/itts_hip.h (decoding with drafted trees): argument
+// The operators on device memory of include/itts_hip.h (drafted trees, paged caches, logits): argument
 // checks and launches.  Nothing here allocates, waits or throws.
 #include <hip/hip_runtime.h>
 
@@ -182,6 +182,133 @@ itts_status scores_args(const itts_token_scores_args *a, TokenScores *o) {
   return ITTS_OK;
 }
 
+constexpr int kMaxTokens = 1 << 20;
+
+// A cache's pages; `writes`: rows are written, so none may share memory with another.
+itts_status pages_args(const itts_pages &g, bool writes, Pages *o) {
+  const int t = g.dtype == ITTS_I4 ? kOpI4 : op_type(g.dtype);
+  if (t < 0) return fail(ITTS_E_VALIDATION, "pages.dtype: must be F32, BF16, F16 or I4");
+  if (g.head_dim != 64 && g.head_dim != 128) return fail(ITTS_E_VALIDATION, "pages.head_dim: must be 64 or 128, got %d", g.head_dim);
+  if (g.n_kv_head < 1 || g.n_kv_head > 1024) return fail(ITTS_E_VALIDATION, "pages.n_kv_head: must be in 1..=1024, got %d", g.n_kv_head);
+  if (g.page_size < 16 || g.page_size > 65536 || g.page_size % 16)
+    return fail(ITTS_E_VALIDATION, "pages.page_size: must be a multiple of 16 in 16..=65536, got %d", g.page_size);
+  if (g.n_pages < 1) return fail(ITTS_E_VALIDATION, "pages.n_pages: must be >= 1, got %d", g.n_pages);
+  if (!g.k || !g.v || (t == kOpI4 && (!g.k_params || !g.v_params))) return fail(ITTS_E_VALIDATION, "pages: k, v or their params: null");
+  const int es = t == kOpI4 ? 1 : op_size(t), row = t == kOpI4 ? g.head_dim / 2 : g.head_dim;
+  const int64_t ks[3] = {g.k_page, g.k_head, g.k_row}, vs[3] = {g.v_page, g.v_head, g.v_row};
+  const int64_t kps[3] = {g.k_params_page, g.k_params_head, g.k_params_row}, vps[3] = {g.v_params_page, g.v_params_head, g.v_params_row};
+  const int ext[3] = {g.n_pages, g.n_kv_head, g.page_size};
+  const int pair_row = 2 * (g.head_dim / 64);  // float16 of a row's pairs
+  for (int i = 0; i < 3; i++) {
+    if (!row_stride(ks[i], ext[i], es) || !aligned16(g.k)) return fail(ITTS_E_VALIDATION, "pages.k: rows must start at multiples of 16 bytes");
+    if (!row_stride(vs[i], ext[i], es) || !aligned16(g.v)) return fail(ITTS_E_VALIDATION, "pages.v: rows must start at multiples of 16 bytes");
+    if (t != kOpI4 || ext[i] <= 1) continue;
+    for (int64_t s : {kps[i], vps[i]})
+      if (s < 0 || s > INT64_MAX / (16ll * ext[i]) || s % pair_row)
+        return fail(ITTS_E_VALIDATION, "pages.k_params, v_params: rows must start at multiples of %d bytes", 2 * pair_row);
+  }
+  if (t == kOpI4 && (reinterpret_cast<uintptr_t>(g.k_params) % (2 * pair_row) || reinterpret_cast<uintptr_t>(g.v_params) % (2 * pair_row)))
+    return fail(ITTS_E_VALIDATION, "pages.k_params, v_params: rows must start at multiples of %d bytes", 2 * pair_row);
+  if (g.k_row * es > kTreeMaxRowBytes || g.v_row * es > kTreeMaxRowBytes ||
+      (t == kOpI4 && (g.k_params_row * 2 > kTreeMaxRowBytes || g.v_params_row * 2 > kTreeMaxRowBytes)))
+    return fail(ITTS_E_VALIDATION, "pages.k_row, v_row: rows must be at most %d bytes apart", kTreeMaxRowBytes);
+  if (writes) {
+    auto meet = [&](const int64_t(&a)[3], const int64_t(&b)[3], const void *x, const void *y, int size, int n) {
+      if (rows_overlap<3>({{{a[0], ext[0]}, {a[1], ext[1]}, {a[2], ext[2]}}}, n) || rows_overlap<3>({{{b[0], ext[0]}, {b[1], ext[1]}, {b[2], ext[2]}}}, n))
+        return true;
+      // Keys and values apart are one more axis where their strides are the same; else each lies outside the other's range, or
+      // they are taken for interleaved.
+      const int64_t apart = std::llabs(reinterpret_cast<intptr_t>(y) - reinterpret_cast<intptr_t>(x)) / size;
+      if (x == y) return true;
+      return a[0] == b[0] && a[1] == b[1] && a[2] == b[2] && apart < INT64_MAX / 16 &&
+             rows_overlap<4>({{{a[0], ext[0]}, {a[1], ext[1]}, {a[2], ext[2]}, {apart, 2}}}, n);
+    };
+    if (meet(ks, vs, g.k, g.v, es, row)) return fail(ITTS_E_VALIDATION, "pages.k, v: rows must not overlap");
+    if (t == kOpI4 && meet(kps, vps, g.k_params, g.v_params, 2, pair_row)) return fail(ITTS_E_VALIDATION, "pages.k_params, v_params: rows must not overlap");
+  }
+  *o = Pages{static_cast<char *>(g.k), static_cast<char *>(g.v), static_cast<char *>(g.k_params), static_cast<char *>(g.v_params),
+             g.n_pages, g.page_size, g.n_kv_head, g.head_dim, t, ks[0] * es, ks[1] * es, ks[2] * es, vs[0] * es, vs[1] * es, vs[2] * es,
+             kps[0] * 2, kps[1] * 2, kps[2] * 2, vps[0] * 2, vps[1] * 2, vps[2] * 2};
+  return ITTS_OK;
+}
+// The type of tensors beside the pages.
+bool goes_with(int type, int pages) { return type >= 0 && (type == pages || pages == kOpI4 || (type == kOpF32 && pages == kOpBf16)); }
+itts_status batch_args(int batch, int tokens, int n_table, int64_t table_batch, bool ragged) {
+  if (batch < 0 || batch > kMaxGridYZ) return fail(ITTS_E_VALIDATION, "batch: must be in 0..=%d, got %d", kMaxGridYZ, batch);
+  if (tokens < 0 || tokens > kMaxTokens) return fail(ITTS_E_VALIDATION, "n_tokens: must be in 0..=2^20, got %d", tokens);
+  if (ragged && batch == 0 && tokens > 0) return fail(ITTS_E_VALIDATION, "batch: %d tokens of no sequence", tokens);
+  if (n_table < 0 || (batch > 1 && (table_batch < 0 || table_batch > INT64_MAX / 16 / batch))) return fail(ITTS_E_VALIDATION, "table: negative size or stride");
+  return ITTS_OK;
+}
+itts_status heads_args(int n_head, int n_kv_head) {
+  if (n_head < 1 || n_head > 1024 || n_head % n_kv_head)
+    return fail(ITTS_E_VALIDATION, "n_head: %d key heads do not divide %d query heads (1..=1024)", n_kv_head, n_head);
+  return ITTS_OK;
+}
+// Rows [tokens][heads] of a tensor.
+bool token_rows(const void *p, int64_t token, int64_t head, int tokens, int heads, int size) {
+  return row_stride(token, tokens, size) && row_stride(head, heads, size) && aligned16(p);
+}
+
+itts_status append_args(const itts_paged_append_args *a, PagedAppend *o) {
+  if (!a) return fail(ITTS_E_VALIDATION, "args: null");
+  Pages g;
+  if (itts_status st = batch_args(a->batch, a->n_tokens, a->n_table, a->table_batch, true)) return st;
+  if (itts_status st = pages_args(a->pages, true, &g)) return st;
+  if (a->n_head != 0)
+    if (itts_status st = heads_args(a->n_head, g.Hk)) return st;
+  const int t = op_type(a->dtype), n = a->n_tokens;
+  if (!goes_with(t, g.type)) return fail(ITTS_E_VALIDATION, "dtype: must be the pages', F32 over BF16, or any over I4");
+  const int es = op_size(t);
+  if (!token_rows(a->k, a->k_token, a->k_head, n, g.Hk, es)) return fail(ITTS_E_VALIDATION, "k: rows must start at multiples of 16 bytes");
+  if (!token_rows(a->v, a->v_token, a->v_head, n, g.Hk, es)) return fail(ITTS_E_VALIDATION, "v: rows must start at multiples of 16 bytes");
+  if (a->n_head > 0) {
+    if (!token_rows(a->q, a->q_token, a->q_head, n, a->n_head, es)) return fail(ITTS_E_VALIDATION, "q: rows must start at multiples of 16 bytes");
+    if (!token_rows(a->q_out, a->q_out_token, a->q_out_head, n, a->n_head, es))
+      return fail(ITTS_E_VALIDATION, "q_out: rows must start at multiples of 16 bytes");
+    if (rows_overlap<2>({{{a->q_out_token, n}, {a->q_out_head, a->n_head}}}, g.D)) return fail(ITTS_E_VALIDATION, "q_out: rows must not overlap");
+    if (a->q == a->q_out && ((n > 1 && a->q_token != a->q_out_token) || (a->n_head > 1 && a->q_head != a->q_out_head)))
+      return fail(ITTS_E_VALIDATION, "q_out: may be q with the same strides alone");
+  }
+  int rot = 0;
+  if (a->rotation) {
+    rot = a->n_rotated;
+    if (rot < 16 || rot > g.D || rot % 16) return fail(ITTS_E_VALIDATION, "n_rotated: must be a multiple of 16 in 16..=%d, got %d", g.D, rot);
+    if (a->n_positions < 0) return fail(ITTS_E_VALIDATION, "n_positions: must be >= 0, got %d", a->n_positions);
+    if (!row_stride(a->rotation_row, a->n_positions, 4) || !aligned16(a->rotation))
+      return fail(ITTS_E_VALIDATION, "rotation: rows must start at multiples of 16 bytes");
+  }
+  *o = PagedAppend{g, a->k, a->v, a->q, a->q_out, a->rotation, a->starts, a->lengths, a->table, a->positions, a->new_lengths, a->batch, n,
+                   a->n_head, a->n_table, rot, a->rotation ? a->n_positions : 0, a->interleaved != 0, t, a->k_token, a->k_head, a->v_token,
+                   a->v_head, a->q_token, a->q_head, a->q_out_token, a->q_out_head, a->rotation_row, a->table_batch};
+  return ITTS_OK;
+}
+
+itts_status paged_args(const itts_paged_attention_args *a, PagedAttn *o) {
+  if (!a) return fail(ITTS_E_VALIDATION, "args: null");
+  Pages g;
+  if (itts_status st = batch_args(a->batch, a->n_tokens, a->n_table, a->table_batch, true)) return st;
+  if (itts_status st = pages_args(a->pages, false, &g)) return st;
+  if (itts_status st = heads_args(a->n_head, g.Hk)) return st;
+  if ((int64_t)a->n_tokens * a->n_head > 1 << 29) return fail(ITTS_E_VALIDATION, "n_tokens: at most 2^29 rows, got %d of %d heads", a->n_tokens, a->n_head);
+  const int t = op_type(a->q_dtype), n = a->n_tokens;
+  if (!goes_with(t, g.type)) return fail(ITTS_E_VALIDATION, "q_dtype: must be the pages', F32 over BF16, or any over I4");
+  const int es = op_size(t);
+  if (!token_rows(a->q, a->q_token, a->q_head, n, a->n_head, es)) return fail(ITTS_E_VALIDATION, "q: rows must start at multiples of 16 bytes");
+  if (!token_rows(a->out, a->out_token, a->out_head, n, a->n_head, es)) return fail(ITTS_E_VALIDATION, "out: rows must start at multiples of 16 bytes");
+  if (rows_overlap<2>({{{a->out_token, n}, {a->out_head, a->n_head}}}, g.D)) return fail(ITTS_E_VALIDATION, "out: rows must not overlap");
+  if (a->max_rows < 0 || a->max_rows > (int64_t)a->n_table * g.size || a->max_rows > kPagesMaxRows)
+    return fail(ITTS_E_VALIDATION, "max_rows: must be in 0..=%d pages of %d rows and at most 2^24, got %d", a->n_table, g.size, a->max_rows);
+  if (a->window < 0 || a->sinks < 0) return fail(ITTS_E_VALIDATION, "window, sinks: must be >= 0, got %d and %d", a->window, a->sinks);
+  if (!(a->scale - a->scale == 0.0f)) return fail(ITTS_E_VALIDATION, "scale: must be finite");
+  // (longer than any sequence is as good as no bound, and leaves room for sums)
+  constexpr int kFar = 2 * kPagesMaxRows;
+  *o = PagedAttn{g, a->q, a->out, a->starts, a->lengths, a->table, a->batch, n, a->n_head, a->n_table, a->max_rows, t,
+                 std::min(a->window, kFar), std::min(a->sinks, kFar), a->scale, a->q_token, a->q_head, a->out_token, a->out_head,
+                 a->table_batch, nullptr};
+  return ITTS_OK;
+}
+
 itts_status check_workspace(const void *ws, uint64_t have, uint64_t need) {
   if (need && (!ws || have < need))
     return fail(ITTS_E_VALIDATION, "workspace: %llu bytes needed, got %llu", (unsigned long long)need,
@@ -301,6 +428,129 @@ itts_status itts_cache_keep(const itts_cache_keep_args *a, void *stream) {
                     a->head_dim / per, a->n_path, ks[0] / per, ks[1] / per, ks[2] / per, ks[3] / per, vs[0] / per, vs[1] / per,
                     vs[2] / per, vs[3] / per, a->path_batch, same ? 1 : 2};
   if (hipError_t e = cache_keep(c, static_cast<hipStream_t>(stream)); e != hipSuccess) return hip_fail(e, "kept rows");
+  return ITTS_OK;
+}
+
+itts_status itts_paged_append(const itts_paged_append_args *args, void *stream) {
+  PagedAppend a;
+  int dev = 0, n_cu = 0;
+  if (itts_status st = append_args(args, &a)) return st;
+  if (a.batch == 0) return ITTS_OK;
+  if (!a.starts || !a.lengths || !a.new_lengths || (a.n_table && !a.table) || (a.tokens && (!a.k || !a.v || (a.H && (!a.q || !a.q_out)))))
+    return fail(ITTS_E_VALIDATION, "k, v, q, q_out, starts, lengths, table, new_lengths: null");
+  if (a.lengths == a.new_lengths) return fail(ITTS_E_VALIDATION, "new_lengths: must not be lengths");
+  if (itts_status st = compute_units(&dev, &n_cu)) return st;
+  const bool any = a.tokens > 0, turn = any && a.H > 0;
+  if (itts_status st = check_device(
+          dev, stream, {{a.pages.k, "pages.k"}, {a.pages.v, "pages.v"}, {a.pages.type == kOpI4 ? a.pages.kp : nullptr, "pages.k_params"},
+                        {a.pages.type == kOpI4 ? a.pages.vp : nullptr, "pages.v_params"}, {any ? a.k : nullptr, "k"}, {any ? a.v : nullptr, "v"},
+                        {turn ? a.q : nullptr, "q"}, {turn ? a.q_out : nullptr, "q_out"}, {a.n_positions ? a.rotation : nullptr, "rotation"},
+                        {a.starts, "starts"}, {a.lengths, "lengths"}, {a.n_table ? a.table : nullptr, "table"},
+                        {any ? a.positions : nullptr, "positions"}, {a.new_lengths, "new_lengths"}}))
+    return st;
+  if (hipError_t e = paged_append(a, static_cast<hipStream_t>(stream)); e != hipSuccess) return hip_fail(e, "paged append");
+  return ITTS_OK;
+}
+
+itts_status itts_paged_attention_workspace(const itts_paged_attention_args *args, uint64_t *bytes) {
+  PagedAttn a;
+  int dev = 0, n_cu = 0;
+  if (itts_status st = paged_args(args, &a)) return st;
+  if (!bytes) return fail(ITTS_E_VALIDATION, "bytes: null");
+  *bytes = 0;
+  if (a.tokens == 0) return ITTS_OK;
+  if (itts_status st = compute_units(&dev, &n_cu)) return st;
+  *bytes = sizeof(float) * paged_attn_ws(a, n_cu);
+  return ITTS_OK;
+}
+
+itts_status itts_paged_attention(const itts_paged_attention_args *args, void *workspace, uint64_t workspace_bytes, void *stream) {
+  PagedAttn a;
+  int dev = 0, n_cu = 0;
+  if (itts_status st = paged_args(args, &a)) return st;
+  if (a.tokens == 0) return ITTS_OK;
+  if (!a.q || !a.out || !a.starts || !a.lengths || (a.n_table && !a.table)) return fail(ITTS_E_VALIDATION, "q, out, starts, lengths, table: null");
+  if (itts_status st = compute_units(&dev, &n_cu)) return st;
+  const uint64_t need = sizeof(float) * paged_attn_ws(a, n_cu);
+  if (itts_status st = check_workspace(workspace, workspace_bytes, need)) return st;
+  if (itts_status st = check_device(
+          dev, stream, {{a.pages.k, "pages.k"}, {a.pages.v, "pages.v"}, {a.pages.type == kOpI4 ? a.pages.kp : nullptr, "pages.k_params"},
+                        {a.pages.type == kOpI4 ? a.pages.vp : nullptr, "pages.v_params"}, {a.q, "q"}, {a.out, "out"}, {a.starts, "starts"},
+                        {a.lengths, "lengths"}, {a.n_table ? a.table : nullptr, "table"}, {need ? workspace : nullptr, "workspace"}}))
+    return st;
+  a.part = static_cast<float *>(workspace);
+  if (hipError_t e = paged_attn(a, n_cu, static_cast<hipStream_t>(stream)); e != hipSuccess) return hip_fail(e, "paged attention");
+  return ITTS_OK;
+}
+
+itts_status itts_paged_gather(const itts_paged_gather_args *a, void *stream) {
+  if (!a) return fail(ITTS_E_VALIDATION, "args: null");
+  Pages g;
+  if (itts_status st = batch_args(a->batch, 0, a->n_table, a->table_batch, false)) return st;
+  if (itts_status st = pages_args(a->pages, false, &g)) return st;
+  if (a->n_rows < 0 || a->n_rows > kPagesMaxRows) return fail(ITTS_E_VALIDATION, "n_rows: must be in 0..=2^24, got %d", a->n_rows);
+  const int t = op_type(a->dtype);
+  if (t < 0 || (t != g.type && g.type != kOpI4)) return fail(ITTS_E_VALIDATION, "dtype: must be the pages', or any over I4");
+  const int es = op_size(t);
+  const int64_t ks[3] = {a->k_batch, a->k_head, a->k_row}, vs[3] = {a->v_batch, a->v_head, a->v_row};
+  const int ext[3] = {a->batch, g.Hk, a->n_rows};
+  for (int i = 0; i < 3; i++) {
+    if (!row_stride(ks[i], ext[i], es) || !aligned16(a->k)) return fail(ITTS_E_VALIDATION, "k: rows must start at multiples of 16 bytes");
+    if (!row_stride(vs[i], ext[i], es) || !aligned16(a->v)) return fail(ITTS_E_VALIDATION, "v: rows must start at multiples of 16 bytes");
+  }
+  if (a->batch == 0 || a->n_rows == 0) return ITTS_OK;
+  if (!a->k || !a->v || !a->lengths || (a->n_table && !a->table)) return fail(ITTS_E_VALIDATION, "k, v, lengths, table: null");
+  if (a->k == a->v || rows_overlap<3>({{{ks[0], ext[0]}, {ks[1], ext[1]}, {ks[2], ext[2]}}}, g.D) ||
+      rows_overlap<3>({{{vs[0], ext[0]}, {vs[1], ext[1]}, {vs[2], ext[2]}}}, g.D))
+    return fail(ITTS_E_VALIDATION, "k, v: rows must not overlap");
+  int dev = 0, n_cu = 0;
+  if (itts_status st = compute_units(&dev, &n_cu)) return st;
+  if (itts_status st = check_device(
+          dev, stream, {{g.k, "pages.k"}, {g.v, "pages.v"}, {g.type == kOpI4 ? g.kp : nullptr, "pages.k_params"},
+                        {g.type == kOpI4 ? g.vp : nullptr, "pages.v_params"}, {a->k, "k"}, {a->v, "v"}, {a->lengths, "lengths"},
+                        {a->n_table ? a->table : nullptr, "table"}}))
+    return st;
+  const PagedGather p{g, a->k, a->v, a->lengths, a->table, a->batch, a->n_rows, a->n_table, t, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
+                      a->table_batch};
+  if (hipError_t e = paged_gather(p, static_cast<hipStream_t>(stream)); e != hipSuccess) return hip_fail(e, "paged gather");
+  return ITTS_OK;
+}
+
+itts_status itts_adjust_logits(const itts_adjust_logits_args *a, void *stream) {
+  if (!a) return fail(ITTS_E_VALIDATION, "args: null");
+  if (a->rows < 0 || a->rows > 1 << 23) return fail(ITTS_E_VALIDATION, "rows: must be in 0..=2^23, got %d", a->rows);
+  if (a->vocab < 1 || a->vocab > 1 << 24) return fail(ITTS_E_VALIDATION, "vocab: must be in 1..=2^24, got %d", a->vocab);
+  if ((int64_t)a->rows * ((a->vocab + 1023) / 1024) > 1 << 30) return fail(ITTS_E_VALIDATION, "rows: too many of %d logits, got %d", a->vocab, a->rows);
+  if (a->n_history < 0 || a->n_history > kAdjustMaxList) return fail(ITTS_E_VALIDATION, "n_history: must be in 0..=%d, got %d", kAdjustMaxList, a->n_history);
+  if (a->n_bias < 0 || a->n_bias > kAdjustMaxList) return fail(ITTS_E_VALIDATION, "n_bias: must be in 0..=%d, got %d", kAdjustMaxList, a->n_bias);
+  const int t = op_type(a->dtype);
+  if (t < 0) return fail(ITTS_E_VALIDATION, "dtype: must be F32, BF16 or F16");
+  if (!a->repetition && !(a->repetition_all > 0.0f && a->repetition_all - a->repetition_all == 0.0f))
+    return fail(ITTS_E_VALIDATION, "repetition: must be above 0 and finite");
+  if ((!a->frequency && !(a->frequency_all - a->frequency_all == 0.0f)) || (!a->presence && !(a->presence_all - a->presence_all == 0.0f)))
+    return fail(ITTS_E_VALIDATION, "frequency, presence: must be finite");
+  if (reinterpret_cast<uintptr_t>(a->logits) % op_size(t) || reinterpret_cast<uintptr_t>(a->out) % op_size(t))
+    return fail(ITTS_E_VALIDATION, "logits, out: misaligned");
+  if (a->rows > 1) {
+    for (int64_t s : {a->logits_row, a->out_row, a->history_row, a->bias_tokens_row, a->bias_row, a->allowed_row})
+      if (s < 0 || s > INT64_MAX / 16 / a->rows) return fail(ITTS_E_VALIDATION, "logits_row, out_row, history_row, bias_row, allowed_row: rows must ascend");
+    if (a->out_row < a->vocab) return fail(ITTS_E_VALIDATION, "out: rows must not overlap");
+    if (a->logits == a->out && a->logits_row != a->out_row) return fail(ITTS_E_VALIDATION, "out: may be logits with the same stride alone");
+  }
+  if (a->rows == 0) return ITTS_OK;
+  if (!a->logits || !a->out || (a->n_history && !a->history) || (a->n_bias && (!a->bias_tokens || !a->bias)))
+    return fail(ITTS_E_VALIDATION, "logits, out, history, bias_tokens, bias: null");
+  int dev = 0, n_cu = 0;
+  if (itts_status st = compute_units(&dev, &n_cu)) return st;
+  if (itts_status st = check_device(
+          dev, stream, {{a->logits, "logits"}, {a->out, "out"}, {a->n_history ? a->history : nullptr, "history"},
+                        {a->n_bias ? a->bias_tokens : nullptr, "bias_tokens"}, {a->n_bias ? a->bias : nullptr, "bias"}, {a->allowed, "allowed"},
+                        {a->repetition, "repetition"}, {a->frequency, "frequency"}, {a->presence, "presence"}}))
+    return st;
+  const AdjustLogits p{a->logits, a->out, a->history, a->bias_tokens, a->bias, a->allowed, a->repetition, a->frequency, a->presence,
+                       a->repetition_all, a->frequency_all, a->presence_all, a->rows, a->vocab, a->n_history, a->n_bias, t, a->logits_row,
+                       a->out_row, a->history_row, a->bias_tokens_row, a->bias_row, a->allowed_row};
+  if (hipError_t e = adjust_logits(p, n_cu, static_cast<hipStream_t>(stream)); e != hipSuccess) return hip_fail(e, "adjusted logits");
   return ITTS_OK;
 }
 

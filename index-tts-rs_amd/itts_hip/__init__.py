@@ -31,7 +31,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("ITTS_HIP_LIB") or os.path.join(os.path.dirname(_HERE), "lib", "libitts_hip.so")
 
 ITTS_OK, ITTS_E_VALIDATION, ITTS_E_WEIGHT, ITTS_E_DEVICE, ITTS_E_CAPACITY, ITTS_E_INTERNAL = range(6)
-ITTS_F16, ITTS_F32, ITTS_BF16 = 1, 2, 3
+ITTS_F16, ITTS_F32, ITTS_BF16, ITTS_I4 = 1, 2, 3, 4
 ITTS_DECODE_AUTO, ITTS_DECODE_MULTI, ITTS_DECODE_PERSISTENT = 0, 1, 2
 
 GPT_MEL_VOCAB = 8194
@@ -136,6 +136,47 @@ class itts_cache_keep_args(C.Structure):
                                           "path_batch")])
 
 
+class itts_pages(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("k", "v", "k_params", "v_params")] +
+                [(n, C.c_int32) for n in ("n_pages", "page_size", "n_kv_head", "head_dim", "dtype")] +
+                [(n, C.c_int64) for n in ("k_page", "k_head", "k_row", "v_page", "v_head", "v_row", "k_params_page",
+                                          "k_params_head", "k_params_row", "v_params_page", "v_params_head",
+                                          "v_params_row")])
+
+
+class itts_paged_append_args(C.Structure):
+    _fields_ = ([("pages", itts_pages)] +
+                [(n, C.c_void_p) for n in ("k", "v", "q", "q_out", "rotation", "starts", "lengths", "table", "positions",
+                                           "new_lengths")] +
+                [(n, C.c_int32) for n in ("batch", "n_tokens", "n_head", "n_table", "n_rotated", "n_positions", "interleaved",
+                                          "dtype")] +
+                [(n, C.c_int64) for n in ("k_token", "k_head", "v_token", "v_head", "q_token", "q_head", "q_out_token",
+                                          "q_out_head", "rotation_row", "table_batch")])
+
+
+class itts_paged_attention_args(C.Structure):
+    _fields_ = ([("pages", itts_pages)] +
+                [(n, C.c_void_p) for n in ("q", "out", "starts", "lengths", "table")] +
+                [(n, C.c_int32) for n in ("batch", "n_tokens", "n_head", "n_table", "max_rows", "window", "sinks",
+                                          "q_dtype")] + [("scale", C.c_float)] +
+                [(n, C.c_int64) for n in ("q_token", "q_head", "out_token", "out_head", "table_batch")])
+
+
+class itts_paged_gather_args(C.Structure):
+    _fields_ = ([("pages", itts_pages)] + [(n, C.c_void_p) for n in ("k", "v", "lengths", "table")] +
+                [(n, C.c_int32) for n in ("batch", "n_rows", "n_table", "dtype")] +
+                [(n, C.c_int64) for n in ("k_batch", "k_head", "k_row", "v_batch", "v_head", "v_row", "table_batch")])
+
+
+class itts_adjust_logits_args(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("logits", "out", "history", "bias_tokens", "bias", "allowed", "repetition",
+                                           "frequency", "presence")] +
+                [(n, C.c_float) for n in ("repetition_all", "frequency_all", "presence_all")] +
+                [(n, C.c_int32) for n in ("rows", "vocab", "n_history", "n_bias", "dtype")] +
+                [(n, C.c_int64) for n in ("logits_row", "out_row", "history_row", "bias_tokens_row", "bias_row",
+                                          "allowed_row")])
+
+
 _SIGS = {
     "itts_kv_last_timing": (C.c_int, [C.c_void_p, C.POINTER(itts_timing)]),
     "itts_version": (C.c_char_p, []),
@@ -212,6 +253,11 @@ _SIGS = {
     "itts_token_scores_workspace": (C.c_int, [C.c_void_p, C.POINTER(C.c_uint64)]),
     "itts_token_scores": (C.c_int, [C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p]),
     "itts_cache_keep": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "itts_paged_append": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "itts_paged_attention_workspace": (C.c_int, [C.c_void_p, C.POINTER(C.c_uint64)]),
+    "itts_paged_attention": (C.c_int, [C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p]),
+    "itts_paged_gather": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "itts_adjust_logits": (C.c_int, [C.c_void_p, C.c_void_p]),
     "itts_cfm_create": (C.c_int, [C.POINTER(itts_cfm_config), C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32,
                                   C.POINTER(C.c_void_p)]),
     "itts_cfm_destroy": (None, [C.c_void_p]),

@@ -26,6 +26,7 @@ pub type itts_dtype = i32;
 pub const ITTS_F16: itts_dtype = 1;
 pub const ITTS_F32: itts_dtype = 2;
 pub const ITTS_BF16: itts_dtype = 3;
+pub const ITTS_I4: itts_dtype = 4;
 
 /// `itts_decode_path`.
 pub type itts_decode_path = i32;
@@ -242,6 +243,145 @@ pub struct itts_cache_keep_args {
     pub path_batch: i64,
 }
 
+/// A paged cache, device memory (strides in elements; of 4 bits in bytes).
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct itts_pages {
+    pub k: *mut c_void,
+    pub v: *mut c_void,
+    pub k_params: *mut c_void,
+    pub v_params: *mut c_void,
+    pub n_pages: i32,
+    pub page_size: i32,
+    pub n_kv_head: i32,
+    pub head_dim: i32,
+    pub dtype: itts_dtype,
+    pub k_page: i64,
+    pub k_head: i64,
+    pub k_row: i64,
+    pub v_page: i64,
+    pub v_head: i64,
+    pub v_row: i64,
+    pub k_params_page: i64,
+    pub k_params_head: i64,
+    pub k_params_row: i64,
+    pub v_params_page: i64,
+    pub v_params_head: i64,
+    pub v_params_row: i64,
+}
+
+/// Appends tokens' keys and values to paged sequences.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct itts_paged_append_args {
+    pub pages: itts_pages,
+    pub k: *const c_void,
+    pub v: *const c_void,
+    pub q: *const c_void,
+    pub q_out: *mut c_void,
+    pub rotation: *const f32,
+    pub starts: *const i32,
+    pub lengths: *const i32,
+    pub table: *const i32,
+    pub positions: *const i32,
+    pub new_lengths: *mut i32,
+    pub batch: i32,
+    pub n_tokens: i32,
+    pub n_head: i32,
+    pub n_table: i32,
+    pub n_rotated: i32,
+    pub n_positions: i32,
+    pub interleaved: i32,
+    pub dtype: itts_dtype,
+    pub k_token: i64,
+    pub k_head: i64,
+    pub v_token: i64,
+    pub v_head: i64,
+    pub q_token: i64,
+    pub q_head: i64,
+    pub q_out_token: i64,
+    pub q_out_head: i64,
+    pub rotation_row: i64,
+    pub table_batch: i64,
+}
+
+/// Attention of tokens over paged sequences.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct itts_paged_attention_args {
+    pub pages: itts_pages,
+    pub q: *const c_void,
+    pub out: *mut c_void,
+    pub starts: *const i32,
+    pub lengths: *const i32,
+    pub table: *const i32,
+    pub batch: i32,
+    pub n_tokens: i32,
+    pub n_head: i32,
+    pub n_table: i32,
+    pub max_rows: i32,
+    pub window: i32,
+    pub sinks: i32,
+    pub q_dtype: itts_dtype,
+    pub scale: f32,
+    pub q_token: i64,
+    pub q_head: i64,
+    pub out_token: i64,
+    pub out_head: i64,
+    pub table_batch: i64,
+}
+
+/// Paged sequences' rows to caches of one piece.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct itts_paged_gather_args {
+    pub pages: itts_pages,
+    pub k: *mut c_void,
+    pub v: *mut c_void,
+    pub lengths: *const i32,
+    pub table: *const i32,
+    pub batch: i32,
+    pub n_rows: i32,
+    pub n_table: i32,
+    pub dtype: itts_dtype,
+    pub k_batch: i64,
+    pub k_head: i64,
+    pub k_row: i64,
+    pub v_batch: i64,
+    pub v_head: i64,
+    pub v_row: i64,
+    pub table_batch: i64,
+}
+
+/// Logits under penalties, biases and a mask.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct itts_adjust_logits_args {
+    pub logits: *const c_void,
+    pub out: *mut c_void,
+    pub history: *const i32,
+    pub bias_tokens: *const i32,
+    pub bias: *const f32,
+    pub allowed: *const u32,
+    pub repetition: *const f32,
+    pub frequency: *const f32,
+    pub presence: *const f32,
+    pub repetition_all: f32,
+    pub frequency_all: f32,
+    pub presence_all: f32,
+    pub rows: i32,
+    pub vocab: i32,
+    pub n_history: i32,
+    pub n_bias: i32,
+    pub dtype: itts_dtype,
+    pub logits_row: i64,
+    pub out_row: i64,
+    pub history_row: i64,
+    pub bias_tokens_row: i64,
+    pub bias_row: i64,
+    pub allowed_row: i64,
+}
+
 #[link(name = "itts_hip")]
 extern "C" {
     pub fn itts_version() -> *const c_char;
@@ -340,6 +480,12 @@ extern "C" {
     pub fn itts_token_scores(args: *const itts_token_scores_args, workspace: *mut c_void, workspace_bytes: u64,
                              stream: *mut c_void) -> itts_status;
     pub fn itts_cache_keep(args: *const itts_cache_keep_args, stream: *mut c_void) -> itts_status;
+    pub fn itts_paged_append(args: *const itts_paged_append_args, stream: *mut c_void) -> itts_status;
+    pub fn itts_paged_attention_workspace(args: *const itts_paged_attention_args, bytes: *mut u64) -> itts_status;
+    pub fn itts_paged_attention(args: *const itts_paged_attention_args, workspace: *mut c_void, workspace_bytes: u64,
+                                stream: *mut c_void) -> itts_status;
+    pub fn itts_paged_gather(args: *const itts_paged_gather_args, stream: *mut c_void) -> itts_status;
+    pub fn itts_adjust_logits(args: *const itts_adjust_logits_args, stream: *mut c_void) -> itts_status;
 
     pub fn itts_cfm_create(cfg: *const itts_cfm_config, names: *const *const c_char, data: *const *const f32,
                            numel: *const i64, n: i32, out: *mut *mut itts_cfm) -> itts_status;
