@@ -99,8 +99,7 @@ __device__ __forceinline__ void cut3(float a, float b, uint32_t (&o)[3]) {
 }
 // The same for probabilities (never negative).  bf16: the last rest is raised by 2^-23 of what it is the rest
 // of in the subtraction itself; the second of two planes is rounded, 2^-16 of the value at most.  fp16: 11 bits a
-// plane, two hold 22, down to its smallest number, 2^-24, which the rest always is at least: the test for
-// 0 took 4% of long caches' time and 12% of many rows', and pack clears masked keys' rests instead.
+// plane, two hold 22, down to its smallest number, 2^-24, which the rest of a positive value always is at least.
 template <class T, int N>
 __device__ __forceinline__ void cut_pos(float a, float b, uint32_t (&o)[N]) {
   constexpr float kUp = 1.0f + 0x1p-23f, kLeast = 0x1.01p-118f;  // (more than the 8 bits of one plane)
@@ -108,7 +107,9 @@ __device__ __forceinline__ void cut_pos(float a, float b, uint32_t (&o)[N]) {
     static_assert(N == 2);
     const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
     o[0] = __builtin_bit_cast(uint32_t, h);
-    o[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(fmaxf(a - (float)h[0], 0x1p-24f), fmaxf(b - (float)h[1], 0x1p-24f)));
+    // (the median: of 0 it is 0)
+    o[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(__builtin_amdgcn_fmed3f(a - (float)h[0], a, 0x1p-24f),
+                                                                   __builtin_amdgcn_fmed3f(b - (float)h[1], b, 0x1p-24f)));
   } else if constexpr (N == 2) {
     o[0] = cut_pair(a, b);
     const f32x2e rest = {__builtin_fmaf(a, kUp, -cut_bits(a)), __builtin_fmaf(b, kUp, -cut_bits(b))};
@@ -263,7 +264,7 @@ struct Rows {
   struct Probs {
     uint32_t p[kWide ? 1 : RT][NP][4];
   };
-  __device__ __forceinline__ void pack(const floatx4 (&s)[2][RT], bool edge, const uint32_t (&seen)[RT], Probs &x) const {
+  __device__ __forceinline__ void pack(const floatx4 (&s)[2][RT], Probs &x) const {
     if constexpr (!kWide) {
 #pragma unroll
       for (int t = 0; t < RT; t++)
@@ -275,15 +276,6 @@ struct Rows {
 #pragma unroll
           for (int k = 0; k < NP; k++) x.p[t][k][i] = w[k];
         }
-      if (std::is_same_v<TKV, F16> && edge) {
-#pragma unroll
-        for (int t = 0; t < RT; t++)
-#pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const uint32_t at = seen[t] >> (16 * (i >> 1) + 2 * (i & 1));
-            x.p[t][1][i] &= (at & 1 ? 0xffffu : 0) | (at & 2 ? 0xffff0000u : 0);
-          }
-      }
     }
   }
 

@@ -34,17 +34,18 @@ struct Args {
   __device__ int token(int row) const { return group == 1 ? row : __umulhi((uint32_t)row, group_mul); }
 };
 
-// The tiles of 32 keys that the tokens at positions p0 .. p1 of a sequence see, counted through: those with rows < S,
+// The tiles of KT keys that the tokens at positions p0 .. p1 of a sequence see, counted through: those with rows < S,
 // then from the window's first one on.
+template <int KT>
 struct Tiles {
   int front, skip, n;
   __device__ __forceinline__ Tiles(const PagedAttn &a, int p0, int p1) {
-    const int from = a.window > 0 ? max(0, p0 - a.window + 1) >> 5 : 0;
-    front = min((a.sinks >> 5) + ((a.sinks & 31) != 0), from);
+    const int from = a.window > 0 ? max(0, p0 - a.window + 1) / KT : 0;
+    front = min(a.sinks / KT + (a.sinks % KT != 0), from);
     skip = from - front;
-    n = p1 < 0 ? 0 : front + (p1 >> 5) + 1 - from;
+    n = p1 < 0 ? 0 : front + p1 / KT + 1 - from;
   }
-  __device__ __forceinline__ int key(int u) const { return (u < front ? u : u + skip) * kTileKeys; }
+  __device__ __forceinline__ int key(int u) const { return (u < front ? u : u + skip) * KT; }
 };
 
 // What block `index` has to do: tiles [first, end) of row tile `tile` of sequence b, whose rows are shared by n blocks (0:
@@ -53,7 +54,7 @@ struct Tiles {
 struct Share {
   int b, tile, n, first, end, from;
 };
-template <int ROWS>
+template <int ROWS, int KT>
 __device__ __forceinline__ Share share_of(const Args &p, int index) {
   const PagedAttn &a = p.a;
   const int lane = threadIdx.x & 63;
@@ -65,8 +66,8 @@ __device__ __forceinline__ Share share_of(const Args &p, int index) {
     const int len = a.lengths[b], rows = span.n * p.group;
     tiles = (rows + ROWS - 1) / ROWS;
     int seen = len < 0 || len > a.max_rows ? 1 : max(len, 1);
-    if (a.window > 0) seen = (int)min((int64_t)seen, (int64_t)a.window + min(a.sinks, a.max_rows) + (ROWS - 1) / p.group + 1 + 2 * kTileKeys);
-    units = tiles == 0 ? 0 : ((seen + kTileKeys - 1) / kTileKeys + (1 << p.unit) - 1) >> p.unit;
+    if (a.window > 0) seen = (int)min((int64_t)seen, (int64_t)a.window + min(a.sinks, a.max_rows) + (ROWS - 1) / p.group + 1 + 2 * KT);
+    units = tiles == 0 ? 0 : ((seen + KT - 1) / KT + (1 << p.unit) - 1) >> p.unit;
   };
   int size = 1 << 30;
   if (p.parts > 0) {
@@ -147,8 +148,9 @@ __device__ __forceinline__ uint32_t seen_bits(const PagedAttn &a, int pos, int k
   return seen;
 }
 // Whether the tokens at p0 .. p1 all see the whole tile.
+template <int KT>
 __device__ __forceinline__ bool all_see(const PagedAttn &a, int p0, int p1, int key0) {
-  return key0 + kTileKeys <= p0 + 1 && (a.window == 0 || key0 > p1 - a.window || key0 + kTileKeys <= a.sinks);
+  return key0 + KT <= p0 + 1 && (a.window == 0 || key0 > p1 - a.window || key0 + KT <= a.sinks);
 }
 
 // The pages of a tile's halves.  Rows from `end` on are not looked up: nothing sees them, the other half's page stands in.
@@ -497,26 +499,29 @@ __device__ __forceinline__ void put4(const Args &p, const Share &share, const Se
 }
 
 // y[0 .. 4) += the values in tiles that not all rows see which are no finite numbers, of the keys that this row sees.
-template <int D, class T>
-__device__ inline void odd_values(float *y, const Args &p, const Seq &seq, const Tiles &tiles, int first, int end, const int32_t *table,
+template <int D, class T, int KT>
+__device__ inline void odd_values(float *y, const Args &p, const Seq &seq, const Tiles<KT> &tiles, int first, int end, const int32_t *table,
                                   int hk, int pos, int d) {
   const PagedAttn &a = p.a;
 #pragma unroll 1
   for (int u = first; u < end; u++) {
-    const int key0 = tiles.key(u);
-    if (all_see(a, seq.p0, seq.p1, key0)) continue;
-    const Ids ids = ids_of(p, table, key0, seq.p1 + 1);
-    const int missing = ids.missing(a);
-    const char *base[2];
-    bases_of(p, ids, a.pages.v + hk * a.pages.v_h, a.pages.v_p, a.pages.v_r, base);
-    const uint32_t seen = seen_bits(a, pos, key0);
+    const int key_u = tiles.key(u);
+    if (all_see<KT>(a, seq.p0, seq.p1, key_u)) continue;
 #pragma unroll 1
-    for (int i = 0; i < kTileKeys; i++) {
-      if (!(seen >> i & 1) || (missing >> (i >> 4) & 1)) continue;
+    for (int key0 = key_u; key0 < min(key_u + KT, seq.p1 + 1); key0 += kTileKeys) {
+      const Ids ids = ids_of(p, table, key0, seq.p1 + 1);
+      const int missing = ids.missing(a);
+      const char *base[2];
+      bases_of(p, ids, a.pages.v + hk * a.pages.v_h, a.pages.v_p, a.pages.v_r, base);
+      const uint32_t seen = seen_bits(a, pos, key0);
+#pragma unroll 1
+      for (int i = 0; i < kTileKeys; i++) {
+        if (!(seen >> i & 1) || (missing >> (i >> 4) & 1)) continue;
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const float v = load1<T>(base[i >> 4] + (i & 15) * a.pages.v_r + (d + e) * T::kBytes);
-        if (!(fabsf(v) < INFINITY)) y[e] += v;
+        for (int e = 0; e < 4; e++) {
+          const float v = load1<T>(base[i >> 4] + (i & 15) * a.pages.v_r + (d + e) * T::kBytes);
+          if (!(fabsf(v) < INFINITY)) y[e] += v;
+        }
       }
     }
   }
@@ -535,11 +540,11 @@ __global__ __launch_bounds__(256, (D == 128 && std::is_same_v<TKV, F32> ? 1 : 2)
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
   const int hk = blockIdx.x % a.pages.Hk, index = blockIdx.x / a.pages.Hk;
   const int2 rest = rest_of(a);
-  const Share share = share_of<kRows>(p, index);
+  const Share share = share_of<kRows, kTileKeys>(p, index);
   if (share.n == 0) return clear_rest<D, TQ>(a, rest);
   if (p.parts > 0 && index == share.from && hk == 0 && threadIdx.x == 0) p.dealt[share.b] = make_int2(share.from, share.n);
   const Seq seq = seq_of<kRows>(p, share);
-  const Tiles tiles(a, seq.p0, seq.p1);
+  const Tiles<kTileKeys> tiles(a, seq.p0, seq.p1);
   const int first = min(share.first, tiles.n), end = min(share.end, tiles.n);
   const int32_t *table = a.table + share.b * a.tab_b;
 
@@ -579,7 +584,7 @@ __global__ __launch_bounds__(256, (D == 128 && std::is_same_v<TKV, F32> ? 1 : 2)
     ids = next;
     x.load_k(p, ids, hk);
     next = ids_of(p, table, tiles.key(min(u + 2 * WK, end - 1)), seq.p1 + 1);
-    const bool edge = !all_see(a, seq.p0, seq.p1, key0) || missing != 0;
+    const bool edge = !all_see<kTileKeys>(a, seq.p0, seq.p1, key0) || missing != 0;
     uint32_t seen[RT] = {};
     if (edge) {
 #pragma unroll
@@ -602,7 +607,7 @@ __global__ __launch_bounds__(256, (D == 128 && std::is_same_v<TKV, F32> ? 1 : 2)
         rows.add_wide(s, x.v);
       } else {
         typename decltype(rows)::Probs probs;
-        rows.pack(s, edge, seen, probs);
+        rows.pack(s, probs);
         rows.add_rows(probs, x.v);
       }
     }
@@ -653,6 +658,301 @@ __global__ __launch_bounds__(256, (D == 128 && std::is_same_v<TKV, F32> ? 1 : 2)
     if constexpr (!kCodes)
       if (odd_any) odd_values<D, TKV>(y, p, seq, tiles, first, end, table, hk, own, d);
     put4<D, TQ, kRows>(p, share, seq, index, hk, rr, d, y, top, sum, own >= 0, first < end);
+  }
+  clear_rest<D, TQ>(a, rest);
+}
+
+// ---- many query rows ----
+constexpr int kLongKeys = 64;  // keys of a tile
+constexpr int kLongRows = 128; // rows of a block: 32 a wave
+
+// A row's 16-byte pieces lie in LDS in the order piece ^ swizzle(row): what a wave reads at a time, one piece of many key rows
+// or a few neighbours of 4 value rows, then falls on different banks.
+template <int D>
+__device__ __forceinline__ int swizzle(int row) {
+  return D == 128 ? (row & 3) << 2 | (row >> 2 & 3) : (row >> 1 & 1) << 2 | (row >> 2 & 3);
+}
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+// 16 bytes a lane from base + offset to LDS at lds + 16 lane, without a register in between.  The compiler does not know of
+// the load: copies_wait() has to come before what it brings is read.
+__device__ __forceinline__ void copy16(const char *base, uint32_t offset, const u32x4 *lds) {
+  const uint32_t m0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void *)lds;
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(m0) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+__device__ __forceinline__ void copies_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+template <class T>
+__device__ __forceinline__ floatx16 mfma32(const uint32_t (&a)[4], const uint32_t (&b)[4], floatx16 c) {
+  const u32x4 x = {a[0], a[1], a[2], a[3]}, y = {b[0], b[1], b[2], b[3]};
+  if constexpr (std::is_same_v<T, Bf16>) return ITTS_MFMABF(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, y), c, 0, 0, 0);
+  else return ITTS_MFMA16(__builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, y), c, 0, 0, 0);
+}
+
+// A pair of 16-bit values times a power of two (what is not 0 stays so).
+template <class T>
+__device__ __forceinline__ uint32_t scale_pair(uint32_t w, float f) {
+  float a, b;
+  if constexpr (std::is_same_v<T, Bf16>) a = __uint_as_float(w << 16), b = __uint_as_float(w & 0xffff0000u);
+  else a = low_half(w), b = high_half(w);
+  constexpr float kLeast = std::is_same_v<T, Bf16> ? 0x1p-126f : 0x1p-24f;
+  const float x = __builtin_copysignf(fmaxf(fabsf(a * f), fminf(fabsf(a), kLeast)), a);
+  const float y = __builtin_copysignf(fmaxf(fabsf(b * f), fminf(fabsf(b), kLeast)), b);
+  if constexpr (std::is_same_v<T, Bf16>) return cut_pair(x, y);
+  else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x, y));
+}
+
+// Many query rows over 16-bit caches: 4 waves with 32 rows each over the same tiles of 64 keys, which come to LDS by direct
+// loads, a tile ahead of their use (keys two: a tile's scores are formed while the exponentials of the one before are).
+// S^T = K Q^T by 32 x 32 products: lane (c, h) holds keys 8 (i / 4) + 4 h + i % 4 of query c in register i, the B operand of
+// O^T = V^T P^T in the order in which the transposing LDS load gives V's rows.
+template <int D, class TQ, class TKV>
+__global__ __launch_bounds__(256, (TQ::kBytes == 4 ? (D == 64 ? 2 : 1) : D == 64 ? 3 : 2)) void paged_rows_kernel(Args p) {
+  constexpr int KT = kLongKeys, kPieces = D * TKV::kBytes / 16, kTile = KT * kPieces, kCopies = kTile / 256;
+  constexpr int NQ = TQ::kBytes == 4 ? 3 : 1, NP = kProbPlanes<TQ>;
+  constexpr float kLag = 5.0f, kUp = std::is_same_v<TKV, F16> ? 10.0f : 0.0f;
+  __shared__ __attribute__((aligned(65536))) u32x4 key_mem[2][kTile];
+  __shared__ __attribute__((aligned(256))) u32x4 value_mem[3][kTile];
+  const PagedAttn &a = p.a;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 31, h = lane >> 5;
+  const int hk = blockIdx.x % a.pages.Hk, index = blockIdx.x / a.pages.Hk;
+  const int2 rest = rest_of(a);
+  const Share share = share_of<kLongRows, KT>(p, index);
+  if (share.n == 0) return clear_rest<D, TQ>(a, rest);
+  if (p.parts > 0 && index == share.from && hk == 0 && threadIdx.x == 0) p.dealt[share.b] = make_int2(share.from, share.n);
+  const Seq seq = seq_of<kLongRows>(p, share);
+  const Tiles<KT> tiles(a, seq.p0, seq.p1);
+  const int first = min(share.first, tiles.n), end = min(share.end, tiles.n);
+  const int32_t *table = a.table + share.b * a.tab_b;
+
+  // This wave's copies: rows 16 wave .. of a tile, in kCopies loads of 64 pieces.
+  const char *kb = a.pages.k + hk * a.pages.k_h, *vb = a.pages.v + hk * a.pages.v_h;
+  uint32_t k_at[kCopies], v_at[kCopies];
+#pragma unroll
+  for (int i = 0; i < kCopies; i++) {
+    const int row = (64 * i + lane) / kPieces, piece = (lane % kPieces) ^ swizzle<D>(row);
+    k_at[i] = row * (uint32_t)a.pages.k_r + 16 * piece, v_at[i] = row * (uint32_t)a.pages.v_r + 16 * piece;
+  }
+  // page of the wave's rows of a tile (rows that nothing sees: the tile's first page), and which of a tile's pages do not exist
+  auto place = [&](int u, int &at) {
+    const int key0 = tiles.key(u), key = key0 + 16 * wave < seq.p1 + 1 ? key0 + 16 * wave : key0, page = page_of(key, p.page_mul);
+    at = key - page * a.pages.size;
+    return uniform_load(table + page);
+  };
+  auto missing_of = [&](int u) {
+    const int key0 = tiles.key(u);
+    int missing = 0;
+#pragma unroll
+    for (int i = 0; i < KT / 16; i++) {
+      const int key = key0 + 16 * i < seq.p1 + 1 ? key0 + 16 * i : key0;
+      missing |= (uint32_t)uniform_load(table + page_of(key, p.page_mul)) < (uint32_t)a.pages.n ? 0 : 1 << i;
+    }
+    return missing;
+  };
+  auto copy = [&](const char *from, int64_t page_step, int64_t row_step, const uint32_t (&offset)[kCopies], int page, int at, u32x4 *to) {
+    const char *base = from + ((uint32_t)page < (uint32_t)a.pages.n ? page : 0) * page_step + at * row_step;
+#pragma unroll
+    for (int i = 0; i < kCopies; i++) copy16(base, offset[i], to + 16 * kPieces * wave + 64 * i);
+  };
+
+  // The wave's query rows: lane (c, h) elements 16 j + 8 h .. of row c.
+  uint32_t q[NQ][D / 16][4];
+  const int r = min(share.tile * kLongRows + 32 * wave + c, seq.rows - 1), token = p.token(r), pos = seq.len - seq.n + token;
+  const float by = a.scale * kLog2e, scale = NQ == 3 ? 1.0f : fmaxf(fabsf(by), 0x1p-120f);
+  {
+    const char *at = static_cast<const char *>(a.q) + ((seq.first_token + token) * a.q_t + (hk * p.group + r - token * p.group) * a.q_h + 8 * h) * TQ::kBytes;
+    const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0;
+#pragma unroll
+    for (int j = 0; j < D / 16; j++) {
+      uint32_t raw[2 * TQ::kBytes];
+      load_dwords<2 * TQ::kBytes>(at + 16 * j * TQ::kBytes, raw);
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        if constexpr (NQ == 3) {
+          uint32_t w[3];
+          cut3(__uint_as_float(raw[2 * e]) * by, __uint_as_float(raw[2 * e + 1]) * by, w);
+#pragma unroll
+          for (int i = 0; i < 3; i++) q[i][j][e] = w[i];
+        } else {
+          q[0][j][e] = raw[e] ^ flip;
+        }
+      }
+    }
+  }
+  floatx16 o[D / 32] = {};
+  float m = -INFINITY, l = 0.0f;
+  uint32_t odd = 0;
+
+  // LDS addresses from a base each, every one an exclusive or away: kept for all reads of a tile they would not fit the registers.
+  // Keys: row c, piece 2 j + h.  Values: rows 8 i + 4 h + (lane / 4) % 4 of 16, the four elements that the transposing load takes.
+  constexpr uint32_t kRowBytes = 16 * kPieces, kTileBytes = KT * kRowBytes;
+  using Lds = __attribute__((address_space(3))) const char;
+  uint32_t key_at, value_at;
+  {
+    const int row = 4 * h + (lane >> 2 & 3), piece = 2 * (lane >> 4 & 1) + (lane >> 1 & 1);
+    key_at = (uint32_t)(uintptr_t)(Lds *)key_mem + c * kRowBytes + 16 * (h ^ swizzle<D>(c));
+    value_at = (uint32_t)(uintptr_t)(Lds *)value_mem + row * kRowBytes + 16 * (piece ^ swizzle<D>(row)) + 8 * (lane & 1);
+  }
+  static_assert(2 * kTileBytes <= 65536 && (2 * kTileBytes & (2 * kTileBytes - 1)) == 0, "a buffer's bit in an address");
+  auto read_keys = [&](u32x4 (&k)[D / 16], int t, uint32_t base) {
+#pragma unroll
+    for (int j = 0; j < D / 16; j++)
+      k[j] = *(__attribute__((address_space(3))) const u32x4 *)(uintptr_t)((base ^ 32 * j) + 32 * t * kRowBytes);
+  };
+  auto scores = [&](floatx16 &s, const u32x4 (&w)[D / 16]) {
+    s = floatx16{};
+#pragma unroll
+    for (int j = 0; j < D / 16; j++) {
+      const uint32_t k[4] = {w[j][0], w[j][1], w[j][2], w[j][3]};
+#pragma unroll
+      for (int i = NQ - 1; i >= 0; i--) s = mfma32<TKV>(k, q[i][j], s);
+    }
+  };
+
+  floatx16 s[2];                      // scores of a tile's halves
+  uint32_t planes[2][2][NP][4] = {};  // their probabilities, of 16 keys each
+  auto weigh = [&](int t, float ms) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][2 * i], scale, -ms));
+      const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][2 * i + 1], scale, -ms));
+      l += p0, l += p1;
+      uint32_t w[NP];
+      cut_pos<TKV, NP>(p0, p1, w);
+#pragma unroll
+      for (int k = 0; k < NP; k++) planes[t][i >> 2][k][i & 3] = w[k];
+    }
+  };
+  auto add = [&](int t, uint32_t base) {
+#pragma unroll
+    for (int g = 0; g < 2; g++)
+#pragma unroll
+      for (int d = 0; d < D / 32; d++) {
+        uint32_t vt[4];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {  // keys 8 i + 4 h .. of the 16
+          typedef short s16x4 __attribute__((ext_vector_type(4)));
+          using Piece = __attribute__((address_space(3))) s16x4;
+          const uint32_t at = (base ^ 64 * d ^ 32 * i) + (32 * t + 16 * g + 8 * i) * kRowBytes;
+          const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Piece *)(uintptr_t)at));
+          vt[2 * i] = w[0], vt[2 * i + 1] = w[1];
+        }
+#pragma unroll
+        for (int k = NP - 1; k >= 0; k--) o[d] = mfma32<TKV>(vt, planes[t][g][k], o[d]);
+      }
+  };
+
+  if (first < end) {
+    int next_page, next_at;  // the page of the tile after the next
+    int page1, at1, at0;     // and of the next one
+    const int page0 = place(first, at0);
+    page1 = place(min(first + 1, end - 1), at1);
+    next_page = place(min(first + 2, end - 1), next_at);
+    copy(kb, a.pages.k_p, a.pages.k_r, k_at, page0, at0, key_mem[0]);
+    copy(kb, a.pages.k_p, a.pages.k_r, k_at, page1, at1, key_mem[1]);
+    copy(vb, a.pages.v_p, a.pages.v_r, v_at, page0, at0, value_mem[0]);
+#pragma unroll
+    for (int i = 0; i < kCopies; i++) value_mem[2][64 * kCopies * wave + 64 * i + lane] = u32x4{};  // (probabilities of 0 times it)
+    copies_wait();
+    __syncthreads();
+    u32x4 k[D / 16];
+    read_keys(k, 0, key_at);
+    scores(s[0], k);
+    read_keys(k, 1, key_at);
+    scores(s[1], k);
+    __syncthreads();
+    // Here: a tile's scores and values (ring), the next one's keys, the probabilities of the second half of the one before and its
+    // values; on their way: what follows.  While the scores of one half become probabilities, the products of what is there run.
+    int ring = 0;
+    for (int u = first; u < end; u++) {
+      const int buf = u - first & 1, ring1 = ring == 2 ? 0 : ring + 1, ring2 = ring == 0 ? 2 : ring - 1;
+      copy(vb, a.pages.v_p, a.pages.v_r, v_at, page1, at1, value_mem[ring1]);
+      copy(kb, a.pages.k_p, a.pages.k_r, k_at, next_page, next_at, key_mem[buf]);
+      page1 = next_page, at1 = next_at;
+      next_page = place(min(u + 3, end - 1), next_at);
+      const int key0 = tiles.key(u), missing = missing_of(u);
+      if (!all_see<KT>(a, seq.p0, seq.p1, key0) || missing != 0) {
+        // values that are no finite numbers leave the tile (odd_values), and whatever lies past the last row; keys that are not
+        // seen count as -inf, those of missing pages as NaN
+#pragma unroll
+        for (int i = 0; i < kCopies; i++) {
+          u32x4 &at = value_mem[ring][64 * kCopies * wave + 64 * i + lane];
+          const bool in = key0 + 16 * wave + (64 * i + lane) / kPieces <= seq.p1;
+          u32x4 w = at;
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            uint32_t keep = (w[e] & TKV::kOddBits) == TKV::kOddBits ? 0xffff0000u : ~0u;
+            keep = (w[e] & TKV::kOddBits << 16) == TKV::kOddBits << 16 ? keep & 0xffffu : keep;
+            odd |= in ? ~keep : 0;
+            w[e] &= in ? keep : 0;
+          }
+          at = w;
+        }
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+          const uint32_t seen = seen_bits(a, pos, key0 + 32 * t) >> (4 * h);
+#pragma unroll
+          for (int i = 0; i < 16; i++) {
+            if (missing >> (2 * t + (i >> 3)) & 1) s[t][i] = NAN;
+            s[t][i] = seen & 1u << (8 * (i >> 2) + (i & 3)) ? s[t][i] : -INFINITY;
+          }
+        }
+        __syncthreads();
+      }
+      float top = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+      for (int i = 1; i < 16; i++) top = fmaxf(fmaxf(s[0][i], s[1][i]), top);
+      top *= scale;
+      if (__ballot(top > m + kLag)) {
+        // (maxima are whole numbers: the probabilities that wait rescale exactly)
+        const float mn = ceilf(fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64))));
+        const float f = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.0f : mn));
+        m = mn;
+        l *= f;
+#pragma unroll
+        for (int d = 0; d < D / 32; d++) o[d] *= f;
+#pragma unroll
+        for (int g = 0; g < 2; g++)
+#pragma unroll
+          for (int k = 0; k < NP; k++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) planes[1][g][k][i] = scale_pair<TKV>(planes[1][g][k][i], f);
+      }
+      const float ms = (m == -INFINITY ? 0.0f : m) - kUp;
+      uint32_t keys = key_at ^ (buf ? 0 : kTileBytes), values = value_at + ring * kTileBytes, waiting = value_at + ring2 * kTileBytes;
+      asm volatile("" : "+v"(keys), "+v"(values), "+v"(waiting));
+      // (the barriers keep what is read ahead where it is)
+      read_keys(k, 0, keys);
+      weigh(0, ms);
+      add(1, waiting);
+      __builtin_amdgcn_sched_barrier(0);
+      scores(s[0], k);
+      read_keys(k, 1, keys);
+      weigh(1, ms);
+      add(0, values);
+      __builtin_amdgcn_sched_barrier(0);
+      scores(s[1], k);
+      ring = ring1;
+      copies_wait();
+      __syncthreads();
+    }
+    add(1, value_at + (ring == 0 ? 2 : ring - 1) * kTileBytes);
+  }
+
+  const bool odd_any = __ballot(odd != 0) != 0;
+  l += __shfl_xor(l, 32, 64);
+  const int row = 32 * wave + c;
+  if (share.tile * kLongRows + row < seq.rows) {
+#pragma unroll
+    for (int d = 0; d < D / 32; d++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        float y[4] = {o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+        const int e = 32 * d + 8 * i + 4 * h;
+        if (odd_any) odd_values<D, TKV>(y, p, seq, tiles, first, end, table, hk, pos, e);
+        put4<D, TQ, kLongRows>(p, share, seq, index, hk, row, e, y, m, l, pos >= 0, first < end);
+      }
   }
   clear_rest<D, TQ>(a, rest);
 }
@@ -710,38 +1010,49 @@ __global__ __launch_bounds__(256) void paged_join_kernel(Args p) {
   store4<TQ>(static_cast<char *>(a.out) + (token * a.o_t + head * a.o_h + d) * TQ::kBytes, x[0], x[1], x[2], x[3]);
 }
 
+// How a launch is laid out: rows of a block, blocks of a key head, or `parts` that share the keys.
 struct Plan {
-  int blocks, parts, RT, unit, least;
+  bool many;  // paged_rows_kernel
+  int rows, blocks, parts, unit, least;
 };
 Plan make_plan(const PagedAttn &a, int n_cu) {
   Plan p;
-  const int group = a.H / a.pages.Hk, rows = 16;
-  p.RT = 1, p.unit = 2, p.least = 2;
-  const int64_t most = std::min<int64_t>((int64_t)a.tokens * group / rows + std::min(a.batch, a.tokens), (int64_t)a.tokens * ((group + rows - 1) / rows));
+  const int group = a.H / a.pages.Hk;
+  p.many = a.pages.type != kOpF32 && a.pages.type != kOpI4 && (int64_t)a.tokens * group >= 64 * (int64_t)a.batch;
+  p.rows = p.many ? kLongRows : 16, p.unit = p.many ? 1 : 2, p.least = 2;
+  // row tiles at most: a sequence's last one may be short
+  const int64_t most = std::min<int64_t>((int64_t)a.tokens * group / p.rows + std::min(a.batch, a.tokens),
+                                         (int64_t)a.tokens * ((group + p.rows - 1) / p.rows));
   p.parts = 0, p.blocks = (int)most;
   const int at_once = n_cu * 2 / a.pages.Hk;
   if (most < at_once && a.max_rows > 512) p.parts = p.blocks = std::max(at_once, (int)most);
   return p;
 }
 
-size_t part_rows(const PagedAttn &a, const Plan &p) { return (size_t)a.pages.Hk * p.parts * 16 * p.RT; }
+size_t part_rows(const PagedAttn &a, const Plan &p) { return (size_t)a.pages.Hk * p.parts * p.rows; }
 Args make_args(const PagedAttn &a, const Plan &p) {
   const int group = a.H / a.pages.Hk;
   float *ml = a.part + part_rows(a, p) * a.pages.D;
   return Args{a, p.blocks, p.parts, group, (uint32_t)(((1ull << 32) + group - 1) / group), page_mul(a.pages.size), p.unit, p.least,
               reinterpret_cast<float2 *>(ml), reinterpret_cast<int2 *>(ml + 2 * part_rows(a, p))};
 }
-template <int D, class TQ, class TKV, int RT>
-hipError_t launch_rt(const PagedAttn &a, const Plan &p, hipStream_t s) {
+template <int D, class TQ, int ROWS, class K>
+hipError_t launch_kernel(K kernel, const PagedAttn &a, const Plan &p, hipStream_t s) {
   const Args args = make_args(a, p);
-  hipLaunchKernelGGL((paged_attn_kernel<D, TQ, TKV, RT>), dim3((unsigned)((int64_t)p.blocks * a.pages.Hk)), dim3(256), 0, s, args);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)((int64_t)p.blocks * a.pages.Hk)), dim3(256), 0, s, args);
   if (hipError_t e = hipGetLastError(); e != hipSuccess || p.parts == 0) return e;
-  hipLaunchKernelGGL((paged_join_kernel<D, TQ, 16 * RT>), dim3((unsigned)(((int64_t)a.tokens * a.H + 3) / 4)), dim3(256), 0, s, args);
+  hipLaunchKernelGGL((paged_join_kernel<D, TQ, ROWS>), dim3((unsigned)(((int64_t)a.tokens * a.H + 3) / 4)), dim3(256), 0, s, args);
   return hipGetLastError();
+}
+template <int D, class TQ, class TKV>
+hipError_t launch_d(const PagedAttn &a, const Plan &p, hipStream_t s) {
+  if constexpr (std::is_same_v<TKV, Bf16> || std::is_same_v<TKV, F16>)
+    if (p.many) return launch_kernel<D, TQ, kLongRows>(paged_rows_kernel<D, TQ, TKV>, a, p, s);
+  return launch_kernel<D, TQ, 16>(paged_attn_kernel<D, TQ, TKV, 1>, a, p, s);
 }
 template <class TQ, class TKV>
 hipError_t launch(const PagedAttn &a, const Plan &p, hipStream_t s) {
-  return a.pages.D == 64 ? launch_rt<64, TQ, TKV, 1>(a, p, s) : launch_rt<128, TQ, TKV, 1>(a, p, s);
+  return a.pages.D == 64 ? launch_d<64, TQ, TKV>(a, p, s) : launch_d<128, TQ, TKV>(a, p, s);
 }
 
 }  // namespace

@@ -377,7 +377,7 @@ __global__ __launch_bounds__(256, 2) void tree_attn_kernel(Args p) {
       rows.add_wide(s, x.v);
     } else {
       typename Wave::Probs probs;
-      rows.pack(s, edge, seen, probs);
+      rows.pack(s, probs);
       rows.add_rows(probs, x.v);
     }
     x.load_v(vb + (uint64_t)(uint32_t)next * v_step);
@@ -542,7 +542,7 @@ __global__ __launch_bounds__(64 * kRowWaves, 2) void tree_attn_rows_kernel(Args 
     scores(s_next, buf ^ 1);
     rows.weigh(s);
     typename Wave::Probs probs;
-    rows.pack(s, kEdge, seen, probs);
+    rows.pack(s, probs);
     rows.add_sums(probs);
 #pragma unroll
     for (int d0 = 0; d0 < D / 16; d0 += 4) {  // (four at a time: fewer registers)
