@@ -364,7 +364,7 @@ struct PagedAppend {
   int batch, tokens, H, n_table, rot, n_positions, interleaved, type;
   int64_t k_t, k_h, v_t, v_h, q_t, q_h, o_t, o_h, rot_r, tab_b;
 };
-hipError_t paged_append(const PagedAppend &a, hipStream_t s);
+hipError_t paged_append(const PagedAppend &a, int n_cu, hipStream_t s);
 // Rows of sequences to k and v [batch][Hk][rows][D] of `type`; zeros behind a sequence's length.
 struct PagedGather {
   Pages pages;

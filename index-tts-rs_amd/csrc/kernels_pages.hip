@@ -40,26 +40,31 @@ __device__ __forceinline__ void store8(char *p, const X (&x)[8]) {
 template <int D>
 __device__ __forceinline__ void store_codes(char *codes, char *pairs, const int (&run)[2], int j, const double (&x)[2][8]) {
   constexpr int kLanes = D / 16, kGroups = D / 64;
+  double least[2], most[2], odd = 0.0;
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    least[i] = most[i] = x[i][0];
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      least[i] = x[i][e] < least[i] ? x[i][e] : least[i], most[i] = x[i][e] > most[i] ? x[i][e] : most[i];
+      odd = __builtin_fma(x[i][e], 0.0, odd);  // NaN for a value that is no finite number
+    }
+    // (which then makes the range infinite)
+    if (odd != 0.0) least[i] = 0.0, most[i] = INFINITY;
+  }
   double lo[kGroups], hi[kGroups];
 #pragma unroll
   for (int G = 0; G < kGroups; G++) {
-    lo[G] = INFINITY, hi[G] = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < 2; i++)
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        if (run[i] >> 3 != G) continue;
-        lo[G] = fmin(lo[G], x[i][e]);
-        // (a value that is no number makes the range infinite)
-        hi[G] = fabs(x[i][e]) < INFINITY ? fmax(hi[G], x[i][e]) : INFINITY;
-      }
+    const bool in0 = kGroups == 1 || run[0] >> 3 == G, in1 = kGroups == 1 || run[1] >> 3 == G;
+    lo[G] = in0 ? least[0] : INFINITY, hi[G] = in0 ? most[0] : -INFINITY;
+    lo[G] = in1 && least[1] < lo[G] ? least[1] : lo[G], hi[G] = in1 && most[1] > hi[G] ? most[1] : hi[G];
 #pragma unroll
     for (int step = 1; step < kLanes; step *= 2) {
-      lo[G] = fmin(lo[G], __shfl_xor(lo[G], step, 64));
-      hi[G] = fmax(hi[G], __shfl_xor(hi[G], step, 64));
+      const double l = __shfl_xor(lo[G], step, 64), h = __shfl_xor(hi[G], step, 64);
+      lo[G] = l < lo[G] ? l : lo[G], hi[G] = h > hi[G] ? h : hi[G];
     }
   }
-  double scale[kGroups], base[kGroups];
+  double scale[kGroups], base[kGroups], inverse[kGroups];
 #pragma unroll
   for (int G = 0; G < kGroups; G++) {
     // (to 32 bits and from there to 16, as the definition has it: left alone, the compiler makes one rounding of the two)
@@ -67,7 +72,8 @@ __device__ __forceinline__ void store_codes(char *codes, char *pairs, const int 
     asm volatile("" : "+v"(s32), "+v"(b32));
     const _Float16 s = (_Float16)s32, b = (_Float16)b32;
     const bool ok = fabsf((float)s) < INFINITY && fabsf((float)b) < INFINITY;
-    scale[G] = ok ? (double)(float)s : 0.0, base[G] = ok ? (double)(float)b : 0.0;
+    scale[G] = ok && s != (_Float16)0 ? (double)(float)s : INFINITY, base[G] = ok ? (double)(float)b : 0.0;
+    inverse[G] = 1.0 / scale[G];  // (0 where there is no scale, or none that holds: codes of 0)
     const uint32_t pair = (uint32_t)__builtin_bit_cast(uint16_t, s) | (uint32_t)__builtin_bit_cast(uint16_t, b) << 16;
     if (j == 0) *reinterpret_cast<uint32_t *>(pairs + 4 * G) = ok ? pair : 0x7e007e00u;
   }
@@ -75,25 +81,29 @@ __device__ __forceinline__ void store_codes(char *codes, char *pairs, const int 
   for (int i = 0; i < 2; i++) {
     const double s = kGroups == 1 || run[i] >> 3 == 0 ? scale[0] : scale[kGroups - 1];
     const double b = kGroups == 1 || run[i] >> 3 == 0 ? base[0] : base[kGroups - 1];
+    const double inv = kGroups == 1 || run[i] >> 3 == 0 ? inverse[0] : inverse[kGroups - 1];
     uint32_t w = 0;
 #pragma unroll
     for (int e = 0; e < 8; e++) {
-      const double c = s == 0.0 ? 0.0 : fmin(fmax(__builtin_rint((x[i][e] - b) / s), 0.0), 15.0);
-      w |= (uint32_t)c << (4 * e);
+      // (x - base) times 1 / scale is off by 2^-51 of at most 16: the quotient itself is needed next to a border alone
+      const double y = (x[i][e] - b) * inv;
+      double c = __builtin_rint(y);
+      if (__builtin_expect(fabs(fabs(y - c) - 0.5) < 1e-12, 0)) c = __builtin_rint((x[i][e] - b) / s);
+      w |= (uint32_t)(int)__builtin_amdgcn_fmed3f((float)c, 0.0f, 15.0f) << (4 * e);
     }
     *reinterpret_cast<uint32_t *>(codes + 4 * run[i]) = w;
   }
 }
 
-// A wave takes 64 pieces of one token: D / 16 lanes a row, query heads first, then those of keys and values.  A lane's 16
-// elements are two runs of 8 that rotate with each other (halves of the rotated part, or neighbours in pairs).  The last
-// waves take a sequence each, for its new length.
+// A wave takes pieces of one token, 64 lanes' at a time: D / 16 lanes a row, query heads first, then those of keys and values.
+// A lane's 16 elements are two runs of 8 that rotate with each other (halves of the rotated part, or neighbours in pairs), the
+// same ones of every row, so that a wave reads the angles once.  The last waves take a sequence each, for its new length.
 template <int D, class TX, class TKV>
-__global__ __launch_bounds__(256) void append_kernel(PagedAppend a, int pieces, uint64_t mul) {
+__global__ __launch_bounds__(256) void append_kernel(PagedAppend a, int pieces, int parts, uint64_t mul) {
   constexpr int kLanes = D / 16;
   const int lane = threadIdx.x & 63;
-  int64_t job = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
-  const int64_t jobs = (int64_t)a.tokens * pieces;
+  const int64_t job = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
+  const int64_t jobs = (int64_t)a.tokens * parts;
   const int max_rows = (int)min((int64_t)a.n_table * a.pages.size, (int64_t)kPagesMaxRows);
   if (job >= jobs) {
     const int b = (int)(job - jobs);
@@ -108,25 +118,32 @@ __global__ __launch_bounds__(256) void append_kernel(PagedAppend a, int pieces, 
     if (lane == 0) a.new_lengths[b] = all ? len + n : -1;
     return;
   }
-  const int token = __builtin_amdgcn_readfirstlane((int)(job / pieces)), item = (int)(job - (int64_t)token * pieces) * 64 + lane;
-  const int head = item / kLanes, j = item % kLanes, Hk = a.pages.Hk;
-  const bool is_q = head < a.H, is_k = !is_q && head < a.H + Hk, is_v = !is_q && !is_k && head < a.H + 2 * Hk;
-  const int own = is_q ? head : is_k ? head - a.H : head - a.H - Hk;
-
-  // its runs, on their way before anything is known of its sequence
+  const int token = (int)(job / parts), part = (int)(job - (int64_t)token * parts), Hk = a.pages.Hk;
   const int turned = a.rot >> 4;  // lanes of a row that rotate
+  const int j = lane % kLanes;
   int run[2];
-  if (a.interleaved) run[0] = 2 * j, run[1] = 2 * j + 1;
-  else if (j < turned) run[0] = j, run[1] = j + turned;
-  else run[0] = 2 * j, run[1] = 2 * j + 1;
-  float raw[2][8] = {};
-  if (is_q || is_k || is_v) {
-    const char *from = is_q ? static_cast<const char *>(a.q) + (token * a.q_t + own * a.q_h) * TX::kBytes
-                     : is_k ? static_cast<const char *>(a.k) + (token * a.k_t + own * a.k_h) * TX::kBytes
-                            : static_cast<const char *>(a.v) + (token * a.v_t + own * a.v_h) * TX::kBytes;
+  if (a.interleaved || j >= turned) run[0] = 2 * j, run[1] = 2 * j + 1;
+  else run[0] = j, run[1] = j + turned;
+
+  // A piece's rows: what they are (0 query, 1 key, 2 value, 3 none) and which head.
+  auto head_of = [&](int piece, int &own) {
+    const int head = (piece * 64 + lane) / kLanes;
+    const int kind = head < a.H ? 0 : head < a.H + Hk ? 1 : head < a.H + 2 * Hk ? 2 : 3;
+    own = kind == 0 ? head : kind == 1 ? head - a.H : head - a.H - Hk;
+    return kind;
+  };
+  auto load = [&](int piece, float (&raw)[2][8]) {
+    int own;
+    const int kind = piece < pieces ? head_of(piece, own) : 3;
+    if (kind == 3) return;
+    const char *from = kind == 0 ? static_cast<const char *>(a.q) + (token * a.q_t + own * a.q_h) * TX::kBytes
+                     : kind == 1 ? static_cast<const char *>(a.k) + (token * a.k_t + own * a.k_h) * TX::kBytes
+                                 : static_cast<const char *>(a.v) + (token * a.v_t + own * a.v_h) * TX::kBytes;
 #pragma unroll
     for (int i = 0; i < 2; i++) load8<TX>(from + 8 * run[i] * TX::kBytes, raw[i]);
-  }
+  };
+  float raw[2][8] = {};
+  load(part, raw);  // (on its way before anything is known of the sequence)
 
   const int b = sequence_of(a.starts, a.batch, token);
   int row = -1, page = -1, pos = -1;  // row: -2 for a token of a sequence that is refused
@@ -142,61 +159,67 @@ __global__ __launch_bounds__(256) void append_kernel(PagedAppend a, int pieces, 
     }
   }
   const bool place = row >= 0 && (uint32_t)page < (uint32_t)a.pages.n, known = (uint32_t)pos < (uint32_t)a.n_positions;
-  double x[2][8];
-#pragma unroll
-  for (int i = 0; i < 2; i++)
-#pragma unroll
-    for (int e = 0; e < 8; e++) x[i][e] = raw[i][e];
-  if (a.rotation && !is_v) {
+  const int64_t at = place ? row - page_of(row, mul) * a.pages.size : 0;
+  float c[8], s[8];
+  const bool turns = a.rotation && j < turned;
+  if (turns) {
     const float *table = a.rotation + (int64_t)(known ? pos : 0) * a.rot_r;
-    if (!known) {
+    load8<F32>(reinterpret_cast<const char *>(table + 8 * j), c);
+    load8<F32>(reinterpret_cast<const char *>(table + a.rot / 2 + 8 * j), s);
+  }
+  for (int piece = part; piece < pieces; piece += parts) {
+    int own;
+    const int kind = head_of(piece, own);
+    double x[2][8];
 #pragma unroll
-      for (int i = 0; i < 2; i++)
+    for (int i = 0; i < 2; i++)
 #pragma unroll
-        for (int e = 0; e < 8; e++) x[i][e] = NAN;
-    } else if (!a.interleaved) {
-      if (j < turned) {
-        float c[8], s[8];
-        load8<F32>(reinterpret_cast<const char *>(table + 8 * j), c);
-        load8<F32>(reinterpret_cast<const char *>(table + a.rot / 2 + 8 * j), s);
+      for (int e = 0; e < 8; e++) x[i][e] = raw[i][e];
+    load(piece + parts, raw);
+    if (kind == 3 || (kind != 0 && !place)) continue;
+    if (a.rotation && kind != 2) {
+      if (!known) {
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-          const double u = x[0][e], w = x[1][e];
-          x[0][e] = u * c[e] - w * s[e], x[1][e] = w * c[e] + u * s[e];
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+          for (int e = 0; e < 8; e++) x[i][e] = NAN;
+      } else if (turns) {
+        if (!a.interleaved) {
+#pragma unroll
+          for (int e = 0; e < 8; e++) {
+            const double u = x[0][e], w = x[1][e];
+            x[0][e] = u * c[e] - w * s[e], x[1][e] = w * c[e] + u * s[e];
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; e++) {
+            const double u = x[e / 4][2 * (e % 4)], w = x[e / 4][2 * (e % 4) + 1];
+            x[e / 4][2 * (e % 4)] = u * c[e] - w * s[e], x[e / 4][2 * (e % 4) + 1] = w * c[e] + u * s[e];
+          }
         }
       }
-    } else if (j < turned) {
-      float c[8], s[8];
-      load8<F32>(reinterpret_cast<const char *>(table + 8 * j), c);
-      load8<F32>(reinterpret_cast<const char *>(table + a.rot / 2 + 8 * j), s);
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const double u = x[e / 4][2 * (e % 4)], w = x[e / 4][2 * (e % 4) + 1];
-        x[e / 4][2 * (e % 4)] = u * c[e] - w * s[e], x[e / 4][2 * (e % 4) + 1] = w * c[e] + u * s[e];
-      }
     }
-  }
-  if (is_q) {
-    char *to = static_cast<char *>(a.q_out) + (token * a.o_t + own * a.o_h) * TX::kBytes;
+    if (kind == 0) {
+      char *to = static_cast<char *>(a.q_out) + (token * a.o_t + own * a.o_h) * TX::kBytes;
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-      if (row < 0) {  // no sequence's token, or one of a refused sequence
+      for (int i = 0; i < 2; i++) {
+        if (row < 0) {  // no sequence's token, or one of a refused sequence
 #pragma unroll
-        for (int e = 0; e < 8; e++) x[i][e] = row == -1 ? 0.0 : NAN;
+          for (int e = 0; e < 8; e++) x[i][e] = row == -1 ? 0.0 : NAN;
+        }
+        store8<TX>(to + 8 * run[i] * TX::kBytes, x[i]);
       }
-      store8<TX>(to + 8 * run[i] * TX::kBytes, x[i]);
-    }
-  } else if ((is_k || is_v) && place) {
-    const int64_t at = row - page_of(row, mul) * a.pages.size;
-    char *to = is_k ? a.pages.k + page * a.pages.k_p + own * a.pages.k_h + at * a.pages.k_r
-                    : a.pages.v + page * a.pages.v_p + own * a.pages.v_h + at * a.pages.v_r;
-    if constexpr (std::is_same_v<TKV, I4>) {
-      char *pairs = is_k ? a.pages.kp + page * a.pages.kp_p + own * a.pages.kp_h + at * a.pages.kp_r
-                         : a.pages.vp + page * a.pages.vp_p + own * a.pages.vp_h + at * a.pages.vp_r;
-      store_codes<D>(to, pairs, run, j, x);
     } else {
+      char *to = kind == 1 ? a.pages.k + page * a.pages.k_p + own * a.pages.k_h + at * a.pages.k_r
+                           : a.pages.v + page * a.pages.v_p + own * a.pages.v_h + at * a.pages.v_r;
+      if constexpr (std::is_same_v<TKV, I4>) {
+        char *pairs = kind == 1 ? a.pages.kp + page * a.pages.kp_p + own * a.pages.kp_h + at * a.pages.kp_r
+                                : a.pages.vp + page * a.pages.vp_p + own * a.pages.vp_h + at * a.pages.vp_r;
+        store_codes<D>(to, pairs, run, j, x);
+      } else {
 #pragma unroll
-      for (int i = 0; i < 2; i++) store8<TKV>(to + 8 * run[i] * TKV::kBytes, x[i]);
+        for (int i = 0; i < 2; i++) store8<TKV>(to + 8 * run[i] * TKV::kBytes, x[i]);
+      }
     }
   }
 }
@@ -240,15 +263,18 @@ __global__ __launch_bounds__(256) void gather_kernel(PagedGather a, uint64_t mul
 }
 
 template <int D, class TX, class TKV>
-hipError_t launch_append(const PagedAppend &a, hipStream_t s) {
+hipError_t launch_append(const PagedAppend &a, int n_cu, hipStream_t s) {
   const int pieces = ((a.H + 2 * a.pages.Hk) * (D / 16) + 63) / 64;
-  const int64_t jobs = (int64_t)a.tokens * pieces + a.batch;
-  hipLaunchKernelGGL((append_kernel<D, TX, TKV>), dim3((unsigned)((jobs + 3) / 4)), dim3(256), 0, s, a, pieces, page_mul(a.pages.size));
+  // a piece a wave, until those fill the card
+  const int64_t waves = 16ll * n_cu;
+  const int parts = (int)std::clamp<int64_t>(waves / std::max(1, a.tokens), 1, pieces);
+  const int64_t jobs = (int64_t)a.tokens * parts + a.batch;
+  hipLaunchKernelGGL((append_kernel<D, TX, TKV>), dim3((unsigned)((jobs + 3) / 4)), dim3(256), 0, s, a, pieces, parts, page_mul(a.pages.size));
   return hipGetLastError();
 }
 template <class TX, class TKV>
-hipError_t launch_append(const PagedAppend &a, hipStream_t s) {
-  return a.pages.D == 64 ? launch_append<64, TX, TKV>(a, s) : launch_append<128, TX, TKV>(a, s);
+hipError_t launch_append(const PagedAppend &a, int n_cu, hipStream_t s) {
+  return a.pages.D == 64 ? launch_append<64, TX, TKV>(a, n_cu, s) : launch_append<128, TX, TKV>(a, n_cu, s);
 }
 template <class TKV, class TO>
 hipError_t launch_gather(const PagedGather &a, hipStream_t s) {
@@ -261,19 +287,19 @@ hipError_t launch_gather(const PagedGather &a, hipStream_t s) {
 
 }  // namespace
 
-hipError_t paged_append(const PagedAppend &a, hipStream_t s) {
+hipError_t paged_append(const PagedAppend &a, int n_cu, hipStream_t s) {
   if (a.batch <= 0) return hipSuccess;
   const int kv = a.pages.type;
   if (a.type == kOpF32) {
-    if (kv == kOpF32) return launch_append<F32, F32>(a, s);
-    if (kv == kOpBf16) return launch_append<F32, Bf16>(a, s);
-    if (kv == kOpI4) return launch_append<F32, I4>(a, s);
+    if (kv == kOpF32) return launch_append<F32, F32>(a, n_cu, s);
+    if (kv == kOpBf16) return launch_append<F32, Bf16>(a, n_cu, s);
+    if (kv == kOpI4) return launch_append<F32, I4>(a, n_cu, s);
   } else if (a.type == kOpBf16) {
-    if (kv == kOpBf16) return launch_append<Bf16, Bf16>(a, s);
-    if (kv == kOpI4) return launch_append<Bf16, I4>(a, s);
+    if (kv == kOpBf16) return launch_append<Bf16, Bf16>(a, n_cu, s);
+    if (kv == kOpI4) return launch_append<Bf16, I4>(a, n_cu, s);
   } else if (a.type == kOpF16) {
-    if (kv == kOpF16) return launch_append<F16, F16>(a, s);
-    if (kv == kOpI4) return launch_append<F16, I4>(a, s);
+    if (kv == kOpF16) return launch_append<F16, F16>(a, n_cu, s);
+    if (kv == kOpI4) return launch_append<F16, I4>(a, n_cu, s);
   }
   return hipErrorInvalidValue;
 }

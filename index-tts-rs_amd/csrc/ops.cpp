@@ -448,7 +448,7 @@ itts_status itts_paged_append(const itts_paged_append_args *args, void *stream) 
                         {a.starts, "starts"}, {a.lengths, "lengths"}, {a.n_table ? a.table : nullptr, "table"},
                         {any ? a.positions : nullptr, "positions"}, {a.new_lengths, "new_lengths"}}))
     return st;
-  if (hipError_t e = paged_append(a, static_cast<hipStream_t>(stream)); e != hipSuccess) return hip_fail(e, "paged append");
+  if (hipError_t e = paged_append(a, n_cu, static_cast<hipStream_t>(stream)); e != hipSuccess) return hip_fail(e, "paged append");
   return ITTS_OK;
 }
 
