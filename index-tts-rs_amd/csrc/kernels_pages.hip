@@ -46,7 +46,7 @@ __device__ __forceinline__ void store_codes(char *codes, char *pairs, const int 
     least[i] = most[i] = x[i][0];
 #pragma unroll
     for (int e = 0; e < 8; e++) {
-      least[i] = x[i][e] < least[i] ? x[i][e] : least[i], most[i] = x[i][e] > most[i] ? x[i][e] : most[i];
+      least[i] = fmin(least[i], x[i][e]), most[i] = fmax(most[i], x[i][e]);
       odd = __builtin_fma(x[i][e], 0.0, odd);  // NaN for a value that is no finite number
     }
     // (which then makes the range infinite)
@@ -57,11 +57,11 @@ __device__ __forceinline__ void store_codes(char *codes, char *pairs, const int 
   for (int G = 0; G < kGroups; G++) {
     const bool in0 = kGroups == 1 || run[0] >> 3 == G, in1 = kGroups == 1 || run[1] >> 3 == G;
     lo[G] = in0 ? least[0] : INFINITY, hi[G] = in0 ? most[0] : -INFINITY;
-    lo[G] = in1 && least[1] < lo[G] ? least[1] : lo[G], hi[G] = in1 && most[1] > hi[G] ? most[1] : hi[G];
+    lo[G] = fmin(lo[G], in1 ? least[1] : INFINITY), hi[G] = fmax(hi[G], in1 ? most[1] : -INFINITY);
 #pragma unroll
     for (int step = 1; step < kLanes; step *= 2) {
-      const double l = __shfl_xor(lo[G], step, 64), h = __shfl_xor(hi[G], step, 64);
-      lo[G] = l < lo[G] ? l : lo[G], hi[G] = h > hi[G] ? h : hi[G];
+      lo[G] = fmin(lo[G], __shfl_xor(lo[G], step, 64));
+      hi[G] = fmax(hi[G], __shfl_xor(hi[G], step, 64));
     }
   }
   double scale[kGroups], base[kGroups], inverse[kGroups];
@@ -82,14 +82,19 @@ __device__ __forceinline__ void store_codes(char *codes, char *pairs, const int 
     const double s = kGroups == 1 || run[i] >> 3 == 0 ? scale[0] : scale[kGroups - 1];
     const double b = kGroups == 1 || run[i] >> 3 == 0 ? base[0] : base[kGroups - 1];
     const double inv = kGroups == 1 || run[i] >> 3 == 0 ? inverse[0] : inverse[kGroups - 1];
+    auto code = [](double y) { return (uint32_t)(int)__builtin_amdgcn_fmed3f((float)__builtin_rint(y), 0.0f, 15.0f); };
     uint32_t w = 0;
+    bool near = false;
 #pragma unroll
     for (int e = 0; e < 8; e++) {
-      // (x - base) times 1 / scale is off by 2^-51 of at most 16: the quotient itself is needed next to a border alone
       const double y = (x[i][e] - b) * inv;
-      double c = __builtin_rint(y);
-      if (__builtin_expect(fabs(fabs(y - c) - 0.5) < 1e-12, 0)) c = __builtin_rint((x[i][e] - b) / s);
-      w |= (uint32_t)(int)__builtin_amdgcn_fmed3f((float)c, 0.0f, 15.0f) << (4 * e);
+      near = near || fabs(y - __builtin_rint(y)) > 0.5 - 1e-12;
+      w |= code(y) << (4 * e);
+    }
+    if (near) {  // the product is off by 2^-51 of at most 16: next to a border the quotient itself decides
+      w = 0;
+#pragma unroll
+      for (int e = 0; e < 8; e++) w |= code((x[i][e] - b) / s) << (4 * e);
     }
     *reinterpret_cast<uint32_t *>(codes + 4 * run[i]) = w;
   }
@@ -266,7 +271,7 @@ template <int D, class TX, class TKV>
 hipError_t launch_append(const PagedAppend &a, int n_cu, hipStream_t s) {
   const int pieces = ((a.H + 2 * a.pages.Hk) * (D / 16) + 63) / 64;
   // a piece a wave, until those fill the card
-  const int64_t waves = 16ll * n_cu;
+  const int64_t waves = 32ll * n_cu;
   const int parts = (int)std::clamp<int64_t>(waves / std::max(1, a.tokens), 1, pieces);
   const int64_t jobs = (int64_t)a.tokens * parts + a.batch;
   hipLaunchKernelGGL((append_kernel<D, TX, TKV>), dim3((unsigned)((jobs + 3) / 4)), dim3(256), 0, s, a, pieces, parts, page_mul(a.pages.size));
