@@ -28,6 +28,7 @@ struct Args {
   int blocks, parts, group;
   uint32_t group_mul;  // 2^32 / group, rounded up: exact for rows < 2^32 / group
   uint64_t page_mul;
+  bool even;           // pages of multiples of 32 rows
   int unit, least;     // a share is at least `least` times 2^unit tiles of keys
   float2 *ml;
   int2 *dealt;
@@ -163,6 +164,12 @@ struct Ids {
 };
 __device__ __forceinline__ Ids ids_of(const Args &p, const int32_t *table, int key0, int end) {
   Ids ids;
+  if (p.even) {  // (pages of whole tiles)
+    const int page = page_of(key0, p.page_mul);
+    ids.page[0] = ids.page[1] = uniform_load(table + page);
+    ids.at[0] = key0 - page * p.a.pages.size, ids.at[1] = ids.at[0] + 16;
+    return ids;
+  }
 #pragma unroll
   for (int h = 0; h < 2; h++) {
     const int key = h == 1 && key0 + 16 >= end ? key0 : key0 + 16 * h, page = page_of(key, p.page_mul);
@@ -173,11 +180,14 @@ __device__ __forceinline__ Ids ids_of(const Args &p, const int32_t *table, int k
 }
 __device__ __forceinline__ void bases_of(const Args &p, const Ids &ids, const char *pages, int64_t page_step, int64_t row_step,
                                          const char *(&base)[2]) {
-#pragma unroll
-  for (int h = 0; h < 2; h++) {
-    const int page = (uint32_t)ids.page[h] < (uint32_t)p.a.pages.n ? ids.page[h] : 0;
-    base[h] = pages + page * page_step + ids.at[h] * row_step;
-  }
+  // (pages are less than 2^32 bytes apart, rows less than 2^31)
+  auto at = [&](int h) {
+    const uint32_t page = (uint32_t)ids.page[h] < (uint32_t)p.a.pages.n ? ids.page[h] : 0;
+    return pages + (uint64_t)page * (uint32_t)page_step + (uint64_t)(uint32_t)ids.at[h] * (uint32_t)row_step;
+  };
+  base[0] = at(0);
+  if (p.even) base[1] = base[0] + 16 * (uint32_t)row_step;
+  else base[1] = at(1);
 }
 
 // A wave's keys and values of one tile: key rows 16 h + c, in runs of 8 elements 32 j + 8 g, and value rows 16 h + 4 g + r,
@@ -214,72 +224,24 @@ struct PageRegs {
   }
 };
 
-// The same of 4 bits: of each key row 16 h + c codes 64 G + 16 g .. + 15, of each value row 16 h + 4 g + r codes 64 G + 4 c .. + 3
-// (two bytes a register: joined where they are loaded, they would be waited for there), and the pairs of rows 16 h + 4 g + r
-// of both.
+// Of a tile of 4 bits: codes 64 G + 16 g .. + 15 of each key row 16 h + c, codes 64 G + 4 c .. + 3 of each value row
+// 16 h + 4 g + r, and the pairs of rows 16 h + 4 g + r of both.
 template <int D>
-struct PageRegs<D, I4> {
+struct CodeRegs {
   static constexpr int G = D / 64;
-  uint32_t k[2][G][2], v[8][G];
-  uint32_t kp[8][G], vp[8][G];
-  uint32_t k_at, v_at[4], kp_at[4], vp_at[4];
-  __device__ __forceinline__ void place(const Pages &g, int c, int q) {
-    k_at = c * (uint32_t)g.k_r + 8 * q;
-#pragma unroll
-    for (int r = 0; r < 4; r++) {
-      v_at[r] = (4 * q + r) * (uint32_t)g.v_r + 2 * c;
-      kp_at[r] = (4 * q + r) * (uint32_t)g.kp_r, vp_at[r] = (4 * q + r) * (uint32_t)g.vp_r;
-    }
-  }
-  static __device__ __forceinline__ void load_pairs(const char *at, uint32_t (&o)[G]) {
-    if constexpr (G == 1) o[0] = *reinterpret_cast<const uint32_t *>(at);
-    else load_dwords<2>(at, o);
-  }
-  __device__ __forceinline__ void load_k(const Args &p, const Ids &ids, int hk) {
-    const char *base[2], *pairs[2];
-    bases_of(p, ids, p.a.pages.k + hk * p.a.pages.k_h, p.a.pages.k_p, p.a.pages.k_r, base);
-    bases_of(p, ids, p.a.pages.kp + hk * p.a.pages.kp_h, p.a.pages.kp_p, p.a.pages.kp_r, pairs);
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-      asm volatile("" : "+v"(k_at));
-#pragma unroll
-      for (int i = 0; i < G; i++) load_dwords<2>(base[h] + 32 * i + k_at, k[h][i]);
-    }
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-      asm volatile("" : "+v"(kp_at[i & 3]));
-      load_pairs(pairs[i >> 2] + kp_at[i & 3], kp[i]);
-    }
-  }
-  __device__ __forceinline__ void load_v(const Args &p, const Ids &ids, int hk) {
-    const char *base[2], *pairs[2];
-    bases_of(p, ids, p.a.pages.v + hk * p.a.pages.v_h, p.a.pages.v_p, p.a.pages.v_r, base);
-    bases_of(p, ids, p.a.pages.vp + hk * p.a.pages.vp_h, p.a.pages.vp_p, p.a.pages.vp_r, pairs);
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-      asm volatile("" : "+v"(v_at[i & 3]));
-#pragma unroll
-      for (int j = 0; j < G; j++) v[i][j] = *reinterpret_cast<const uint16_t *>(base[i >> 2] + 32 * j + v_at[i & 3]);
-    }
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-      asm volatile("" : "+v"(vp_at[i & 3]));
-      load_pairs(pairs[i >> 2] + vp_at[i & 3], vp[i]);
-    }
-  }
+  uint32_t k[2][G][2], v[8][G], kp[8][G], vp[8][G];
 };
 
 // Of a dword with four codes in each half, codes d as bf16 pairs 1 + code / 16: one shift and one mask, the bits above are
 // the exponent of 1.  Sums of such products minus the sum of the other operand are 1/16 of those of the codes.
-template <int d>
-__device__ __forceinline__ uint32_t code_pair(uint32_t w) {
-  if constexpr (d == 0) w <<= 3;
-  else w >>= 4 * d - 3;
-  return (w & 0x00780078u) | 0x3f803f80u;
-}
-__device__ __forceinline__ void code_pairs(uint32_t w, uint32_t (&o)[4]) {
-  o[0] = code_pair<0>(w), o[1] = code_pair<1>(w), o[2] = code_pair<2>(w), o[3] = code_pair<3>(w);
-}
+struct CodeBits {
+  // (in registers of their own: one instruction takes both)
+  uint32_t mask = 0x00780078u, one = 0x3f803f80u;
+  __device__ __forceinline__ CodeBits() { asm volatile("" : "+s"(mask), "+v"(one)); }
+  __device__ __forceinline__ void pairs(uint32_t w, uint32_t (&o)[4]) const {
+    o[0] = (w << 3 & mask) | one, o[1] = (w >> 1 & mask) | one, o[2] = (w >> 5 & mask) | one, o[3] = (w >> 9 & mask) | one;
+  }
+};
 __device__ __forceinline__ float low_half(uint32_t w) { return (float)__builtin_bit_cast(f16x2v, w)[0]; }
 __device__ __forceinline__ float high_half(uint32_t w) { return (float)__builtin_bit_cast(f16x2v, w)[1]; }
 
@@ -293,18 +255,19 @@ struct Rows4 {
   static constexpr int G = D / 64, NQ = TQ::kBytes == 4 ? 3 : std::is_same_v<TQ, Bf16> ? 1 : 2, NP = kProbPlanes<TQ>;
   static constexpr float kLag = 5.0f;
   uint32_t q[NQ][RT][G][2][4];  // elements 64 G + 16 g + 8 j + (i, i + 4)
-  float qs[RT][G];              // sums of a group's elements
+  float qs[RT][G], qs16[RT][G]; // sums of a group's elements, and 1/16 of them
   float scale;
   floatx4 o[RT][D / 16];        // element 64 G + 4 (4 g + r) + d in register r of 4 G + d: sums with 1 + code / 16
   float ob[RT][G];              // sums of p (base - 16 scale), over this lane's keys
   float m[RT], l[RT];
+  CodeBits bits;
 
   // at[t]: the first element of tile t's row c
   __device__ __forceinline__ void load(const char *const (&at)[RT], float score_scale, int g) {
     const float by = score_scale * kLog2e;
     // (fp32 queries carry the scale, rounded once as their caller's own product would; 16-bit ones stay exact)
-    const float in = NQ == 3 ? by : 1.0f;
-    scale = NQ == 3 ? 16.0f : 16.0f * by;
+    const float in = NQ == 3 ? by : score_scale < 0.0f ? -1.0f : 1.0f;
+    scale = NQ == 3 ? 16.0f : fmaxf(16.0f * fabsf(by), 0x1p-120f);  // (0 times a mask's -inf would be NaN)
 #pragma unroll
     for (int t = 0; t < RT; t++) {
 #pragma unroll
@@ -317,9 +280,10 @@ struct Rows4 {
           float x[8];
 #pragma unroll
           for (int e = 0; e < 8; e++) {
-            if constexpr (TQ::kBytes == 4) x[e] = __uint_as_float(raw[e]) * in;
+            if constexpr (TQ::kBytes == 4) x[e] = __uint_as_float(raw[e]);
             else if constexpr (std::is_same_v<TQ, Bf16>) x[e] = __uint_as_float(e % 2 ? raw[e / 2] & 0xffff0000u : raw[e / 2] << 16);
             else x[e] = e % 2 ? high_half(raw[e / 2]) : low_half(raw[e / 2]);
+            x[e] *= in;
             sum += x[e];
           }
 #pragma unroll
@@ -332,7 +296,7 @@ struct Rows4 {
             }
           }
         }
-        qs[t][i] = col_sum(sum);
+        qs[t][i] = col_sum(sum), qs16[t][i] = qs[t][i] * 0.0625f;
         ob[t][i] = 0.0f;
       }
       m[t] = -INFINITY, l[t] = 0.0f;
@@ -341,7 +305,7 @@ struct Rows4 {
     }
   }
 
-  __device__ __forceinline__ void scores(floatx4 (&s)[2][RT], const PageRegs<D, I4> &x) const {
+  __device__ __forceinline__ void scores(floatx4 (&s)[2][RT], const CodeRegs<D> &x) const {
 #pragma unroll
     for (int h = 0; h < 2; h++) {
       floatx4 acc[G][RT];
@@ -352,7 +316,7 @@ struct Rows4 {
 #pragma unroll
         for (int j = 0; j < 2; j++) {
           uint32_t codes[4];
-          code_pairs(x.k[h][i][j], codes);
+          bits.pairs(x.k[h][i][j], codes);
 #pragma unroll
           for (int k = NQ - 1; k >= 0; k--)
 #pragma unroll
@@ -367,27 +331,27 @@ struct Rows4 {
 #pragma unroll
           for (int i = 0; i < G; i++) {
             const uint32_t pair = x.kp[4 * h + r][i];
-            v = __builtin_fmaf(high_half(pair), qs[t][i] * 0.0625f, v);
+            v = __builtin_fmaf(high_half(pair), qs16[t][i], v);
             v = __builtin_fmaf(low_half(pair), acc[i][t][r], v);
           }
           s[h][t][r] = v;
         }
     }
   }
-  // Running maxima; at an edge keys that are not seen count as -inf, those of a missing page as NaN.
+  // Running maxima; at an edge keys that are not seen count as -inf.
   __device__ __forceinline__ void limit(floatx4 (&s)[2][RT], bool edge, const uint32_t (&seen)[RT]) {
     float top[RT];
     bool grows = false;
 #pragma unroll
     for (int t = 0; t < RT; t++) {
+      if (edge) {
 #pragma unroll
-      for (int i = 0; i < 8; i++) {
-        s[i >> 2][t][i & 3] *= scale;
-        if (edge) s[i >> 2][t][i & 3] = seen[t] & 1u << (16 * (i >> 2) + (i & 3)) ? s[i >> 2][t][i & 3] : -INFINITY;
+        for (int i = 0; i < 8; i++) s[i >> 2][t][i & 3] = seen[t] & 1u << (16 * (i >> 2) + (i & 3)) ? s[i >> 2][t][i & 3] : -INFINITY;
       }
       top[t] = s[0][t][0];
 #pragma unroll
-      for (int i = 1; i < 8; i++) top[t] = fmaxf(top[t], s[i >> 2][t][i & 3]);
+      for (int i = 1; i < 7; i += 2) top[t] = fmaxf(fmaxf(s[i >> 2][t][i & 3], s[(i + 1) >> 2][t][(i + 1) & 3]), top[t]);
+      top[t] = fmaxf(s[1][t][3], top[t]) * scale;
       grows = grows || top[t] > m[t] + kLag;
     }
     if (__ballot(grows)) {
@@ -410,13 +374,14 @@ struct Rows4 {
       const float ms = m[t] == -INFINITY ? 0.0f : m[t];
 #pragma unroll
       for (int i = 0; i < 8; i++) {
-        const float p = __builtin_amdgcn_exp2f(s[i >> 2][t][i & 3] - ms);
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 2][t][i & 3], scale, -ms));
         s[i >> 2][t][i & 3] = p;
         l[t] += p;
       }
     }
   }
-  __device__ __forceinline__ void add(const floatx4 (&s)[2][RT], bool edge, const uint32_t (&seen)[RT], const PageRegs<D, I4> &x) {
+  template <bool EDGE>
+  __device__ __forceinline__ void add(const floatx4 (&s)[2][RT], const uint32_t (&seen)[RT], const CodeRegs<D> &x) {
 #pragma unroll
     for (int i = 0; i < G; i++) {
       uint32_t planes[RT][NP][4];
@@ -427,12 +392,14 @@ struct Rows4 {
 #pragma unroll
         for (int t = 0; t < RT; t++) {
           const float p0 = s[n >> 1][t][2 * (n & 1)], p1 = s[n >> 1][t][2 * (n & 1) + 1];
-          float a0 = p0 * s0, a1 = p1 * s1, c0 = p0 * b0, c1 = p1 * b1;
-          if (edge) {  // (0 times what a row that is not seen may hold: NaN)
+          float a0 = __builtin_fmaf(p0, s0, 0.0f), a1 = __builtin_fmaf(p1, s1, 0.0f);  // (takes fp16 as it is)
+          if constexpr (EDGE) {  // (0 times what a row that is not seen may hold: NaN)
             const uint32_t at = seen[t] >> (16 * (n >> 1) + 2 * (n & 1));
-            a0 = at & 1 ? a0 : 0.0f, c0 = at & 1 ? c0 : 0.0f, a1 = at & 2 ? a1 : 0.0f, c1 = at & 2 ? c1 : 0.0f;
+            a0 = at & 1 ? a0 : 0.0f, a1 = at & 2 ? a1 : 0.0f;
+            ob[t][i] += (at & 1 ? p0 * b0 : 0.0f) + (at & 2 ? p1 * b1 : 0.0f);
+          } else {
+            ob[t][i] = __builtin_fmaf(p0, b0, __builtin_fmaf(p1, b1, ob[t][i]));
           }
-          ob[t][i] += c0 + c1;
           uint32_t w[NP];
           cut_pos<Bf16, NP>(a0, a1, w);
 #pragma unroll
@@ -443,7 +410,7 @@ struct Rows4 {
 #pragma unroll
       for (int n = 0; n < 4; n++) {
         uint32_t w[4];
-        code_pairs(x.v[2 * n][i] | x.v[2 * n + 1][i] << 16, w);
+        bits.pairs(x.v[2 * n][i] | x.v[2 * n + 1][i] << 16, w);
 #pragma unroll
         for (int d = 0; d < 4; d++) codes[d][n] = w[d];
       }
@@ -456,12 +423,6 @@ struct Rows4 {
     }
   }
 };
-
-// Element of a row's run of four d .. d + 3 that register r of a lane group g holds.
-template <int D, class TKV>
-__device__ __forceinline__ int run_at(int g, int r, int d) {
-  return std::is_same_v<TKV, I4> ? 16 * d + 4 * (4 * g + r) : D / 16 * (4 * g + r) + d;
-}
 
 // Tokens in front of the first sequence (x) and from y on belong to none: their rows are zeros, which all blocks write.
 __device__ __forceinline__ int2 rest_of(const PagedAttn &a) {
@@ -527,12 +488,35 @@ __device__ inline void odd_values(float *y, const Args &p, const Seq &seq, const
   }
 }
 
+// The results of a block's waves over keys of their own, joined and put away; more(y, position, d) adds to a row's elements.
+template <int D, class TQ, int ROWS, int WK, class F>
+__device__ __forceinline__ void join_waves(const Args &p, const Share &share, const Seq &seq, int index, int hk, bool keys,
+                                           const float (&so)[WK][ROWS][D + 4], const float (&sm)[WK][ROWS], const float (&sl)[WK][ROWS], F more) {
+  for (int i = threadIdx.x; i < ROWS * (D / 4); i += 64 * WK) {
+    const int rr = i / (D / 4), d = i % (D / 4) * 4, r = share.tile * ROWS + rr;
+    if (r >= seq.rows) continue;
+    const int own = seq.len - seq.n + p.token(r);
+    float top = -INFINITY, sum = 0.0f, y[4] = {};
+#pragma unroll
+    for (int w = 0; w < WK; w++) top = fmaxf(top, sm[w][rr]);
+    const float ms = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+    for (int w = 0; w < WK; w++) {
+      const float f = __builtin_amdgcn_exp2f(sm[w][rr] - ms);
+      const float4 v = *reinterpret_cast<const float4 *>(&so[w][rr][d]);
+      sum += f * sl[w][rr];
+      y[0] += f * v.x, y[1] += f * v.y, y[2] += f * v.z, y[3] += f * v.w;
+    }
+    more(y, own, d);
+    put4<D, TQ, ROWS>(p, share, seq, index, hk, rr, d, y, top, sum, own >= 0, keys);
+  }
+}
+
 // Few query rows: 4 waves over tiles of keys of their own, straight from memory into registers, one tile ahead; joined at
 // the end.
 template <int D, class TQ, class TKV, int RT>
-__global__ __launch_bounds__(256, (D == 128 && std::is_same_v<TKV, F32> ? 1 : 2)) void paged_attn_kernel(Args p) {
+__global__ __launch_bounds__(256, (D == 128 && TKV::kBytes == 4 ? 1 : 2)) void paged_attn_kernel(Args p) {
   constexpr int WK = 4, kRows = 16 * RT;
-  constexpr bool kCodes = std::is_same_v<TKV, I4>;
   __shared__ float so[WK][kRows][D + 4];
   __shared__ float sm[WK][kRows], sl[WK][kRows];
   __shared__ int sodd[WK];
@@ -554,9 +538,9 @@ __global__ __launch_bounds__(256, (D == 128 && std::is_same_v<TKV, F32> ? 1 : 2)
   for (int t = 0; t < RT; t++) {
     const int r = min(share.tile * kRows + 16 * t + c, seq.rows - 1), i = p.token(r), head = hk * p.group + r - i * p.group;
     pos[t] = seq.len - seq.n + i;
-    at[t] = static_cast<const char *>(a.q) + ((seq.first_token + i) * a.q_t + head * a.q_h + (kCodes ? 0 : 8 * g)) * TQ::kBytes;
+    at[t] = static_cast<const char *>(a.q) + ((seq.first_token + i) * a.q_t + head * a.q_h + 8 * g) * TQ::kBytes;
   }
-  typename std::conditional<kCodes, Rows4<D, TQ, RT>, Rows<D, TQ, typename std::conditional<kCodes, Bf16, TKV>::type, RT, false>>::type rows;
+  Rows<D, TQ, TKV, RT, false> rows;
   PageRegs<D, TKV> x;
   x.place(a.pages, c, g);
   uint32_t odd = 0;  // a value that is no finite number was taken out
@@ -568,18 +552,13 @@ __global__ __launch_bounds__(256, (D == 128 && std::is_same_v<TKV, F32> ? 1 : 2)
     x.load_k(p, ids, hk);
     x.load_v(p, ids, hk);
   }
-  if constexpr (kCodes) rows.load(at, a.scale, g);
-  else rows.load(at, a.scale);
+  rows.load(at, a.scale);
 
   for (; u < end; u += WK) {
     const int key0 = tiles.key(u), missing = ids.missing(a);
     floatx4 s[2][RT] = {};
-    if constexpr (kCodes) {
-      rows.scores(s, x);
-    } else {
 #pragma unroll
-      for (int j = 0; j < D / 32; j++) rows.scores(s, j, x.k[0][j], x.k[1][j]);
-    }
+    for (int j = 0; j < D / 32; j++) rows.scores(s, j, x.k[0][j], x.k[1][j]);
     // the wave's next tile (past the last one: that one again)
     ids = next;
     x.load_k(p, ids, hk);
@@ -599,66 +578,245 @@ __global__ __launch_bounds__(256, (D == 128 && std::is_same_v<TKV, F32> ? 1 : 2)
     }
     rows.limit(s, edge, seen);
     rows.weigh(s);
-    if constexpr (kCodes) {
-      rows.add(s, edge, seen, x);
+    if (edge) odd |= take_odd<TKV>(x.v, key0, 0, seq.p1 + 1, g);
+    if constexpr (TKV::kBytes == 4) {
+      rows.add_wide(s, x.v);
     } else {
-      if (edge) odd |= take_odd<TKV>(x.v, key0, 0, seq.p1 + 1, g);
-      if constexpr (TKV::kBytes == 4) {
-        rows.add_wide(s, x.v);
-      } else {
-        typename decltype(rows)::Probs probs;
-        rows.pack(s, probs);
-        rows.add_rows(probs, x.v);
-      }
+      typename decltype(rows)::Probs probs;
+      rows.pack(s, probs);
+      rows.add_rows(probs, x.v);
     }
     x.load_v(p, ids, hk);
   }
 
   // The waves joined.
-  if (const bool any = __ballot(odd != 0) != 0; lane == 0) sodd[wave] = any;
+  const bool any = __ballot(odd != 0) != 0;
+  if (lane == 0) sodd[wave] = any;
 #pragma unroll
   for (int t = 0; t < RT; t++) {
     const float l = col_sum(rows.l[t]);
     if (g == 0) sm[wave][16 * t + c] = rows.m[t], sl[wave][16 * t + c] = l;
-    float by = 1.0f, plus[D / 64] = {};
-    if constexpr (kCodes) {
-      by = 16.0f;
-#pragma unroll
-      for (int i = 0; i < D / 64; i++) plus[i] = col_sum(rows.ob[t][i]);
-    }
 #pragma unroll
     for (int r = 0; r < 4; r++)
 #pragma unroll
-      for (int d = 0; d < D / 16; d += 4) {
-        float y[4];
-#pragma unroll
-        for (int e = 0; e < 4; e++) y[e] = kCodes ? __builtin_fmaf(rows.o[t][d + e][r], by, plus[d / 4 % (D / 64)]) : rows.o[t][d + e][r];
-        *reinterpret_cast<float4 *>(&so[wave][16 * t + c][run_at<D, TKV>(g, r, d)]) = make_float4(y[0], y[1], y[2], y[3]);
-      }
+      for (int d = 0; d < D / 16; d += 4)
+        *reinterpret_cast<float4 *>(&so[wave][16 * t + c][D / 16 * (4 * g + r) + d]) =
+            make_float4(rows.o[t][d][r], rows.o[t][d + 1][r], rows.o[t][d + 2][r], rows.o[t][d + 3][r]);
   }
   __syncthreads();
   int odd_any = 0;
 #pragma unroll
   for (int w = 0; w < WK; w++) odd_any |= sodd[w];
-  for (int i = threadIdx.x; i < kRows * (D / 4); i += 64 * WK) {
-    const int rr = i / (D / 4), d = i % (D / 4) * 4, r = share.tile * kRows + rr;
-    if (r >= seq.rows) continue;
-    const int own = seq.len - seq.n + p.token(r);
-    float top = -INFINITY, sum = 0.0f, y[4] = {};
+  join_waves<D, TQ, kRows>(p, share, seq, index, hk, first < end, so, sm, sl, [&](float *y, int own, int d) {
+    if (odd_any) odd_values<D, TKV>(y, p, seq, tiles, first, end, table, hk, own, d);
+  });
+  clear_rest<D, TQ>(a, rest);
+}
+
+// ---- 4 bits ----
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+// 16 or 4 bytes a lane from anywhere to LDS at lds + 16 (4) lane, without a register in between.  The compiler does not know of
+// these loads: copies_wait() has to come before what they bring is read.
+__device__ __forceinline__ void copy16(const char *from, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(lds) : "memory", "m0");
+}
+__device__ __forceinline__ void copy4(const char *from, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(from), "s"(lds) : "memory", "m0");
+}
+// (from a base that all lanes share)
+__device__ __forceinline__ void copy16(const char *base, uint32_t offset, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(lds) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+// Waits until at most N of the wave's copies are on their way, and for its reads of LDS.
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ uint32_t lds_address(const void *p) {
+  return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void *)p;
+}
+
+// Few query rows (or many) over 4 bits: 4 waves over tiles of 32 keys of their own, each with a ring of tiles in LDS that direct
+// loads fill: few instructions for many small rows, no registers for what is on its way, and the operands' order comes from
+// how LDS is read.  Row r of 16 lies in slot 4 (r % 4) + r / 4, its 16-byte pieces in another order by row (piece ^ r % 4, of two
+// pieces piece ^ r / 2 % 2): reads of 16 key rows' same piece and of four value rows' same part fall on different banks.
+template <int D, class TQ>
+constexpr int kCodeBlocks = D == 64 ? (TQ::kBytes == 4 ? 3 : 4) : TQ::kBytes == 4 ? 2 : 3;  // a compute unit
+template <int D, class TQ, int RT>
+__global__ __launch_bounds__(256, (kCodeBlocks<D, TQ>)) void paged_codes_kernel(Args p) {
+  constexpr int WK = 4, kRows = 16 * RT, G = D / 64, kStages = kCodeBlocks<D, TQ> == 2 ? 4 : D == 64 ? 3 : 2, kLoads = D == 128 ? 6 : 3;
+  constexpr int kRow = D / 2, kCodes = kTileKeys * kRow, kPairs = kTileKeys * 4 * G, kStage = 2 * (kCodes + kPairs);  // bytes
+  struct Join {
+    float so[WK][kRows][D + 4], sm[WK][kRows], sl[WK][kRows];
+  };
+  constexpr size_t kRing = (size_t)WK * kStages * kStage, kBytes = kRing > sizeof(Join) ? kRing : sizeof(Join);
+  __shared__ __attribute__((aligned(256))) char mem[kBytes];
+  const PagedAttn &a = p.a;
+  const Pages &pg = a.pages;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
+  const int hk = blockIdx.x % pg.Hk, index = blockIdx.x / pg.Hk;
+  const int2 rest = rest_of(a);
+  const Share share = share_of<kRows, kTileKeys>(p, index);
+  if (share.n == 0) return clear_rest<D, TQ>(a, rest);
+  if (p.parts > 0 && index == share.from && hk == 0 && threadIdx.x == 0) p.dealt[share.b] = make_int2(share.from, share.n);
+  const Seq seq = seq_of<kRows>(p, share);
+  const Tiles<kTileKeys> tiles(a, seq.p0, seq.p1);
+  const int first = min(share.first, tiles.n), end = min(share.end, tiles.n);
+  const int32_t *table = a.table + share.b * a.tab_b;
+
+  // Copies of a tile.
+  const uint32_t ring = lds_address(mem) + wave * kStages * kStage;
+  const int slot = D == 128 ? lane >> 2 : (lane & 31) >> 1, row = (slot & 3) * 4 + (slot >> 2);
+  const int piece = D == 128 ? (lane & 3) ^ (row & 3) : (lane & 1) ^ (row >> 1 & 1);
+  const uint32_t k_at = row * (uint32_t)pg.k_r + 16 * piece, v_at = row * (uint32_t)pg.v_r + 16 * piece;
+  const uint32_t kp_at = D == 128 ? (lane >> 1 & 15) * (uint32_t)pg.kp_r + 4 * (lane & 1) : (lane & 15) * (uint32_t)(lane < 32 ? pg.kp_r : pg.vp_r);
+  const uint32_t vp_at = (lane >> 1 & 15) * (uint32_t)pg.vp_r + 4 * (lane & 1);
+  const char *kb = pg.k + hk * pg.k_h, *vb = pg.v + hk * pg.v_h, *kpb = pg.kp + hk * pg.kp_h, *vpb = pg.vp + hk * pg.vp_h;
+  auto copy = [&](const Ids &ids, uint32_t lds) {
+    const char *k[2], *v[2], *kp[2], *vp[2];
+    bases_of(p, ids, kb, pg.k_p, pg.k_r, k), bases_of(p, ids, vb, pg.v_p, pg.v_r, v);
+    bases_of(p, ids, kpb, pg.kp_p, pg.kp_r, kp), bases_of(p, ids, vpb, pg.vp_p, pg.vp_r, vp);
+    if constexpr (D == 128) {
 #pragma unroll
-    for (int w = 0; w < WK; w++) top = fmaxf(top, sm[w][rr]);
-    const float ms = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-    for (int w = 0; w < WK; w++) {
-      const float f = __builtin_amdgcn_exp2f(sm[w][rr] - ms);
-      const float4 v = *reinterpret_cast<const float4 *>(&so[w][rr][d]);
-      sum += f * sl[w][rr];
-      y[0] += f * v.x, y[1] += f * v.y, y[2] += f * v.z, y[3] += f * v.w;
+      for (int h = 0; h < 2; h++) {
+        copy16(k[h], k_at, lds + h * 16 * kRow);
+        copy16(v[h], v_at, lds + kCodes + h * 16 * kRow);
+      }
+      copy4((lane < 32 ? kp[0] : kp[1]) + kp_at, lds + 2 * kCodes);
+      copy4((lane < 32 ? vp[0] : vp[1]) + vp_at, lds + 2 * kCodes + kPairs);
+    } else {
+      copy16((lane < 32 ? k[0] : k[1]) + k_at, lds);
+      copy16((lane < 32 ? v[0] : v[1]) + v_at, lds + kCodes);
+      const char *lo = lane < 32 ? kp[0] : vp[0], *hi = lane < 32 ? kp[1] : vp[1];
+      copy4((lane & 16 ? hi : lo) + kp_at, lds + 2 * kCodes);
     }
-    if constexpr (!kCodes)
-      if (odd_any) odd_values<D, TKV>(y, p, seq, tiles, first, end, table, hk, own, d);
-    put4<D, TQ, kRows>(p, share, seq, index, hk, rr, d, y, top, sum, own >= 0, first < end);
+  };
+  // Reads of a tile.
+  const uint32_t key_at = ((c & 3) * 4 + (c >> 2)) * kRow + 16 * ((g >> 1) ^ (D == 128 ? c & 3 : c >> 1 & 1)) + 8 * (g & 1);
+  const uint32_t value_at = kCodes + g * kRow + 16 * (c >> 3) + 2 * (c & 7), pair_at = 2 * kCodes + 16 * G * g;
+  auto read = [&](CodeRegs<D> &x, uint32_t lds) {
+    using Two = __attribute__((address_space(3))) const u32x2;
+    using Four = __attribute__((address_space(3))) const u32x4;
+    using Short = __attribute__((address_space(3))) const uint16_t;
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+#pragma unroll
+      for (int i = 0; i < G; i++) {
+        const u32x2 w = *(Two *)(uintptr_t)(lds + (key_at ^ 32 * i) + h * 16 * kRow);
+        x.k[h][i][0] = w[0], x.k[h][i][1] = w[1];
+      }
+#pragma unroll
+      for (int i = 0; i < G; i++) {
+        const u32x4 kp = *(Four *)(uintptr_t)(lds + pair_at + h * 64 * G + 16 * i);
+        const u32x4 vp = *(Four *)(uintptr_t)(lds + pair_at + kPairs + h * 64 * G + 16 * i);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const int at = 4 * i + e;  // dwords [row][group]
+          x.kp[4 * h + at / G][at % G] = kp[e], x.vp[4 * h + at / G][at % G] = vp[e];
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < 4; r++)
+#pragma unroll
+        for (int i = 0; i < G; i++)
+          x.v[4 * h + r][i] = *(Short *)(uintptr_t)(lds + (value_at ^ 32 * i ^ 16 * (D == 128 ? r : r >> 1)) + (4 * r + 16 * h) * kRow);
+    }
+  };
+
+  const char *at[RT];
+  int pos[RT];
+#pragma unroll
+  for (int t = 0; t < RT; t++) {
+    const int r = min(share.tile * kRows + 16 * t + c, seq.rows - 1), i = p.token(r), head = hk * p.group + r - i * p.group;
+    pos[t] = seq.len - seq.n + i;
+    at[t] = static_cast<const char *>(a.q) + ((seq.first_token + i) * a.q_t + head * a.q_h) * TQ::kBytes;
   }
+  Rows4<D, TQ, RT> rows;
+  rows.load(at, a.scale, g);
+  copies_wait<0>();  // (the queries are there: from here on the wave's loads are counted by hand)
+
+  // Tiles first + wave, in steps of WK: n of them.  `missing`: two bits a tile, the next one's lowest.
+  const int n = max(0, (end - first - wave + WK - 1) / WK), u0 = first + wave;
+  uint32_t missing = 0;
+  Ids next;
+  auto fetch = [&](int i) { return ids_of(p, table, tiles.key(u0 + WK * min(i, n - 1)), seq.p1 + 1); };
+  auto issue = [&](int i) {
+    missing |= next.missing(a) << 2 * (kStages - 1);
+    copy(next, ring + i % kStages * kStage);
+    next = fetch(i + 1);
+  };
+  if (n > 0) {
+    next = fetch(0);
+#pragma unroll
+    for (int i = 0; i < kStages - 1; i++) {
+      if (i < n) issue(i);
+      missing >>= 2;
+    }
+  }
+  auto step = [&](auto is_edge, int i, int key0, int gone) {
+    constexpr bool kEdge = decltype(is_edge)::value;
+    CodeRegs<D> x;
+    read(x, ring + i % kStages * kStage);
+    floatx4 s[2][RT];
+    rows.scores(s, x);
+    uint32_t seen[RT] = {};
+    if constexpr (kEdge) {
+#pragma unroll
+      for (int t = 0; t < RT; t++) {
+        seen[t] = seen_bits(a, pos[t], key0) >> (4 * g);
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+          if (gone >> (e >> 2) & 1) s[e >> 2][t][e & 3] = NAN;
+      }
+    }
+    rows.limit(s, kEdge, seen);
+    rows.weigh(s);
+    rows.template add<kEdge>(s, seen, x);
+  };
+  // waits for tile i, sends for the one kStages - 1 later into the place of the one before
+  auto turn = [&](int i, int &key0, int &gone) {
+    if (i + kStages - 2 < n) copies_wait<kLoads * (kStages - 2)>();
+    else copies_wait<0>();
+    if (i + kStages - 1 < n) issue(i + kStages - 1);
+    key0 = tiles.key(u0 + WK * i), gone = missing & 3;
+    missing >>= 2;
+  };
+  for (int i = 0; i < n;) {
+    int key0, gone;
+    turn(i, key0, gone);
+    while (all_see<kTileKeys>(a, seq.p0, seq.p1, key0) && gone == 0) {
+      step(std::false_type{}, i, key0, 0);
+      if (++i == n) break;
+      turn(i, key0, gone);
+    }
+    if (i == n) break;
+    step(std::true_type{}, i, key0, gone);
+    i++;
+  }
+
+  copies_wait<0>();
+  __syncthreads();  // (the rings' memory is used again)
+  Join &join = *reinterpret_cast<Join *>(mem);
+#pragma unroll
+  for (int t = 0; t < RT; t++) {
+    const float l = col_sum(rows.l[t]);
+    if (g == 0) join.sm[wave][16 * t + c] = rows.m[t], join.sl[wave][16 * t + c] = l;
+#pragma unroll
+    for (int i = 0; i < G; i++) {
+      const float plus = col_sum(rows.ob[t][i]);
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        float y[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) y[e] = __builtin_fmaf(rows.o[t][4 * i + e][r], 16.0f, plus);
+        *reinterpret_cast<float4 *>(&join.so[wave][16 * t + c][64 * i + 4 * (4 * g + r)]) = make_float4(y[0], y[1], y[2], y[3]);
+      }
+    }
+  }
+  __syncthreads();
+  join_waves<D, TQ, kRows>(p, share, seq, index, hk, first < end, join.so, join.sm, join.sl, [](float *, int, int) {});
   clear_rest<D, TQ>(a, rest);
 }
 
@@ -672,17 +830,6 @@ template <int D>
 __device__ __forceinline__ int swizzle(int row) {
   return D == 128 ? (row & 3) << 2 | (row >> 2 & 3) : (row >> 1 & 1) << 2 | (row >> 2 & 3);
 }
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"
-// 16 bytes a lane from base + offset to LDS at lds + 16 lane, without a register in between.  The compiler does not know of
-// the load: copies_wait() has to come before what it brings is read.
-__device__ __forceinline__ void copy16(const char *base, uint32_t offset, const u32x4 *lds) {
-  const uint32_t m0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void *)lds;
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(m0) : "memory", "m0");
-}
-#pragma clang diagnostic pop
-__device__ __forceinline__ void copies_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
-
 template <class T>
 __device__ __forceinline__ floatx16 mfma32(const uint32_t (&a)[4], const uint32_t (&b)[4], floatx16 c) {
   const u32x4 x = {a[0], a[1], a[2], a[3]}, y = {b[0], b[1], b[2], b[3]};
@@ -753,7 +900,7 @@ __global__ __launch_bounds__(256, (TQ::kBytes == 4 ? (D == 64 ? 2 : 1) : D == 64
   auto copy = [&](const char *from, int64_t page_step, int64_t row_step, const uint32_t (&offset)[kCopies], int page, int at, u32x4 *to) {
     const char *base = from + ((uint32_t)page < (uint32_t)a.pages.n ? page : 0) * page_step + at * row_step;
 #pragma unroll
-    for (int i = 0; i < kCopies; i++) copy16(base, offset[i], to + 16 * kPieces * wave + 64 * i);
+    for (int i = 0; i < kCopies; i++) copy16(base, offset[i], lds_address(to + 16 * kPieces * wave + 64 * i));
   };
 
   // The wave's query rows: lane (c, h) elements 16 j + 8 h .. of row c.
@@ -854,7 +1001,7 @@ __global__ __launch_bounds__(256, (TQ::kBytes == 4 ? (D == 64 ? 2 : 1) : D == 64
     copy(vb, a.pages.v_p, a.pages.v_r, v_at, page0, at0, value_mem[0]);
 #pragma unroll
     for (int i = 0; i < kCopies; i++) value_mem[2][64 * kCopies * wave + 64 * i + lane] = u32x4{};  // (probabilities of 0 times it)
-    copies_wait();
+    copies_wait<0>();
     __syncthreads();
     u32x4 k[D / 16];
     read_keys(k, 0, key_at);
@@ -934,7 +1081,7 @@ __global__ __launch_bounds__(256, (TQ::kBytes == 4 ? (D == 64 ? 2 : 1) : D == 64
       __builtin_amdgcn_sched_barrier(0);
       scores(s[1], k);
       ring = ring1;
-      copies_wait();
+      copies_wait<0>();
       __syncthreads();
     }
     add(1, value_at + (ring == 0 ? 2 : ring - 1) * kTileBytes);
@@ -1010,6 +1157,10 @@ __global__ __launch_bounds__(256) void paged_join_kernel(Args p) {
   store4<TQ>(static_cast<char *>(a.out) + (token * a.o_t + head * a.o_h + d) * TQ::kBytes, x[0], x[1], x[2], x[3]);
 }
 
+int code_blocks(int D, int type) {
+  return D == 64 ? (type == kOpF32 ? kCodeBlocks<64, F32> : kCodeBlocks<64, Bf16>)
+                 : type == kOpF32 ? kCodeBlocks<128, F32> : type == kOpBf16 ? kCodeBlocks<128, Bf16> : kCodeBlocks<128, F16>;
+}
 // How a launch is laid out: rows of a block, blocks of a key head, or `parts` that share the keys.
 struct Plan {
   bool many;  // paged_rows_kernel
@@ -1024,7 +1175,7 @@ Plan make_plan(const PagedAttn &a, int n_cu) {
   const int64_t most = std::min<int64_t>((int64_t)a.tokens * group / p.rows + std::min(a.batch, a.tokens),
                                          (int64_t)a.tokens * ((group + p.rows - 1) / p.rows));
   p.parts = 0, p.blocks = (int)most;
-  const int at_once = n_cu * 2 / a.pages.Hk;
+  const int at_once = n_cu * (a.pages.type != kOpI4 ? 2 : code_blocks(a.pages.D, a.type)) / a.pages.Hk;
   if (most < at_once && a.max_rows > 512) p.parts = p.blocks = std::max(at_once, (int)most);
   return p;
 }
@@ -1033,7 +1184,7 @@ size_t part_rows(const PagedAttn &a, const Plan &p) { return (size_t)a.pages.Hk 
 Args make_args(const PagedAttn &a, const Plan &p) {
   const int group = a.H / a.pages.Hk;
   float *ml = a.part + part_rows(a, p) * a.pages.D;
-  return Args{a, p.blocks, p.parts, group, (uint32_t)(((1ull << 32) + group - 1) / group), page_mul(a.pages.size), p.unit, p.least,
+  return Args{a, p.blocks, p.parts, group, (uint32_t)(((1ull << 32) + group - 1) / group), page_mul(a.pages.size), a.pages.size % 32 == 0, p.unit, p.least,
               reinterpret_cast<float2 *>(ml), reinterpret_cast<int2 *>(ml + 2 * part_rows(a, p))};
 }
 template <int D, class TQ, int ROWS, class K>
@@ -1048,7 +1199,8 @@ template <int D, class TQ, class TKV>
 hipError_t launch_d(const PagedAttn &a, const Plan &p, hipStream_t s) {
   if constexpr (std::is_same_v<TKV, Bf16> || std::is_same_v<TKV, F16>)
     if (p.many) return launch_kernel<D, TQ, kLongRows>(paged_rows_kernel<D, TQ, TKV>, a, p, s);
-  return launch_kernel<D, TQ, 16>(paged_attn_kernel<D, TQ, TKV, 1>, a, p, s);
+  if constexpr (std::is_same_v<TKV, I4>) return launch_kernel<D, TQ, 16>(paged_codes_kernel<D, TQ, 1>, a, p, s);
+  else return launch_kernel<D, TQ, 16>(paged_attn_kernel<D, TQ, TKV, 1>, a, p, s);
 }
 template <class TQ, class TKV>
 hipError_t launch(const PagedAttn &a, const Plan &p, hipStream_t s) {

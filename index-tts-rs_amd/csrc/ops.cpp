@@ -212,6 +212,9 @@ itts_status pages_args(const itts_pages &g, bool writes, Pages *o) {
   if (g.k_row * es > kTreeMaxRowBytes || g.v_row * es > kTreeMaxRowBytes ||
       (t == kOpI4 && (g.k_params_row * 2 > kTreeMaxRowBytes || g.v_params_row * 2 > kTreeMaxRowBytes)))
     return fail(ITTS_E_VALIDATION, "pages.k_row, v_row: rows must be at most %d bytes apart", kTreeMaxRowBytes);
+  if (g.n_pages > 1 && (g.k_page * es > UINT32_MAX || g.v_page * es > UINT32_MAX ||
+                        (t == kOpI4 && (g.k_params_page * 2 > UINT32_MAX || g.v_params_page * 2 > UINT32_MAX))))
+    return fail(ITTS_E_VALIDATION, "pages.k_page, v_page: pages must be less than 2^32 bytes apart");
   if (writes) {
     auto meet = [&](const int64_t(&a)[3], const int64_t(&b)[3], const void *x, const void *y, int size, int n) {
       if (rows_overlap<3>({{{a[0], ext[0]}, {a[1], ext[1]}, {a[2], ext[2]}}}, n) || rows_overlap<3>({{{b[0], ext[0]}, {b[1], ext[1]}, {b[2], ext[2]}}}, n))
