@@ -645,7 +645,7 @@ __device__ __forceinline__ uint32_t lds_address(const void *p) {
 template <int D, class TQ>
 constexpr int kCodeBlocks = D == 64 ? (TQ::kBytes == 4 ? 3 : 4) : TQ::kBytes == 4 ? 2 : 3;  // a compute unit
 template <int D, class TQ, int RT>
-__global__ __launch_bounds__(256, (kCodeBlocks<D, TQ>)) void paged_codes_kernel(Args p) {
+__global__ __launch_bounds__(256, (RT == 2 ? 2 : kCodeBlocks<D, TQ>)) void paged_codes_kernel(Args p) {
   constexpr int WK = 4, kRows = 16 * RT, G = D / 64, kStages = kCodeBlocks<D, TQ> == 2 ? 4 : D == 64 ? 3 : 2, kLoads = D == 128 ? 6 : 3;
   constexpr int kRow = D / 2, kCodes = kTileKeys * kRow, kPairs = kTileKeys * 4 * G, kStage = 2 * (kCodes + kPairs);  // bytes
   struct Join {
@@ -848,6 +848,16 @@ __device__ __forceinline__ uint32_t scale_pair(uint32_t w, float f) {
   const float y = __builtin_copysignf(fmaxf(fabsf(b * f), fminf(fabsf(b), kLeast)), b);
   if constexpr (std::is_same_v<T, Bf16>) return cut_pair(x, y);
   else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x, y));
+}
+
+// Whether it is so anywhere in a block of four waves, by way of LDS that is no longer needed.
+__device__ __forceinline__ bool any_in_block(bool v, void *mem) {
+  int *flags = static_cast<int *>(mem);
+  const bool wave = __ballot(v) != 0;
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) flags[threadIdx.x >> 6] = wave;
+  __syncthreads();
+  return (flags[0] | flags[1] | flags[2] | flags[3]) != 0;
 }
 
 // Many query rows over 16-bit caches: 4 waves with 32 rows each over the same tiles of 64 keys, which come to LDS by direct
@@ -1087,7 +1097,7 @@ __global__ __launch_bounds__(256, (TQ::kBytes == 4 ? (D == 64 ? 2 : 1) : D == 64
     add(1, value_at + (ring == 0 ? 2 : ring - 1) * kTileBytes);
   }
 
-  const bool odd_any = __ballot(odd != 0) != 0;
+  const bool odd_any = any_in_block(odd != 0, key_mem);  // (a wave has cleaned its rows of the tiles)
   l += __shfl_xor(l, 32, 64);
   const int row = 32 * wave + c;
   if (share.tile * kLongRows + row < seq.rows) {
@@ -1164,19 +1174,28 @@ int code_blocks(int D, int type) {
 // How a launch is laid out: rows of a block, blocks of a key head, or `parts` that share the keys.
 struct Plan {
   bool many;  // paged_rows_kernel
+  int RT;     // tiles of 16 rows of a block otherwise
   int rows, blocks, parts, unit, least;
 };
 Plan make_plan(const PagedAttn &a, int n_cu) {
   Plan p;
-  const int group = a.H / a.pages.Hk;
-  p.many = a.pages.type != kOpF32 && a.pages.type != kOpI4 && (int64_t)a.tokens * group >= 64 * (int64_t)a.batch;
-  p.rows = p.many ? kLongRows : 16, p.unit = p.many ? 1 : 2, p.least = 2;
+  const int group = a.H / a.pages.Hk, D = a.pages.D;
+  const bool wide = a.type == kOpF32, codes = a.pages.type == kOpI4;
+  // Query rows of a sequence on average.  Shared tiles pay from here on (8 sequences of 4,000 rows, us, waves with keys of their own
+  // and shared tiles): bf16, 8 key heads of 128, 32 rows 34, 41, 64 rows 51, 43, 128 rows 81, 50; 16 of 64, 64 rows 38, 45, 128
+  // rows 52, 51; fp32 over bf16 64 rows 53, 74, 128 rows 83, 83; of 64, 128 rows 57, 70.
+  const int64_t rows = (int64_t)a.tokens * group / std::max(1, a.batch);
+  p.many = !codes && a.pages.type != kOpF32 && rows >= 8192 / D * (wide ? 2 : 1);
+  // (fp32 queries of 128 elements would not fit the registers twice)
+  p.RT = !p.many && rows >= 32 && (D == 64 || (codes && !wide)) ? 2 : 1;
+  p.rows = p.many ? kLongRows : 16 * p.RT, p.unit = p.many ? 1 : 2, p.least = 2;
   // row tiles at most: a sequence's last one may be short
   const int64_t most = std::min<int64_t>((int64_t)a.tokens * group / p.rows + std::min(a.batch, a.tokens),
                                          (int64_t)a.tokens * ((group + p.rows - 1) / p.rows));
   p.parts = 0, p.blocks = (int)most;
-  const int at_once = n_cu * (a.pages.type != kOpI4 ? 2 : code_blocks(a.pages.D, a.type)) / a.pages.Hk;
-  if (most < at_once && a.max_rows > 512) p.parts = p.blocks = std::max(at_once, (int)most);
+  const int at_once = n_cu * (codes && !p.many && p.RT == 1 ? code_blocks(D, a.type) : 2) / a.pages.Hk;
+  const int64_t seen = a.window > 0 ? std::min<int64_t>(a.max_rows, (int64_t)a.window + std::min(a.sinks, a.max_rows)) : a.max_rows;
+  if (most < at_once && seen > (a.pages.type == kOpF32 ? 512 : 1024)) p.parts = p.blocks = std::max(at_once, (int)most);
   return p;
 }
 
@@ -1199,8 +1218,15 @@ template <int D, class TQ, class TKV>
 hipError_t launch_d(const PagedAttn &a, const Plan &p, hipStream_t s) {
   if constexpr (std::is_same_v<TKV, Bf16> || std::is_same_v<TKV, F16>)
     if (p.many) return launch_kernel<D, TQ, kLongRows>(paged_rows_kernel<D, TQ, TKV>, a, p, s);
-  if constexpr (std::is_same_v<TKV, I4>) return launch_kernel<D, TQ, 16>(paged_codes_kernel<D, TQ, 1>, a, p, s);
-  else return launch_kernel<D, TQ, 16>(paged_attn_kernel<D, TQ, TKV, 1>, a, p, s);
+  if constexpr (std::is_same_v<TKV, I4>) {
+    if constexpr (D == 64 || TQ::kBytes == 2)
+      if (p.RT == 2) return launch_kernel<D, TQ, 32>(paged_codes_kernel<D, TQ, 2>, a, p, s);
+    return launch_kernel<D, TQ, 16>(paged_codes_kernel<D, TQ, 1>, a, p, s);
+  } else {
+    if constexpr (D == 64)
+      if (p.RT == 2) return launch_kernel<D, TQ, 32>(paged_attn_kernel<D, TQ, TKV, 2>, a, p, s);
+    return launch_kernel<D, TQ, 16>(paged_attn_kernel<D, TQ, TKV, 1>, a, p, s);
+  }
 }
 template <class TQ, class TKV>
 hipError_t launch(const PagedAttn &a, const Plan &p, hipStream_t s) {

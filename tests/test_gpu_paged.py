@@ -235,6 +235,28 @@ def test_attention_odd_values_stay_where_they_are_seen(ops, types, value, window
     assert fin[25, 2:].all() == (window > 0)
 
 
+@pytest.mark.parametrize("types", [(F32, BF16), (F32, F32), (BF16, BF16), (F16, F16)])
+@pytest.mark.parametrize("value", [NAN, INF, -INF])
+@pytest.mark.parametrize("d,window", [(64, 0), (128, 0), (64, 70), (128, 70)])
+def test_attention_odd_values_in_long_prompts(ops, types, value, d, window):
+    """The same where blocks of many query rows share tiles, in every quarter of a tile, seen by all rows of a block or by some."""
+    say(f"[gpu] paged attention odd values of prompts {types} {value} d={d} window={window}")
+    s = Seqs(ops, types, [210, 150], [170, 150], 4, 2, d, 16, window, 5, seed=7)
+    rows = (2, 41, 57, 70, 84, 99, 111, 130, 200)  # (values of a head each, one element each)
+    for i, row in enumerate(rows):
+        s.cache.v[s.map[0][row // 16], i % 2, row % 16, 3 * i] = value
+        s.rows[0][2][i % 2, row, 3 * i] = value
+    s.cache.k[s.map[1][90 // 16], 1, 90 % 16, 3] = value
+    s.rows[1][0][1, 90, 3] = value
+    ref, tol = s.ref()
+    got = s.run(ops)
+    assert torch.equal(torch.isnan(got), torch.isnan(ref)) and torch.equal(torch.isinf(got), torch.isinf(ref))
+    fin = torch.isfinite(ref)
+    assert torch.equal(got[~fin & ~torch.isnan(ref)].double(), ref[~fin & ~torch.isnan(ref)])
+    assert ((got.double() - ref).abs()[fin] <= tol[fin]).all()
+    assert not fin[100, :2, 0].all() and fin[:170, :, 60:].all()
+
+
 @pytest.mark.parametrize("types", TYPES)
 def test_attention_odd_calls(ops, types):
     """Lengths out of range, more tokens than rows, pages that do not exist, tokens of no sequence."""
@@ -285,8 +307,8 @@ def test_attention_strides(ops, types):
         x = torch.empty((n, size, 2, hk, d), dtype=types[1], device="cuda").permute(2, 0, 3, 1, 4)
         return ops.PagedCache(x[0], x[1])
 
-    for d in (64, 128):
-        s = Seqs(ops, types, [100, 33, 260], [5, 1, 18], 6, 2, d, 16, seed=5, layout=layout)
+    for d, news in ((64, [5, 1, 18]), (128, [5, 1, 18]), (64, [70, 33, 60]), (128, [70, 33, 60])):
+        s = Seqs(ops, types, [100, 33, 260], news, 6, 2, d, 16, seed=5, layout=layout)
         wide = torch.zeros((s.q.shape[0], 10, d), dtype=s.q_type, device="cuda")
         wide[:, 1:7] = s.q
         s.q = wide[:, 1:7]
@@ -342,7 +364,7 @@ def test_attention_graphs_and_streams(ops, types, lens, news):
             assert torch.equal(out, want)
 
 
-@pytest.mark.parametrize("types", [(BF16, BF16), (F16, F16), (F32, BF16), (BF16, 4)])
+@pytest.mark.parametrize("types", [(BF16, BF16), (F16, F16), (F32, BF16), (F32, F32), (BF16, 4), (F16, 4), (F32, 4)])
 def test_attention_of_long_prompts(ops, types):
     """Pieces of prompts of many tiles beside single tokens, against a whole product in float64."""
     say(f"[gpu] paged attention prompts {types}")
@@ -351,7 +373,7 @@ def test_attention_of_long_prompts(ops, types):
         g = gen(9)
         page, q_type, kv = 64, *types
         wide = 24
-        cache = ops.paged_cache(5 * wide, hk, page, d, BF16 if kv == 4 else kv, bits=4 if kv == 4 else 16)
+        cache = ops.paged_cache(5 * wide, hk, page, d, BF16 if kv == 4 else kv, bits=4 if kv == 4 else 32 if kv == F32 else 16)
         table = torch.randperm(5 * wide, generator=torch.Generator().manual_seed(1)).int().view(5, wide).cuda()
         rows = []
         for which in range(2):
