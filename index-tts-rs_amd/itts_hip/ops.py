@@ -77,9 +77,9 @@ def _tensor(t, name: str, dims: int, device=None, dtype=None, last=False):
             _refuse(f"{name}: a GPU tensor is needed, got one on {t.device}")
         if device is not None:
             _refuse(f"{name}: on {t.device}, the other tensors on cuda:{device}")
-    if t.requires_grad and torch.is_grad_enabled():
-        _refuse(f"{name}: requires a gradient, which this operator does not give")
     if dtype is not torch.int32:  # (what its memory does not show)
+        if t.requires_grad and torch.is_grad_enabled():
+            _refuse(f"{name}: requires a gradient, which this operator does not give")
         if t.is_neg():
             _refuse(f"{name}: is negated when it is read, its memory is not what it says (resolve_neg() gives one that is)")
         if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
@@ -93,6 +93,7 @@ def _tensor(t, name: str, dims: int, device=None, dtype=None, last=False):
 # Host time is most of a small call.  The current stream's handle without a Stream object around it saves
 # 2 us, a new tensor without torch.empty's reading of its arguments 0.5 to 0.9 (of 1.3 to 1.6).
 _stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 try:
     from torch._C._dynamo.guards import _empty_strided_cuda as _empty
 except ImportError:
@@ -127,7 +128,7 @@ def _on_device(op):
         if isinstance(t, PagedCache):
             t = t.k
         try:
-            if isinstance(t, torch.Tensor) and t.is_cuda and t.device.index != torch.cuda.current_device():
+            if isinstance(t, torch.Tensor) and t.is_cuda and t.get_device() != _current_device():
                 with torch.cuda.device(t.device):
                     return op(*args, **kwargs)
             return op(*args, **kwargs)
