@@ -1084,12 +1084,15 @@ __global__ __launch_bounds__(256, (TQ::kBytes == 4 ? (D == 64 ? 2 : 1) : D == 64
       weigh(0, ms);
       add(1, waiting);
       __builtin_amdgcn_sched_barrier(0);
+      // (whoever is in this half goes first: two waves of a SIMD then leave each other the vector unit and the matrix unit in turn)
+      __builtin_amdgcn_s_setprio(1);
       scores(s[0], k);
       read_keys(k, 1, keys);
       weigh(1, ms);
       add(0, values);
       __builtin_amdgcn_sched_barrier(0);
       scores(s[1], k);
+      __builtin_amdgcn_s_setprio(0);
       ring = ring1;
       copies_wait<0>();
       __syncthreads();
