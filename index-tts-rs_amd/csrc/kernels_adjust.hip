@@ -40,12 +40,6 @@ struct __attribute__((packed, aligned(alignof(E)))) Run {
   E v[kPer];
 };
 
-// x / r from inv = 1 / r: one step of refinement rounds it as the division would (the plain product where that is no number).
-__device__ __forceinline__ float divide(float x, float r, float inv) {
-  const float q = x * inv, y = __builtin_fmaf(__builtin_fmaf(-q, r, x), inv, q);
-  return fabsf(y) < INFINITY ? y : q;
-}
-
 // 8 x THREADS x RUNS tokens a block.  Every block goes through the row's whole lists, so pieces are large: 256 bf16 rows of 60,510
 // under a mask, a history of 2,000 and 50 biases, a call: blocks of 4,096 tokens 29.3 us, 8,192 25.9, 16,384 20 (66 MB; without
 // lists 13).
@@ -139,7 +133,6 @@ __global__ __launch_bounds__(kThreads) void adjust_kernel(AdjustLogits a, int pi
     });
     __syncthreads();
   }
-  const float inv = 1.0f / r;
   auto again = [&](int, const uint32_t (&t)[kAhead]) {
     // (step by step for all entries of the turn: their loads are on their way together)
     uint32_t w[kAhead];
@@ -162,7 +155,7 @@ __global__ __launch_bounds__(kThreads) void adjust_kernel(AdjustLogits a, int pi
       if (w[k] == 0) continue;
       const uint32_t c = w[k] & 0xffffu;
       float y1 = Elem<TYPE>::get(v[k]);
-      if (c > 0) y1 = (y1 < 0.0f ? y1 * r : divide(y1, r, inv)) - __builtin_fmaf(f, (float)c, p);
+      if (c > 0) y1 = (y1 < 0.0f ? y1 * r : y1 / r) - __builtin_fmaf(f, (float)c, p);
       if (w[k] >> 16) y1 += bias[k];
       y[first + t[k]] = Elem<TYPE>::put(y1);
     }

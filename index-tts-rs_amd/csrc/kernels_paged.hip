@@ -53,12 +53,15 @@ struct Tiles {
 // nothing is left for this one).  Every share has the same size, the smallest one with which `blocks` are enough.  Found by
 // every wave from the starts and lengths, a lane a sequence.  A sequence's last tokens, which see most, come first.
 struct Share {
-  int b, tile, n, first, end, from;
+  int b, tile, n, first, end;
 };
 template <int ROWS, int KT>
-__device__ __forceinline__ Share share_of(const Args &p, int index) {
+__device__ __forceinline__ Share share_of(const Args &p, int index, int hk) {
   const PagedAttn &a = p.a;
   const int lane = threadIdx.x & 63;
+  // (the first block of all says for every sequence where its shares are; where starts fall and sequences have more rows than
+  // there are tokens, those that have no blocks any more are left out)
+  const bool tells = p.parts > 0 && index == 0 && hk == 0;
   // row tiles of a sequence, and the units of keys that one of them sees at most
   auto count = [&](int b, int &tiles, int &units) {
     tiles = 0, units = 0;
@@ -95,29 +98,29 @@ __device__ __forceinline__ Share share_of(const Args &p, int index) {
     }
     size = __builtin_amdgcn_readfirstlane(size);
   }
-  Share share{0, 0, 0, 0, 0, 0};
+  Share share{0, 0, 0, 0, 0};
   int before = 0;
-  for (int b0 = 0; b0 < a.batch && share.n == 0; b0 += 64) {
+  for (int b0 = 0; b0 < a.batch && (share.n == 0 || tells); b0 += 64) {
     int tiles, units;
     count(b0 + lane, tiles, units);
     const int each = (int)(((int64_t)units + size - 1) / size), own = tiles * each;
-    int to = own;
+    int to = own;  // (counted to one more than there are blocks)
 #pragma unroll
     for (int step = 1; step < 64; step *= 2) {
       const int up = __shfl_up(to, step, 64);
-      if (lane >= step) to += up;
+      if (lane >= step) to = min(to + up, p.blocks + 1);
     }
-    if (const uint64_t at = __ballot(index >= before + to - own && index < before + to); at != 0) {
-      const int src = __builtin_ctzll(at);
+    if (tells && b0 + lane < a.batch) p.dealt[b0 + lane] = before + to <= p.parts ? make_int2(before + to - own, each) : make_int2(0, 0);
+    if (const uint64_t at = __ballot(index < before + to); at != 0 && share.n == 0) {
+      const int src = __builtin_ctzll(at), from = before + (src > 0 ? __builtin_amdgcn_readlane(to, src - 1) : 0);
       share.b = b0 + src, share.n = __builtin_amdgcn_readlane(each, src);
-      share.from = before + __builtin_amdgcn_readlane(to, src) - __builtin_amdgcn_readlane(own, src);
-      const int local = index - share.from, tile = local / share.n;
+      const int local = index - from, tile = local / share.n;
       share.tile = __builtin_amdgcn_readlane(tiles, src) - 1 - tile;
       const int part = local - tile * share.n;
       share.first = share.n == 1 ? 0 : part * size << p.unit;
       share.end = share.n == 1 ? 1 << 30 : share.first + (size << p.unit);
     }
-    before += __builtin_amdgcn_readlane(to, 63);
+    before = min(before + __builtin_amdgcn_readlane(to, 63), p.blocks + 1);
   }
   return share;
 }
@@ -524,9 +527,8 @@ __global__ __launch_bounds__(256, (D == 128 && TKV::kBytes == 4 ? 1 : 2)) void p
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
   const int hk = blockIdx.x % a.pages.Hk, index = blockIdx.x / a.pages.Hk;
   const int2 rest = rest_of(a);
-  const Share share = share_of<kRows, kTileKeys>(p, index);
+  const Share share = share_of<kRows, kTileKeys>(p, index, hk);
   if (share.n == 0) return clear_rest<D, TQ>(a, rest);
-  if (p.parts > 0 && index == share.from && hk == 0 && threadIdx.x == 0) p.dealt[share.b] = make_int2(share.from, share.n);
   const Seq seq = seq_of<kRows>(p, share);
   const Tiles<kTileKeys> tiles(a, seq.p0, seq.p1);
   const int first = min(share.first, tiles.n), end = min(share.end, tiles.n);
@@ -658,9 +660,8 @@ __global__ __launch_bounds__(256, (RT == 2 ? 2 : kCodeBlocks<D, TQ>)) void paged
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
   const int hk = blockIdx.x % pg.Hk, index = blockIdx.x / pg.Hk;
   const int2 rest = rest_of(a);
-  const Share share = share_of<kRows, kTileKeys>(p, index);
+  const Share share = share_of<kRows, kTileKeys>(p, index, hk);
   if (share.n == 0) return clear_rest<D, TQ>(a, rest);
-  if (p.parts > 0 && index == share.from && hk == 0 && threadIdx.x == 0) p.dealt[share.b] = make_int2(share.from, share.n);
   const Seq seq = seq_of<kRows>(p, share);
   const Tiles<kTileKeys> tiles(a, seq.p0, seq.p1);
   const int first = min(share.first, tiles.n), end = min(share.end, tiles.n);
@@ -875,9 +876,8 @@ __global__ __launch_bounds__(256, (TQ::kBytes == 4 ? (D == 64 ? 2 : 1) : D == 64
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 31, h = lane >> 5;
   const int hk = blockIdx.x % a.pages.Hk, index = blockIdx.x / a.pages.Hk;
   const int2 rest = rest_of(a);
-  const Share share = share_of<kLongRows, KT>(p, index);
+  const Share share = share_of<kLongRows, KT>(p, index, hk);
   if (share.n == 0) return clear_rest<D, TQ>(a, rest);
-  if (p.parts > 0 && index == share.from && hk == 0 && threadIdx.x == 0) p.dealt[share.b] = make_int2(share.from, share.n);
   const Seq seq = seq_of<kLongRows>(p, share);
   const Tiles<KT> tiles(a, seq.p0, seq.p1);
   const int first = min(share.first, tiles.n), end = min(share.end, tiles.n);
@@ -1133,7 +1133,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(Args p) {
   if (token < span.first || token >= span.first + span.n) return;
   const int2 dealt = p.dealt[b];
   const int S = dealt.y;
-  if (S == 1) return;  // (that block has written the row)
+  if (S <= 1) return;  // (that block has written the row; 0: a sequence that was left out)
   const int r = (token - span.first) * p.group + head - hk * p.group, tile = r / ROWS, tiles = (span.n * p.group + ROWS - 1) / ROWS;
   const int index = dealt.x + (tiles - 1 - tile) * S;
   const size_t at = ((size_t)hk * p.parts + index) * ROWS + (r - tile * ROWS);

@@ -410,6 +410,49 @@ def test_attention_of_long_prompts(ops, types):
                 check(got[starts[b]:starts[b + 1], head], ref, tol + 1e-30, f"d={d} sequence {b} head {head}")
 
 
+@pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_of_many_rows_at_the_ends(ops, types, d):
+    """More tokens than rows, empty and bad sequences, missing pages and tokens of no sequence among blocks of many rows; more than
+    64 sequences."""
+    say(f"[gpu] paged attention many rows at the ends {types} d={d}")
+    s = Seqs(ops, types, [150, 0, 3, 170, 90, 200], [150, 0, 170, 100, 90, 130], 8, 2, d, 16, seed=11)
+    s.table[3, 6] = 10 ** 6    # rows 96 .. 111 of sequence 3, seen from its 27th token on
+    lens = s.lengths.clone()
+    lens[4] = -7
+    ref, tol = s.ref()
+    at = s.starts_list
+    got = ops.paged_attention(s.q, s.cache, s.starts, lens, s.table)
+    for b in (0, 2, 5):
+        check(got[at[b]:at[b + 1]], ref[at[b]:at[b + 1]], tol[at[b]:at[b + 1]], f"sequence {b}")
+    assert (got[at[2]:at[2] + 167] == 0).all()
+    check(got[at[3]:at[3] + 26], ref[at[3]:at[3] + 26], tol[at[3]:at[3] + 26])
+    assert torch.isnan(got[at[3] + 26:at[4]]).all() and torch.isnan(got[at[4]:at[5]]).all()
+    starts = s.starts.clone()
+    starts[0], starts[6] = 4, at[6] - 9
+    out = torch.full_like(s.q, 5.0)
+    ops.paged_attention(s.q, s.cache, starts, lens, s.table, out=out)
+    assert (out[:4] == 0).all() and (out[at[6] - 9:] == 0).all()
+    lens, news = [60 + 7 * (i % 9) for i in range(70)], [30 + i % 20 for i in range(70)]
+    s = Seqs(ops, types, lens, news, 8, 2, d, 16, seed=12)
+    check(s.run(ops), *s.ref())
+
+
+@pytest.mark.parametrize("types", [(BF16, BF16), (F32, F32), (F16, 4)])
+@pytest.mark.parametrize("tokens", [3, 90])
+def test_attention_of_starts_that_fall(ops, types, tokens):
+    """Starts that name the same tokens again and again give more rows than there are tokens: nothing leaves its memory, and a call
+    with good ones after it is what it was (long sequences, so that blocks share them)."""
+    say(f"[gpu] paged attention falling starts {types} {tokens}")
+    s = Seqs(ops, types, [3000] * 40, [tokens] + [0] * 39, 4, 2, 64, 16, seed=13)
+    first = s.run(ops)
+    starts = ints([0, tokens] * 20 + [0])
+    for over in ({}, dict(max_length=100)):
+        assert ops.paged_attention(s.q, s.cache, starts, s.lengths, s.table, **over).shape == s.q.shape
+    assert torch.equal(first, s.run(ops))
+    check(first, *s.ref())
+
+
 def test_attention_refuses(ops):
     s = Seqs(ops, (F32, BF16), [20], [1], 4, 2, 64)
     for over, match in ((dict(window=-1), "window"), (dict(max_length=33), "max_length"), (dict(scale=NAN), "scale"),
@@ -528,6 +571,32 @@ def test_append_codes_at_borders(ops):
     k, _ = ops.paged_gather(cache, ints([8]), ints([[0]]), 8)
     assert torch.isnan(k[0, 0, 4:7]).all() and torch.isfinite(k[0, 0, [0, 1, 2, 3, 7]]).all()
     assert torch.equal(k[0, 0, 0].double(), (x[0, 0].double()).round()) and (k[0, 0, 1] == 3.25).all()
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_append_into_rows_of_all_heads(ops, bits):
+    """Pages whose rows hold all heads, keys beside values, as one tensor; several sequences, a table inside a larger one."""
+    say(f"[gpu] paged append strides {bits}")
+    g, d, hk = gen(14), 128, 3
+    k, v = (randn(g, 40, hk, d, dtype=BF16) for _ in range(2))
+    wide = torch.full((3, 9), -1, dtype=torch.int32, device="cuda")
+    wide[:, 2:4] = ints([[4, 0], [2, 5], [1, 3]])
+    starts, lens = ints([0, 17, 17, 40]), ints([3, 5, 0])
+    plain = ops.paged_cache(6, hk, 16, d, BF16, bits=bits)
+    if bits == 4:
+        x, p = torch.zeros((6, 16, 2, hk, d // 2), dtype=torch.uint8, device="cuda"), torch.zeros((6, 16, 2, hk, d // 64, 2), dtype=F16, device="cuda")
+        y, z = x.permute(2, 0, 3, 1, 4), p.permute(2, 0, 3, 1, 4, 5)
+        other = ops.PagedCache(y[0], y[1], z[0], z[1])
+    else:
+        y = torch.zeros((6, 16, 2, hk, d), dtype=BF16, device="cuda").permute(2, 0, 3, 1, 4)
+        other = ops.PagedCache(y[0], y[1])
+    for c in (plain, other):
+        for t in c:
+            if t is not None:
+                t.zero_()
+        assert ops.paged_append(c, k, v, starts, lens, wide[:, 2:4]).lengths.tolist() == [20, 5, 23]
+    for a, b in zip(plain, other):
+        assert a is None and b is None or torch.equal(a, b)
 
 
 def test_append_pairs_round_twice(ops):
