@@ -515,8 +515,14 @@ __device__ __forceinline__ void join_waves(const Args &p, const Share &share, co
   }
 }
 
-// Few query rows: 4 waves over tiles of keys of their own, straight from memory into registers, one tile ahead; joined at
-// the end.
+// Few query rows (many over fp32 caches): 4 waves over tiles of keys of their own, straight from memory into registers, one tile
+// ahead; joined at the end.  Decode steps are bound by memory: 64 tokens, 8 key heads of 128, 501 .. 6,001 bf16 rows in pages of 16,
+// 853 MB, 164 us (5.2 TB/s); 24 sequences of up to 3 tokens, 16 heads of 64, a window of 4,000 fp16 rows, 394 MB, 75 us.  Short
+// ones by the chain from load to result: one token, 20 heads, 235 rows 7.6 us.  Many rows over fp32 caches by the fp32 matrix
+// instructions: 4 x 547 tokens, a window of 256 rows and 232 first ones 70 us, 39 of them those instructions' time at full rate;
+// keys and values cut into three bf16 planes in LDS for 128 rows at a time (six products of bf16 for one) took as long: the cutting and
+// the chain of one tile's steps cost what the matrix units saved.  Two row tiles a wave there: 124 -> 121 us for 4 x 547 tokens over
+// 1,200 rows.
 template <int D, class TQ, class TKV, int RT>
 __global__ __launch_bounds__(256, (D == 128 && TKV::kBytes == 4 ? 1 : 2)) void paged_attn_kernel(Args p) {
   constexpr int WK = 4, kRows = 16 * RT;
@@ -642,7 +648,10 @@ __device__ __forceinline__ uint32_t lds_address(const void *p) {
 
 // Few query rows (or many) over 4 bits: 4 waves over tiles of 32 keys of their own, each with a ring of tiles in LDS that direct
 // loads fill: few instructions for many small rows, no registers for what is on its way, and the operands' order comes from
-// how LDS is read.  Row r of 16 lies in slot 4 (r % 4) + r / 4, its 16-byte pieces in another order by row (piece ^ r % 4, of two
+// how LDS is read.  Bound by instructions: 16 tokens, 8 key heads of 128, 8,191 .. 32,768 rows, 378 MB, 86 us (4.4 TB/s), about 400
+// vector and 180 scalar instructions a tile and wave, the vector units busy 58% of the time.  Straight into registers, 36 loads a
+// tile, 125 us for the call that takes 91 now.  Three blocks a compute unit with two tiles each 99 us, two with four tiles 112 (16-bit
+// queries, D 128).  Two row tiles of 16 for prompts: 4,096 tokens 484 -> 400 us (343 TFLOP/s).  Row r of 16 lies in slot 4 (r % 4) + r / 4, its 16-byte pieces in another order by row (piece ^ r % 4, of two
 // pieces piece ^ r / 2 % 2): reads of 16 key rows' same piece and of four value rows' same part fall on different banks.
 template <int D, class TQ>
 constexpr int kCodeBlocks = D == 64 ? (TQ::kBytes == 4 ? 3 : 4) : TQ::kBytes == 4 ? 2 : 3;  // a compute unit
@@ -865,6 +874,12 @@ __device__ __forceinline__ bool any_in_block(bool v, void *mem) {
 // loads, a tile ahead of their use (keys two: a tile's scores are formed while the exponentials of the one before are).
 // S^T = K Q^T by 32 x 32 products: lane (c, h) holds keys 8 (i / 4) + 4 h + i % 4 of query c in register i, the B operand of
 // O^T = V^T P^T in the order in which the transposing LDS load gives V's rows.
+// One prompt of 8,192 tokens, 32 heads of 128 over 8 key heads, bf16: 777 us, 707 TFLOP/s (818 us without the waves' priorities); the
+// matrix units are busy 58% of its cycles (a probability's second plane is a third of their work), the vector units 51%, at
+// 1.74 GHz (the card lowers its clock under this load).  On the way there: 16 x 16 tiles copied through registers 1,380 us;
+// 32 x 32 with both kinds of tiles in one loop 1,083 (accumulators copied every turn, queries spilled); a loop of its own for tiles
+// that all see 828; probabilities of a tile's second half left waiting for the next tile's first exponentials 820; keys read
+// ahead of their products 796.
 template <int D, class TQ, class TKV>
 __global__ __launch_bounds__(256, (TQ::kBytes == 4 ? (D == 64 ? 2 : 1) : D == 64 ? 3 : 2)) void paged_rows_kernel(Args p) {
   constexpr int KT = kLongKeys, kPieces = D * TKV::kBytes / 16, kTile = KT * kPieces, kCopies = kTile / 256;
@@ -1118,7 +1133,7 @@ __global__ __launch_bounds__(256, (TQ::kBytes == 4 ? (D == 64 ? 2 : 1) : D == 64
 }
 
 // Joins the shares' results of a row: a wave a row, D / 4 lanes with four elements each for every fourth (D 128: second)
-// share, added in their order there and then over the lane groups.
+// share, added in their order there and then over the lane groups.  4 to 5 us, most of them the launch.
 template <int D, class TQ, int ROWS>
 __global__ __launch_bounds__(256) void paged_join_kernel(Args p) {
   constexpr int kLanes = D / 4, kGroups = 64 / kLanes;
@@ -1198,7 +1213,17 @@ Plan make_plan(const PagedAttn &a, int n_cu) {
   p.parts = 0, p.blocks = (int)most;
   const int at_once = n_cu * (codes && !p.many && p.RT == 1 ? code_blocks(D, a.type) : 2) / a.pages.Hk;
   const int64_t seen = a.window > 0 ? std::min<int64_t>(a.max_rows, (int64_t)a.window + std::min(a.sinks, a.max_rows)) : a.max_rows;
-  if (most < at_once && seen > (a.pages.type == kOpF32 ? 512 : 1024)) p.parts = p.blocks = std::max(at_once, (int)most);
+  // Keys are shared where row tiles alone would not fill the card and rows may be enough for the second launch to pay: a wave's
+  // time goes by their bytes, over 4 bits by their number.  One token, us a call, alone and shared: 20 bf16 heads of 64 over
+  // 1,734 rows 15.4, 18.6, 2,000 rows 17.4, 16.0, 3,200 rows 22.1, 16.2; 8 of 128 over 1,100 rows 16.5, 16.2, 2,800 rows 30.3, 16.3;
+  // 20 fp32 heads of 64 over 850 rows 15.4, 16.3, 1,100 rows 17.7, 16.7; 4 bits, 16 of 64 over 1,100 rows 16.6, 17.5, 1,600 rows
+  // 20.9, 17.9; 8 of 128 over 1,100 rows 18.4, 18.0, 3,000 rows 38.1, 18.4.  Shared tiles of 64 keys pay where a block loses more
+  // than ten of them, one of two on a compute unit being slower by 1.6: 128 of 1,100 rows, 20 heads of 64, 30.5, 19.7; 512 of them
+  // 31.3, 29.3; 1,100 of them 30.0, 37.1; 1,536 of 4,000 88.6, 80.7; 32 heads of 128 over 8, 512 of 2,000 62.3, 46.7; 1,024 of
+  // them 64.9, 66.7; 1,024 of 6,000 173, 146.
+  const bool far = p.many ? seen / 64 * (5 * at_once - 8 * most) > (int64_t)50 * at_once
+                   : codes ? seen > 1152 : seen * D * (a.pages.type == kOpF32 ? 4 : 2) > (224 << 10);
+  if (most < at_once && far) p.parts = p.blocks = std::max(at_once, (int)most);
   return p;
 }
 

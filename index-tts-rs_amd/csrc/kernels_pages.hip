@@ -5,8 +5,12 @@
 //   (a, b) -> (a cos t - b sin t, b cos t + a sin t),
 // the cosines and sines from a table.  A cache of 4 bits takes every 64 elements x as
 //   base = min x, scale = (max x - min x) / 15 (to fp32 and to fp16), code = rint((x - base) / scale) in 0 .. 15 (scale 0: 0),
-// the quantiser of the decoder's weights.  Rotation and quantiser work in 64 bits, which run at the rate of 32 here and hide
-// behind memory: codes are those of the definition, also where a value lies next to the border of two.
+// the quantiser of the decoder's weights.  Rotation and quantiser work in 64 bits, which run at the rate of 32 here:
+// codes are those of the definition, also where a value lies next to the border of two.
+// 7,428 tokens, 32 heads and 8 key heads of 128, all turned: into bf16 33 us (184 MB, 5.5 TB/s: memory), into 4 bits 49 us (169 MB):
+// 1,180 vector instructions a wave of three pieces, half of the time, beside memory.
+//
+// Gather.  A copy: 147 MB of bf16 rows 21 us, 84 MB of 4 bits and the values they stand for 17 us.
 #include <algorithm>
 #include <type_traits>
 

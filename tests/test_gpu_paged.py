@@ -201,6 +201,22 @@ def test_attention_split_over_keys(ops, types, lens, news, h, hk, d, window, sin
     check(s.run(ops, max_length=max(lens)), ref, tol)
 
 
+@pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("d,window,sinks", [(64, 0, 0), (128, 0, 0), (64, 1500, 70), (128, 1500, 0)])
+def test_attention_of_many_rows_split_over_keys(ops, types, d, window, sinks):
+    """Pieces of prompts whose keys blocks share, beside one that sees few rows, one without tokens and a bad length."""
+    say(f"[gpu] paged attention split of many rows {types} d={d} window={window}")
+    s = Seqs(ops, types, [2600, 150, 40, 2000, 300], [140, 150, 0, 130, 20], 8, 2, d, 16, window, sinks, seed=21)
+    ref, tol = s.ref()
+    check(s.run(ops), ref, tol)
+    lens = s.lengths.clone()
+    lens[3] = -1
+    got = ops.paged_attention(s.q, s.cache, s.starts, lens, s.table, window=window, sinks=sinks)
+    assert torch.isnan(got[290:420]).all()
+    check(got[:290], ref[:290], tol[:290])
+    check(got[420:], ref[420:], tol[420:])
+
+
 @pytest.mark.parametrize("types", [(F32, BF16), (BF16, BF16), (F16, 4)])
 @pytest.mark.parametrize("batch", [65, 300])
 def test_attention_many_sequences(ops, types, batch):
