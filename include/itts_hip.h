@@ -432,7 +432,8 @@ itts_status itts_cache_keep(const itts_cache_keep_args *args, void *stream);
  * dtype F32, BF16, F16, or I4: rows are then head_dim / 2 bytes (strides in bytes), two codes each, the lower half first, and
  * k_params and v_params hold (scale, base) pairs of float16 for every 64 elements, [n_pages][n_kv_head][page_size]
  * [head_dim / 64][2] (the last two dimensions contiguous; strides in float16): value = scale * code + base.  Rows start at
- * multiples of 16 bytes, pairs at multiples of 4 * (head_dim / 64).
+ * multiples of 16 bytes, pairs at multiples of 4 * (head_dim / 64); pages are less than 2^32 bytes
+ * apart, rows at most 2^26.
  *
  * Tokens of a batch stand one sequence after the other, those of sequence b from starts[b] to starts[b + 1] - 1 (starts
  * [batch + 1], rising, equal for a sequence without any).  A sequence whose starts fall or leave the n_tokens has none. */

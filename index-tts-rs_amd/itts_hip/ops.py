@@ -288,7 +288,7 @@ class PagedCache(NamedTuple):
     or float16; or uint8 [pages][key heads][page size][dim / 2], 4 bits: two codes a byte, the lower half first, and
     k_params, v_params float16 [pages][key heads][page size][dim / 64][2] with the (scale, base) of every 64 elements, a value
     being scale * code + base.  dim 64 or 128, page sizes multiples of 16; any strides whose rows start at multiples of 16
-    bytes (pairs: dim / 16)."""
+    bytes (pairs: dim / 16), pages less than 2^32 bytes apart, rows at most 2^26."""
     k: torch.Tensor
     v: torch.Tensor
     k_params: Optional[torch.Tensor] = None

@@ -67,7 +67,8 @@ SHARED = [("batch", dict(batch=-1)), ("batch", dict(batch=65536)), ("table", dic
           ("pages.page_size", dict(pages_page_size=24)), ("pages.page_size", dict(pages_page_size=65552)),
           ("pages.n_pages", dict(pages_n_pages=0)), ("pages: k", dict(pages_k=None)), ("pages.k", dict(pages_k=P + 8)),
           ("pages.k", dict(pages_k_row=60)), ("pages.v", dict(pages_v_head=-2048)), ("pages.v", dict(pages_v=9 * P + 4)),
-          ("pages.k_row", dict(pages_k_row=1 << 27)), ("pages: k", dict(pages_dtype=H.ITTS_I4)),
+          ("pages.k_row", dict(pages_k_row=1 << 27)), ("pages.k_page", dict(pages_k_page=1 << 31)),
+          ("pages.k_page", dict(pages_v_page=1 << 31)), ("pages: k", dict(pages_dtype=H.ITTS_I4)),
           ("pages.k_params", dict({"pages_" + k: v for k, v in CODES.items()}, pages_k_params=17 * P + 2)),
           ("pages.k_params", dict({"pages_" + k: v for k, v in CODES.items()}, pages_v_params_row=3)),
           ("pages.k", dict({"pages_" + k: v for k, v in CODES.items()}, pages_k_row=24))]
