@@ -26,13 +26,17 @@ struct I4 {};
 struct Args {
   PagedAttn a;
   int blocks, parts, group;
-  uint32_t group_mul;  // 2^32 / group, rounded up: exact for rows < 2^32 / group
+  uint32_t group_mul;  // 2^32 / group, rounded up: one too many at most
   uint64_t page_mul;
   bool even;           // pages of multiples of 32 rows
   int unit, least;     // a share is at least `least` times 2^unit tiles of keys
   float2 *ml;
   int2 *dealt;
-  __device__ int token(int row) const { return group == 1 ? row : __umulhi((uint32_t)row, group_mul); }
+  __device__ int token(int row) const {
+    if (group == 1) return row;
+    const int i = __umulhi((uint32_t)row, group_mul);
+    return i * group > row ? i - 1 : i;
+  }
 };
 
 // The tiles of KT keys that the tokens at positions p0 .. p1 of a sequence see, counted through: those with rows < S,

@@ -469,6 +469,34 @@ def test_attention_of_starts_that_fall(ops, types, tokens):
     check(first, *s.ref())
 
 
+@pytest.mark.parametrize("kv", [BF16, 4])
+def test_attention_of_more_rows_than_a_quotient_holds(ops, kv):
+    """320,000 tokens of 127 heads, each of which sees its own row alone: results are the values.  (2^32 / 127, rounded up, gives a
+    token too many from row 2^32 / 111 on.)"""
+    say(f"[gpu] paged attention 320,000 tokens of 127 heads {kv}")
+    n, group, d = 320_000, 127, 64
+    cache = ops.paged_cache(n // 64, 1, 64, d, BF16, bits=4 if kv == 4 else 16)
+    for t in cache[:2]:
+        t.zero_() if t.is_floating_point() else t.random_(0, 256)
+    if kv == 4:
+        cache.k_params.zero_()
+        cache.v_params[..., 0], cache.v_params[..., 1] = 0.125, -1.0  # (values in eighths, exact in 16 bits)
+        # 4 bits: a value is the difference of scale (16 + code) p / l, at most 4, and (16 scale - base) p / l = 3, where p and l are fp32
+        # numbers with a rounding each and the sums and products round four times more: 8 steps of 2^-24 of 7 in all
+        tol = 8 * 2.0 ** -24 * 7
+        want = values(cache.v, cache.v_params)[:, 0].flatten(0, 1).to(BF16)
+    else:
+        cache.v.copy_(randn(gen(3), *cache.v.shape))
+        want = cache.v[:, 0].flatten(0, 1)
+    table = torch.arange(n // 64, dtype=torch.int32, device="cuda").unsqueeze(0)
+    q = torch.zeros((n, group, d), dtype=BF16, device="cuda")
+    got = ops.paged_attention(q, cache, ints([0, n]), ints([n]), table, window=1)
+    del q
+    for at in range(0, n, 20_000):
+        off = (got[at:at + 20_000].float() - want[at:at + 20_000].unsqueeze(1).float()).abs()
+        assert off.max() <= (tol + HALF[BF16] * want.abs().max() if kv == 4 else 0.0)
+
+
 def test_attention_refuses(ops):
     s = Seqs(ops, (F32, BF16), [20], [1], 4, 2, 64)
     for over, match in ((dict(window=-1), "window"), (dict(max_length=33), "max_length"), (dict(scale=NAN), "scale"),
