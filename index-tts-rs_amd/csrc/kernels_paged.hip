@@ -239,14 +239,17 @@ struct CodeRegs {
   uint32_t k[2][G][2], v[8][G], kp[8][G], vp[8][G];
 };
 
-// Of a dword with four codes in each half, codes d as bf16 pairs 1 + code / 16: one shift and one mask, the bits above are
+// Of a dword with four codes in each half, codes d as 16-bit pairs 1 + code / 16: one shift and one mask, the bits above are
 // the exponent of 1.  Sums of such products minus the sum of the other operand are 1/16 of those of the codes.
+template <class T>
 struct CodeBits {
+  static constexpr int kAt = std::is_same_v<T, Bf16> ? 3 : 6;  // the highest bits of a fraction of 7 or 10
   // (in registers of their own: one instruction takes both)
-  uint32_t mask = 0x00780078u, one = 0x3f803f80u;
+  uint32_t mask = 0x000f000fu << kAt, one = std::is_same_v<T, Bf16> ? 0x3f803f80u : 0x3c003c00u;
   __device__ __forceinline__ CodeBits() { asm volatile("" : "+s"(mask), "+v"(one)); }
   __device__ __forceinline__ void pairs(uint32_t w, uint32_t (&o)[4]) const {
-    o[0] = (w << 3 & mask) | one, o[1] = (w >> 1 & mask) | one, o[2] = (w >> 5 & mask) | one, o[3] = (w >> 9 & mask) | one;
+#pragma unroll
+    for (int d = 0; d < 4; d++) o[d] = ((4 * d < kAt ? w << (kAt - 4 * d) : w >> (4 * d - kAt)) & mask) | one;
   }
 };
 __device__ __forceinline__ float low_half(uint32_t w) { return (float)__builtin_bit_cast(f16x2v, w)[0]; }
@@ -255,11 +258,12 @@ __device__ __forceinline__ float high_half(uint32_t w) { return (float)__builtin
 // Rows (attn_tiles.h) over 4 bits.  With key t's codes c, scale s and base b in each group of 64 elements,
 //   q . k_t = sum_groups s sum_e q_e c_e + b sum_e q_e,
 // so the products run on codes, exact in 16 bits, and the pairs come in by two multiply-adds a score and group.  In the second
-// product the scale goes with the probability, and sum_t p_t b_t is one number a row and group.  Everything in bf16, whose
+// product the scale goes with the probability, and sum_t p_t b_t is one number a row and group: in bf16, whose
 // range holds a probability times any scale.
 template <int D, class TQ, int RT>
 struct Rows4 {
-  static constexpr int G = D / 64, NQ = TQ::kBytes == 4 ? 3 : std::is_same_v<TQ, Bf16> ? 1 : 2, NP = kProbPlanes<TQ>;
+  using TK = std::conditional_t<std::is_same_v<TQ, F16>, F16, Bf16>;  // of the scores' products
+  static constexpr int G = D / 64, NQ = TQ::kBytes == 4 ? 3 : 1, NP = kProbPlanes<TQ>;
   static constexpr float kLag = 5.0f;
   uint32_t q[NQ][RT][G][2][4];  // elements 64 G + 16 g + 8 j + (i, i + 4)
   float qs[RT][G], qs16[RT][G]; // sums of a group's elements, and 1/16 of them
@@ -267,7 +271,8 @@ struct Rows4 {
   floatx4 o[RT][D / 16];        // element 64 G + 4 (4 g + r) + d in register r of 4 G + d: sums with 1 + code / 16
   float ob[RT][G];              // sums of p (base - 16 scale), over this lane's keys
   float m[RT], l[RT];
-  CodeBits bits;
+  CodeBits<TK> key_bits;
+  CodeBits<Bf16> value_bits;
 
   // at[t]: the first element of tile t's row c
   __device__ __forceinline__ void load(const char *const (&at)[RT], float score_scale, int g) {
@@ -298,7 +303,8 @@ struct Rows4 {
             float a = x[e], b = x[e + 4];
 #pragma unroll
             for (int k = 0; k < NQ; k++) {
-              q[k][t][i][j][e] = cut_pair(a, b);
+              if constexpr (std::is_same_v<TQ, F16>) q[k][t][i][j][e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
+              else q[k][t][i][j][e] = cut_pair(a, b);
               a -= cut_bits(a), b -= cut_bits(b);
             }
           }
@@ -323,11 +329,11 @@ struct Rows4 {
 #pragma unroll
         for (int j = 0; j < 2; j++) {
           uint32_t codes[4];
-          bits.pairs(x.k[h][i][j], codes);
+          key_bits.pairs(x.k[h][i][j], codes);
 #pragma unroll
           for (int k = NQ - 1; k >= 0; k--)
 #pragma unroll
-            for (int t = 0; t < RT; t++) acc[i][t] = mfma16<Bf16>(codes, q[k][t][i][j], acc[i][t]);
+            for (int t = 0; t < RT; t++) acc[i][t] = mfma16<TK>(codes, q[k][t][i][j], acc[i][t]);
         }
       }
 #pragma unroll
@@ -417,7 +423,7 @@ struct Rows4 {
 #pragma unroll
       for (int n = 0; n < 4; n++) {
         uint32_t w[4];
-        bits.pairs(x.v[2 * n][i] | x.v[2 * n + 1][i] << 16, w);
+        value_bits.pairs(x.v[2 * n][i] | x.v[2 * n + 1][i] << 16, w);
 #pragma unroll
         for (int d = 0; d < 4; d++) codes[d][n] = w[d];
       }
@@ -652,11 +658,13 @@ __device__ __forceinline__ uint32_t lds_address(const void *p) {
 
 // Few query rows (or many) over 4 bits: 4 waves over tiles of 32 keys of their own, each with a ring of tiles in LDS that direct
 // loads fill: few instructions for many small rows, no registers for what is on its way, and the operands' order comes from
-// how LDS is read.  Bound by instructions: 16 tokens, 8 key heads of 128, 8,191 .. 32,768 rows, 378 MB, 86 us (4.4 TB/s), about 400
-// vector and 180 scalar instructions a tile and wave, the vector units busy 58% of the time.  Straight into registers, 36 loads a
-// tile, 125 us for the call that takes 91 now.  Three blocks a compute unit with two tiles each 99 us, two with four tiles 112 (16-bit
-// queries, D 128).  Two row tiles of 16 for prompts: 4,096 tokens 484 -> 400 us (343 TFLOP/s).  Row r of 16 lies in slot 4 (r % 4) + r / 4, its 16-byte pieces in another order by row (piece ^ r % 4, of two
+// how LDS is read.  Row r of 16 lies in slot 4 (r % 4) + r / 4, its 16-byte pieces in another order by row (piece ^ r % 4, of two
 // pieces piece ^ r / 2 % 2): reads of 16 key rows' same piece and of four value rows' same part fall on different banks.
+// Bound by instructions: 16 tokens, 8 key heads of 128, 8,191 .. 32,768 rows, 378 MB, 86 us (4.4 TB/s), about 400 vector and 180
+// scalar instructions a tile and wave, the vector units busy 58% of the time.  Straight into registers, 36 loads a tile, the call
+// that takes 91 us now took 125.  Three blocks a compute unit with two tiles each 99 us, two with four tiles 112 (16-bit queries,
+// D 128).  Two row tiles of 16 for prompts: 4,096 tokens 484 -> 400 us (343 TFLOP/s).  fp16 queries as they are, by fp16 products of the
+// codes, instead of two bf16 planes: 487 -> 399 us there, 109 -> 105 for 16 tokens.
 template <int D, class TQ>
 constexpr int kCodeBlocks = D == 64 ? (TQ::kBytes == 4 ? 3 : 4) : TQ::kBytes == 4 ? 2 : 3;  // a compute unit
 template <int D, class TQ, int RT>
@@ -1191,7 +1199,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(Args p) {
 
 int code_blocks(int D, int type) {
   return D == 64 ? (type == kOpF32 ? kCodeBlocks<64, F32> : kCodeBlocks<64, Bf16>)
-                 : type == kOpF32 ? kCodeBlocks<128, F32> : type == kOpBf16 ? kCodeBlocks<128, Bf16> : kCodeBlocks<128, F16>;
+                 : (type == kOpF32 ? kCodeBlocks<128, F32> : kCodeBlocks<128, Bf16>);
 }
 // How a launch is laid out: rows of a block, blocks of a key head, or `parts` that share the keys.
 struct Plan {
