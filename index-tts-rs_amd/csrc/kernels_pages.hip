@@ -7,10 +7,10 @@
 //   base = min x, scale = (max x - min x) / 15 (to fp32 and to fp16), code = rint((x - base) / scale) in 0 .. 15 (scale 0: 0),
 // the quantiser of the decoder's weights.  Rotation and quantiser work in 64 bits, which run at the rate of 32 here:
 // codes are those of the definition, also where a value lies next to the border of two.
-// 7,428 tokens, 32 heads and 8 key heads of 128, all turned: into bf16 33 us (184 MB, 5.5 TB/s: memory), into 4 bits 49 us (169 MB):
-// 1,180 vector instructions a wave of three pieces, half of the time, beside memory.
+// 6,582 tokens, 32 heads and 8 key heads of 128, all turned, us a call: into bf16 30.5 (162 MB, 5.3 TB/s: memory), into 4 bits 43.4
+// (142 MB): half of it are its waves' 64-bit instructions (two exchanges through LDS a step and canonical operands more: 45).
 //
-// Gather.  A copy: 147 MB of bf16 rows 21 us, 84 MB of 4 bits and the values they stand for 17 us.
+// Gather.  A copy: 147 MB of bf16 rows 19 us; 4 bits to fp32 values, 186 MB, 25 us (one piece a thread: 31).
 #include <algorithm>
 #include <type_traits>
 
@@ -40,6 +40,28 @@ __device__ __forceinline__ void store8(char *p, const X (&x)[8]) {
   store4<T>(p + 4 * T::kBytes, (float)x[4], (float)x[5], (float)x[6], (float)x[7]);
 }
 
+// (in one instruction: fmin and fmax have both operands made canonical first)
+__device__ __forceinline__ double lesser(double a, double b) {
+  double r;
+  asm("v_min_f64 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+  return r;
+}
+__device__ __forceinline__ double greater(double a, double b) {
+  double r;
+  asm("v_max_f64 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+  return r;
+}
+// The other lane's value, a step of 1, 2 or 4 lanes away in a group of 8 (4: mirrored, which does where all lanes of four agree).
+template <int STEP>
+__device__ __forceinline__ double near_lane(double v) {
+  constexpr int kMove = STEP == 1 ? 0xb1 : STEP == 2 ? 0x4e : 0x141;  // quad_perm [1 0 3 2], [2 3 0 1], row_half_mirror
+  asm("s_nop 1" : "+v"(v));  // (what the instructions above wrote is read by other lanes two wait states later at the earliest)
+  const uint64_t w = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (uint32_t)w, kMove, 0xf, 0xf, true);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (uint32_t)(w >> 32), kMove, 0xf, 0xf, true);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
 // A row's lanes (D / 16 of them, 16 elements each in two runs of 8 with numbers run[0], run[1]) to codes and pairs.
 template <int D>
 __device__ __forceinline__ void store_codes(char *codes, char *pairs, const int (&run)[2], int j, const double (&x)[2][8]) {
@@ -50,7 +72,7 @@ __device__ __forceinline__ void store_codes(char *codes, char *pairs, const int 
     least[i] = most[i] = x[i][0];
 #pragma unroll
     for (int e = 0; e < 8; e++) {
-      least[i] = fmin(least[i], x[i][e]), most[i] = fmax(most[i], x[i][e]);
+      least[i] = lesser(least[i], x[i][e]), most[i] = greater(most[i], x[i][e]);
       odd = __builtin_fma(x[i][e], 0.0, odd);  // NaN for a value that is no finite number
     }
     // (which then makes the range infinite)
@@ -61,12 +83,10 @@ __device__ __forceinline__ void store_codes(char *codes, char *pairs, const int 
   for (int G = 0; G < kGroups; G++) {
     const bool in0 = kGroups == 1 || run[0] >> 3 == G, in1 = kGroups == 1 || run[1] >> 3 == G;
     lo[G] = in0 ? least[0] : INFINITY, hi[G] = in0 ? most[0] : -INFINITY;
-    lo[G] = fmin(lo[G], in1 ? least[1] : INFINITY), hi[G] = fmax(hi[G], in1 ? most[1] : -INFINITY);
-#pragma unroll
-    for (int step = 1; step < kLanes; step *= 2) {
-      lo[G] = fmin(lo[G], __shfl_xor(lo[G], step, 64));
-      hi[G] = fmax(hi[G], __shfl_xor(hi[G], step, 64));
-    }
+    lo[G] = lesser(lo[G], in1 ? least[1] : INFINITY), hi[G] = greater(hi[G], in1 ? most[1] : -INFINITY);
+    lo[G] = lesser(lo[G], near_lane<1>(lo[G])), hi[G] = greater(hi[G], near_lane<1>(hi[G]));
+    lo[G] = lesser(lo[G], near_lane<2>(lo[G])), hi[G] = greater(hi[G], near_lane<2>(hi[G]));
+    if constexpr (kLanes == 8) lo[G] = lesser(lo[G], near_lane<4>(lo[G])), hi[G] = greater(hi[G], near_lane<4>(hi[G]));
   }
   double scale[kGroups], base[kGroups], inverse[kGroups];
 #pragma unroll
@@ -233,42 +253,63 @@ __global__ __launch_bounds__(256) void append_kernel(PagedAppend a, int pieces, 
   }
 }
 
-// A thread per eight elements of an output row; blocks of a sequence, key head and cache.
+// A thread takes kAtOnce pieces of 16 bytes of an output's rows; blocks of a sequence, key head and cache.
+constexpr int kAtOnce = 4;
 template <int D, class TKV, class TO>
 __global__ __launch_bounds__(256) void gather_kernel(PagedGather a, uint64_t mul) {
+  constexpr int kPer = 16 / TO::kBytes, kPieces = D / kPer;
   const int b = blockIdx.y, is_v = blockIdx.z & 1, head = blockIdx.z >> 1;
-  const int i = blockIdx.x * 256 + threadIdx.x, row = i / (D / 8), run = i % (D / 8);
-  if (row >= a.rows) return;
+  const int i0 = blockIdx.x * 256 * kAtOnce + threadIdx.x;
   const int len = uniform_load(a.lengths + b);
   const bool bad = len < 0 || len > (int)min((int64_t)a.n_table * a.pages.size, (int64_t)kPagesMaxRows);
-  float x[8] = {};
-  if (!bad && row < len) {
-    const int p = page_of(row, mul), page = a.table[b * a.tab_b + p];
-    const int64_t at = row - p * a.pages.size;
-    if ((uint32_t)page < (uint32_t)a.pages.n) {
-      const char *from = is_v ? a.pages.v + page * a.pages.v_p + head * a.pages.v_h + at * a.pages.v_r
-                              : a.pages.k + page * a.pages.k_p + head * a.pages.k_h + at * a.pages.k_r;
-      if constexpr (std::is_same_v<TKV, I4>) {
-        const char *pairs = is_v ? a.pages.vp + page * a.pages.vp_p + head * a.pages.vp_h + at * a.pages.vp_r
-                                 : a.pages.kp + page * a.pages.kp_p + head * a.pages.kp_h + at * a.pages.kp_r;
-        const uint32_t w = *reinterpret_cast<const uint32_t *>(from + 4 * run);
-        const uint32_t pair = *reinterpret_cast<const uint32_t *>(pairs + 4 * (run >> 3));
-        const float s = half_bits_to_float(pair & 0xffffu), base = half_bits_to_float(pair >> 16);
+  const int rows = bad ? 0 : min(len, a.rows);
+  const char *pages = is_v ? a.pages.v + head * a.pages.v_h : a.pages.k + head * a.pages.k_h;
+  const int64_t page_step = is_v ? a.pages.v_p : a.pages.k_p, row_step = is_v ? a.pages.v_r : a.pages.k_r;
+  const char *all_pairs = is_v ? a.pages.vp + head * a.pages.vp_h : a.pages.kp + head * a.pages.kp_h;
+  const int64_t pair_page = is_v ? a.pages.vp_p : a.pages.kp_p, pair_row = is_v ? a.pages.vp_r : a.pages.kp_r;
+  int page[kAtOnce], at[kAtOnce];
 #pragma unroll
-        for (int e = 0; e < 8; e++) x[e] = __builtin_fmaf((float)(w >> (4 * e) & 15u), s, base);
-      } else {
-        load8<TKV>(from + 8 * run * TKV::kBytes, x);
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; e++) x[e] = NAN;
-    }
-  } else if (bad) {
-#pragma unroll
-    for (int e = 0; e < 8; e++) x[e] = NAN;
+  for (int u = 0; u < kAtOnce; u++) {
+    const int row = (i0 + 256 * u) / kPieces, p = row < rows ? page_of(row, mul) : 0;
+    page[u] = row < rows ? a.table[b * a.tab_b + p] : -1;
+    at[u] = row - p * a.pages.size;
   }
-  const int64_t to = is_v ? b * a.v_b + head * a.v_h + row * a.v_r : b * a.k_b + head * a.k_h + row * a.k_r;
-  store8<TO>(static_cast<char *>(is_v ? a.v : a.k) + (to + 8 * run) * TO::kBytes, x);
+  constexpr bool kCodes = std::is_same_v<TKV, I4>;
+  uint32_t w[kAtOnce][kCodes ? 2 : 4];
+#pragma unroll
+  for (int u = 0; u < kAtOnce; u++) {
+    const int run = (i0 + 256 * u) % kPieces;
+    if ((uint32_t)page[u] >= (uint32_t)a.pages.n) continue;
+    const char *from = pages + page[u] * page_step + at[u] * row_step;
+    if constexpr (kCodes) {
+      if constexpr (kPer == 8) w[u][0] = *reinterpret_cast<const uint32_t *>(from + 4 * run);
+      else w[u][0] = *reinterpret_cast<const uint16_t *>(from + 2 * run);
+      w[u][1] = *reinterpret_cast<const uint32_t *>(all_pairs + page[u] * pair_page + at[u] * pair_row + 4 * (run * kPer >> 6));
+    } else {
+      load_dwords<4>(from + 16 * run, w[u]);
+    }
+  }
+  char *to = static_cast<char *>(is_v ? a.v : a.k) + (is_v ? b * a.v_b + head * a.v_h : b * a.k_b + head * a.k_h) * TO::kBytes;
+  const int64_t to_row = is_v ? a.v_r : a.k_r;
+#pragma unroll
+  for (int u = 0; u < kAtOnce; u++) {
+    const int row = (i0 + 256 * u) / kPieces, run = (i0 + 256 * u) % kPieces;
+    if (row >= a.rows) return;
+    const bool there = (uint32_t)page[u] < (uint32_t)a.pages.n;
+    const float rest = bad || row < rows ? NAN : 0.0f;  // of rows that are not there
+    char *p = to + (row * to_row + kPer * run) * TO::kBytes;
+    if constexpr (kCodes) {
+      const float s = half_bits_to_float(w[u][1] & 0xffffu), base = half_bits_to_float(w[u][1] >> 16);
+      float x[kPer];
+#pragma unroll
+      for (int e = 0; e < kPer; e++) x[e] = there ? __builtin_fmaf((float)(w[u][0] >> (4 * e) & 15u), s, base) : rest;
+      if constexpr (kPer == 8) store8<TO>(p, x);
+      else store4<TO>(p, x[0], x[1], x[2], x[3]);
+    } else {
+      const uint32_t fill = rest == 0.0f ? 0u : TO::kBytes == 4 ? 0x7fc00000u : std::is_same_v<TO, Bf16> ? 0x7fc07fc0u : 0x7e007e00u;
+      *reinterpret_cast<u32x4 *>(p) = there ? u32x4{w[u][0], w[u][1], w[u][2], w[u][3]} : u32x4{fill, fill, fill, fill};
+    }
+  }
 }
 
 template <int D, class TX, class TKV>
@@ -288,7 +329,8 @@ hipError_t launch_append(const PagedAppend &a, int n_cu, hipStream_t s) {
 template <class TKV, class TO>
 hipError_t launch_gather(const PagedGather &a, hipStream_t s) {
   const int D = a.pages.D;
-  const dim3 grid((unsigned)(((int64_t)a.rows * (D / 8) + 255) / 256), a.batch, 2 * a.pages.Hk);
+  const int pieces = D * TO::kBytes / 16;
+  const dim3 grid((unsigned)(((int64_t)a.rows * pieces + 256 * kAtOnce - 1) / (256 * kAtOnce)), a.batch, 2 * a.pages.Hk);
   if (D == 64) hipLaunchKernelGGL((gather_kernel<64, TKV, TO>), grid, dim3(256), 0, s, a, page_mul(a.pages.size));
   else hipLaunchKernelGGL((gather_kernel<128, TKV, TO>), grid, dim3(256), 0, s, a, page_mul(a.pages.size));
   return hipGetLastError();
