@@ -42,7 +42,7 @@ struct __attribute__((packed, aligned(alignof(E)))) Run {
 
 // 8 x THREADS x RUNS tokens a block.  Every block goes through the row's whole lists, so pieces are large: 256 bf16 rows of 60,510
 // under a mask, a history of 2,000 and 50 biases, a call: blocks of 4,096 tokens 29.3 us, 8,192 25.9, 16,384 20 (66 MB; without
-// lists 13).
+// lists 13).  Blocks that take several pieces in turn, the next one's loads ahead of the lists of the one before: 22.
 // All tokens pass with the mask alone; those of the lists, few, are then written again by whoever takes their word out of LDS
 // first.
 template <int TYPE, int kThreads, int RUNS>
