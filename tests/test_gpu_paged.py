@@ -469,6 +469,30 @@ def test_attention_of_starts_that_fall(ops, types, tokens):
     check(first, *s.ref())
 
 
+@pytest.mark.parametrize("q_type", [F32, F16, BF16])
+@pytest.mark.parametrize("batch", [1, 64])
+def test_attention_of_even_weights_over_long_contexts(ops, q_type, batch):
+    """4 bits, 60,000 rows of the same weight: the mean of their values, much smaller than each, as exact as their number lets it be.
+
+    A sum's running value is a walk of n steps of at most 31 scales, within 3 * 24 sqrt(n) scales; it is rounded n / 16 times at random,
+    by 2^-24 of that at most, four waves' sums being less.  Four deviations: 4 * 2^-24 * 72 sqrt(n) * sqrt(n / 16) scales, over n."""
+    say(f"[gpu] paged attention even weights {q_type} batch={batch}")
+    n, hk, d, page = 60_000, 8, 128, 64
+    count, g = -(-n // page), gen(4)
+    cache = ops.paged_cache(count, hk, page, d, bits=4)
+    cache.k.zero_(), cache.k_params.zero_()
+    cache.v.random_(0, 256, generator=g)
+    scale = 0.125 + 0.125 * torch.rand(cache.v_params.shape[:-1], generator=g, device="cuda")
+    cache.v_params.copy_(torch.stack([scale, -7.5 * scale * (0.9 + 0.2 * torch.rand(scale.shape, generator=g, device="cuda"))], -1))
+    ref = torch.stack([values(cache.v[:, h], cache.v_params[:, h]).flatten(0, 1)[:n].mean(0) for h in range(hk)])
+    table = torch.arange(count, dtype=torch.int32, device="cuda").expand(batch, -1).contiguous()
+    q = torch.zeros((batch, 2 * hk, d), dtype=q_type, device="cuda")
+    got = ops.paged_attention(q, cache, ints(range(batch + 1)), ints([n] * batch), table)
+    ref = ref.repeat_interleave(2, 0).expand(batch, -1, -1)
+    tol = 4 * 2.0 ** -24 * 72 / 4 * 0.25 + (0 if q_type == F32 else HALF[q_type] * ref.abs())
+    check(got, ref, tol)
+
+
 @pytest.mark.parametrize("kv", [BF16, 4])
 def test_attention_of_more_rows_than_a_quotient_holds(ops, kv):
     """320,000 tokens of 127 heads, each of which sees its own row alone: results are the values.  (2^32 / 127, rounded up, gives a
