@@ -436,7 +436,8 @@ itts_status itts_cache_keep(const itts_cache_keep_args *args, void *stream);
  * apart, rows at most 2^26.
  *
  * Tokens of a batch stand one sequence after the other, those of sequence b from starts[b] to starts[b + 1] - 1 (starts
- * [batch + 1], rising, equal for a sequence without any).  A sequence whose starts fall or leave the n_tokens has none. */
+ * [batch + 1], rising, equal for a sequence without any).  A sequence whose starts fall or leave the n_tokens has none; of
+ * more than 64 sequences its neighbours may then have none either. */
 typedef struct itts_pages {
   void *k, *v;
   void *k_params, *v_params;

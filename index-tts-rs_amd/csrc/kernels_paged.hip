@@ -29,6 +29,7 @@ struct Args {
   uint32_t group_mul;  // 2^32 / group, rounded up: one too many at most
   uint64_t page_mul;
   bool even;           // pages of multiples of 32 rows
+  int per_token;       // without shares: blocks that stand for a token (0: tokens together, and one more a sequence)
   int unit, least;     // a share is at least `least` times 2^unit tiles of keys
   float2 *ml;
   int2 *dealt;
@@ -54,18 +55,47 @@ struct Tiles {
 };
 
 // What block `index` has to do: tiles [first, end) of row tile `tile` of sequence b, whose rows are shared by n blocks (0:
-// nothing is left for this one).  Every share has the same size, the smallest one with which `blocks` are enough.  Found by
-// every wave from the starts and lengths, a lane a sequence.  A sequence's last tokens, which see most, come first.
+// nothing is left for this one).  A sequence's last tokens, which see most, come first.
 struct Share {
   int b, tile, n, first, end;
 };
+// Blocks with all keys of a row tile: those of a sequence stand from a number on that its first token alone tells, with room
+// for as many as it can have, so that a wave finds its own in a search by 64 starts.  (By all sequences' row tiles, a lane a
+// sequence, 64 at a time: 2,048 tokens over 200 .. 499 rows 778 us for 518, 16,384 over 64 rows 11,540 for 730.)
+template <int ROWS>
+__device__ __forceinline__ Share whole_of(const Args &p, int index) {
+  const PagedAttn &a = p.a;
+  const int lane = threadIdx.x & 63;
+  auto first_of = [&](int b) {
+    const int token = min(max(a.starts[b], 0), a.tokens);
+    return p.per_token > 0 ? token * p.per_token : token * p.group / ROWS + b;
+  };
+  int b = 0, n = a.batch;
+  for (bool any = false; n > 1 || !any; any = true) {
+    const int step = (n + 63) >> 6, at = lane * step;
+    const uint64_t in = __ballot(at < n && first_of(b + min(at, n - 1)) <= index);
+    if (in == 0) return Share{0, 0, 0, 0, 0};
+    const int i = 63 - __builtin_clzll(in);
+    b += i * step, n = min(step, n - i * step);
+  }
+  b = __builtin_amdgcn_readfirstlane(b);
+  const int start = uniform_load(a.starts + b);
+  const Span span = span_of(start, uniform_load(a.starts + b + 1), a.tokens);
+  const int tiles = (span.n * p.group + ROWS - 1) / ROWS, token = min(max(start, 0), a.tokens);
+  const int local = index - (p.per_token > 0 ? token * p.per_token : token * p.group / ROWS + b);
+  if (local >= tiles) return Share{0, 0, 0, 0, 0};
+  return Share{b, tiles - 1 - local, 1, 0, 1 << 30};
+}
+// Blocks that share the keys: every share has the same size, the smallest one with which `blocks` are enough.  Found by
+// every wave from the starts and lengths, a lane a sequence.
 template <int ROWS, int KT>
 __device__ __forceinline__ Share share_of(const Args &p, int index, int hk) {
+  if (p.parts == 0) return whole_of<ROWS>(p, index);
   const PagedAttn &a = p.a;
   const int lane = threadIdx.x & 63;
   // (the first block of all says for every sequence where its shares are; where starts fall and sequences have more rows than
   // there are tokens, those that have no blocks any more are left out)
-  const bool tells = p.parts > 0 && index == 0 && hk == 0;
+  const bool tells = index == 0 && hk == 0;
   // row tiles of a sequence, and the units of keys that one of them sees at most
   auto count = [&](int b, int &tiles, int &units) {
     tiles = 0, units = 0;
@@ -77,31 +107,28 @@ __device__ __forceinline__ Share share_of(const Args &p, int index, int hk) {
     if (a.window > 0) seen = (int)min((int64_t)seen, (int64_t)a.window + min(a.sinks, a.max_rows) + (ROWS - 1) / p.group + 1 + 2 * KT);
     units = tiles == 0 ? 0 : ((seen + KT - 1) / KT + (1 << p.unit) - 1) >> p.unit;
   };
-  int size = 1 << 30;
-  if (p.parts > 0) {
-    float total = 0.0f, longest = 0.0f;
+  float total = 0.0f, longest = 0.0f;
+  for (int b0 = 0; b0 < a.batch; b0 += 64) {
+    int tiles, units;
+    count(b0 + lane, tiles, units);
+    total += (float)tiles * units, longest = fmaxf(longest, units);
+  }
+  total = wave_sum(total), longest = wave_max(longest);
+  // (64 blocks of a row tile at most: the joining kernel's lanes)
+  int size = (int)fmaxf(ceilf(fmaxf(total / p.parts, longest / 64)), (float)p.least);
+  for (int i = 0; i < 16; i++) {
+    float blocks = 0.0f;
     for (int b0 = 0; b0 < a.batch; b0 += 64) {
       int tiles, units;
       count(b0 + lane, tiles, units);
-      total += (float)tiles * units, longest = fmaxf(longest, units);
+      blocks += (float)tiles * ((units + size - 1) / size);
     }
-    total = wave_sum(total), longest = wave_max(longest);
-    // (64 blocks of a row tile at most: the joining kernel's lanes)
-    size = (int)fmaxf(ceilf(fmaxf(total / p.parts, longest / 64)), (float)p.least);
-    for (int i = 0; i < 16; i++) {
-      float blocks = 0.0f;
-      for (int b0 = 0; b0 < a.batch; b0 += 64) {
-        int tiles, units;
-        count(b0 + lane, tiles, units);
-        blocks += (float)tiles * ((units + size - 1) / size);
-      }
-      blocks = wave_sum(blocks);
-      if (blocks <= p.parts) break;
-      // (at last a share for each row tile; blocks are enough for those)
-      size = i < 14 ? max(size + 1, (int)ceilf(size * (blocks / p.parts))) : (int)longest + 1;
-    }
-    size = __builtin_amdgcn_readfirstlane(size);
+    blocks = wave_sum(blocks);
+    if (blocks <= p.parts) break;
+    // (at last a share for each row tile; blocks are enough for those)
+    size = i < 14 ? max(size + 1, (int)ceilf(size * (blocks / p.parts))) : (int)longest + 1;
   }
+  size = __builtin_amdgcn_readfirstlane(size);
   Share share{0, 0, 0, 0, 0};
   int before = 0;
   for (int b0 = 0; b0 < a.batch && (share.n == 0 || tells); b0 += 64) {
@@ -1210,7 +1237,7 @@ int code_blocks(int D, int type) {
 struct Plan {
   bool many;  // paged_rows_kernel
   int RT;     // tiles of 16 rows of a block otherwise
-  int rows, blocks, parts, unit, least;
+  int rows, blocks, parts, unit, least, per_token;
 };
 Plan make_plan(const PagedAttn &a, int n_cu) {
   Plan p;
@@ -1225,8 +1252,9 @@ Plan make_plan(const PagedAttn &a, int n_cu) {
   p.RT = !p.many && rows >= 32 && (D == 64 || (codes && !wide)) ? 2 : 1;
   p.rows = p.many ? kLongRows : 16 * p.RT, p.unit = p.many ? 1 : 2, p.least = 2;
   // row tiles at most: a sequence's last one may be short
-  const int64_t most = std::min<int64_t>((int64_t)a.tokens * group / p.rows + std::min(a.batch, a.tokens),
-                                         (int64_t)a.tokens * ((group + p.rows - 1) / p.rows));
+  const int a_token = (group + p.rows - 1) / p.rows;
+  const int64_t apart = (int64_t)a.tokens * a_token, together = (int64_t)a.tokens * group / p.rows + a.batch, most = std::min(apart, together);
+  p.per_token = apart <= together ? a_token : 0;
   p.parts = 0, p.blocks = (int)most;
   const int at_once = n_cu * (codes && !p.many && p.RT == 1 ? code_blocks(D, a.type) : 2) / a.pages.Hk;
   const int64_t seen = a.window > 0 ? std::min<int64_t>(a.max_rows, (int64_t)a.window + std::min(a.sinks, a.max_rows)) : a.max_rows;
@@ -1248,7 +1276,7 @@ size_t part_rows(const PagedAttn &a, const Plan &p) { return (size_t)a.pages.Hk 
 Args make_args(const PagedAttn &a, const Plan &p) {
   const int group = a.H / a.pages.Hk;
   float *ml = a.part + part_rows(a, p) * a.pages.D;
-  return Args{a, p.blocks, p.parts, group, (uint32_t)(((1ull << 32) + group - 1) / group), page_mul(a.pages.size), a.pages.size % 32 == 0, p.unit, p.least,
+  return Args{a, p.blocks, p.parts, group, (uint32_t)(((1ull << 32) + group - 1) / group), page_mul(a.pages.size), a.pages.size % 32 == 0, p.per_token, p.unit, p.least,
               reinterpret_cast<float2 *>(ml), reinterpret_cast<int2 *>(ml + 2 * part_rows(a, p))};
 }
 template <int D, class TQ, int ROWS, class K>

@@ -229,6 +229,29 @@ def test_attention_many_sequences(ops, types, batch):
     assert torch.equal(s.run(ops, max_length=16 * s.table.shape[1]), s.run(ops))
 
 
+@pytest.mark.parametrize("types", [(F32, BF16), (BF16, BF16), (F16, F16), (F32, F32)])
+@pytest.mark.parametrize("news", [1, 37, 300])
+@pytest.mark.parametrize("h,hk", [(2, 2), (20, 1)])
+def test_attention_of_thousands_of_sequences(ops, types, news, h, hk):
+    """Every third one without tokens; each token sees its own row alone, so that results are the values."""
+    say(f"[gpu] paged attention thousands {types} {news} {h}/{hk}")
+    d, page, batch = 64, 16, 70_000 // (news + 6)
+    count = torch.tensor([0 if i % 3 == 1 else 1 + i * 7 % news for i in range(batch)], dtype=torch.int32)
+    wide = -(-news // page)
+    cache = ops.paged_cache(batch * wide, hk, page, d, types[1], bits=32 if types[1] == F32 else 16)
+    cache.k.zero_(), cache.v.copy_(randn(gen(8), *cache.v.shape))
+    table = torch.randperm(batch * wide, generator=torch.Generator().manual_seed(9)).int().view(batch, wide).cuda()
+    starts = torch.cat([torch.zeros(1, dtype=torch.int32), count.cumsum(0).int()])
+    own = torch.repeat_interleave(torch.arange(batch), count)
+    row = torch.arange(len(own)) - starts[own]
+    q = randn(gen(9), len(own), h, d, dtype=types[0])
+    got = ops.paged_attention(q, cache, starts.cuda(), count.cuda(), table, window=1)
+    want = cache.v[table[own.cuda(), row.cuda() // page].long(), :, row.cuda() % page].repeat_interleave(h // hk, 1).to(types[0])
+    # (a probability over itself: two roundings of 2^-24, under fp32 queries seen)
+    tol = 4 * EPS * want.double().abs() if types[0] == F32 else torch.zeros_like(want, dtype=torch.float64)
+    assert ((got.double() - want.double()).abs() <= tol).all()
+
+
 @pytest.mark.parametrize("types", [(F32, BF16), (F32, F32), (BF16, BF16), (F16, F16)])
 @pytest.mark.parametrize("value", [NAN, INF, -INF])
 @pytest.mark.parametrize("window", [0, 12])
