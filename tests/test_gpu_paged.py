@@ -5,8 +5,8 @@ magnitudes (A = sum |q k| scale), and one or two roundings on its way through th
 twice that, relative, and a row of n keys sums to within 2 sqrt(n) roundings.  Under 16-bit queries a probability enters the second
 product as two planes, off by 2^-16 of it (bf16; 2^-21 fp16), in the product and in the sum of what is divided by; outputs of 16
 bits add half a step of the result.  Over 4 bits a score is formed as sum q (1 + c / 16) - sum q, times 16 scale, plus base sum q:
-sums of magnitudes up to A4 = sum_groups (48 |scale| + |base|) sum |q|; values in the same way with V4 = sum p (48 |scale| + |base|)
-in place of P = sum p |v|.
+sums of magnitudes up to A4 = sum_groups (48 |scale| + |base|) sum |q|; values in the same way, from 16 + c of one key and c - 31 of the next,
+with V4 = sum p (48 |scale| + |base|) in place of P = sum p |v| (48 is less than the second kind's 62: on the strict side).
 Appended and gathered rows: worked out in 64 bits (append) or with one operation (gather), so one rounding; codes are exact.
 Logits: at most six operations in float32 and one rounding to the type."""
 import itertools
