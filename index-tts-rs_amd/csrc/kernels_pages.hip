@@ -66,9 +66,10 @@ __device__ __forceinline__ double near_lane(double v) {
 template <int D>
 __device__ __forceinline__ void store_codes(char *codes, char *pairs, const int (&run)[2], int j, const double (&x)[2][8]) {
   constexpr int kLanes = D / 16, kGroups = D / 64;
-  double least[2], most[2], odd = 0.0;
+  double least[2], most[2];
 #pragma unroll
   for (int i = 0; i < 2; i++) {
+    double odd = 0.0;  // (of each run by itself: the two may lie in different groups)
     least[i] = most[i] = x[i][0];
 #pragma unroll
     for (int e = 0; e < 8; e++) {

@@ -690,6 +690,37 @@ def test_append_into_rows_of_all_heads(ops, bits):
         assert a is None and b is None or torch.equal(a, b)
 
 
+@pytest.mark.parametrize("q_type", [F32, BF16, F16])
+@pytest.mark.parametrize("value", [NAN, INF, -INF])
+@pytest.mark.parametrize("rot,interleaved", [(128, False), (96, False), (80, False), (64, False), (128, True), (0, False)])
+def test_append_odd_values_stay_in_their_group(ops, q_type, value, rot, interleaved):
+    """4 bits of 128: one of a row's two groups of 64 holds a value that is no finite number, at either end of a run of 8 and in
+    every run; the other group's codes and pair are as without it.  Keys turn, so that a pair's other element is odd as well."""
+    say(f"[gpu] paged append odd groups {q_type} {value} rot={rot} interleaved={interleaved}")
+    g, d, hk, at = gen(31), 128, 2, [*range(0, 128, 8), *range(7, 128, 8), 5, 70]
+    n = len(at) + 2
+    k, v = (randn(g, n, hk, d, dtype=q_type) for _ in range(2))
+    for i, e in enumerate(at):
+        k[i, i % 2, e] = v[i, 1 - i % 2, e] = value
+    k[n - 2, 0, 3] = k[n - 2, 0, 90] = v[n - 2, 0, 3] = v[n - 2, 0, 90] = value     # both groups; the last row has none
+    cache, table = ops.paged_cache(3, hk, 16, d, bits=4), rotation_table(n + 5, rot) if rot else None
+    for t in cache:
+        t.zero_()
+    pos = torch.arange(5, n + 5, device="cuda")
+    got = ops.paged_append(cache, k, v, ints([0, n]), ints([0]), ints([[2, 0, 1]]), rotation=table, positions=pos.int(), interleaved=interleaved)
+    assert got.lengths.tolist() == [n]
+    page, row = ints([2, 0, 1])[torch.arange(n, device="cuda") // 16].long(), torch.arange(n, device="cuda") % 16
+    back = ops.paged_gather(cache, ints([n]), ints([[2, 0, 1]]), n)
+    for which, want in ((0, turn(k, table, pos, interleaved) if rot else k.double()), (1, v.double())):
+        fine = torch.isfinite(want).unflatten(-1, (2, 64)).all(-1)
+        assert fine.any(-1).sum() > n and (~fine).sum() > len(at)
+        codes, pairs = quantise(want)
+        mine, own = cache[which][page, :, row].unflatten(-1, (2, 32)), cache[2 + which][page, :, row]
+        assert torch.equal(mine[fine], codes.unflatten(-1, (2, 32))[fine]) and torch.equal(own[fine], pairs[fine])
+        read = back[which][0].transpose(0, 1).unflatten(-1, (2, 64))
+        assert torch.isfinite(read[fine]).all() and torch.isnan(read[~fine]).all()
+
+
 def test_append_pairs_round_twice(ops):
     """Scale and base go to float16 by way of float32, for every one of many turned rows."""
     say("[gpu] paged append pairs")
