@@ -99,17 +99,25 @@ __device__ __forceinline__ void cut3(float a, float b, uint32_t (&o)[3]) {
 }
 // The same for probabilities (never negative).  bf16: the last rest is raised by 2^-23 of what it is the rest
 // of in the subtraction itself; the second of two planes is rounded, 2^-16 of the value at most.  fp16: 11 bits a
-// plane, two hold 22, down to its smallest number, 2^-24, which the rest of a positive value always is at least.
+// plane, two hold 22, down to its smallest number, 2^-24, which both planes of a positive value are at least: 0 times an
+// infinity that is seen would be NaN, however small its weight.  A weight comes out 2^-23 too large at most by that, 2^-33 of
+// the largest one as probabilities are held.
+typedef unsigned short u16x2e __attribute__((ext_vector_type(2)));
 template <class T, int N>
 __device__ __forceinline__ void cut_pos(float a, float b, uint32_t (&o)[N]) {
   constexpr float kUp = 1.0f + 0x1p-23f, kLeast = 0x1.01p-118f;  // (more than the 8 bits of one plane)
   if constexpr (std::is_same_v<T, F16>) {
     static_assert(N == 2);
     const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
-    o[0] = __builtin_bit_cast(uint32_t, h);
-    // (the median: of 0 it is 0)
-    o[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(__builtin_amdgcn_fmed3f(a - (float)h[0], a, 0x1p-24f),
-                                                                   __builtin_amdgcn_fmed3f(b - (float)h[1], b, 0x1p-24f)));
+    const auto rest = __builtin_amdgcn_cvt_pkrtz(a - (float)h[0], b - (float)h[1]);
+    // 1, the bits of 2^-24, where a value is positive: bits of floats as whole numbers, brought down to 16 bits, and no more than 1
+    // (a number that the compiler does not know, or it compares the halves one by one).
+    uint32_t one = 0x00010001u;
+    asm("" : "+s"(one));
+    const u16x2e some = __builtin_elementwise_min(
+        __builtin_bit_cast(u16x2e, __builtin_amdgcn_cvt_pk_u16(__float_as_uint(a), __float_as_uint(b))), __builtin_bit_cast(u16x2e, one));
+    o[0] = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2e, h), some));
+    o[1] = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2e, rest), some));
   } else if constexpr (N == 2) {
     o[0] = cut_pair(a, b);
     const f32x2e rest = {__builtin_fmaf(a, kUp, -cut_bits(a)), __builtin_fmaf(b, kUp, -cut_bits(b))};

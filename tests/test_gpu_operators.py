@@ -348,6 +348,37 @@ def test_attention_shared_tiles_in_a_graph(ops, types):
         check(out[1:2], *attention_ref(q[1:2], k[1:2], v[1:2], ln[1:2], par[1:2]))
 
 
+@pytest.mark.parametrize("value", [INF, -INF])
+@pytest.mark.parametrize("n,h,hk,d,length", [(1, 2, 2, 64, 290), (1, 4, 2, 128, 9000), (9, 8, 2, 64, 700), (72, 8, 8, 64, 300), (48, 16, 2, 128, 300),
+                                             (72, 8, 8, 64, 2000), (130, 16, 16, 64, 900)])
+def test_attention_infinities_of_small_weights(ops, value, n, h, hk, d, length):
+    """Float16: keys whose weight is 2^-40 and 2^-100 of the others' sum hold an infinity in one element, which is then the result's; the
+    finite ones stay as they are."""
+    say(f"[gpu] tree attention infinities of small weights {value} n={n} h={h}/{hk} d={d} length={length}")
+    g = gen(22)
+    x = torch.ones(1, n, h, d, device="cuda", dtype=F16)
+    k, v = (torch.zeros(1, hk, length + n, d, device="cuda", dtype=F16) for _ in range(2))
+    v.copy_(randn(g, *v.shape))
+    ln, par = ints([length]), ints([[-1] + [0] * (n - 1)])
+    scale = 1.0 / d                                          # a score is a key's elements
+    k[:, :, :length] = -28.0                                 # 2^-40
+    k[:, :, :length:8] = 0.0                                 # (some in every tile: the maximum is theirs for every wave)
+    k[:, :, 3:length:64] = -69.0                             # 2^-99.5
+    v[:, 0, 67, 5] = v[:, 0, 131, 40] = value                # such a key's, among keys that all nodes see
+    v[:, 1, 100, 17] = value                                 # one of the first kind
+    got = ops.tree_attention(x, k, v, ln, par, scale=scale)
+    rows = sorted({0, 1 % n, n - 1})
+    ref, tol = attention_ref(x, k, v, ln, par, scale=scale) if n < 10 else (None, None)
+    if ref is not None:
+        inf = torch.isinf(ref)
+        assert torch.equal(torch.isnan(got), torch.isnan(ref)) and torch.equal(got.double()[inf], ref[inf])
+        assert ((got.double() - ref).abs()[~inf] <= tol[~inf]).all()
+    group = h // hk
+    odd = torch.zeros(h, d, dtype=torch.bool, device="cuda")
+    odd[:group, 5] = odd[:group, 40] = odd[group:2 * group, 17] = True
+    assert (got[0, rows][:, odd] == value).all() and torch.isfinite(got[0, rows][:, ~odd]).all()
+
+
 @pytest.mark.parametrize("types", [(F32, BF16), (F32, F32), (BF16, BF16)])
 def test_attention_blocks_of_no_weight(ops, types):
     """A block's keys lie so far below the row's largest score that their weight is 0 as a float: what their values are, finite

@@ -296,6 +296,32 @@ def test_attention_odd_values_in_long_prompts(ops, types, value, d, window):
     assert not fin[100, :2, 0].all() and fin[:170, :, 60:].all()
 
 
+@pytest.mark.parametrize("value", [INF, -INF])
+@pytest.mark.parametrize("lens,news,h,hk,d", [([290], [1], 2, 2, 64), ([9000], [1], 4, 2, 128), ([700, 300], [20, 9], 8, 2, 64), ([700, 400], [150, 70], 8, 2, 64),
+                                              ([400], [200], 4, 2, 128), ([5000, 600], [140, 130], 8, 4, 128)])
+def test_attention_infinities_of_small_weights(ops, value, lens, news, h, hk, d):
+    """Float16: keys whose weight is 2^-40 and 2^-100 of the others' sum hold an infinity in one element, which is then the result's; the
+    finite ones stay as they are."""
+    say(f"[gpu] paged attention infinities of small weights {value} {lens} {news} h={h}/{hk} d={d}")
+    s, scale = Seqs(ops, (F16, F16), lens, news, h, hk, d, 16, seed=23), 1.0 / d
+    s.q.fill_(1.0)                                                # a score is a key's elements
+    for b, n in enumerate(lens):
+        row, page = torch.arange(n, device="cuda"), torch.tensor([s.map[b][t // 16] for t in range(n)], device="cuda")
+        key = torch.full((n,), -28.0, device="cuda")              # 2^-40
+        key[::8], key[3::64] = 0.0, -69.0                         # (some in every tile: the maximum is theirs for every wave); 2^-99.5
+        s.cache.k[page, :, row % 16] = key.half().view(n, 1, 1)
+        s.rows[b][0].copy_(key.view(1, n, 1).expand_as(s.rows[b][0]))
+        for head, t, e in ((0, 67, 5), (0, 131, 40), (1, 100, 17)):
+            s.cache.v[s.map[b][t // 16], head, t % 16, e] = value
+            s.rows[b][2][head, t, e] = value
+    ref, tol = s.ref(scale)
+    got, inf = s.run(ops, scale=scale), torch.isinf(ref)
+    group = h // hk
+    assert inf[:, :group, 5].all() and inf[:, group:2 * group, 17].all() and inf.sum() == len(ref) * 3 * group
+    assert torch.equal(torch.isnan(got), torch.isnan(ref)) and torch.equal(got.double()[inf], ref[inf])
+    assert ((got.double() - ref).abs()[~inf] <= tol[~inf]).all()
+
+
 @pytest.mark.parametrize("types", TYPES)
 def test_attention_odd_calls(ops, types):
     """Lengths out of range, more tokens than rows, pages that do not exist, tokens of no sequence."""
