@@ -436,8 +436,9 @@ itts_status itts_cache_keep(const itts_cache_keep_args *args, void *stream);
  * apart, rows at most 2^26.
  *
  * Tokens of a batch stand one sequence after the other, those of sequence b from starts[b] to starts[b + 1] - 1 (starts
- * [batch + 1], rising, equal for a sequence without any).  A sequence whose starts fall or leave the n_tokens has none; of
- * more than 64 sequences its neighbours may then have none either. */
+ * [batch + 1], rising, equal for a sequence without any).  Where starts do not rise a sequence has all of its tokens or none: none
+ * if they fall or leave the n_tokens, nor if it starts in front of where an earlier one ends; of more than 64 sequences its
+ * neighbours may then have none either. */
 typedef struct itts_pages {
   void *k, *v;
   void *k_params, *v_params;
@@ -458,9 +459,9 @@ typedef struct itts_pages {
  * I4: base = min x and scale = (max x - min x) / 15 of every 64 turned elements x, each rounded to float32 and to
  * float16, code = (x - base) / scale to the nearest (ties to even) in 0 .. 15, 0 where scale is 0; 64 elements with
  * one that is no finite number, or beyond float16's, read back as NaN.
- * A sequence with a negative length or no room (n_table pages, 2^24 rows) is not written, nor is a row whose page is not in
- * 0 .. n_pages - 1: its new length is -1 (and its q_out NaN in the first case).  Rows of q_out of tokens outside all sequences are
- * zeros.  Rows of one page must not be written by two sequences.
+ * A sequence with a negative length or no room (n_table pages, 2^24 rows) is not written, nor is one whose starts leave it without
+ * its tokens, nor a row whose page is not in 0 .. n_pages - 1: its new length is -1 (and its q_out NaN in the first case).  Rows of
+ * q_out of tokens outside all sequences are zeros.  Rows of one page must not be written by two sequences.
  * dtype (of k, v, q): the pages', F32 over BF16, or any over I4.  n_rotated is a multiple of 16. */
 typedef struct itts_paged_append_args {
   itts_pages pages;

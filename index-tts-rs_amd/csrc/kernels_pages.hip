@@ -141,6 +141,7 @@ __global__ __launch_bounds__(256) void append_kernel(PagedAppend a, int pieces, 
     const int start = a.starts[b], end = a.starts[b + 1], len = a.lengths[b], n = end - start;
     bool ok = start >= 0 && end >= start && end <= a.tokens && len >= 0 && len <= max_rows - n;
     if (ok && n > 0) {
+      ok = owner_of(a.starts, a.batch, a.tokens, start).b == b;
       const int last = page_of(len + n - 1, mul);
       for (int p = page_of(len, mul) + lane; p <= last; p += 64) ok = ok && (uint32_t)a.table[b * a.tab_b + p] < (uint32_t)a.pages.n;
     }
@@ -175,17 +176,14 @@ __global__ __launch_bounds__(256) void append_kernel(PagedAppend a, int pieces, 
   float raw[2][8] = {};
   load(part, raw);  // (on its way before anything is known of the sequence)
 
-  const int b = sequence_of(a.starts, a.batch, token);
+  const Owner of = owner_of(a.starts, a.batch, a.tokens, token);
   int row = -1, page = -1, pos = -1;  // row: -2 for a token of a sequence that is refused
-  if (b >= 0) {
-    const int start = uniform_load(a.starts + b), end = uniform_load(a.starts + b + 1), len = uniform_load(a.lengths + b);
-    const Span span = span_of(start, end, a.tokens);
-    if (token >= span.first && token < span.first + span.n) {
-      row = len >= 0 && len <= max_rows - span.n ? len + token - span.first : -2;
-      if (row >= 0) {
-        page = uniform_load(a.table + b * a.tab_b + page_of(row, mul));
-        pos = a.positions ? uniform_load(a.positions + token) : row;
-      }
+  if (of.b >= 0) {
+    const int len = uniform_load(a.lengths + of.b);
+    row = len >= 0 && len <= max_rows - of.n ? len + token - of.first : -2;
+    if (row >= 0) {
+      page = uniform_load(a.table + of.b * a.tab_b + page_of(row, mul));
+      pos = a.positions ? uniform_load(a.positions + token) : row;
     }
   }
   const bool place = row >= 0 && (uint32_t)page < (uint32_t)a.pages.n, known = (uint32_t)pos < (uint32_t)a.n_positions;

@@ -385,9 +385,10 @@ def paged_append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, starts: to
     4 bits: of every 64 elements base = min, scale = (max - min) / 15, both as float16, and codes to the nearest.  64 elements of
     which one is no finite number, or too large for float16, read back as NaN.
     Returns the new lengths and the queries.  A sequence with a negative length, or without room in its table, is not written, nor
-    is a row whose table entry is no page of the cache: its new length is -1 (and its queries NaN in the first case).  A
-    position outside `rotation` makes its rows NaN.  Queries of tokens that belong to no sequence become zeros.  Two sequences must
-    not be given the same row of a page to write."""
+    is a row whose table entry is no page of the cache: its new length is -1 (and its queries NaN in the first case).  So it is, too,
+    for a sequence whose starts fall, leave the tensors or lie in front of where an earlier one ends (of more than 64 perhaps for its
+    neighbours): it has no tokens.  A position outside `rotation` makes its rows NaN.  Queries of tokens that belong to no sequence
+    become zeros.  Two sequences must not be given the same row of a page to write."""
     pages, hk, size, d, dev = _cache(cache)
     sk = _tensor(k, "k", 3, dev, last=True)
     sv = _tensor(v, "v", 3, dev, k.dtype, last=True)

@@ -821,6 +821,66 @@ def test_append_in_place_and_captured(ops):
     assert torch.equal(cache.k[5, :, 8], codes[0]) and torch.equal(cache.k_params[5, :, 8], pairs[0])
 
 
+# ---- starts that do not rise --------------------------------------------------------------
+def spans_of(starts, tokens):
+    """(first token, tokens) of each sequence, or None: starts that fall or leave the tensors, or come back to in front of where an
+    earlier sequence ends."""
+    reach, out = 0, []
+    for i, j in zip(starts, starts[1:]):
+        fits = 0 <= i <= j <= tokens
+        out.append((i, j - i) if fits and (i == j or i >= reach) else None)
+        reach = max(reach, j) if fits and j > i else reach
+    return out
+
+
+def bad_starts(s):
+    """Starts of at least six sequences, each with something wrong about it."""
+    yield "past the end", s[:2] + [10 ** 6] + s[3:]
+    yield "below 0", s[:2] + [-5] + s[3:]
+    yield "falls", s[:3] + [s[1]] + s[4:]
+    yield "first too large", [s[4]] + s[1:]
+    yield "last too small", s[:-1] + [s[2]]
+    yield "around others", s[:1] + [s[5]] + s[2:]
+    yield "first and last", [s[3]] + s[1:-1] + [s[1]]
+    yield "nothing fits", [0, s[-1] + 50] + [s[-1]] * (len(s) - 2)
+
+
+@pytest.mark.parametrize("types", [(F32, BF16), (BF16, 4)])
+def test_append_of_tokens_without_a_sequence(ops, types):
+    """The same of appended rows: a sequence's are all there, or none and its new length is -1."""
+    say(f"[gpu] paged append bad starts {types}")
+    q_type, kv = types
+    g, hk, d, lens, news = gen(42), 2, 64, [3, 14, 0, 31, 7, 9, 20], [4, 1, 5, 40, 2, 3, 0]
+    good = [0] + list(itertools.accumulate(news))
+    n = good[-1]
+    k, v, q = randn(g, n, hk, d, dtype=q_type), randn(g, n, hk, d, dtype=q_type), randn(g, n, 4, d, dtype=q_type)
+    table = torch.arange(7 * 6, dtype=torch.int32).view(7, 6).cuda()
+    for what, starts in [*bad_starts(good), ("falls", [0, 5, 2, n + 9]), ("falls", [0, 7, 3, 7, 20])]:
+        b = len(starts) - 1
+        say("  ", what, starts)
+        cache = ops.paged_cache(42, hk, 16, d, BF16, bits=kv if kv == 4 else 16)
+        for t in cache:
+            if t is not None:
+                t.fill_(0)
+        got = ops.paged_append(cache, k, v, ints(starts), ints(lens[:b]), table[:b], q=q)
+        spans = spans_of(starts, n)
+        assert got.lengths.tolist() == [m + x[1] if x else -1 for m, x in zip(lens, spans)], what
+        want_q, rows = torch.zeros_like(q), [torch.zeros_like(t) if t is not None else None for t in cache]
+        for i, x in enumerate(spans):
+            if not x:
+                continue
+            own = slice(x[0], x[0] + x[1])
+            want_q[own] = q[own]
+            at = torch.arange(lens[i], lens[i] + x[1], device="cuda")
+            for which, src in ((0, k), (1, v)):
+                if kv == 4:
+                    rows[which][table[i][at // 16].long(), :, at % 16], rows[2 + which][table[i][at // 16].long(), :, at % 16] = quantise(src[own].double())
+                else:
+                    rows[which][table[i][at // 16].long(), :, at % 16] = src[own].to(BF16)
+        assert torch.equal(got.q, want_q), what
+        assert all(torch.equal(x, y) for x, y in zip(cache, rows) if x is not None), what
+
+
 # ---- gather ------------------------------------------------------------------------------
 @pytest.mark.parametrize("kv", [F32, BF16, F16, 4])
 @pytest.mark.parametrize("lens,hk,d,page,rows", [([0, 1, 16, 17, 50], 3, 64, 16, 50), ([100, 33], 1, 128, 48, 120), ([70], 2, 64, 64, 31)])
