@@ -62,30 +62,66 @@ struct Share {
 // Blocks with all keys of a row tile: those of a sequence stand from a number on that its first token alone tells, with room
 // for as many as it can have, so that a wave finds its own in a search by 64 starts.  (By all sequences' row tiles, a lane a
 // sequence, 64 at a time: 2,048 tokens over 200 .. 499 rows 778 us for 518, 16,384 over 64 rows 11,540 for 730.)
+//
+// Where a block stands for several tokens: the sequence of block `place`, or (TOKEN) of token `place`, its first block and blocks
+// (b = -1: none).  A sequence has its blocks if it has its tokens (owner_of) and all blocks lead to it too.
+template <int ROWS, bool TOKEN>
+__device__ __forceinline__ Owner blocks_of(const Args &p, int place) {
+  const PagedAttn &a = p.a;
+  const int lane = threadIdx.x & 63;
+  auto keys = [&](int start, int b) { return make_int2(start, min(max(start, 0), a.tokens) * p.group / ROWS + b); };
+  const Way w = way_to<!TOKEN>(a.batch, place, [&](int b) { return keys(a.starts[b], b); });
+  const bool in = lane < w.n;
+  const int start = in ? a.starts[w.b0 + lane] : 0, end = in ? a.starts[w.b0 + lane + 1] : 0, block = keys(start, w.b0 + lane).y;
+  const bool has = start >= 0 && end > start && end <= a.tokens;
+  const int n = has ? ((end - start) * p.group + ROWS - 1) / ROWS : 0;
+  // (the first one: blocks of a sequence that starts behind all earlier ones' ends stand behind theirs)
+  const uint64_t holds = __ballot(TOKEN ? has && start <= place && place < end : block <= place && place < block + n);
+  if (holds == 0) return Owner{-1, 0, 0};
+  const int i = __builtin_ctzll(holds), first = __builtin_amdgcn_readlane(start, i), stop = __builtin_amdgcn_readlane(end, i);
+  const Owner of{w.b0 + i, __builtin_amdgcn_readlane(block, i), __builtin_amdgcn_readlane(n, i)};
+  if (__ballot(has && lane < i && end > first) != 0 || !w.leads_x(first, stop - 1) || !w.leads_y(of.first, of.first + of.n - 1)) return Owner{-1, 0, 0};
+  return of;
+}
 template <int ROWS>
 __device__ __forceinline__ Share whole_of(const Args &p, int index) {
   const PagedAttn &a = p.a;
-  const int lane = threadIdx.x & 63;
-  auto first_of = [&](int b) {
-    const int token = min(max(a.starts[b], 0), a.tokens);
-    return p.per_token > 0 ? token * p.per_token : token * p.group / ROWS + b;
-  };
-  int b = 0, n = a.batch;
-  for (bool any = false; n > 1 || !any; any = true) {
-    const int step = (n + 63) >> 6, at = lane * step;
-    const uint64_t in = __ballot(at < n && first_of(b + min(at, n - 1)) <= index);
-    if (in == 0) return Share{0, 0, 0, 0, 0};
-    const int i = 63 - __builtin_clzll(in);
-    b += i * step, n = min(step, n - i * step);
+  Owner of;  // (its blocks)
+  if (p.per_token > 0) {
+    of = owner_of(a.starts, a.batch, a.tokens, p.per_token == 1 ? index : index / p.per_token);
+    of.first *= p.per_token, of.n = (of.n * p.group + ROWS - 1) / ROWS;
+  } else {
+    of = blocks_of<ROWS, false>(p, index);
   }
-  b = __builtin_amdgcn_readfirstlane(b);
-  const int start = uniform_load(a.starts + b);
-  const Span span = span_of(start, uniform_load(a.starts + b + 1), a.tokens);
-  const int tiles = (span.n * p.group + ROWS - 1) / ROWS, token = min(max(start, 0), a.tokens);
-  const int local = index - (p.per_token > 0 ? token * p.per_token : token * p.group / ROWS + b);
-  if (local >= tiles) return Share{0, 0, 0, 0, 0};
-  return Share{b, tiles - 1 - local, 1, 0, 1 << 30};
+  const int local = index - of.first;
+  if (of.b < 0 || local >= of.n) return Share{0, 0, 0, 0, 0};
+  return Share{of.b, of.n - 1 - local, 1, 0, 1 << 30};
 }
+
+// The number of tokens of sequence b0 + lane: as owner_of has it, but of all sequences, 64 after the other.  reach: the furthest
+// end of those before.
+__device__ __forceinline__ int tokens_of(const PagedAttn &a, int b0, int &reach) {
+  const int lane = threadIdx.x & 63;
+  const bool in = b0 + lane < a.batch;
+  const int start = in ? a.starts[b0 + lane] : 0, end = in ? a.starts[b0 + lane + 1] : 0;
+  const bool rises = start >= 0 && end >= start && end <= a.tokens, has = rises && end > start;
+  int before = reach;  // the furthest end in front of the lane's sequence
+  if (__ballot(!rises) == 0) {  // (each starts where the one in front of it ends)
+    reach = max(reach, __builtin_amdgcn_readlane(end, min(a.batch - b0, 64) - 1));
+  } else {
+    int to = has ? end : 0;
+#pragma unroll
+    for (int step = 1; step < 64; step *= 2) {
+      const int up = __shfl_up(to, step, 64);
+      if (lane >= step) to = max(to, up);
+    }
+    const int up = __shfl_up(to, 1, 64);
+    before = lane > 0 ? max(reach, up) : reach;
+    reach = max(reach, __builtin_amdgcn_readlane(to, 63));
+  }
+  return has && start >= before ? end - start : 0;
+}
+
 // Blocks that share the keys: every share has the same size, the smallest one with which `blocks` are enough.  Found by
 // every wave from the starts and lengths, a lane a sequence.
 template <int ROWS, int KT>
@@ -93,15 +129,15 @@ __device__ __forceinline__ Share share_of(const Args &p, int index, int hk) {
   if (p.parts == 0) return whole_of<ROWS>(p, index);
   const PagedAttn &a = p.a;
   const int lane = threadIdx.x & 63;
-  // (the first block of all says for every sequence where its shares are; where starts fall and sequences have more rows than
-  // there are tokens, those that have no blocks any more are left out)
+  // (the first block of all says for every sequence where its shares are)
   const bool tells = index == 0 && hk == 0;
   // row tiles of a sequence, and the units of keys that one of them sees at most
-  auto count = [&](int b, int &tiles, int &units) {
-    tiles = 0, units = 0;
-    if (b >= a.batch) return;
-    const Span span = span_of(a.starts[b], a.starts[b + 1], a.tokens);
-    const int len = a.lengths[b], rows = span.n * p.group;
+  // (those of the first 64 once for all turns)
+  int reach = 0;
+  const int tokens0 = tokens_of(a, 0, reach), reach0 = reach, len0 = a.lengths[min(lane, a.batch - 1)];
+  auto count = [&](int b0, int &tiles, int &units) {
+    if (b0 == 0) reach = reach0;
+    const int rows = (b0 == 0 ? tokens0 : tokens_of(a, b0, reach)) * p.group, len = b0 == 0 ? len0 : a.lengths[min(b0 + lane, a.batch - 1)];
     tiles = (rows + ROWS - 1) / ROWS;
     int seen = len < 0 || len > a.max_rows ? 1 : max(len, 1);
     if (a.window > 0) seen = (int)min((int64_t)seen, (int64_t)a.window + min(a.sinks, a.max_rows) + (ROWS - 1) / p.group + 1 + 2 * KT);
@@ -110,7 +146,7 @@ __device__ __forceinline__ Share share_of(const Args &p, int index, int hk) {
   float total = 0.0f, longest = 0.0f;
   for (int b0 = 0; b0 < a.batch; b0 += 64) {
     int tiles, units;
-    count(b0 + lane, tiles, units);
+    count(b0, tiles, units);
     total += (float)tiles * units, longest = fmaxf(longest, units);
   }
   total = wave_sum(total), longest = wave_max(longest);
@@ -120,7 +156,7 @@ __device__ __forceinline__ Share share_of(const Args &p, int index, int hk) {
     float blocks = 0.0f;
     for (int b0 = 0; b0 < a.batch; b0 += 64) {
       int tiles, units;
-      count(b0 + lane, tiles, units);
+      count(b0, tiles, units);
       blocks += (float)tiles * ((units + size - 1) / size);
     }
     blocks = wave_sum(blocks);
@@ -133,7 +169,7 @@ __device__ __forceinline__ Share share_of(const Args &p, int index, int hk) {
   int before = 0;
   for (int b0 = 0; b0 < a.batch && (share.n == 0 || tells); b0 += 64) {
     int tiles, units;
-    count(b0 + lane, tiles, units);
+    count(b0, tiles, units);
     const int each = (int)(((int64_t)units + size - 1) / size), own = tiles * each;
     int to = own;  // (counted to one more than there are blocks)
 #pragma unroll
@@ -153,6 +189,7 @@ __device__ __forceinline__ Share share_of(const Args &p, int index, int hk) {
     }
     before = min(before + __builtin_amdgcn_readlane(to, 63), p.blocks + 1);
   }
+  if (a.batch > 64 && share.n > 0 && owner_of(a.starts, a.batch, a.tokens, uniform_load(a.starts + share.b)).b != share.b) share.n = 0;
   return share;
 }
 
@@ -469,18 +506,36 @@ struct Rows4 {
   }
 };
 
-// Tokens in front of the first sequence (x) and from y on belong to none: their rows are zeros, which all blocks write.
-__device__ __forceinline__ int2 rest_of(const PagedAttn &a) {
-  const int front = min(max(uniform_load(a.starts), 0), a.tokens);
-  return make_int2(front, min(max(uniform_load(a.starts + a.batch), front), a.tokens));
-}
-template <int D, class TQ>
-__device__ __forceinline__ void clear_rest(const PagedAttn &a, int2 rest) {
-  const int64_t n = (int64_t)(rest.x + a.tokens - rest.y) * a.H * (D / 4);
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
-    const int d = (int)(i % (D / 4)) * 4, head = (int)(i / (D / 4) % a.H), k = (int)(i / (D / 4) / a.H);
-    const int token = k < rest.x ? k : rest.y + k - rest.x;
+// Rows of tokens that belong to no sequence are zeros.  Blocks that share keys leave them to the joining kernel; others write them
+// where they are done: of up to 64 sequences whose starts rise the tokens in front of the first one and behind the last; else
+// each token is looked at, a wave a token.
+template <int D, class TQ, int ROWS>
+__device__ __forceinline__ void clear_rest(const Args &p) {
+  const PagedAttn &a = p.a;
+  if (p.parts > 0) return;
+  const int per = a.H * (D / 4);
+  auto clear = [&](int token, int at) {
+    const int d = at % (D / 4) * 4, head = at / (D / 4);
     store4<TQ>(static_cast<char *>(a.out) + (token * a.o_t + head * a.o_h + d) * TQ::kBytes, 0.0f, 0.0f, 0.0f, 0.0f);
+  };
+  const int lane = threadIdx.x & 63, b = min(lane, a.batch - 1);
+  if (a.batch <= 64) {
+    const int start = a.starts[b], end = a.starts[b + 1];
+    if (__ballot(start < 0 || end < start || end > a.tokens) == 0) {
+      const int front = __builtin_amdgcn_readlane(start, 0), back = __builtin_amdgcn_readlane(end, 63);
+      const int64_t n = (int64_t)(front + a.tokens - back) * per;
+      for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
+        const int k = (int)(i / per);
+        clear(k < front ? k : back + k - front, (int)(i - (int64_t)k * per));
+      }
+      return;
+    }
+  }
+  const int waves = gridDim.x * 4;
+  for (int token = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)); token < a.tokens; token += waves) {
+    const Owner of = p.per_token > 0 ? owner_of(a.starts, a.batch, a.tokens, token) : blocks_of<ROWS, true>(p, token);
+    if (of.b >= 0) continue;
+    for (int at = lane; at < per; at += 64) clear(token, at);
   }
 }
 
@@ -574,9 +629,8 @@ __global__ __launch_bounds__(256, (D == 128 && TKV::kBytes == 4 ? 1 : 2)) void p
   const PagedAttn &a = p.a;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
   const int hk = blockIdx.x % a.pages.Hk, index = blockIdx.x / a.pages.Hk;
-  const int2 rest = rest_of(a);
   const Share share = share_of<kRows, kTileKeys>(p, index, hk);
-  if (share.n == 0) return clear_rest<D, TQ>(a, rest);
+  if (share.n == 0) return clear_rest<D, TQ, kRows>(p);
   const Seq seq = seq_of<kRows>(p, share);
   const Tiles<kTileKeys> tiles(a, seq.p0, seq.p1);
   const int first = min(share.first, tiles.n), end = min(share.end, tiles.n);
@@ -660,7 +714,7 @@ __global__ __launch_bounds__(256, (D == 128 && TKV::kBytes == 4 ? 1 : 2)) void p
   join_waves<D, TQ, kRows>(p, share, seq, index, hk, first < end, so, sm, sl, [&](float *y, int own, int d) {
     if (odd_any) odd_values<D, TKV>(y, p, seq, tiles, first, end, table, hk, own, d);
   });
-  clear_rest<D, TQ>(a, rest);
+  clear_rest<D, TQ, kRows>(p);
 }
 
 // ---- 4 bits ----
@@ -712,9 +766,8 @@ __global__ __launch_bounds__(256, (RT == 2 ? 2 : kCodeBlocks<D, TQ>)) void paged
   const Pages &pg = a.pages;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
   const int hk = blockIdx.x % pg.Hk, index = blockIdx.x / pg.Hk;
-  const int2 rest = rest_of(a);
   const Share share = share_of<kRows, kTileKeys>(p, index, hk);
-  if (share.n == 0) return clear_rest<D, TQ>(a, rest);
+  if (share.n == 0) return clear_rest<D, TQ, kRows>(p);
   const Seq seq = seq_of<kRows>(p, share);
   const Tiles<kTileKeys> tiles(a, seq.p0, seq.p1);
   const int first = min(share.first, tiles.n), end = min(share.end, tiles.n);
@@ -871,7 +924,7 @@ __global__ __launch_bounds__(256, (RT == 2 ? 2 : kCodeBlocks<D, TQ>)) void paged
   }
   __syncthreads();
   join_waves<D, TQ, kRows>(p, share, seq, index, hk, first < end, join.so, join.sm, join.sl, [](float *, int, int) {});
-  clear_rest<D, TQ>(a, rest);
+  clear_rest<D, TQ, kRows>(p);
 }
 
 // ---- many query rows ----
@@ -934,9 +987,8 @@ __global__ __launch_bounds__(256, (TQ::kBytes == 4 ? (D == 64 ? 2 : 1) : D == 64
   const PagedAttn &a = p.a;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 31, h = lane >> 5;
   const int hk = blockIdx.x % a.pages.Hk, index = blockIdx.x / a.pages.Hk;
-  const int2 rest = rest_of(a);
   const Share share = share_of<kLongRows, KT>(p, index, hk);
-  if (share.n == 0) return clear_rest<D, TQ>(a, rest);
+  if (share.n == 0) return clear_rest<D, TQ, kLongRows>(p);
   const Seq seq = seq_of<kLongRows>(p, share);
   const Tiles<KT> tiles(a, seq.p0, seq.p1);
   const int first = min(share.first, tiles.n), end = min(share.end, tiles.n);
@@ -1173,7 +1225,7 @@ __global__ __launch_bounds__(256, (TQ::kBytes == 4 ? (D == 64 ? 2 : 1) : D == 64
         put4<D, TQ, kLongRows>(p, share, seq, index, hk, row, e, y, m, l, pos >= 0, first < end);
       }
   }
-  clear_rest<D, TQ>(a, rest);
+  clear_rest<D, TQ, kLongRows>(p);
 }
 
 // Joins the shares' results of a row: a wave a row, D / 4 lanes with four elements each for every fourth (D 128: second)
@@ -1186,14 +1238,15 @@ __global__ __launch_bounds__(256) void paged_join_kernel(Args p) {
   const int item = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
   if (item >= a.tokens * a.H) return;
   const int token = item / a.H, head = item - token * a.H, hk = head / p.group;
-  const int b = sequence_of(a.starts, a.batch, token);
-  if (b < 0) return;
-  const Span span = span_of(uniform_load(a.starts + b), uniform_load(a.starts + b + 1), a.tokens);
-  if (token < span.first || token >= span.first + span.n) return;
-  const int2 dealt = p.dealt[b];
+  const Owner of = owner_of(a.starts, a.batch, a.tokens, token);
+  const int2 dealt = of.b < 0 ? make_int2(0, 0) : p.dealt[of.b];
   const int S = dealt.y;
-  if (S <= 1) return;  // (that block has written the row; 0: a sequence that was left out)
-  const int r = (token - span.first) * p.group + head - hk * p.group, tile = r / ROWS, tiles = (span.n * p.group + ROWS - 1) / ROWS;
+  char *out = static_cast<char *>(a.out) + (token * a.o_t + head * a.o_h + d) * TQ::kBytes;
+  if (S <= 1) {  // (1: that block has written the row; 0: the token belongs to no sequence)
+    if (S == 0 && s0 == 0) store4<TQ>(out, 0.0f, 0.0f, 0.0f, 0.0f);
+    return;
+  }
+  const int r = (token - of.first) * p.group + head - hk * p.group, tile = r / ROWS, tiles = (of.n * p.group + ROWS - 1) / ROWS;
   const int index = dealt.x + (tiles - 1 - tile) * S;
   const size_t at = ((size_t)hk * p.parts + index) * ROWS + (r - tile * ROWS);
   const float *part = a.part + at * D + d;
@@ -1226,7 +1279,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(Args p) {
   const float inv = 1.0f / sum;
 #pragma unroll
   for (int e = 0; e < 4; e++) x[e] = none ? 0.0f : x[e] * inv;
-  store4<TQ>(static_cast<char *>(a.out) + (token * a.o_t + head * a.o_h + d) * TQ::kBytes, x[0], x[1], x[2], x[3]);
+  store4<TQ>(out, x[0], x[1], x[2], x[3]);
 }
 
 int code_blocks(int D, int type) {

@@ -12,22 +12,6 @@ __device__ __forceinline__ int32_t uniform_load(const int32_t *p) {
   return *(Const *)(uintptr_t)p;
 }
 
-// The sequence b that holds a token, the same in all lanes of the wave: the last one that starts at or in front of it, found
-// 64 starts at a time; -1 for a token in front of the first sequence.  Empty sequences start where the next one does.
-__device__ __forceinline__ int sequence_of(const int32_t *starts, int batch, int token) {
-  const int lane = threadIdx.x & 63;
-  int b = 0, n = batch;
-  bool any = false;
-  while (n > 1 || !any) {
-    const int step = (n + 63) >> 6, at = lane * step;
-    const uint64_t in = __ballot(at < n && starts[b + min(at, n - 1)] <= token);
-    if (in == 0) return -1;
-    const int i = 63 - __builtin_clzll(in);
-    b += i * step, n = min(step, n - i * step), any = true;
-  }
-  return __builtin_amdgcn_readfirstlane(b);
-}
-
 // Tokens first .. first + n - 1 of a sequence; n = 0 for starts that do not rise or leave the tensors.
 struct Span {
   int first, n;
@@ -37,32 +21,38 @@ __device__ __forceinline__ Span span_of(int start, int end, int tokens) {
   return Span{ok ? start : 0, ok ? end - start : 0};
 }
 
-// What a search over more than 64 sequences found on its way: of each level the key it went by (the largest), and the keys of
-// the lanes behind that.
+// What a search over more than 64 sequences found on its way.  A sequence has two keys, its first token (x) and another (y); of each
+// level those it went by (the largest), and those of the lanes behind them.
 struct Way {
-  int b0, n;  // the sequences left, 64 at most; n = 0: `at` lies in front of them all
-  int own, later[2];
-  // whether every place from `first` to `last` leads here too: places lead to rising sequences, whatever the keys are
-  __device__ __forceinline__ bool leads(int first, int last) const {
-    return own <= first && __ballot(later[0] <= last || later[1] <= last) == 0;
+  int b0, n;  // the sequences left, 64 at most; n = 0: the place lies in front of them all
+  int2 own, later[2];
+  // Whether all places from `first` to `last` lead here too: they lead to rising sequences, whatever the keys are.
+  __device__ __forceinline__ bool leads_x(int first, int last) const {
+    return own.x <= first && __ballot(later[0].x <= last || later[1].x <= last) == 0;
+  }
+  __device__ __forceinline__ bool leads_y(int first, int last) const {
+    return own.y <= first && __ballot(later[0].y <= last || later[1].y <= last) == 0;
   }
 };
-// The group of sequences that place `at` leads to: at each of two levels at most the last of 64 whose key is not above it.
-template <class F>
-__device__ __forceinline__ Way way_to(int batch, int at, F key) {
+// The group of sequences that a place leads to: at each of two levels at most the last of 64 whose key (BY_Y: y) is not above it.
+template <bool BY_Y, class F>
+__device__ __forceinline__ Way way_to(int batch, int place, F keys) {
+  constexpr int kMost = 0x7fffffff;
   const int lane = threadIdx.x & 63;
-  Way w{0, batch, -0x7fffffff - 1, {0x7fffffff, 0x7fffffff}};
+  Way w{0, batch, make_int2(-kMost, -kMost), {make_int2(kMost, kMost), make_int2(kMost, kMost)}};
 #pragma unroll
   for (int level = 0; level < 2; level++) {  // (65,535 sequences: groups of 1,024, of 16)
     if (w.n <= 64) break;
-    const int step = (w.n + 63) >> 6, k = lane * step < w.n ? key(w.b0 + lane * step) : 0x7fffffff;
-    const uint64_t in = __ballot(k <= at);
+    const int step = (w.n + 63) >> 6;
+    const int2 k = lane * step < w.n ? keys(w.b0 + lane * step) : make_int2(kMost, kMost);
+    const uint64_t in = __ballot((BY_Y ? k.y : k.x) <= place);
     if (in == 0) {
       w.n = 0;
       break;
     }
     const int i = 63 - __builtin_clzll(in);
-    w.own = max(w.own, __builtin_amdgcn_readlane(k, i)), w.later[level] = lane > i ? k : 0x7fffffff;
+    w.own.x = max(w.own.x, __builtin_amdgcn_readlane(k.x, i)), w.own.y = max(w.own.y, __builtin_amdgcn_readlane(k.y, i));
+    w.later[level] = lane > i ? k : make_int2(kMost, kMost);
     w.b0 = __builtin_amdgcn_readfirstlane(w.b0 + i * step), w.n = min(step, w.n - i * step);
   }
   return w;
@@ -77,14 +67,14 @@ struct Owner {
 };
 __device__ __forceinline__ Owner owner_of(const int32_t *starts, int batch, int tokens, int token) {
   const int lane = threadIdx.x & 63;
-  const Way w = way_to(batch, token, [&](int b) { return starts[b]; });
+  const Way w = way_to<false>(batch, token, [&](int b) { return make_int2(starts[b], 0); });
   const bool in = lane < w.n;
   const int start = in ? starts[w.b0 + lane] : 0, end = in ? starts[w.b0 + lane + 1] : 0;
   const bool has = start >= 0 && end > start && end <= tokens;
   const uint64_t holds = __ballot(has && start <= token && token < end);
   if (holds == 0) return Owner{-1, 0, 0};
   const int i = __builtin_ctzll(holds), first = __builtin_amdgcn_readlane(start, i), stop = __builtin_amdgcn_readlane(end, i);
-  if (__ballot(has && lane < i && end > first) != 0 || !w.leads(first, stop - 1)) return Owner{-1, 0, 0};
+  if (__ballot(has && lane < i && end > first) != 0 || !w.leads_x(first, stop - 1)) return Owner{-1, 0, 0};
   return Owner{w.b0 + i, first, stop - first};
 }
 

@@ -455,7 +455,8 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, starts: torch.Tensor, le
              with one launch
     out      where to write (default: a new tensor)
 
-    A token at a position below 0 (more tokens than rows) gets zeros, as do tokens that belong to no sequence.  A length that is
+    A token at a position below 0 (more tokens than rows) gets zeros, as do tokens that belong to no sequence (starts that do not
+    rise: as paged_append has it).  A length that is
     negative or too long, and a row in sight whose table entry is no page of the cache, gives NaN.  Returns out
     [tokens][heads][dim] in q's type."""
     sq = _tensor(q, "q", 3, last=True)

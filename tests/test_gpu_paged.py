@@ -845,6 +845,35 @@ def bad_starts(s):
     yield "nothing fits", [0, s[-1] + 50] + [s[-1]] * (len(s) - 2)
 
 
+# blocks of a token's rows, of several tokens' rows, of many rows over shared tiles; and keys shared by blocks
+ENDS = [([60, 33, 70, 16, 100, 45, 8], [1] * 7, 4, 2, 64), ([50] * 5 + [200], [4, 4, 4, 4, 20, 3], 4, 2, 64),
+        ([220, 180, 40, 200, 300, 90], [60, 50, 10, 40, 50, 9], 8, 2, 64), ([3000] * 6, [2, 1, 3, 1, 2, 1], 4, 2, 128),
+        ([2600] * 6, [40, 30, 50, 20, 40, 39], 8, 2, 64)]
+
+
+@pytest.mark.parametrize("types", [(F32, BF16), (BF16, BF16), (F32, F32), (F16, 4)])
+@pytest.mark.parametrize("lens,news,h,hk,d", ENDS)
+def test_attention_of_tokens_without_a_sequence(ops, types, lens, news, h, hk, d):
+    """Starts that do not rise: tokens of no sequence get zeros, those of the others their results, every time."""
+    say(f"[gpu] paged attention bad starts {types} {lens} {news}")
+    s = Seqs(ops, types, lens, news, h, hk, d, 16, seed=41)
+    good = s.starts_list
+    for what, starts in bad_starts(good):
+        say("  ", what, starts)
+        spans = spans_of(starts, good[-1])
+        s.starts_list, s.news = [x[0] if x else 0 for x in spans], [x[1] if x else 0 for x in spans]
+        ref, tol = s.ref()
+        none = torch.ones(good[-1], dtype=torch.bool, device="cuda")
+        for i, n in zip(s.starts_list, s.news):
+            none[i:i + n] = False
+        assert (ref[none] == 0).all()
+        for _ in range(3):
+            out = torch.full_like(s.q, 7.0)
+            ops.paged_attention(s.q, s.cache, ints(starts), s.lengths, s.table, out=out)
+            assert (out[none] == 0).all(), what
+            check(out, ref, tol, what)
+
+
 @pytest.mark.parametrize("types", [(F32, BF16), (BF16, 4)])
 def test_append_of_tokens_without_a_sequence(ops, types):
     """The same of appended rows: a sequence's are all there, or none and its new length is -1."""
@@ -879,6 +908,60 @@ def test_append_of_tokens_without_a_sequence(ops, types):
                     rows[which][table[i][at // 16].long(), :, at % 16] = src[own].to(BF16)
         assert torch.equal(got.q, want_q), what
         assert all(torch.equal(x, y) for x, y in zip(cache, rows) if x is not None), what
+
+
+@pytest.mark.parametrize("types", [(F32, BF16), (F16, 4)])
+@pytest.mark.parametrize("batch,news,long", [(70, 1, 0), (70, 3, 2500), (200, 40, 0), (100, 300, 0), (500, 2, 0), (5000, 2, 0), (5000, 9, 0)])
+@pytest.mark.parametrize("hk", [1, 8])
+def test_bad_starts_of_many_sequences(ops, types, batch, news, long, hk):
+    """More sequences than a wave has lanes: what is wrong about some starts may leave neighbours without tokens, but each sequence has all
+    its rows and results, or a new length of -1 and zeros."""
+    say(f"[gpu] paged bad starts of many sequences {types} {batch} {news} {long} {hk}")
+    q_type, kv = types
+    gt = torch.Generator().manual_seed(batch + news)
+    count = torch.randint(0, news + 1, (batch,), generator=gt)
+    good = [0] + count.cumsum(0).tolist()
+    n, d, wide = good[-1], 64, -(-news // 16) + -(-long // 16)
+    cache = ops.paged_cache(batch * wide, hk, 16, d, BF16, bits=kv if kv == 4 else 16)
+    table, lens = torch.arange(batch * wide, dtype=torch.int32).view(batch, wide).cuda(), ints([long] * batch)
+    num = torch.arange(n) % 13 + 1.0                                 # a token's value in all its elements: exact in every type
+    v = num.to(q_type).cuda().view(n, 1, 1).expand(n, hk, d).contiguous()
+    k, q = torch.zeros_like(v), torch.ones_like(v)
+    for trial in range(12):
+        starts = list(good)
+        for _ in range(trial % 4):
+            at, what = (int(x) for x in torch.randint(0, 10 ** 6, (2,), generator=gt))
+            starts[at % (batch + 1)] = [10 ** 6, -1, 0, n, what % (n + 1)][what % 5]
+        say("  ", trial, [(i, x) for i, (x, y) in enumerate(zip(starts, good)) if x != y])
+        for t in cache:
+            if t is not None:
+                t.zero_()
+        r = ops.paged_append(cache, k, v, ints(starts), lens, table, q=q)
+        owned, want, long_ones = torch.zeros(n, dtype=torch.bool), torch.zeros(batch, wide * 16), torch.zeros(n, dtype=torch.bool)
+        for b, (i, j, m) in enumerate(zip(starts, starts[1:], r.lengths.tolist())):
+            assert m == -1 or (0 <= i <= j <= n and m == long + j - i)
+            if 0 <= i <= j <= n and long + j - i > wide * 16:  # (no room: none is written, queries are NaN)
+                long_ones[i:j] = True
+            if m > long:
+                assert not owned[i:j].any()
+                owned[i:j], want[b, long:m] = True, num[i:j]
+        assert owned.all() or trial % 4
+        rows = ops.paged_gather(cache, ints([wide * 16] * batch), table, wide * 16, dtype=None if kv != 4 else q_type)[1]
+        assert (rows == want.cuda().view(batch, 1, -1, 1)).all()
+        owned, odd = owned.cuda(), torch.isnan(r.q)
+        assert ((r.q == owned.view(n, 1, 1)) | odd & long_ones.cuda().view(n, 1, 1)).all() and not odd[owned].any()
+        # each token over its own row alone, so that results are the values; and over all rows
+        held = r.lengths.clamp(min=0)
+        for window in (1, 0):
+            first = None
+            for _ in range(2):
+                out = torch.full_like(q, 7.0)
+                ops.paged_attention(q, cache, ints(starts), held, table, window=window, out=out)
+                zero = (out == 0).flatten(1).all(1)
+                fits = ((out.float() - v.float()).abs() < 1e-2 if window else (out > 0) & (out < 13.5)).flatten(1).all(1)
+                assert (zero | fits).all() and zero[~owned].all() and (fits.all() or trial % 4)
+                assert first is None or torch.equal(out, first)
+                first = out
 
 
 # ---- gather ------------------------------------------------------------------------------
