@@ -451,7 +451,7 @@ typedef struct itts_pages {
 } itts_pages;
 
 /* Appends tokens' keys and values k, v [n_tokens][n_kv_head][head_dim] to their sequences: token i of sequence b becomes row
- * lengths[b] + i; new_lengths[b] = lengths[b] + its tokens.  With `rotation` [n_positions][n_rotated], each row n_rotated / 2
+ * lengths[b] + i; new_lengths[b] = lengths[b] + its tokens.  With `rotation` [n_positions >= 1][n_rotated], each row n_rotated / 2
  * cosines, then the sines of the same angles, the first n_rotated elements of keys turn by those of the token's position
  * (positions[token], or its row where positions is NULL): (x, y) -> (x cos - y sin, y cos + x sin), pairs being elements
  * i and i + n_rotated / 2, or with `interleaved` 2 i and 2 i + 1.  q [n_tokens][n_head][head_dim] (n_head 0: none) turns the same

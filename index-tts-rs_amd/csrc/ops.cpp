@@ -277,7 +277,8 @@ itts_status append_args(const itts_paged_append_args *a, PagedAppend *o) {
   if (a->rotation) {
     rot = a->n_rotated;
     if (rot < 16 || rot > g.D || rot % 16) return fail(ITTS_E_VALIDATION, "n_rotated: must be a multiple of 16 in 16..=%d, got %d", g.D, rot);
-    if (a->n_positions < 0) return fail(ITTS_E_VALIDATION, "n_positions: must be >= 0, got %d", a->n_positions);
+    // (positions that are not in the table read its first row)
+    if (a->n_positions < 1) return fail(ITTS_E_VALIDATION, "n_positions: a rotation needs one at least, got %d", a->n_positions);
     if (!row_stride(a->rotation_row, a->n_positions, 4) || !aligned16(a->rotation))
       return fail(ITTS_E_VALIDATION, "rotation: rows must start at multiples of 16 bytes");
   }
@@ -447,7 +448,7 @@ itts_status itts_paged_append(const itts_paged_append_args *args, void *stream) 
   if (itts_status st = check_device(
           dev, stream, {{a.pages.k, "pages.k"}, {a.pages.v, "pages.v"}, {a.pages.type == kOpI4 ? a.pages.kp : nullptr, "pages.k_params"},
                         {a.pages.type == kOpI4 ? a.pages.vp : nullptr, "pages.v_params"}, {any ? a.k : nullptr, "k"}, {any ? a.v : nullptr, "v"},
-                        {turn ? a.q : nullptr, "q"}, {turn ? a.q_out : nullptr, "q_out"}, {a.n_positions ? a.rotation : nullptr, "rotation"},
+                        {turn ? a.q : nullptr, "q"}, {turn ? a.q_out : nullptr, "q_out"}, {a.rotation, "rotation"},
                         {a.starts, "starts"}, {a.lengths, "lengths"}, {a.n_table ? a.table : nullptr, "table"},
                         {any ? a.positions : nullptr, "positions"}, {a.new_lengths, "new_lengths"}}))
     return st;

@@ -176,3 +176,11 @@ def test_cache_memory():
     assert c.k.shape == (3, 4, 16, 64) and c.k.dtype == torch.uint8 and c.v_params.shape == (3, 4, 16, 2, 2)
     c = ops.paged_cache(3, 4, 16, 128, torch.float32, bits=32, device="cpu")
     assert c.k.shape == (3, 4, 16, 128) and c.k.dtype == torch.float32 and c.k_params is None
+
+
+def test_a_rotation_has_positions():
+    """Without one a token's row of the table, which is read before anything says that its position is not there, would lie outside it."""
+    with pytest.raises(H.ValidationError) as e:
+        call(append, append(n_positions=0))
+    assert e.value.message.startswith("n_positions"), e.value.message
+    assert takes(append, n_positions=0, rotation=None) and takes(append, n_positions=1)
