@@ -8,6 +8,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
+#include <initializer_list>
 
 #include "../../include/itts_hip.h"
 #include "kernels.h"
@@ -128,6 +129,39 @@ bool rows_overlap(std::array<Axis, N> axes, int64_t row) {
     if (i + 1 >= N) return false;
     d[i]++;
   }
+}
+
+// Whether rows of `row` bytes at x and at multiples of a tensor's strides from there meet rows of another one at y.  The axis with
+// the longest stride goes first, index by index (of an axis of both: difference by difference) as far as what is left
+// can meet at all; more than a million steps count as meeting.
+struct Rows {
+  Axis axes[3];  // bytes; the longest stride last
+  int n;
+  int64_t reach;  // bytes from the first row's start to the last one's end
+};
+Rows rows_of(std::initializer_list<Axis> axes, int size, int64_t row) {
+  Rows r{{}, 0, row};
+  for (const Axis &x : axes)
+    if (x.extent > 1 && x.stride > 0) r.axes[r.n++] = Axis{x.stride * size, x.extent}, r.reach += (x.extent - 1) * x.stride * size;
+  std::sort(r.axes, r.axes + r.n, [](const Axis &x, const Axis &y) { return x.stride < y.stride; });
+  return r;
+}
+bool rows_meet(int64_t apart, Rows a, Rows b, int *left) {  // apart: y - x
+  if (apart >= a.reach || -apart >= b.reach) return false;
+  if ((a.n == 0 && b.n == 0) || --*left < 0) return true;
+  const int64_t in_a = a.n > 0 ? a.axes[a.n - 1].stride : 0, in_b = b.n > 0 ? b.axes[b.n - 1].stride : 0, step = std::max(in_a, in_b);
+  int64_t low = 0, high = 0;  // apart + step * (low .. high)
+  if (in_a == step) a.n--, low = 1 - a.axes[a.n].extent, a.reach -= (a.axes[a.n].extent - 1) * step;
+  if (in_b == step) b.n--, high = b.axes[b.n].extent - 1, b.reach -= (b.axes[b.n].extent - 1) * step;
+  // -b.reach < apart + step i < a.reach (one more at either end: quotients round towards 0)
+  low = std::max(low, (-b.reach - apart) / step - 1), high = std::min(high, (a.reach - apart) / step + 1);
+  for (int64_t i = low; i <= high; i++)
+    if (rows_meet(apart + step * i, a, b, left)) return true;
+  return false;
+}
+bool rows_meet(const void *x, const Rows &a, const void *y, const Rows &b) {
+  int left = 1000000;
+  return rows_meet(reinterpret_cast<intptr_t>(y) - reinterpret_cast<intptr_t>(x), a, b, &left);
 }
 
 itts_status tree_args(const itts_tree_attention_args *a, TreeAttn *o) {
@@ -539,11 +573,15 @@ itts_status itts_adjust_logits(const itts_adjust_logits_args *a, void *stream) {
     for (int64_t s : {a->logits_row, a->out_row, a->history_row, a->bias_tokens_row, a->bias_row, a->allowed_row})
       if (s < 0 || s > INT64_MAX / 16 / a->rows) return fail(ITTS_E_VALIDATION, "logits_row, out_row, history_row, bias_row, allowed_row: rows must ascend");
     if (a->out_row < a->vocab) return fail(ITTS_E_VALIDATION, "out: rows must not overlap");
-    if (a->logits == a->out && a->logits_row != a->out_row) return fail(ITTS_E_VALIDATION, "out: may be logits with the same stride alone");
   }
   if (a->rows == 0) return ITTS_OK;
   if (!a->logits || !a->out || (a->n_history && !a->history) || (a->n_bias && (!a->bias_tokens || !a->bias)))
     return fail(ITTS_E_VALIDATION, "logits, out, history, bias_tokens, bias: null");
+  // (a block reads what it has not written yet: its own tokens)
+  const int es = op_size(t);
+  if (!(a->logits == a->out && (a->rows == 1 || a->logits_row == a->out_row)) &&
+      rows_meet(a->logits, rows_of({{a->logits_row, a->rows}}, es, (int64_t)a->vocab * es), a->out, rows_of({{a->out_row, a->rows}}, es, (int64_t)a->vocab * es)))
+    return fail(ITTS_E_VALIDATION, "out: may be logits with the same stride, but must not share memory with them otherwise");
   int dev = 0, n_cu = 0;
   if (itts_status st = compute_units(&dev, &n_cu)) return st;
   if (itts_status st = check_device(

@@ -1100,6 +1100,20 @@ def test_adjust_odd_values(ops, dtype):
             ops.adjust_logits(x, **kw)
 
 
+def test_adjust_refuses_shifted_memory(ops):
+    """Out beside logits in their memory is fine, over them in other places is not."""
+    say("[gpu] adjust logits in shifted memory")
+    wide = randn(gen(3), 4, 2100)
+    x = wide[:, 3:2096]
+    for out in (wide[:, :2093], wide[:, 7:2100], wide.flatten()[2100 + 3:2100 + 3 + 3 * 2093].view(3, 2093)):
+        with pytest.raises(H.ValidationError, match="out: "):
+            ops.adjust_logits(x[:len(out)], out=out)
+    both = torch.cat([x, x], 1)
+    want = ops.adjust_logits(x, repetition=2.0, history=ints([[5, 9]]).expand(4, -1))
+    ops.adjust_logits(both[:, :2093], repetition=2.0, history=ints([[5, 9]]).expand(4, -1), out=both[:, 2093:])
+    assert torch.equal(both[:, 2093:], want) and torch.equal(both[:, :2093], x)
+
+
 # ---- together ----------------------------------------------------------------------------
 @pytest.mark.parametrize("types", [(F32, BF16), (BF16, 4)])
 def test_decoding_over_pages(ops, types):

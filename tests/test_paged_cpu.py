@@ -184,3 +184,20 @@ def test_a_rotation_has_positions():
         call(append, append(n_positions=0))
     assert e.value.message.startswith("n_positions"), e.value.message
     assert takes(append, n_positions=0, rotation=None) and takes(append, n_positions=1)
+
+
+@pytest.mark.parametrize("over,fine", [
+    (dict(out=P + 4), False), (dict(out=P - 4), False), (dict(out=P + 4 * 99), False), (dict(out=P + 4 * 100), False), (dict(out=P + 4 * 300), True),
+    (dict(out=P - 4 * 300), True), (dict(out=P, logits_row=200, out_row=200), True), (dict(out=P, logits_row=200), False),
+    (dict(out=P + 400, logits_row=200, out_row=200), True), (dict(out=P + 396, logits_row=200, out_row=200), False),
+    (dict(out=P + 404, logits_row=200, out_row=200), False), (dict(out=P, logits_row=0, out_row=100), False), (dict(out=P, rows=1, out_row=0), True),
+    (dict(out=P + 4, rows=1), False), (dict(out=P + 400, logits_row=0), True), (dict(out=P + 200, dtype=H.ITTS_BF16), False),
+    (dict(out=P + 600, dtype=H.ITTS_BF16), True)], ids=str)
+def test_adjusted_logits_in_the_memory_of_logits(over, fine):
+    """Rows of 100 logits, 400 bytes: in place with the same stride, beside each other, but not shifted against each other."""
+    if fine:
+        assert takes(adjust, **over)
+    else:
+        with pytest.raises(H.ValidationError) as e:
+            call(adjust, adjust(**over))
+        assert e.value.message.startswith("out: "), e.value.message
