@@ -538,8 +538,9 @@ itts_status itts_paged_gather(const itts_paged_gather_args *a, void *stream) {
   }
   if (a->batch == 0 || a->n_rows == 0) return ITTS_OK;
   if (!a->k || !a->v || !a->lengths || (a->n_table && !a->table)) return fail(ITTS_E_VALIDATION, "k, v, lengths, table: null");
-  if (a->k == a->v || rows_overlap<3>({{{ks[0], ext[0]}, {ks[1], ext[1]}, {ks[2], ext[2]}}}, g.D) ||
-      rows_overlap<3>({{{vs[0], ext[0]}, {vs[1], ext[1]}, {vs[2], ext[2]}}}, g.D))
+  auto rows = [&](const int64_t(&s)[3]) { return rows_of({{s[0], ext[0]}, {s[1], ext[1]}, {s[2], ext[2]}}, es, g.D * es); };
+  if (rows_overlap<3>({{{ks[0], ext[0]}, {ks[1], ext[1]}, {ks[2], ext[2]}}}, g.D) ||
+      rows_overlap<3>({{{vs[0], ext[0]}, {vs[1], ext[1]}, {vs[2], ext[2]}}}, g.D) || rows_meet(a->k, rows(ks), a->v, rows(vs)))
     return fail(ITTS_E_VALIDATION, "k, v: rows must not overlap");
   int dev = 0, n_cu = 0;
   if (itts_status st = compute_units(&dev, &n_cu)) return st;

@@ -1,6 +1,7 @@
 """Refusals of the operators over paged caches and on logits, without a GPU: wrong sizes, types, strides and alignments at the
 C entries, and wrong tensors at the Python ones."""
 import ctypes as C
+import random
 
 import pytest
 import torch
@@ -201,3 +202,40 @@ def test_adjusted_logits_in_the_memory_of_logits(over, fine):
         with pytest.raises(H.ValidationError) as e:
             call(adjust, adjust(**over))
         assert e.value.message.startswith("out: "), e.value.message
+
+
+def gathered(rng, es):
+    """Strides of [batch][heads][rows] rows of 64 elements: nested in any order, or rows of two axes that interleave, in some places
+    a little too close."""
+    ext, order, strides, at = [rng.randint(1, 3) for _ in range(3)], rng.sample(range(3), 3), [0, 0, 0], 64
+    for axis in order:
+        strides[axis] = at + rng.choice([0, 0, 8, 64, 96])
+        at = strides[axis] * rng.choice([ext[axis], ext[axis], 1, 2])
+    return ext, strides
+
+
+def taken(at, strides, ext, es):
+    """The pieces of 16 bytes of all rows, in their order."""
+    return [at // 16 + (b * strides[0] + h * strides[1] + r * strides[2]) * es // 16 + i
+            for b in range(ext[0]) for h in range(ext[1]) for r in range(ext[2]) for i in range(64 * es // 16)]
+
+
+@pytest.mark.parametrize("seed", range(400))
+def test_gathered_rows_that_meet(seed):
+    """Keys and values of any strides and distance: taken exactly where no two rows share memory."""
+    rng = random.Random(seed)
+    ext, ks = gathered(rng, 2)
+    vs = list(ks)
+    if rng.random() < 0.7:
+        rng2 = random.Random(seed + 10 ** 6)
+        _, vs = gathered(rng2, 2)
+    v = P + 16 * rng.randint(-600, 600)
+    pieces = taken(P, ks, ext, 2) + taken(v, vs, ext, 2)
+    over = dict(k=P, v=v, batch=ext[0], pages_n_kv_head=ext[1], n_rows=ext[2], k_batch=ks[0], k_head=ks[1], k_row=ks[2], v_batch=vs[0],
+                v_head=vs[1], v_row=vs[2])
+    if len(set(pieces)) == len(pieces):
+        assert takes(gather, **over)
+    else:
+        with pytest.raises(H.ValidationError) as e:
+            call(gather, gather(**over))
+        assert e.value.message.startswith("k, v: rows must not overlap"), e.value.message
