@@ -250,18 +250,18 @@ itts_status pages_args(const itts_pages &g, bool writes, Pages *o) {
                         (t == kOpI4 && (g.k_params_page * 2 > UINT32_MAX || g.v_params_page * 2 > UINT32_MAX))))
     return fail(ITTS_E_VALIDATION, "pages.k_page, v_page: pages must be less than 2^32 bytes apart");
   if (writes) {
+    auto rows = [&](const int64_t(&s)[3], int size, int n) { return rows_of({{s[0], ext[0]}, {s[1], ext[1]}, {s[2], ext[2]}}, size, (int64_t)n * size); };
     auto meet = [&](const int64_t(&a)[3], const int64_t(&b)[3], const void *x, const void *y, int size, int n) {
-      if (rows_overlap<3>({{{a[0], ext[0]}, {a[1], ext[1]}, {a[2], ext[2]}}}, n) || rows_overlap<3>({{{b[0], ext[0]}, {b[1], ext[1]}, {b[2], ext[2]}}}, n))
-        return true;
-      // Keys and values apart are one more axis where their strides are the same; else each lies outside the other's range, or
-      // they are taken for interleaved.
-      const int64_t apart = std::llabs(reinterpret_cast<intptr_t>(y) - reinterpret_cast<intptr_t>(x)) / size;
-      if (x == y) return true;
-      return a[0] == b[0] && a[1] == b[1] && a[2] == b[2] && apart < INT64_MAX / 16 &&
-             rows_overlap<4>({{{a[0], ext[0]}, {a[1], ext[1]}, {a[2], ext[2]}, {apart, 2}}}, n);
+      return rows_overlap<3>({{{a[0], ext[0]}, {a[1], ext[1]}, {a[2], ext[2]}}}, n) || rows_overlap<3>({{{b[0], ext[0]}, {b[1], ext[1]}, {b[2], ext[2]}}}, n) ||
+             rows_meet(x, rows(a, size, n), y, rows(b, size, n));
     };
     if (meet(ks, vs, g.k, g.v, es, row)) return fail(ITTS_E_VALIDATION, "pages.k, v: rows must not overlap");
-    if (t == kOpI4 && meet(kps, vps, g.k_params, g.v_params, 2, pair_row)) return fail(ITTS_E_VALIDATION, "pages.k_params, v_params: rows must not overlap");
+    if (t == kOpI4) {
+      if (meet(kps, vps, g.k_params, g.v_params, 2, pair_row)) return fail(ITTS_E_VALIDATION, "pages.k_params, v_params: rows must not overlap");
+      const Rows k = rows(ks, es, row), v = rows(vs, es, row), kp = rows(kps, 2, pair_row), vp = rows(vps, 2, pair_row);
+      if (rows_meet(g.k, k, g.k_params, kp) || rows_meet(g.k, k, g.v_params, vp) || rows_meet(g.v, v, g.k_params, kp) || rows_meet(g.v, v, g.v_params, vp))
+        return fail(ITTS_E_VALIDATION, "pages.k, v: rows must not overlap those of k_params, v_params");
+    }
   }
   *o = Pages{static_cast<char *>(g.k), static_cast<char *>(g.v), static_cast<char *>(g.k_params), static_cast<char *>(g.v_params),
              g.n_pages, g.page_size, g.n_kv_head, g.head_dim, t, ks[0] * es, ks[1] * es, ks[2] * es, vs[0] * es, vs[1] * es, vs[2] * es,

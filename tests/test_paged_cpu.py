@@ -239,3 +239,36 @@ def test_gathered_rows_that_meet(seed):
         with pytest.raises(H.ValidationError) as e:
             call(gather, gather(**over))
         assert e.value.message.startswith("k, v: rows must not overlap"), e.value.message
+
+
+I4 = {"pages_" + k: v for k, v in CODES.items()}
+
+
+@pytest.mark.parametrize("over,match", [
+    # keys [page][head][row], values [page][row][head] in one memory, a page's keys in front of its values
+    (dict(pages_v=P + 2 * 8192, pages_k_page=16384, pages_v_page=16384, pages_v_head=64, pages_v_row=256), None),
+    (dict(pages_v=P + 2 * 8064, pages_k_page=16384, pages_v_page=16384, pages_v_head=64, pages_v_row=256), "pages.k, v"),
+    (dict(pages_v=P + 2 * 8192, pages_k_page=16384, pages_v_page=16256, pages_v_head=64, pages_v_row=256), "pages.k, v"),
+    # one page: its stride is of no account
+    (dict(pages_n_pages=1, pages_v=P + 128, pages_v_page=0), "pages.k, v"),
+    # values inside the keys' range, their rows between the keys'
+    (dict(pages_v=P + 128, pages_k_row=128, pages_k_head=4096, pages_k_page=16384, pages_v_row=128, pages_v_head=4096, pages_v_page=32768), None),
+    (dict(pages_v=P + 128, pages_k_row=128, pages_k_head=4096, pages_k_page=16384, pages_v_row=64, pages_v_head=4096, pages_v_page=16384), "pages.k, v"),
+    (dict(pages_v=P + 1000 * 16384, pages_n_pages=4000, pages_v_page=32768), "pages.k, v"),
+    (dict(pages_v=P + 4000 * 16384, pages_n_pages=4000, pages_v_page=32768), None),
+    # pairs behind a page's codes, and over them
+    (dict(I4, pages_v=P + 4096, pages_k_page=8192 + 1024, pages_v_page=8192 + 1024, pages_k_params=P + 8192, pages_v_params=P + 8704,
+          pages_k_params_page=4608, pages_v_params_page=4608), None),
+    (dict(I4, pages_v=P + 4096, pages_k_page=8192 + 1024, pages_v_page=8192 + 1024, pages_k_params=P + 8192, pages_v_params=P + 8704,
+          pages_k_params_page=4608, pages_v_params_page=4096), "pages.k"),
+    (dict(I4, pages_v_params=P + 40), "pages.k, v: rows must not overlap those"), (dict(I4, pages_k_params=9 * P + 40900), "pages.k, v: rows must not overlap those"),
+], ids=lambda x: str(x)[-70:])
+def test_pages_that_meet(over, match):
+    """Keys, values and pairs of any strides are written where none meets another; they may all be read."""
+    assert takes(attention, **over) and takes(gather, **dict(over, **({"dtype": H.ITTS_F16} if over.get("pages_dtype") == H.ITTS_I4 else {})))
+    if match is None:
+        assert takes(append, **over)
+    else:
+        with pytest.raises(H.ValidationError) as e:
+            call(append, append(**dict(over)))
+        assert e.value.message.startswith(match), e.value.message
