@@ -484,8 +484,8 @@ itts_status itts_paged_append(const itts_paged_append_args *args, void *stream);
  * A token at a negative position sees nothing: zeros.  Tokens of a sequence with a length that is negative or above max_rows,
  * and tokens that see a row whose page is not in 0 .. n_pages - 1, get NaN.  Values in rows that a token does not see never
  * reach it, NaN and infinities among them.  Rows of tokens outside all sequences are zeros.
- * q, out [n_tokens][n_head][head_dim], query head h with key head h / (n_head / n_kv_head).  q_dtype: as in itts_paged_append.
- * max_rows: the longest length that may come, at most n_table pages. */
+ * q, out [n_tokens][n_head][head_dim] (out may be q, with the same strides), query head h with key head
+ * h / (n_head / n_kv_head).  q_dtype: as in itts_paged_append.  max_rows: the longest length that may come, at most n_table pages. */
 typedef struct itts_paged_attention_args {
   itts_pages pages;
   const void *q;

@@ -287,6 +287,15 @@ bool token_rows(const void *p, int64_t token, int64_t head, int tokens, int head
   return row_stride(token, tokens, size) && row_stride(head, heads, size) && aligned16(p);
 }
 
+// Whether rows [tokens][heads] are written to where others of their size are read without one meeting another's: all in the same
+// places, or none.
+bool in_place(const void *in, int64_t in_token, int64_t in_head, const void *out, int64_t out_token, int64_t out_head, int tokens, int heads,
+              int size, int dim) {
+  if (in == out && (tokens <= 1 || in_token == out_token) && (heads <= 1 || in_head == out_head)) return true;
+  return tokens == 0 || !rows_meet(in, rows_of({{in_token, tokens}, {in_head, heads}}, size, dim * size), out,
+                                   rows_of({{out_token, tokens}, {out_head, heads}}, size, dim * size));
+}
+
 itts_status append_args(const itts_paged_append_args *a, PagedAppend *o) {
   if (!a) return fail(ITTS_E_VALIDATION, "args: null");
   Pages g;
@@ -304,8 +313,8 @@ itts_status append_args(const itts_paged_append_args *a, PagedAppend *o) {
     if (!token_rows(a->q_out, a->q_out_token, a->q_out_head, n, a->n_head, es))
       return fail(ITTS_E_VALIDATION, "q_out: rows must start at multiples of 16 bytes");
     if (rows_overlap<2>({{{a->q_out_token, n}, {a->q_out_head, a->n_head}}}, g.D)) return fail(ITTS_E_VALIDATION, "q_out: rows must not overlap");
-    if (a->q == a->q_out && ((n > 1 && a->q_token != a->q_out_token) || (a->n_head > 1 && a->q_head != a->q_out_head)))
-      return fail(ITTS_E_VALIDATION, "q_out: may be q with the same strides alone");
+    if (!in_place(a->q, a->q_token, a->q_head, a->q_out, a->q_out_token, a->q_out_head, n, a->n_head, es, g.D))
+      return fail(ITTS_E_VALIDATION, "q_out: may be q with the same strides, but must not share memory with it otherwise");
   }
   int rot = 0;
   if (a->rotation) {
@@ -335,6 +344,8 @@ itts_status paged_args(const itts_paged_attention_args *a, PagedAttn *o) {
   if (!token_rows(a->q, a->q_token, a->q_head, n, a->n_head, es)) return fail(ITTS_E_VALIDATION, "q: rows must start at multiples of 16 bytes");
   if (!token_rows(a->out, a->out_token, a->out_head, n, a->n_head, es)) return fail(ITTS_E_VALIDATION, "out: rows must start at multiples of 16 bytes");
   if (rows_overlap<2>({{{a->out_token, n}, {a->out_head, a->n_head}}}, g.D)) return fail(ITTS_E_VALIDATION, "out: rows must not overlap");
+  if (!in_place(a->q, a->q_token, a->q_head, a->out, a->out_token, a->out_head, n, a->n_head, es, g.D))
+    return fail(ITTS_E_VALIDATION, "out: may be q with the same strides, but must not share memory with it otherwise");
   if (a->max_rows < 0 || a->max_rows > (int64_t)a->n_table * g.size || a->max_rows > kPagesMaxRows)
     return fail(ITTS_E_VALIDATION, "max_rows: must be in 0..=%d pages of %d rows and at most 2^24, got %d", a->n_table, g.size, a->max_rows);
   if (a->window < 0 || a->sinks < 0) return fail(ITTS_E_VALIDATION, "window, sinks: must be >= 0, got %d and %d", a->window, a->sinks);

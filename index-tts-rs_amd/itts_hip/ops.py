@@ -453,7 +453,7 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, starts: torch.Tensor, le
     sinks    first rows of a sequence that stay in sight of every token beside the window
     max_length  the longest length that may come (default: the table's pages); a tight one lets short sequences do
              with one launch
-    out      where to write (default: a new tensor)
+    out      where to write (default: a new tensor; q itself is fine)
 
     A token at a position below 0 (more tokens than rows) gets zeros, as do tokens that belong to no sequence (starts that do not
     rise: as paged_append has it).  A length that is

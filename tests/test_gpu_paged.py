@@ -143,6 +143,12 @@ class Seqs:
         return ops.paged_attention(self.q, self.cache, self.starts, self.lengths, self.table, **f)
 
 
+# blocks of a token's rows, of several tokens' rows, of many rows over shared tiles; and keys shared by blocks
+ENDS = [([60, 33, 70, 16, 100, 45, 8], [1] * 7, 4, 2, 64), ([50] * 5 + [200], [4, 4, 4, 4, 20, 3], 4, 2, 64),
+        ([220, 180, 40, 200, 300, 90], [60, 50, 10, 40, 50, 9], 8, 2, 64), ([3000] * 6, [2, 1, 3, 1, 2, 1], 4, 2, 128),
+        ([2600] * 6, [40, 30, 50, 20, 40, 39], 8, 2, 64)]
+
+
 def check(got, ref, tol, what=""):
     bad_nan = torch.isnan(ref) != torch.isnan(got.double())
     assert not bad_nan.any(), f"{what}: NaN in other places ({int(bad_nan.sum())})"
@@ -570,6 +576,21 @@ def test_attention_of_more_rows_than_a_quotient_holds(ops, kv):
         assert off.max() <= (tol + HALF[BF16] * want.abs().max() if kv == 4 else 0.0)
 
 
+@pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("lens,news,h,hk,d", ENDS)
+def test_attention_in_place(ops, types, lens, news, h, hk, d):
+    """The result where the queries are: every kernel and layout gives what it gives elsewhere, tokens of no sequence among them."""
+    say(f"[gpu] paged attention in place {types} {lens} {news}")
+    s = Seqs(ops, types, lens, news, h, hk, d, 16, seed=44)
+    for starts in (s.starts_list, s.starts_list[:2] + [10 ** 6] + s.starts_list[3:]):
+        want, q = ops.paged_attention(s.q, s.cache, ints(starts), s.lengths, s.table), s.q.clone()
+        assert ops.paged_attention(q, s.cache, ints(starts), s.lengths, s.table, out=q).data_ptr() == q.data_ptr()
+        assert torch.equal(q, want)
+    for x, out in ((q[:-1], q[1:]), (q[1:], q[:-1])):
+        with pytest.raises(H.ValidationError, match="out: "):
+            ops.paged_attention(x, s.cache, s.starts, s.lengths, s.table, out=out)
+
+
 def test_attention_refuses(ops):
     s = Seqs(ops, (F32, BF16), [20], [1], 4, 2, 64)
     for over, match in ((dict(window=-1), "window"), (dict(max_length=33), "max_length"), (dict(scale=NAN), "scale"),
@@ -843,12 +864,6 @@ def bad_starts(s):
     yield "around others", s[:1] + [s[5]] + s[2:]
     yield "first and last", [s[3]] + s[1:-1] + [s[1]]
     yield "nothing fits", [0, s[-1] + 50] + [s[-1]] * (len(s) - 2)
-
-
-# blocks of a token's rows, of several tokens' rows, of many rows over shared tiles; and keys shared by blocks
-ENDS = [([60, 33, 70, 16, 100, 45, 8], [1] * 7, 4, 2, 64), ([50] * 5 + [200], [4, 4, 4, 4, 20, 3], 4, 2, 64),
-        ([220, 180, 40, 200, 300, 90], [60, 50, 10, 40, 50, 9], 8, 2, 64), ([3000] * 6, [2, 1, 3, 1, 2, 1], 4, 2, 128),
-        ([2600] * 6, [40, 30, 50, 20, 40, 39], 8, 2, 64)]
 
 
 @pytest.mark.parametrize("types", [(F32, BF16), (BF16, BF16), (F32, F32), (F16, 4)])

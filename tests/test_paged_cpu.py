@@ -272,3 +272,19 @@ def test_pages_that_meet(over, match):
         with pytest.raises(H.ValidationError) as e:
             call(append, append(**dict(over)))
         assert e.value.message.startswith(match), e.value.message
+
+
+@pytest.mark.parametrize("kind,out", [(append, "q_out"), (attention, "out")])
+@pytest.mark.parametrize("at,strides,fine", [(0, {}, True), (16, {}, False), (-256, {}, False), (2048, {}, False), (7 * 2048, {}, True), (-7 * 2048, {}, True),
+                                             (0, dict(token=1024), False), (2048, dict(token=1024, q_token=1024), True),
+                                             (2032, dict(token=1024, q_token=1024), False), (0, dict(n_tokens=1, token=4096), True),
+                                             (256, dict(n_tokens=1), False)])
+def test_queries_and_results_in_one_memory(kind, out, at, strides, fine):
+    """7 tokens of 8 heads of 64, 2,048 bytes: in place with the same strides, or beside each other."""
+    over = {out: P + at, **{f"{out}_token" if k == "token" else k: v for k, v in strides.items()}}
+    if fine:
+        assert takes(kind, **over)
+    else:
+        with pytest.raises(H.ValidationError) as e:
+            call(kind, kind(**over))
+        assert e.value.message.startswith(f"{out}: "), e.value.message
