@@ -518,7 +518,9 @@ itts_status itts_paged_gather(const itts_paged_gather_args *args, void *stream);
  *   then    x += bias of t in the row's (bias_tokens, bias) [n_bias] (the last one, where t is there more than once)
  *   then    x = -inf unless bit t % 32 of allowed[row][t / 32] is set (allowed NULL: every token may follow).
  * Computed in float32, rounded once to the type.  Entries of lists outside the vocabulary count for nothing.  repetition,
- * frequency, presence: [rows], or NULL for the value in *_all.  n_history and n_bias <= 65535; row strides may be 0. */
+ * frequency, presence: [rows], or NULL for the value in *_all.  n_history and n_bias <= 65535; row strides may be 0.
+ * rows: up to 2^23 of 2,048 logits, and less than 2^22 pieces of 16,384 of longer ones.  out must not share memory with logits in
+ * other places than its own. */
 typedef struct itts_adjust_logits_args {
   const void *logits;
   void *out;

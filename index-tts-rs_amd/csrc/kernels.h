@@ -344,6 +344,7 @@ struct CacheKeep {
 };
 hipError_t cache_keep(const CacheKeep &a, hipStream_t s);
 // ---- paged caches ----
+constexpr int64_t kMaxLaunch = UINT32_MAX;  // threads along a launch's axis
 // Pages of `size` rows a key head; row r of sequence b is row r % size of page table[b][r / size].  kOpI4: rows of D / 2
 // bytes, two codes each, and D / 64 (scale, base) pairs of fp16.  Strides in bytes.
 constexpr int kPagesMaxRows = 1 << 24;  // of a sequence
@@ -385,6 +386,7 @@ struct PagedAttn {
   int64_t q_t, q_h, o_t, o_h, tab_b;
   float *part;  // paged_attn_ws(a, n_cu) floats
 };
+bool paged_attn_fits(const PagedAttn &a);  // whether its threads are a launch's
 size_t paged_attn_ws(const PagedAttn &a, int n_cu);
 hipError_t paged_attn(const PagedAttn &a, int n_cu, hipStream_t s);
 // Logits [rows][vocab] under penalties for the tokens of a history, biases and a mask of allowed tokens.
@@ -400,6 +402,7 @@ struct AdjustLogits {
   int rows, vocab, n_history, n_bias, type;
   int64_t x_row, out_row, history_row, bias_tokens_row, bias_row, allowed_row;
 };
+bool adjust_logits_fits(int rows, int vocab);  // whether their threads are a launch's
 hipError_t adjust_logits(const AdjustLogits &a, int n_cu, hipStream_t s);
 // Rows of logits: log-probabilities of given tokens, entropy, the top_n most probable tokens.
 constexpr int kScoresMaxTop = 64;

@@ -181,6 +181,11 @@ hipError_t launch(const AdjustLogits &a, int n_cu, hipStream_t s) {
 
 }  // namespace
 
+// (small pieces come with few rows)
+bool adjust_logits_fits(int rows, int vocab) {
+  return (vocab <= 2048 ? 256ll * rows : 1024ll * rows * ((vocab + 16383) / 16384)) <= kMaxLaunch;
+}
+
 hipError_t adjust_logits(const AdjustLogits &a, int n_cu, hipStream_t s) {
   if (a.rows <= 0) return hipSuccess;
   switch (a.type) {

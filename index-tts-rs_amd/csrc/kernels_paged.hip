@@ -1361,6 +1361,9 @@ hipError_t launch(const PagedAttn &a, const Plan &p, hipStream_t s) {
 
 }  // namespace
 
+// (blocks that share keys are no more than fill the card)
+bool paged_attn_fits(const PagedAttn &a) { return a.tokens == 0 || 256ll * make_plan(a, 1).blocks * a.pages.Hk <= kMaxLaunch; }
+
 size_t paged_attn_ws(const PagedAttn &a, int n_cu) {
   const Plan p = make_plan(a, n_cu);
   return p.parts == 0 ? 0 : part_rows(a, p) * (a.pages.D + 2) + 2 * (size_t)a.batch;

@@ -355,6 +355,8 @@ itts_status paged_args(const itts_paged_attention_args *a, PagedAttn *o) {
   *o = PagedAttn{g, a->q, a->out, a->starts, a->lengths, a->table, a->batch, n, a->n_head, a->n_table, a->max_rows, t,
                  std::min(a->window, kFar), std::min(a->sinks, kFar), a->scale, a->q_token, a->q_head, a->out_token, a->out_head,
                  a->table_batch, nullptr};
+  if (!paged_attn_fits(*o))
+    return fail(ITTS_E_VALIDATION, "n_tokens: too many of %d sequences and %d key heads for one launch, got %d", a->batch, g.Hk, n);
   return ITTS_OK;
 }
 
@@ -570,7 +572,7 @@ itts_status itts_adjust_logits(const itts_adjust_logits_args *a, void *stream) {
   if (!a) return fail(ITTS_E_VALIDATION, "args: null");
   if (a->rows < 0 || a->rows > 1 << 23) return fail(ITTS_E_VALIDATION, "rows: must be in 0..=2^23, got %d", a->rows);
   if (a->vocab < 1 || a->vocab > 1 << 24) return fail(ITTS_E_VALIDATION, "vocab: must be in 1..=2^24, got %d", a->vocab);
-  if ((int64_t)a->rows * ((a->vocab + 1023) / 1024) > 1 << 30) return fail(ITTS_E_VALIDATION, "rows: too many of %d logits, got %d", a->vocab, a->rows);
+  if (!adjust_logits_fits(a->rows, a->vocab)) return fail(ITTS_E_VALIDATION, "rows: too many of %d logits, got %d", a->vocab, a->rows);
   if (a->n_history < 0 || a->n_history > kAdjustMaxList) return fail(ITTS_E_VALIDATION, "n_history: must be in 0..=%d, got %d", kAdjustMaxList, a->n_history);
   if (a->n_bias < 0 || a->n_bias > kAdjustMaxList) return fail(ITTS_E_VALIDATION, "n_bias: must be in 0..=%d, got %d", kAdjustMaxList, a->n_bias);
   const int t = op_type(a->dtype);

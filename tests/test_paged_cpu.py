@@ -288,3 +288,28 @@ def test_queries_and_results_in_one_memory(kind, out, at, strides, fine):
         with pytest.raises(H.ValidationError) as e:
             call(kind, kind(**over))
         assert e.value.message.startswith(f"{out}: "), e.value.message
+
+
+@pytest.mark.parametrize("kind,field,over", [
+    (adjust, "rows", dict(rows=1 << 22, vocab=2049)), (adjust, "rows", dict(rows=1 << 22, vocab=16384)), (adjust, "rows", dict(rows=1 << 21, vocab=16385)),
+    (adjust, None, dict(rows=(1 << 22) - 1, vocab=2049)), (adjust, None, dict(rows=(1 << 22) - 1, vocab=16384)), (adjust, None, dict(rows=1 << 23, vocab=2048)),
+    (adjust, None, dict(rows=4095, vocab=1 << 24)), (adjust, "rows", dict(rows=4096, vocab=1 << 24)),
+    (attention, "n_tokens", dict(n_tokens=1 << 20, batch=65535, n_head=512, n_kv_head=512)),
+    (attention, "n_tokens", dict(n_tokens=1 << 19, batch=65535, n_head=1024, n_kv_head=512)),
+    (attention, None, dict(n_tokens=1 << 20, batch=65535, n_head=100, n_kv_head=100)),
+    (attention, None, dict(n_tokens=1 << 20, batch=1, n_head=512, n_kv_head=512))], ids=str)
+def test_more_threads_than_a_launch_has(kind, field, over):
+    """Sizes that are fine one by one, at and past what one launch holds."""
+    over = dict(over)
+    if kind is adjust:
+        v = over["vocab"]
+        over.update(logits=1 << 40, out=1 << 50, logits_row=v, out_row=v, allowed_row=0, history_row=0, bias_tokens_row=0, bias_row=0)
+    else:
+        h, hk = over["n_head"], over.pop("n_kv_head")
+        over.update(q=1 << 40, out=1 << 50, q_token=64 * h, out_token=64 * h, pages_n_kv_head=hk)
+    if field is None:
+        assert takes(kind, **over)
+    else:
+        with pytest.raises(H.ValidationError) as e:
+            call(kind, kind(**over))
+        assert e.value.message.startswith(field), e.value.message
