@@ -297,12 +297,13 @@ class PagedCache(NamedTuple):
 
 def paged_cache(pages: int, heads: int, page_size: int, dim: int, dtype: torch.dtype = torch.bfloat16, *, bits: int = 16,
                 device: Union[None, int, str, torch.device] = "cuda") -> PagedCache:
-    """Memory for `pages` pages (what it holds is not set): of `dtype`, or with bits 4 of codes and their pairs."""
+    """Memory for `pages` pages (what it holds is not set): of `dtype` (bits 32 with float32 alone, which may leave them out), or
+    with bits 4 of codes and their pairs."""
     if bits == 4:
         k, v = (torch.empty((pages, heads, page_size, dim // 2), dtype=torch.uint8, device=device) for _ in range(2))
         kp, vp = (torch.empty((pages, heads, page_size, dim // 64, 2), dtype=torch.float16, device=device) for _ in range(2))
         return PagedCache(k, v, kp, vp)
-    if bits not in (16, 32) or dtype not in _DTYPES or dtype.itemsize * 8 != (32 if dtype == torch.float32 else 16):
+    if bits not in (16, 32) or dtype not in _DTYPES or (bits == 32 and dtype != torch.float32):
         _refuse(f"bits, dtype: float32, bfloat16 or float16, or 4 bits expected, got {bits} and {dtype}")
     k, v = (torch.empty((pages, heads, page_size, dim), dtype=dtype, device=device) for _ in range(2))
     return PagedCache(k, v)

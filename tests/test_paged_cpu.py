@@ -313,3 +313,14 @@ def test_more_threads_than_a_launch_has(kind, field, over):
         with pytest.raises(H.ValidationError) as e:
             call(kind, kind(**over))
         assert e.value.message.startswith(field), e.value.message
+
+
+def test_cache_of_32_bits_is_float32():
+    """32 bits of a type of 16 were given as 16; float32 need not say its bits."""
+    for dtype in (torch.bfloat16, torch.float16):
+        with pytest.raises(H.ValidationError, match="bits"):
+            ops.paged_cache(3, 4, 16, 128, dtype, bits=32, device="cpu")
+    with pytest.raises(H.ValidationError, match="bits"):
+        ops.paged_cache(3, 4, 16, 128, bits=32, device="cpu")
+    assert ops.paged_cache(3, 4, 16, 128, torch.float32, device="cpu").k.dtype == torch.float32
+    assert ops.paged_cache(3, 4, 16, 128, torch.float16, device="cpu").k.dtype == torch.float16
