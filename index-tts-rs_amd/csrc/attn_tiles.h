@@ -141,6 +141,8 @@ __device__ __forceinline__ floatx4 mfma16(const uint32_t *a, const uint32_t *b, 
 
 // Planes of 16 bits that hold a probability: two under 16-bit queries (16 bits of bf16, 22 of fp16) leave no
 // more than the result's own rounding, whichever kernel a launch takes; three under fp32 ones, an fp32's bits.
+// (64 bf16 tokens over up to 6,001 rows are 1.7e-3 of their 2-norm off the 64-bit result, as that result rounded to bf16 is; with
+// three planes just as much, prompts 557 us -> 739, 4 bits 95 -> 107.)
 template <class TQ>
 constexpr int kProbPlanes = TQ::kBytes == 4 ? 3 : 2;
 

@@ -325,7 +325,8 @@ __device__ __forceinline__ float high_half(uint32_t w) { return (float)__builtin
 //   q . k_t = sum_groups s sum_e q_e c_e + b sum_e q_e,
 // so the products run on codes, exact in 16 bits, and the pairs come in by two multiply-adds a score and group.  In the second
 // product the scale goes with the probability, and sum_t p_t b_t is one number a row and group: in bf16, whose
-// range holds a probability times any scale.
+// range holds a probability times any scale.  (Two planes of it, 2^-16, also under fp16 queries, whose results are rounded by 2^-11:
+// 2.055e-4 of their 2-norm off the 64-bit result, which rounded to fp16 is 2.052e-4 off.)
 // Every second key's codes are turned round there: 16 + c of one and c - 31 of the other leave nothing of their 16 where keys
 // weigh alike, and sums over long contexts do not grow.  (With 16 + c alone 60,000 keys of one weight came out 8e-4 of their mean off,
 // four roundings to fp16; so it is 3e-8.)
@@ -971,7 +972,8 @@ __device__ __forceinline__ bool any_in_block(bool v, void *mem) {
 // loads, a tile ahead of their use (keys two: a tile's scores are formed while the exponentials of the one before are).
 // S^T = K Q^T by 32 x 32 products: lane (c, h) holds keys 8 (i / 4) + 4 h + i % 4 of query c in register i, the B operand of
 // O^T = V^T P^T in the order in which the transposing LDS load gives V's rows.
-// One prompt of 8,192 tokens, 32 heads of 128 over 8 key heads, bf16: 777 us, 707 TFLOP/s (818 us without the waves' priorities); the
+// One prompt of 8,192 tokens, 32 heads of 128 over 8 key heads, bf16: 680 to 780 us by the card's clock, 809 to 705 TFLOP/s (in turn
+// on one card 755 us, without the waves' priorities 803); the
 // matrix units are busy 58% of its cycles (a probability's second plane is a third of their work), the vector units 51%, at
 // 1.74 GHz (the card lowers its clock under this load).  On the way there: 16 x 16 tiles copied through registers 1,380 us;
 // 32 x 32 with both kinds of tiles in one loop 1,083 (accumulators copied every turn, queries spilled); a loop of its own for tiles
