@@ -501,7 +501,8 @@ itts_status itts_paged_attention(const itts_paged_attention_args *args, void *wo
 
 /* The first n_rows rows of every sequence out of its pages into k and v [batch][n_kv_head][n_rows][head_dim], zeros from
  * lengths[b] on: caches of one piece, as itts_tree_attention takes them.  Rows of a sequence with a bad length, and rows in a page
- * that does not exist, are NaN.  dtype: the pages', or for I4 any (the codes' values, rounded once). */
+ * that does not exist, are NaN.  dtype: the pages', or for I4 any (the codes' values, rounded once).  No two rows of k and v may share
+ * memory. */
 typedef struct itts_paged_gather_args {
   itts_pages pages;
   void *k, *v;

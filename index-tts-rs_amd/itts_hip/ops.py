@@ -551,7 +551,7 @@ def adjust_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = Non
     bias_tokens, bias  [rows][n] int32 and float32: added to those tokens' logits (where one stands twice, the last one's)
     allowed  [rows][(vocab + 31) // 32] int32: bit t % 32 of word t // 32 says whether token t may follow; the others
              become -inf
-    out      where to write (default: a new tensor; logits itself is fine)
+    out      where to write (default: a new tensor; logits itself is fine, but not its memory shifted)
 
     Rows of lists and masks may be one for all (expand()).  Worked out in float32, rounded once.  Returns out."""
     sx = _tensor(logits, "logits", 2, last=True)
